@@ -1,4 +1,4 @@
-"""ctypes declarations for the C ABI in include/nvtext_amd.h (libnvtext_amd.so)."""
+"""ctypes declarations for the C ABI in include/nvtext_amd.h and its companions (libnvtext_amd.so)."""
 from __future__ import annotations
 
 import ctypes as C
@@ -10,6 +10,7 @@ LIB_PATH = os.environ.get("NVTEXT_AMD_LIB") or os.path.join(_HERE, "libnvtext_am
 
 SUCCESS, INVALID_ARGUMENT, OVERFLOW, LOGIC_ERROR, DEVICE_ERROR, ALLOC_FAILED = range(6)
 TYPE_INT32, TYPE_UINT32, TYPE_UINT64, TYPE_FLOAT32 = 3, 7, 8, 9
+TYPE_FLOAT16, TYPE_BFLOAT16 = 101, 102
 
 EXPORTS = [
     "nvtext_amd_version",
@@ -35,6 +36,13 @@ EXPORTS = [
     "nvtext_amd_wordpiece_vocabulary_unk_id",
     "nvtext_amd_wordpiece_tokenize",
     "nvtext_amd_list_column_free",
+    "nvtext_amd_embedding",
+    "nvtext_amd_embedding_backward",
+    "nvtext_amd_dropout",
+    "nvtext_amd_layer_norm",
+    "nvtext_amd_layer_norm_backward",
+    "nvtext_amd_linear",
+    "nvtext_amd_linear_backward",
     "nvtext_amd_profile_enable",
     "nvtext_amd_profile_read",
     "nvtext_amd_profile_set_range_tiles",
@@ -115,6 +123,16 @@ class StringsResult(C.Structure):
         ("offsets_bytes", C.c_size_t),
         ("chars_bytes", C.c_size_t),
         ("null_mask_bytes", C.c_size_t),
+    ]
+
+
+class Matrix(C.Structure):
+    _fields_ = [
+        ("data", C.c_void_p),
+        ("rows", C.c_int64),
+        ("cols", C.c_int64),
+        ("stride", C.c_int64),
+        ("type", C.c_int32),
     ]
 
 
@@ -239,6 +257,17 @@ def load():
     L.nvtext_amd_wordpiece_tokenize.argtypes = [C.POINTER(StringsColumn), C.c_void_p] + common_tail
     L.nvtext_amd_list_column_free.restype = None
     L.nvtext_amd_list_column_free.argtypes = [C.POINTER(ListColumn), C.c_void_p, C.POINTER(Allocator)]
+    column, matrix, mr, ptr = C.POINTER(ListColumn), C.POINTER(Matrix), C.POINTER(Allocator), C.c_void_p
+    draws = [C.c_double, C.c_uint64, C.c_uint32, ptr]
+    for f, args in ((L.nvtext_amd_embedding, [column, matrix, matrix, ptr, matrix]),
+                    (L.nvtext_amd_embedding_backward, [column, matrix, ptr, mr, matrix, matrix]),
+                    (L.nvtext_amd_dropout, [matrix] + draws + [matrix]),
+                    (L.nvtext_amd_layer_norm, [matrix] * 4 + [C.c_double] + draws + [matrix, matrix, ptr, ptr]),
+                    (L.nvtext_amd_layer_norm_backward, [matrix, matrix, ptr, ptr, matrix, matrix] + draws + [mr] + [matrix] * 4),
+                    (L.nvtext_amd_linear, [matrix] * 3 + [C.c_int32, matrix, ptr, mr, matrix, matrix]),
+                    (L.nvtext_amd_linear_backward, [matrix] * 3 + [C.c_int32, matrix, ptr, mr] + [matrix] * 3)):
+        f.restype = C.c_int
+        f.argtypes = args
     L.nvtext_amd_profile_enable.restype = None
     L.nvtext_amd_profile_enable.argtypes = [C.c_int32]
     L.nvtext_amd_profile_read.restype = C.c_int32

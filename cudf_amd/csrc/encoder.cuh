@@ -1,0 +1,191 @@
+// Shared by the encoder operators (embedding, dropout, layer norm, linear): element types, eight values at a time, the
+// dropout's generator, sums over a wavefront and over columns, and the checks of matrices.
+#pragma once
+
+#include "../../include/nvtext_amd_encoder.h"
+#include "common.cuh"
+
+namespace nvtext_amd {
+
+using half_t = _Float16;
+using bf16_t = __bf16;
+
+// calls f with a value of the element type
+template <typename F>
+inline auto with_type(int32_t type, F&& f)
+{
+  if (type == NVTEXT_AMD_TYPE_FLOAT16) return f(half_t{});
+  if (type == NVTEXT_AMD_TYPE_BFLOAT16) return f(bf16_t{});
+  return f(float{});
+}
+
+inline size_t type_bytes(int32_t type) { return type == NVTEXT_AMD_TYPE_FLOAT32 ? 4 : 2; }
+
+// What a kernel is given of a matrix.
+template <typename T>
+struct Rows {
+  T* data;
+  int64_t stride;
+  __device__ __forceinline__ T* row(int64_t i) const { return data + i * stride; }
+  __device__ __forceinline__ explicit operator bool() const { return data != nullptr; }
+};
+
+template <typename T>
+inline Rows<T> rows_of(const nvtext_amd_matrix* m)
+{
+  return m ? Rows<T>{static_cast<T*>(m->data), m->rows < 2 ? m->cols : m->stride} : Rows<T>{nullptr, 0};
+}
+
+// ------------------------------------------------------------------ checks
+// nullptr if `m` can be used, else what is wrong with it
+inline const char* bad_matrix(const nvtext_amd_matrix* m)
+{
+  if (m->type != NVTEXT_AMD_TYPE_FLOAT32 && m->type != NVTEXT_AMD_TYPE_FLOAT16 && m->type != NVTEXT_AMD_TYPE_BFLOAT16)
+    return "matrices must be of FLOAT32, FLOAT16 or BFLOAT16";
+  if (m->rows < 0 || m->cols < 0 || m->rows > (int64_t{1} << 40) || m->cols > INT32_MAX) return "invalid matrix sizes";
+  if (m->rows >= 2 && (m->stride < m->cols || m->stride > (int64_t{1} << 40))) return "a matrix' stride must not be less than its width";
+  if (m->rows > 0 && m->cols > 0) {
+    if (!m->data) return "a matrix has no data";
+    if (reinterpret_cast<uintptr_t>(m->data) % type_bytes(m->type) != 0) return "a matrix must be aligned to its type";
+  }
+  return nullptr;
+}
+
+inline bool is_shape(const nvtext_amd_matrix* m, int64_t rows, int64_t cols) { return m->rows == rows && m->cols == cols; }
+
+// ------------------------------------------------------------------ eight values
+// Rows need not begin at multiples of 16 bytes: global loads and stores of four words take any address of the element
+// type's alignment, at a cost only where they cross a cache line.
+template <typename T>
+struct Eight {
+  typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+};
+
+// values p[0 .. n), zeros from n on
+template <typename T>
+__device__ __forceinline__ void load8(float (&f)[8], const T* p, int64_t n)
+{
+  if (n >= 8) {
+    auto const v = *reinterpret_cast<const typename Eight<T>::type*>(p);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = static_cast<float>(v[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = k < n ? static_cast<float>(p[k]) : 0.f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, float const (&f)[8], int64_t n)
+{
+  if (n >= 8) {
+    typename Eight<T>::type v;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = static_cast<T>(f[k]);
+    *reinterpret_cast<typename Eight<T>::type*>(p) = v;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < n) p[k] = static_cast<T>(f[k]);
+  }
+}
+
+// ------------------------------------------------------------------ dropout
+// Philox4x32-10 (J. Salmon, M. Moraes, R. Dror, D. Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011): ten rounds
+// of two 32 x 32 -> 64 bit products each, one instruction apiece here.  A counter gives four words, eight draws of 16 bits.
+__device__ __forceinline__ uint4 philox4x32(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0, uint32_t k1)
+{
+#pragma unroll
+  for (int round = 0; round < 10; ++round) {
+    uint64_t const a = static_cast<uint64_t>(c0) * 0xD2511F53u;
+    uint64_t const b = static_cast<uint64_t>(c2) * 0xCD9E8D57u;
+    c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ k0;
+    c1 = static_cast<uint32_t>(b);
+    c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ k1;
+    c3 = static_cast<uint32_t>(a);
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return make_uint4(c0, c1, c2, c3);
+}
+
+// The probability rounded to 1/65536, and the reciprocal of what is left of it: what is kept is multiplied by exactly the
+// reciprocal of the share that is kept on average.
+struct Dropout {
+  uint32_t dropped;  // draws below are dropped; 0: none, 65536: all
+  float scale;
+  uint32_t k0, k1, offset;
+
+  // values 8 * block .. 8 * block + 7 of row `row`
+  __device__ __forceinline__ void apply(float (&f)[8], int64_t row, int64_t block) const
+  {
+    uint4 const r = philox4x32(static_cast<uint32_t>(block), static_cast<uint32_t>(row), static_cast<uint32_t>(row >> 32), offset, k0, k1);
+    uint32_t const w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      uint32_t const draw = k % 2 ? w[k / 2] >> 16 : w[k / 2] & 0xffffu;
+      f[k]                = draw >= dropped ? f[k] * scale : 0.f;  // (chosen, not multiplied: what is dropped may be NaN)
+    }
+  }
+};
+
+inline Dropout make_dropout(double p, uint64_t seed, uint32_t offset)
+{
+  uint32_t const dropped = static_cast<uint32_t>(p * 65536 + 0.5);
+  float const scale      = dropped >= 65536 ? 0.f : static_cast<float>(65536.0 / (65536 - dropped));
+  return Dropout{dropped, scale, static_cast<uint32_t>(seed), static_cast<uint32_t>(seed >> 32), offset};
+}
+
+inline bool is_probability(double p) { return p >= 0 && p <= 1; }  // (not NaN)
+
+// ------------------------------------------------------------------ sums
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ float dpp_zero_f(float v)
+{
+  return __builtin_bit_cast(float, dpp_zero<CTRL, ROW_MASK>(__builtin_bit_cast(uint32_t, v)));
+}
+
+// the sum over the wavefront, in every lane
+__device__ __forceinline__ float wave_sum(float v)
+{
+  v += dpp_zero_f<0x111, 0xf>(v);
+  v += dpp_zero_f<0x112, 0xf>(v);
+  v += dpp_zero_f<0x114, 0xf>(v);
+  v += dpp_zero_f<0x118, 0xf>(v);
+  v += dpp_zero_f<0x142, 0xa>(v);
+  v += dpp_zero_f<0x143, 0xc>(v);
+  return __builtin_bit_cast(float, wave_bcast(__builtin_bit_cast(uint32_t, v), kWave - 1));
+}
+
+// the sum over the workgroup, in every thread; `lds` needs a value a wavefront
+template <int THREADS>
+__device__ __forceinline__ float block_sum(float v, float* lds)
+{
+  v = wave_sum(v);
+  __syncthreads();  // lds may still be read from the call before
+  if (lane_id() == 0) lds[threadIdx.x / kWave] = v;
+  __syncthreads();
+  float sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < THREADS / kWave; ++w) sum += lds[w];
+  return sum;
+}
+
+// Sums over the rows of a matrix: parts [parts, cols] of them are added up, in order, into a row of type T.
+template <typename T>
+__global__ void __launch_bounds__(256) add_parts_kernel(const float* parts, int64_t count, int64_t cols, T* out)
+{
+  int64_t const j = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (j >= cols) return;
+  float sum = 0.f;
+  for (int64_t i = 0; i < count; ++i) sum += parts[i * cols + j];
+  out[j] = static_cast<T>(sum);
+}
+
+template <typename T>
+inline void launch_add_parts(const float* parts, int64_t count, int64_t cols, T* out, hipStream_t stream)
+{
+  hipLaunchKernelGGL(add_parts_kernel<T>, dim3(static_cast<unsigned>((cols + 255) / 256)), dim3(256), 0, stream, parts, count, cols, out);
+}
+
+}  // namespace nvtext_amd
