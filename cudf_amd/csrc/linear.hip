@@ -44,32 +44,311 @@ struct Operand {
   __device__ __forceinline__ float at(int64_t i, int64_t k) const { return static_cast<float>(data[i * of_i + k * of_k]); }
 };
 
-// What becomes of a sum over k.
+// What becomes of eight sums over k.
 template <typename T>
 struct Epilogue {
   Rows<const T> bias, residual;
   Rows<T> out, preactivation;
   int activation;
-  __device__ __forceinline__ void finish(float z, int64_t i, int64_t j) const
+
+  struct Columns {
+    float bias[8];
+    __device__ __forceinline__ Columns(Epilogue const& e, int64_t j, int64_t n)
+    {
+      if (e.bias)
+        load8(bias, e.bias.data + j, n - j);
+      else
+#pragma unroll
+        for (int k = 0; k < 8; ++k) bias[k] = 0.f;
+    }
+  };
+  __device__ __forceinline__ void finish(float (&z)[8], Columns const& columns, int64_t i, int64_t j, int64_t n) const
   {
-    if (bias) z += static_cast<float>(bias.data[j]);
-    if (preactivation) preactivation.row(i)[j] = static_cast<T>(z);
-    z = activate(z, activation);
-    if (residual) z += static_cast<float>(residual.row(i)[j]);
-    out.row(i)[j] = static_cast<T>(z);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) z[k] += columns.bias[k];
+    if (preactivation) store8(preactivation.row(i) + j, z, n - j);
+    if (activation != NVTEXT_AMD_ACTIVATION_NONE) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) z[k] = activate(z[k], activation);
+    }
+    if (residual) {
+      float r[8];
+      load8(r, residual.row(i) + j, n - j);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) z[k] += r[k];
+    }
+    store8(out.row(i) + j, z, n - j);
   }
 };
 
-// out (i, j) = sum over k of a (i, k) * b (j, k).  A workgroup a tile of 64 x 64, a thread 4 x 4 of it.
+// ------------------------------------------------------------------ products of 16-bit types
+// out (i, j) = sum over k of a (i, k) * b (j, k) on the matrix cores.  An operand lies either with its k next to each other
+// (K_NEXT: value (i, k) at i * stride + k) or with its rows next to each other (k * stride + i); both come into LDS as they lie,
+// 32 values of k a stage, by loads that write LDS without a register in between.
+//
+// LDS image of a stage of EXT rows, EXT * 64 bytes, of which a wavefront's load fills 1 KB from one 16-byte piece a lane:
+//   K_NEXT: row i has 64 bytes, its piece c (8 values of k) lies at c ^ (i >> 1 & 3): the 16 rows that a fragment reads at one c
+//           are spread over all banks.
+//   else:   value k has EXT * 2 bytes, its units of 16 rows (32 bytes) lie at u ^ ((k & 3) | (k >> 3 & 1) << 2), for the same reason;
+//           a fragment is read by the transposing load, four values of k at a time.
+// What lies outside the operands is read as zeros: its offset lies beyond the buffer's range.
+constexpr int kStageK     = 32;
+constexpr uint32_t kFar   = 0x80000000u;  // an offset outside every buffer
+constexpr uint32_t kRange = 0x7fffff00u;  // of offsets inside
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+template <typename T>
+using Fragment = T __attribute__((ext_vector_type(8)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef short s16x8_t __attribute__((ext_vector_type(8)));
+using LdsBytes = __attribute__((address_space(3))) char*;
+
+__device__ __forceinline__ f32x4_t multiply(Fragment<bf16_t> a, Fragment<bf16_t> b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4_t multiply(Fragment<half_t> a, Fragment<half_t> b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// An operand: a multiple of 8 values next to each other in each line, lines at multiples of 16 bytes.
+struct Side {
+  const void* data;
+  int64_t stride;  // in values
+};
+
+// What a wavefront loads of an operand for a stage: PIECES loads.
+template <bool K_NEXT, int EXT, int WAVES>
+struct Loader {
+  static constexpr int kPieces = EXT / 16 / WAVES;
+  const char* base;      // of the tile's first value at k = 0
+  int64_t step;          // bytes from a stage to the next
+  uint32_t offset[kPieces];
+  int k_of[kPieces];     // the first k of the lane's pieces, in the stage
+
+  __device__ __forceinline__ Loader(Side const& side, int64_t i0, int64_t extent, int64_t k0, int wave, int lane)
+  {
+    base = static_cast<const char*>(side.data) + 2 * (K_NEXT ? i0 * side.stride + k0 : k0 * side.stride + i0);
+    step = K_NEXT ? 2 * kStageK : 2 * kStageK * side.stride;
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      int const q = wave * kPieces + p;
+      if constexpr (K_NEXT) {
+        int const row = q * 16 + lane / 4, piece = (lane % 4) ^ (row >> 1 & 3);
+        k_of[p]   = piece * 8;
+        offset[p] = i0 + row < extent ? static_cast<uint32_t>(row * side.stride * 2 + piece * 16) : kFar;
+      } else {
+        constexpr int kLine = EXT / 8;  // lanes that a value of k takes
+        int const k = q * (kWave / kLine) + lane / kLine, at = lane % kLine;
+        int const piece = ((at >> 1) ^ ((k & 3) | (k >> 3 & 1) << 2)) * 2 + (at & 1);
+        k_of[p]   = k;
+        offset[p] = i0 + piece * 8 < extent ? static_cast<uint32_t>(k * side.stride * 2 + piece * 16) : kFar;
+      }
+    }
+  }
+  // The next stage, of whose 32 values of k `left` are there (any number), into `to`.
+  __device__ __forceinline__ void load(LdsBytes to, int64_t left, int wave)
+  {
+    auto const buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), static_cast<short>(0), static_cast<int>(kRange), 0x00027000);
+    int const here    = static_cast<int>(left < kStageK ? left : kStageK);
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, to + (wave * kPieces + p) * 1024, 16, k_of[p] < here ? offset[p] : kFar, 0, 0, 0);
+    base += step;
+  }
+};
+
+// Where a lane finds the fragments of 16 rows each, the first beginning at row `first` of the tile.
+template <typename T, bool K_NEXT, int EXT>
+struct Reader {
+  uint32_t at;
+  __device__ __forceinline__ Reader(int first, int lane)
+  {
+    int const i = lane % 16, g = lane / 16;
+    if constexpr (K_NEXT)
+      at = (first + i) * 64 + ((g ^ (i >> 1 & 3)) * 16);
+    else  // value k = 8 g + i / 4, and four further on
+      at = (g * 8 + i / 4) * EXT * 2 + (((first / 16) ^ ((i >> 2) | (g & 1) << 2)) * 32) + i % 4 * 8;
+  }
+  __device__ __forceinline__ Fragment<T> read(LdsBytes stage, int number) const
+  {
+    if constexpr (K_NEXT) {
+      return *reinterpret_cast<__attribute__((address_space(3))) Fragment<T>*>(stage + at + number * 1024);
+    } else {
+      LdsBytes const p   = stage + (at ^ number * 32);
+      s16x4_t const low  = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(p));
+      s16x4_t const high = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(p + 4 * EXT * 2));
+      s16x8_t const both = __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
+      return __builtin_bit_cast(Fragment<T>, both);
+    }
+  }
+};
+
+// All wavefronts have come here, their reads of LDS are done, and of the loads of each all but the last N.  (Written out: a fence in
+// front of the barrier would wait for all loads, because they write LDS.)
+template <int N>
+__device__ __forceinline__ void stage_barrier()
+{
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);
+  asm volatile("s_barrier" ::: "memory");
+}
+
+// A workgroup a tile of BM x BN (blockIdx.x), over the values of k of its part of them (blockIdx.y).  WAVES_M x WAVES_N wavefronts,
+// each with MI x NI fragments of 16 x 16.  STAGES stages of LDS: while the fragments of one, which were read before, are
+// multiplied, those of the next are read, and the stages behind it are on their way.
+template <typename T, bool A_NEXT, bool B_NEXT, int BM, int BN, int WAVES_M, int WAVES_N, int STAGES>
+__device__ __forceinline__ void tile_product(Side a, Side b, int64_t m, int64_t n, int64_t depth, int64_t part, float* sums, Epilogue<T> end)
+{
+  constexpr int kWaves = WAVES_M * WAVES_N, MI = BM / WAVES_M / 16, NI = BN / WAVES_N / 16;
+  constexpr int kStage = (BM + BN) * 64, kLoads = (BM + BN) / 16 / kWaves;
+  __shared__ __attribute__((aligned(1024))) char lds[STAGES * kStage];
+  LdsBytes const stages = (LdsBytes)lds;
+  int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
+  int const wm = wave / WAVES_N, wn = wave % WAVES_N;
+
+  // Workgroups go to the eight XCDs in turn: each takes a run of tiles, within which eight tiles of rows share their columns.
+  int64_t const tiles_m = (m + BM - 1) / BM, tiles_n = (n + BN - 1) / BN, tiles = tiles_m * tiles_n;
+  constexpr int kXcds = 8, kGroup = 8;
+  int64_t const per_xcd = tiles / kXcds, more = tiles % kXcds, xcd = blockIdx.x % kXcds;
+  int64_t const tile  = blockIdx.x / kXcds + xcd * per_xcd + (xcd < more ? xcd : more);
+  int64_t const group = tile / (kGroup * tiles_n), in_group = tile % (kGroup * tiles_n);
+  int64_t const rows_here = tiles_m - group * kGroup < kGroup ? tiles_m - group * kGroup : kGroup;
+  int64_t const i0 = (group * kGroup + in_group % rows_here) * BM, j0 = in_group / rows_here * BN;
+
+  int64_t const k0 = static_cast<int64_t>(blockIdx.y) * part;
+  int64_t left     = depth - k0 < part ? depth - k0 : part;  // values of k that are still to be loaded
+  int const steps  = static_cast<int>((left + kStageK - 1) / kStageK);
+  Loader<A_NEXT, BM, kWaves> load_a(a, i0, m, k0, wave, lane);
+  Loader<B_NEXT, BN, kWaves> load_b(b, j0, n, k0, wave, lane);
+  Reader<T, A_NEXT, BM> const read_a(wm * MI * 16, lane);
+  Reader<T, B_NEXT, BN> const read_b(wn * NI * 16, lane);
+  auto const load = [&](int slot) {
+    load_a.load(stages + slot * kStage, left, wave);
+    load_b.load(stages + slot * kStage + BM * 64, left, wave);
+    left -= kStageK;
+  };
+  f32x4_t sum[MI][NI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; ++j) sum[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  struct Fragments {
+    Fragment<T> a[MI], b[NI];
+  };
+  Fragments f[2];
+  auto const read = [&](Fragments& to, int slot) {
+#pragma unroll
+    for (int j = 0; j < NI; ++j) to.b[j] = read_b.read(stages + slot * kStage + BM * 64, j);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) to.a[i] = read_a.read(stages + slot * kStage, i);
+  };
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s) load(s);
+  stage_barrier<(STAGES - 1) * kLoads>();
+  read(f[0], 0);
+  int slot        = 0;  // of the stage whose fragments are in registers
+  auto const step = [&](Fragments& now, Fragments& next) {
+    stage_barrier<(STAGES - 2) * kLoads>();  // the next stage is there, all of it, and all wavefronts have read this one
+    load(slot);
+    slot = slot + 1 == STAGES ? 0 : slot + 1;
+    read(next, slot);
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) sum[i][j] = multiply(now.b[j], now.a[i], sum[i][j]);  // (the transposed tile: a lane has four values of a row)
+    // a read of LDS, then two products, and so on: left alone, the compiler puts the reads behind the products
+    constexpr int kReads = (A_NEXT ? MI : 2 * MI) + (B_NEXT ? NI : 2 * NI), kEach = MI * NI / kReads;
+#pragma unroll
+    for (int r = 0; r < kReads; ++r) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x8, kEach, 0);
+    }
+    if constexpr (MI * NI > kReads * kEach) __builtin_amdgcn_sched_group_barrier(0x8, MI * NI - kReads * kEach, 0);
+  };
+  int t = 0;
+  for (; t + 2 <= steps; t += 2) {
+    step(f[0], f[1]);
+    step(f[1], f[0]);
+  }
+  if (t < steps) step(f[0], f[1]);
+  stage_barrier<0>();
+
+  // Every wavefront turns its tile round in its own part of LDS, 64 rows at a time, and goes on with eight values of a row a lane.
+  // (A row's 16 units of four values lie at unit ^ row % 16.)
+  static_assert(NI == 4 && MI % 4 == 0 && kWaves * 64 * 256 <= STAGES * kStage, "");
+  LdsBytes const mine = stages + wave * (64 * 256);
+  int64_t const j     = j0 + wn * 64 + lane % 8 * 8;
+  typename Epilogue<T>::Columns const columns(end, j, n);
+#pragma unroll
+  for (int half = 0; half < MI / 4; ++half) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < NI; ++c)
+        *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(mine + (i * 16 + lane % 16) * 256 + ((c * 4 + lane / 16) ^ (lane % 16)) * 16) = sum[half * 4 + i][c];
+    wave_lds_fence();
+    int64_t const first = i0 + (wm * MI + half * 4) * 16;
+#pragma nounroll
+    for (int row = lane / 8; row < 64; row += 8) {
+      auto const unit = [&](int u) { return *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(mine + row * 256 + (u ^ (row % 16)) * 16); };
+      f32x4_t const x = unit(lane % 8 * 2), y = unit(lane % 8 * 2 + 1);
+      float z[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+      if (first + row < m && j < n) {
+        if (sums)
+          store8(sums + (static_cast<int64_t>(blockIdx.y) * m + first + row) * n + j, z, n - j);
+        else
+          end.finish(z, columns, first + row, j, n);
+      }
+    }
+    wave_lds_fence();
+  }
+}
+
+template <typename T, bool A_NEXT, bool B_NEXT, int BM, int BN, int WAVES_M, int WAVES_N, int STAGES>
+__global__ void __launch_bounds__(WAVES_M * WAVES_N * kWave, 2)
+tile_product_kernel(Side a, Side b, int64_t m, int64_t n, int64_t depth, int64_t part, float* sums, Epilogue<T> end)
+{
+  tile_product<T, A_NEXT, B_NEXT, BM, BN, WAVES_M, WAVES_N, STAGES>(a, b, m, n, depth, part, sums, end);
+}
+
+// The parts of a product that was cut along k, added up in order.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) join_parts_kernel(const float* sums, int64_t parts, int64_t m, int64_t n, Epilogue<T> end)
+{
+  int64_t const blocks = (n + 7) / 8;
+  for (int64_t x = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; x < m * blocks; x += static_cast<int64_t>(gridDim.x) * kThreads) {
+    int64_t const i = x / blocks, j = x % blocks * 8;
+    float z[8] = {};
+    for (int64_t p = 0; p < parts; ++p) {
+      float more[8];
+      load8(more, sums + (p * m + i) * n + j, n - j);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) z[k] += more[k];
+    }
+    end.finish(z, typename Epilogue<T>::Columns(end, j, n), i, j, n);
+  }
+}
+
+// Lines of `cols` values, aligned anyhow, into lines of a multiple of 8 values, zeros behind the last.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) align_kernel(Rows<const T> in, int64_t rows, int64_t cols, T* out)
+{
+  int64_t const blocks = (cols + 7) / 8;
+  for (int64_t x = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; x < rows * blocks; x += static_cast<int64_t>(gridDim.x) * kThreads) {
+    int64_t const i = x / blocks, j = x % blocks * 8;
+    float f[8];
+    load8(f, in.row(i) + j, cols - j);
+    store8(out + i * blocks * 8 + j, f, 8);
+  }
+}
+
+// ------------------------------------------------------------------ products of 32-bit types
+// out (i, j) = sum over k of a (i, k) * b (j, k).  A workgroup a tile of 64 x 64, a thread two rows of eight.
 constexpr int kTile = 64, kDepth = 16;
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) product_kernel(Operand<T> a, Operand<T> b, int64_t m, int64_t n, int64_t depth, Epilogue<T> end)
+__global__ void __launch_bounds__(kThreads) product_kernel(Operand<float> a, Operand<float> b, int64_t m, int64_t n, int64_t depth, Epilogue<float> end)
 {
   __shared__ float la[kDepth][kTile + 4], lb[kDepth][kTile + 4];
-  int64_t const i0 = static_cast<int64_t>(blockIdx.y) * kTile, j0 = static_cast<int64_t>(blockIdx.x) * kTile;
-  int const ti = threadIdx.x / 16 * 4, tj = threadIdx.x % 16 * 4;
-  float sum[4][4] = {};
+  int64_t const tiles_n = (n + kTile - 1) / kTile;
+  int64_t const i0 = blockIdx.x / tiles_n * kTile, j0 = blockIdx.x % tiles_n * kTile;
+  int const ti = threadIdx.x / 8 * 2, tj = threadIdx.x % 8 * 8;
+  float sum[2][8] = {};
   for (int64_t k0 = 0; k0 < depth; k0 += kDepth) {
     for (int x = threadIdx.x; x < kTile * kDepth; x += kThreads) {
       // neighbouring threads read neighbouring values
@@ -82,17 +361,17 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Operand<T> a, Operand
 #pragma unroll
     for (int k = 0; k < kDepth; ++k) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sum[i][j] += la[k][ti + i] * lb[k][tj + j];
+        for (int j = 0; j < 8; ++j) sum[i][j] += la[k][ti + i] * lb[k][tj + j];
     }
     __syncthreads();
   }
+  if (j0 + tj >= n) return;
+  Epilogue<float>::Columns const columns(end, j0 + tj, n);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (i0 + ti + i < m && j0 + tj + j < n) end.finish(sum[i][j], i0 + ti + i, j0 + tj + j);
+  for (int i = 0; i < 2; ++i)
+    if (i0 + ti + i < m) end.finish(sum[i], columns, i0 + ti + i, j0 + tj, n);
 }
 
 // d = grad * activation'(z) where it is wanted, and the sums of the columns of it: a workgroup 2048 columns and every
@@ -119,11 +398,69 @@ activation_backward_kernel(Rows<const T> grad, Rows<const T> z, int activation, 
   if (parts) store8(parts + blockIdx.y * cols + j, sum, cols - j);
 }
 
+// An operand of a product of `extent` rows and `depth` values of k each.
 template <typename T>
-void launch_product(Operand<T> const& a, Operand<T> const& b, int64_t m, int64_t n, int64_t depth, Epilogue<T> const& end, hipStream_t stream)
+struct Factor {
+  Rows<const T> rows;
+  bool k_next;  // value (i, k) in line i, else in line k
+};
+
+// Fits what Side and Loader ask for.
+template <typename T>
+bool is_aligned(Factor<T> const& f, int64_t extent, int64_t depth)
 {
-  hipLaunchKernelGGL(product_kernel<T>, dim3(static_cast<unsigned>((n + kTile - 1) / kTile), static_cast<unsigned>((m + kTile - 1) / kTile)), dim3(kThreads), 0, stream, a, b, m, n,
-                     depth, end);
+  int64_t const cols = f.k_next ? depth : extent;
+  return reinterpret_cast<uintptr_t>(f.rows.data) % 16 == 0 && f.rows.stride % 8 == 0 && cols % 8 == 0 && f.rows.stride <= (1 << 21);
+}
+
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, int STAGES>
+void launch_tiles(Side a, bool a_next, Side b, bool b_next, int64_t m, int64_t n, int64_t depth, int64_t part, float* sums, Epilogue<T> const& end, hipStream_t stream)
+{
+  dim3 const grid(static_cast<unsigned>((m + BM - 1) / BM * ((n + BN - 1) / BN)), static_cast<unsigned>((depth + part - 1) / part));
+  dim3 const threads(WAVES_M * WAVES_N * kWave);
+  if (a_next && b_next)
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, true, true, BM, BN, WAVES_M, WAVES_N, STAGES>), grid, threads, 0, stream, a, b, m, n, depth, part, sums, end);
+  else if (a_next)
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, true, false, BM, BN, WAVES_M, WAVES_N, STAGES>), grid, threads, 0, stream, a, b, m, n, depth, part, sums, end);
+  else
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, false, false, BM, BN, WAVES_M, WAVES_N, STAGES>), grid, threads, 0, stream, a, b, m, n, depth, part, sums, end);
+}
+
+#ifndef TILE_BM
+#define TILE_BM 256
+#define TILE_BN 256
+#define TILE_WM 2
+#define TILE_WN 4
+#define TILE_ST 4
+#endif
+
+// out (m x n) = a (m x depth) * b (n x depth)^T
+template <typename T>
+nvtext_amd_status launch_product(Factor<T> a, Factor<T> b, int64_t m, int64_t n, int64_t depth, Epilogue<T> const& end, Mr const& mr, hipStream_t stream)
+{
+  if constexpr (sizeof(T) == 4) {
+    auto const operand = [](Factor<T> const& f) { return Operand<T>{f.rows.data, f.k_next ? f.rows.stride : 1, f.k_next ? 1 : f.rows.stride}; };
+    hipLaunchKernelGGL(product_kernel, dim3(static_cast<unsigned>((n + kTile - 1) / kTile * ((m + kTile - 1) / kTile))), dim3(kThreads), 0, stream, operand(a), operand(b), m, n, depth,
+                       end);
+    return NVTEXT_AMD_SUCCESS;
+  } else {
+    bool const copy_a = depth > 0 && !is_aligned(a, m, depth), copy_b = depth > 0 && !is_aligned(b, n, depth);
+    auto const lines  = [&](Factor<T> const& f, int64_t extent) { return f.k_next ? extent : depth; };
+    auto const width  = [&](Factor<T> const& f, int64_t extent) { return ((f.k_next ? depth : extent) + 7) / 8 * 8; };
+    TempParts<2> const temp(mr, {copy_a ? static_cast<size_t>(lines(a, m) * width(a, m)) * sizeof(T) : 0, copy_b ? static_cast<size_t>(lines(b, n) * width(b, n)) * sizeof(T) : 0},
+                            copy_a || copy_b);
+    if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
+    auto const align = [&](Factor<T>& f, int64_t extent, T* to) {
+      int64_t const work = lines(f, extent) * width(f, extent) / 8;
+      hipLaunchKernelGGL(align_kernel<T>, dim3(static_cast<unsigned>(std::min<int64_t>((work + kThreads - 1) / kThreads, 16 * device_cus()))), dim3(kThreads), 0, stream, f.rows,
+                         lines(f, extent), f.k_next ? depth : extent, to);
+      f.rows = Rows<const T>{to, width(f, extent)};
+    };
+    if (copy_a) align(a, m, temp.template part<T>(0));
+    if (copy_b) align(b, n, temp.template part<T>(1));
+    launch_tiles<T, TILE_BM, TILE_BN, TILE_WM, TILE_WN, TILE_ST>(Side{a.rows.data, a.rows.stride}, a.k_next, Side{b.rows.data, b.rows.stride}, b.k_next, m, n, depth, std::max<int64_t>(depth, 1), nullptr, end, stream);
+    return NVTEXT_AMD_SUCCESS;
+  }
 }
 
 bool is_activation(int32_t a) { return a >= NVTEXT_AMD_ACTIVATION_NONE && a <= NVTEXT_AMD_ACTIVATION_SILU; }
@@ -160,14 +497,16 @@ nvtext_amd_status nvtext_amd_linear(const nvtext_amd_matrix* x, const nvtext_amd
   if (!is_activation(activation)) return fail(NVTEXT_AMD_INVALID_ARGUMENT, "unknown activation");
   if (m == 0 || n == 0) return NVTEXT_AMD_SUCCESS;
   hipStream_t stream = static_cast<hipStream_t>(stream_);
+  Mr const mr{mr_, stream};
+  nvtext_amd_status st = NVTEXT_AMD_SUCCESS;
   with_type(x->type, [&](auto zero) {
-    using T        = decltype(zero);
-    auto const xs  = rows_of<const T>(x);
-    auto const ws  = rows_of<const T>(weight);
+    using T       = decltype(zero);
+    auto const xs = rows_of<const T>(x), ws = rows_of<const T>(weight);
     ProfileScope const scope("linear", stream);
-    launch_product<T>({xs.data, xs.stride, 1}, {ws.data, ws.stride, 1}, m, n, depth,
-                      {rows_of<const T>(bias), rows_of<const T>(residual), rows_of<T>(out), rows_of<T>(preactivation), activation}, stream);
+    st = launch_product<T>({xs, true}, {ws, true}, m, n, depth, {rows_of<const T>(bias), rows_of<const T>(residual), rows_of<T>(out), rows_of<T>(preactivation), activation}, mr,
+                           stream);
   });
+  if (st != NVTEXT_AMD_SUCCESS) return st;
   NVTEXT_HIP_TRY(hipGetLastError());
   return NVTEXT_AMD_SUCCESS;
 }
@@ -198,6 +537,7 @@ nvtext_amd_status nvtext_amd_linear_backward(const nvtext_amd_matrix* grad, cons
   int64_t const parts = std::max<int64_t>(1, std::min<int64_t>(m, 256));
   TempParts<2> const temp(mr, {slopes ? static_cast<size_t>(m * n) * type_bytes(x->type) : 0, bias_grad ? static_cast<size_t>(parts * n) * sizeof(float) : 0});
   if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
+  nvtext_amd_status st = NVTEXT_AMD_SUCCESS;
   with_type(x->type, [&](auto zero) {
     using T       = decltype(zero);
     auto const xs = rows_of<const T>(x), ws = rows_of<const T>(weight), gs = rows_of<const T>(grad);
@@ -213,13 +553,14 @@ nvtext_amd_status nvtext_amd_linear_backward(const nvtext_amd_matrix* grad, cons
     auto const plain = [](const nvtext_amd_matrix* o) { return Epilogue<T>{{nullptr, 0}, {nullptr, 0}, rows_of<T>(o), {nullptr, 0}, NVTEXT_AMD_ACTIVATION_NONE}; };
     if (x_grad && m > 0 && depth > 0) {
       ProfileScope const scope("linear_x_backward", stream);
-      launch_product<T>({ds.data, ds.stride, 1}, {ws.data, 1, ws.stride}, m, depth, n, plain(x_grad), stream);
+      st = launch_product<T>({ds, true}, {ws, false}, m, depth, n, plain(x_grad), mr, stream);
     }
-    if (weight_grad && n > 0 && depth > 0) {
+    if (st == NVTEXT_AMD_SUCCESS && weight_grad && n > 0 && depth > 0) {
       ProfileScope const scope("linear_weight_backward", stream);
-      launch_product<T>({ds.data, 1, ds.stride}, {xs.data, 1, xs.stride}, n, depth, m, plain(weight_grad), stream);
+      st = launch_product<T>({ds, false}, {xs, false}, n, depth, m, plain(weight_grad), mr, stream);
     }
   });
+  if (st != NVTEXT_AMD_SUCCESS) return st;
   NVTEXT_HIP_TRY(hipGetLastError());
   return NVTEXT_AMD_SUCCESS;
 }
