@@ -171,21 +171,33 @@ __device__ __forceinline__ float block_sum(float v, float* lds)
   return sum;
 }
 
-// Sums over the rows of a matrix: parts [parts, cols] of them are added up, in order, into a row of type T.
+// Sums over the rows of a matrix: parts [count, cols] of them are added up into a row of type T, by a workgroup for 64 columns,
+// whose wavefronts take a run of parts each.
 template <typename T>
-__global__ void __launch_bounds__(256) add_parts_kernel(const float* parts, int64_t count, int64_t cols, T* out)
+__global__ void __launch_bounds__(512) add_parts_kernel(const float* parts, int64_t count, int64_t cols, T* out)
 {
-  int64_t const j = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (j >= cols) return;
+  constexpr int kWaves = 512 / kWave;
+  __shared__ float lds[kWaves][kWave];
+  int const wave = threadIdx.x / kWave, lane = lane_id();
+  int64_t const j = static_cast<int64_t>(blockIdx.x) * kWave + lane;
+  int64_t const each = (count + kWaves - 1) / kWaves, first = wave * each, last = first + each < count ? first + each : count;
   float sum = 0.f;
-  for (int64_t i = 0; i < count; ++i) sum += parts[i * cols + j];
+  if (j < cols) {
+#pragma unroll 8
+    for (int64_t i = first; i < last; ++i) sum += parts[i * cols + j];
+  }
+  lds[wave][lane] = sum;
+  __syncthreads();
+  if (wave != 0 || j >= cols) return;
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) sum += lds[w][lane];
   out[j] = static_cast<T>(sum);
 }
 
 template <typename T>
 inline void launch_add_parts(const float* parts, int64_t count, int64_t cols, T* out, hipStream_t stream)
 {
-  hipLaunchKernelGGL(add_parts_kernel<T>, dim3(static_cast<unsigned>((cols + 255) / 256)), dim3(256), 0, stream, parts, count, cols, out);
+  hipLaunchKernelGGL(add_parts_kernel<T>, dim3(static_cast<unsigned>((cols + kWave - 1) / kWave)), dim3(512), 0, stream, parts, count, cols, out);
 }
 
 }  // namespace nvtext_amd

@@ -2,37 +2,82 @@
 #include "encoder.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace nvtext_amd {
 namespace {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ float activate(float z, int activation)
+// ------------------------------------------------------------------ activations
+// gelu needs the normal distribution's integral: for a >= 0, 1 - Phi(a) = exp(-a^2 / 2) * q(a), where q is the smooth factor
+// that a polynomial in t = 1 / (1 + 0.27 a) without a constant gives to 1.2e-6 of itself for all a up to 14 (fitted here, relative
+// error levelled; behind 14 the result is less than 1e-44).  16 instructions; erff is 50 and took a product of 32768 x 1024 x 4096
+// 30 % longer.  The other two are z times a logistic function.
+struct Normal {
+  float below;  // Phi(z)
+  float power;  // exp(-z^2 / 2)
+};
+__device__ __forceinline__ Normal normal_integral(float z)
 {
-  switch (activation) {
-    case NVTEXT_AMD_ACTIVATION_RELU: return z > 0.f ? z : 0.f;
-    case NVTEXT_AMD_ACTIVATION_GELU: return z * (0.5f + 0.5f * erff(z * 0.70710678118654752f));
-    case NVTEXT_AMD_ACTIVATION_GELU_TANH: return z * (0.5f + 0.5f * tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z)));
-    case NVTEXT_AMD_ACTIVATION_SILU: return z / (1.f + expf(-z));
-    default: return z;
-  }
+  float const a = fabsf(z);
+  float const t = __builtin_amdgcn_rcpf(fmaf(0.27f, a, 1.f));
+  float const e = __builtin_amdgcn_exp2f(-0.72134752044448170f * a * a);
+  float p       = -0.060750546003806f;
+  p             = fmaf(p, t, 0.158194570433751f);
+  p             = fmaf(p, t, -0.023792406020599f);
+  p             = fmaf(p, t, 0.117305767865979f);
+  p             = fmaf(p, t, 0.092921671108990f);
+  p             = fmaf(p, t, 0.108432858593045f);
+  p             = fmaf(p, t, 0.107687495523215f);
+  float const q = p * t * e;
+  return Normal{z < 0.f ? q : 1.f - q, e};
 }
 
-__device__ __forceinline__ float slope(float z, int activation)
+__device__ __forceinline__ float logistic(float u) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * u)); }
+
+constexpr float kTwoRootTwoOverPi = 1.5957691216057308f;  // (1 + tanh u) / 2 is logistic(2 u)
+
+template <int ACTIVATION>
+__device__ __forceinline__ float activate(float z)
+{
+  if constexpr (ACTIVATION == NVTEXT_AMD_ACTIVATION_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
+  if constexpr (ACTIVATION == NVTEXT_AMD_ACTIVATION_GELU) return z * normal_integral(z).below;
+  if constexpr (ACTIVATION == NVTEXT_AMD_ACTIVATION_GELU_TANH) return z * logistic(kTwoRootTwoOverPi * fmaf(0.044715f * z * z, z, z));
+  if constexpr (ACTIVATION == NVTEXT_AMD_ACTIVATION_SILU) return z * logistic(z);
+  return z;
+}
+
+template <int ACTIVATION>
+__device__ __forceinline__ float slope(float z)
+{
+  if constexpr (ACTIVATION == NVTEXT_AMD_ACTIVATION_RELU) return z > 0.f ? 1.f : 0.f;
+  if constexpr (ACTIVATION == NVTEXT_AMD_ACTIVATION_GELU) {
+    Normal const n = normal_integral(z);
+    return fmaf(z * n.power, 0.39894228040143268f, n.below);
+  }
+  if constexpr (ACTIVATION == NVTEXT_AMD_ACTIVATION_GELU_TANH) {
+    float const s = logistic(kTwoRootTwoOverPi * fmaf(0.044715f * z * z, z, z));
+    float const c = fminf(fmaxf(z, -30.f), 30.f);  // (s is 0 or 1 long before, and z^2 must not become infinite beside it)
+    return fmaf(c * (s - s * s), kTwoRootTwoOverPi * fmaf(0.134145f * c, c, 1.f), s);
+  }
+  if constexpr (ACTIVATION == NVTEXT_AMD_ACTIVATION_SILU) {
+    float const s = logistic(z);
+    return fmaf(z, s - s * s, s);
+  }
+  return 1.f;
+}
+
+// calls f with the activation as a constant
+template <typename F>
+__device__ __forceinline__ void with_activation(int activation, F&& f)
 {
   switch (activation) {
-    case NVTEXT_AMD_ACTIVATION_RELU: return z > 0.f ? 1.f : 0.f;
-    case NVTEXT_AMD_ACTIVATION_GELU: return 0.5f + 0.5f * erff(z * 0.70710678118654752f) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
-    case NVTEXT_AMD_ACTIVATION_GELU_TANH: {
-      float const t = tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z));
-      return 0.5f + 0.5f * t + 0.5f * z * (1.f - t * t) * 0.79788456080286536f * (1.f + 0.134145f * z * z);
-    }
-    case NVTEXT_AMD_ACTIVATION_SILU: {
-      float const s = 1.f / (1.f + expf(-z));
-      return s * (1.f + z * (1.f - s));
-    }
-    default: return 1.f;
+    case NVTEXT_AMD_ACTIVATION_RELU: f(std::integral_constant<int, NVTEXT_AMD_ACTIVATION_RELU>{}); break;
+    case NVTEXT_AMD_ACTIVATION_GELU: f(std::integral_constant<int, NVTEXT_AMD_ACTIVATION_GELU>{}); break;
+    case NVTEXT_AMD_ACTIVATION_GELU_TANH: f(std::integral_constant<int, NVTEXT_AMD_ACTIVATION_GELU_TANH>{}); break;
+    case NVTEXT_AMD_ACTIVATION_SILU: f(std::integral_constant<int, NVTEXT_AMD_ACTIVATION_SILU>{}); break;
+    default: break;
   }
 }
 
@@ -67,10 +112,10 @@ struct Epilogue {
 #pragma unroll
     for (int k = 0; k < 8; ++k) z[k] += columns.bias[k];
     if (preactivation) store8(preactivation.row(i) + j, z, n - j);
-    if (activation != NVTEXT_AMD_ACTIVATION_NONE) {
+    with_activation(activation, [&](auto which) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) z[k] = activate(z[k], activation);
-    }
+      for (int k = 0; k < 8; ++k) z[k] = activate<decltype(which)::value>(z[k]);
+    });
     if (residual) {
       float r[8];
       load8(r, residual.row(i) + j, n - j);
@@ -84,15 +129,15 @@ struct Epilogue {
 // ------------------------------------------------------------------ products of 16-bit types
 // out (i, j) = sum over k of a (i, k) * b (j, k) on the matrix cores.  An operand lies either with its k next to each other
 // (K_NEXT: value (i, k) at i * stride + k) or with its rows next to each other (k * stride + i); both come into LDS as they lie,
-// 32 values of k a stage, by loads that write LDS without a register in between.
+// 64 values of k a stage, by loads that write LDS without a register in between.
 //
-// LDS image of a stage of EXT rows, EXT * 64 bytes, of which a wavefront's load fills 1 KB from one 16-byte piece a lane:
-//   K_NEXT: row i has 64 bytes, its piece c (8 values of k) lies at c ^ (i >> 1 & 3): the 16 rows that a fragment reads at one c
-//           are spread over all banks.
-//   else:   value k has EXT * 2 bytes, its units of 16 rows (32 bytes) lie at u ^ ((k & 3) | (k >> 3 & 1) << 2), for the same reason;
+// LDS image of a stage of EXT rows, EXT * 128 bytes, of which a wavefront's load fills 1 KB from one 16-byte piece a lane:
+//   K_NEXT: row i has 128 bytes (whole cache lines: with 64 L2 answered as many requests for half the bytes), its piece c (8 values
+//           of k) lies at c ^ (i & 7): the rows that a fragment reads at one c are spread over all banks.
+//   else:   value k has EXT * 2 bytes, its units of 16 rows (32 bytes) lie at u ^ (k & 3 | (k >> 3 & 1) << 2), for the same reason;
 //           a fragment is read by the transposing load, four values of k at a time.
 // What lies outside the operands is read as zeros: its offset lies beyond the buffer's range.
-constexpr int kStageK     = 32;
+constexpr int kStageK     = 64;
 constexpr uint32_t kFar   = 0x80000000u;  // an offset outside every buffer
 constexpr uint32_t kRange = 0x7fffff00u;  // of offsets inside
 
@@ -115,7 +160,7 @@ struct Side {
 // What a wavefront loads of an operand for a stage: PIECES loads.
 template <bool K_NEXT, int EXT, int WAVES>
 struct Loader {
-  static constexpr int kPieces = EXT / 16 / WAVES;
+  static constexpr int kPieces = EXT / 8 / WAVES;
   const char* base;      // of the tile's first value at k = 0
   int64_t step;          // bytes from a stage to the next
   uint32_t offset[kPieces];
@@ -129,7 +174,7 @@ struct Loader {
     for (int p = 0; p < kPieces; ++p) {
       int const q = wave * kPieces + p;
       if constexpr (K_NEXT) {
-        int const row = q * 16 + lane / 4, piece = (lane % 4) ^ (row >> 1 & 3);
+        int const row = q * 8 + lane / 8, piece = (lane % 8) ^ (row & 7);
         k_of[p]   = piece * 8;
         offset[p] = i0 + row < extent ? static_cast<uint32_t>(row * side.stride * 2 + piece * 16) : kFar;
       } else {
@@ -141,16 +186,14 @@ struct Loader {
       }
     }
   }
-  // The next stage, of whose 32 values of k `left` are there (any number), into `to`.
-  __device__ __forceinline__ void load(LdsBytes to, int64_t left, int wave)
+  // Piece `p` of the next stage, of whose 64 values of k `left` are there (any number), into `to`.
+  __device__ __forceinline__ void load(LdsBytes to, int64_t left, int wave, int p) const
   {
     auto const buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), static_cast<short>(0), static_cast<int>(kRange), 0x00027000);
     int const here    = static_cast<int>(left < kStageK ? left : kStageK);
-#pragma unroll
-    for (int p = 0; p < kPieces; ++p)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, to + (wave * kPieces + p) * 1024, 16, k_of[p] < here ? offset[p] : kFar, 0, 0, 0);
-    base += step;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, to + (wave * kPieces + p) * 1024, 16, k_of[p] < here ? offset[p] : kFar, 0, 0, 0);
   }
+  __device__ __forceinline__ void next() { base += step; }
 };
 
 // Where a lane finds the fragments of 16 rows each, the first beginning at row `first` of the tile.
@@ -161,16 +204,17 @@ struct Reader {
   {
     int const i = lane % 16, g = lane / 16;
     if constexpr (K_NEXT)
-      at = (first + i) * 64 + ((g ^ (i >> 1 & 3)) * 16);
+      at = (first + i) * 128 + ((g ^ (i & 7)) * 16);
     else  // value k = 8 g + i / 4, and four further on
       at = (g * 8 + i / 4) * EXT * 2 + (((first / 16) ^ ((i >> 2) | (g & 1) << 2)) * 32) + i % 4 * 8;
   }
-  __device__ __forceinline__ Fragment<T> read(LdsBytes stage, int number) const
+  // fragment `number` of the first or second 32 values of k
+  __device__ __forceinline__ Fragment<T> read(LdsBytes stage, int half, int number) const
   {
     if constexpr (K_NEXT) {
-      return *reinterpret_cast<__attribute__((address_space(3))) Fragment<T>*>(stage + at + number * 1024);
+      return *reinterpret_cast<__attribute__((address_space(3))) Fragment<T>*>(stage + (at ^ half * 64) + number * 2048);
     } else {
-      LdsBytes const p   = stage + (at ^ number * 32);
+      LdsBytes const p   = stage + (at ^ number * 32) + half * 64 * EXT;
       s16x4_t const low  = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(p));
       s16x4_t const high = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(p + 4 * EXT * 2));
       s16x8_t const both = __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -190,14 +234,13 @@ __device__ __forceinline__ void stage_barrier()
 }
 
 // A workgroup a tile of BM x BN (blockIdx.x), over the values of k of its part of them (blockIdx.y).  WAVES_M x WAVES_N wavefronts,
-// each with MI x NI fragments of 16 x 16.  STAGES stages of LDS: while the fragments of one, which were read before, are
-// multiplied, those of the next are read, and the stages behind it are on their way.
-template <typename T, bool A_NEXT, bool B_NEXT, int BM, int BN, int WAVES_M, int WAVES_N, int STAGES>
+// each with MI x NI fragments of 16 x 16.
+template <typename T, bool A_NEXT, bool B_NEXT, int BM, int BN, int WAVES_M, int WAVES_N>
 __device__ __forceinline__ void tile_product(Side a, Side b, int64_t m, int64_t n, int64_t depth, int64_t part, float* sums, Epilogue<T> end)
 {
   constexpr int kWaves = WAVES_M * WAVES_N, MI = BM / WAVES_M / 16, NI = BN / WAVES_N / 16;
-  constexpr int kStage = (BM + BN) * 64, kLoads = (BM + BN) / 16 / kWaves;
-  __shared__ __attribute__((aligned(1024))) char lds[STAGES * kStage];
+  constexpr int kStage = (BM + BN) * 128, kLoads = (BM + BN) / 8 / kWaves;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
   LdsBytes const stages = (LdsBytes)lds;
   int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
   int const wm = wave / WAVES_N, wn = wave % WAVES_N;
@@ -218,10 +261,18 @@ __device__ __forceinline__ void tile_product(Side a, Side b, int64_t m, int64_t 
   Loader<B_NEXT, BN, kWaves> load_b(b, j0, n, k0, wave, lane);
   Reader<T, A_NEXT, BM> const read_a(wm * MI * 16, lane);
   Reader<T, B_NEXT, BN> const read_b(wn * NI * 16, lane);
-  auto const load = [&](int slot) {
-    load_a.load(stages + slot * kStage, left, wave);
-    load_b.load(stages + slot * kStage + BM * 64, left, wave);
-    left -= kStageK;
+  // Two stages are in LDS.  Load number `p` of the next one, into place `slot`:
+  auto const load = [&](int slot, int p) {
+    LdsBytes const to = stages + slot * kStage;
+    if (p < BM / 8 / kWaves)
+      load_a.load(to, left, wave, p);
+    else
+      load_b.load(to + BM * 128, left, wave, p - BM / 8 / kWaves);
+    if (p == kLoads - 1) {
+      load_a.next();
+      load_b.next();
+      left -= kStageK;
+    }
   };
   f32x4_t sum[MI][NI];
 #pragma unroll
@@ -232,46 +283,58 @@ __device__ __forceinline__ void tile_product(Side a, Side b, int64_t m, int64_t 
     Fragment<T> a[MI], b[NI];
   };
   Fragments f[2];
-  auto const read = [&](Fragments& to, int slot) {
 #pragma unroll
-    for (int j = 0; j < NI; ++j) to.b[j] = read_b.read(stages + slot * kStage + BM * 64, j);
+  for (int s = 0; s < 2; ++s)
 #pragma unroll
-    for (int i = 0; i < MI; ++i) to.a[i] = read_a.read(stages + slot * kStage, i);
-  };
+    for (int p = 0; p < kLoads; ++p) load(s, p);
+  stage_barrier<kLoads>();
 #pragma unroll
-  for (int s = 0; s < STAGES; ++s) load(s);
-  stage_barrier<(STAGES - 1) * kLoads>();
-  read(f[0], 0);
-  int slot        = 0;  // of the stage whose fragments are in registers
-  auto const step = [&](Fragments& now, Fragments& next) {
-    stage_barrier<(STAGES - 2) * kLoads>();  // the next stage is there, all of it, and all wavefronts have read this one
-    load(slot);
-    slot = slot + 1 == STAGES ? 0 : slot + 1;
-    read(next, slot);
+  for (int j = 0; j < NI; ++j) f[0].b[j] = read_b.read(stages + BM * 128, 0, j);
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+  for (int i = 0; i < MI; ++i) f[0].a[i] = read_a.read(stages, 0, i);
+  // Multiplies the fragments of one half of a stage and reads those of the next, a little of either in turn: left to itself, the
+  // compiler puts all reads behind the products.  SECOND: the next half is the first of the other stage, for which everybody waits
+  // after a row of products; this stage has been read then and makes room for the one after that.
+  auto const step = [&](Fragments const& now, Fragments& next, int slot, auto second) {
+    constexpr bool kSecond = decltype(second)::value;
+    LdsBytes const from    = stages + (kSecond ? slot ^ 1 : slot) * kStage;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      // read number r: a fragment of a, all of b, the others of a
+      auto const read = [&](int r) {
+        if (r == 0 || r > NI)
+          next.a[r == 0 ? 0 : r - NI] = read_a.read(from, kSecond ? 0 : 1, r == 0 ? 0 : r - NI);
+        else
+          next.b[r - 1] = read_b.read(from + BM * 128, kSecond ? 0 : 1, r - 1);
+      };
+      constexpr int kRows  = kSecond ? MI - 1 : MI;  // that loads and reads go with
+      constexpr int kReads = (MI + NI + kRows - 1) / kRows, kLoadsEach = (kLoads + kRows - 1) / kRows;
+      if constexpr (kSecond) {
+        if (i == 1) stage_barrier<0>();
+#pragma unroll
+        for (int p = (i - 1) * kLoadsEach; p < i * kLoadsEach; ++p)
+          if (i >= 1 && p < kLoads) load(slot, p);
+      }
+      int const g = kSecond ? i - 1 : i;
+#pragma unroll
+      for (int r = g * kReads; r < (g + 1) * kReads; ++r)
+        if (g >= 0 && r < MI + NI) read(r);
 #pragma unroll
       for (int j = 0; j < NI; ++j) sum[i][j] = multiply(now.b[j], now.a[i], sum[i][j]);  // (the transposed tile: a lane has four values of a row)
-    // a read of LDS, then two products, and so on: left alone, the compiler puts the reads behind the products
-    constexpr int kReads = (A_NEXT ? MI : 2 * MI) + (B_NEXT ? NI : 2 * NI), kEach = MI * NI / kReads;
-#pragma unroll
-    for (int r = 0; r < kReads; ++r) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x8, kEach, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (MI * NI > kReads * kEach) __builtin_amdgcn_sched_group_barrier(0x8, MI * NI - kReads * kEach, 0);
   };
-  int t = 0;
-  for (; t + 2 <= steps; t += 2) {
-    step(f[0], f[1]);
-    step(f[1], f[0]);
+  int slot = 0;  // of the stage that is multiplied
+  for (int t = 0; t < steps; ++t) {
+    step(f[0], f[1], slot, std::false_type{});
+    step(f[1], f[0], slot, std::true_type{});
+    slot ^= 1;
   }
-  if (t < steps) step(f[0], f[1]);
   stage_barrier<0>();
 
   // Every wavefront turns its tile round in its own part of LDS, 64 rows at a time, and goes on with eight values of a row a lane.
   // (A row's 16 units of four values lie at unit ^ row % 16.)
-  static_assert(NI == 4 && MI % 4 == 0 && kWaves * 64 * 256 <= STAGES * kStage, "");
+  static_assert(NI == 4 && MI % 4 == 0 && kWaves * 64 * 256 <= 2 * kStage, "");
   LdsBytes const mine = stages + wave * (64 * 256);
   int64_t const j     = j0 + wn * 64 + lane % 8 * 8;
   typename Epilogue<T>::Columns const columns(end, j, n);
@@ -300,11 +363,11 @@ __device__ __forceinline__ void tile_product(Side a, Side b, int64_t m, int64_t 
   }
 }
 
-template <typename T, bool A_NEXT, bool B_NEXT, int BM, int BN, int WAVES_M, int WAVES_N, int STAGES>
+template <typename T, bool A_NEXT, bool B_NEXT, int BM, int BN, int WAVES_M, int WAVES_N>
 __global__ void __launch_bounds__(WAVES_M * WAVES_N * kWave, 2)
 tile_product_kernel(Side a, Side b, int64_t m, int64_t n, int64_t depth, int64_t part, float* sums, Epilogue<T> end)
 {
-  tile_product<T, A_NEXT, B_NEXT, BM, BN, WAVES_M, WAVES_N, STAGES>(a, b, m, n, depth, part, sums, end);
+  tile_product<T, A_NEXT, B_NEXT, BM, BN, WAVES_M, WAVES_N>(a, b, m, n, depth, part, sums, end);
 }
 
 // The parts of a product that was cut along k, added up in order.
@@ -374,28 +437,45 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Operand<float> a, Ope
     if (i0 + ti + i < m) end.finish(sum[i], columns, i0 + ti + i, j0 + tj, n);
 }
 
-// d = grad * activation'(z) where it is wanted, and the sums of the columns of it: a workgroup 2048 columns and every
-// gridDim.y-th row.
+// d = grad * activation'(z) where it is wanted, and the sums of the columns of it: a workgroup takes 512 columns and every
+// gridDim.y-th run of four rows, a wavefront one of the four, and the wavefronts' sums are added up in the end.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 activation_backward_kernel(Rows<const T> grad, Rows<const T> z, int activation, int64_t rows, int64_t cols, Rows<T> d, float* parts)
 {
-  int64_t const j = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * 8;
-  if (j >= cols) return;
-  float sum[8] = {};
-  for (int64_t i = blockIdx.y; i < rows; i += gridDim.y) {
-    float g[8], v[8];
-    load8(g, grad.row(i) + j, cols - j);
-    if (z) {
-      load8(v, z.row(i) + j, cols - j);
+  constexpr int kWaves = kThreads / kWave;
+  __shared__ float lds[kWaves][8][kWave];
+  int const wave = threadIdx.x / kWave, lane = lane_id();
+  int64_t const j    = (static_cast<int64_t>(blockIdx.x) * kWave + lane) * 8;
+  int64_t const step = static_cast<int64_t>(gridDim.y) * kWaves;
+  float sum[8]       = {};
+  if (j < cols) {
+#pragma unroll 2
+    for (int64_t i = static_cast<int64_t>(blockIdx.y) * kWaves + wave; i < rows; i += step) {
+      float g[8], v[8];
+      load8(g, grad.row(i) + j, cols - j);
+      if (z) {
+        load8(v, z.row(i) + j, cols - j);
+        with_activation(activation, [&](auto which) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) g[k] *= slope(v[k], activation);
-      if (d) store8(d.row(i) + j, g, cols - j);
+          for (int k = 0; k < 8; ++k) g[k] *= slope<decltype(which)::value>(v[k]);
+        });
+        if (d) store8(d.row(i) + j, g, cols - j);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum[k] += g[k];
     }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) sum[k] += g[k];
   }
-  if (parts) store8(parts + blockIdx.y * cols + j, sum, cols - j);
+  if (!parts) return;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) lds[wave][k][lane] = sum[k];
+  __syncthreads();
+  if (wave != 0 || j >= cols) return;
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) sum[k] += lds[w][k][lane];
+  store8(parts + blockIdx.y * cols + j, sum, cols - j);
 }
 
 // An operand of a product of `extent` rows and `depth` values of k each.
@@ -413,26 +493,48 @@ bool is_aligned(Factor<T> const& f, int64_t extent, int64_t depth)
   return reinterpret_cast<uintptr_t>(f.rows.data) % 16 == 0 && f.rows.stride % 8 == 0 && cols % 8 == 0 && f.rows.stride <= (1 << 21);
 }
 
-template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, int STAGES>
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
 void launch_tiles(Side a, bool a_next, Side b, bool b_next, int64_t m, int64_t n, int64_t depth, int64_t part, float* sums, Epilogue<T> const& end, hipStream_t stream)
 {
-  dim3 const grid(static_cast<unsigned>((m + BM - 1) / BM * ((n + BN - 1) / BN)), static_cast<unsigned>((depth + part - 1) / part));
+  dim3 const grid(static_cast<unsigned>((m + BM - 1) / BM * ((n + BN - 1) / BN)), static_cast<unsigned>(std::max<int64_t>(1, (depth + part - 1) / part)));
   dim3 const threads(WAVES_M * WAVES_N * kWave);
   if (a_next && b_next)
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, true, true, BM, BN, WAVES_M, WAVES_N, STAGES>), grid, threads, 0, stream, a, b, m, n, depth, part, sums, end);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, true, true, BM, BN, WAVES_M, WAVES_N>), grid, threads, 0, stream, a, b, m, n, depth, part, sums, end);
   else if (a_next)
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, true, false, BM, BN, WAVES_M, WAVES_N, STAGES>), grid, threads, 0, stream, a, b, m, n, depth, part, sums, end);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, true, false, BM, BN, WAVES_M, WAVES_N>), grid, threads, 0, stream, a, b, m, n, depth, part, sums, end);
   else
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, false, false, BM, BN, WAVES_M, WAVES_N, STAGES>), grid, threads, 0, stream, a, b, m, n, depth, part, sums, end);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, false, false, BM, BN, WAVES_M, WAVES_N>), grid, threads, 0, stream, a, b, m, n, depth, part, sums, end);
 }
 
-#ifndef TILE_BM
-#define TILE_BM 256
-#define TILE_BN 256
-#define TILE_WM 2
-#define TILE_WN 4
-#define TILE_ST 4
-#endif
+// How a product is shared out: tiles of 256 x 256 or of 128 x 128, and so many parts of the values of k.
+struct Plan {
+  bool large;
+  int64_t parts, part;  // values of k a part
+};
+
+// The one that takes the least by this measure, in microseconds: CUs go through their workgroups in rounds, and parts are written and
+// read once more.
+inline Plan plan_product(int64_t m, int64_t n, int64_t depth)
+{
+  int64_t const cus = device_cus(), steps = std::max<int64_t>(1, (depth + kStageK - 1) / kStageK);
+  Plan best{true, 1, std::max<int64_t>(depth, 1)};
+  double least = 1e300;
+  for (bool large : {true, false}) {
+    int64_t const edge = large ? 256 : 128, tiles = (m + edge - 1) / edge * ((n + edge - 1) / edge);
+    for (int64_t parts = 1; parts <= std::min<int64_t>(steps, 32); ++parts) {
+      int64_t const each = (steps + parts - 1) / parts, really = (steps + each - 1) / each;
+      if (really != parts) continue;
+      int64_t const load = (tiles * parts + cus - 1) / cus;  // workgroups a CU
+      double const rounds = large ? load * (each * 1.7 + 5) : (load == 1 ? each * 0.8 + 4 : load * (each * 0.6 + 3));
+      double const time   = rounds + (parts > 1 ? 5 + parts * m * n * 8e-6 / 5 : 0);
+      if (time < least) {
+        least = time;
+        best  = Plan{large, parts, each * kStageK};
+      }
+    }
+  }
+  return best;
+}
 
 // out (m x n) = a (m x depth) * b (n x depth)^T
 template <typename T>
@@ -447,8 +549,11 @@ nvtext_amd_status launch_product(Factor<T> a, Factor<T> b, int64_t m, int64_t n,
     bool const copy_a = depth > 0 && !is_aligned(a, m, depth), copy_b = depth > 0 && !is_aligned(b, n, depth);
     auto const lines  = [&](Factor<T> const& f, int64_t extent) { return f.k_next ? extent : depth; };
     auto const width  = [&](Factor<T> const& f, int64_t extent) { return ((f.k_next ? depth : extent) + 7) / 8 * 8; };
-    TempParts<2> const temp(mr, {copy_a ? static_cast<size_t>(lines(a, m) * width(a, m)) * sizeof(T) : 0, copy_b ? static_cast<size_t>(lines(b, n) * width(b, n)) * sizeof(T) : 0},
-                            copy_a || copy_b);
+    Plan const plan   = plan_product(m, n, depth);
+    TempParts<3> const temp(mr,
+                            {copy_a ? static_cast<size_t>(lines(a, m) * width(a, m)) * sizeof(T) : 0, copy_b ? static_cast<size_t>(lines(b, n) * width(b, n)) * sizeof(T) : 0,
+                             plan.parts > 1 ? static_cast<size_t>(plan.parts * m * n) * sizeof(float) : 0},
+                            copy_a || copy_b || plan.parts > 1);
     if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
     auto const align = [&](Factor<T>& f, int64_t extent, T* to) {
       int64_t const work = lines(f, extent) * width(f, extent) / 8;
@@ -458,7 +563,15 @@ nvtext_amd_status launch_product(Factor<T> a, Factor<T> b, int64_t m, int64_t n,
     };
     if (copy_a) align(a, m, temp.template part<T>(0));
     if (copy_b) align(b, n, temp.template part<T>(1));
-    launch_tiles<T, TILE_BM, TILE_BN, TILE_WM, TILE_WN, TILE_ST>(Side{a.rows.data, a.rows.stride}, a.k_next, Side{b.rows.data, b.rows.stride}, b.k_next, m, n, depth, std::max<int64_t>(depth, 1), nullptr, end, stream);
+    float* const sums = plan.parts > 1 ? temp.template part<float>(2) : nullptr;
+    Side const sa{a.rows.data, a.rows.stride}, sb{b.rows.data, b.rows.stride};
+    if (plan.large)
+      launch_tiles<T, 256, 256, 2, 4>(sa, a.k_next, sb, b.k_next, m, n, depth, plan.part, sums, end, stream);
+    else
+      launch_tiles<T, 128, 128, 2, 2>(sa, a.k_next, sb, b.k_next, m, n, depth, plan.part, sums, end, stream);
+    if (sums)
+      hipLaunchKernelGGL(join_parts_kernel<T>, dim3(static_cast<unsigned>(std::min<int64_t>((m * ((n + 7) / 8) + kThreads - 1) / kThreads, 32 * device_cus()))), dim3(kThreads), 0, stream,
+                         sums, plan.parts, m, n, end);
     return NVTEXT_AMD_SUCCESS;
   }
 }
@@ -534,7 +647,7 @@ nvtext_amd_status nvtext_amd_linear_backward(const nvtext_amd_matrix* grad, cons
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   Mr const mr{mr_, stream};
   bool const slopes   = activation != NVTEXT_AMD_ACTIVATION_NONE;
-  int64_t const parts = std::max<int64_t>(1, std::min<int64_t>(m, 256));
+  int64_t const parts = std::max<int64_t>(1, std::min<int64_t>((m + 15) / 16, 256));
   TempParts<2> const temp(mr, {slopes ? static_cast<size_t>(m * n) * type_bytes(x->type) : 0, bias_grad ? static_cast<size_t>(parts * n) * sizeof(float) : 0});
   if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
   nvtext_amd_status st = NVTEXT_AMD_SUCCESS;
@@ -545,7 +658,7 @@ nvtext_amd_status nvtext_amd_linear_backward(const nvtext_amd_matrix* grad, cons
     float* const sums = bias_grad ? temp.part<float>(1) : nullptr;
     if (n > 0 && (slopes || bias_grad)) {
       ProfileScope const scope("linear_activation_backward", stream);
-      hipLaunchKernelGGL(activation_backward_kernel<T>, dim3(static_cast<unsigned>((n + 8 * kThreads - 1) / (8 * kThreads)), static_cast<unsigned>(parts)), dim3(kThreads), 0, stream, gs,
+      hipLaunchKernelGGL(activation_backward_kernel<T>, dim3(static_cast<unsigned>((n + 8 * kWave - 1) / (8 * kWave)), static_cast<unsigned>(parts)), dim3(kThreads), 0, stream, gs,
                          slopes ? rows_of<const T>(preactivation) : Rows<const T>{nullptr, 0}, activation, m, n, d, sums);
       if (bias_grad) launch_add_parts(sums, parts, n, static_cast<T*>(bias_grad->data), stream);
     }
