@@ -157,6 +157,19 @@ struct Side {
   int64_t stride;  // in values
 };
 
+// 16 bytes a lane from base + offset (nothing but zeros where the offset is kFar) to 16 bytes a lane from `to` on.  Written out: the
+// compiler would wait for loads that it knows to write LDS before every transposing read of LDS (a product of which one operand
+// is read that way took 153 us instead of 118).  It has no register as a result, so it is waited for by stage_barrier alone.
+__device__ __forceinline__ void load_to_lds(const char* base, LdsBytes to, uint32_t offset)
+{
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  uint64_t const address = reinterpret_cast<uint64_t>(base);
+  // a buffer of kRange bytes: address, no stride, length, plain 32-bit data
+  u32x4 const buffer = {static_cast<uint32_t>(address), static_cast<uint32_t>(address >> 32) & 0xffffu, kRange, 0x00027000u};
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to))), "v"(offset), "s"(buffer)
+               : "memory");  // (m0 is set wherever the compiler uses it itself)
+}
+
 // What a wavefront loads of an operand for a stage: PIECES loads.
 template <bool K_NEXT, int EXT, int WAVES>
 struct Loader {
@@ -189,9 +202,7 @@ struct Loader {
   // Piece `p` of the next stage, of whose 64 values of k `left` are there (any number), into `to`.
   __device__ __forceinline__ void load(LdsBytes to, int64_t left, int wave, int p) const
   {
-    auto const buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), static_cast<short>(0), static_cast<int>(kRange), 0x00027000);
-    int const here    = static_cast<int>(left < kStageK ? left : kStageK);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, to + (wave * kPieces + p) * 1024, 16, k_of[p] < here ? offset[p] : kFar, 0, 0, 0);
+    load_to_lds(base, to + (wave * kPieces + p) * 1024, k_of[p] < (left < kStageK ? static_cast<int>(left) : kStageK) ? offset[p] : kFar);
   }
   __device__ __forceinline__ void next() { base += step; }
 };
