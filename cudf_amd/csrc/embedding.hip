@@ -57,60 +57,117 @@ embedding_kernel(Tokens tokens, Rows<const T> table, int64_t vocabulary, Rows<co
 
 // ------------------------------------------------------------------ tokens in the order of their ids
 // A stable sort: tokens of one id stay in their order, so that sums over them are added in one order at every call.  Least
-// significant digit first, eight bits a pass: count the digits of every tile, add the counts up digit by digit, place.
-constexpr int kDigitBits = 8;
-constexpr int kDigits    = 1 << kDigitBits;
-constexpr int kTile      = 2048;
-constexpr int kRounds    = kTile / kThreads;
+// significant digit first, eight bits a pass: count the digits of every tile, then place, for which every workgroup adds up the
+// counts that it needs (of more than kDirectTiles tiles, device_exclusive_scan does).  Up to a tile of tokens is sorted by one
+// workgroup, in LDS: one launch.
+constexpr int kDigitBits      = 8;
+constexpr int kDigits         = 1 << kDigitBits;
+constexpr int kSortThreads    = 1024;
+constexpr int kSortWaves      = kSortThreads / kWave;
+constexpr int kTile           = 8192;
+constexpr int kRounds         = kTile / kSortThreads;
+constexpr int kDirectTiles    = 256;
 
 struct Sorted {
   uint32_t* keys;  // id, or the size of the vocabulary for what belongs to no entry
   uint32_t* tokens;
 };
 
-__global__ void __launch_bounds__(kThreads) token_keys_kernel(Tokens tokens, uint32_t vocabulary, Sorted out)
+// Where a pass reads: the column itself at first.
+struct Unsorted {
+  Tokens column;
+  uint32_t vocabulary;
+  __device__ __forceinline__ uint32_t key(int64_t t) const
+  {
+    uint32_t const id = static_cast<uint32_t>(column.ids[t]);
+    bool const inside = column.rows > 0 && t >= column.offsets[0] && t < column.offsets[column.rows];
+    return inside && id < vocabulary ? id : vocabulary;
+  }
+  __device__ __forceinline__ uint32_t token(int64_t t) const { return static_cast<uint32_t>(t); }
+};
+struct Half {
+  Sorted from;
+  __device__ __forceinline__ uint32_t key(int64_t i) const { return from.keys[i]; }
+  __device__ __forceinline__ uint32_t token(int64_t i) const { return from.tokens[i]; }
+};
+
+// Of the wavefront's 64 keys (`here`: there is one): the lanes that have the same digit.
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, bool here)
 {
-  int64_t const t = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (t >= tokens.count) return;
-  uint32_t const id = static_cast<uint32_t>(tokens.ids[t]);
-  bool const inside = tokens.rows > 0 && t >= tokens.offsets[0] && t < tokens.offsets[tokens.rows];
-  out.keys[t]       = inside && id < vocabulary ? id : vocabulary;
-  out.tokens[t]     = static_cast<uint32_t>(t);
+  uint64_t same = ballot64(here);
+#pragma unroll
+  for (int bit = 0; bit < kDigitBits; ++bit) {
+    bool const set        = (digit >> bit) & 1u;
+    uint64_t const others = ballot64(set);
+    same &= set ? others : ~others;
+  }
+  return same;
 }
 
-__global__ void __launch_bounds__(kThreads) digit_counts_kernel(const uint32_t* keys, int32_t n, int shift, int32_t tiles, uint32_t* counts)
+// counts[tile][digit], or [digit][tile] for the scan
+template <typename From>
+__global__ void __launch_bounds__(kSortThreads) digit_counts_kernel(From from, int32_t n, int shift, int32_t tiles, bool by_digit, uint32_t* counts)
 {
   __shared__ uint32_t lds[kDigits];
-  lds[threadIdx.x] = 0;
+  if (threadIdx.x < kDigits) lds[threadIdx.x] = 0;
   __syncthreads();
+#pragma unroll
   for (int r = 0; r < kRounds; ++r) {
-    int64_t const i = static_cast<int64_t>(blockIdx.x) * kTile + r * kThreads + threadIdx.x;
-    if (i < n) atomicAdd(&lds[(keys[i] >> shift) & (kDigits - 1)], 1u);
+    int64_t const i = static_cast<int64_t>(blockIdx.x) * kTile + r * kSortThreads + threadIdx.x;
+    if (i < n) atomicAdd(&lds[(from.key(i) >> shift) & (kDigits - 1)], 1u);
   }
   __syncthreads();
-  counts[static_cast<int64_t>(threadIdx.x) * tiles + blockIdx.x] = lds[threadIdx.x];
+  if (threadIdx.x < kDigits) counts[by_digit ? static_cast<int64_t>(threadIdx.x) * tiles + blockIdx.x : static_cast<int64_t>(blockIdx.x) * kDigits + threadIdx.x] = lds[threadIdx.x];
 }
 
-__global__ void __launch_bounds__(kThreads) digit_place_kernel(Sorted in, int32_t n, int shift, int32_t tiles, const uint32_t* places, Sorted out)
+// `summed`: counts[digit][tile] are places already.
+template <typename From>
+__global__ void __launch_bounds__(kSortThreads) digit_place_kernel(From from, int32_t n, int shift, int32_t tiles, bool summed, const uint32_t* counts, Sorted out)
 {
-  __shared__ uint32_t lds[kWaves][kDigits];
+  __shared__ uint32_t lds[kSortWaves][kDigits];
+  __shared__ uint32_t before[4][kDigits], all[4][kDigits], scan[kSortWaves + 1];
   int const wave = threadIdx.x / kWave, lane = lane_id();
-  for (int w = 0; w < kWaves; ++w) lds[w][threadIdx.x] = 0;
+  for (int w = threadIdx.x / kDigits; w < kSortWaves; w += kSortThreads / kDigits) lds[w][threadIdx.x % kDigits] = 0;
   __syncthreads();
   // a wavefront's keys are consecutive, 64 a round
   uint32_t key[kRounds];
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
     int64_t const i = static_cast<int64_t>(blockIdx.x) * kTile + (wave * kRounds + r) * kWave + lane;
-    key[r]          = i < n ? in.keys[i] : 0;
+    key[r]          = i < n ? from.key(i) : 0;
     if (i < n) atomicAdd(&lds[wave][(key[r] >> shift) & (kDigits - 1)], 1u);
   }
-  __syncthreads();
-  uint32_t place = places[static_cast<int64_t>(threadIdx.x) * tiles + blockIdx.x];
-  for (int w = 0; w < kWaves; ++w) {
-    uint32_t const count = lds[w][threadIdx.x];
-    lds[w][threadIdx.x]  = place;
-    place += count;
+  uint32_t place = 0;
+  if (summed) {
+    if (threadIdx.x < kDigits) place = counts[static_cast<int64_t>(threadIdx.x) * tiles + blockIdx.x];
+    __syncthreads();
+  } else {
+    // four threads a digit add up the tiles' counts: those before this one, and all
+    int const part = threadIdx.x / kDigits, digit = threadIdx.x % kDigits;
+    uint32_t mine = 0, every = 0;
+#pragma unroll 8
+    for (int32_t t = part; t < tiles; t += 4) {
+      uint32_t const c = counts[static_cast<int64_t>(t) * kDigits + digit];
+      every += c;
+      mine += t < static_cast<int32_t>(blockIdx.x) ? c : 0;
+    }
+    before[part][digit] = mine;
+    all[part][digit]    = every;
+    __syncthreads();
+    uint32_t total = 0, behind = 0;
+    if (threadIdx.x < kDigits) {
+      every = all[0][digit] + all[1][digit] + all[2][digit] + all[3][digit];
+      mine  = before[0][digit] + before[1][digit] + before[2][digit] + before[3][digit];
+    }
+    behind = block_exclusive_scan<kSortThreads>(threadIdx.x < kDigits ? every : 0, scan, &total);
+    place  = behind + mine;
+  }
+  if (threadIdx.x < kDigits) {
+    for (int w = 0; w < kSortWaves; ++w) {
+      uint32_t const count = lds[w][threadIdx.x];
+      lds[w][threadIdx.x]  = place;
+      place += count;
+    }
   }
   __syncthreads();
 #pragma unroll
@@ -118,21 +175,83 @@ __global__ void __launch_bounds__(kThreads) digit_place_kernel(Sorted in, int32_
     int64_t const i      = static_cast<int64_t>(blockIdx.x) * kTile + (wave * kRounds + r) * kWave + lane;
     bool const here      = i < n;
     uint32_t const digit = (key[r] >> shift) & (kDigits - 1);
-    uint64_t same        = ballot64(here);
-#pragma unroll
-    for (int bit = 0; bit < kDigitBits; ++bit) {
-      bool const set        = (digit >> bit) & 1u;
-      uint64_t const others = ballot64(set);
-      same &= set ? others : ~others;
-    }
-    uint32_t at = 0;
+    uint64_t const same  = same_digit(digit, here);
+    uint32_t at          = 0;
     if (here) at = lds[wave][digit] + lanes_below(same);
     wave_lds_fence();
     if (here && lanes_below(same) == 0) lds[wave][digit] += static_cast<uint32_t>(__builtin_popcountll(same));
     wave_lds_fence();
     if (here) {
       out.keys[at]   = key[r];
-      out.tokens[at] = in.tokens[i];
+      out.tokens[at] = from.token(i);
+    }
+  }
+}
+
+// All passes over up to a tile of tokens.
+__global__ void __launch_bounds__(kSortThreads) small_sort_kernel(Unsorted from, int32_t n, Sorted out)
+{
+  __shared__ uint32_t lds[kSortWaves][kDigits];
+  __shared__ uint32_t keys[kTile];
+  __shared__ uint16_t tokens[kTile];
+  __shared__ uint32_t scan[kSortWaves + 1];
+  int const wave = threadIdx.x / kWave, lane = lane_id();
+  uint32_t key[kRounds], token[kRounds];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    int const i = (wave * kRounds + r) * kWave + lane;
+    key[r]      = i < n ? from.key(i) : 0;
+    token[r]    = i;
+  }
+  for (int shift = 0; shift < 32 && (from.vocabulary >> shift) != 0; shift += kDigitBits) {
+    for (int w = threadIdx.x / kDigits; w < kSortWaves; w += kSortThreads / kDigits) lds[w][threadIdx.x % kDigits] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r)
+      if ((wave * kRounds + r) * kWave + lane < n) atomicAdd(&lds[wave][(key[r] >> shift) & (kDigits - 1)], 1u);
+    __syncthreads();
+    uint32_t every = 0, total;
+    if (threadIdx.x < kDigits)
+      for (int w = 0; w < kSortWaves; ++w) every += lds[w][threadIdx.x];
+    uint32_t place = block_exclusive_scan<kSortThreads>(every, scan, &total);
+    if (threadIdx.x < kDigits)
+      for (int w = 0; w < kSortWaves; ++w) {
+        uint32_t const count = lds[w][threadIdx.x];
+        lds[w][threadIdx.x]  = place;
+        place += count;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      bool const here      = (wave * kRounds + r) * kWave + lane < n;
+      uint32_t const digit = (key[r] >> shift) & (kDigits - 1);
+      uint64_t const same  = same_digit(digit, here);
+      uint32_t at          = 0;
+      if (here) at = lds[wave][digit] + lanes_below(same);
+      wave_lds_fence();
+      if (here && lanes_below(same) == 0) lds[wave][digit] += static_cast<uint32_t>(__builtin_popcountll(same));
+      wave_lds_fence();
+      if (here) {
+        keys[at]   = key[r];
+        tokens[at] = static_cast<uint16_t>(token[r]);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      int const i = (wave * kRounds + r) * kWave + lane;
+      if (i < n) {
+        key[r]   = keys[i];
+        token[r] = tokens[i];
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    int const i = (wave * kRounds + r) * kWave + lane;
+    if (i < n) {
+      out.keys[i]   = key[r];
+      out.tokens[i] = token[r];
     }
   }
 }
@@ -142,124 +261,272 @@ struct Counts {
   __device__ uint64_t operator()(int64_t i) const { return counts[i]; }
 };
 
-// ------------------------------------------------------------------ the table's gradient
-// The sorted tokens are cut into chunks of kChunk.  A wavefront adds up the gradients of a chunk, id by id, 512 columns at a
-// time; an id whose tokens all lie in the chunk is done then, the sums of others go to the chunk's two places: the first for
-// an id that began in a chunk before, the second for one that begins here and goes on.
-constexpr int kChunk = 32;
+// ------------------------------------------------------------------ the tables' gradients
+// Columns are taken 256 at a time, a slice: VEC = 4 values a lane, and the lanes behind the last column take the last four once more,
+// so that no load has a condition.  (Of less than four columns, VEC = 1.)
+constexpr int kAhead     = 16;  // rows of the gradient that a wavefront asks for before it adds the first
+constexpr int kSumWaves  = 8;
+constexpr int kSumThreads = kSumWaves * kWave;
+// The sorted tokens are cut into chunks, a token a lane.  A wavefront adds up the gradients of a chunk, id by id; an id whose
+// tokens all lie in the chunk is done then, the sums of others go to the chunk's two places: the first for an id that began in a
+// chunk before, the second for one that begins here and goes on.
+constexpr int kChunk = kWave;
 
-template <typename T, typename G>
-__global__ void __launch_bounds__(kThreads)
-chunk_sums_kernel(Sorted sorted, int32_t n, uint32_t vocabulary, Rows<const T> grad, int64_t cols, float* parts, Rows<G> out)
+template <typename T, int VEC>
+struct Some {
+  typedef T type __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
+};
+template <typename T, int VEC>
+using some_t = typename Some<T, VEC>::type;
+
+template <typename T, int VEC>
+__device__ __forceinline__ void add(float (&f)[VEC], some_t<T, VEC> const& v)
 {
-  int32_t const chunk = static_cast<int32_t>(blockIdx.x) * kWaves + static_cast<int32_t>(threadIdx.x) / kWave;
-  int64_t const first = static_cast<int64_t>(chunk) * kChunk;
-  if (first >= n) return;
-  int64_t const last = std::min<int64_t>(first + kChunk, n);
-  int64_t const j    = (static_cast<int64_t>(blockIdx.y) * kWave + lane_id()) * 8;
-  float f[8]         = {};
-  bool begun         = first == 0 || sorted.keys[first - 1] != sorted.keys[first];
-  for (int64_t i = first; i < last; ++i) {
-    uint32_t const id = sorted.keys[i];
-    if (id >= vocabulary) break;
-    float g[8];
-    if (j < cols) {
-      load8(g, grad.row(sorted.tokens[i]) + j, cols - j);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] += g[k];
-    }
-    bool const ends = i + 1 == n || sorted.keys[i + 1] != id;
-    if (!ends && i + 1 < last) continue;
-    if (j < cols) {
-      if (begun && ends)
-        store8(out.row(id) + j, f, cols - j);
-      else
-        store8(parts + (2 * static_cast<int64_t>(chunk) + (begun ? 1 : 0)) * cols + j, f, cols - j);
-    }
+  for (int k = 0; k < VEC; ++k) f[k] += static_cast<float>(v[k]);
+}
+template <int VEC, typename T>
+__device__ __forceinline__ some_t<T, VEC> load_some(const T* p)
+{
+  return *reinterpret_cast<const some_t<T, VEC>*>(p);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_some(T* p, float const (&f)[VEC])
+{
+  some_t<T, VEC> v;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = 0.f;
-    begun = true;
-  }
+  for (int k = 0; k < VEC; ++k) v[k] = static_cast<T>(f[k]);
+  *reinterpret_cast<some_t<T, VEC>*>(p) = v;
 }
 
-// A wavefront a chunk: if an id begins in it and goes on into the next, its parts are added up, chunk after chunk.
-template <typename G>
-__global__ void __launch_bounds__(kThreads) join_chunks_kernel(Sorted sorted, int32_t n, uint32_t vocabulary, int64_t cols, const float* parts, Rows<G> out)
+// What the sums are made from and where they go.
+template <typename T, typename G>
+struct Sums {
+  Sorted sorted;
+  int32_t n, chunks;
+  uint32_t vocabulary;
+  Tokens column;
+  Rows<const T> grad;
+  int64_t cols;
+  Rows<G> tokens;
+  float* token_parts;  // [chunk][2][cols]
+  int32_t places, groups, group;  // positions, runs of rows, rows a run
+  Rows<G> positions;
+  float* position_parts;  // [run][place][cols], where there are several
+};
+
+// A wavefront a chunk.
+template <int VEC, typename T, typename G>
+__device__ __forceinline__ void add_chunk(Sums<T, G> const& s, int32_t chunk, int64_t j)
 {
-  int32_t const chunk = static_cast<int32_t>(blockIdx.x) * kWaves + static_cast<int32_t>(threadIdx.x) / kWave;
-  int64_t const first = static_cast<int64_t>(chunk) * kChunk, last = first + kChunk;
-  if (last >= n) return;
-  uint32_t const id = sorted.keys[last];
-  if (id >= vocabulary || sorted.keys[last - 1] != id) return;
-  if (sorted.keys[first] == id && first > 0 && sorted.keys[first - 1] == id) return;  // it began before
-  int64_t const j = (static_cast<int64_t>(blockIdx.y) * kWave + lane_id()) * 8;
-  if (j >= cols) return;
-  float f[8];
-  load8(f, parts + (2 * static_cast<int64_t>(chunk) + 1) * cols + j, cols - j);
-  for (int64_t c = chunk + 1; c * kChunk < n && sorted.keys[c * kChunk] == id; ++c) {
-    float g[8];
-    load8(g, parts + 2 * c * cols + j, cols - j);
+  int const lane      = lane_id();
+  int64_t const first = static_cast<int64_t>(chunk) * kChunk;
+  int64_t const i     = first + lane;
+  uint32_t const none = 0xffffffffu;  // (no key)
+  uint32_t const key = i < s.n ? s.sorted.keys[i] : none, token = i < s.n ? s.sorted.tokens[i] : 0;
+  uint32_t const behind = i + 1 < s.n ? s.sorted.keys[i + 1] : none;
+  uint64_t const ends   = ballot64(key != behind);
+  int const count       = __builtin_popcountll(ballot64(key < s.vocabulary));  // (the lowest ones)
+  bool begun            = first == 0 || s.sorted.keys[first - 1] != wave_bcast(key, 0);
+  float f[VEC]          = {};
+  for (int base = 0; base < count; base += kAhead) {
+    some_t<T, VEC> g[kAhead];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] += g[k];
+    for (int u = 0; u < kAhead; ++u) g[u] = load_some<VEC>(s.grad.row(wave_bcast(token, base + u)) + j);  // (kAhead divides kChunk; what is not counted is some row all the same)
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (base + u < count) {
+        add<T, VEC>(f, g[u]);
+        bool const end = (ends >> (base + u)) & 1u;
+        if (end || base + u + 1 == count) {
+          if (begun && end)
+            store_some<G, VEC>(s.tokens.row(wave_bcast(key, base + u)) + j, f);
+          else
+            store_some<float, VEC>(s.token_parts + (2 * static_cast<int64_t>(chunk) + (begun ? 1 : 0)) * s.cols + j, f);
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) f[k] = 0.f;
+          begun = true;
+        }
+      }
+    }
   }
-  store8(out.row(id) + j, f, cols - j);
 }
 
 // Zeros for the entries that do not occur: a wavefront looks 64 of them up in the sorted ids.
-template <typename G>
-__global__ void __launch_bounds__(kThreads) absent_rows_kernel(Sorted sorted, int32_t n, uint32_t vocabulary, int64_t cols, Rows<G> out)
+template <int VEC, typename T, typename G>
+__device__ __forceinline__ void clear_absent(Sums<T, G> const& s, int64_t first, int64_t j)
 {
-  int64_t const first = (static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / kWave) * kWave;
-  if (first >= vocabulary) return;
   uint32_t const id = static_cast<uint32_t>(first) + lane_id();
-  int32_t lo = 0, hi = n;
+  int32_t lo = 0, hi = s.n;
   while (lo < hi) {
     int32_t const mid = lo + (hi - lo) / 2;
-    if (sorted.keys[mid] < id)
+    if (s.sorted.keys[mid] < id)
       lo = mid + 1;
     else
       hi = mid;
   }
-  uint64_t absent     = ballot64(id < vocabulary && (lo >= n || sorted.keys[lo] != id));
-  float const zero[8] = {};
-  for (; absent; absent &= absent - 1) {
-    int64_t const row = first + __builtin_ctzll(absent);
-    for (int64_t j = lane_id() * 8; j < cols; j += kWave * 8) store8(out.row(row) + j, zero, cols - j);
-  }
+  uint64_t absent       = ballot64(id < s.vocabulary && (lo >= s.n || s.sorted.keys[lo] != id));
+  float const zero[VEC] = {};
+  for (; absent; absent &= absent - 1) store_some<G, VEC>(s.tokens.row(first + __builtin_ctzll(absent)) + j, zero);
 }
 
-// ------------------------------------------------------------------ the positions' gradient
-// A workgroup a place and 512 columns: its wavefronts share the rows that are long enough, and add up what they found in the end.
-template <typename T, typename G>
-__global__ void __launch_bounds__(kThreads) position_sums_kernel(Tokens tokens, Rows<const T> grad, int64_t places, int64_t cols, Rows<G> out)
+// A workgroup a place and a run of rows: its wavefronts share the rows that are long enough, and add up what they found in the end.
+template <int VEC, typename T, typename G>
+__device__ __forceinline__ void add_place(Sums<T, G> const& s, int32_t place, int32_t run, int64_t j, float (*lds)[VEC * kWave])
 {
-  __shared__ float lds[kWaves][8 * kWave];
   int const wave = threadIdx.x / kWave, lane = lane_id();
-  int64_t const at = blockIdx.x;
-  int64_t const j  = (static_cast<int64_t>(blockIdx.y) * kWave + lane) * 8;
-  float f[8]       = {};
-  for (int64_t base = wave * kWave; base < tokens.rows; base += kThreads) {
-    int64_t const r   = base + lane;
-    int64_t const t   = r < tokens.rows ? tokens.offsets[r] + at : 0;
-    uint64_t enough   = ballot64(r < tokens.rows && t >= 0 && t < tokens.offsets[r + 1] && t < tokens.count);
-    for (; enough; enough &= enough - 1) {
-      int64_t const token = wave_bcast(static_cast<uint32_t>(t), __builtin_ctzll(enough));
-      float g[8];
-      if (j < cols) {
-        load8(g, grad.row(token) + j, cols - j);
+  int64_t const first = static_cast<int64_t>(run) * s.group, last = first + s.group < s.column.rows ? first + s.group : s.column.rows;
+  float f[VEC] = {};
+  for (int64_t base = first + wave * kWave; base < last; base += kSumThreads) {
+    int64_t const r = base + lane;
+    int64_t const t = r < last ? static_cast<int64_t>(s.column.offsets[r]) + place : 0;
+    uint64_t enough = ballot64(r < last && t >= 0 && t < s.column.offsets[r + 1] && t < s.n);
+    while (enough) {
+      some_t<T, VEC> g[kAhead];
+      int const count = __builtin_popcountll(enough);
+      int at          = 0;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) f[k] += g[k];
+      for (int u = 0; u < kAhead; ++u) {
+        if (enough) at = __builtin_ctzll(enough);  // (else the last one again, which is not counted)
+        enough &= enough - 1;
+        g[u] = load_some<VEC>(s.grad.row(wave_bcast(static_cast<uint32_t>(t), at)) + j);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (u < count) add<T, VEC>(f, g[u]);
       }
     }
   }
 #pragma unroll
-  for (int k = 0; k < 8; ++k) lds[wave][k * kWave + lane] = f[k];
+  for (int k = 0; k < VEC; ++k) lds[wave][k * kWave + lane] = f[k];
   __syncthreads();
-  if (wave == 0 && j < cols) {
+  if (wave != 0) return;
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      for (int w = 1; w < kWaves; ++w) f[k] += lds[w][k * kWave + lane];
-    store8(out.row(at) + j, f, cols - j);
+  for (int k = 0; k < VEC; ++k)
+#pragma unroll
+    for (int w = 1; w < kSumWaves; ++w) f[k] += lds[w][k * kWave + lane];
+  if (s.groups == 1)
+    store_some<G, VEC>(s.positions.row(place) + j, f);
+  else
+    store_some<float, VEC>(s.position_parts + (static_cast<int64_t>(run) * s.places + place) * s.cols + j, f);
+}
+
+// The first of a lane's columns in a slice.
+template <int VEC>
+__device__ __forceinline__ int64_t columns_of(int64_t slice, int64_t cols)
+{
+  int64_t const j = (slice * kWave + lane_id()) * VEC;
+  return j + VEC <= cols ? j : cols - VEC;
+}
+
+// Slice after slice, so that what both sums read of a slice is read once from memory and once from the cache behind L2: places first,
+// which take longest, then chunks, then what does not occur.
+template <int VEC, typename T, typename G>
+__global__ void __launch_bounds__(kSumThreads) embedding_sums_kernel(Sums<T, G> s)
+{
+  __shared__ float lds[kSumWaves][VEC * kWave];
+  int64_t const of_places = static_cast<int64_t>(s.places) * s.groups, of_chunks = (s.chunks + kSumWaves - 1) / kSumWaves;
+  int64_t const of_slice = of_places + of_chunks + (static_cast<int64_t>(s.vocabulary) + kSumThreads - 1) / kSumThreads;
+  int64_t const j        = columns_of<VEC>(blockIdx.x / of_slice, s.cols);
+  int64_t at             = blockIdx.x % of_slice;
+  int const wave         = threadIdx.x / kWave;
+  if (at < of_places) {
+    add_place<VEC>(s, static_cast<int32_t>(at / s.groups), static_cast<int32_t>(at % s.groups), j, lds);
+  } else if (at -= of_places; at < of_chunks) {
+    int64_t const chunk = at * kSumWaves + wave;
+    if (chunk < s.chunks) add_chunk<VEC>(s, static_cast<int32_t>(chunk), j);
+  } else {
+    int64_t const first = ((at - of_chunks) * kSumWaves + wave) * kWave;
+    if (first < s.vocabulary) clear_absent<VEC>(s, first, j);
+  }
+}
+
+// Adds up parts[0], parts[step], ... `count` (> 0) of them, kAhead asked for at a time.
+template <int VEC>
+__device__ __forceinline__ void add_rows(float (&f)[VEC], const float* parts, int64_t step, int64_t count)
+{
+  for (int64_t base = 0; base < count; base += kAhead) {
+    some_t<float, VEC> g[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) g[u] = load_some<VEC>(parts + (base + u < count ? base + u : base) * step);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (base + u < count) add<float, VEC>(f, g[u]);
+    }
+  }
+}
+
+// Joins the parts: of an id that begins in a chunk and goes on into others, by a wavefront, or, where these are many, by all of the
+// workgroup's; and of the places, where rows were cut into runs.
+template <int VEC, typename T, typename G>
+__global__ void __launch_bounds__(kSumThreads) embedding_join_kernel(Sums<T, G> s)
+{
+  __shared__ float lds[kSumWaves][VEC * kWave];
+  __shared__ int32_t length[kSumWaves];
+  constexpr int32_t kAlone = 32;  // parts that a wavefront adds up by itself
+  int64_t const of_chunks = (s.chunks + kSumWaves - 1) / kSumWaves;
+  int64_t const of_places = s.groups > 1 ? (s.places + kSumWaves - 1) / kSumWaves : 0;
+  int const wave = threadIdx.x / kWave, lane = lane_id();
+  int64_t const j  = columns_of<VEC>(blockIdx.x / (of_chunks + of_places), s.cols);
+  int64_t const at = blockIdx.x % (of_chunks + of_places);
+  float f[VEC]     = {};
+  if (at >= of_chunks) {
+    int64_t const place = (at - of_chunks) * kSumWaves + wave;
+    if (place >= s.places) return;
+    add_rows<VEC>(f, s.position_parts + place * s.cols + j, static_cast<int64_t>(s.places) * s.cols, s.groups);
+    store_some<G, VEC>(s.positions.row(place) + j, f);
+    return;
+  }
+  auto const parts_of = [&](int64_t chunk) { return s.token_parts + (2 * chunk + 1) * s.cols + j; };  // the second of its places, the first ones of the next lie behind
+  int64_t const chunk = at * kSumWaves + wave;
+  int64_t const first = chunk * kChunk, last = first + kChunk;
+  int32_t more        = 0;  // chunks that the id goes on into
+  uint32_t id         = 0;
+  if (last < s.n) {
+    id                 = s.sorted.keys[last];
+    bool const goes_on = id < s.vocabulary && s.sorted.keys[last - 1] == id;
+    if (goes_on && (first == 0 || s.sorted.keys[first] != id || s.sorted.keys[first - 1] != id)) {
+      for (;;) {
+        int64_t const next  = last + (static_cast<int64_t>(more) + lane) * kChunk;
+        uint64_t const same = ballot64(next < s.n && s.sorted.keys[next < s.n ? next : 0] == id);
+        int const run       = same == ~0ull ? kWave : __builtin_ctzll(~same);
+        more += run;
+        if (run < kWave) break;
+      }
+    }
+  }
+  auto const begin = [&](const float* part) {
+    auto const v = load_some<VEC>(part);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) f[k] = v[k];
+  };
+  if (more > 0 && more <= kAlone) {
+    begin(parts_of(chunk));
+    add_rows<VEC>(f, parts_of(chunk) + s.cols, 2 * s.cols, more);
+    store_some<G, VEC>(s.tokens.row(id) + j, f);
+  }
+  if (lane == 0) length[wave] = more;
+  __syncthreads();
+  for (int w = 0; w < kSumWaves; ++w) {
+    if (length[w] <= kAlone) continue;
+    int64_t const from = at * kSumWaves + w, each = (length[w] + kSumWaves - 1) / kSumWaves, mine = wave * each;
+    int64_t const here = mine + each < length[w] ? each : length[w] - mine;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) f[k] = 0.f;
+    if (wave == 0) begin(parts_of(from));
+    if (here > 0) add_rows<VEC>(f, parts_of(from) + s.cols + 2 * mine * s.cols, 2 * s.cols, here);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) lds[wave][k * kWave + lane] = f[k];
+    __syncthreads();
+    if (wave == w) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        f[k] = 0.f;
+        for (int v = 0; v < kSumWaves; ++v) f[k] += lds[v][k * kWave + lane];
+      }
+      store_some<G, VEC>(s.tokens.row(id) + j, f);
+    }
+    __syncthreads();
   }
 }
 
@@ -328,44 +595,68 @@ nvtext_amd_status nvtext_amd_embedding_backward(const nvtext_amd_list_column* to
   uint32_t const vocabulary = static_cast<uint32_t>(token_grad->rows);
   int32_t const n           = view.count;
   int64_t const cols        = grad->cols;
+  bool const small          = n <= kTile;
   int32_t const tiles       = (n + kTile - 1) / kTile;
-  int64_t const chunks      = (static_cast<int64_t>(n) + kChunk - 1) / kChunk;
+  bool const direct         = tiles <= kDirectTiles;
+  int32_t const chunks      = vocabulary > 0 ? static_cast<int32_t>((static_cast<int64_t>(n) + kChunk - 1) / kChunk) : 0;
   int64_t const counts      = static_cast<int64_t>(tiles) * kDigits;
-  unsigned const slices     = static_cast<unsigned>((cols + 8 * kWave - 1) / (8 * kWave));
-  size_t const list         = static_cast<size_t>(n) * sizeof(uint32_t);
-  TempParts<7> const temp(mr, {list, list, list, list, static_cast<size_t>(counts + 1) * sizeof(uint32_t), scan_temp_bytes(counts), static_cast<size_t>(2 * chunks * cols) * sizeof(float)});
+  int64_t const vec         = cols >= 4 ? 4 : 1, slices = (cols + vec * kWave - 1) / (vec * kWave);
+  // Rows in runs of 2,048 or, if these were more than 16, in 16 runs: a place's rows are read by one workgroup a run, 30 us for 2,048.
+  int32_t const places = position_grad ? static_cast<int32_t>(position_grad->rows) : 0;
+  int32_t const group  = std::max<int32_t>(2048, static_cast<int32_t>((static_cast<int64_t>(view.rows) + 15) / 16));
+  int32_t const groups = std::max<int32_t>(1, static_cast<int32_t>((static_cast<int64_t>(view.rows) + group - 1) / group));
+  size_t const list    = static_cast<size_t>(n) * sizeof(uint32_t);
+  TempParts<8> const temp(mr, {list, list, small ? 0 : list, small ? 0 : list, small ? 0 : static_cast<size_t>(counts + 1) * sizeof(uint32_t), direct ? 0 : scan_temp_bytes(counts),
+                               static_cast<size_t>(2 * cols) * static_cast<size_t>(chunks > 1 ? chunks : 0) * sizeof(float),
+                               groups > 1 ? static_cast<size_t>(groups) * static_cast<size_t>(places * cols) * sizeof(float) : 0});
   if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
   Sorted sorted{temp.part<uint32_t>(0), temp.part<uint32_t>(1)}, other{temp.part<uint32_t>(2), temp.part<uint32_t>(3)};
-  if (n > 0 && vocabulary > 0) {
+  if (chunks > 0) {
     ProfileScope const scope("embedding_sort", stream);
-    hipLaunchKernelGGL(token_keys_kernel, dim3((n + kThreads - 1) / kThreads), dim3(kThreads), 0, stream, view, vocabulary, sorted);
-    for (int shift = 0; shift < 32 && (vocabulary >> shift) != 0; shift += kDigitBits) {
-      uint32_t* const places = temp.part<uint32_t>(4);
-      hipLaunchKernelGGL(digit_counts_kernel, dim3(tiles), dim3(kThreads), 0, stream, sorted.keys, n, shift, tiles, places);
-      device_exclusive_scan(Counts{places}, counts, places, temp.part<uint64_t>(5), stream, TellNobody{});
-      hipLaunchKernelGGL(digit_place_kernel, dim3(tiles), dim3(kThreads), 0, stream, sorted, n, shift, tiles, places, other);
-      std::swap(sorted, other);
+    Unsorted const column{view, vocabulary};
+    if (small) {
+      hipLaunchKernelGGL(small_sort_kernel, dim3(1), dim3(kSortThreads), 0, stream, column, n, sorted);
+    } else {
+      uint32_t* const places_of = temp.part<uint32_t>(4);
+      auto const pass           = [&](auto from, int shift, Sorted to) {
+        using From = decltype(from);
+        hipLaunchKernelGGL(digit_counts_kernel<From>, dim3(tiles), dim3(kSortThreads), 0, stream, from, n, shift, tiles, !direct, places_of);
+        if (!direct) device_exclusive_scan(Counts{places_of}, counts, places_of, temp.part<uint64_t>(5), stream, TellNobody{});
+        hipLaunchKernelGGL(digit_place_kernel<From>, dim3(tiles), dim3(kSortThreads), 0, stream, from, n, shift, tiles, !direct, places_of, to);
+      };
+      pass(column, 0, sorted);
+      for (int shift = kDigitBits; shift < 32 && (vocabulary >> shift) != 0; shift += kDigitBits) {
+        pass(Half{sorted}, shift, other);
+        std::swap(sorted, other);
+      }
     }
   }
   with_type(grad->type, [&](auto zero) {
     using T         = decltype(zero);
     auto const sums = [&](auto result) {
-      using G            = decltype(result);
-      float* const parts = temp.part<float>(6);
-      dim3 const by_chunk(static_cast<unsigned>((chunks + kWaves - 1) / kWaves), slices);
-      if (n > 0 && vocabulary > 0) {
-        ProfileScope const scope("embedding_token_sums", stream);
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(chunk_sums_kernel<T, G>), by_chunk, dim3(kThreads), 0, stream, sorted, n, vocabulary, rows_of<const T>(grad), cols, parts, rows_of<G>(token_grad));
-        hipLaunchKernelGGL(join_chunks_kernel<G>, by_chunk, dim3(kThreads), 0, stream, sorted, n, vocabulary, cols, parts, rows_of<G>(token_grad));
+      using G = decltype(result);
+      Sums<T, G> const s{sorted, n, chunks, vocabulary, view, rows_of<const T>(grad), cols, rows_of<G>(token_grad), temp.part<float>(6), places, groups, group,
+                         rows_of<G>(position_grad), temp.part<float>(7)};
+      int64_t const of_chunks = (chunks + kSumWaves - 1) / kSumWaves;
+      int64_t const all = slices * (static_cast<int64_t>(places) * groups + of_chunks + (static_cast<int64_t>(vocabulary) + kSumThreads - 1) / kSumThreads);
+      if (all > 0) {
+        ProfileScope const scope("embedding_sums", stream);
+        dim3 const grid(static_cast<unsigned>(all)), threads(kSumThreads);
+        if (vec == 4)
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(embedding_sums_kernel<4, T, G>), grid, threads, 0, stream, s);
+        else
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(embedding_sums_kernel<1, T, G>), grid, threads, 0, stream, s);
       }
-      if (vocabulary > 0) {
-        ProfileScope const scope("embedding_absent_rows", stream);
-        hipLaunchKernelGGL(absent_rows_kernel<G>, dim3((vocabulary + kThreads - 1) / kThreads), dim3(kThreads), 0, stream, sorted, n, vocabulary, cols, rows_of<G>(token_grad));
-      }
-      if (position_grad && position_grad->rows > 0) {
-        ProfileScope const scope("embedding_position_sums", stream);
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(position_sums_kernel<T, G>), dim3(static_cast<unsigned>(position_grad->rows), slices), dim3(kThreads), 0, stream, view, rows_of<const T>(grad),
-                           position_grad->rows, cols, rows_of<G>(position_grad));
+      int64_t const joins = slices * ((chunks > 1 ? of_chunks : 0) + (groups > 1 ? (places + kSumWaves - 1) / kSumWaves : 0));
+      if (joins > 0) {
+        ProfileScope const scope("embedding_join", stream);
+        Sums<T, G> some = s;
+        if (chunks <= 1) some.chunks = 0;
+        dim3 const grid(static_cast<unsigned>(joins)), threads(kSumThreads);
+        if (vec == 4)
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(embedding_join_kernel<4, T, G>), grid, threads, 0, stream, some);
+        else
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(embedding_join_kernel<1, T, G>), grid, threads, 0, stream, some);
       }
     };
     if (token_grad->type == NVTEXT_AMD_TYPE_FLOAT32)

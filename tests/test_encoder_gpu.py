@@ -113,7 +113,8 @@ def test_embedding_of_the_tokenizers_result():
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,tokens,vocabulary,places,width,pad", [
     (1, 1, 1, 1, 1, 0), (3, 70, 11, 5, 768, 0), (40, 333, 1000, 512, 129, 0), (5, 65, 7, 64, 1031, 3), (300, 100, 50, 2, 64, 8), (2, 5000, 300, 2000, 24, 0),
-    (1, 3, 40, 0, 2056, 0), (7, 2048, 255, 3, 40, 0), (7, 2049, 256, 3, 40, 0), (900, 9000, 70000, 30, 8, 0),
+    (1, 3, 40, 0, 2056, 0), (7, 2048, 255, 3, 40, 0), (7, 2049, 256, 3, 40, 0), (900, 9000, 70000, 30, 8, 0), (5000, 20000, 3000, 9, 260, 0), (40000, 50000, 100, 6, 4, 0),
+    (60, 8192, 3, 200, 3, 1), (60, 8193, 70000, 200, 5, 0), (3, 64, 2, 64, 4, 0), (3, 65, 1, 64, 300, 0), (3, 128, 5, 64, 2, 0),
 ])
 def test_embedding_backward(dtype, rows, tokens, vocabulary, places, width, pad):
     rng = np.random.default_rng(tokens + 1)
@@ -130,6 +131,20 @@ def test_embedding_backward(dtype, rows, tokens, vocabulary, places, width, pad)
             assert got_p is None
         again = encoder.embedding_backward(column(offsets, ids), grad, vocabulary, places, dtype=result)
         assert torch.equal(got_t, again[0]) and (not places or torch.equal(got_p, again[1]))
+
+
+def test_embedding_backward_of_many_tokens():
+    """More tiles than a workgroup adds up the counts of: in whole numbers, so that every sum is exact."""
+    n, vocabulary, width = 256 * 8192 + 77, 300, 4
+    rng = np.random.default_rng(4)
+    ids = rng.integers(-1, vocabulary, n).astype(np.int32)
+    offsets = np.arange(0, n + 1, 7, dtype=np.int32)
+    g = rng.integers(-4, 5, (n, width)).astype(np.float32)
+    dt, dp = encoder.embedding_backward(column(offsets, ids), torch.from_numpy(g).cuda(), vocabulary, 8)
+    rows, inside = len(offsets) - 1, int(offsets[-1])
+    want = np.stack([np.bincount(ids[:inside][ids[:inside] >= 0], g[:inside, k][ids[:inside] >= 0], vocabulary) for k in range(width)], 1)
+    assert (dt.cpu().numpy() == want).all()
+    assert (dp.cpu().numpy() == np.concatenate([g[:inside].reshape(rows, 7, width).sum(0), np.zeros((1, width))])).all()
 
 
 # ------------------------------------------------------------------ dropout
