@@ -58,13 +58,15 @@ embedding_kernel(Tokens tokens, Rows<const T> table, int64_t vocabulary, Rows<co
 // ------------------------------------------------------------------ tokens in the order of their ids
 // A stable sort: tokens of one id stay in their order, so that sums over them are added in one order at every call.  Least
 // significant digit first, eight bits a pass: count the digits of every tile, then place, for which every workgroup adds up the
-// counts that it needs (of more than kDirectTiles tiles, device_exclusive_scan does).  Up to a tile of tokens is sorted by one
-// workgroup, in LDS: one launch.
+// counts that it needs (of more than kDirectTiles tiles, device_exclusive_scan does).  Up to kSmall tokens are sorted by one
+// workgroup, in LDS: one launch.  Digits repeat as the words of a text do, so lanes with the same one are counted at once: with an
+// atomic a lane the four launches over 262,139 tokens took 43 us.
 constexpr int kDigitBits      = 8;
 constexpr int kDigits         = 1 << kDigitBits;
 constexpr int kSortThreads    = 1024;
 constexpr int kSortWaves      = kSortThreads / kWave;
-constexpr int kTile           = 8192;
+constexpr int kSmall          = 8192;  // tokens that one workgroup sorts
+constexpr int kTile           = 2048;
 constexpr int kRounds         = kTile / kSortThreads;
 constexpr int kDirectTiles    = 256;
 
@@ -104,20 +106,37 @@ __device__ __forceinline__ uint64_t same_digit(uint32_t digit, bool here)
   return same;
 }
 
+// Counts the wavefront's keys in `counts`, digit by digit; returns how many with the same digit were counted before the lane's own.
+__device__ __forceinline__ uint32_t count_digit(uint32_t* counts, uint32_t digit, bool here)
+{
+  uint64_t const same   = same_digit(digit, here);
+  uint32_t const below  = lanes_below(same);
+  uint32_t const before = here ? counts[digit] : 0;
+  wave_lds_fence();
+  if (here && below == 0) counts[digit] = before + static_cast<uint32_t>(__builtin_popcountll(same));
+  wave_lds_fence();
+  return before + below;
+}
+
 // counts[tile][digit], or [digit][tile] for the scan
 template <typename From>
 __global__ void __launch_bounds__(kSortThreads) digit_counts_kernel(From from, int32_t n, int shift, int32_t tiles, bool by_digit, uint32_t* counts)
 {
-  __shared__ uint32_t lds[kDigits];
-  if (threadIdx.x < kDigits) lds[threadIdx.x] = 0;
+  __shared__ uint32_t lds[kSortWaves][kDigits];
+  int const wave = threadIdx.x / kWave;
+  for (int w = threadIdx.x / kDigits; w < kSortWaves; w += kSortThreads / kDigits) lds[w][threadIdx.x % kDigits] = 0;
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
     int64_t const i = static_cast<int64_t>(blockIdx.x) * kTile + r * kSortThreads + threadIdx.x;
-    if (i < n) atomicAdd(&lds[(from.key(i) >> shift) & (kDigits - 1)], 1u);
+    bool const here = i < n;
+    count_digit(lds[wave], ((here ? from.key(i) : 0) >> shift) & (kDigits - 1), here);
   }
   __syncthreads();
-  if (threadIdx.x < kDigits) counts[by_digit ? static_cast<int64_t>(threadIdx.x) * tiles + blockIdx.x : static_cast<int64_t>(blockIdx.x) * kDigits + threadIdx.x] = lds[threadIdx.x];
+  if (threadIdx.x >= kDigits) return;
+  uint32_t sum = 0;
+  for (int w = 0; w < kSortWaves; ++w) sum += lds[w][threadIdx.x];
+  counts[by_digit ? static_cast<int64_t>(threadIdx.x) * tiles + blockIdx.x : static_cast<int64_t>(blockIdx.x) * kDigits + threadIdx.x] = sum;
 }
 
 // `summed`: counts[digit][tile] are places already.
@@ -130,13 +149,16 @@ __global__ void __launch_bounds__(kSortThreads) digit_place_kernel(From from, in
   for (int w = threadIdx.x / kDigits; w < kSortWaves; w += kSortThreads / kDigits) lds[w][threadIdx.x % kDigits] = 0;
   __syncthreads();
   // a wavefront's keys are consecutive, 64 a round
-  uint32_t key[kRounds];
+  uint32_t key[kRounds], token[kRounds], rank[kRounds];
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
     int64_t const i = static_cast<int64_t>(blockIdx.x) * kTile + (wave * kRounds + r) * kWave + lane;
     key[r]          = i < n ? from.key(i) : 0;
-    if (i < n) atomicAdd(&lds[wave][(key[r] >> shift) & (kDigits - 1)], 1u);
+    token[r]        = i < n ? from.token(i) : 0;
   }
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r)
+    rank[r] = count_digit(lds[wave], (key[r] >> shift) & (kDigits - 1), static_cast<int64_t>(blockIdx.x) * kTile + (wave * kRounds + r) * kWave + lane < n);
   uint32_t place = 0;
   if (summed) {
     if (threadIdx.x < kDigits) place = counts[static_cast<int64_t>(threadIdx.x) * tiles + blockIdx.x];
@@ -172,43 +194,39 @@ __global__ void __launch_bounds__(kSortThreads) digit_place_kernel(From from, in
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
-    int64_t const i      = static_cast<int64_t>(blockIdx.x) * kTile + (wave * kRounds + r) * kWave + lane;
-    bool const here      = i < n;
-    uint32_t const digit = (key[r] >> shift) & (kDigits - 1);
-    uint64_t const same  = same_digit(digit, here);
-    uint32_t at          = 0;
-    if (here) at = lds[wave][digit] + lanes_below(same);
-    wave_lds_fence();
-    if (here && lanes_below(same) == 0) lds[wave][digit] += static_cast<uint32_t>(__builtin_popcountll(same));
-    wave_lds_fence();
-    if (here) {
-      out.keys[at]   = key[r];
-      out.tokens[at] = from.token(i);
+    int64_t const i = static_cast<int64_t>(blockIdx.x) * kTile + (wave * kRounds + r) * kWave + lane;
+    if (i < n) {
+      uint32_t const at = lds[wave][(key[r] >> shift) & (kDigits - 1)] + rank[r];
+      out.keys[at]      = key[r];
+      out.tokens[at]    = token[r];
     }
   }
 }
 
-// All passes over up to a tile of tokens.
+// All passes over up to kSmall tokens.
 __global__ void __launch_bounds__(kSortThreads) small_sort_kernel(Unsorted from, int32_t n, Sorted out)
 {
   __shared__ uint32_t lds[kSortWaves][kDigits];
-  __shared__ uint32_t keys[kTile];
-  __shared__ uint16_t tokens[kTile];
+  __shared__ uint32_t keys[kSmall];
+  __shared__ uint16_t tokens[kSmall];
   __shared__ uint32_t scan[kSortWaves + 1];
   int const wave = threadIdx.x / kWave, lane = lane_id();
-  uint32_t key[kRounds], token[kRounds];
+  // a wavefront's keys are consecutive, and shared evenly
+  int const rounds = (n + kSortThreads - 1) / kSortThreads;
+  constexpr int kMost = kSmall / kSortThreads;
+  uint32_t key[kMost], token[kMost], rank[kMost];
 #pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
-    int const i = (wave * kRounds + r) * kWave + lane;
-    key[r]      = i < n ? from.key(i) : 0;
+  for (int r = 0; r < kMost; ++r) {
+    int const i = (wave * rounds + r) * kWave + lane;
+    key[r]      = r < rounds && i < n ? from.key(i) : 0;
     token[r]    = i;
   }
   for (int shift = 0; shift < 32 && (from.vocabulary >> shift) != 0; shift += kDigitBits) {
     for (int w = threadIdx.x / kDigits; w < kSortWaves; w += kSortThreads / kDigits) lds[w][threadIdx.x % kDigits] = 0;
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r)
-      if ((wave * kRounds + r) * kWave + lane < n) atomicAdd(&lds[wave][(key[r] >> shift) & (kDigits - 1)], 1u);
+    for (int r = 0; r < kMost; ++r)
+      if (r < rounds) rank[r] = count_digit(lds[wave], (key[r] >> shift) & (kDigits - 1), (wave * rounds + r) * kWave + lane < n);
     __syncthreads();
     uint32_t every = 0, total;
     if (threadIdx.x < kDigits)
@@ -222,34 +240,27 @@ __global__ void __launch_bounds__(kSortThreads) small_sort_kernel(Unsorted from,
       }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-      bool const here      = (wave * kRounds + r) * kWave + lane < n;
-      uint32_t const digit = (key[r] >> shift) & (kDigits - 1);
-      uint64_t const same  = same_digit(digit, here);
-      uint32_t at          = 0;
-      if (here) at = lds[wave][digit] + lanes_below(same);
-      wave_lds_fence();
-      if (here && lanes_below(same) == 0) lds[wave][digit] += static_cast<uint32_t>(__builtin_popcountll(same));
-      wave_lds_fence();
-      if (here) {
-        keys[at]   = key[r];
-        tokens[at] = static_cast<uint16_t>(token[r]);
+    for (int r = 0; r < kMost; ++r) {
+      if (r < rounds && (wave * rounds + r) * kWave + lane < n) {
+        uint32_t const at = lds[wave][(key[r] >> shift) & (kDigits - 1)] + rank[r];
+        keys[at]          = key[r];
+        tokens[at]        = static_cast<uint16_t>(token[r]);
       }
     }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-      int const i = (wave * kRounds + r) * kWave + lane;
-      if (i < n) {
+    for (int r = 0; r < kMost; ++r) {
+      int const i = (wave * rounds + r) * kWave + lane;
+      if (r < rounds && i < n) {
         key[r]   = keys[i];
         token[r] = tokens[i];
       }
     }
   }
 #pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
-    int const i = (wave * kRounds + r) * kWave + lane;
-    if (i < n) {
+  for (int r = 0; r < kMost; ++r) {
+    int const i = (wave * rounds + r) * kWave + lane;
+    if (r < rounds && i < n) {
       out.keys[i]   = key[r];
       out.tokens[i] = token[r];
     }
@@ -595,7 +606,7 @@ nvtext_amd_status nvtext_amd_embedding_backward(const nvtext_amd_list_column* to
   uint32_t const vocabulary = static_cast<uint32_t>(token_grad->rows);
   int32_t const n           = view.count;
   int64_t const cols        = grad->cols;
-  bool const small          = n <= kTile;
+  bool const small          = n <= kSmall;
   int32_t const tiles       = (n + kTile - 1) / kTile;
   bool const direct         = tiles <= kDirectTiles;
   int32_t const chunks      = vocabulary > 0 ? static_cast<int32_t>((static_cast<int64_t>(n) + kChunk - 1) / kChunk) : 0;
