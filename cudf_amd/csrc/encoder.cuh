@@ -90,6 +90,28 @@ __device__ __forceinline__ void store8(T* p, float const (&f)[8], int64_t n)
   }
 }
 
+// The same in two steps, so that several loads are on their way before the first is waited for.
+template <typename T>
+__device__ __forceinline__ typename Eight<T>::type load_raw8(const T* p, int64_t n)
+{
+  typename Eight<T>::type v{};
+  if (n >= 8) {
+    v = *reinterpret_cast<const typename Eight<T>::type*>(p);
+  } else if (n > 0) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < n) v[k] = p[k];
+  }
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void widen(float (&f)[8], typename Eight<T>::type const& v)
+{
+#pragma unroll
+  for (int k = 0; k < 8; ++k) f[k] = static_cast<float>(v[k]);
+}
+
 // ------------------------------------------------------------------ dropout
 // Philox4x32-10 (J. Salmon, M. Moraes, R. Dror, D. Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011): ten rounds
 // of two 32 x 32 -> 64 bit products each, one instruction apiece here.  A counter gives four words, eight draws of 16 bits.
@@ -172,15 +194,16 @@ __device__ __forceinline__ float block_sum(float v, float* lds)
 }
 
 // Sums over the rows of a matrix: parts [count, cols] of them are added up into a row of type T, by a workgroup for 64 columns,
-// whose wavefronts take a run of parts each.
+// whose wavefronts take a run of parts each.  Of two such arrays one after the other the second becomes `second`.
 template <typename T>
-__global__ void __launch_bounds__(512) add_parts_kernel(const float* parts, int64_t count, int64_t cols, T* out)
+__global__ void __launch_bounds__(512) add_parts_kernel(const float* parts, int64_t count, int64_t cols, T* out, T* second)
 {
   constexpr int kWaves = 512 / kWave;
   __shared__ float lds[kWaves][kWave];
   int const wave = threadIdx.x / kWave, lane = lane_id();
   int64_t const j = static_cast<int64_t>(blockIdx.x) * kWave + lane;
   int64_t const each = (count + kWaves - 1) / kWaves, first = wave * each, last = first + each < count ? first + each : count;
+  parts += blockIdx.y * count * cols;
   float sum = 0.f;
   if (j < cols) {
 #pragma unroll 8
@@ -191,13 +214,13 @@ __global__ void __launch_bounds__(512) add_parts_kernel(const float* parts, int6
   if (wave != 0 || j >= cols) return;
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) sum += lds[w][lane];
-  out[j] = static_cast<T>(sum);
+  (blockIdx.y == 0 ? out : second)[j] = static_cast<T>(sum);
 }
 
 template <typename T>
-inline void launch_add_parts(const float* parts, int64_t count, int64_t cols, T* out, hipStream_t stream)
+inline void launch_add_parts(const float* parts, int64_t count, int64_t cols, T* out, T* second, hipStream_t stream)
 {
-  hipLaunchKernelGGL(add_parts_kernel<T>, dim3(static_cast<unsigned>((cols + kWave - 1) / kWave)), dim3(512), 0, stream, parts, count, cols, out);
+  hipLaunchKernelGGL(add_parts_kernel<T>, dim3(static_cast<unsigned>((cols + kWave - 1) / kWave), second ? 2 : 1), dim3(512), 0, stream, parts, count, cols, out, second);
 }
 
 }  // namespace nvtext_amd

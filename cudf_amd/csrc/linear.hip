@@ -671,7 +671,7 @@ nvtext_amd_status nvtext_amd_linear_backward(const nvtext_amd_matrix* grad, cons
       ProfileScope const scope("linear_activation_backward", stream);
       hipLaunchKernelGGL(activation_backward_kernel<T>, dim3(static_cast<unsigned>((n + 8 * kWave - 1) / (8 * kWave)), static_cast<unsigned>(parts)), dim3(kThreads), 0, stream, gs,
                          slopes ? rows_of<const T>(preactivation) : Rows<const T>{nullptr, 0}, activation, m, n, d, sums);
-      if (bias_grad) launch_add_parts(sums, parts, n, static_cast<T*>(bias_grad->data), stream);
+      if (bias_grad) launch_add_parts<T>(sums, parts, n, static_cast<T*>(bias_grad->data), nullptr, stream);
     }
     Rows<const T> const ds = slopes ? Rows<const T>{d.data, d.stride} : gs;
     auto const plain = [](const nvtext_amd_matrix* o) { return Epilogue<T>{{nullptr, 0}, {nullptr, 0}, rows_of<T>(o), {nullptr, 0}, NVTEXT_AMD_ACTIVATION_NONE}; };

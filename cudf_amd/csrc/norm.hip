@@ -2,6 +2,7 @@
 #include "encoder.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace nvtext_amd {
 namespace {
@@ -61,9 +62,94 @@ __device__ __forceinline__ void load_sum(float (&f)[8], Rows<const T> x, Rows<co
   }
 }
 
-// A workgroup a row, which it goes through three times.
+// The sum over the lanes of a row's WAVES wavefronts.  lds: a value a wavefront, which two calls in turn do not share: that one
+// barrier a call is enough.
+template <int WAVES>
+__device__ __forceinline__ float row_sum(float v, float* lds)
+{
+  v = wave_sum(v);
+  if constexpr (WAVES > 1) {
+    int const wave = threadIdx.x / kWave % WAVES;
+    if (lane_id() == 0) lds[wave] = v;
+    lds_barrier();
+    v = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) v += lds[w];
+  }
+  return v;
+}
+
+// Rows that fit into registers: WAVES wavefronts a row, BLOCKS times eight values a lane, each read once; the mean first, then the
+// squares around it.  A workgroup takes several rows one after the other and keeps the weights.
+template <typename T, int WAVES, int BLOCKS>
+__global__ void __launch_bounds__(WAVES > 4 ? WAVES * kWave : kThreads)
+layer_norm_kernel(Rows<const T> x, Rows<const T> residual, Weights weight, Weights bias, float eps, Dropout d, Rows<T> out, Rows<T> sum, float* mean_out,
+                  float* rstd_out, int64_t rows, int64_t cols)
+{
+  constexpr int kThreadsHere = WAVES > 4 ? WAVES * kWave : kThreads, kRows = kThreadsHere / (WAVES * kWave);
+  __shared__ float lds[2][kRows][WAVES];
+  int const place = threadIdx.x / (WAVES * kWave), lane = threadIdx.x % (WAVES * kWave);  // the row of the workgroup, the lane of the row
+  float const width = static_cast<float>(cols);
+  float w[BLOCKS][8], c[BLOCKS][8];
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b) {
+    int64_t const j = (static_cast<int64_t>(b) * WAVES * kWave + lane) * 8;
+    weight.load<T>(w[b], j, cols - j);
+    bias.load<T>(c[b], j, cols - j);
+  }
+  // (all wavefronts of a workgroup go round equally often, for the barriers)
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * kRows; first < rows; first += static_cast<int64_t>(gridDim.x) * kRows) {
+    int64_t const i = first + place < rows ? first + place : rows - 1;  // (behind the last: the last once more)
+    typename Eight<T>::type vx[BLOCKS], vr[BLOCKS];
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+      int64_t const j = (static_cast<int64_t>(b) * WAVES * kWave + lane) * 8;
+      vx[b]           = load_raw8<T>(x.row(i) + j, cols - j);
+      if (residual) vr[b] = load_raw8<T>(residual.row(i) + j, cols - j);
+    }
+    float f[BLOCKS][8], s = 0.f;
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+      widen<T>(f[b], vx[b]);
+      if (d.dropped) d.apply(f[b], i, static_cast<int64_t>(b) * WAVES * kWave + lane);
+      if (residual) {
+        float r[8];
+        widen<T>(r, vr[b]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[b][k] += r[k];
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += f[b][k];
+    }
+    float const mean = row_sum<WAVES>(s, lds[0][place]) / width;  // (not times 1 / width: the mean of equal values is that value)
+    s                = 0.f;
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+      int64_t const left = cols - (static_cast<int64_t>(b) * WAVES * kWave + lane) * 8;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += k < left ? (f[b][k] - mean) * (f[b][k] - mean) : 0.f;
+    }
+    float const rstd = 1.f / sqrtf(row_sum<WAVES>(s, lds[1][place]) / width + eps);
+    if (first + place < rows) {
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) {
+        int64_t const j = (static_cast<int64_t>(b) * WAVES * kWave + lane) * 8;
+        if (sum) store8(sum.row(i) + j, f[b], cols - j);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[b][k] = (f[b][k] - mean) * rstd * w[b][k] + c[b][k];
+        store8(out.row(i) + j, f[b], cols - j);
+      }
+      if (lane == 0) {
+        if (mean_out) mean_out[i] = mean;
+        if (rstd_out) rstd_out[i] = rstd;
+      }
+    }
+  }
+}
+
+// Wider ones: a workgroup a row, which it goes through three times.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) layer_norm_kernel(Rows<const T> x, Rows<const T> residual, Weights weight, Weights bias, float eps, Dropout d,
+__global__ void __launch_bounds__(kThreads) wide_layer_norm_kernel(Rows<const T> x, Rows<const T> residual, Weights weight, Weights bias, float eps, Dropout d,
                                                               Rows<T> out, Rows<T> sum, float* mean_out, float* rstd_out, int64_t rows, int64_t cols)
 {
   __shared__ float lds[kThreads / kWave];
@@ -102,6 +188,111 @@ __global__ void __launch_bounds__(kThreads) layer_norm_kernel(Rows<const T> x, R
   }
 }
 
+// The gradient of rows that fit into registers, read once.  The workgroup's sums over its rows of grad * h and of grad go to parts
+// [workgroup] and [number of workgroups + workgroup]: a lane adds them up for its columns, and the workgroup's rows are added up in
+// order in the end.
+template <typename T, int WAVES, int BLOCKS>
+__global__ void __launch_bounds__(WAVES > 4 ? WAVES * kWave : kThreads)
+layer_norm_backward_kernel(Rows<const T> grad, Rows<const T> sum, const float* mean_in, const float* rstd_in, Weights weight, Rows<const T> sum_grad, Dropout d, Rows<T> x_grad,
+                           Rows<T> residual_grad, float* parts, int64_t rows, int64_t cols)
+{
+  constexpr int kThreadsHere = WAVES > 4 ? WAVES * kWave : kThreads, kRows = kThreadsHere / (WAVES * kWave), kCols = WAVES * BLOCKS * kWave * 8;
+  __shared__ float lds[2][kRows][WAVES];
+  __shared__ float joined[kRows > 1 ? 2 : 1][kRows > 1 ? kCols : 1];
+  int const place = threadIdx.x / (WAVES * kWave), lane = threadIdx.x % (WAVES * kWave);
+  float const width = static_cast<float>(cols);
+  float w[BLOCKS][8], dw[BLOCKS][8], db[BLOCKS][8];
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b) {
+    int64_t const j = (static_cast<int64_t>(b) * WAVES * kWave + lane) * 8;
+    weight.load<T>(w[b], j, cols - j);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) dw[b][k] = db[b][k] = 0.f;
+  }
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * kRows; first < rows; first += static_cast<int64_t>(gridDim.x) * kRows) {
+    bool const here  = first + place < rows;
+    int64_t const i  = here ? first + place : rows - 1;
+    float const mean = mean_in[i], rstd = rstd_in[i];
+    typename Eight<T>::type vg[BLOCKS], vs[BLOCKS], ve[BLOCKS];
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+      int64_t const j = (static_cast<int64_t>(b) * WAVES * kWave + lane) * 8;
+      vg[b]           = load_raw8<T>(grad.row(i) + j, cols - j);
+      vs[b]           = load_raw8<T>(sum.row(i) + j, cols - j);
+      if (sum_grad) ve[b] = load_raw8<T>(sum_grad.row(i) + j, cols - j);
+    }
+    float sa = 0.f, sh = 0.f;
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+      float g[8], s[8];
+      widen<T>(g, vg[b]);
+      widen<T>(s, vs[b]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {  // (behind the last column grad is 0)
+        float const h = (s[k] - mean) * rstd, gh = g[k] * h;
+        sa += g[k] * w[b][k];
+        sh += gh * w[b][k];
+        if (here) {
+          dw[b][k] += gh;
+          db[b][k] += g[k];
+        }
+      }
+    }
+    float const ma = row_sum<WAVES>(sa, lds[0][place]) / width, mh = row_sum<WAVES>(sh, lds[1][place]) / width;
+    if (here) {
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) {
+        int64_t const j = (static_cast<int64_t>(b) * WAVES * kWave + lane) * 8;
+        float g[8], s[8], e[8];
+        widen<T>(g, vg[b]);
+        widen<T>(s, vs[b]);
+        if (sum_grad) widen<T>(e, ve[b]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          s[k] = rstd * (g[k] * w[b][k] - ma - (s[k] - mean) * rstd * mh);
+          if (sum_grad) s[k] += e[k];
+        }
+        store8(residual_grad.row(i) + j, s, cols - j);
+        if (x_grad) {
+          if (d.dropped) d.apply(s, i, static_cast<int64_t>(b) * WAVES * kWave + lane);
+          store8(x_grad.row(i) + j, s, cols - j);
+        }
+      }
+    }
+  }
+  if (!parts) return;
+  float* const out[2] = {parts + blockIdx.x * cols, parts + (static_cast<int64_t>(gridDim.x) + blockIdx.x) * cols};
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    if constexpr (kRows > 1) __syncthreads();
+    if (place != r) continue;
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+      int const j = (b * WAVES * kWave + lane) * 8;
+      if constexpr (kRows > 1) {
+        if (r > 0) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            dw[b][k] += joined[0][j + k];
+            db[b][k] += joined[1][j + k];
+          }
+        }
+        if (r + 1 < kRows) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            joined[0][j + k] = dw[b][k];
+            joined[1][j + k] = db[b][k];
+          }
+          continue;
+        }
+      }
+      store8(out[0] + j, dw[b], cols - j);
+      store8(out[1] + j, db[b], cols - j);
+    }
+  }
+}
+
+// The gradient of wider rows, in two kernels.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 layer_norm_rows_backward_kernel(Rows<const T> grad, Rows<const T> sum, const float* mean_in, const float* rstd_in, Weights weight, Rows<const T> sum_grad,
@@ -169,6 +360,22 @@ layer_norm_weights_backward_kernel(Rows<const T> grad, Rows<const T> sum, const 
   store8(parts + (gridDim.y + static_cast<int64_t>(blockIdx.y)) * cols + b * 8, db, cols - b * 8);
 }
 
+// Calls f with the wavefronts a row and the blocks of eight values a lane that hold a row of `cols` values, or with none: up to 2048
+// values one wavefront, which needs no barrier.
+template <typename F>
+void with_shape(int64_t cols, F&& f)
+{
+  using std::integral_constant;
+  if (cols <= 512) f(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+  else if (cols <= 1024) f(integral_constant<int, 1>{}, integral_constant<int, 2>{});
+  else if (cols <= 1536) f(integral_constant<int, 1>{}, integral_constant<int, 3>{});
+  else if (cols <= 2048) f(integral_constant<int, 1>{}, integral_constant<int, 4>{});
+  else if (cols <= 4096) f(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+  else if (cols <= 8192) f(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+  else if (cols <= 16384) f(integral_constant<int, 16>{}, integral_constant<int, 2>{});
+  else f(integral_constant<int, 0>{}, integral_constant<int, 0>{});
+}
+
 bool is_weights(const nvtext_amd_matrix* w, const nvtext_amd_matrix* x) { return is_shape(w, 1, x->cols) && (w->type == x->type || w->type == NVTEXT_AMD_TYPE_FLOAT32); }
 bool is_like(const nvtext_amd_matrix* m, const nvtext_amd_matrix* x) { return is_shape(m, x->rows, x->cols) && m->type == x->type; }
 
@@ -222,9 +429,19 @@ nvtext_amd_status nvtext_amd_layer_norm(const nvtext_amd_matrix* x, const nvtext
   with_type(x->type, [&](auto zero) {
     using T = decltype(zero);
     ProfileScope const scope("layer_norm", stream);
-    hipLaunchKernelGGL(layer_norm_kernel<T>, dim3(grid_for(x->rows, 8)), dim3(kThreads), 0, stream, rows_of<const T>(x), rows_of<const T>(residual),
-                       Weights{weight->data, weight->type}, Weights{bias->data, bias->type}, static_cast<float>(eps), d, rows_of<T>(out), rows_of<T>(sum), mean, rstd,
-                       x->rows, x->cols);
+    with_shape(x->cols, [&](auto waves, auto blocks) {
+      constexpr int W = decltype(waves)::value, B = decltype(blocks)::value;
+      auto const launch = [&](auto kernel, int threads, int64_t groups) {
+        hipLaunchKernelGGL(kernel, dim3(grid_for(groups, 2048 / threads)), dim3(threads), 0, stream, rows_of<const T>(x), rows_of<const T>(residual), Weights{weight->data, weight->type},
+                           Weights{bias->data, bias->type}, static_cast<float>(eps), d, rows_of<T>(out), rows_of<T>(sum), mean, rstd, x->rows, x->cols);
+      };
+      if constexpr (W == 0)
+        launch(wide_layer_norm_kernel<T>, kThreads, x->rows);
+      else if constexpr (W > 4)
+        launch(layer_norm_kernel<T, W, B>, W * kWave, x->rows);
+      else
+        launch(layer_norm_kernel<T, W, B>, kThreads, (x->rows * W + 3) / 4);
+    });
   });
   NVTEXT_HIP_TRY(hipGetLastError());
   return NVTEXT_AMD_SUCCESS;
@@ -254,29 +471,43 @@ nvtext_amd_status nvtext_amd_layer_norm_backward(const nvtext_amd_matrix* grad, 
   Mr const mr{mr_, stream};
   Dropout const d    = make_dropout(p, seed, offset);
   int64_t const rows = grad->rows, cols = grad->cols;
-  // rows = 0: the sums of the weights' gradients are zeros, of one part
-  int64_t const parts = std::max<int64_t>(1, std::min<int64_t>(rows, 256));
+  int64_t parts      = 0;
+  with_shape(cols, [&](auto waves, auto) {
+    constexpr int W = decltype(waves)::value;
+    // rows = 0: the sums of the weights' gradients are zeros, of one part
+    parts = W == 0 ? std::max<int64_t>(1, std::min<int64_t>(rows, 256)) : grid_for(W > 4 ? rows : (rows * W + 3) / 4, W > 4 ? 1 : 4);
+  });
   Temp const sums(mr, weight_grad ? static_cast<size_t>(2 * parts * cols) * sizeof(float) : 0);
   if (!sums.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
+  Weights const w{weight->data, weight->type};
   with_type(grad->type, [&](auto zero) {
     using T = decltype(zero);
-    if (weight_grad) {
-      ProfileScope const scope("layer_norm_weights_backward", stream);
-      hipLaunchKernelGGL(layer_norm_weights_backward_kernel<T>, dim3(static_cast<unsigned>((cols + 8 * kThreads - 1) / (8 * kThreads)), static_cast<unsigned>(parts)), dim3(kThreads),
-                         0, stream, rows_of<const T>(grad), rows_of<const T>(sum), mean, rstd, rows, cols, sums.as<float>());
-    }
-    if (rows > 0) {
-      ProfileScope const scope("layer_norm_rows_backward", stream);
-      hipLaunchKernelGGL(layer_norm_rows_backward_kernel<T>, dim3(grid_for(rows, 8)), dim3(kThreads), 0, stream, rows_of<const T>(grad), rows_of<const T>(sum), mean, rstd,
-                         Weights{weight->data, weight->type}, rows_of<const T>(sum_grad), d, rows_of<T>(x_grad), rows_of<T>(residual_grad), rows, cols);
-    }
+    with_shape(cols, [&](auto waves, auto blocks) {
+      constexpr int W = decltype(waves)::value, B = decltype(blocks)::value;
+      if constexpr (W > 0) {
+        ProfileScope const scope("layer_norm_backward", stream);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(layer_norm_backward_kernel<T, W, B>), dim3(static_cast<unsigned>(parts)), dim3(W > 4 ? W * kWave : kThreads), 0, stream, rows_of<const T>(grad),
+                           rows_of<const T>(sum), mean, rstd, w, rows_of<const T>(sum_grad), d, rows_of<T>(x_grad), rows_of<T>(residual_grad), weight_grad ? sums.as<float>() : nullptr,
+                           rows, cols);
+      } else {
+        if (weight_grad) {
+          ProfileScope const scope("layer_norm_weights_backward", stream);
+          hipLaunchKernelGGL(layer_norm_weights_backward_kernel<T>, dim3(static_cast<unsigned>((cols + 8 * kThreads - 1) / (8 * kThreads)), static_cast<unsigned>(parts)),
+                             dim3(kThreads), 0, stream, rows_of<const T>(grad), rows_of<const T>(sum), mean, rstd, rows, cols, sums.as<float>());
+        }
+        if (rows > 0) {
+          ProfileScope const scope("layer_norm_rows_backward", stream);
+          hipLaunchKernelGGL(layer_norm_rows_backward_kernel<T>, dim3(grid_for(rows, 8)), dim3(kThreads), 0, stream, rows_of<const T>(grad), rows_of<const T>(sum), mean, rstd, w,
+                             rows_of<const T>(sum_grad), d, rows_of<T>(x_grad), rows_of<T>(residual_grad), rows, cols);
+        }
+      }
+    });
   });
   if (weight_grad)
     with_type(weight->type, [&](auto zero) {
       using W = decltype(zero);
       ProfileScope const scope("layer_norm_add_parts", stream);
-      launch_add_parts(sums.as<float>(), parts, cols, static_cast<W*>(weight_grad->data), stream);
-      launch_add_parts(sums.as<float>() + parts * cols, parts, cols, static_cast<W*>(bias_grad->data), stream);
+      launch_add_parts(sums.as<float>(), parts, cols, static_cast<W*>(weight_grad->data), static_cast<W*>(bias_grad->data), stream);
     });
   NVTEXT_HIP_TRY(hipGetLastError());
   return NVTEXT_AMD_SUCCESS;
