@@ -381,6 +381,55 @@ tile_product_kernel(Side a, Side b, int64_t m, int64_t n, int64_t depth, int64_t
   tile_product<T, A_NEXT, B_NEXT, BM, BN, WAVES_M, WAVES_N>(a, b, m, n, depth, part, sums, end);
 }
 
+// ------------------------------------------------------------------ products of few rows
+// A call for one token, or a few: nothing but the reading of the weights, which no workgroup shares.  A workgroup takes 16 outputs
+// and all values of k, its wavefronts a run of k each; the weights go from memory into the fragments of the matrix
+// instructions, kDeep loads of 16 bytes a lane on their way at a time, as do up to 16 * MI rows of x, which the caches hold; the
+// wavefronts' sums are added up in order in LDS.  One launch and no temporaries.  Rows may lie anyhow.
+template <typename T, int MI, int WAVES>
+__global__ void __launch_bounds__(WAVES * kWave) few_rows_kernel(Rows<const T> x, Rows<const T> weight, int64_t m, int64_t n, int64_t depth, Epilogue<T> end)
+{
+  constexpr int kDeep = MI == 4 ? 4 : WAVES == 16 ? 6 : 8;  // (as many as the registers hold)
+  __shared__ __attribute__((aligned(16))) float lds[WAVES][MI][16][20];  // (16 outputs a row, and room against conflicts)
+  int const wave = threadIdx.x / kWave, lane = lane_id();
+  int64_t const j0 = static_cast<int64_t>(blockIdx.x) * 16;
+  const T* const w = weight.row(j0 + lane % 16 < n ? j0 + lane % 16 : n - 1);  // (outputs and rows behind the last: the last once more, not written)
+  const T* rows[MI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) rows[i] = x.row(i * 16 + lane % 16 < m ? i * 16 + lane % 16 : m - 1);
+  f32x4_t sum[MI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) sum[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  int64_t const steps = (depth + 31) / 32, each = (steps + WAVES - 1) / WAVES;
+  int64_t const first = wave * each, last = first + each < steps ? first + each : steps;
+  for (int64_t t = first; t < last; t += kDeep) {
+    typename Eight<T>::type vw[kDeep], vx[kDeep][MI];
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+      int64_t const k = (t + u) * 32 + lane / 16 * 8, left = t + u < last ? depth - k : 0;
+      vw[u]           = load_raw8<T>(w + k, left);
+#pragma unroll
+      for (int i = 0; i < MI; ++i) vx[u][i] = load_raw8<T>(rows[i] + k, left);
+    }
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u)
+#pragma unroll
+      for (int i = 0; i < MI; ++i) sum[i] = multiply(__builtin_bit_cast(Fragment<T>, vw[u]), __builtin_bit_cast(Fragment<T>, vx[u][i]), sum[i]);
+  }
+  // a lane has outputs lane / 16 * 4 .. + 3 of row lane % 16
+#pragma unroll
+  for (int i = 0; i < MI; ++i) *reinterpret_cast<f32x4_t*>(&lds[wave][i][lane % 16][lane / 16 * 4]) = sum[i];
+  __syncthreads();
+  int const i = threadIdx.x / 2, j = threadIdx.x % 2 * 8;
+  if (i >= MI * 16 || i >= m || j0 + j >= n) return;
+  float z[8] = {};
+#pragma unroll
+  for (int v = 0; v < WAVES; ++v)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) z[k] += lds[v][i / 16][i % 16][j + k];
+  end.finish(z, typename Epilogue<T>::Columns(end, j0 + j, n), i, j0 + j, n);
+}
+
 // The parts of a product that was cut along k, added up in order.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) join_parts_kernel(const float* sums, int64_t parts, int64_t m, int64_t n, Epilogue<T> end)
@@ -547,6 +596,19 @@ inline Plan plan_product(int64_t m, int64_t n, int64_t depth)
   return best;
 }
 
+// Whether few_rows_kernel takes less time than tiles: microseconds of either, fitted to calls of 1 to 64 rows with 1024 to 8192
+// inputs and outputs.  It goes through k in one workgroup for 16 outputs, which takes longer with every 16 rows; tiles cost a launch
+// more, and then read the weights as fast as memory gives them.  (16 rows: 1024 to 4096 4.9 us against 11.5, 4096 to 1024 10.5
+// against 19.5, 8192 to 8192 44 against 34; 64 rows: 8.3 against 12.3, 21 against 18, 84 against 38.)
+inline bool few_rows_are_faster(int64_t m, int64_t n, int64_t depth)
+{
+  if (m > 64) return false;
+  double const by_16 = m <= 16 ? 1 : m <= 32 ? 2 : 4, thousands = depth / 1024.0;
+  double const few   = 3 + 0.95 * thousands * (1 + by_16) * static_cast<double>((n + 16 * 256 - 1) / (16 * 256));
+  double const tiles = std::max(11 + thousands, static_cast<double>(n) * depth * 2 / 4.2e6);
+  return few < tiles;
+}
+
 // out (m x n) = a (m x depth) * b (n x depth)^T
 template <typename T>
 nvtext_amd_status launch_product(Factor<T> a, Factor<T> b, int64_t m, int64_t n, int64_t depth, Epilogue<T> const& end, Mr const& mr, hipStream_t stream)
@@ -557,6 +619,27 @@ nvtext_amd_status launch_product(Factor<T> a, Factor<T> b, int64_t m, int64_t n,
                        end);
     return NVTEXT_AMD_SUCCESS;
   } else {
+    if (a.k_next && b.k_next && few_rows_are_faster(m, n, depth)) {
+      // enough wavefronts that each has about one round of loads
+      auto const launch = [&](auto rows_of_16, auto waves) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, decltype(rows_of_16)::value, decltype(waves)::value>), dim3(static_cast<unsigned>((n + 15) / 16)),
+                           dim3(decltype(waves)::value * kWave), 0, stream, a.rows, b.rows, m, n, depth, end);
+      };
+      auto const by_depth = [&](auto rows_of_16, auto most) {
+        if (depth >= 2048)
+          launch(rows_of_16, most);
+        else
+          launch(rows_of_16, std::integral_constant<int, 4>{});
+      };
+      using std::integral_constant;
+      if (m <= 16)
+        by_depth(integral_constant<int, 1>{}, integral_constant<int, 16>{});
+      else if (m <= 32)
+        by_depth(integral_constant<int, 2>{}, integral_constant<int, 8>{});
+      else
+        by_depth(integral_constant<int, 4>{}, integral_constant<int, 8>{});
+      return NVTEXT_AMD_SUCCESS;
+    }
     bool const copy_a = depth > 0 && !is_aligned(a, m, depth), copy_b = depth > 0 && !is_aligned(b, n, depth);
     auto const lines  = [&](Factor<T> const& f, int64_t extent) { return f.k_next ? extent : depth; };
     auto const width  = [&](Factor<T> const& f, int64_t extent) { return ((f.k_next ? depth : extent) + 7) / 8 * 8; };

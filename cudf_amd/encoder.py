@@ -20,6 +20,7 @@ ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 _TYPES = {torch.float32: _capi.TYPE_FLOAT32, torch.float16: _capi.TYPE_FLOAT16, torch.bfloat16: _capi.TYPE_BFLOAT16}
 _INT32 = np.dtype(np.int32)
+_Matrix = _capi.Matrix
 
 
 class LayerNormSaved(NamedTuple):
@@ -46,16 +47,24 @@ def _matrix(t: torch.Tensor, name: str) -> _capi.Matrix:
         rows, stride = shape[0], strides[0]
     elif n == 1:
         rows, stride = 1, cols
+    elif t.is_contiguous():
+        rows, stride = t.numel() // cols if cols else shape[:-1].numel(), cols
     else:
-        t = t.view(-1, cols)  # raises where the rows are not evenly spaced
-        rows, stride = t.shape[0], t.stride(0)
+        u = t.view(-1, cols)  # raises where the rows are not evenly spaced
+        rows, stride = u.shape[0], u.stride(0)
     if rows < 2 and stride < cols:
         stride = cols
-    return _capi.Matrix(t.data_ptr(), rows, cols, stride, kind)
+    return _Matrix(t.data_ptr(), rows, cols, stride, kind)
 
 
-def _optional(t: Optional[torch.Tensor], name: str):
-    return None if t is None else _matrix(t, name)
+def _new(t: torch.Tensor, rows: int, cols: int) -> _capi.Matrix:
+    """The view of a contiguous tensor that was made here."""
+    return _Matrix(t.data_ptr(), rows, cols, cols, _TYPES[t.dtype])
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    # (empty_like costs a third of empty, but would take over the strides of a view)
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
 def _vector(t: torch.Tensor, name: str) -> _capi.Matrix:
@@ -85,9 +94,9 @@ def embedding(tokens: DeviceListColumn, token_table: torch.Tensor, position_tabl
     `position_table` for its place in its row.  An id that is no row of the table (-1) and a place beyond the last row of
     the other add nothing."""
     column, table = _ids(tokens), _matrix(token_table, "token_table")
-    positions = _optional(position_table, "position_table")
-    out = torch.empty((tokens.child_size, token_table.shape[-1]), dtype=token_table.dtype, device=token_table.device)
-    st = _capi.load().nvtext_amd_embedding(column, table, positions, _stream_handle(), _matrix(out, "out"))
+    positions = None if position_table is None else _matrix(position_table, "position_table")
+    out = token_table.new_empty((tokens.child_size, table.cols))
+    st = _capi.load().nvtext_amd_embedding(column, table, positions, _stream_handle(), _new(out, tokens.child_size, table.cols))
     if st != _capi.SUCCESS:
         _raise(st)
     return out
@@ -100,12 +109,11 @@ def embedding_backward(tokens: DeviceListColumn, grad: torch.Tensor, vocabulary_
     if vocabulary_size < 0 or positions < 0:
         raise ValueError("the tables' sizes must not be negative")
     column, g = _ids(tokens), _matrix(grad, "grad")
-    dtype = dtype or grad.dtype
-    width = grad.shape[-1]
-    token_grad = torch.empty((vocabulary_size, width), dtype=dtype, device=grad.device)
-    position_grad = torch.empty((positions, width), dtype=dtype, device=grad.device) if positions else None
-    st = _capi.load().nvtext_amd_embedding_backward(column, g, _stream_handle(), _mr().struct, _matrix(token_grad, "token_grad"),
-                                                    _optional(position_grad, "position_grad"))
+    width = g.cols
+    token_grad = grad.new_empty((vocabulary_size, width), dtype=dtype)
+    position_grad = grad.new_empty((positions, width), dtype=dtype) if positions else None
+    st = _capi.load().nvtext_amd_embedding_backward(column, g, _stream_handle(), _mr().struct, _matrix(token_grad, "the gradient"),
+                                                    None if position_grad is None else _new(position_grad, positions, width))
     if st != _capi.SUCCESS:
         _raise(st)
     return token_grad, position_grad
@@ -116,8 +124,9 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: int = 0) -> torch.Tens
     1 / (1 - p).  What is dropped follows from `seed`, `offset` (a call's own number under that seed) and the place of the
     value alone, so no mask is kept: dropout(grad, p, seed, offset) is the gradient."""
     seed, offset = _seed(seed, offset)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    st = _capi.load().nvtext_amd_dropout(_matrix(x, "x"), p, seed, offset, _stream_handle(), _matrix(out, "out"))
+    m = _matrix(x, "x")
+    out = _like(x)
+    st = _capi.load().nvtext_amd_dropout(m, p, seed, offset, _stream_handle(), _new(out, m.rows, m.cols))
     if st != _capi.SUCCESS:
         _raise(st)
     return out
@@ -130,15 +139,18 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, eps: f
     there is neither a residual nor dropout).  weight and bias are of x's type or float32."""
     seed, offset = _seed(seed, offset)
     m = _matrix(x, "x")
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    total = mean = rstd = None
+    rows, cols = m.rows, m.cols
+    out = _like(x)
+    total = mean = rstd = m_total = None
     if keep:
-        total = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None or p != 0 else x
-        mean, rstd = torch.empty((2,) + x.shape[:-1], dtype=torch.float32, device=x.device)
+        total = x
+        if residual is not None or p != 0:
+            total = _like(x)
+            m_total = _new(total, rows, cols)
+        mean, rstd = x.new_empty(x.shape[:-1], dtype=torch.float32), x.new_empty(x.shape[:-1], dtype=torch.float32)
     st = _capi.load().nvtext_amd_layer_norm(
-        m, _optional(residual, "residual"), _vector(weight, "weight"), _vector(bias, "bias"), eps, p, seed, offset, _stream_handle(),
-        _matrix(out, "out"), _matrix(total, "sum") if keep and total is not x else None, mean.data_ptr() if keep else None,
-        rstd.data_ptr() if keep else None)
+        m, None if residual is None else _matrix(residual, "residual"), _vector(weight, "weight"), _vector(bias, "bias"), eps, p, seed, offset, _stream_handle(),
+        _new(out, rows, cols), m_total, mean.data_ptr() if keep else None, rstd.data_ptr() if keep else None)
     if st != _capi.SUCCESS:
         _raise(st)
     return (out, LayerNormSaved(total, mean, rstd)) if keep else out
@@ -153,13 +165,14 @@ def layer_norm_backward(grad: torch.Tensor, saved: LayerNormSaved, weight: torch
     for t in (saved.mean, saved.rstd):
         if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != g.rows or not t.is_cuda:
             raise ValueError("mean and rstd must be contiguous float32 tensors of one value a row")
-    residual_grad = torch.empty(grad.shape, dtype=grad.dtype, device=grad.device)
-    x_grad = torch.empty(grad.shape, dtype=grad.dtype, device=grad.device) if p != 0 else residual_grad
-    weight_grad, bias_grad = torch.empty((2,) + weight.shape, dtype=weight.dtype, device=weight.device)
+    rows, cols = g.rows, g.cols
+    m_weight = _vector(weight, "weight")
+    residual_grad, weight_grad, bias_grad = _like(grad), _like(weight), _like(weight)
+    x_grad = _like(grad) if p != 0 else residual_grad
     st = _capi.load().nvtext_amd_layer_norm_backward(
-        g, _matrix(saved.sum, "sum"), saved.mean.data_ptr(), saved.rstd.data_ptr(), _vector(weight, "weight"), _optional(sum_grad, "sum_grad"),
-        p, seed, offset, _stream_handle(), _mr().struct, _matrix(x_grad, "x_grad") if p != 0 else None, _matrix(residual_grad, "residual_grad"),
-        _vector(weight_grad, "weight_grad"), _vector(bias_grad, "bias_grad"))
+        g, _matrix(saved.sum, "sum"), saved.mean.data_ptr(), saved.rstd.data_ptr(), m_weight, None if sum_grad is None else _matrix(sum_grad, "sum_grad"),
+        p, seed, offset, _stream_handle(), _mr().struct, _new(x_grad, rows, cols) if p != 0 else None, _new(residual_grad, rows, cols),
+        _new(weight_grad, 1, m_weight.cols), _new(bias_grad, 1, m_weight.cols))
     if st != _capi.SUCCESS:
         _raise(st)
     return x_grad, residual_grad, weight_grad, bias_grad
@@ -178,10 +191,12 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     was applied to) for linear_backward."""
     act = _activation(activation)
     m, w = _matrix(x, "x"), _matrix(weight, "weight")
-    out = torch.empty(x.shape[:-1] + weight.shape[:1], dtype=x.dtype, device=x.device)
+    rows, outputs = m.rows, w.rows
+    shape = (rows, outputs) if x.dim() == 2 else x.shape[:-1] + (outputs,)
+    out = x.new_empty(shape)
     z = torch.empty_like(out) if keep else None
-    st = _capi.load().nvtext_amd_linear(m, w, None if bias is None else _vector(bias, "bias"), act, _optional(residual, "residual"), _stream_handle(),
-                                        _mr().struct, _matrix(out, "out"), _optional(z, "preactivation"))
+    st = _capi.load().nvtext_amd_linear(m, w, None if bias is None else _vector(bias, "bias"), act, None if residual is None else _matrix(residual, "residual"),
+                                        _stream_handle(), _mr().struct, _new(out, rows, outputs), _new(z, rows, outputs) if keep else None)
     if st != _capi.SUCCESS:
         _raise(st)
     return (out, z) if keep else out
@@ -192,11 +207,10 @@ def linear_backward(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, a
     """(grad of x, grad of weight, grad of bias) of linear(); the residual's gradient is grad itself."""
     act = _activation(activation)
     g, m, w = _matrix(grad, "grad"), _matrix(x, "x"), _matrix(weight, "weight")
-    x_grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    weight_grad = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
-    bias_grad = torch.empty(weight.shape[:1], dtype=weight.dtype, device=weight.device)
-    st = _capi.load().nvtext_amd_linear_backward(g, m, w, act, _optional(preactivation, "preactivation"), _stream_handle(), _mr().struct,
-                                                 _matrix(x_grad, "x_grad"), _matrix(weight_grad, "weight_grad"), _vector(bias_grad, "bias_grad"))
+    x_grad, weight_grad = _like(x), _like(weight)
+    bias_grad = weight.new_empty(w.rows)
+    st = _capi.load().nvtext_amd_linear_backward(g, m, w, act, None if preactivation is None else _matrix(preactivation, "preactivation"), _stream_handle(), _mr().struct,
+                                                 _new(x_grad, m.rows, m.cols), _new(weight_grad, w.rows, w.cols), _new(bias_grad, 1, w.rows))
     if st != _capi.SUCCESS:
         _raise(st)
     return x_grad, weight_grad, bias_grad

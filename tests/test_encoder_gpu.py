@@ -312,7 +312,7 @@ def test_layer_norm_gradient_against_differences():
 
 # tokens, inputs, outputs, padding of the rows
 PRODUCTS = [(1, 1, 1, 0), (1, 1024, 64, 0), (1, 77, 333, 0), (2, 256, 48, 8), (3, 130, 17, 3), (5, 4096, 96, 0), (8, 64, 200, 0), (15, 33, 31, 1), (16, 512, 128, 0), (17, 96, 40, 8),
-            (31, 1000, 64, 0), (64, 64, 64, 0), (65, 65, 65, 1), (100, 31, 260, 0), (128, 256, 128, 0), (129, 264, 136, 8), (255, 72, 257, 0), (256, 128, 512, 0), (300, 40, 300, 4),
+            (31, 1000, 64, 0), (64, 64, 64, 0), (1, 2100, 40, 0), (20, 2051, 33, 3), (50, 2304, 24, 0), (40, 2048, 4200, 0), (65, 65, 65, 1), (100, 31, 260, 0), (128, 256, 128, 0), (129, 264, 136, 8), (255, 72, 257, 0), (256, 128, 512, 0), (300, 40, 300, 4),
             (513, 200, 520, 0), (700, 1032, 72, 0), (1, 8, 1000, 0), (2000, 16, 24, 0), (640, 320, 768, 0), (40, 2051, 24, 0)]
 # how much larger a slope than 1 an activation has, and what its own evaluation is off by, in units of 2^-24 of |z| + |result|
 STEEP = 1.15
@@ -476,6 +476,28 @@ def test_on_another_stream():
         got = calls()
     stream.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_more_dimensions_and_other_strides():
+    """Tensors of more dimensions are taken as the rows of their last; results are contiguous whatever the strides."""
+    big = torch.randn(3, 5, 4, 96, device="cuda", dtype=F16)
+    w, b = torch.randn(64, 64, device="cuda", dtype=F16), torch.randn(64, device="cuda", dtype=F16)
+    x = big[:, :, :, 16:80]
+    flat = x.reshape(60, 64)
+    y, z = encoder.linear(x, w, b, "silu", x, keep=True)
+    y2, z2 = encoder.linear(flat, w, b, "silu", flat, keep=True)
+    assert y.shape == x.shape and y.is_contiguous() and torch.equal(y.view(60, 64), y2) and torch.equal(z.view(60, 64), z2)
+    for a, c in zip(encoder.linear_backward(x, x, w, "silu", z), encoder.linear_backward(flat, flat, w, "silu", z2)):
+        assert torch.equal(a.reshape(c.shape), c)
+    n, saved = encoder.layer_norm(x, b, b, p=0.2, seed=1, residual=x, keep=True)
+    n2, saved2 = encoder.layer_norm(flat, b, b, p=0.2, seed=1, residual=flat, keep=True)
+    assert torch.equal(n.view(60, 64), n2) and saved.mean.shape == (3, 5, 4) and torch.equal(saved.rstd.view(60), saved2.rstd)
+    for a, c in zip(encoder.layer_norm_backward(x, saved, b, 0.2, 1), encoder.layer_norm_backward(flat, saved2, b, 0.2, 1)):
+        assert torch.equal(a.reshape(c.shape), c)
+    with pytest.raises(RuntimeError):
+        encoder.dropout(big.transpose(0, 1), 0.1, 1)  # rows that are not evenly spaced
+    wide = torch.randn(8, 128, device="cuda")[:, :64]
+    assert encoder.dropout(wide, 0.1, 1).is_contiguous() and torch.equal(encoder.dropout(wide, 0.1, 1), encoder.dropout(wide.contiguous(), 0.1, 1))
 
 
 def test_refusals():
