@@ -136,10 +136,9 @@ struct Epilogue {
 //           of k) lies at c ^ (i & 7): the rows that a fragment reads at one c are spread over all banks.
 //   else:   value k has EXT * 2 bytes, its units of 16 rows (32 bytes) lie at u ^ (k & 3 | (k >> 3 & 1) << 2), for the same reason;
 //           a fragment is read by the transposing load, four values of k at a time.
-// What lies outside the operands is read as zeros: its offset lies beyond the buffer's range.
+// What lies outside the operands is read as zeros: its offset lies beyond the buffer's range (at most 256 lines of 2^22 bytes).
 constexpr int kStageK     = 64;
-constexpr uint32_t kFar   = 0x80000000u;  // an offset outside every buffer
-constexpr uint32_t kRange = 0x7fffff00u;  // of offsets inside
+constexpr uint32_t kFar   = 0x80000000u;  // an offset outside every buffer, whatever is added for a row of the tile
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 template <typename T>
@@ -157,54 +156,64 @@ struct Side {
   int64_t stride;  // in values
 };
 
-// 16 bytes a lane from base + offset (nothing but zeros where the offset is kFar) to 16 bytes a lane from `to` on.  Written out: the
+// The same in every lane, and known to be.
+__device__ __forceinline__ int32_t uniform(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// 16 bytes a lane from base + offset to 16 bytes a lane from `to` on; zeros where the offset is not less than `range`.  Written out: the
 // compiler would wait for loads that it knows to write LDS before every transposing read of LDS (a product of which one operand
 // is read that way took 153 us instead of 118).  It has no register as a result, so it is waited for by stage_barrier alone.
-__device__ __forceinline__ void load_to_lds(const char* base, LdsBytes to, uint32_t offset)
+__device__ __forceinline__ void load_to_lds(const char* base, uint32_t range, LdsBytes to, uint32_t offset)
 {
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   uint64_t const address = reinterpret_cast<uint64_t>(base);
-  // a buffer of kRange bytes: address, no stride, length, plain 32-bit data
-  u32x4 const buffer = {static_cast<uint32_t>(address), static_cast<uint32_t>(address >> 32) & 0xffffu, kRange, 0x00027000u};
+  // a buffer: address, no stride, length, plain 32-bit data
+  u32x4 const buffer = {static_cast<uint32_t>(address), static_cast<uint32_t>(address >> 32) & 0xffffu, range, 0x00027000u};
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to))), "v"(offset), "s"(buffer)
                : "memory");  // (m0 is set wherever the compiler uses it itself)
 }
 
-// What a wavefront loads of an operand for a stage: PIECES loads.
+// What a wavefront loads of an operand for a stage: kPieces loads.  Lines behind the last, rows or values of k, lie behind the
+// buffer's range; the other direction is looked at lane by lane.
 template <bool K_NEXT, int EXT, int WAVES>
 struct Loader {
   static constexpr int kPieces = EXT / 8 / WAVES;
-  const char* base;      // of the tile's first value at k = 0
-  int64_t step;          // bytes from a stage to the next
-  uint32_t offset[kPieces];
-  int k_of[kPieces];     // the first k of the lane's pieces, in the stage
+  static constexpr int kLine   = EXT / 8;  // (not K_NEXT) lanes that a value of k takes
+  const char* base;  // of the tile's first value of the next stage
+  uint32_t line;     // bytes from a line to the next
+  uint32_t rows;     // (K_NEXT) bytes of the rows that are there
+  uint32_t offset[K_NEXT ? 1 : kPieces];
+  int k_first;       // (K_NEXT) of the lane's pieces, in the stage
 
-  __device__ __forceinline__ Loader(Side const& side, int64_t i0, int64_t extent, int64_t k0, int wave, int lane)
+  // at the tile of rows from i0 on, and at value k0 of k
+  __device__ __forceinline__ void aim(Side const& side, int64_t i0, int64_t extent, int64_t k0, int wave, int lane)
   {
     base = static_cast<const char*>(side.data) + 2 * (K_NEXT ? i0 * side.stride + k0 : k0 * side.stride + i0);
-    step = K_NEXT ? 2 * kStageK : 2 * kStageK * side.stride;
+    line = static_cast<uint32_t>(side.stride * 2);
+    if constexpr (K_NEXT) {
+      rows            = static_cast<uint32_t>(extent - i0 < EXT ? extent - i0 : EXT) * line;
+      int const row   = wave * kPieces * 8 + lane / 8;
+      int const piece = (lane % 8) ^ (lane / 8);
+      k_first         = piece * 8;
+      offset[0]       = row * line + piece * 16;
+    } else {
 #pragma unroll
-    for (int p = 0; p < kPieces; ++p) {
-      int const q = wave * kPieces + p;
-      if constexpr (K_NEXT) {
-        int const row = q * 8 + lane / 8, piece = (lane % 8) ^ (row & 7);
-        k_of[p]   = piece * 8;
-        offset[p] = i0 + row < extent ? static_cast<uint32_t>(row * side.stride * 2 + piece * 16) : kFar;
-      } else {
-        constexpr int kLine = EXT / 8;  // lanes that a value of k takes
-        int const k = q * (kWave / kLine) + lane / kLine, at = lane % kLine;
+      for (int p = 0; p < kPieces; ++p) {
+        int const k = (wave * kPieces + p) * (kWave / kLine) + lane / kLine, at = lane % kLine;
         int const piece = ((at >> 1) ^ ((k & 3) | (k >> 3 & 1) << 2)) * 2 + (at & 1);
-        k_of[p]   = k;
-        offset[p] = i0 + piece * 8 < extent ? static_cast<uint32_t>(k * side.stride * 2 + piece * 16) : kFar;
+        offset[p] = i0 + piece * 8 < extent ? k * line + piece * 16 : kFar;
       }
     }
   }
-  // Piece `p` of the next stage, of whose 64 values of k `left` are there (any number), into `to`.
-  __device__ __forceinline__ void load(LdsBytes to, int64_t left, int wave, int p) const
+  // Piece `p` of the next stage, of whose 64 values of k `here` are there, into `to`.
+  __device__ __forceinline__ void load(LdsBytes to, int here, int wave, int p) const
   {
-    load_to_lds(base, to + (wave * kPieces + p) * 1024, k_of[p] < (left < kStageK ? static_cast<int>(left) : kStageK) ? offset[p] : kFar);
+    LdsBytes const place = to + (wave * kPieces + p) * 1024;
+    if constexpr (K_NEXT)
+      load_to_lds(base, rows, place, (k_first < here ? offset[0] : kFar) + p * 8 * line);
+    else
+      load_to_lds(base, here * line, place, offset[p]);
   }
-  __device__ __forceinline__ void next() { base += step; }
+  __device__ __forceinline__ void next() { base += K_NEXT ? 2 * kStageK : static_cast<int64_t>(kStageK) * line; }
 };
 
 // Where a lane finds the fragments of 16 rows each, the first beginning at row `first` of the tile.
@@ -244,41 +253,71 @@ __device__ __forceinline__ void stage_barrier()
   asm volatile("s_barrier" ::: "memory");
 }
 
-// A workgroup a tile of BM x BN (blockIdx.x), over the values of k of its part of them (blockIdx.y).  WAVES_M x WAVES_N wavefronts,
-// each with MI x NI fragments of 16 x 16.
+// Where an item of work, a tile of the result and a part of the values of k, begins.
+struct Item {
+  int64_t i0, j0;
+  int32_t part;
+};
+
+// A workgroup takes items of BM x BN one after the other.  WAVES_M x WAVES_N wavefronts, each with MI x NI fragments of 16 x 16.
+// The loads are a stream of stages that goes on from an item into the next: the first two stages of an item come while the
+// one before is finished and written, for which the wavefronts have LDS of their own (waiting for them anew at every item
+// cost 30 of 265 us at 32768 x 1024 x 4096).
 template <typename T, bool A_NEXT, bool B_NEXT, int BM, int BN, int WAVES_M, int WAVES_N>
-__device__ __forceinline__ void tile_product(Side a, Side b, int64_t m, int64_t n, int64_t depth, int64_t part, float* sums, Epilogue<T> end)
+__device__ __forceinline__ void tile_product(Side a, Side b, int64_t m, int64_t n, int64_t depth, int32_t parts, int64_t part, float* sums, Epilogue<T> end)
 {
   constexpr int kWaves = WAVES_M * WAVES_N, MI = BM / WAVES_M / 16, NI = BN / WAVES_N / 16;
   constexpr int kStage = (BM + BN) * 128, kLoads = (BM + BN) / 8 / kWaves;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+  static_assert(NI == 4, "");
+  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage + kWaves * 16 * 256];
   LdsBytes const stages = (LdsBytes)lds;
   int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
   int const wm = wave / WAVES_N, wn = wave % WAVES_N;
 
-  // Workgroups go to the eight XCDs in turn: each takes a run of tiles, within which eight tiles of rows share their columns.
-  int64_t const tiles_m = (m + BM - 1) / BM, tiles_n = (n + BN - 1) / BN, tiles = tiles_m * tiles_n;
+  // Workgroups go to the eight XCDs in turn: each takes a run of items, within which eight tiles of rows share their columns.
+  int32_t const tiles_m = uniform(static_cast<int32_t>((m + BM - 1) / BM)), tiles_n = uniform(static_cast<int32_t>((n + BN - 1) / BN)), tiles = tiles_m * tiles_n;
+  int32_t const items = tiles * parts;
   constexpr int kXcds = 8, kGroup = 8;
-  int64_t const per_xcd = tiles / kXcds, more = tiles % kXcds, xcd = blockIdx.x % kXcds;
-  int64_t const tile  = blockIdx.x / kXcds + xcd * per_xcd + (xcd < more ? xcd : more);
-  int64_t const group = tile / (kGroup * tiles_n), in_group = tile % (kGroup * tiles_n);
-  int64_t const rows_here = tiles_m - group * kGroup < kGroup ? tiles_m - group * kGroup : kGroup;
-  int64_t const i0 = (group * kGroup + in_group % rows_here) * BM, j0 = in_group / rows_here * BN;
+  int32_t const xcd = blockIdx.x % kXcds, per_xcd = items / kXcds, more = items % kXcds;
+  int32_t const begin = xcd * per_xcd + (xcd < more ? xcd : more), last = begin + per_xcd + (xcd < more ? 1 : 0);
+  int32_t const stride = gridDim.x / kXcds + (xcd < static_cast<int32_t>(gridDim.x % kXcds) ? 1 : 0);  // workgroups of this XCD
+  auto const place = [&](int32_t item) {
+    int32_t const p = uniform(item / tiles), tile = item - p * tiles, group = uniform(tile / (kGroup * tiles_n)), in_group = tile - group * kGroup * tiles_n;
+    int32_t const rows_here = tiles_m - group * kGroup < kGroup ? tiles_m - group * kGroup : kGroup;
+    int32_t const column    = uniform(in_group / rows_here);
+    return Item{static_cast<int64_t>(group * kGroup + in_group - column * rows_here) * BM, static_cast<int64_t>(column) * BN, p};
+  };
+  auto const values_of = [&](Item const& at) { return depth - at.part * part < part ? depth - at.part * part : part; };
 
-  int64_t const k0 = static_cast<int64_t>(blockIdx.y) * part;
-  int64_t left     = depth - k0 < part ? depth - k0 : part;  // values of k that are still to be loaded
-  int const steps  = static_cast<int>((left + kStageK - 1) / kStageK);
-  Loader<A_NEXT, BM, kWaves> load_a(a, i0, m, k0, wave, lane);
-  Loader<B_NEXT, BN, kWaves> load_b(b, j0, n, k0, wave, lane);
+  Loader<A_NEXT, BM, kWaves> load_a;
+  Loader<B_NEXT, BN, kWaves> load_b;
   Reader<T, A_NEXT, BM> const read_a(wm * MI * 16, lane);
   Reader<T, B_NEXT, BN> const read_b(wn * NI * 16, lane);
-  // Two stages are in LDS.  Load number `p` of the next one, into place `slot`:
+  int32_t const first = begin + static_cast<int32_t>(blockIdx.x / kXcds);
+  int32_t loaded      = first;  // the item whose stages are loaded
+  int64_t left        = 0;      // values of k of it that are still to be loaded
+  auto const aim = [&] {
+    Item const at = place(loaded);
+    load_a.aim(a, at.i0, m, at.part * part, wave, lane);
+    load_b.aim(b, at.j0, n, at.part * part, wave, lane);
+    left = values_of(at);
+  };
+  if (loaded >= last) return;
+  aim();
+  // Two stages are in LDS.  Load number `p` of the next one, into place `slot`; behind the last stage of all, zeros.
+  auto const before_stage = [&] {
+    if (left <= 0 && depth > 0 && loaded + stride < last) {
+      loaded += stride;
+      aim();
+    }
+  };
   auto const load = [&](int slot, int p) {
     LdsBytes const to = stages + slot * kStage;
+    int const here    = static_cast<int>(left < 0 ? 0 : left < kStageK ? left : kStageK);
     if (p < BM / 8 / kWaves)
-      load_a.load(to, left, wave, p);
+      load_a.load(to, here, wave, p);
     else
-      load_b.load(to + BM * 128, left, wave, p - BM / 8 / kWaves);
+      load_b.load(to + BM * 128, here, wave, p - BM / 8 / kWaves);
     if (p == kLoads - 1) {
       load_a.next();
       load_b.next();
@@ -286,99 +325,118 @@ __device__ __forceinline__ void tile_product(Side a, Side b, int64_t m, int64_t 
     }
   };
   f32x4_t sum[MI][NI];
-#pragma unroll
-  for (int i = 0; i < MI; ++i)
-#pragma unroll
-    for (int j = 0; j < NI; ++j) sum[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   struct Fragments {
     Fragment<T> a[MI], b[NI];
   };
   Fragments f[2];
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
+  for (int s = 0; s < 2; ++s) {
+    before_stage();
 #pragma unroll
     for (int p = 0; p < kLoads; ++p) load(s, p);
+  }
   stage_barrier<kLoads>();
+  // (in the order of the reads in the loop: what the compiler waits for there follows from both)
 #pragma unroll
-  for (int j = 0; j < NI; ++j) f[0].b[j] = read_b.read(stages + BM * 128, 0, j);
-#pragma unroll
-  for (int i = 0; i < MI; ++i) f[0].a[i] = read_a.read(stages, 0, i);
-  // Multiplies the fragments of one half of a stage and reads those of the next, a little of either in turn: left to itself, the
-  // compiler puts all reads behind the products.  SECOND: the next half is the first of the other stage, for which everybody waits
-  // after a row of products; this stage has been read then and makes room for the one after that.
+  for (int r = 0; r < MI + NI; ++r) {
+    if (r == 0 || r > NI)
+      f[0].a[r == 0 ? 0 : r - NI] = read_a.read(stages, 0, r == 0 ? 0 : r - NI);
+    else
+      f[0].b[r - 1] = read_b.read(stages + BM * 128, 0, r - 1);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // Multiplies the fragments of one half of a stage, reads those of the next and asks for stages to come: after each product, which
+  // keeps the matrix core busy for 16 cycles, at most one read or load, in this order (left to itself, the compiler puts the
+  // products together).  SECOND: the next half is the first of the other stage, for which everybody waits after a row of
+  // products; this stage has been read then and makes room for the one after that.
   auto const step = [&](Fragments const& now, Fragments& next, int slot, auto second) {
     constexpr bool kSecond = decltype(second)::value;
     LdsBytes const from    = stages + (kSecond ? slot ^ 1 : slot) * kStage;
+    if constexpr (kSecond) before_stage();
+    // read number r: a fragment of a, all of b, the others of a
+    auto const read = [&](int r) {
+      if (r == 0 || r > NI)
+        next.a[r == 0 ? 0 : r - NI] = read_a.read(from, kSecond ? 0 : 1, r == 0 ? 0 : r - NI);
+      else
+        next.b[r - 1] = read_b.read(from + BM * 128, kSecond ? 0 : 1, r - 1);
+    };
+    constexpr int kReads = MI + NI, kOps = kReads + (kSecond ? kLoads : 0), kFrom = kSecond ? NI : 0, kSlots = MI * NI - kFrom - 2;
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      // read number r: a fragment of a, all of b, the others of a
-      auto const read = [&](int r) {
-        if (r == 0 || r > NI)
-          next.a[r == 0 ? 0 : r - NI] = read_a.read(from, kSecond ? 0 : 1, r == 0 ? 0 : r - NI);
-        else
-          next.b[r - 1] = read_b.read(from + BM * 128, kSecond ? 0 : 1, r - 1);
-      };
-      constexpr int kRows  = kSecond ? MI - 1 : MI;  // that loads and reads go with
-      constexpr int kReads = (MI + NI + kRows - 1) / kRows, kLoadsEach = (kLoads + kRows - 1) / kRows;
-      if constexpr (kSecond) {
-        if (i == 1) stage_barrier<0>();
+    for (int q = 0; q < MI * NI; ++q) {
+      int const i = q / NI, j = q % NI;
+      if (kSecond && q == NI) stage_barrier<0>();
+      sum[i][j] = multiply(now.b[j], now.a[i], sum[i][j]);  // (the transposed tile: a lane has four values of a row)
 #pragma unroll
-        for (int p = (i - 1) * kLoadsEach; p < i * kLoadsEach; ++p)
-          if (i >= 1 && p < kLoads) load(slot, p);
+      for (int o = 0; o < kOps; ++o) {
+        if (kFrom + o * kSlots / kOps != q) continue;
+        // reads and loads in turn, as far as there are both
+        constexpr int kBoth = kSecond ? (kReads < kLoads ? kReads : kLoads) : 0;
+        if (o < 2 * kBoth) {
+          if (o % 2 == 0)
+            read(o / 2);
+          else
+            load(slot, o / 2);
+        } else if (kReads > kBoth) {
+          read(o - kBoth);
+        } else {
+          load(slot, o - kBoth);
+        }
       }
-      int const g = kSecond ? i - 1 : i;
-#pragma unroll
-      for (int r = g * kReads; r < (g + 1) * kReads; ++r)
-        if (g >= 0 && r < MI + NI) read(r);
-#pragma unroll
-      for (int j = 0; j < NI; ++j) sum[i][j] = multiply(now.b[j], now.a[i], sum[i][j]);  // (the transposed tile: a lane has four values of a row)
       __builtin_amdgcn_sched_barrier(0);
     }
   };
   int slot = 0;  // of the stage that is multiplied
-  for (int t = 0; t < steps; ++t) {
-    step(f[0], f[1], slot, std::false_type{});
-    step(f[1], f[0], slot, std::true_type{});
-    slot ^= 1;
-  }
-  stage_barrier<0>();
-
-  // Every wavefront turns its tile round in its own part of LDS, 64 rows at a time, and goes on with eight values of a row a lane.
-  // (A row's 16 units of four values lie at unit ^ row % 16.)
-  static_assert(NI == 4 && MI % 4 == 0 && kWaves * 64 * 256 <= 2 * kStage, "");
-  LdsBytes const mine = stages + wave * (64 * 256);
-  int64_t const j     = j0 + wn * 64 + lane % 8 * 8;
-  typename Epilogue<T>::Columns const columns(end, j, n);
+  for (int32_t item = first; item < last; item += stride) {
+    Item const at   = place(item);
+    int const steps = static_cast<int>((values_of(at) + kStageK - 1) / kStageK);
 #pragma unroll
-  for (int half = 0; half < MI / 4; ++half) {
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int c = 0; c < NI; ++c)
-        *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(mine + (i * 16 + lane % 16) * 256 + ((c * 4 + lane / 16) ^ (lane % 16)) * 16) = sum[half * 4 + i][c];
-    wave_lds_fence();
-    int64_t const first = i0 + (wm * MI + half * 4) * 16;
-#pragma nounroll
-    for (int row = lane / 8; row < 64; row += 8) {
-      auto const unit = [&](int u) { return *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(mine + row * 256 + (u ^ (row % 16)) * 16); };
-      f32x4_t const x = unit(lane % 8 * 2), y = unit(lane % 8 * 2 + 1);
-      float z[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-      if (first + row < m && j < n) {
-        if (sums)
-          store8(sums + (static_cast<int64_t>(blockIdx.y) * m + first + row) * n + j, z, n - j);
-        else
-          end.finish(z, columns, first + row, j, n);
-      }
+      for (int j = 0; j < NI; ++j) sum[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < steps; ++t) {
+      step(f[0], f[1], slot, std::false_type{});
+      step(f[1], f[0], slot, std::true_type{});
+      slot ^= 1;
     }
-    wave_lds_fence();
+    // Every wavefront turns its tile round in its own part of LDS, 16 rows at a time, and goes on with eight values of a row a lane.
+    // (A row's 16 units of four values lie at unit ^ row.)
+    LdsBytes const mine = stages + 2 * kStage + wave * (16 * 256);
+    int64_t const j     = at.j0 + wn * 64 + lane % 8 * 8;
+    typename Epilogue<T>::Columns const columns(end, j, n);
+#pragma nounroll
+    for (int rows = 0; rows < MI; ++rows) {
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        if (i != rows) continue;
+#pragma unroll
+        for (int c = 0; c < NI; ++c)
+          *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(mine + lane % 16 * 256 + ((c * 4 + lane / 16) ^ (lane % 16)) * 16) = sum[i][c];
+      }
+      wave_lds_fence();
+#pragma nounroll
+      for (int row = lane / 8; row < 16; row += 8) {
+        auto const unit = [&](int u) { return *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(mine + row * 256 + (u ^ row) * 16); };
+        f32x4_t const x = unit(lane % 8 * 2), y = unit(lane % 8 * 2 + 1);
+        float z[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        int64_t const i = at.i0 + (wm * MI + rows) * 16 + row;
+        if (i < m && j < n) {
+          if (sums)
+            store8(sums + (at.part * m + i) * n + j, z, n - j);
+          else
+            end.finish(z, columns, i, j, n);
+        }
+      }
+      wave_lds_fence();
+    }
   }
+  stage_barrier<0>();  // (the loads behind the last stage write LDS as well, which is not to be given away before)
 }
 
 template <typename T, bool A_NEXT, bool B_NEXT, int BM, int BN, int WAVES_M, int WAVES_N>
 __global__ void __launch_bounds__(WAVES_M * WAVES_N * kWave, 2)
-tile_product_kernel(Side a, Side b, int64_t m, int64_t n, int64_t depth, int64_t part, float* sums, Epilogue<T> end)
+tile_product_kernel(Side a, Side b, int64_t m, int64_t n, int64_t depth, int32_t parts, int64_t part, float* sums, Epilogue<T> end)
 {
-  tile_product<T, A_NEXT, B_NEXT, BM, BN, WAVES_M, WAVES_N>(a, b, m, n, depth, part, sums, end);
+  tile_product<T, A_NEXT, B_NEXT, BM, BN, WAVES_M, WAVES_N>(a, b, m, n, depth, parts, part, sums, end);
 }
 
 // ------------------------------------------------------------------ products of few rows
@@ -554,22 +612,25 @@ bool is_aligned(Factor<T> const& f, int64_t extent, int64_t depth)
 }
 
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
-void launch_tiles(Side a, bool a_next, Side b, bool b_next, int64_t m, int64_t n, int64_t depth, int64_t part, float* sums, Epilogue<T> const& end, hipStream_t stream)
+void launch_tiles(Side a, bool a_next, Side b, bool b_next, int64_t m, int64_t n, int64_t depth, int32_t parts, int64_t part, float* sums, Epilogue<T> const& end, hipStream_t stream)
 {
-  dim3 const grid(static_cast<unsigned>((m + BM - 1) / BM * ((n + BN - 1) / BN)), static_cast<unsigned>(std::max<int64_t>(1, (depth + part - 1) / part)));
+  // as many workgroups as the CUs hold at once
+  int64_t const items = (m + BM - 1) / BM * ((n + BN - 1) / BN) * parts, at_once = (BM == 256 ? 1 : 2) * static_cast<int64_t>(device_cus());
+  dim3 const grid(static_cast<unsigned>(std::min(items, at_once)));
   dim3 const threads(WAVES_M * WAVES_N * kWave);
   if (a_next && b_next)
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, true, true, BM, BN, WAVES_M, WAVES_N>), grid, threads, 0, stream, a, b, m, n, depth, part, sums, end);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, true, true, BM, BN, WAVES_M, WAVES_N>), grid, threads, 0, stream, a, b, m, n, depth, parts, part, sums, end);
   else if (a_next)
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, true, false, BM, BN, WAVES_M, WAVES_N>), grid, threads, 0, stream, a, b, m, n, depth, part, sums, end);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, true, false, BM, BN, WAVES_M, WAVES_N>), grid, threads, 0, stream, a, b, m, n, depth, parts, part, sums, end);
   else
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, false, false, BM, BN, WAVES_M, WAVES_N>), grid, threads, 0, stream, a, b, m, n, depth, part, sums, end);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, false, false, BM, BN, WAVES_M, WAVES_N>), grid, threads, 0, stream, a, b, m, n, depth, parts, part, sums, end);
 }
 
 // How a product is shared out: tiles of 256 x 256 or of 128 x 128, and so many parts of the values of k.
 struct Plan {
   bool large;
-  int64_t parts, part;  // values of k a part
+  int32_t parts;
+  int64_t part;  // values of k a part
 };
 
 // The one that takes the least by this measure, in microseconds: CUs go through their workgroups in rounds, and parts are written and
@@ -589,7 +650,7 @@ inline Plan plan_product(int64_t m, int64_t n, int64_t depth)
       double const time   = rounds + (parts > 1 ? 5 + parts * m * n * 8e-6 / 5 : 0);
       if (time < least) {
         least = time;
-        best  = Plan{large, parts, each * kStageK};
+        best  = Plan{large, static_cast<int32_t>(parts), each * kStageK};
       }
     }
   }
@@ -644,6 +705,7 @@ nvtext_amd_status launch_product(Factor<T> a, Factor<T> b, int64_t m, int64_t n,
     auto const lines  = [&](Factor<T> const& f, int64_t extent) { return f.k_next ? extent : depth; };
     auto const width  = [&](Factor<T> const& f, int64_t extent) { return ((f.k_next ? depth : extent) + 7) / 8 * 8; };
     Plan const plan   = plan_product(m, n, depth);
+    if ((m + 127) / 128 * ((n + 127) / 128) > INT32_MAX / 32) return fail(NVTEXT_AMD_OVERFLOW, "the product is too large");
     TempParts<3> const temp(mr,
                             {copy_a ? static_cast<size_t>(lines(a, m) * width(a, m)) * sizeof(T) : 0, copy_b ? static_cast<size_t>(lines(b, n) * width(b, n)) * sizeof(T) : 0,
                              plan.parts > 1 ? static_cast<size_t>(plan.parts * m * n) * sizeof(float) : 0},
@@ -660,9 +722,9 @@ nvtext_amd_status launch_product(Factor<T> a, Factor<T> b, int64_t m, int64_t n,
     float* const sums = plan.parts > 1 ? temp.template part<float>(2) : nullptr;
     Side const sa{a.rows.data, a.rows.stride}, sb{b.rows.data, b.rows.stride};
     if (plan.large)
-      launch_tiles<T, 256, 256, 2, 4>(sa, a.k_next, sb, b.k_next, m, n, depth, plan.part, sums, end, stream);
+      launch_tiles<T, 256, 256, 2, 4>(sa, a.k_next, sb, b.k_next, m, n, depth, plan.parts, plan.part, sums, end, stream);
     else
-      launch_tiles<T, 128, 128, 2, 2>(sa, a.k_next, sb, b.k_next, m, n, depth, plan.part, sums, end, stream);
+      launch_tiles<T, 128, 128, 2, 2>(sa, a.k_next, sb, b.k_next, m, n, depth, plan.parts, plan.part, sums, end, stream);
     if (sums)
       hipLaunchKernelGGL(join_parts_kernel<T>, dim3(static_cast<unsigned>(std::min<int64_t>((m * ((n + 7) / 8) + kThreads - 1) / kThreads, 32 * device_cus()))), dim3(kThreads), 0, stream,
                          sums, plan.parts, m, n, end);
