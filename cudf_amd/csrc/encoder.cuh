@@ -75,14 +75,18 @@ __device__ __forceinline__ void load8(float (&f)[8], const T* p, int64_t n)
   }
 }
 
-template <typename T>
+// PAST: past the caches
+template <bool PAST = false, typename T>
 __device__ __forceinline__ void store8(T* p, float const (&f)[8], int64_t n)
 {
   if (n >= 8) {
     typename Eight<T>::type v;
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = static_cast<T>(f[k]);
-    *reinterpret_cast<typename Eight<T>::type*>(p) = v;
+    if constexpr (PAST)
+      __builtin_nontemporal_store(v, reinterpret_cast<typename Eight<T>::type*>(p));
+    else
+      *reinterpret_cast<typename Eight<T>::type*>(p) = v;
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
