@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 namespace nvtext_amd {
 namespace {
@@ -251,6 +252,18 @@ __device__ __forceinline__ void stage_barrier()
   asm volatile("s_barrier" ::: "memory");
 }
 
+// f(0), ... f(N - 1) with the numbers as constants, so that arrays that they index stay in registers.
+template <typename F, int... I>
+__device__ __forceinline__ void for_each(std::integer_sequence<int, I...>, F&& f)
+{
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void for_each(F&& f)
+{
+  for_each(std::make_integer_sequence<int, N>{}, f);
+}
+
 // Where an item of work, a tile of the result and a part of the values of k, begins.
 struct Item {
   int64_t i0, j0;
@@ -265,9 +278,9 @@ template <typename T, bool A_NEXT, bool B_NEXT, int BM, int BN, int WAVES_M, int
 __device__ __forceinline__ void tile_product(Side a, Side b, int64_t m, int64_t n, int64_t depth, int32_t parts, int64_t part, float* sums, Epilogue<T> end)
 {
   constexpr int kWaves = WAVES_M * WAVES_N, MI = BM / WAVES_M / 16, NI = BN / WAVES_N / 16;
+  constexpr int kCols = NI * 16, kRowLanes = kCols / 8;  // of a wavefront's tile: columns, lanes that a row takes in the end
   constexpr int kStage = (BM + BN) * 128, kLoads = (BM + BN) / 8 / kWaves;
-  static_assert(NI == 4, "");
-  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage + kWaves * 16 * 256];
+  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage + kWaves * 16 * kCols * 4];
   LdsBytes const stages = (LdsBytes)lds;
   int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
   int const wm = wave / WAVES_N, wn = wave % WAVES_N;
@@ -359,62 +372,57 @@ __device__ __forceinline__ void tile_product(Side a, Side b, int64_t m, int64_t 
         next.b[r - 1] = read_b.read(from + BM * 128, kSecond ? 0 : 1, r - 1);
     };
     constexpr int kReads = MI + NI, kOps = kReads + (kSecond ? kLoads : 0), kFrom = kSecond ? NI : 0, kSlots = MI * NI - kFrom - 2;
-#pragma unroll
-    for (int q = 0; q < MI * NI; ++q) {
-      int const i = q / NI, j = q % NI;
-      if (kSecond && q == NI) stage_barrier<0>();
+    for_each<MI * NI>([&](auto slot_of) {
+      constexpr int q = decltype(slot_of)::value, i = q / NI, j = q % NI;
+      if constexpr (kSecond && q == NI) stage_barrier<0>();
       sum[i][j] = multiply(now.b[j], now.a[i], sum[i][j]);  // (the transposed tile: a lane has four values of a row)
-#pragma unroll
-      for (int o = 0; o < kOps; ++o) {
-        if (kFrom + o * kSlots / kOps != q) continue;
-        // reads and loads in turn, as far as there are both
-        constexpr int kBoth = kSecond ? (kReads < kLoads ? kReads : kLoads) : 0;
-        if (o < 2 * kBoth) {
-          if (o % 2 == 0)
-            read(o / 2);
-          else
-            load(slot, o / 2);
-        } else if (kReads > kBoth) {
-          read(o - kBoth);
-        } else {
-          load(slot, o - kBoth);
+      for_each<kOps>([&](auto op) {
+        constexpr int o = decltype(op)::value;
+        if constexpr (kFrom + o * kSlots / kOps == q) {
+          // reads and loads in turn, as far as there are both
+          constexpr int kBoth = kSecond ? (kReads < kLoads ? kReads : kLoads) : 0;
+          if constexpr (o < 2 * kBoth) {
+            if constexpr (o % 2 == 0)
+              read(o / 2);
+            else
+              load(slot, o / 2);
+          } else if constexpr (kReads > kBoth) {
+            read(o - kBoth);
+          } else {
+            load(slot, o - kBoth);
+          }
         }
-      }
+      });
       __builtin_amdgcn_sched_barrier(0);
-    }
+    });
   };
   int slot = 0;  // of the stage that is multiplied
   for (int32_t item = first; item < last; item += stride) {
     Item const at   = place(item);
     int const steps = static_cast<int>((values_of(at) + kStageK - 1) / kStageK);
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int j = 0; j < NI; ++j) sum[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for_each<MI * NI>([&](auto q) { sum[decltype(q)::value / NI][decltype(q)::value % NI] = f32x4_t{0.f, 0.f, 0.f, 0.f}; });
     for (int t = 0; t < steps; ++t) {
       step(f[0], f[1], slot, std::false_type{});
       step(f[1], f[0], slot, std::true_type{});
       slot ^= 1;
     }
     // Every wavefront turns its tile round in its own part of LDS, 16 rows at a time, and goes on with eight values of a row a lane.
-    // (A row's 16 units of four values lie at unit ^ row.)
-    LdsBytes const mine = stages + 2 * kStage + wave * (16 * 256);
-    int64_t const j     = at.j0 + wn * 64 + lane % 8 * 8;
+    // (A row's units of four values lie at unit ^ row.)
+    LdsBytes const mine = stages + 2 * kStage + wave * (16 * kCols * 4);
+    int64_t const j     = at.j0 + wn * kCols + lane % kRowLanes * 8;
     typename Epilogue<T>::Columns const columns(end, j, n);
 #pragma nounroll
     for (int rows = 0; rows < MI; ++rows) {
-#pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        if (i != rows) continue;
-#pragma unroll
-        for (int c = 0; c < NI; ++c)
-          *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(mine + lane % 16 * 256 + ((c * 4 + lane / 16) ^ (lane % 16)) * 16) = sum[i][c];
-      }
+      for_each<MI * NI>([&](auto q) {
+        constexpr int i = decltype(q)::value / NI, c = decltype(q)::value % NI;
+        if (i == rows)
+          *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(mine + lane % 16 * kCols * 4 + ((c * 4 + lane / 16) ^ (lane % 16)) * 16) = sum[i][c];
+      });
       wave_lds_fence();
 #pragma nounroll
-      for (int row = lane / 8; row < 16; row += 8) {
-        auto const unit = [&](int u) { return *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(mine + row * 256 + (u ^ row) * 16); };
-        f32x4_t const x = unit(lane % 8 * 2), y = unit(lane % 8 * 2 + 1);
+      for (int row = lane / kRowLanes; row < 16; row += kWave / kRowLanes) {
+        auto const unit = [&](int u) { return *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(mine + row * kCols * 4 + (u ^ row) * 16); };
+        f32x4_t const x = unit(lane % kRowLanes * 2), y = unit(lane % kRowLanes * 2 + 1);
         float z[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
         int64_t const i = at.i0 + (wm * MI + rows) * 16 + row;
         if (i < m && j < n) {
@@ -431,7 +439,7 @@ __device__ __forceinline__ void tile_product(Side a, Side b, int64_t m, int64_t 
 }
 
 template <typename T, bool A_NEXT, bool B_NEXT, int BM, int BN, int WAVES_M, int WAVES_N>
-__global__ void __launch_bounds__(WAVES_M * WAVES_N * kWave, 2)
+__global__ void __launch_bounds__(WAVES_M * WAVES_N * kWave, BM * BN / (WAVES_M * WAVES_N) > 8192 ? 1 : 2)
 tile_product_kernel(Side a, Side b, int64_t m, int64_t n, int64_t depth, int32_t parts, int64_t part, float* sums, Epilogue<T> end)
 {
   tile_product<T, A_NEXT, B_NEXT, BM, BN, WAVES_M, WAVES_N>(a, b, m, n, depth, parts, part, sums, end);
