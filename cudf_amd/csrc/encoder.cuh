@@ -27,7 +27,7 @@ struct Rows {
   T* data;
   int64_t stride;
   __device__ __forceinline__ T* row(int64_t i) const { return data + i * stride; }
-  __device__ __forceinline__ explicit operator bool() const { return data != nullptr; }
+  __host__ __device__ __forceinline__ explicit operator bool() const { return data != nullptr; }
 };
 
 template <typename T>

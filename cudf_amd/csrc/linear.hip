@@ -264,6 +264,17 @@ __device__ __forceinline__ void for_each(F&& f)
   for_each(std::make_integer_sequence<int, N>{}, f);
 }
 
+// A product: out (m x n) of operands a and b, with `depth` values of k in `parts` parts of `part` values; of several parts the sums go
+// to sums [part][m][n] and are finished by join_kernel.
+template <typename T>
+struct Problem {
+  Side a, b;
+  int64_t m, n, depth, part;
+  int32_t parts;
+  float* sums;
+  Epilogue<T> end;
+};
+
 // Where an item of work, a tile of the result and a part of the values of k, begins.
 struct Item {
   int64_t i0, j0;
@@ -275,13 +286,24 @@ struct Item {
 // one before is finished and written, for which the wavefronts have LDS of their own (waiting for them anew at every item
 // cost 30 of 265 us at 32768 x 1024 x 4096).
 template <typename T, bool A_NEXT, bool B_NEXT, int BM, int BN, int WAVES_M, int WAVES_N>
-__device__ __forceinline__ void tile_product(Side a, Side b, int64_t m, int64_t n, int64_t depth, int32_t parts, int64_t part, float* sums, Epilogue<T> end)
+struct TileProduct {
+  static constexpr int kWaves = WAVES_M * WAVES_N, MI = BM / WAVES_M / 16, NI = BN / WAVES_N / 16;
+  static constexpr int kCols = NI * 16, kRowLanes = kCols / 8;  // of a wavefront's tile: columns, lanes that a row takes in the end
+  static constexpr int kStage = (BM + BN) * 128, kLoads = (BM + BN) / 8 / kWaves;
+  static constexpr int kLds = 2 * kStage + kWaves * 16 * kCols * 4;
+  // as workgroup `block` of `blocks`
+  static __device__ __forceinline__ void run(Problem<T> const& problem, LdsBytes stages, int32_t block, int32_t blocks);
+};
+
+template <typename T, bool A_NEXT, bool B_NEXT, int BM, int BN, int WAVES_M, int WAVES_N>
+__device__ __forceinline__ void TileProduct<T, A_NEXT, B_NEXT, BM, BN, WAVES_M, WAVES_N>::run(Problem<T> const& problem, LdsBytes stages, int32_t block, int32_t blocks)
 {
-  constexpr int kWaves = WAVES_M * WAVES_N, MI = BM / WAVES_M / 16, NI = BN / WAVES_N / 16;
-  constexpr int kCols = NI * 16, kRowLanes = kCols / 8;  // of a wavefront's tile: columns, lanes that a row takes in the end
-  constexpr int kStage = (BM + BN) * 128, kLoads = (BM + BN) / 8 / kWaves;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage + kWaves * 16 * kCols * 4];
-  LdsBytes const stages = (LdsBytes)lds;
+  Side const a = problem.a, b = problem.b;
+  int64_t const m = problem.m, n = problem.n, depth = problem.depth, part = problem.part;
+  int32_t const parts    = problem.parts;
+  float* const sums      = problem.sums;
+  Epilogue<T> const& end = problem.end;
+
   int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
   int const wm = wave / WAVES_N, wn = wave % WAVES_N;
 
@@ -289,9 +311,9 @@ __device__ __forceinline__ void tile_product(Side a, Side b, int64_t m, int64_t 
   int32_t const tiles_m = uniform(static_cast<int32_t>((m + BM - 1) / BM)), tiles_n = uniform(static_cast<int32_t>((n + BN - 1) / BN)), tiles = tiles_m * tiles_n;
   int32_t const items = tiles * parts;
   constexpr int kXcds = 8, kGroup = 8;
-  int32_t const xcd = blockIdx.x % kXcds, per_xcd = items / kXcds, more = items % kXcds;
+  int32_t const xcd = block % kXcds, per_xcd = items / kXcds, more = items % kXcds;
   int32_t const begin = xcd * per_xcd + (xcd < more ? xcd : more), last = begin + per_xcd + (xcd < more ? 1 : 0);
-  int32_t const stride = gridDim.x / kXcds + (xcd < static_cast<int32_t>(gridDim.x % kXcds) ? 1 : 0);  // workgroups of this XCD
+  int32_t const stride = blocks / kXcds + (xcd < blocks % kXcds ? 1 : 0);  // workgroups of this XCD
   auto const place = [&](int32_t item) {
     int32_t const p = uniform(item / tiles), tile = item - p * tiles, group = uniform(tile / (kGroup * tiles_n)), in_group = tile - group * kGroup * tiles_n;
     int32_t const rows_here = tiles_m - group * kGroup < kGroup ? tiles_m - group * kGroup : kGroup;
@@ -304,7 +326,7 @@ __device__ __forceinline__ void tile_product(Side a, Side b, int64_t m, int64_t 
   Loader<B_NEXT, BN, kWaves> load_b;
   Reader<T, A_NEXT, BM> const read_a(wm * MI * 16, lane);
   Reader<T, B_NEXT, BN> const read_b(wn * NI * 16, lane);
-  int32_t const first = begin + static_cast<int32_t>(blockIdx.x / kXcds);
+  int32_t const first = begin + block / kXcds;
   int32_t loaded      = first;  // the item whose stages are loaded
   int64_t left        = 0;      // values of k of it that are still to be loaded
   auto const aim = [&] {
@@ -439,10 +461,25 @@ __device__ __forceinline__ void tile_product(Side a, Side b, int64_t m, int64_t 
 }
 
 template <typename T, bool A_NEXT, bool B_NEXT, int BM, int BN, int WAVES_M, int WAVES_N>
-__global__ void __launch_bounds__(WAVES_M * WAVES_N * kWave, BM * BN / (WAVES_M * WAVES_N) > 8192 ? 1 : 2)
-tile_product_kernel(Side a, Side b, int64_t m, int64_t n, int64_t depth, int32_t parts, int64_t part, float* sums, Epilogue<T> end)
+__global__ void __launch_bounds__(WAVES_M * WAVES_N * kWave, 2) tile_product_kernel(Problem<T> problem)
 {
-  tile_product<T, A_NEXT, B_NEXT, BM, BN, WAVES_M, WAVES_N>(a, b, m, n, depth, parts, part, sums, end);
+  using Tiles = TileProduct<T, A_NEXT, B_NEXT, BM, BN, WAVES_M, WAVES_N>;
+  __shared__ __attribute__((aligned(1024))) char lds[Tiles::kLds];
+  Tiles::run(problem, (LdsBytes)lds, blockIdx.x, gridDim.x);
+}
+
+// The two products of a gradient in one launch: the first `first` workgroups (of which `used` have work) take that of x, the
+// others that of the weights.
+template <typename T>
+__global__ void __launch_bounds__(256, 2) gradient_products_kernel(Problem<T> of_x, Problem<T> of_weight, int32_t first, int32_t used)
+{
+  using Tiles = TileProduct<T, true, false, 128, 128, 2, 2>;
+  __shared__ __attribute__((aligned(1024))) char lds[Tiles::kLds];
+  int32_t const block = static_cast<int32_t>(blockIdx.x);
+  if (block >= first)
+    TileProduct<T, false, false, 128, 128, 2, 2>::run(of_weight, (LdsBytes)lds, block - first, static_cast<int32_t>(gridDim.x) - first);
+  else if (block < used)
+    Tiles::run(of_x, (LdsBytes)lds, block, used);
 }
 
 // ------------------------------------------------------------------ products of few rows
@@ -494,14 +531,20 @@ __global__ void __launch_bounds__(WAVES * kWave) few_rows_kernel(Rows<const T> x
   end.finish(z, typename Epilogue<T>::Columns(end, j0 + j, n), i, j0 + j, n);
 }
 
-// The parts of a product that was cut along k, added up in order.
+// ------------------------------------------------------------------ before and after
+// The parts of a product that was cut along k.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) join_parts_kernel(const float* sums, int64_t parts, int64_t m, int64_t n, Epilogue<T> end)
-{
-  int64_t const blocks = (n + 7) / 8;
-  for (int64_t x = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; x < m * blocks; x += static_cast<int64_t>(gridDim.x) * kThreads) {
-    int64_t const i = x / blocks, j = x % blocks * 8;
+struct Join {
+  const float* sums;
+  int64_t parts, m, n;
+  Epilogue<T> end;
+  __device__ __forceinline__ void run(int64_t block) const
+  {
+    int64_t const blocks = (n + 7) / 8, at = block * kThreads + threadIdx.x;
+    if (at >= m * blocks) return;
+    int64_t const i = at / blocks, j = at % blocks * 8;
     float z[8] = {};
+#pragma unroll 4
     for (int64_t p = 0; p < parts; ++p) {
       float more[8];
       load8(more, sums + (p * m + i) * n + j, n - j);
@@ -510,19 +553,128 @@ __global__ void __launch_bounds__(kThreads) join_parts_kernel(const float* sums,
     }
     end.finish(z, typename Epilogue<T>::Columns(end, j, n), i, j, n);
   }
+};
+
+// The parts of the sums of columns: a workgroup 64 columns, a wavefront a run of parts.
+template <typename T>
+struct JoinColumns {
+  const float* sums;
+  int64_t parts, n;
+  T* out;
+  __device__ __forceinline__ void run(int64_t block) const
+  {
+    constexpr int kWaves = kThreads / kWave;
+    __shared__ float lds[kWaves][kWave];
+    int const wave = threadIdx.x / kWave, lane = lane_id();
+    int64_t const j = block * kWave + lane, each = (parts + kWaves - 1) / kWaves, first = wave * each, last = first + each < parts ? first + each : parts;
+    float sum = 0.f;
+    if (j < n) {
+#pragma unroll 8
+      for (int64_t p = first; p < last; ++p) sum += sums[p * n + j];
+    }
+    lds[wave][lane] = sum;
+    __syncthreads();
+    if (wave != 0 || j >= n) return;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) sum += lds[w][lane];
+    out[j] = static_cast<T>(sum);
+  }
+};
+
+// What is left after the products, in one launch: `first` workgroups, `second` workgroups, and the columns'.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) join_kernel(Join<T> a, int64_t first, Join<T> b, int64_t second, JoinColumns<T> columns)
+{
+  int64_t const block = blockIdx.x;
+  if (block < first)
+    a.run(block);
+  else if (block < first + second)
+    b.run(block - first);
+  else
+    columns.run(block - first - second);
 }
 
 // Lines of `cols` values, aligned anyhow, into lines of a multiple of 8 values, zeros behind the last.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) align_kernel(Rows<const T> in, int64_t rows, int64_t cols, T* out)
-{
-  int64_t const blocks = (cols + 7) / 8;
-  for (int64_t x = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; x < rows * blocks; x += static_cast<int64_t>(gridDim.x) * kThreads) {
-    int64_t const i = x / blocks, j = x % blocks * 8;
+struct Align {
+  Rows<const T> in;
+  int64_t rows, cols;
+  T* out;
+  __device__ __forceinline__ void run(int64_t block) const
+  {
+    int64_t const blocks = (cols + 7) / 8, at = block * kThreads + threadIdx.x;
+    if (at >= rows * blocks) return;
+    int64_t const i = at / blocks, j = at % blocks * 8;
     float f[8];
     load8(f, in.row(i) + j, cols - j);
     store8(out + i * blocks * 8 + j, f, 8);
   }
+};
+
+// d = grad * activation'(z) where it is wanted (d's rows have a multiple of 8 values, zeros behind the last), and the sums of the
+// columns of it: a workgroup takes 512 columns and every count-th run of four rows, a wavefront one of the four, and the
+// wavefronts' sums are added up in the end, to the bias' gradient itself if that is all (count = 1).
+template <typename T>
+struct Slopes {
+  Rows<const T> grad, z;
+  int activation;
+  int64_t rows, cols;
+  Rows<T> d;
+  int64_t count;
+  float* parts;
+  T* bias;
+  __device__ __forceinline__ void run(int64_t block) const
+  {
+    constexpr int kWaves = kThreads / kWave;
+    __shared__ float lds[kWaves][8][kWave];
+    int const wave = threadIdx.x / kWave, lane = lane_id();
+    int64_t const slices = (cols + 8 * kWave - 1) / (8 * kWave), slice = block % slices, number = block / slices;
+    int64_t const j      = (slice * kWave + lane) * 8;
+    float sum[8]         = {};
+    if (j < cols) {
+#pragma unroll 2
+      for (int64_t i = number * kWaves + wave; i < rows; i += count * kWaves) {
+        float g[8], v[8];
+        load8(g, grad.row(i) + j, cols - j);
+        if (z) {
+          load8(v, z.row(i) + j, cols - j);
+          with_activation(activation, [&](auto which) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) g[k] *= slope<decltype(which)::value>(v[k]);
+          });
+        }
+        if (d) store8(d.row(i) + j, g, 8);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum[k] += g[k];
+      }
+    }
+    if (!parts && !bias) return;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) lds[wave][k][lane] = sum[k];
+    __syncthreads();
+    if (wave != 0 || j >= cols) return;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) sum[k] += lds[w][k][lane];
+    if (bias)
+      store8(bias + j, sum, cols - j);
+    else
+      store8(parts + number * cols + j, sum, cols - j);
+  }
+};
+
+// What the products need, in one launch: `first` workgroups, `second` workgroups, and the slopes'.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) prepare_kernel(Align<T> a, int64_t first, Align<T> b, int64_t second, Slopes<T> slopes)
+{
+  int64_t const block = blockIdx.x;
+  if (block < first)
+    a.run(block);
+  else if (block < first + second)
+    b.run(block - first);
+  else
+    slopes.run(block - first - second);
 }
 
 // ------------------------------------------------------------------ products of 32-bit types
@@ -561,76 +713,21 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Operand<float> a, Ope
     if (i0 + ti + i < m) end.finish(sum[i], columns, i0 + ti + i, j0 + tj, n);
 }
 
-// d = grad * activation'(z) where it is wanted, and the sums of the columns of it: a workgroup takes 512 columns and every
-// gridDim.y-th run of four rows, a wavefront one of the four, and the wavefronts' sums are added up in the end.
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-activation_backward_kernel(Rows<const T> grad, Rows<const T> z, int activation, int64_t rows, int64_t cols, Rows<T> d, float* parts)
-{
-  constexpr int kWaves = kThreads / kWave;
-  __shared__ float lds[kWaves][8][kWave];
-  int const wave = threadIdx.x / kWave, lane = lane_id();
-  int64_t const j    = (static_cast<int64_t>(blockIdx.x) * kWave + lane) * 8;
-  int64_t const step = static_cast<int64_t>(gridDim.y) * kWaves;
-  float sum[8]       = {};
-  if (j < cols) {
-#pragma unroll 2
-    for (int64_t i = static_cast<int64_t>(blockIdx.y) * kWaves + wave; i < rows; i += step) {
-      float g[8], v[8];
-      load8(g, grad.row(i) + j, cols - j);
-      if (z) {
-        load8(v, z.row(i) + j, cols - j);
-        with_activation(activation, [&](auto which) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) g[k] *= slope<decltype(which)::value>(v[k]);
-        });
-        if (d) store8(d.row(i) + j, g, cols - j);
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) sum[k] += g[k];
-    }
-  }
-  if (!parts) return;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) lds[wave][k][lane] = sum[k];
-  __syncthreads();
-  if (wave != 0 || j >= cols) return;
-#pragma unroll
-  for (int k = 0; k < 8; ++k)
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) sum[k] += lds[w][k][lane];
-  store8(parts + blockIdx.y * cols + j, sum, cols - j);
-}
-
 // An operand of a product of `extent` rows and `depth` values of k each.
 template <typename T>
 struct Factor {
   Rows<const T> rows;
-  bool k_next;  // value (i, k) in line i, else in line k
+  bool k_next;          // value (i, k) in line i, else in line k
+  bool padded = false;  // lines have a multiple of 8 values, zeros behind the last
+
+  int64_t lines(int64_t extent, int64_t depth) const { return k_next ? extent : depth; }
+  int64_t cols(int64_t extent, int64_t depth) const { return k_next ? depth : extent; }
+  // fits what Side and Loader ask for
+  bool is_aligned(int64_t extent, int64_t depth) const
+  {
+    return reinterpret_cast<uintptr_t>(rows.data) % 16 == 0 && rows.stride % 8 == 0 && (padded || cols(extent, depth) % 8 == 0) && rows.stride <= (1 << 21);
+  }
 };
-
-// Fits what Side and Loader ask for.
-template <typename T>
-bool is_aligned(Factor<T> const& f, int64_t extent, int64_t depth)
-{
-  int64_t const cols = f.k_next ? depth : extent;
-  return reinterpret_cast<uintptr_t>(f.rows.data) % 16 == 0 && f.rows.stride % 8 == 0 && cols % 8 == 0 && f.rows.stride <= (1 << 21);
-}
-
-template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
-void launch_tiles(Side a, bool a_next, Side b, bool b_next, int64_t m, int64_t n, int64_t depth, int32_t parts, int64_t part, float* sums, Epilogue<T> const& end, hipStream_t stream)
-{
-  // as many workgroups as the CUs hold at once
-  int64_t const items = (m + BM - 1) / BM * ((n + BN - 1) / BN) * parts, at_once = (BM == 256 ? 1 : 2) * static_cast<int64_t>(device_cus());
-  dim3 const grid(static_cast<unsigned>(std::min(items, at_once)));
-  dim3 const threads(WAVES_M * WAVES_N * kWave);
-  if (a_next && b_next)
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, true, true, BM, BN, WAVES_M, WAVES_N>), grid, threads, 0, stream, a, b, m, n, depth, parts, part, sums, end);
-  else if (a_next)
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, true, false, BM, BN, WAVES_M, WAVES_N>), grid, threads, 0, stream, a, b, m, n, depth, parts, part, sums, end);
-  else
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, false, false, BM, BN, WAVES_M, WAVES_N>), grid, threads, 0, stream, a, b, m, n, depth, parts, part, sums, end);
-}
 
 // How a product is shared out: tiles of 256 x 256 or of 128 x 128, and so many parts of the values of k.
 struct Plan {
@@ -676,66 +773,194 @@ inline bool few_rows_are_faster(int64_t m, int64_t n, int64_t depth)
   return few < tiles;
 }
 
-// out (m x n) = a (m x depth) * b (n x depth)^T
+inline int64_t blocks_of(int64_t work) { return (work + kThreads - 1) / kThreads; }
+
+// out (m x n) = a (m x depth) * b (n x depth)^T, by tiles: what it takes, and its launch.
 template <typename T>
-nvtext_amd_status launch_product(Factor<T> a, Factor<T> b, int64_t m, int64_t n, int64_t depth, Epilogue<T> const& end, Mr const& mr, hipStream_t stream)
+struct Product {
+  Factor<T> a, b;
+  int64_t m, n, depth;
+  Epilogue<T> end;
+  Plan plan{};
+  bool copy_a = false, copy_b = false;
+  float* sums = nullptr;
+
+  bool wanted() const { return m > 0 && n > 0; }
+  bool fits() const { return (m + 127) / 128 * ((n + 127) / 128) <= INT32_MAX / 64; }
+  void make_plan()
+  {
+    plan   = plan_product(m, n, depth);
+    copy_a = depth > 0 && !a.is_aligned(m, depth);
+    copy_b = depth > 0 && !b.is_aligned(n, depth);
+  }
+  static size_t copy_bytes(Factor<T> const& f, int64_t extent, int64_t depth)
+  {
+    return static_cast<size_t>(f.lines(extent, depth)) * static_cast<size_t>((f.cols(extent, depth) + 7) / 8 * 8) * sizeof(T);
+  }
+  size_t bytes_a() const { return copy_a ? copy_bytes(a, m, depth) : 0; }
+  size_t bytes_b() const { return copy_b ? copy_bytes(b, n, depth) : 0; }
+  size_t bytes_sums() const { return plan.parts > 1 ? static_cast<size_t>(plan.parts) * static_cast<size_t>(m * n) * sizeof(float) : 0; }
+  static Align<T> align(Factor<T>& f, int64_t extent, int64_t depth, T* to)
+  {
+    Align<T> const copy{f.rows, f.lines(extent, depth), f.cols(extent, depth), to};
+    f.rows   = Rows<const T>{to, (copy.cols + 7) / 8 * 8};
+    f.padded = true;
+    return copy;
+  }
+  Problem<T> problem() const { return Problem<T>{{a.rows.data, a.rows.stride}, {b.rows.data, b.rows.stride}, m, n, depth, plan.part, plan.parts, sums, end}; }
+  // workgroups: as many as the CUs hold at once
+  int64_t workgroups() const
+  {
+    int64_t const edge = plan.large ? 256 : 128, items = (m + edge - 1) / edge * ((n + edge - 1) / edge) * plan.parts;
+    return std::min<int64_t>(items, (plan.large ? 1 : 2) * static_cast<int64_t>(device_cus()));
+  }
+  template <int BM, int BN, int WAVES_M, int WAVES_N>
+  void launch_as(hipStream_t stream) const
+  {
+    dim3 const grid(static_cast<unsigned>(workgroups())), threads(WAVES_M * WAVES_N * kWave);
+    if (a.k_next && b.k_next)
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, true, true, BM, BN, WAVES_M, WAVES_N>), grid, threads, 0, stream, problem());
+    else if (a.k_next)
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, true, false, BM, BN, WAVES_M, WAVES_N>), grid, threads, 0, stream, problem());
+    else
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, false, false, BM, BN, WAVES_M, WAVES_N>), grid, threads, 0, stream, problem());
+  }
+  void launch(hipStream_t stream) const
+  {
+    if (plan.large)
+      launch_as<256, 256, 2, 4>(stream);
+    else
+      launch_as<128, 128, 2, 2>(stream);
+  }
+  Join<T> join() const { return Join<T>{sums, plan.parts, m, n, end}; }
+  int64_t join_blocks() const { return wanted() && sums ? blocks_of(m * ((n + 7) / 8)) : 0; }
+};
+
+void launch_product(Factor<float> const& a, Factor<float> const& b, int64_t m, int64_t n, int64_t depth, Epilogue<float> const& end, hipStream_t stream)
+{
+  auto const operand = [](Factor<float> const& f) { return Operand<float>{f.rows.data, f.k_next ? f.rows.stride : 1, f.k_next ? 1 : f.rows.stride}; };
+  hipLaunchKernelGGL(product_kernel, dim3(static_cast<unsigned>((n + kTile - 1) / kTile * ((m + kTile - 1) / kTile))), dim3(kThreads), 0, stream, operand(a), operand(b), m, n, depth, end);
+}
+
+template <typename T>
+void launch_few_rows(Rows<const T> x, Rows<const T> weight, int64_t m, int64_t n, int64_t depth, Epilogue<T> const& end, hipStream_t stream)
+{
+  using std::integral_constant;
+  auto const launch = [&](auto rows_of_16, auto waves) {
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, decltype(rows_of_16)::value, decltype(waves)::value>), dim3(static_cast<unsigned>((n + 15) / 16)),
+                       dim3(decltype(waves)::value * kWave), 0, stream, x, weight, m, n, depth, end);
+  };
+  // enough wavefronts that each has about one round of loads
+  auto const by_depth = [&](auto rows_of_16, auto most) {
+    if (depth >= 2048)
+      launch(rows_of_16, most);
+    else
+      launch(rows_of_16, integral_constant<int, 4>{});
+  };
+  if (m <= 16)
+    by_depth(integral_constant<int, 1>{}, integral_constant<int, 16>{});
+  else if (m <= 32)
+    by_depth(integral_constant<int, 2>{}, integral_constant<int, 8>{});
+  else
+    by_depth(integral_constant<int, 4>{}, integral_constant<int, 8>{});
+}
+
+template <typename T>
+nvtext_amd_status linear(Rows<const T> x, Rows<const T> weight, int64_t m, int64_t n, int64_t depth, Epilogue<T> const& end, Mr const& mr, hipStream_t stream)
 {
   if constexpr (sizeof(T) == 4) {
-    auto const operand = [](Factor<T> const& f) { return Operand<T>{f.rows.data, f.k_next ? f.rows.stride : 1, f.k_next ? 1 : f.rows.stride}; };
-    hipLaunchKernelGGL(product_kernel, dim3(static_cast<unsigned>((n + kTile - 1) / kTile * ((m + kTile - 1) / kTile))), dim3(kThreads), 0, stream, operand(a), operand(b), m, n, depth,
-                       end);
-    return NVTEXT_AMD_SUCCESS;
+    launch_product({x, true}, {weight, true}, m, n, depth, end, stream);
   } else {
-    if (a.k_next && b.k_next && few_rows_are_faster(m, n, depth)) {
-      // enough wavefronts that each has about one round of loads
-      auto const launch = [&](auto rows_of_16, auto waves) {
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, decltype(rows_of_16)::value, decltype(waves)::value>), dim3(static_cast<unsigned>((n + 15) / 16)),
-                           dim3(decltype(waves)::value * kWave), 0, stream, a.rows, b.rows, m, n, depth, end);
-      };
-      auto const by_depth = [&](auto rows_of_16, auto most) {
-        if (depth >= 2048)
-          launch(rows_of_16, most);
-        else
-          launch(rows_of_16, std::integral_constant<int, 4>{});
-      };
-      using std::integral_constant;
-      if (m <= 16)
-        by_depth(integral_constant<int, 1>{}, integral_constant<int, 16>{});
-      else if (m <= 32)
-        by_depth(integral_constant<int, 2>{}, integral_constant<int, 8>{});
-      else
-        by_depth(integral_constant<int, 4>{}, integral_constant<int, 8>{});
+    if (few_rows_are_faster(m, n, depth)) {
+      launch_few_rows(x, weight, m, n, depth, end, stream);
       return NVTEXT_AMD_SUCCESS;
     }
-    bool const copy_a = depth > 0 && !is_aligned(a, m, depth), copy_b = depth > 0 && !is_aligned(b, n, depth);
-    auto const lines  = [&](Factor<T> const& f, int64_t extent) { return f.k_next ? extent : depth; };
-    auto const width  = [&](Factor<T> const& f, int64_t extent) { return ((f.k_next ? depth : extent) + 7) / 8 * 8; };
-    Plan const plan   = plan_product(m, n, depth);
-    if ((m + 127) / 128 * ((n + 127) / 128) > INT32_MAX / 32) return fail(NVTEXT_AMD_OVERFLOW, "the product is too large");
-    TempParts<3> const temp(mr,
-                            {copy_a ? static_cast<size_t>(lines(a, m) * width(a, m)) * sizeof(T) : 0, copy_b ? static_cast<size_t>(lines(b, n) * width(b, n)) * sizeof(T) : 0,
-                             plan.parts > 1 ? static_cast<size_t>(plan.parts * m * n) * sizeof(float) : 0},
-                            copy_a || copy_b || plan.parts > 1);
+    Product<T> p{{x, true}, {weight, true}, m, n, depth, end};
+    if (!p.fits()) return fail(NVTEXT_AMD_OVERFLOW, "the product is too large");
+    p.make_plan();
+    TempParts<3> const temp(mr, {p.bytes_a(), p.bytes_b(), p.bytes_sums()}, p.bytes_a() + p.bytes_b() + p.bytes_sums() > 0);
     if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
-    auto const align = [&](Factor<T>& f, int64_t extent, T* to) {
-      int64_t const work = lines(f, extent) * width(f, extent) / 8;
-      hipLaunchKernelGGL(align_kernel<T>, dim3(static_cast<unsigned>(std::min<int64_t>((work + kThreads - 1) / kThreads, 16 * device_cus()))), dim3(kThreads), 0, stream, f.rows,
-                         lines(f, extent), f.k_next ? depth : extent, to);
-      f.rows = Rows<const T>{to, width(f, extent)};
-    };
-    if (copy_a) align(a, m, temp.template part<T>(0));
-    if (copy_b) align(b, n, temp.template part<T>(1));
-    float* const sums = plan.parts > 1 ? temp.template part<float>(2) : nullptr;
-    Side const sa{a.rows.data, a.rows.stride}, sb{b.rows.data, b.rows.stride};
-    if (plan.large)
-      launch_tiles<T, 256, 256, 2, 4>(sa, a.k_next, sb, b.k_next, m, n, depth, plan.parts, plan.part, sums, end, stream);
-    else
-      launch_tiles<T, 128, 128, 2, 2>(sa, a.k_next, sb, b.k_next, m, n, depth, plan.parts, plan.part, sums, end, stream);
-    if (sums)
-      hipLaunchKernelGGL(join_parts_kernel<T>, dim3(static_cast<unsigned>(std::min<int64_t>((m * ((n + 7) / 8) + kThreads - 1) / kThreads, 32 * device_cus()))), dim3(kThreads), 0, stream,
-                         sums, plan.parts, m, n, end);
-    return NVTEXT_AMD_SUCCESS;
+    Align<T> a{}, b{};
+    if (p.copy_a) a = p.align(p.a, m, depth, temp.template part<T>(0));
+    if (p.copy_b) b = p.align(p.b, n, depth, temp.template part<T>(1));
+    int64_t const first = blocks_of(a.rows * ((a.cols + 7) / 8)), second = blocks_of(b.rows * ((b.cols + 7) / 8));
+    if (first + second > 0) hipLaunchKernelGGL(prepare_kernel<T>, dim3(static_cast<unsigned>(first + second)), dim3(kThreads), 0, stream, a, first, b, second, Slopes<T>{});
+    if (p.plan.parts > 1) p.sums = temp.template part<float>(2);
+    p.launch(stream);
+    if (p.sums) hipLaunchKernelGGL(join_kernel<T>, dim3(static_cast<unsigned>(p.join_blocks())), dim3(kThreads), 0, stream, p.join(), p.join_blocks(), Join<T>{}, 0, JoinColumns<T>{});
   }
+  return NVTEXT_AMD_SUCCESS;
+}
+
+// The gradients that are wanted (of those of x and the weights, whose `out` has data).
+template <typename T>
+nvtext_amd_status linear_backward(Rows<const T> grad, Rows<const T> x, Rows<const T> weight, int64_t m, int64_t n, int64_t depth, int activation, Rows<const T> z, Rows<T> x_grad,
+                                  Rows<T> weight_grad, T* bias_grad, Mr const& mr, hipStream_t stream)
+{
+  auto const plain = [](Rows<T> out) { return Epilogue<T>{{nullptr, 0}, {nullptr, 0}, out, {nullptr, 0}, NVTEXT_AMD_ACTIVATION_NONE}; };
+  bool const slopes = activation != NVTEXT_AMD_ACTIVATION_NONE, large = sizeof(T) == 4;
+  // x_grad (m x depth) = d * weight, weight_grad (n x depth) = d^T * x
+  Product<T> of_x{{grad, true}, {weight, false}, x_grad ? m : 0, depth, n, plain(x_grad)}, of_weight{{grad, false}, {x, false}, weight_grad ? n : 0, depth, m, plain(weight_grad)};
+  if (!of_x.fits() || !of_weight.fits()) return fail(NVTEXT_AMD_OVERFLOW, "the product is too large");
+  if (!large) {
+    of_x.make_plan();
+    of_weight.make_plan();
+  }
+  // d is written where grad is not what the products can read
+  bool const write_d     = m > 0 && n > 0 && (slopes || (of_x.wanted() && of_x.copy_a) || (of_weight.wanted() && of_weight.copy_a));
+  int64_t const d_stride = (n + 7) / 8 * 8;
+  // few rows: one workgroup adds up a column's, without parts
+  int64_t const count    = m <= 64 ? 1 : std::min<int64_t>((m + 15) / 16, 256);
+  bool const sums        = bias_grad && count > 1;
+  TempParts<6> const temp(mr, {write_d ? static_cast<size_t>(m) * static_cast<size_t>(d_stride) * sizeof(T) : 0, sums ? static_cast<size_t>(count * n) * sizeof(float) : 0,
+                               of_x.wanted() ? of_x.bytes_b() : 0, of_weight.wanted() ? of_weight.bytes_b() : 0, of_x.wanted() ? of_x.bytes_sums() : 0,
+                               of_weight.wanted() ? of_weight.bytes_sums() : 0});
+  if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
+  Rows<T> const d = write_d ? Rows<T>{temp.template part<T>(0), d_stride} : Rows<T>{nullptr, 0};
+  if (write_d) {
+    of_x.a      = Factor<T>{{d.data, d.stride}, true, true};
+    of_weight.a = Factor<T>{{d.data, d.stride}, false, true};
+  }
+  Align<T> a{}, b{};
+  if (of_x.wanted() && of_x.copy_b) a = of_x.align(of_x.b, depth, n, temp.template part<T>(2));
+  if (of_weight.wanted() && of_weight.copy_b) b = of_weight.align(of_weight.b, depth, m, temp.template part<T>(3));
+  Slopes<T> const act{grad, slopes ? z : Rows<const T>{nullptr, 0}, activation, m, n, d, count, sums ? temp.template part<float>(1) : nullptr, sums ? nullptr : bias_grad};
+  int64_t const first = blocks_of(a.rows * ((a.cols + 7) / 8)), second = blocks_of(b.rows * ((b.cols + 7) / 8));
+  int64_t const third = write_d || bias_grad ? (n + 8 * kWave - 1) / (8 * kWave) * count : 0;
+  if (first + second + third > 0) {
+    ProfileScope const scope("linear_prepare_backward", stream);
+    hipLaunchKernelGGL(prepare_kernel<T>, dim3(static_cast<unsigned>(first + second + third)), dim3(kThreads), 0, stream, a, first, b, second, act);
+  }
+  if constexpr (sizeof(T) == 4) {
+    ProfileScope const scope("linear_products_backward", stream);
+    if (of_x.wanted() && depth > 0) launch_product(of_x.a, of_x.b, m, depth, n, of_x.end, stream);
+    if (of_weight.wanted() && depth > 0) launch_product(of_weight.a, of_weight.b, n, depth, m, of_weight.end, stream);
+  } else {
+    if (of_x.bytes_sums()) of_x.sums = temp.template part<float>(4);
+    if (of_weight.bytes_sums()) of_weight.sums = temp.template part<float>(5);
+    if (of_x.wanted() && of_weight.wanted() && !of_x.plan.large && !of_weight.plan.large) {
+      ProfileScope const scope("linear_products_backward", stream);
+      int64_t const used = of_x.workgroups(), from = (used + 7) / 8 * 8;  // (workgroups go to the eight XCDs in turn)
+      hipLaunchKernelGGL(gradient_products_kernel<T>, dim3(static_cast<unsigned>(from + of_weight.workgroups())), dim3(256), 0, stream, of_x.problem(), of_weight.problem(),
+                         static_cast<int32_t>(from), static_cast<int32_t>(used));
+    } else {
+      if (of_x.wanted()) {
+        ProfileScope const scope("linear_x_backward", stream);
+        of_x.launch(stream);
+      }
+      if (of_weight.wanted()) {
+        ProfileScope const scope("linear_weight_backward", stream);
+        of_weight.launch(stream);
+      }
+    }
+  }
+  int64_t const join_x = of_x.join_blocks(), join_weight = of_weight.join_blocks(), join_columns = sums ? (n + kWave - 1) / kWave : 0;
+  if (join_x + join_weight + join_columns > 0) {
+    ProfileScope const scope("linear_join_backward", stream);
+    hipLaunchKernelGGL(join_kernel<T>, dim3(static_cast<unsigned>(join_x + join_weight + join_columns)), dim3(kThreads), 0, stream, of_x.join(), join_x, of_weight.join(), join_weight,
+                       JoinColumns<T>{act.parts, count, n, bias_grad});
+  }
+  return NVTEXT_AMD_SUCCESS;
 }
 
 bool is_activation(int32_t a) { return a >= NVTEXT_AMD_ACTIVATION_NONE && a <= NVTEXT_AMD_ACTIVATION_SILU; }
@@ -776,10 +1001,9 @@ nvtext_amd_status nvtext_amd_linear(const nvtext_amd_matrix* x, const nvtext_amd
   nvtext_amd_status st = NVTEXT_AMD_SUCCESS;
   with_type(x->type, [&](auto zero) {
     using T       = decltype(zero);
-    auto const xs = rows_of<const T>(x), ws = rows_of<const T>(weight);
     ProfileScope const scope("linear", stream);
-    st = launch_product<T>({xs, true}, {ws, true}, m, n, depth, {rows_of<const T>(bias), rows_of<const T>(residual), rows_of<T>(out), rows_of<T>(preactivation), activation}, mr,
-                           stream);
+    st = linear<T>(rows_of<const T>(x), rows_of<const T>(weight), m, n, depth, {rows_of<const T>(bias), rows_of<const T>(residual), rows_of<T>(out), rows_of<T>(preactivation), activation},
+                   mr, stream);
   });
   if (st != NVTEXT_AMD_SUCCESS) return st;
   NVTEXT_HIP_TRY(hipGetLastError());
@@ -808,32 +1032,11 @@ nvtext_amd_status nvtext_amd_linear_backward(const nvtext_amd_matrix* grad, cons
   if (activation != NVTEXT_AMD_ACTIVATION_NONE && !preactivation) return fail(NVTEXT_AMD_INVALID_ARGUMENT, "the gradient of an activation needs what it was applied to");
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   Mr const mr{mr_, stream};
-  bool const slopes   = activation != NVTEXT_AMD_ACTIVATION_NONE;
-  int64_t const parts = std::max<int64_t>(1, std::min<int64_t>((m + 15) / 16, 256));
-  TempParts<2> const temp(mr, {slopes ? static_cast<size_t>(m * n) * type_bytes(x->type) : 0, bias_grad ? static_cast<size_t>(parts * n) * sizeof(float) : 0});
-  if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
   nvtext_amd_status st = NVTEXT_AMD_SUCCESS;
   with_type(x->type, [&](auto zero) {
-    using T       = decltype(zero);
-    auto const xs = rows_of<const T>(x), ws = rows_of<const T>(weight), gs = rows_of<const T>(grad);
-    Rows<T> const d = slopes ? Rows<T>{temp.part<T>(0), n} : Rows<T>{nullptr, 0};
-    float* const sums = bias_grad ? temp.part<float>(1) : nullptr;
-    if (n > 0 && (slopes || bias_grad)) {
-      ProfileScope const scope("linear_activation_backward", stream);
-      hipLaunchKernelGGL(activation_backward_kernel<T>, dim3(static_cast<unsigned>((n + 8 * kWave - 1) / (8 * kWave)), static_cast<unsigned>(parts)), dim3(kThreads), 0, stream, gs,
-                         slopes ? rows_of<const T>(preactivation) : Rows<const T>{nullptr, 0}, activation, m, n, d, sums);
-      if (bias_grad) launch_add_parts<T>(sums, parts, n, static_cast<T*>(bias_grad->data), nullptr, stream);
-    }
-    Rows<const T> const ds = slopes ? Rows<const T>{d.data, d.stride} : gs;
-    auto const plain = [](const nvtext_amd_matrix* o) { return Epilogue<T>{{nullptr, 0}, {nullptr, 0}, rows_of<T>(o), {nullptr, 0}, NVTEXT_AMD_ACTIVATION_NONE}; };
-    if (x_grad && m > 0 && depth > 0) {
-      ProfileScope const scope("linear_x_backward", stream);
-      st = launch_product<T>({ds, true}, {ws, false}, m, depth, n, plain(x_grad), mr, stream);
-    }
-    if (st == NVTEXT_AMD_SUCCESS && weight_grad && n > 0 && depth > 0) {
-      ProfileScope const scope("linear_weight_backward", stream);
-      st = launch_product<T>({ds, false}, {xs, false}, n, depth, m, plain(weight_grad), mr, stream);
-    }
+    using T = decltype(zero);
+    st      = linear_backward<T>(rows_of<const T>(grad), rows_of<const T>(x), rows_of<const T>(weight), m, n, depth, activation, rows_of<const T>(preactivation), rows_of<T>(x_grad),
+                            rows_of<T>(weight_grad), bias_grad ? static_cast<T*>(bias_grad->data) : nullptr, mr, stream);
   });
   if (st != NVTEXT_AMD_SUCCESS) return st;
   NVTEXT_HIP_TRY(hipGetLastError());
