@@ -532,7 +532,8 @@ __global__ void __launch_bounds__(WAVES * kWave) few_rows_kernel(Rows<const T> x
 }
 
 // ------------------------------------------------------------------ before and after
-// The parts of a product that was cut along k.
+// The parts of a product that was cut along k: a workgroup 64 times eight values, a wavefront a run of parts, eight of them asked for
+// at a time.
 template <typename T>
 struct Join {
   const float* sums;
@@ -540,17 +541,31 @@ struct Join {
   Epilogue<T> end;
   __device__ __forceinline__ void run(int64_t block) const
   {
-    int64_t const blocks = (n + 7) / 8, at = block * kThreads + threadIdx.x;
-    if (at >= m * blocks) return;
+    constexpr int kWaves = kThreads / kWave;
+    __shared__ float lds[kWaves][8][kWave];
+    int const wave = threadIdx.x / kWave, lane = lane_id();
+    int64_t const blocks = (n + 7) / 8, at = block * kWave + lane;
     int64_t const i = at / blocks, j = at % blocks * 8;
+    bool const here = at < m * blocks;
+    int64_t const each = (parts + kWaves - 1) / kWaves, first = wave * each, last = first + each < parts ? first + each : parts;
     float z[8] = {};
-#pragma unroll 4
-    for (int64_t p = 0; p < parts; ++p) {
-      float more[8];
-      load8(more, sums + (p * m + i) * n + j, n - j);
+    if (here) {
+#pragma unroll 8
+      for (int64_t p = first; p < last; ++p) {
+        float more[8];
+        load8(more, sums + (p * m + i) * n + j, n - j);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) z[k] += more[k];
+        for (int k = 0; k < 8; ++k) z[k] += more[k];
+      }
     }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) lds[wave][k][lane] = z[k];
+    __syncthreads();
+    if (wave != 0 || !here) return;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) z[k] += lds[w][k][lane];
     end.finish(z, typename Epilogue<T>::Columns(end, j, n), i, j, n);
   }
 };
@@ -632,7 +647,7 @@ struct Slopes {
     int64_t const j      = (slice * kWave + lane) * 8;
     float sum[8]         = {};
     if (j < cols) {
-#pragma unroll 2
+#pragma unroll 4
       for (int64_t i = number * kWaves + wave; i < rows; i += count * kWaves) {
         float g[8], v[8];
         load8(g, grad.row(i) + j, cols - j);
@@ -736,8 +751,10 @@ struct Plan {
   int64_t part;  // values of k a part
 };
 
-// The one that takes the least by this measure, in microseconds: CUs go through their workgroups in rounds, and parts are written and
-// read once more.
+// The one that takes the least by this measure, in microseconds, fitted to products of 256 x 256 to 4096 x 4096 with 64 to 4096
+// values of k: a launch, then rounds of workgroups, each with so much for a stage of 64 values of k (more where all CUs are busy) and
+// for writing its tile; parts are written and read once more.  (4096 x 4096 x 64: 13.6 us in large tiles, 15.1 in small ones;
+// x 4096: 111 and 131.  2048 x 2048 x 4096: 80 and 49; 128 x 4096 x 4096: 77 and 43 in one part, 31 and 21 in four.)
 inline Plan plan_product(int64_t m, int64_t n, int64_t depth)
 {
   int64_t const cus = device_cus(), steps = std::max<int64_t>(1, (depth + kStageK - 1) / kStageK);
@@ -748,9 +765,10 @@ inline Plan plan_product(int64_t m, int64_t n, int64_t depth)
     for (int64_t parts = 1; parts <= std::min<int64_t>(steps, 32); ++parts) {
       int64_t const each = (steps + parts - 1) / parts, really = (steps + each - 1) / each;
       if (really != parts) continue;
-      int64_t const load = (tiles * parts + cus - 1) / cus;  // workgroups a CU
-      double const rounds = large ? load * (each * 1.7 + 5) : (load == 1 ? each * 0.8 + 4 : load * (each * 0.6 + 3));
-      double const time   = rounds + (parts > 1 ? 5 + parts * m * n * 8e-6 / 5 : 0);
+      int64_t const groups = tiles * parts, load = (groups + cus - 1) / cus;  // workgroups, and of them a CU
+      double const busy    = std::min(1.0, static_cast<double>(groups) / cus);
+      double const work    = large ? 6 + load * (each * (1.05 + 0.45 * busy) + 5) : load == 1 ? 6 + each * (0.4 + 0.25 * busy) : 4 + (load + 1) / 2 * (each * 0.92 + 5);
+      double const time    = work + (parts > 1 ? 3 + parts * m * n * 8e-6 / 5 : 0);
       if (time < least) {
         least = time;
         best  = Plan{large, static_cast<int32_t>(parts), each * kStageK};
@@ -833,7 +851,7 @@ struct Product {
       launch_as<128, 128, 2, 2>(stream);
   }
   Join<T> join() const { return Join<T>{sums, plan.parts, m, n, end}; }
-  int64_t join_blocks() const { return wanted() && sums ? blocks_of(m * ((n + 7) / 8)) : 0; }
+  int64_t join_blocks() const { return wanted() && sums ? (m * ((n + 7) / 8) + kWave - 1) / kWave : 0; }
 };
 
 void launch_product(Factor<float> const& a, Factor<float> const& b, int64_t m, int64_t n, int64_t depth, Epilogue<float> const& end, hipStream_t stream)
