@@ -87,14 +87,27 @@ __device__ __forceinline__ void store8(T* p, float const (&f)[8], int64_t n)
       __builtin_nontemporal_store(v, reinterpret_cast<typename Eight<T>::type*>(p));
     else
       *reinterpret_cast<typename Eight<T>::type*>(p) = v;
-  } else {
+  } else if (n > 0) {
+    // four, two and one of them
+    typedef T V4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    typedef T V2 __attribute__((ext_vector_type(2), aligned(sizeof(T))));
+    T v[4] = {static_cast<T>(f[0]), static_cast<T>(f[1]), static_cast<T>(f[2]), static_cast<T>(f[3])};
+    if (n & 4) {
+      *reinterpret_cast<V4*>(p) = V4{v[0], v[1], v[2], v[3]};
+      p += 4;
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < n) p[k] = static_cast<T>(f[k]);
+      for (int k = 0; k < 3; ++k) v[k] = static_cast<T>(f[4 + k]);
+    }
+    if (n & 2) {
+      *reinterpret_cast<V2*>(p) = V2{v[0], v[1]};
+      p += 2;
+      v[0] = v[2];
+    }
+    if (n & 1) *p = v[0];
   }
 }
 
-// The same in two steps, so that several loads are on their way before the first is waited for.
+// values p[0 .. n) as they are, zeros from n on
 template <typename T>
 __device__ __forceinline__ typename Eight<T>::type load_raw8(const T* p, int64_t n)
 {
@@ -107,6 +120,41 @@ __device__ __forceinline__ typename Eight<T>::type load_raw8(const T* p, int64_t
       if (k < n) v[k] = p[k];
   }
   return v;
+}
+
+// Values j .. j + 7 of a row of `cols`, in two steps, so that several loads are on their way before the first is waited for, and
+// without a condition on any of them: a lane behind the last eight values loads these, and the second step moves its own to the
+// front and puts zeros behind them.  (Loaded one by one under conditions, what was left of rows of 1023 values doubled the time of
+// a layer norm.)
+template <typename T>
+__device__ __forceinline__ typename Eight<T>::type load_row8(const T* row, int64_t j, int64_t cols)
+{
+  if (cols >= 8) return *reinterpret_cast<const typename Eight<T>::type*>(row + (j + 8 <= cols ? j : cols - 8));
+  return load_raw8<T>(row + j, cols - j);
+}
+
+template <typename T>
+__device__ __forceinline__ void settle_row8(typename Eight<T>::type& v, int64_t j, int64_t cols)
+{
+  if (cols < 8) return;
+  constexpr int kWords = 8 * sizeof(T) / 4, kEach = 4 / sizeof(T);  // 32-bit words, and values in one
+  typedef uint32_t W __attribute__((ext_vector_type(kWords)));
+  W w             = __builtin_bit_cast(W, v);
+  int const ahead = j + 8 > cols ? static_cast<int>(j + 8 - cols) : 0;
+  if (cols % 8 != 0) {  // (the same for all lanes: no width is left to a branch of single lanes)
+    if constexpr (kEach == 2) {
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) w[k] = ahead & 1 ? __builtin_amdgcn_alignbit(k + 1 < kWords ? w[k + 1] : 0u, w[k], 16) : w[k];
+    }
+#pragma unroll
+    for (int by = 1; by < kWords; by *= 2) {
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) w[k] = !(ahead & by * kEach) ? w[k] : k + by < kWords ? w[k + by] : 0u;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kWords; ++k) w[k] = ahead >= 8 ? 0u : w[k];
+  v = __builtin_bit_cast(typename Eight<T>::type, w);
 }
 
 template <typename T>
