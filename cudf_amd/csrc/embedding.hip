@@ -35,7 +35,8 @@ struct Tokens {
 // A wavefront takes `each` consecutive tokens: a lane finds the place of one of them in its row, all at once (a search for each token
 // on its own, a dozen reads one after the other, took 555 us of what is 294 now), then the rows of the tables are added up, kAtOnce
 // tokens asked for at a time.  VEC = 8 columns a lane; the lanes behind the last column take the last eight once more.  (VEC = 1 for
-// less than eight columns.)  Bound by memory: 512,011 tokens of 1024 16-bit values move 1.18 GB in 294 us, 4.0 TB/s, where a copy
+// less than eight columns.)  Rows of up to 256 columns lie side by side in a wavefront, LANES lanes each: 1,276,351 tokens of 64
+// columns took 185 us with one.  Bound by memory: 512,011 tokens of 1024 16-bit values move 1.18 GB in 294 us, 4.0 TB/s, where a copy
 // reaches 5; rows of the table that occur again come from the caches, and the results are stored past them (372 us without that).
 // With 8, 32 or 64 tokens a wavefront 308, 308 and 315 us, with 4 at a time 307.
 constexpr int kAtOnce = 8, kMostEach = 16;
@@ -53,12 +54,13 @@ __device__ __forceinline__ some_t<T, VEC> load_some(const T* p)
   return *reinterpret_cast<const some_t<T, VEC>*>(p);
 }
 
-template <int VEC, typename T>
+template <int VEC, int LANES, typename T>
 __global__ void __launch_bounds__(kThreads)
 embedding_kernel(Tokens tokens, Rows<const T> table, int64_t vocabulary, Rows<const T> positions, int64_t places, int64_t cols, int32_t each, Rows<T> out)
 {
-  int const lane      = lane_id();
-  int64_t const first = (static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / kWave) * each;
+  constexpr int kAcross = kWave / LANES;  // tokens side by side
+  int const lane        = lane_id(), beside = lane / LANES;
+  int64_t const first   = (static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / kWave) * each;
   if (first >= tokens.count) return;
   int const count = static_cast<int>(tokens.count - first < each ? tokens.count - first : each);
   int32_t id = -1, at = -1;  // (-1: nothing)
@@ -68,25 +70,33 @@ embedding_kernel(Tokens tokens, Rows<const T> table, int64_t vocabulary, Rows<co
     id                  = place >= 0 && id < vocabulary ? id : -1;
     at                  = place < places ? static_cast<int32_t>(place) : -1;
   }
-  for (int64_t slice = 0; slice < cols; slice += VEC * kWave) {
-    int64_t const j = slice + lane * VEC + VEC <= cols ? slice + lane * VEC : cols - VEC;
-    for (int base = 0; base < count; base += kAtOnce) {
+  for (int64_t slice = 0; slice < cols; slice += VEC * LANES) {
+    int64_t const j = slice + lane % LANES * VEC + VEC <= cols ? slice + lane % LANES * VEC : cols - VEC;
+    for (int base = 0; base < count; base += kAtOnce * kAcross) {
       some_t<T, VEC> e[kAtOnce], p[kAtOnce];
 #pragma unroll
       for (int u = 0; u < kAtOnce; ++u) {
-        int const from = base + u < count ? base + u : base;  // (behind the last: the first once more, not written)
-        int32_t const row = static_cast<int32_t>(wave_bcast(id, from)), place = static_cast<int32_t>(wave_bcast(at, from));
+        int const from = base + u * kAcross + beside;  // (behind the last there is nothing, or it is one before, not written)
+        int32_t row, place;
+        if constexpr (kAcross == 1) {
+          row   = static_cast<int32_t>(wave_bcast(id, from % kWave));
+          place = static_cast<int32_t>(wave_bcast(at, from % kWave));
+        } else {
+          row   = __shfl(id, from % kWave);
+          place = __shfl(at, from % kWave);
+        }
         e[u] = p[u] = some_t<T, VEC>{};
         if (row >= 0) e[u] = load_some<VEC>(table.row(row) + j);
         if (place >= 0) p[u] = load_some<VEC>(positions.row(place) + j);
       }
 #pragma unroll
       for (int u = 0; u < kAtOnce; ++u) {
-        if (base + u < count) {
+        int const from = base + u * kAcross + beside;
+        if (from < count) {
           some_t<T, VEC> sum;
 #pragma unroll
           for (int k = 0; k < VEC; ++k) sum[k] = static_cast<T>(static_cast<float>(e[u][k]) + static_cast<float>(p[u][k]));
-          __builtin_nontemporal_store(sum, reinterpret_cast<some_t<T, VEC>*>(out.row(first + base + u) + j));
+          __builtin_nontemporal_store(sum, reinterpret_cast<some_t<T, VEC>*>(out.row(first + from) + j));
         }
       }
     }
@@ -603,17 +613,24 @@ nvtext_amd_status nvtext_amd_embedding(const nvtext_amd_list_column* tokens, con
   with_type(out->type, [&](auto zero) {
     using T = decltype(zero);
     ProfileScope const scope("embedding", stream);
-    // as many tokens a wavefront as leave every SIMD four wavefronts
-    int64_t const each = std::max<int64_t>(1, std::min<int64_t>(kMostEach, out->rows / (16 * device_cus())));
-    dim3 const grid(static_cast<unsigned>(((out->rows + each - 1) / each + kWaves - 1) / kWaves)), threads(kThreads);
-    auto const launch = [&](auto kernel) {
+    auto const launch = [&](auto kernel, int lanes) {
+      // as many tokens a wavefront as leave every SIMD four wavefronts, and those that are side by side
+      int64_t const across = kWave / lanes, most = std::min<int64_t>(kMostEach * across, kWave);
+      int64_t const each   = std::max<int64_t>(across, std::min<int64_t>(most, out->rows / (16 * device_cus())));
+      dim3 const grid(static_cast<unsigned>(((out->rows + each - 1) / each + kWaves - 1) / kWaves)), threads(kThreads);
       hipLaunchKernelGGL(kernel, grid, threads, 0, stream, view_of(tokens), rows_of<const T>(token_table), token_table->rows, rows_of<const T>(position_table),
                          position_table ? std::min<int64_t>(position_table->rows, INT32_MAX) : 0, out->cols, static_cast<int32_t>(each), rows_of<T>(out));
     };
-    if (out->cols >= 8)
-      launch(embedding_kernel<8, T>);
+    if (out->cols < 8)
+      launch(embedding_kernel<1, 8, T>, 8);
+    else if (out->cols <= 64)
+      launch(embedding_kernel<8, 8, T>, 8);
+    else if (out->cols <= 128)
+      launch(embedding_kernel<8, 16, T>, 16);
+    else if (out->cols <= 256)
+      launch(embedding_kernel<8, 32, T>, 32);
     else
-      launch(embedding_kernel<1, T>);
+      launch(embedding_kernel<8, kWave, T>, kWave);
   });
   NVTEXT_HIP_TRY(hipGetLastError());
   return NVTEXT_AMD_SUCCESS;
