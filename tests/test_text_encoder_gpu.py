@@ -1,5 +1,8 @@
 """The encoder's operators together: the example's model against the formulas in 64 bits, its training, on another stream, and
 captured in a graph."""
+import os
+import subprocess
+
 import numpy as np
 import pytest
 
@@ -133,3 +136,10 @@ def test_one_text_alone_is_as_among_others(data):
         begin = int(tokens.offsets.view(torch.int32)[row])
         alone, _ = model.forward(one)
         assert (alone - out[begin : begin + one.child_size]).abs().max() <= 4e-5 * out.abs().max()
+
+
+def test_cpp_api():
+    exe = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "encoder_api_test")
+    assert os.path.exists(exe), "build it with __graft_entry__.build() or make -C tests/cpp"
+    run = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert run.returncode == 0 and "ALL PASSED" in run.stdout, run.stdout + run.stderr
