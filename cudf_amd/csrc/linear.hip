@@ -429,7 +429,8 @@ __device__ __forceinline__ void TileProduct<T, A_NEXT, B_NEXT, BM, BN, WAVES_M, 
       slot ^= 1;
     }
     // Every wavefront turns its tile round in its own part of LDS, 16 rows at a time, and goes on with eight values of a row a lane.
-    // (A row's units of four values lie at unit ^ row.)
+    // (A row's units of four values lie at unit ^ row, within the row.)
+    constexpr int kUnits = kCols / 4 < 16 ? kCols / 4 - 1 : 15;
     LdsBytes const mine = stages + 2 * kStage + wave * (16 * kCols * 4);
     int64_t const j     = at.j0 + wn * kCols + lane % kRowLanes * 8;
     typename Epilogue<T>::Columns const columns(end, j, n);
@@ -438,12 +439,12 @@ __device__ __forceinline__ void TileProduct<T, A_NEXT, B_NEXT, BM, BN, WAVES_M, 
       for_each<MI * NI>([&](auto q) {
         constexpr int i = decltype(q)::value / NI, c = decltype(q)::value % NI;
         if (i == rows)
-          *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(mine + lane % 16 * kCols * 4 + ((c * 4 + lane / 16) ^ (lane % 16)) * 16) = sum[i][c];
+          *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(mine + lane % 16 * kCols * 4 + ((c * 4 + lane / 16) ^ (lane % 16 & kUnits)) * 16) = sum[i][c];
       });
       wave_lds_fence();
 #pragma nounroll
       for (int row = lane / kRowLanes; row < 16; row += kWave / kRowLanes) {
-        auto const unit = [&](int u) { return *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(mine + row * kCols * 4 + (u ^ row) * 16); };
+        auto const unit = [&](int u) { return *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(mine + row * kCols * 4 + (u ^ (row & kUnits)) * 16); };
         f32x4_t const x = unit(lane % kRowLanes * 2), y = unit(lane % kRowLanes * 2 + 1);
         float z[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
         int64_t const i = at.i0 + (wm * MI + rows) * 16 + row;
@@ -744,34 +745,46 @@ struct Factor {
   }
 };
 
-// How a product is shared out: tiles of 256 x 256 or of 128 x 128, and so many parts of the values of k.
+// How a product is shared out: tiles of 256 x 256, 128 x 128 or 128 x 64, and so many parts of the values of k.
+enum class Tile { k256, k128, k64 };
 struct Plan {
-  bool large;
+  Tile tile;
   int32_t parts;
   int64_t part;  // values of k a part
+  int64_t rows() const { return tile == Tile::k256 ? 256 : 128; }
+  int64_t cols() const { return tile == Tile::k256 ? 256 : tile == Tile::k128 ? 128 : 64; }
+  int64_t tiles(int64_t m, int64_t n) const { return (m + rows() - 1) / rows() * ((n + cols() - 1) / cols()); }
 };
 
 // The one that takes the least by this measure, in microseconds, fitted to products of 256 x 256 to 4096 x 4096 with 64 to 4096
 // values of k: a launch, then rounds of workgroups, each with so much for a stage of 64 values of k (more where all CUs are busy) and
-// for writing its tile; parts are written and read once more.  (4096 x 4096 x 64: 13.6 us in large tiles, 15.1 in small ones;
-// x 4096: 111 and 131.  2048 x 2048 x 4096: 80 and 49; 128 x 4096 x 4096: 77 and 43 in one part, 31 and 21 in four.)
-inline Plan plan_product(int64_t m, int64_t n, int64_t depth)
+// for writing its tile; parts are written and read once more.  (4096 x 4096 x 64: 13.6 us in large tiles, 15.1 in those of 128;
+// x 4096: 111 and 131.  2048 x 2048 x 4096: 80 and 49; 128 x 4096 x 4096: 77 and 43 in one part, 31 and 21 in four.  In tiles of 128
+// and in half ones: 512 x 512 x 512 10.7 and 7.4; 2048 x 1024 x 1024 13.7 and 11.0; 4096 x 1024 x 1024 15.5 and 15.6.)  `halves`:
+// both operands have their k next to each other, which half tiles are made for.
+inline Plan plan_product(int64_t m, int64_t n, int64_t depth, bool halves)
 {
   int64_t const cus = device_cus(), steps = std::max<int64_t>(1, (depth + kStageK - 1) / kStageK);
-  Plan best{true, 1, std::max<int64_t>(depth, 1)};
+  Plan best{Tile::k256, 1, std::max<int64_t>(depth, 1)};
   double least = 1e300;
-  for (bool large : {true, false}) {
-    int64_t const edge = large ? 256 : 128, tiles = (m + edge - 1) / edge * ((n + edge - 1) / edge);
+  for (Tile tile : {Tile::k256, Tile::k128, Tile::k64}) {
+    if (tile == Tile::k64 && !halves) continue;
     for (int64_t parts = 1; parts <= std::min<int64_t>(steps, 32); ++parts) {
       int64_t const each = (steps + parts - 1) / parts, really = (steps + each - 1) / each;
       if (really != parts) continue;
-      int64_t const groups = tiles * parts, load = (groups + cus - 1) / cus;  // workgroups, and of them a CU
+      Plan const plan{tile, static_cast<int32_t>(parts), each * kStageK};
+      int64_t const groups = plan.tiles(m, n) * parts, load = (groups + cus - 1) / cus;  // workgroups, and of them a CU
       double const busy    = std::min(1.0, static_cast<double>(groups) / cus);
-      double const work    = large ? 6 + load * (each * (1.05 + 0.45 * busy) + 5) : load == 1 ? 6 + each * (0.4 + 0.25 * busy) : 4 + (load + 1) / 2 * (each * 0.92 + 5);
-      double const time    = work + (parts > 1 ? 3 + parts * m * n * 8e-6 / 5 : 0);
+      double work          = 0;
+      switch (tile) {
+        case Tile::k256: work = 6 + load * (each * (1.05 + 0.45 * busy) + 5); break;
+        case Tile::k128: work = load == 1 ? 6 + each * (0.4 + 0.25 * busy) : 4 + (load + 1) / 2 * (each * 0.92 + 5); break;
+        case Tile::k64: work = load == 1 ? 4 + each * (0.38 + 0.14 * busy) : 3 + (load + 1) / 2 * (each * 0.66 + 2); break;
+      }
+      double const time = work + (parts > 1 ? 3 + parts * m * n * 8e-6 / 5 : 0);
       if (time < least) {
         least = time;
-        best  = Plan{large, static_cast<int32_t>(parts), each * kStageK};
+        best  = plan;
       }
     }
   }
@@ -807,7 +820,7 @@ struct Product {
   bool fits() const { return (m + 127) / 128 * ((n + 127) / 128) <= INT32_MAX / 64; }
   void make_plan()
   {
-    plan   = plan_product(m, n, depth);
+    plan   = plan_product(m, n, depth, a.k_next && b.k_next);
     copy_a = depth > 0 && !a.is_aligned(m, depth);
     copy_b = depth > 0 && !b.is_aligned(n, depth);
   }
@@ -829,26 +842,32 @@ struct Product {
   // workgroups: as many as the CUs hold at once
   int64_t workgroups() const
   {
-    int64_t const edge = plan.large ? 256 : 128, items = (m + edge - 1) / edge * ((n + edge - 1) / edge) * plan.parts;
-    return std::min<int64_t>(items, (plan.large ? 1 : 2) * static_cast<int64_t>(device_cus()));
+    return std::min<int64_t>(plan.tiles(m, n) * plan.parts, (plan.tile == Tile::k256 ? 1 : 2) * static_cast<int64_t>(device_cus()));
   }
-  template <int BM, int BN, int WAVES_M, int WAVES_N>
+  template <bool A_NEXT, bool B_NEXT, int BM, int BN, int WAVES_M, int WAVES_N>
   void launch_as(hipStream_t stream) const
   {
-    dim3 const grid(static_cast<unsigned>(workgroups())), threads(WAVES_M * WAVES_N * kWave);
-    if (a.k_next && b.k_next)
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, true, true, BM, BN, WAVES_M, WAVES_N>), grid, threads, 0, stream, problem());
-    else if (a.k_next)
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, true, false, BM, BN, WAVES_M, WAVES_N>), grid, threads, 0, stream, problem());
-    else
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, false, false, BM, BN, WAVES_M, WAVES_N>), grid, threads, 0, stream, problem());
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(tile_product_kernel<T, A_NEXT, B_NEXT, BM, BN, WAVES_M, WAVES_N>), dim3(static_cast<unsigned>(workgroups())), dim3(WAVES_M * WAVES_N * kWave), 0,
+                       stream, problem());
+  }
+  template <bool A_NEXT, bool B_NEXT>
+  void launch_as(hipStream_t stream) const
+  {
+    if (plan.tile == Tile::k256)
+      launch_as<A_NEXT, B_NEXT, 256, 256, 2, 4>(stream);
+    else if (plan.tile == Tile::k128)
+      launch_as<A_NEXT, B_NEXT, 128, 128, 2, 2>(stream);
+    else if constexpr (A_NEXT && B_NEXT)
+      launch_as<A_NEXT, B_NEXT, 128, 64, 2, 2>(stream);
   }
   void launch(hipStream_t stream) const
   {
-    if (plan.large)
-      launch_as<256, 256, 2, 4>(stream);
+    if (a.k_next && b.k_next)
+      launch_as<true, true>(stream);
+    else if (a.k_next)
+      launch_as<true, false>(stream);
     else
-      launch_as<128, 128, 2, 2>(stream);
+      launch_as<false, false>(stream);
   }
   Join<T> join() const { return Join<T>{sums, plan.parts, m, n, end}; }
   int64_t join_blocks() const { return wanted() && sums ? (m * ((n + 7) / 8) + kWave - 1) / kWave : 0; }
@@ -956,7 +975,7 @@ nvtext_amd_status linear_backward(Rows<const T> grad, Rows<const T> x, Rows<cons
   } else {
     if (of_x.bytes_sums()) of_x.sums = temp.template part<float>(4);
     if (of_weight.bytes_sums()) of_weight.sums = temp.template part<float>(5);
-    if (of_x.wanted() && of_weight.wanted() && !of_x.plan.large && !of_weight.plan.large) {
+    if (of_x.wanted() && of_weight.wanted() && of_x.plan.tile == Tile::k128 && of_weight.plan.tile == Tile::k128) {
       ProfileScope const scope("linear_products_backward", stream);
       int64_t const used = of_x.workgroups(), from = (used + 7) / 8 * 8;  // (workgroups go to the eight XCDs in turn)
       hipLaunchKernelGGL(gradient_products_kernel<T>, dim3(static_cast<unsigned>(from + of_weight.workgroups())), dim3(256), 0, stream, of_x.problem(), of_weight.problem(),
