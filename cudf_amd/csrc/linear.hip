@@ -620,59 +620,83 @@ struct Align {
   {
     int64_t const blocks = (cols + 7) / 8, at = block * kThreads + threadIdx.x;
     if (at >= rows * blocks) return;
-    int64_t const i = at / blocks, j = at % blocks * 8;
-    float f[8];
-    load8(f, in.row(i) + j, cols - j);
-    store8(out + i * blocks * 8 + j, f, 8);
+    // (32 bits where they do: a division of 64 takes as long as the rest)
+    int64_t const i = rows * blocks <= UINT32_MAX ? static_cast<uint32_t>(at) / static_cast<uint32_t>(blocks) : at / blocks, j = (at - i * blocks) * 8;
+    auto v = load_row8<T>(in.row(i), j, cols);
+    settle_row8<T>(v, j, cols);
+    *reinterpret_cast<typename Eight<T>::type*>(out + i * blocks * 8 + j) = v;
   }
 };
 
 // d = grad * activation'(z) where it is wanted (d's rows have a multiple of 8 values, zeros behind the last), and the sums of the
-// columns of it: a workgroup takes 512 columns and every count-th run of four rows, a wavefront one of the four, and the
-// wavefronts' sums are added up in the end, to the bias' gradient itself if that is all (count = 1).
+// columns of it: a workgroup takes up to 512 columns and every count-th run of rows, `lanes` lanes of a wavefront a row (fewer than
+// 64 for narrow rows, which lie side by side then); the sums are added up in order in the end, to the bias' gradient itself if that
+// is all (count = 1).
 template <typename T>
 struct Slopes {
   Rows<const T> grad, z;
   int activation;
   int64_t rows, cols;
   Rows<T> d;
+  int32_t lanes;
   int64_t count;
   float* parts;
   T* bias;
+  static int32_t lanes_of(int64_t cols) { return cols <= 64 ? 8 : cols <= 128 ? 16 : cols <= 256 ? 32 : kWave; }
+  // runs of rows: up to 64 for each place in a wavefront are left to one workgroup, without parts
+  static int64_t count_of(int64_t rows, int32_t lanes)
+  {
+    int64_t const across = kWave / lanes;
+    return rows <= 64 * across ? 1 : std::min<int64_t>((rows + 16 * across - 1) / (16 * across), 256);
+  }
+  int64_t workgroups() const { return (cols + 8 * lanes - 1) / (8 * lanes) * count; }
   __device__ __forceinline__ void run(int64_t block) const
   {
-    constexpr int kWaves = kThreads / kWave;
-    __shared__ float lds[kWaves][8][kWave];
-    int const wave = threadIdx.x / kWave, lane = lane_id();
-    int64_t const slices = (cols + 8 * kWave - 1) / (8 * kWave), slice = block % slices, number = block / slices;
-    int64_t const j      = (slice * kWave + lane) * 8;
+    constexpr int kWaves = kThreads / kWave, kAtOnce = 4;  // rows that a lane asks for at a time
+    __shared__ float lds[8][kThreads];
+    int const across     = kWave / lanes, place = threadIdx.x / lanes, at = threadIdx.x % lanes;
+    int64_t const slices = (cols + 8 * lanes - 1) / (8 * lanes), slice = block % slices, number = block / slices;
+    int64_t const j      = (slice * lanes + at) * 8;
     float sum[8]         = {};
     if (j < cols) {
-#pragma unroll 4
-      for (int64_t i = number * kWaves + wave; i < rows; i += count * kWaves) {
-        float g[8], v[8];
-        load8(g, grad.row(i) + j, cols - j);
-        if (z) {
-          load8(v, z.row(i) + j, cols - j);
-          with_activation(activation, [&](auto which) {
+      int64_t const step = count * kWaves * across;
+      for (int64_t first = number * kWaves * across + place; first < rows; first += kAtOnce * step) {
+        typename Eight<T>::type vg[kAtOnce], vz[kAtOnce];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) g[k] *= slope<decltype(which)::value>(v[k]);
-          });
+        for (int u = 0; u < kAtOnce; ++u) {
+          int64_t const i = first + u * step < rows ? first + u * step : first;  // (behind the last the first once more, not counted)
+          vg[u]           = load_row8<T>(grad.row(i), j, cols);
+          if (z) vz[u] = load_row8<T>(z.row(i), j, cols);
         }
-        if (d) store8(d.row(i) + j, g, 8);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) sum[k] += g[k];
+        for (int u = 0; u < kAtOnce; ++u) {
+          int64_t const i = first + u * step;
+          if (i >= rows) break;
+          float g[8], v[8];
+          if (cols % 8 != 0) settle_row8<T>(vg[u], j, cols);
+          widen<T>(g, vg[u]);
+          if (z) {
+            if (cols % 8 != 0) settle_row8<T>(vz[u], j, cols);
+            widen<T>(v, vz[u]);
+            with_activation(activation, [&](auto which) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) g[k] *= slope<decltype(which)::value>(v[k]);
+            });
+          }
+          if (d) store8(d.row(i) + j, g, 8);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) sum[k] += g[k];
+        }
       }
     }
     if (!parts && !bias) return;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) lds[wave][k][lane] = sum[k];
+    for (int k = 0; k < 8; ++k) lds[k][threadIdx.x] = sum[k];
     __syncthreads();
-    if (wave != 0 || j >= cols) return;
+    if (place != 0 || j >= cols) return;
+    for (int p = 1; p < kWaves * across; ++p)
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) sum[k] += lds[w][k][lane];
+      for (int k = 0; k < 8; ++k) sum[k] += lds[k][p * lanes + at];
     if (bias)
       store8(bias + j, sum, cols - j);
     else
@@ -946,8 +970,8 @@ nvtext_amd_status linear_backward(Rows<const T> grad, Rows<const T> x, Rows<cons
   // d is written where grad is not what the products can read
   bool const write_d     = m > 0 && n > 0 && (slopes || (of_x.wanted() && of_x.copy_a) || (of_weight.wanted() && of_weight.copy_a));
   int64_t const d_stride = (n + 7) / 8 * 8;
-  // few rows: one workgroup adds up a column's, without parts
-  int64_t const count    = m <= 64 ? 1 : std::min<int64_t>((m + 15) / 16, 256);
+  int32_t const lanes    = Slopes<T>::lanes_of(n);
+  int64_t const count    = Slopes<T>::count_of(m, lanes);
   bool const sums        = bias_grad && count > 1;
   TempParts<6> const temp(mr, {write_d ? static_cast<size_t>(m) * static_cast<size_t>(d_stride) * sizeof(T) : 0, sums ? static_cast<size_t>(count * n) * sizeof(float) : 0,
                                of_x.wanted() ? of_x.bytes_b() : 0, of_weight.wanted() ? of_weight.bytes_b() : 0, of_x.wanted() ? of_x.bytes_sums() : 0,
@@ -961,9 +985,9 @@ nvtext_amd_status linear_backward(Rows<const T> grad, Rows<const T> x, Rows<cons
   Align<T> a{}, b{};
   if (of_x.wanted() && of_x.copy_b) a = of_x.align(of_x.b, depth, n, temp.template part<T>(2));
   if (of_weight.wanted() && of_weight.copy_b) b = of_weight.align(of_weight.b, depth, m, temp.template part<T>(3));
-  Slopes<T> const act{grad, slopes ? z : Rows<const T>{nullptr, 0}, activation, m, n, d, count, sums ? temp.template part<float>(1) : nullptr, sums ? nullptr : bias_grad};
+  Slopes<T> const act{grad, slopes ? z : Rows<const T>{nullptr, 0}, activation, m, n, d, lanes, count, sums ? temp.template part<float>(1) : nullptr, sums ? nullptr : bias_grad};
   int64_t const first = blocks_of(a.rows * ((a.cols + 7) / 8)), second = blocks_of(b.rows * ((b.cols + 7) / 8));
-  int64_t const third = write_d || bias_grad ? (n + 8 * kWave - 1) / (8 * kWave) * count : 0;
+  int64_t const third = write_d || bias_grad ? act.workgroups() : 0;
   if (first + second + third > 0) {
     ProfileScope const scope("linear_prepare_backward", stream);
     hipLaunchKernelGGL(prepare_kernel<T>, dim3(static_cast<unsigned>(first + second + third)), dim3(kThreads), 0, stream, a, first, b, second, act);
