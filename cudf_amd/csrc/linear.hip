@@ -78,14 +78,6 @@ __device__ __forceinline__ void with_activation(int activation, F&& f)
   }
 }
 
-// An operand of a product: value (i, k) is data[i * of_i + k * of_k].
-template <typename T>
-struct Operand {
-  const T* data;
-  int64_t of_i, of_k;
-  __device__ __forceinline__ float at(int64_t i, int64_t k) const { return static_cast<float>(data[i * of_i + k * of_k]); }
-};
-
 // What becomes of eight sums over k.
 template <typename T>
 struct Epilogue {
@@ -148,6 +140,14 @@ using LdsBytes = __attribute__((address_space(3))) char*;
 
 __device__ __forceinline__ f32x4_t multiply(Fragment<bf16_t> a, Fragment<bf16_t> b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4_t multiply(Fragment<half_t> a, Fragment<half_t> b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// (16 x 16 x 4 at a time: that value e of every lane goes into product e is as good an order of k as another)
+__device__ __forceinline__ f32x4_t multiply(Fragment<float> a, Fragment<float> b, f32x4_t c)
+{
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+  return c;
+}
 
 // An operand: a multiple of 8 values next to each other in each line, lines at multiples of 16 bytes.
 struct Side {
@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(256, 2) gradient_products_kernel(Problem<T> of
 template <typename T, int MI, int WAVES>
 __global__ void __launch_bounds__(WAVES * kWave) few_rows_kernel(Rows<const T> x, Rows<const T> weight, int64_t m, int64_t n, int64_t depth, Epilogue<T> end)
 {
-  constexpr int kDeep = MI == 4 ? 4 : WAVES == 16 ? 6 : 8;  // (as many as the registers hold)
+  constexpr int kDeep = sizeof(T) == 4 ? (MI == 1 && WAVES < 16 ? 4 : 2) : MI == 4 ? 4 : WAVES == 16 ? 6 : 8;  // (as many as the registers hold)
   __shared__ __attribute__((aligned(16))) float lds[WAVES][MI][16][20];  // (16 outputs a row, and room against conflicts)
   int const wave = threadIdx.x / kWave, lane = lane_id();
   int64_t const j0 = static_cast<int64_t>(blockIdx.x) * 16;
@@ -718,39 +718,116 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(Align<T> a, int64_t f
 }
 
 // ------------------------------------------------------------------ products of 32-bit types
-// out (i, j) = sum over k of a (i, k) * b (j, k).  A workgroup a tile of 64 x 64, a thread two rows of eight.
-constexpr int kTile = 64, kDepth = 16;
+// The same of float, on the matrix cores' products of 16 x 16 x 4, which keep float's precision at a sixteenth of the rate: so slow
+// that plain loads through registers, one stage of 16 values of k ahead, keep up, and rows may lie anyhow.  A stage lies in
+// LDS as [k][row], lines 16 banks apart from each other: the four lines that a fragment is read from take all 64.
+// Bound by the matrix cores: 8192 x 1024 outputs of 4096 values 600 us, 114 TFLOP/s of 157 (a product of plain additions and
+// multiplications in tiles of 64 x 64: 1440).
+constexpr int kStage32 = 16;
 
-__global__ void __launch_bounds__(kThreads) product_kernel(Operand<float> a, Operand<float> b, int64_t m, int64_t n, int64_t depth, Epilogue<float> end)
-{
-  __shared__ float la[kDepth][kTile + 4], lb[kDepth][kTile + 4];
-  int64_t const tiles_n = (n + kTile - 1) / kTile;
-  int64_t const i0 = blockIdx.x / tiles_n * kTile, j0 = blockIdx.x % tiles_n * kTile;
-  int const ti = threadIdx.x / 8 * 2, tj = threadIdx.x % 8 * 8;
-  float sum[2][8] = {};
-  for (int64_t k0 = 0; k0 < depth; k0 += kDepth) {
-    for (int x = threadIdx.x; x < kTile * kDepth; x += kThreads) {
-      // neighbouring threads read neighbouring values
-      int const ia = a.of_k == 1 ? x / kDepth : x % kTile, ka = a.of_k == 1 ? x % kDepth : x / kTile;
-      int const ib = b.of_k == 1 ? x / kDepth : x % kTile, kb = b.of_k == 1 ? x % kDepth : x / kTile;
-      la[ka][ia] = i0 + ia < m && k0 + ka < depth ? a.at(i0 + ia, k0 + ka) : 0.f;
-      lb[kb][ib] = j0 + ib < n && k0 + kb < depth ? b.at(j0 + ib, k0 + kb) : 0.f;
+template <bool K_NEXT, int EXT>
+struct Loader32 {
+  static constexpr int kPieces = EXT * kStage32 / 4 / kThreads;  // of four values a thread
+  static constexpr int kLine   = EXT / 4;                        // (not K_NEXT) threads that a value of k takes
+  static constexpr int kStride = EXT + 16;                       // of a line in LDS
+  typedef float Four __attribute__((ext_vector_type(4), aligned(4)));
+  Four v[kPieces];
+  static __device__ __forceinline__ int row_of(int p) { return K_NEXT ? p * (kThreads / 4) + threadIdx.x / 4 : threadIdx.x % kLine * 4; }
+  static __device__ __forceinline__ int k_of(int p) { return K_NEXT ? threadIdx.x % 4 * 4 : p * (kThreads / kLine) + threadIdx.x / kLine; }
+  // rows from i0 on of `extent`, values from k0 on up to `last`; zeros behind them
+  __device__ __forceinline__ void load(Side const& side, int64_t i0, int64_t extent, int64_t k0, int64_t last)
+  {
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      int64_t const i = i0 + row_of(p), k = k0 + k_of(p);
+      int64_t const left = K_NEXT ? (i < extent ? last - k : 0) : (k < last ? extent - i : 0);
+      const float* const at = static_cast<const float*>(side.data) + (K_NEXT ? i * side.stride + k : k * side.stride + i);
+      v[p] = Four{0.f, 0.f, 0.f, 0.f};
+      if (left >= 4) {
+        v[p] = *reinterpret_cast<const Four*>(at);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (e < left) v[p][e] = at[e];
+      }
     }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kDepth; ++k) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum[i][j] += la[k][ti + i] * lb[k][tj + j];
-    }
-    __syncthreads();
   }
-  if (j0 + tj >= n) return;
-  Epilogue<float>::Columns const columns(end, j0 + tj, n);
+  __device__ __forceinline__ void store(float* lds) const
+  {
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (i0 + ti + i < m) end.finish(sum[i], columns, i0 + ti + i, j0 + tj, n);
+    for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) lds[(k_of(p) + (K_NEXT ? e : 0)) * kStride + row_of(p) + (K_NEXT ? 0 : e)] = v[p][e];
+  }
+};
+
+template <bool A_NEXT, bool B_NEXT, int BN>
+__global__ void __launch_bounds__(kThreads, 2) product_kernel(Problem<float> problem)
+{
+  constexpr int BM = 128, MI = BM / 32, NI = BN / 32, kCols = NI * 16, kRowLanes = kCols / 8;  // 2 x 2 wavefronts
+  constexpr int kA = kStage32 * (BM + 16), kB = kStage32 * (BN + 16);
+  __shared__ __attribute__((aligned(16))) float lds[2][kA + kB];
+  static_assert(4 * 16 * kCols <= 2 * (kA + kB));
+  int64_t const m = problem.m, n = problem.n;
+  int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id(), wm = wave / 2, wn = wave % 2;
+  // workgroups go to the eight XCDs in turn: each takes a run of tiles
+  int32_t const items = gridDim.x, xcd = blockIdx.x % 8, per_xcd = items / 8, more = items % 8;
+  int32_t const item = xcd * per_xcd + (xcd < more ? xcd : more) + blockIdx.x / 8;
+  int32_t const tiles_n = static_cast<int32_t>((n + BN - 1) / BN), tiles = static_cast<int32_t>((m + BM - 1) / BM) * tiles_n, part = item / tiles, tile = item % tiles;
+  int64_t const i0 = static_cast<int64_t>(tile / tiles_n) * BM, j0 = static_cast<int64_t>(tile % tiles_n) * BN;
+  int64_t const first = part * problem.part, last = first + problem.part < problem.depth ? first + problem.part : problem.depth;
+  Loader32<A_NEXT, BM> a;
+  Loader32<B_NEXT, BN> b;
+  f32x4_t sum[MI][NI] = {};
+  a.load(problem.a, i0, m, first, last);
+  b.load(problem.b, j0, n, first, last);
+  int buffer = 0;
+  for (int64_t k0 = first; k0 < last; k0 += kStage32, buffer ^= 1) {
+    float *const la = lds[buffer], *const lb = la + kA;
+    a.store(la);
+    b.store(lb);
+    __syncthreads();
+    a.load(problem.a, i0, m, k0 + kStage32, last);
+    b.load(problem.b, j0, n, k0 + kStage32, last);
+#pragma unroll
+    for (int k = 0; k < kStage32; k += 4) {
+      float fa[MI], fb[NI];
+#pragma unroll
+      for (int i = 0; i < MI; ++i) fa[i] = la[(k + lane / 16) * (BM + 16) + (wm * MI + i) * 16 + lane % 16];
+#pragma unroll
+      for (int j = 0; j < NI; ++j) fb[j] = lb[(k + lane / 16) * (BN + 16) + (wn * NI + j) * 16 + lane % 16];
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) sum[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[j], fa[i], sum[i][j], 0, 0, 0);  // (transposed: a lane has four values of a row)
+    }
+  }
+  // every wavefront turns its tile round, 16 rows at a time, as above
+  __syncthreads();
+  constexpr int kUnits = kCols / 4 - 1;
+  float* const mine    = &lds[0][0] + wave * 16 * kCols;
+  int64_t const j      = j0 + wn * kCols + lane % kRowLanes * 8;
+  Epilogue<float>::Columns const columns(problem.end, j, n);
+#pragma unroll
+  for (int rows = 0; rows < MI; ++rows) {
+#pragma unroll
+    for (int c = 0; c < NI; ++c) *reinterpret_cast<f32x4_t*>(mine + lane % 16 * kCols + ((c * 4 + lane / 16) ^ (lane % 16 & kUnits)) * 4) = sum[rows][c];
+    wave_lds_fence();
+#pragma nounroll
+    for (int row = lane / kRowLanes; row < 16; row += kWave / kRowLanes) {
+      auto const unit = [&](int u) { return *reinterpret_cast<const f32x4_t*>(mine + row * kCols + (u ^ (row & kUnits)) * 4); };
+      f32x4_t const x = unit(lane % kRowLanes * 2), y = unit(lane % kRowLanes * 2 + 1);
+      float z[8]      = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+      int64_t const i = i0 + (wm * MI + rows) * 16 + row;
+      if (i < m && j < n) {
+        if (problem.sums)
+          store8(problem.sums + (part * m + i) * n + j, z, n - j);
+        else
+          problem.end.finish(z, columns, i, j, n);
+      }
+    }
+    wave_lds_fence();
+  }
 }
 
 // An operand of a product of `extent` rows and `depth` values of k each.
@@ -815,6 +892,28 @@ inline Plan plan_product(int64_t m, int64_t n, int64_t depth, bool halves)
   return best;
 }
 
+// The same for 32-bit types, in tiles of 128 x 128 or 128 x 64: a stage of 16 values of k takes the matrix cores 0.9 us or half of that.
+inline Plan plan_product32(int64_t m, int64_t n, int64_t depth)
+{
+  int64_t const cus = device_cus(), steps = std::max<int64_t>(1, (depth + kStage32 - 1) / kStage32);
+  Plan best{Tile::k128, 1, std::max<int64_t>(depth, 1)};
+  double least = 1e300;
+  for (Tile tile : {Tile::k128, Tile::k64}) {
+    for (int64_t parts = 1; parts <= std::min<int64_t>(steps, 32); ++parts) {
+      int64_t const each = (steps + parts - 1) / parts;
+      if ((steps + each - 1) / each != parts) continue;
+      Plan const plan{tile, static_cast<int32_t>(parts), each * kStage32};
+      int64_t const load = (plan.tiles(m, n) * parts + cus - 1) / cus;
+      double const time  = 5 + load * (each * (tile == Tile::k128 ? 0.95 : 0.5) + 2) + (parts > 1 ? 3 + parts * m * n * 8e-6 / 5 : 0);
+      if (time < least) {
+        least = time;
+        best  = plan;
+      }
+    }
+  }
+  return best;
+}
+
 // Whether few_rows_kernel takes less time than tiles: microseconds of either, fitted to calls of 1 to 64 rows with 1024 to 8192
 // inputs and outputs.  It goes through k in one workgroup for 16 outputs, which takes longer with every 16 rows; tiles cost a launch
 // more, and then read the weights as fast as memory gives them.  (16 rows: 1024 to 4096 4.9 us against 11.5, 4096 to 1024 10.5
@@ -844,6 +943,10 @@ struct Product {
   bool fits() const { return (m + 127) / 128 * ((n + 127) / 128) <= INT32_MAX / 64; }
   void make_plan()
   {
+    if constexpr (sizeof(T) == 4) {
+      plan = plan_product32(m, n, depth);
+      return;
+    }
     plan   = plan_product(m, n, depth, a.k_next && b.k_next);
     copy_a = depth > 0 && !a.is_aligned(m, depth);
     copy_b = depth > 0 && !b.is_aligned(n, depth);
@@ -877,7 +980,13 @@ struct Product {
   template <bool A_NEXT, bool B_NEXT>
   void launch_as(hipStream_t stream) const
   {
-    if (plan.tile == Tile::k256)
+    if constexpr (sizeof(T) == 4) {
+      dim3 const grid(static_cast<unsigned>(plan.tiles(m, n) * plan.parts));
+      if (plan.tile == Tile::k128)
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<A_NEXT, B_NEXT, 128>), grid, dim3(kThreads), 0, stream, problem());
+      else
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<A_NEXT, B_NEXT, 64>), grid, dim3(kThreads), 0, stream, problem());
+    } else if (plan.tile == Tile::k256)
       launch_as<A_NEXT, B_NEXT, 256, 256, 2, 4>(stream);
     else if (plan.tile == Tile::k128)
       launch_as<A_NEXT, B_NEXT, 128, 128, 2, 2>(stream);
@@ -896,12 +1005,6 @@ struct Product {
   Join<T> join() const { return Join<T>{sums, plan.parts, m, n, end}; }
   int64_t join_blocks() const { return wanted() && sums ? (m * ((n + 7) / 8) + kWave - 1) / kWave : 0; }
 };
-
-void launch_product(Factor<float> const& a, Factor<float> const& b, int64_t m, int64_t n, int64_t depth, Epilogue<float> const& end, hipStream_t stream)
-{
-  auto const operand = [](Factor<float> const& f) { return Operand<float>{f.rows.data, f.k_next ? f.rows.stride : 1, f.k_next ? 1 : f.rows.stride}; };
-  hipLaunchKernelGGL(product_kernel, dim3(static_cast<unsigned>((n + kTile - 1) / kTile * ((m + kTile - 1) / kTile))), dim3(kThreads), 0, stream, operand(a), operand(b), m, n, depth, end);
-}
 
 template <typename T>
 void launch_few_rows(Rows<const T> x, Rows<const T> weight, int64_t m, int64_t n, int64_t depth, Epilogue<T> const& end, hipStream_t stream)
@@ -929,27 +1032,23 @@ void launch_few_rows(Rows<const T> x, Rows<const T> weight, int64_t m, int64_t n
 template <typename T>
 nvtext_amd_status linear(Rows<const T> x, Rows<const T> weight, int64_t m, int64_t n, int64_t depth, Epilogue<T> const& end, Mr const& mr, hipStream_t stream)
 {
-  if constexpr (sizeof(T) == 4) {
-    launch_product({x, true}, {weight, true}, m, n, depth, end, stream);
-  } else {
-    if (few_rows_are_faster(m, n, depth)) {
-      launch_few_rows(x, weight, m, n, depth, end, stream);
-      return NVTEXT_AMD_SUCCESS;
-    }
-    Product<T> p{{x, true}, {weight, true}, m, n, depth, end};
-    if (!p.fits()) return fail(NVTEXT_AMD_OVERFLOW, "the product is too large");
-    p.make_plan();
-    TempParts<3> const temp(mr, {p.bytes_a(), p.bytes_b(), p.bytes_sums()}, p.bytes_a() + p.bytes_b() + p.bytes_sums() > 0);
-    if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
-    Align<T> a{}, b{};
-    if (p.copy_a) a = p.align(p.a, m, depth, temp.template part<T>(0));
-    if (p.copy_b) b = p.align(p.b, n, depth, temp.template part<T>(1));
-    int64_t const first = blocks_of(a.rows * ((a.cols + 7) / 8)), second = blocks_of(b.rows * ((b.cols + 7) / 8));
-    if (first + second > 0) hipLaunchKernelGGL(prepare_kernel<T>, dim3(static_cast<unsigned>(first + second)), dim3(kThreads), 0, stream, a, first, b, second, Slopes<T>{});
-    if (p.plan.parts > 1) p.sums = temp.template part<float>(2);
-    p.launch(stream);
-    if (p.sums) hipLaunchKernelGGL(join_kernel<T>, dim3(static_cast<unsigned>(p.join_blocks())), dim3(kThreads), 0, stream, p.join(), p.join_blocks(), Join<T>{}, 0, JoinColumns<T>{});
+  if (few_rows_are_faster(m, n, depth)) {
+    launch_few_rows(x, weight, m, n, depth, end, stream);
+    return NVTEXT_AMD_SUCCESS;
   }
+  Product<T> p{{x, true}, {weight, true}, m, n, depth, end};
+  if (!p.fits()) return fail(NVTEXT_AMD_OVERFLOW, "the product is too large");
+  p.make_plan();
+  TempParts<3> const temp(mr, {p.bytes_a(), p.bytes_b(), p.bytes_sums()}, p.bytes_a() + p.bytes_b() + p.bytes_sums() > 0);
+  if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
+  Align<T> a{}, b{};
+  if (p.copy_a) a = p.align(p.a, m, depth, temp.template part<T>(0));
+  if (p.copy_b) b = p.align(p.b, n, depth, temp.template part<T>(1));
+  int64_t const first = blocks_of(a.rows * ((a.cols + 7) / 8)), second = blocks_of(b.rows * ((b.cols + 7) / 8));
+  if (first + second > 0) hipLaunchKernelGGL(prepare_kernel<T>, dim3(static_cast<unsigned>(first + second)), dim3(kThreads), 0, stream, a, first, b, second, Slopes<T>{});
+  if (p.plan.parts > 1) p.sums = temp.template part<float>(2);
+  p.launch(stream);
+  if (p.sums) hipLaunchKernelGGL(join_kernel<T>, dim3(static_cast<unsigned>(p.join_blocks())), dim3(kThreads), 0, stream, p.join(), p.join_blocks(), Join<T>{}, 0, JoinColumns<T>{});
   return NVTEXT_AMD_SUCCESS;
 }
 
@@ -959,14 +1058,12 @@ nvtext_amd_status linear_backward(Rows<const T> grad, Rows<const T> x, Rows<cons
                                   Rows<T> weight_grad, T* bias_grad, Mr const& mr, hipStream_t stream)
 {
   auto const plain = [](Rows<T> out) { return Epilogue<T>{{nullptr, 0}, {nullptr, 0}, out, {nullptr, 0}, NVTEXT_AMD_ACTIVATION_NONE}; };
-  bool const slopes = activation != NVTEXT_AMD_ACTIVATION_NONE, large = sizeof(T) == 4;
+  bool const slopes = activation != NVTEXT_AMD_ACTIVATION_NONE;
   // x_grad (m x depth) = d * weight, weight_grad (n x depth) = d^T * x
   Product<T> of_x{{grad, true}, {weight, false}, x_grad ? m : 0, depth, n, plain(x_grad)}, of_weight{{grad, false}, {x, false}, weight_grad ? n : 0, depth, m, plain(weight_grad)};
   if (!of_x.fits() || !of_weight.fits()) return fail(NVTEXT_AMD_OVERFLOW, "the product is too large");
-  if (!large) {
-    of_x.make_plan();
-    of_weight.make_plan();
-  }
+  of_x.make_plan();
+  of_weight.make_plan();
   // d is written where grad is not what the products can read
   bool const write_d     = m > 0 && n > 0 && (slopes || (of_x.wanted() && of_x.copy_a) || (of_weight.wanted() && of_weight.copy_a));
   int64_t const d_stride = (n + 7) / 8 * 8;
@@ -992,28 +1089,25 @@ nvtext_amd_status linear_backward(Rows<const T> grad, Rows<const T> x, Rows<cons
     ProfileScope const scope("linear_prepare_backward", stream);
     hipLaunchKernelGGL(prepare_kernel<T>, dim3(static_cast<unsigned>(first + second + third)), dim3(kThreads), 0, stream, a, first, b, second, act);
   }
-  if constexpr (sizeof(T) == 4) {
-    ProfileScope const scope("linear_products_backward", stream);
-    if (of_x.wanted() && depth > 0) launch_product(of_x.a, of_x.b, m, depth, n, of_x.end, stream);
-    if (of_weight.wanted() && depth > 0) launch_product(of_weight.a, of_weight.b, n, depth, m, of_weight.end, stream);
-  } else {
-    if (of_x.bytes_sums()) of_x.sums = temp.template part<float>(4);
-    if (of_weight.bytes_sums()) of_weight.sums = temp.template part<float>(5);
-    if (of_x.wanted() && of_weight.wanted() && of_x.plan.tile == Tile::k128 && of_weight.plan.tile == Tile::k128) {
+  if (of_x.bytes_sums()) of_x.sums = temp.template part<float>(4);
+  if (of_weight.bytes_sums()) of_weight.sums = temp.template part<float>(5);
+  bool both = false;  // in one launch
+  if constexpr (sizeof(T) == 2) {
+    both = of_x.wanted() && of_weight.wanted() && of_x.plan.tile == Tile::k128 && of_weight.plan.tile == Tile::k128;
+    if (both) {
       ProfileScope const scope("linear_products_backward", stream);
       int64_t const used = of_x.workgroups(), from = (used + 7) / 8 * 8;  // (workgroups go to the eight XCDs in turn)
       hipLaunchKernelGGL(gradient_products_kernel<T>, dim3(static_cast<unsigned>(from + of_weight.workgroups())), dim3(256), 0, stream, of_x.problem(), of_weight.problem(),
                          static_cast<int32_t>(from), static_cast<int32_t>(used));
-    } else {
-      if (of_x.wanted()) {
-        ProfileScope const scope("linear_x_backward", stream);
-        of_x.launch(stream);
-      }
-      if (of_weight.wanted()) {
-        ProfileScope const scope("linear_weight_backward", stream);
-        of_weight.launch(stream);
-      }
     }
+  }
+  if (of_x.wanted() && !both) {
+    ProfileScope const scope("linear_x_backward", stream);
+    of_x.launch(stream);
+  }
+  if (of_weight.wanted() && !both) {
+    ProfileScope const scope("linear_weight_backward", stream);
+    of_weight.launch(stream);
   }
   int64_t const join_x = of_x.join_blocks(), join_weight = of_weight.join_blocks(), join_columns = sums ? (n + kWave - 1) / kWave : 0;
   if (join_x + join_weight + join_columns > 0) {
