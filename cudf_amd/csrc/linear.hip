@@ -533,40 +533,49 @@ __global__ void __launch_bounds__(WAVES * kWave) few_rows_kernel(Rows<const T> x
 }
 
 // ------------------------------------------------------------------ before and after
-// The parts of a product that was cut along k: a workgroup 64 times eight values, a wavefront a run of parts, eight of them asked for
-// at a time.
+// The parts of a product that was cut along k, eight of them asked for at a time.  Where there are many results a thread has eight of
+// them, else (`spread`) a workgroup has 64 times eight, and each of its wavefronts a run of the parts.  (4 parts of 4096 x 1024
+// 20 us, spread 26; many parts of a small result 55 -> 39 us for the whole of a gradient of 34 x 924 x 4928.)
 template <typename T>
 struct Join {
   const float* sums;
   int64_t parts, m, n;
   Epilogue<T> end;
+  bool spread;
+  __device__ __forceinline__ void add(float (&z)[8], int64_t i, int64_t j, int64_t first, int64_t last) const
+  {
+#pragma unroll 8
+    for (int64_t p = first; p < last; ++p) {
+      float more[8];
+      load8(more, sums + (p * m + i) * n + j, n - j);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) z[k] += more[k];
+    }
+  }
   __device__ __forceinline__ void run(int64_t block) const
   {
     constexpr int kWaves = kThreads / kWave;
     __shared__ float lds[kWaves][8][kWave];
     int const wave = threadIdx.x / kWave, lane = lane_id();
-    int64_t const blocks = (n + 7) / 8, at = block * kWave + lane;
-    int64_t const i = at / blocks, j = at % blocks * 8;
+    int64_t const blocks = (n + 7) / 8, at = spread ? block * kWave + lane : block * kThreads + threadIdx.x;
+    int64_t const i = m * blocks <= UINT32_MAX ? static_cast<uint32_t>(at) / static_cast<uint32_t>(blocks) : at / blocks, j = (at - i * blocks) * 8;
     bool const here = at < m * blocks;
-    int64_t const each = (parts + kWaves - 1) / kWaves, first = wave * each, last = first + each < parts ? first + each : parts;
-    float z[8] = {};
-    if (here) {
-#pragma unroll 8
-      for (int64_t p = first; p < last; ++p) {
-        float more[8];
-        load8(more, sums + (p * m + i) * n + j, n - j);
+    float z[8]      = {};
+    if (!spread) {
+      if (!here) return;
+      add(z, i, j, 0, parts);
+    } else {
+      int64_t const each = (parts + kWaves - 1) / kWaves, first = wave * each, last = first + each < parts ? first + each : parts;
+      if (here) add(z, i, j, first, last);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) z[k] += more[k];
-      }
+      for (int k = 0; k < 8; ++k) lds[wave][k][lane] = z[k];
+      __syncthreads();
+      if (wave != 0 || !here) return;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) z[k] += lds[w][k][lane];
     }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) lds[wave][k][lane] = z[k];
-    __syncthreads();
-    if (wave != 0 || !here) return;
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) z[k] += lds[w][k][lane];
     end.finish(z, typename Epilogue<T>::Columns(end, j, n), i, j, n);
   }
 };
@@ -1002,8 +1011,10 @@ struct Product {
     else
       launch_as<false, false>(stream);
   }
-  Join<T> join() const { return Join<T>{sums, plan.parts, m, n, end}; }
-  int64_t join_blocks() const { return wanted() && sums ? (m * ((n + 7) / 8) + kWave - 1) / kWave : 0; }
+  int64_t eights() const { return m * ((n + 7) / 8); }
+  bool spread() const { return eights() < 256 * device_cus(); }
+  Join<T> join() const { return Join<T>{sums, plan.parts, m, n, end, spread()}; }
+  int64_t join_blocks() const { return wanted() && sums ? (spread() ? (eights() + kWave - 1) / kWave : blocks_of(eights())) : 0; }
 };
 
 template <typename T>
