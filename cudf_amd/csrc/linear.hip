@@ -619,12 +619,16 @@ __global__ void __launch_bounds__(kThreads) join_kernel(Join<T> a, int64_t first
     columns.run(block - first - second);
 }
 
+// From a line of a copy to the next: a multiple of 8 values, or of 64, whole cache lines, where these are few more (a stage's 128
+// bytes lie in one of them then: 1777 x 2051 x 1003 33 us instead of 38).
+inline int64_t copy_stride(int64_t cols) { return cols >= 512 ? (cols + 63) / 64 * 64 : (cols + 7) / 8 * 8; }
+
 // Lines of `cols` values, aligned anyhow, into lines of a multiple of 8 values, zeros behind the last.
 template <typename T>
 struct Align {
   Rows<const T> in;
   int64_t rows, cols;
-  T* out;
+  Rows<T> out;
   __device__ __forceinline__ void run(int64_t block) const
   {
     int64_t const blocks = (cols + 7) / 8, at = block * kThreads + threadIdx.x;
@@ -633,7 +637,7 @@ struct Align {
     int64_t const i = rows * blocks <= UINT32_MAX ? static_cast<uint32_t>(at) / static_cast<uint32_t>(blocks) : at / blocks, j = (at - i * blocks) * 8;
     auto v = load_row8<T>(in.row(i), j, cols);
     settle_row8<T>(v, j, cols);
-    *reinterpret_cast<typename Eight<T>::type*>(out + i * blocks * 8 + j) = v;
+    *reinterpret_cast<typename Eight<T>::type*>(out.row(i) + j) = v;
   }
 };
 
@@ -962,15 +966,16 @@ struct Product {
   }
   static size_t copy_bytes(Factor<T> const& f, int64_t extent, int64_t depth)
   {
-    return static_cast<size_t>(f.lines(extent, depth)) * static_cast<size_t>((f.cols(extent, depth) + 7) / 8 * 8) * sizeof(T);
+    return static_cast<size_t>(f.lines(extent, depth)) * static_cast<size_t>(copy_stride(f.cols(extent, depth))) * sizeof(T);
   }
   size_t bytes_a() const { return copy_a ? copy_bytes(a, m, depth) : 0; }
   size_t bytes_b() const { return copy_b ? copy_bytes(b, n, depth) : 0; }
   size_t bytes_sums() const { return plan.parts > 1 ? static_cast<size_t>(plan.parts) * static_cast<size_t>(m * n) * sizeof(float) : 0; }
   static Align<T> align(Factor<T>& f, int64_t extent, int64_t depth, T* to)
   {
-    Align<T> const copy{f.rows, f.lines(extent, depth), f.cols(extent, depth), to};
-    f.rows   = Rows<const T>{to, (copy.cols + 7) / 8 * 8};
+    int64_t const cols = f.cols(extent, depth);
+    Align<T> const copy{f.rows, f.lines(extent, depth), cols, {to, copy_stride(cols)}};
+    f.rows   = Rows<const T>{to, copy_stride(cols)};
     f.padded = true;
     return copy;
   }
@@ -1077,7 +1082,7 @@ nvtext_amd_status linear_backward(Rows<const T> grad, Rows<const T> x, Rows<cons
   of_weight.make_plan();
   // d is written where grad is not what the products can read
   bool const write_d     = m > 0 && n > 0 && (slopes || (of_x.wanted() && of_x.copy_a) || (of_weight.wanted() && of_weight.copy_a));
-  int64_t const d_stride = (n + 7) / 8 * 8;
+  int64_t const d_stride = copy_stride(n);
   int32_t const lanes    = Slopes<T>::lanes_of(n);
   int64_t const count    = Slopes<T>::count_of(m, lanes);
   bool const sums        = bias_grad && count > 1;
