@@ -532,6 +532,172 @@ __global__ void __launch_bounds__(WAVES * kWave) few_rows_kernel(Rows<const T> x
   end.finish(z, typename Epilogue<T>::Columns(end, j0 + j, n), i, j0 + j, n);
 }
 
+// The gradients of a call of up to 16 * MI rows, in one launch or, where many outputs are cut into parts, two.  A workgroup takes 64
+// inputs and a part of the outputs, 64 of them at a time: it makes d for them (which every workgroup of the part does anew: it
+// is small), stages it and the 64 x 64 weights in LDS through registers, one stage ahead, and has of both the sums that x's gradient
+// needs, which it keeps, and the weights' gradient, which is complete after one stage.  A wavefront has 16 of the inputs.
+// Rows may lie anyhow.  Bound by launches and, of many weights, by memory: with gelu 7 x 64 x 64 5.9 us (12.6 in three
+// launches with tiles), 34 x 924 x 4928 28 (39).
+template <typename T>
+struct FewRowsBackward {
+  Rows<const T> grad, z, x, weight;
+  Rows<T> x_grad, weight_grad;
+  T* bias_grad;
+  int activation;
+  int64_t m, n, depth;
+  int64_t part;  // outputs a part, a multiple of 64
+  int32_t parts;
+  float* sums;   // [part][m][depth], of several parts
+};
+
+constexpr int kFewEdge = 64, kFewPitch = kFewEdge + 8;
+
+// eight values of k for each of 16 columns from `at` on, k along the rows
+template <typename T>
+__device__ __forceinline__ Fragment<T> read_turned(const T* at, int lane)
+{
+  int const i = lane % 16, g = lane / 16;
+  auto const p       = (LdsBytes)(at + (g * 8 + i / 4) * kFewPitch + i % 4 * 4);
+  s16x4_t const low  = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(p));
+  s16x4_t const high = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(p + 4 * kFewPitch * 2));
+  return __builtin_bit_cast(Fragment<T>, __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// four of a row's values from p on, of which n are there
+template <typename T>
+__device__ __forceinline__ void store4(T* p, f32x4_t const& f, int64_t n)
+{
+  typedef T V __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  if (n >= 4) {
+    *reinterpret_cast<V*>(p) = V{static_cast<T>(f[0]), static_cast<T>(f[1]), static_cast<T>(f[2]), static_cast<T>(f[3])};
+  } else {
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      if (k < n) p[k] = static_cast<T>(f[k]);
+  }
+}
+
+template <typename T, int MI>
+__global__ void __launch_bounds__(kThreads, 2) few_rows_backward_kernel(FewRowsBackward<T> w)
+{
+  // (MI = 1: 32 values of k all the same, the second half zeros)
+  constexpr int kRows = MI == 1 ? 32 : MI * 16, KI = kRows / 32, kEach = kRows * 8 / kThreads;  // pieces of eight of d (and x) a thread
+  static_assert(kEach >= 1 && kThreads == 4 * kWave);
+  __shared__ __attribute__((aligned(16))) T ld[2][kRows][kFewPitch], lw[2][kFewEdge][kFewPitch], lx[kRows][kFewPitch];
+  __shared__ float added[kThreads / 8][kFewEdge];
+  using Raw = typename Eight<T>::type;
+  int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
+  int const row = threadIdx.x / 8, piece = threadIdx.x % 8 * 8;  // of the first of a thread's pieces; the others lie 32 rows on
+  int64_t const blocks = (w.depth + kFewEdge - 1) / kFewEdge, c0 = blockIdx.x % blocks * kFewEdge, part = blockIdx.x / blocks;
+  int64_t const first = part * w.part, last = first + w.part < w.n ? first + w.part : w.n;
+  bool const sum_bias = w.bias_grad && c0 == 0;
+
+  // a piece of row i of `rows`, at column j of `cols`: zeros outside
+  auto const load = [](Rows<const T> const& from, int64_t i, int64_t rows, int64_t j, int64_t cols) {
+    Raw v{};
+    if (i < rows && j < cols) {
+      v = load_row8<T>(from.row(i), j, cols);
+      settle_row8<T>(v, j, cols);
+    }
+    return v;
+  };
+  Raw vg[kEach], vz[kEach], vw[2];
+  auto const ask = [&](int64_t r0) {
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+      vg[u] = load(w.grad, row + u * 32, w.m, r0 + piece, w.n);
+      if (w.z) vz[u] = load(w.z, row + u * 32, w.m, r0 + piece, w.n);
+    }
+    if (w.x_grad) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) vw[u] = load(w.weight, r0 + row + u * 32, w.n, c0 + piece, w.depth);
+    }
+  };
+  ask(first);
+#pragma unroll
+  for (int u = 0; u < kEach; ++u) *reinterpret_cast<Raw*>(&lx[row + u * 32][piece]) = load(w.x, row + u * 32, w.m, c0 + piece, w.depth);
+  f32x4_t sum[MI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) sum[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  Fragment<T> fx[KI];
+  int64_t const j = c0 + wave * 16 + lane / 16 * 4;  // the lane's four inputs
+  int buffer      = 0;
+  for (int64_t r0 = first; r0 < last; r0 += kFewEdge, buffer ^= 1) {
+    float bias[8] = {};
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+      float g[8];
+      widen<T>(g, vg[u]);
+      if (w.z) {
+        float v[8];
+        widen<T>(v, vz[u]);
+        with_activation(w.activation, [&](auto which) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) g[k] *= slope<decltype(which)::value>(v[k]);
+        });
+      }
+      Raw d;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        d[k] = static_cast<T>(g[k]);
+        bias[k] += g[k];
+      }
+      *reinterpret_cast<Raw*>(&ld[buffer][row + u * 32][piece]) = d;
+    }
+    if (w.x_grad) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) *reinterpret_cast<Raw*>(&lw[buffer][row + u * 32][piece]) = vw[u];
+    }
+    if (sum_bias) {
+      if (r0 > first) __syncthreads();  // (what was added before has been read)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) added[row][piece + k] = bias[k];
+    }
+    __syncthreads();
+    if (r0 == first) {
+#pragma unroll
+      for (int k = 0; k < KI; ++k) fx[k] = read_turned<T>(&lx[k * 32][wave * 16], lane);
+    }
+    ask(r0 + kFewEdge);  // (behind the last: zeros)
+    if (sum_bias && threadIdx.x < kFewEdge && r0 + threadIdx.x < w.n) {
+      float all = 0.f;
+      for (int q = 0; q < kThreads / 8; ++q) all += added[q][threadIdx.x];
+      w.bias_grad[r0 + threadIdx.x] = static_cast<T>(all);
+    }
+    if (w.x_grad) {
+#pragma unroll
+      for (int k = 0; k < kFewEdge / 32; ++k) {
+        Fragment<T> const fw = read_turned<T>(&lw[buffer][k * 32][wave * 16], lane);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+          Fragment<T> const fd = *reinterpret_cast<const Fragment<T>*>(&ld[buffer][i * 16 + lane % 16][k * 32 + lane / 16 * 8]);
+          sum[i]               = multiply(fw, fd, sum[i]);  // (a lane has four inputs of a row)
+        }
+      }
+    }
+    if (w.weight_grad) {
+#pragma unroll
+      for (int r = 0; r < kFewEdge / 16; ++r) {
+        f32x4_t of_weight = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KI; ++k) of_weight = multiply(fx[k], read_turned<T>(&ld[buffer][k * 32][r * 16], lane), of_weight);
+        int64_t const o = r0 + r * 16 + lane % 16;
+        if (o < w.n && j < w.depth) store4(w.weight_grad.row(o) + j, of_weight, w.depth - j);
+      }
+    }
+  }
+  if (!w.x_grad || j >= w.depth) return;
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    int64_t const of = i * 16 + lane % 16;
+    if (of >= w.m) continue;
+    if (w.sums)
+      store4(w.sums + (part * w.m + of) * w.depth + j, sum[i], w.depth - j);
+    else
+      store4(w.x_grad.row(of) + j, sum[i], w.depth - j);
+  }
+}
+
 // ------------------------------------------------------------------ before and after
 // The parts of a product that was cut along k, eight of them asked for at a time.  Where there are many results a thread has eight of
 // them, else (`spread`) a workgroup has 64 times eight, and each of its wavefronts a run of the parts.  (4 parts of 4096 x 1024
@@ -542,6 +708,8 @@ struct Join {
   int64_t parts, m, n;
   Epilogue<T> end;
   bool spread;
+  // workgroups
+  int64_t blocks() const { return spread ? (m * ((n + 7) / 8) + kWave - 1) / kWave : (m * ((n + 7) / 8) + kThreads - 1) / kThreads; }
   __device__ __forceinline__ void add(float (&z)[8], int64_t i, int64_t j, int64_t first, int64_t last) const
   {
 #pragma unroll 8
@@ -579,6 +747,12 @@ struct Join {
     end.finish(z, typename Epilogue<T>::Columns(end, j, n), i, j, n);
   }
 };
+
+template <typename T>
+Join<T> join_of(const float* sums, int64_t parts, int64_t m, int64_t n, Epilogue<T> const& end)
+{
+  return Join<T>{sums, parts, m, n, end, m * ((n + 7) / 8) < 256 * static_cast<int64_t>(device_cus())};
+}
 
 // The parts of the sums of columns: a workgroup 64 columns, a wavefront a run of parts.
 template <typename T>
@@ -1016,10 +1190,8 @@ struct Product {
     else
       launch_as<false, false>(stream);
   }
-  int64_t eights() const { return m * ((n + 7) / 8); }
-  bool spread() const { return eights() < 256 * device_cus(); }
-  Join<T> join() const { return Join<T>{sums, plan.parts, m, n, end, spread()}; }
-  int64_t join_blocks() const { return wanted() && sums ? (spread() ? (eights() + kWave - 1) / kWave : blocks_of(eights())) : 0; }
+  Join<T> join() const { return join_of(sums, plan.parts, m, n, end); }
+  int64_t join_blocks() const { return wanted() && sums ? join().blocks() : 0; }
 };
 
 template <typename T>
@@ -1068,11 +1240,76 @@ nvtext_amd_status linear(Rows<const T> x, Rows<const T> weight, int64_t m, int64
   return NVTEXT_AMD_SUCCESS;
 }
 
+// The parts of the outputs that few_rows_backward_kernel takes the least time with, by this measure: so much for 64 outputs, twice
+// as many workgroups at a time as there are CUs, and a launch that joins the parts.
+inline int64_t few_rows_parts(int64_t m, int64_t n, int64_t depth, bool slopes)
+{
+  double const step = (slopes ? 1.6 : 1.2) * (m <= 32 ? 1 : m <= 64 ? 1.3 : 1.8);
+  int64_t const blocks = (depth + kFewEdge - 1) / kFewEdge, steps = (n + kFewEdge - 1) / kFewEdge;
+  int64_t best = 1;
+  double least = 1e300;
+  for (int64_t parts = 1; parts <= std::min<int64_t>(steps, 64); ++parts) {
+    int64_t const each = (steps + parts - 1) / parts;
+    if ((steps + each - 1) / each != parts) continue;
+    double const time = step * static_cast<double>(each * ((blocks * parts + 2 * device_cus() - 1) / (2 * device_cus()))) + (parts > 1 ? 5 + parts * m * depth * 8e-6 / 5 : 0);
+    if (time < least) {
+      least = time;
+      best  = parts;
+    }
+  }
+  return best;
+}
+
+// Whether few_rows_backward_kernel takes less time than tiles.  (d is made once for every 64 inputs, which many weights make dear.  64 rows: 576 x 1064
+// weights with gelu 12.8 us against 33.8, 4096 x 4096 45 against 54, 8192 x 8192 150 against 117; 96 rows: 17.6 against 24.5, 1024 x 1024 18.5 against 19.5,
+// 4096 x 4096 65 against 49.)
+inline bool few_rows_backward_is_faster(int64_t m, int64_t n, int64_t depth)
+{
+  if (m <= 64) return n * depth <= (int64_t{1} << 31) / m;
+  return m <= 128 && n * depth < (1 << 20);
+}
+
+template <typename T>
+nvtext_amd_status few_rows_backward(FewRowsBackward<T> w, Mr const& mr, hipStream_t stream)
+{
+  int64_t const steps = (w.n + kFewEdge - 1) / kFewEdge, parts = few_rows_parts(w.m, w.n, w.depth, static_cast<bool>(w.z));
+  w.parts             = static_cast<int32_t>(parts);
+  w.part              = (steps + parts - 1) / parts * kFewEdge;
+  bool const join     = w.x_grad && parts > 1;
+  Temp const sums(mr, join ? static_cast<size_t>(parts) * static_cast<size_t>(w.m * w.depth) * sizeof(float) : 0);
+  if (!sums.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
+  if (join) w.sums = sums.template as<float>();
+  dim3 const grid(static_cast<unsigned>((w.depth + kFewEdge - 1) / kFewEdge * parts));
+  {
+    ProfileScope const scope("linear_few_rows_backward", stream);
+    if (w.m <= 16)
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_backward_kernel<T, 1>), grid, dim3(kThreads), 0, stream, w);
+    else if (w.m <= 32)
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_backward_kernel<T, 2>), grid, dim3(kThreads), 0, stream, w);
+    else if (w.m <= 64)
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_backward_kernel<T, 4>), grid, dim3(kThreads), 0, stream, w);
+    else
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_backward_kernel<T, 8>), grid, dim3(kThreads), 0, stream, w);
+  }
+  if (join) {
+    ProfileScope const scope("linear_join_backward", stream);
+    Join<T> const j = join_of(w.sums, parts, w.m, w.depth, Epilogue<T>{{nullptr, 0}, {nullptr, 0}, w.x_grad, {nullptr, 0}, NVTEXT_AMD_ACTIVATION_NONE});
+    hipLaunchKernelGGL(join_kernel<T>, dim3(static_cast<unsigned>(j.blocks())), dim3(kThreads), 0, stream, j, j.blocks(), Join<T>{}, 0, JoinColumns<T>{});
+  }
+  return NVTEXT_AMD_SUCCESS;
+}
+
 // The gradients that are wanted (of those of x and the weights, whose `out` has data).
 template <typename T>
 nvtext_amd_status linear_backward(Rows<const T> grad, Rows<const T> x, Rows<const T> weight, int64_t m, int64_t n, int64_t depth, int activation, Rows<const T> z, Rows<T> x_grad,
                                   Rows<T> weight_grad, T* bias_grad, Mr const& mr, hipStream_t stream)
 {
+  if constexpr (sizeof(T) == 2) {
+    if (m > 0 && n > 0 && depth > 0 && few_rows_backward_is_faster(m, n, depth))
+      return few_rows_backward(FewRowsBackward<T>{grad, activation != NVTEXT_AMD_ACTIVATION_NONE ? z : Rows<const T>{nullptr, 0}, x, weight, x_grad, weight_grad, bias_grad, activation, m, n, depth, 0,
+                                                  0, nullptr},
+                               mr, stream);
+  }
   auto const plain = [](Rows<T> out) { return Epilogue<T>{{nullptr, 0}, {nullptr, 0}, out, {nullptr, 0}, NVTEXT_AMD_ACTIVATION_NONE}; };
   bool const slopes = activation != NVTEXT_AMD_ACTIVATION_NONE;
   // x_grad (m x depth) = d * weight, weight_grad (n x depth) = d^T * x

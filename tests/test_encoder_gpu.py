@@ -418,6 +418,15 @@ def test_linear_backward(dtype, m, k, n, pad, activation):
     assert all(torch.equal(a, b) for a, b in zip(got, again))
 
 
+# few rows and many outputs or inputs, which are cut into parts; the most rows that are few, and one more
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("m,k,n,pad", [(7, 64, 6400, 0), (33, 100, 3001, 1), (48, 3000, 70, 0), (63, 130, 2049, 3), (64, 72, 64, 8), (96, 200, 1500, 0), (127, 9, 700, 1), (128, 1000, 1048, 0),
+                                       (128, 1024, 1032, 0), (100, 1101, 1003, 0)])
+@pytest.mark.parametrize("activation", ["none", "relu", "gelu_tanh", "silu"])
+def test_linear_backward_few_rows(dtype, m, k, n, pad, activation):
+    test_linear_backward(dtype, m, k, n, pad, activation)
+
+
 @pytest.mark.parametrize("activation", ACTIVATIONS[1:])
 def test_linear_backward_activations(activation):
     rng = np.random.default_rng(12)
