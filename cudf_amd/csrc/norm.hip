@@ -98,11 +98,11 @@ __device__ __forceinline__ float row_sum(float v, float* lds)
 }
 
 // A row of `cols` values over LANES lanes with BLOCKS times eight values each.
-constexpr int threads_of(int lanes) { return lanes > kThreads ? lanes : kThreads; }
+constexpr int threads_of(int lanes, int threads) { return lanes > threads ? lanes : threads; }
 
-template <int LANES, int BLOCKS>
+template <int LANES, int BLOCKS, int THREADS = kThreads>
 struct Shape {
-  static constexpr int kThreadsHere = threads_of(LANES);
+  static constexpr int kThreadsHere = threads_of(LANES, THREADS);
   static constexpr int kRows        = kThreadsHere / LANES;  // that a workgroup has at a time
   static constexpr int kCols        = LANES * BLOCKS * 8;        // at most
   static constexpr int kWaves       = LANES > kWave ? LANES / kWave : 1;
@@ -119,7 +119,7 @@ struct Shape {
 // after the other and keeps the weights.  Bound by memory: 32768 rows of 1024 16-bit values with dropout and residual 48 us,
 // 5.6 TB/s; the generator's 60 instructions for eight values are hidden.
 template <typename T, int LANES, int BLOCKS>
-__global__ void __launch_bounds__(threads_of(LANES))
+__global__ void __launch_bounds__(threads_of(LANES, kThreads))
 layer_norm_kernel(Rows<const T> x, Rows<const T> residual, Weights weight, Weights bias, float eps, Dropout d, Rows<T> out, Rows<T> sum, float* mean_out,
                   float* rstd_out, int64_t rows, int64_t cols)
 {
@@ -249,20 +249,30 @@ struct WeightGrads {
       store8(static_cast<T*>(which == 0 ? weight : bias) + j, f, cols - j);
     }
   }
+  template <typename T>
+  __device__ __forceinline__ void store_one(int which, float f, int64_t j, int64_t cols) const
+  {
+    if (gridDim.x > 1)
+      parts[(which * static_cast<int64_t>(gridDim.x) + blockIdx.x) * cols + j] = f;
+    else if (type == NVTEXT_AMD_TYPE_FLOAT32)
+      static_cast<float*>(which == 0 ? weight : bias)[j] = f;
+    else
+      static_cast<T*>(which == 0 ? weight : bias)[j] = static_cast<T>(f);
+  }
 };
 
 // The gradient of rows that fit into registers, read once.  A lane adds up grad * h and grad for its columns, the workgroup's rows
 // are added up in order in the end.  Bound by memory: 20011 rows of 1536 16-bit values with dropout 51 us, 4.8 TB/s, and 7 us
 // for the parts of 1024 workgroups.
-template <typename T, int LANES, int BLOCKS>
-__global__ void __launch_bounds__(threads_of(LANES))
+template <typename T, int LANES, int BLOCKS, int THREADS>
+__global__ void __launch_bounds__(threads_of(LANES, THREADS))
 layer_norm_backward_kernel(Rows<const T> grad, Rows<const T> sum, const float* mean_in, const float* rstd_in, Weights weight, Rows<const T> sum_grad, Dropout d, Rows<T> x_grad,
                            Rows<T> residual_grad, WeightGrads weights, int64_t rows, int64_t cols)
 {
-  using S             = Shape<LANES, BLOCKS>;
+  using S             = Shape<LANES, BLOCKS, THREADS>;
   constexpr int kRows = S::kRows;
   __shared__ float lds[2][kRows][S::kWaves];
-  __shared__ float joined[kRows > 1 ? 2 : 1][kRows > 1 ? S::kCols : 1];
+  __shared__ float joined[kRows > 1 ? kRows * S::kCols : 1];
   int const place = S::place(), lane = threadIdx.x % LANES;
   float const width = static_cast<float>(cols);
   float w[BLOCKS][8], dw[BLOCKS][8], db[BLOCKS][8];
@@ -335,32 +345,28 @@ layer_norm_backward_kernel(Rows<const T> grad, Rows<const T> sum, const float* m
     }
   }
   if (!weights.weight) return;
-#pragma unroll 1
-  for (int r = 0; r < kRows; ++r) {
-    if constexpr (kRows > 1) __syncthreads();
-    if (place != r) continue;
+  if constexpr (kRows == 1) {
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b) {
       unsigned const j = S::block(b, lane) * 8;
-      if constexpr (kRows > 1) {
-        if (r > 0) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            dw[b][k] += joined[0][j + k];
-            db[b][k] += joined[1][j + k];
-          }
-        }
-        if (r + 1 < kRows) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            joined[0][j + k] = dw[b][k];
-            joined[1][j + k] = db[b][k];
-          }
-          continue;
-        }
-      }
       weights.store<T>(0, dw[b], j, cols);
       weights.store<T>(1, db[b], j, cols);
+    }
+  } else {
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      __syncthreads();
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) joined[place * S::kCols + S::block(b, lane) * 8 + k] = which == 0 ? dw[b][k] : db[b][k];
+      __syncthreads();
+      for (int j = threadIdx.x; j < cols; j += S::kThreadsHere) {
+        float all = joined[j];
+#pragma unroll
+        for (int r = 1; r < kRows; ++r) all += joined[r * S::kCols + j];
+        weights.store_one<T>(which, all, j, cols);
+      }
     }
   }
 }
@@ -545,19 +551,22 @@ nvtext_amd_status nvtext_amd_layer_norm_backward(const nvtext_amd_matrix* grad, 
   Mr const mr{mr_, stream};
   Dropout const d    = make_dropout(p, seed, offset);
   int64_t const rows = grad->rows, cols = grad->cols;
-  // the workgroups: as many as the registers let run at a time (32768 rows of 1024 16-bit values, 3 a CU: 73 us; 4: 83), and one alone for a few rows, which then needs no parts
-  int64_t groups = 0;
-  bool wide      = false;
+  // the workgroups: as many as the registers let run at a time (32768 rows of 1024 16-bit values, 3 a CU: 73 us; 4: 83), and one
+  // alone, of twice the wavefronts, for rows that it goes through in kAlone rounds: it needs no parts and no second launch (54 rows
+  // of 192 values: 14 us for the call instead of 20)
+  constexpr int kMany = 2 * kThreads, kAlone = 6;
+  int64_t groups      = 0;
+  bool wide = false, alone = false;
   with_shape(cols, [&](auto lanes, auto blocks) {
     constexpr int L = decltype(lanes)::value, B = decltype(blocks)::value;
     wide            = L == 0;
     if constexpr (L > 0) {
-      using S = Shape<L, B>;
-      groups  = (rows + S::kRows - 1) / S::kRows;
+      groups = (rows + Shape<L, B>::kRows - 1) / Shape<L, B>::kRows;
+      alone  = rows <= kAlone * Shape<L, B, kMany>::kRows;
     } else {
       groups = std::min<int64_t>(rows, 256);
     }
-    groups = !wide && groups <= 4 ? 1 : grid_for(groups, L > kThreads ? 1 : B <= 1 ? 4 : B == 2 && grad->type != NVTEXT_AMD_TYPE_FLOAT32 ? 3 : 2);
+    groups = alone ? 1 : grid_for(groups, L > kThreads ? 1 : B <= 1 ? 4 : B == 2 && grad->type != NVTEXT_AMD_TYPE_FLOAT32 ? 3 : 2);
   });
   bool const parts = weight_grad && (wide || groups > 1);
   Temp const sums(mr, parts ? static_cast<size_t>(2 * groups * cols) * sizeof(float) : 0);
@@ -570,8 +579,15 @@ nvtext_amd_status nvtext_amd_layer_norm_backward(const nvtext_amd_matrix* grad, 
       constexpr int L = decltype(lanes)::value, B = decltype(blocks)::value;
       if constexpr (L > 0) {
         ProfileScope const scope("layer_norm_backward", stream);
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(layer_norm_backward_kernel<T, L, B>), dim3(static_cast<unsigned>(groups)), dim3(Shape<L, B>::kThreadsHere), 0, stream, rows_of<const T>(grad),
-                           rows_of<const T>(sum), mean, rstd, w, rows_of<const T>(sum_grad), d, rows_of<T>(x_grad), rows_of<T>(residual_grad), grads, rows, cols);
+        auto const launch = [&](auto kernel, int threads) {
+          hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(threads), 0, stream, rows_of<const T>(grad), rows_of<const T>(sum), mean, rstd, w, rows_of<const T>(sum_grad), d,
+                             rows_of<T>(x_grad), rows_of<T>(residual_grad), grads, rows, cols);
+        };
+        constexpr int kMost = L < kMany ? kMany : kThreads;
+        if (alone)
+          launch(layer_norm_backward_kernel<T, L, B, kMost>, Shape<L, B, kMost>::kThreadsHere);
+        else
+          launch(layer_norm_backward_kernel<T, L, B, kThreads>, Shape<L, B>::kThreadsHere);
       } else {
         if (weight_grad) {
           ProfileScope const scope("layer_norm_weights_backward", stream);
