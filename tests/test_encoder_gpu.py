@@ -147,6 +147,38 @@ def test_embedding_backward_of_many_tokens():
     assert (dp.cpu().numpy() == np.concatenate([g[:inside].reshape(rows, 7, width).sum(0), np.zeros((1, width))])).all()
 
 
+def whole_numbers(tokens, vocabulary, width=4, length=7):
+    """Gradients in whole numbers, so that every sum is exact."""
+    rng = np.random.default_rng(tokens + vocabulary)
+    ids = rng.integers(-1, vocabulary, tokens).astype(np.int32)
+    ids[:2] = vocabulary - 1, 0
+    offsets = np.arange(0, tokens + 1, length, dtype=np.int32)
+    g = rng.integers(-4, 5, (tokens, width)).astype(np.float32)
+    dt, _ = encoder.embedding_backward(column(offsets, ids), torch.from_numpy(g).cuda(), vocabulary, 0)
+    inside = int(offsets[-1])
+    known = ids[:inside] >= 0
+    want = np.stack([np.bincount(ids[:inside][known], g[:inside, k][known], vocabulary) for k in range(width)], 1)
+    assert (dt.cpu().numpy() == want).all()
+
+
+@pytest.mark.parametrize("vocabulary", [254, 255, 256, 511, 512, 1022, 1023, 1024, 65535, 65536, 262143, 262144, 1048575, 1048576])
+@pytest.mark.parametrize("tokens", [700, 9001])
+def test_embedding_backward_sizes_of_ids(vocabulary, tokens):
+    """Around the sizes at which the sort takes other digits."""
+    whole_numbers(tokens, vocabulary)
+
+
+@pytest.mark.parametrize("vocabulary", [1000, 40000, 250000])
+def test_embedding_backward_of_many_tokens_of_other_ids(vocabulary):
+    whole_numbers(256 * 2048 + 2050, vocabulary)
+
+
+@pytest.mark.parametrize("tokens", [15, 16, 17, 31, 32, 33, 32767, 32768, 32769])
+@pytest.mark.parametrize("vocabulary", [1, 3])
+def test_embedding_backward_around_chunks(tokens, vocabulary):
+    whole_numbers(tokens, vocabulary, width=8, length=1)
+
+
 # ------------------------------------------------------------------ dropout
 
 @pytest.mark.parametrize("dtype", TYPES)
