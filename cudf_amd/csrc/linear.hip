@@ -469,20 +469,6 @@ __global__ void __launch_bounds__(WAVES_M * WAVES_N * kWave, 2) tile_product_ker
   Tiles::run(problem, (LdsBytes)lds, blockIdx.x, gridDim.x);
 }
 
-// The two products of a gradient in one launch: the first `first` workgroups (of which `used` have work) take that of x, the
-// others that of the weights.
-template <typename T>
-__global__ void __launch_bounds__(256, 2) gradient_products_kernel(Problem<T> of_x, Problem<T> of_weight, int32_t first, int32_t used)
-{
-  using Tiles = TileProduct<T, true, false, 128, 128, 2, 2>;
-  __shared__ __attribute__((aligned(1024))) char lds[Tiles::kLds];
-  int32_t const block = static_cast<int32_t>(blockIdx.x);
-  if (block >= first)
-    TileProduct<T, false, false, 128, 128, 2, 2>::run(of_weight, (LdsBytes)lds, block - first, static_cast<int32_t>(gridDim.x) - first);
-  else if (block < used)
-    Tiles::run(of_x, (LdsBytes)lds, block, used);
-}
-
 // ------------------------------------------------------------------ products of few rows
 // A call for one token, or a few: nothing but the reading of the weights, which no workgroup shares.  A workgroup takes 16 outputs
 // and all values of k, its wavefronts a run of k each; the weights go from memory into the fragments of the matrix
@@ -837,10 +823,9 @@ struct Slopes {
     return rows <= 64 * across ? 1 : std::min<int64_t>((rows + 16 * across - 1) / (16 * across), 256);
   }
   int64_t workgroups() const { return (cols + 8 * lanes - 1) / (8 * lanes) * count; }
-  __device__ __forceinline__ void run(int64_t block) const
+  __device__ __forceinline__ void run(int64_t block, float (*lds)[kThreads]) const
   {
     constexpr int kWaves = kThreads / kWave, kAtOnce = 4;  // rows that a lane asks for at a time
-    __shared__ float lds[8][kThreads];
     int const across     = kWave / lanes, place = threadIdx.x / lanes, at = threadIdx.x % lanes;
     int64_t const slices = (cols + 8 * lanes - 1) / (8 * lanes), slice = block % slices, number = block / slices;
     int64_t const j      = (slice * lanes + at) * 8;
@@ -895,13 +880,31 @@ struct Slopes {
 template <typename T>
 __global__ void __launch_bounds__(kThreads) prepare_kernel(Align<T> a, int64_t first, Align<T> b, int64_t second, Slopes<T> slopes)
 {
+  __shared__ float lds[8][kThreads];
   int64_t const block = blockIdx.x;
   if (block < first)
     a.run(block);
   else if (block < first + second)
     b.run(block - first);
   else
-    slopes.run(block - first - second);
+    slopes.run(block - first - second, lds);
+}
+
+// The two products of a gradient in one launch: the first `first` workgroups (of which `used` have work) take that of x, those up to
+// `last` that of the weights, the others, if any, the sums of the columns (where d is grad, so that nothing waits for them: a
+// launch less: 4848 x 64 x 320 16 us instead of 20).
+template <typename T>
+__global__ void __launch_bounds__(256, 2) gradient_products_kernel(Problem<T> of_x, Problem<T> of_weight, int32_t first, int32_t used, int32_t last, Slopes<T> slopes)
+{
+  using Tiles = TileProduct<T, true, false, 128, 128, 2, 2>;
+  __shared__ __attribute__((aligned(1024))) char lds[Tiles::kLds];
+  int32_t const block = static_cast<int32_t>(blockIdx.x);
+  if (block >= last)
+    slopes.run(block - last, reinterpret_cast<float(*)[kThreads]>(lds));
+  else if (block >= first)
+    TileProduct<T, false, false, 128, 128, 2, 2>::run(of_weight, (LdsBytes)lds, block - first, last - first);
+  else if (block < used)
+    Tiles::run(of_x, (LdsBytes)lds, block, used);
 }
 
 // ------------------------------------------------------------------ products of 32-bit types
@@ -1338,20 +1341,21 @@ nvtext_amd_status linear_backward(Rows<const T> grad, Rows<const T> x, Rows<cons
   Slopes<T> const act{grad, slopes ? z : Rows<const T>{nullptr, 0}, activation, m, n, d, lanes, count, sums ? temp.template part<float>(1) : nullptr, sums ? nullptr : bias_grad};
   int64_t const first = blocks_of(a.rows * ((a.cols + 7) / 8)), second = blocks_of(b.rows * ((b.cols + 7) / 8));
   int64_t const third = write_d || bias_grad ? act.workgroups() : 0;
-  if (first + second + third > 0) {
+  bool both = false;  // in one launch
+  if constexpr (sizeof(T) == 2) both = of_x.wanted() && of_weight.wanted() && of_x.plan.tile == Tile::k128 && of_weight.plan.tile == Tile::k128;
+  bool const sums_beside = both && !write_d && first + second == 0;
+  if (first + second + third > 0 && !sums_beside) {
     ProfileScope const scope("linear_prepare_backward", stream);
     hipLaunchKernelGGL(prepare_kernel<T>, dim3(static_cast<unsigned>(first + second + third)), dim3(kThreads), 0, stream, a, first, b, second, act);
   }
   if (of_x.bytes_sums()) of_x.sums = temp.template part<float>(4);
   if (of_weight.bytes_sums()) of_weight.sums = temp.template part<float>(5);
-  bool both = false;  // in one launch
   if constexpr (sizeof(T) == 2) {
-    both = of_x.wanted() && of_weight.wanted() && of_x.plan.tile == Tile::k128 && of_weight.plan.tile == Tile::k128;
     if (both) {
       ProfileScope const scope("linear_products_backward", stream);
-      int64_t const used = of_x.workgroups(), from = (used + 7) / 8 * 8;  // (workgroups go to the eight XCDs in turn)
-      hipLaunchKernelGGL(gradient_products_kernel<T>, dim3(static_cast<unsigned>(from + of_weight.workgroups())), dim3(256), 0, stream, of_x.problem(), of_weight.problem(),
-                         static_cast<int32_t>(from), static_cast<int32_t>(used));
+      int64_t const used = of_x.workgroups(), from = (used + 7) / 8 * 8, last = from + of_weight.workgroups();  // (workgroups go to the eight XCDs in turn)
+      hipLaunchKernelGGL(gradient_products_kernel<T>, dim3(static_cast<unsigned>(last + (sums_beside ? third : 0))), dim3(kThreads), 0, stream, of_x.problem(), of_weight.problem(),
+                         static_cast<int32_t>(from), static_cast<int32_t>(used), static_cast<int32_t>(last), act);
     }
   }
   if (of_x.wanted() && !both) {
