@@ -593,3 +593,42 @@ def test_no_memory_for_temporaries():
     finally:
         mr.fail_after = None
     assert len(mr.live) == live
+
+
+# rows that one workgroup goes through alone, one round more and less, at each number of lanes
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,cols", [(191, 100), (192, 128), (193, 127), (95, 250), (96, 256), (97, 129), (47, 600), (48, 1024), (49, 2047), (12, 4000), (13, 8191), (6, 16000), (7, 16383)])
+def test_layer_norm_backward_around_one_workgroup(dtype, rows, cols):
+    test_layer_norm_backward(dtype, rows, cols, 0, 0.3, True, True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m", [3, 70])
+def test_rows_far_apart(dtype, m):
+    """Values more than 2^31 values (and 2^32 bytes) from the first: what the same rows next to each other give."""
+    stride, width = 2**31 // (m - 1) + 24, 72
+    far = torch.empty(stride * (m - 1) + 2 * width, device="cuda", dtype=dtype)
+
+    def spread(rows, at):
+        view = far.as_strided((rows.shape[0], rows.shape[1]), (stride, 1), at)
+        view.copy_(rows)
+        return view
+    x, g = torch.randn(m, width, device="cuda", dtype=dtype), torch.randn(m, width, device="cuda", dtype=dtype)
+    w, b = torch.randn(width, width, device="cuda", dtype=dtype) * 0.1, torch.randn(width, device="cuda", dtype=dtype)
+    fx, fg = spread(x, 0), spread(g, width)
+    offsets, ids = np.array([0, m], np.int32), np.arange(m)[::-1].astype(np.int32)
+    tokens = column(offsets, ids)
+
+    def same(a, c):
+        for u, v in zip(a, c):
+            assert torch.equal(u, v)
+    same([encoder.dropout(fx, 0.3, 5)], [encoder.dropout(x, 0.3, 5)])
+    same([encoder.embedding(tokens, fx, fg)], [encoder.embedding(tokens, x, g)])
+    same(encoder.embedding_backward(tokens, fx, 100, 3), encoder.embedding_backward(tokens, x, 100, 3))
+    n, s = encoder.layer_norm(fx, b, b, residual=fg, p=0.2, seed=1, keep=True)
+    n2, s2 = encoder.layer_norm(x, b, b, residual=g, p=0.2, seed=1, keep=True)
+    same([n, *s], [n2, *s2])
+    same(encoder.layer_norm_backward(fg, encoder.LayerNormSaved(fx, s.mean, s.rstd), b, 0.2, 1), encoder.layer_norm_backward(g, encoder.LayerNormSaved(x, s.mean, s.rstd), b, 0.2, 1))
+    same(encoder.linear(fx, w, b, "gelu", fg, keep=True), encoder.linear(x, w, b, "gelu", g, keep=True))
+    same([encoder.linear(w, fx)], [encoder.linear(w, x)])
+    same(encoder.linear_backward(fg, fx, w, "silu", fx), encoder.linear_backward(g, x, w, "silu", x))
