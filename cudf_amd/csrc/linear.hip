@@ -320,7 +320,12 @@ __device__ __forceinline__ void TileProduct<T, A_NEXT, B_NEXT, BM, BN, WAVES_M, 
     int32_t const column    = uniform(in_group / rows_here);
     return Item{static_cast<int64_t>(group * kGroup + in_group - column * rows_here) * BM, static_cast<int64_t>(column) * BN, p};
   };
-  auto const values_of = [&](Item const& at) { return depth - at.part * part < part ? depth - at.part * part : part; };
+  // (in 32 bits: a comparison of 64 is a vector one, whose operand was kept in memory and waited for at every item, with all loads)
+  int32_t const depth32 = static_cast<int32_t>(depth), part32 = static_cast<int32_t>(part);
+  auto const values_of  = [&](Item const& at) {
+    int32_t const rest = depth32 - at.part * part32;
+    return rest < part32 ? rest : part32;
+  };
 
   Loader<A_NEXT, BM, kWaves> load_a;
   Loader<B_NEXT, BN, kWaves> load_b;
@@ -328,7 +333,7 @@ __device__ __forceinline__ void TileProduct<T, A_NEXT, B_NEXT, BM, BN, WAVES_M, 
   Reader<T, B_NEXT, BN> const read_b(wn * NI * 16, lane);
   int32_t const first = begin + block / kXcds;
   int32_t loaded      = first;  // the item whose stages are loaded
-  int64_t left        = 0;      // values of k of it that are still to be loaded
+  int32_t left        = 0;      // values of k of it that are still to be loaded
   auto const aim = [&] {
     Item const at = place(loaded);
     load_a.aim(a, at.i0, m, at.part * part, wave, lane);
@@ -339,14 +344,14 @@ __device__ __forceinline__ void TileProduct<T, A_NEXT, B_NEXT, BM, BN, WAVES_M, 
   aim();
   // Two stages are in LDS.  Load number `p` of the next one, into place `slot`; behind the last stage of all, zeros.
   auto const before_stage = [&] {
-    if (left <= 0 && depth > 0 && loaded + stride < last) {
+    if (left <= 0 && depth32 > 0 && loaded + stride < last) {
       loaded += stride;
       aim();
     }
   };
   auto const load = [&](int slot, int p) {
     LdsBytes const to = stages + slot * kStage;
-    int const here    = static_cast<int>(left < 0 ? 0 : left < kStageK ? left : kStageK);
+    int const here    = uniform(left < 0 ? 0 : left < kStageK ? left : kStageK);
     if (p < BM / 8 / kWaves)
       load_a.load(to, here, wave, p);
     else
@@ -421,7 +426,7 @@ __device__ __forceinline__ void TileProduct<T, A_NEXT, B_NEXT, BM, BN, WAVES_M, 
   int slot = 0;  // of the stage that is multiplied
   for (int32_t item = first; item < last; item += stride) {
     Item const at   = place(item);
-    int const steps = static_cast<int>((values_of(at) + kStageK - 1) / kStageK);
+    int const steps = (values_of(at) + kStageK - 1) / kStageK;
     for_each<MI * NI>([&](auto q) { sum[decltype(q)::value / NI][decltype(q)::value % NI] = f32x4_t{0.f, 0.f, 0.f, 0.f}; });
     for (int t = 0; t < steps; ++t) {
       step(f[0], f[1], slot, std::false_type{});
@@ -1130,7 +1135,7 @@ struct Product {
   float* sums = nullptr;
 
   bool wanted() const { return m > 0 && n > 0; }
-  bool fits() const { return (m + 127) / 128 * ((n + 127) / 128) <= INT32_MAX / 64; }
+  bool fits() const { return (m + 127) / 128 * ((n + 127) / 128) <= INT32_MAX / 64 && depth <= INT32_MAX - (1 << 20); }
   void make_plan()
   {
     if constexpr (sizeof(T) == 4) {
