@@ -1109,17 +1109,18 @@ inline Plan plan_product32(int64_t m, int64_t n, int64_t depth)
   return best;
 }
 
-// Whether few_rows_kernel takes less time than tiles: microseconds of either, fitted to calls of 1 to 64 rows with 1024 to 8192
-// inputs and outputs.  It goes through k in one workgroup for 16 outputs, which takes longer with every 16 rows; tiles cost a launch
-// more, and then read the weights as fast as memory gives them.  (16 rows: 1024 to 4096 4.9 us against 11.5, 4096 to 1024 10.5
-// against 19.5, 8192 to 8192 44 against 34; 64 rows: 8.3 against 12.3, 21 against 18, 84 against 38.)
-inline bool few_rows_are_faster(int64_t m, int64_t n, int64_t depth)
+// Whether few_rows_kernel takes less time than tiles: microseconds of either, fitted to calls of 1 to 64 rows with 64 to 8192
+// inputs and outputs.  It goes through k in one workgroup for 16 outputs, which takes longer with every 16 rows; tiles may be cut along k and
+// joined, and read the weights as fast as memory gives them.  Rows that tiles cannot read are copied for them, and read at half the rate here.
+// (16 rows: 1024 to 4096 5.5 us against 9.9, 4096 to 1024 11.5 against 10.5, 8192 to 8192 36 against 29, 2051 to 1003 13.5 against 14.7; 64 rows: 8.6 against 10.6,
+// 21 against 12, 76 against 31, 25 against 16.)
+inline bool few_rows_are_faster(int64_t m, int64_t n, int64_t depth, bool aligned)
 {
   if (m > 64) return false;
   double const by_16 = m <= 16 ? 1 : m <= 32 ? 2 : 4, thousands = depth / 1024.0;
   double const few   = 3 + 0.95 * thousands * (1 + by_16) * static_cast<double>((n + 16 * 256 - 1) / (16 * 256));
-  double const tiles = std::max(11 + thousands, static_cast<double>(n) * depth * 2 / 4.2e6);
-  return few < tiles;
+  double const tiles = 2 + std::max(8.5 + 0.7 * thousands, static_cast<double>(n) * depth * 2 / 4.6e6);  // (2: memory for the parts)
+  return aligned ? few < tiles : 1.9 * few < tiles + 5;
 }
 
 inline int64_t blocks_of(int64_t work) { return (work + kThreads - 1) / kThreads; }
@@ -1228,11 +1229,11 @@ void launch_few_rows(Rows<const T> x, Rows<const T> weight, int64_t m, int64_t n
 template <typename T>
 nvtext_amd_status linear(Rows<const T> x, Rows<const T> weight, int64_t m, int64_t n, int64_t depth, Epilogue<T> const& end, Mr const& mr, hipStream_t stream)
 {
-  if (few_rows_are_faster(m, n, depth)) {
+  Product<T> p{{x, true}, {weight, true}, m, n, depth, end};
+  if (few_rows_are_faster(m, n, depth, sizeof(T) == 4 || (p.a.is_aligned(m, depth) && p.b.is_aligned(n, depth)))) {
     launch_few_rows(x, weight, m, n, depth, end, stream);
     return NVTEXT_AMD_SUCCESS;
   }
-  Product<T> p{{x, true}, {weight, true}, m, n, depth, end};
   if (!p.fits()) return fail(NVTEXT_AMD_OVERFLOW, "the product is too large");
   p.make_plan();
   TempParts<3> const temp(mr, {p.bytes_a(), p.bytes_b(), p.bytes_sums()}, p.bytes_a() + p.bytes_b() + p.bytes_sums() > 0);

@@ -262,8 +262,8 @@ struct WeightGrads {
 };
 
 // The gradient of rows that fit into registers, read once.  A lane adds up grad * h and grad for its columns, the workgroup's rows
-// are added up in order in the end.  Bound by memory: 20011 rows of 1536 16-bit values with dropout 51 us, 4.8 TB/s, and 7 us
-// for the parts of 1024 workgroups.
+// are added up in order in the end.  Bound by memory: 20011 rows of 1536 16-bit values with dropout 56 us, 4.4 TB/s, and 5 us
+// for the parts of 512 workgroups.
 template <typename T, int LANES, int BLOCKS, int THREADS>
 __global__ void __launch_bounds__(threads_of(LANES, THREADS))
 layer_norm_backward_kernel(Rows<const T> grad, Rows<const T> sum, const float* mean_in, const float* rstd_in, Weights weight, Rows<const T> sum_grad, Dropout d, Rows<T> x_grad,
