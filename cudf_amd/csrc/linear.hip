@@ -127,9 +127,11 @@ struct Epilogue {
 //           of k) lies at c ^ (i & 7): the rows that a fragment reads at one c are spread over all banks.
 //   else:   value k has EXT * 2 bytes, its units of 16 rows (32 bytes) lie at u ^ (k & 3 | (k >> 3 & 1) << 2), for the same reason;
 //           a fragment is read by the transposing load, four values of k at a time.
-// What lies outside the operands is read as zeros: its offset lies beyond the buffer's range (at most 256 lines of 2^22 bytes).
+// What lies outside the operands is read as zeros: its offset lies beyond the buffer's range, which is at most 2^31 bytes: the lines
+// of a tile (K_NEXT) or of a stage, so lines of more values than most_line() allows are not for these loads (product_kernel has 64 bits).
 constexpr int kStageK     = 64;
 constexpr uint32_t kFar   = 0x80000000u;  // an offset outside every buffer, whatever is added for a row of the tile
+constexpr int64_t most_line(int64_t lines) { return (int64_t{1} << 31) / (2 * lines); }  // values, of `lines` lines at a time
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 template <typename T>
@@ -917,15 +919,16 @@ __global__ void __launch_bounds__(256, 2) gradient_products_kernel(Problem<T> of
 // that plain loads through registers, one stage of 16 values of k ahead, keep up, and rows may lie anyhow.  A stage lies in
 // LDS as [k][row], lines 16 banks apart from each other: the four lines that a fragment is read from take all 64.
 // Bound by the matrix cores: 8192 x 1024 outputs of 4096 values 600 us, 114 TFLOP/s of 157 (a product of plain additions and
-// multiplications in tiles of 64 x 64: 1440).
+// multiplications in tiles of 64 x 64: 1440).  16-bit types whose lines are too wide for load_to_lds (4 million values and more) are
+// widened on their way and multiplied here: places are counted in 64 bits.
 constexpr int kStage32 = 16;
 
-template <bool K_NEXT, int EXT>
+template <typename T, bool K_NEXT, int EXT>
 struct Loader32 {
   static constexpr int kPieces = EXT * kStage32 / 4 / kThreads;  // of four values a thread
   static constexpr int kLine   = EXT / 4;                        // (not K_NEXT) threads that a value of k takes
   static constexpr int kStride = EXT + 16;                       // of a line in LDS
-  typedef float Four __attribute__((ext_vector_type(4), aligned(4)));
+  typedef T Four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
   Four v[kPieces];
   static __device__ __forceinline__ int row_of(int p) { return K_NEXT ? p * (kThreads / 4) + threadIdx.x / 4 : threadIdx.x % kLine * 4; }
   static __device__ __forceinline__ int k_of(int p) { return K_NEXT ? threadIdx.x % 4 * 4 : p * (kThreads / kLine) + threadIdx.x / kLine; }
@@ -936,8 +939,8 @@ struct Loader32 {
     for (int p = 0; p < kPieces; ++p) {
       int64_t const i = i0 + row_of(p), k = k0 + k_of(p);
       int64_t const left = K_NEXT ? (i < extent ? last - k : 0) : (k < last ? extent - i : 0);
-      const float* const at = static_cast<const float*>(side.data) + (K_NEXT ? i * side.stride + k : k * side.stride + i);
-      v[p] = Four{0.f, 0.f, 0.f, 0.f};
+      const T* const at  = static_cast<const T*>(side.data) + (K_NEXT ? i * side.stride + k : k * side.stride + i);
+      v[p]               = Four{};
       if (left >= 4) {
         v[p] = *reinterpret_cast<const Four*>(at);
       } else {
@@ -952,12 +955,12 @@ struct Loader32 {
 #pragma unroll
     for (int p = 0; p < kPieces; ++p)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) lds[(k_of(p) + (K_NEXT ? e : 0)) * kStride + row_of(p) + (K_NEXT ? 0 : e)] = v[p][e];
+      for (int e = 0; e < 4; ++e) lds[(k_of(p) + (K_NEXT ? e : 0)) * kStride + row_of(p) + (K_NEXT ? 0 : e)] = static_cast<float>(v[p][e]);
   }
 };
 
-template <bool A_NEXT, bool B_NEXT, int BN>
-__global__ void __launch_bounds__(kThreads, 2) product_kernel(Problem<float> problem)
+template <typename T, bool A_NEXT, bool B_NEXT, int BN>
+__global__ void __launch_bounds__(kThreads, 2) product_kernel(Problem<T> problem)
 {
   constexpr int BM = 128, MI = BM / 32, NI = BN / 32, kCols = NI * 16, kRowLanes = kCols / 8;  // 2 x 2 wavefronts
   constexpr int kA = kStage32 * (BM + 16), kB = kStage32 * (BN + 16);
@@ -971,8 +974,8 @@ __global__ void __launch_bounds__(kThreads, 2) product_kernel(Problem<float> pro
   int32_t const tiles_n = static_cast<int32_t>((n + BN - 1) / BN), tiles = static_cast<int32_t>((m + BM - 1) / BM) * tiles_n, part = item / tiles, tile = item % tiles;
   int64_t const i0 = static_cast<int64_t>(tile / tiles_n) * BM, j0 = static_cast<int64_t>(tile % tiles_n) * BN;
   int64_t const first = part * problem.part, last = first + problem.part < problem.depth ? first + problem.part : problem.depth;
-  Loader32<A_NEXT, BM> a;
-  Loader32<B_NEXT, BN> b;
+  Loader32<T, A_NEXT, BM> a;
+  Loader32<T, B_NEXT, BN> b;
   f32x4_t sum[MI][NI] = {};
   a.load(problem.a, i0, m, first, last);
   b.load(problem.b, j0, n, first, last);
@@ -1002,7 +1005,7 @@ __global__ void __launch_bounds__(kThreads, 2) product_kernel(Problem<float> pro
   constexpr int kUnits = kCols / 4 - 1;
   float* const mine    = &lds[0][0] + wave * 16 * kCols;
   int64_t const j      = j0 + wn * kCols + lane % kRowLanes * 8;
-  Epilogue<float>::Columns const columns(problem.end, j, n);
+  typename Epilogue<T>::Columns const columns(problem.end, j, n);
 #pragma unroll
   for (int rows = 0; rows < MI; ++rows) {
 #pragma unroll
@@ -1034,11 +1037,15 @@ struct Factor {
 
   int64_t lines(int64_t extent, int64_t depth) const { return k_next ? extent : depth; }
   int64_t cols(int64_t extent, int64_t depth) const { return k_next ? depth : extent; }
+  // the most values from a line to the next that Loader can take, of tiles of so many rows
+  int64_t most_stride(int64_t tile_rows) const { return most_line(k_next ? tile_rows : kStageK); }
   // fits what Side and Loader ask for
   bool is_aligned(int64_t extent, int64_t depth) const
   {
-    return reinterpret_cast<uintptr_t>(rows.data) % 16 == 0 && rows.stride % 8 == 0 && (padded || cols(extent, depth) % 8 == 0) && rows.stride <= (1 << 21);
+    return reinterpret_cast<uintptr_t>(rows.data) % 16 == 0 && rows.stride % 8 == 0 && (padded || cols(extent, depth) % 8 == 0) && rows.stride <= most_stride(128);
   }
+  // whether lines next to each other, as a copy has them, fit tiles of so many rows
+  bool copy_fits(int64_t extent, int64_t depth, int64_t tile_rows) const { return copy_stride(cols(extent, depth)) <= most_stride(tile_rows); }
 };
 
 // How a product is shared out: tiles of 256 x 256, 128 x 128 or 128 x 64, and so many parts of the values of k.
@@ -1057,14 +1064,14 @@ struct Plan {
 // for writing its tile; parts are written and read once more.  (4096 x 4096 x 64: 13.6 us in large tiles, 15.1 in those of 128;
 // x 4096: 111 and 131.  2048 x 2048 x 4096: 80 and 49; 128 x 4096 x 4096: 77 and 43 in one part, 31 and 21 in four.  In tiles of 128
 // and in half ones: 512 x 512 x 512 10.7 and 7.4; 2048 x 1024 x 1024 13.7 and 11.0; 4096 x 1024 x 1024 15.5 and 15.6.)  `halves`:
-// both operands have their k next to each other, which half tiles are made for.
-inline Plan plan_product(int64_t m, int64_t n, int64_t depth, bool halves)
+// both operands have their k next to each other, which half tiles are made for.  `large`: lines are not too wide for tiles of 256 rows.
+inline Plan plan_product(int64_t m, int64_t n, int64_t depth, bool halves, bool large)
 {
   int64_t const cus = device_cus(), steps = std::max<int64_t>(1, (depth + kStageK - 1) / kStageK);
-  Plan best{Tile::k256, 1, std::max<int64_t>(depth, 1)};
+  Plan best{Tile::k128, 1, std::max<int64_t>(depth, 1)};
   double least = 1e300;
   for (Tile tile : {Tile::k256, Tile::k128, Tile::k64}) {
-    if (tile == Tile::k64 && !halves) continue;
+    if (tile == Tile::k64 ? !halves : tile == Tile::k256 && !large) continue;
     for (int64_t parts = 1; parts <= std::min<int64_t>(steps, 32); ++parts) {
       int64_t const each = (steps + parts - 1) / parts, really = (steps + each - 1) / each;
       if (really != parts) continue;
@@ -1087,14 +1094,15 @@ inline Plan plan_product(int64_t m, int64_t n, int64_t depth, bool halves)
   return best;
 }
 
-// The same for 32-bit types, in tiles of 128 x 128 or 128 x 64: a stage of 16 values of k takes the matrix cores 0.9 us or half of that.
-inline Plan plan_product32(int64_t m, int64_t n, int64_t depth)
+// The same for product_kernel, in tiles of 128 x 128 or 128 x 64: a stage of 16 values of k takes the matrix cores 0.9 us or half of
+// that.  At most `most` parts.
+inline Plan plan_product32(int64_t m, int64_t n, int64_t depth, int64_t most)
 {
   int64_t const cus = device_cus(), steps = std::max<int64_t>(1, (depth + kStage32 - 1) / kStage32);
   Plan best{Tile::k128, 1, std::max<int64_t>(depth, 1)};
   double least = 1e300;
   for (Tile tile : {Tile::k128, Tile::k64}) {
-    for (int64_t parts = 1; parts <= std::min<int64_t>(steps, 32); ++parts) {
+    for (int64_t parts = 1; parts <= std::min<int64_t>(steps, most); ++parts) {
       int64_t const each = (steps + parts - 1) / parts;
       if ((steps + each - 1) / each != parts) continue;
       Plan const plan{tile, static_cast<int32_t>(parts), each * kStage32};
@@ -1132,6 +1140,7 @@ struct Product {
   int64_t m, n, depth;
   Epilogue<T> end;
   Plan plan{};
+  bool plain = sizeof(T) == 4;  // by product_kernel
   bool copy_a = false, copy_b = false;
   float* sums = nullptr;
 
@@ -1139,13 +1148,17 @@ struct Product {
   bool fits() const { return (m + 127) / 128 * ((n + 127) / 128) <= INT32_MAX / 64 && depth <= INT32_MAX - (1 << 20); }
   void make_plan()
   {
-    if constexpr (sizeof(T) == 4) {
-      plan = plan_product32(m, n, depth);
+    // (what decides follows from sizes alone: rows further apart than they are wide are copied)
+    plain = sizeof(T) == 4 || !a.copy_fits(m, depth, 128) || !b.copy_fits(n, depth, 128);
+    if (plain) {
+      // (very wide: as many parts as there are CUs, there is little else to share out)
+      plan = plan_product32(m, n, depth, sizeof(T) == 4 ? 32 : 256);
       return;
     }
-    plan   = plan_product(m, n, depth, a.k_next && b.k_next);
-    copy_a = depth > 0 && !a.is_aligned(m, depth);
-    copy_b = depth > 0 && !b.is_aligned(n, depth);
+    bool const large = a.copy_fits(m, depth, 256) && b.copy_fits(n, depth, 256);
+    plan             = plan_product(m, n, depth, a.k_next && b.k_next, large);
+    copy_a           = depth > 0 && !(a.is_aligned(m, depth) && a.rows.stride <= a.most_stride(plan.rows()));
+    copy_b           = depth > 0 && !(b.is_aligned(n, depth) && b.rows.stride <= b.most_stride(plan.rows()));
   }
   static size_t copy_bytes(Factor<T> const& f, int64_t extent, int64_t depth)
   {
@@ -1177,18 +1190,20 @@ struct Product {
   template <bool A_NEXT, bool B_NEXT>
   void launch_as(hipStream_t stream) const
   {
-    if constexpr (sizeof(T) == 4) {
+    if (plain) {
       dim3 const grid(static_cast<unsigned>(plan.tiles(m, n) * plan.parts));
       if (plan.tile == Tile::k128)
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<A_NEXT, B_NEXT, 128>), grid, dim3(kThreads), 0, stream, problem());
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<T, A_NEXT, B_NEXT, 128>), grid, dim3(kThreads), 0, stream, problem());
       else
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<A_NEXT, B_NEXT, 64>), grid, dim3(kThreads), 0, stream, problem());
-    } else if (plan.tile == Tile::k256)
-      launch_as<A_NEXT, B_NEXT, 256, 256, 2, 4>(stream);
-    else if (plan.tile == Tile::k128)
-      launch_as<A_NEXT, B_NEXT, 128, 128, 2, 2>(stream);
-    else if constexpr (A_NEXT && B_NEXT)
-      launch_as<A_NEXT, B_NEXT, 128, 64, 2, 2>(stream);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<T, A_NEXT, B_NEXT, 64>), grid, dim3(kThreads), 0, stream, problem());
+    } else if constexpr (sizeof(T) == 2) {
+      if (plan.tile == Tile::k256)
+        launch_as<A_NEXT, B_NEXT, 256, 256, 2, 4>(stream);
+      else if (plan.tile == Tile::k128)
+        launch_as<A_NEXT, B_NEXT, 128, 128, 2, 2>(stream);
+      else if constexpr (A_NEXT && B_NEXT)
+        launch_as<A_NEXT, B_NEXT, 128, 64, 2, 2>(stream);
+    }
   }
   void launch(hipStream_t stream) const
   {
@@ -1348,7 +1363,7 @@ nvtext_amd_status linear_backward(Rows<const T> grad, Rows<const T> x, Rows<cons
   int64_t const first = blocks_of(a.rows * ((a.cols + 7) / 8)), second = blocks_of(b.rows * ((b.cols + 7) / 8));
   int64_t const third = write_d || bias_grad ? act.workgroups() : 0;
   bool both = false;  // in one launch
-  if constexpr (sizeof(T) == 2) both = of_x.wanted() && of_weight.wanted() && of_x.plan.tile == Tile::k128 && of_weight.plan.tile == Tile::k128;
+  if constexpr (sizeof(T) == 2) both = of_x.wanted() && of_weight.wanted() && !of_x.plain && !of_weight.plain && of_x.plan.tile == Tile::k128 && of_weight.plan.tile == Tile::k128;
   bool const sums_beside = both && !write_d && first + second == 0;
   if (first + second + third > 0 && !sums_beside) {
     ProfileScope const scope("linear_prepare_backward", stream);
