@@ -671,7 +671,7 @@ nvtext_amd_status nvtext_amd_embedding_backward(const nvtext_amd_list_column* to
   int32_t const n           = view.count;
   int64_t const cols        = grad->cols;
   bool const small          = n <= kSmall;
-  int32_t const tiles       = (n + kTile - 1) / kTile;
+  int32_t const tiles       = static_cast<int32_t>((static_cast<int64_t>(n) + kTile - 1) / kTile);
   bool const direct         = tiles <= kDirectTiles;
   int32_t const chunk       = n <= kFewTokens ? kSmallChunk : kChunk;
   int32_t const chunks      = vocabulary > 0 ? static_cast<int32_t>((static_cast<int64_t>(n) + chunk - 1) / chunk) : 0;
@@ -721,6 +721,7 @@ nvtext_amd_status nvtext_amd_embedding_backward(const nvtext_amd_list_column* to
       sort(std::integral_constant<int, 9>{});
     else
       sort(std::integral_constant<int, 10>{});
+    NVTEXT_HIP_TRY(hipGetLastError());  // (what comes next takes the sorted tokens for rows of grad)
   }
   with_type(grad->type, [&](auto zero) {
     using T         = decltype(zero);

@@ -3,10 +3,11 @@
 Values are whole numbers whose sums stay below 2^24, so that every sum is exact and a result may differ from the formula by
 nothing but its one rounding: equality is asked for.
 """
+import numpy as np
 import pytest
 import torch
 
-from cudf_amd import encoder
+from cudf_amd import encoder, nvtext
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +58,37 @@ def test_linear_backward_of_very_wide_rows(m, n, k, activation):
         want_w = torch.cat([(d.double().t().contiguous() @ x[:, i:i + 2**18].double()).to(BF16) for i in range(0, k, 2**18)], 1)
         want_b = d.double().sum(0)
     assert torch.equal(dx, want_x.to(BF16)) and torch.equal(dw, want_w.to(BF16)) and torch.equal(db, want_b.to(BF16))
+
+
+# ------------------------------------------------------------------ embedding
+
+def test_embedding_of_as_many_tokens_as_a_column_holds():
+    n, length, vocabulary, places = 2**31 - 5, 4096, 1000, 3
+    gen = torch.Generator("cuda").manual_seed(5)
+    ids = torch.empty(n, device="cuda", dtype=torch.int32)
+    grad = torch.empty(n, 1, device="cuda", dtype=BF16)
+    pieces = [slice(i, min(i + 2**26, n)) for i in range(0, n, 2**26)]
+    for s in pieces:
+        ids[s] = torch.randint(-1, vocabulary, (s.stop - s.start,), generator=gen, device="cuda", dtype=torch.int32)
+        grad[s, 0] = torch.randint(-1, 2, (s.stop - s.start,), generator=gen, device="cuda", dtype=torch.int8).to(BF16)
+    rows = n // length  # what is behind them belongs to no row
+    offsets = torch.arange(rows + 1, device="cuda", dtype=torch.int32) * length
+    tokens = nvtext.DeviceListColumn(offsets, ids, None, rows, 0, np.dtype(np.int32), n)
+    inside = rows * length
+    want_tokens = torch.zeros(vocabulary + 1, device="cuda", dtype=torch.float64)
+    for s in pieces:
+        s = slice(s.start, min(s.stop, inside))
+        want_tokens += torch.bincount(ids[s] + 1, grad[s, 0].double(), vocabulary + 1)
+    want_places = grad[:inside, 0].view(rows, length)[:, :places].double().sum(0)
+    got_tokens, got_places = encoder.embedding_backward(tokens, grad, vocabulary, places, dtype=F32)
+    assert torch.equal(got_tokens[:, 0].double(), want_tokens[1:]) and torch.equal(got_places[:, 0].double(), want_places)
+    del grad
+    table, positions = whole((vocabulary, 1), BF16, 6, 9), whole((length, 1), BF16, 7, 9)
+    got = encoder.embedding(tokens, table, positions)
+    at = torch.arange(2**26, device="cuda") % length
+    for s in pieces:
+        count = s.stop - s.start
+        want = torch.where(ids[s] >= 0, table[ids[s].clamp(min=0).long(), 0], 0.0) + positions[at[:count], 0]
+        if s.stop > inside:
+            want[inside - s.start:] = 0
+        assert torch.equal(got[s, 0], want)
