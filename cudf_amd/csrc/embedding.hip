@@ -486,9 +486,11 @@ __global__ void __launch_bounds__(kSumThreads) embedding_sums_kernel(Sums<T, G> 
   __shared__ float lds[kSumWaves][VEC * kWave];
   int64_t const of_places = static_cast<int64_t>(s.places) * s.groups, of_chunks = (s.chunks + kSumWaves - 1) / kSumWaves;
   int64_t const of_slice = of_places + of_chunks + (static_cast<int64_t>(s.vocabulary) + kSumThreads - 1) / kSumThreads;
-  int64_t const j        = columns_of<VEC>(blockIdx.x / of_slice, s.cols);
-  int64_t at             = blockIdx.x % of_slice;
-  int const wave         = threadIdx.x / kWave;
+  int64_t const block    = block_number();
+  if (block / of_slice * kWave * VEC >= s.cols) return;
+  int64_t const j = columns_of<VEC>(block / of_slice, s.cols);
+  int64_t at      = block % of_slice;
+  int const wave  = threadIdx.x / kWave;
   if (at < of_places) {
     add_place<VEC>(s, static_cast<int32_t>(at / s.groups), static_cast<int32_t>(at % s.groups), j, lds);
   } else if (at -= of_places; at < of_chunks) {
@@ -526,8 +528,9 @@ __global__ void __launch_bounds__(kSumThreads) embedding_join_kernel(Sums<T, G> 
   int64_t const of_chunks = (s.chunks + kSumWaves - 1) / kSumWaves;
   int64_t const of_places = s.groups > 1 ? (s.places + kSumWaves - 1) / kSumWaves : 0;
   int const wave = threadIdx.x / kWave, lane = lane_id();
-  int64_t const j  = columns_of<VEC>(blockIdx.x / (of_chunks + of_places), s.cols);
-  int64_t const at = blockIdx.x % (of_chunks + of_places);
+  int64_t const slice = block_number() / (of_chunks + of_places), at = block_number() % (of_chunks + of_places);
+  if (slice * kWave * VEC >= s.cols) return;
+  int64_t const j = columns_of<VEC>(slice, s.cols);
   float f[VEC]     = {};
   if (at >= of_chunks) {
     int64_t const place = (at - of_chunks) * kSumWaves + wave;
@@ -733,7 +736,7 @@ nvtext_amd_status nvtext_amd_embedding_backward(const nvtext_amd_list_column* to
       int64_t const all = slices * (static_cast<int64_t>(places) * groups + of_chunks + (static_cast<int64_t>(vocabulary) + kSumThreads - 1) / kSumThreads);
       if (all > 0) {
         ProfileScope const scope("embedding_sums", stream);
-        dim3 const grid(static_cast<unsigned>(all)), threads(kSumThreads);
+        dim3 const grid = grid_of(all, kSumThreads), threads(kSumThreads);
         if (vec == 4)
           hipLaunchKernelGGL(HIP_KERNEL_NAME(embedding_sums_kernel<4, T, G>), grid, threads, 0, stream, s);
         else
@@ -744,7 +747,7 @@ nvtext_amd_status nvtext_amd_embedding_backward(const nvtext_amd_list_column* to
         ProfileScope const scope("embedding_join", stream);
         Sums<T, G> some = s;
         if (chunks <= 1) some.chunks = 0;
-        dim3 const grid(static_cast<unsigned>(joins)), threads(kSumThreads);
+        dim3 const grid = grid_of(joins, kSumThreads), threads(kSumThreads);
         if (vec == 4)
           hipLaunchKernelGGL(HIP_KERNEL_NAME(embedding_join_kernel<4, T, G>), grid, threads, 0, stream, some);
         else

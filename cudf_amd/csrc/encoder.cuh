@@ -5,6 +5,8 @@
 #include "../../include/nvtext_amd_encoder.h"
 #include "common.cuh"
 
+#include <algorithm>
+
 namespace nvtext_amd {
 
 using half_t = _Float16;
@@ -52,6 +54,17 @@ inline const char* bad_matrix(const nvtext_amd_matrix* m)
 }
 
 inline bool is_shape(const nvtext_amd_matrix* m, int64_t rows, int64_t cols) { return m->rows == rows && m->cols == cols; }
+
+// ------------------------------------------------------------------ workgroups
+// A dimension of a launch counts threads in 32 bits: of 2^32 and more the runtime starts what is left modulo 2^32, without an error.
+// Workgroups beyond 2^31 threads lie in several rows of the second dimension, whose last one may go on past the end.
+inline dim3 grid_of(int64_t blocks, int threads)
+{
+  int64_t const most = (int64_t{1} << 31) / threads, rows = std::max<int64_t>(1, (blocks + most - 1) / most);
+  return dim3(static_cast<unsigned>((blocks + rows - 1) / rows), static_cast<unsigned>(rows));
+}
+
+__device__ __forceinline__ int64_t block_number() { return static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x; }
 
 // ------------------------------------------------------------------ eight values
 // Rows need not begin at multiples of 16 bytes: global loads and stores of four words take any address of the element
@@ -253,9 +266,9 @@ __global__ void __launch_bounds__(512) add_parts_kernel(const float* parts, int6
   constexpr int kWaves = 512 / kWave;
   __shared__ float lds[kWaves][kWave];
   int const wave = threadIdx.x / kWave, lane = lane_id();
-  int64_t const j = static_cast<int64_t>(blockIdx.x) * kWave + lane;
+  int64_t const j = block_number() * kWave + lane;
   int64_t const each = (count + kWaves - 1) / kWaves, first = wave * each, last = first + each < count ? first + each : count;
-  parts += blockIdx.y * count * cols;
+  parts += blockIdx.z * count * cols;
   float sum = 0.f;
   if (j < cols) {
 #pragma unroll 8
@@ -266,13 +279,15 @@ __global__ void __launch_bounds__(512) add_parts_kernel(const float* parts, int6
   if (wave != 0 || j >= cols) return;
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) sum += lds[w][lane];
-  (blockIdx.y == 0 ? out : second)[j] = static_cast<T>(sum);
+  (blockIdx.z == 0 ? out : second)[j] = static_cast<T>(sum);
 }
 
 template <typename T>
 inline void launch_add_parts(const float* parts, int64_t count, int64_t cols, T* out, T* second, hipStream_t stream)
 {
-  hipLaunchKernelGGL(add_parts_kernel<T>, dim3(static_cast<unsigned>((cols + kWave - 1) / kWave), second ? 2 : 1), dim3(512), 0, stream, parts, count, cols, out, second);
+  dim3 grid = grid_of((cols + kWave - 1) / kWave, 512);
+  grid.z    = second ? 2 : 1;
+  hipLaunchKernelGGL(add_parts_kernel<T>, grid, dim3(512), 0, stream, parts, count, cols, out, second);
 }
 
 }  // namespace nvtext_amd

@@ -487,7 +487,8 @@ __global__ void __launch_bounds__(WAVES * kWave) few_rows_kernel(Rows<const T> x
   constexpr int kDeep = sizeof(T) == 4 ? (MI == 1 && WAVES < 16 ? 4 : 2) : MI == 4 ? 4 : WAVES == 16 ? 6 : 8;  // (as many as the registers hold)
   __shared__ __attribute__((aligned(16))) float lds[WAVES][MI][16][20];  // (16 outputs a row, and room against conflicts)
   int const wave = threadIdx.x / kWave, lane = lane_id();
-  int64_t const j0 = static_cast<int64_t>(blockIdx.x) * 16;
+  int64_t const j0 = block_number() * 16;
+  if (j0 >= n) return;
   const T* const w = weight.row(j0 + lane % 16 < n ? j0 + lane % 16 : n - 1);  // (outputs and rows behind the last: the last once more, not written)
   const T* rows[MI];
 #pragma unroll
@@ -581,7 +582,8 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_backward_kernel(FewRowsB
   using Raw = typename Eight<T>::type;
   int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
   int const row = threadIdx.x / 8, piece = threadIdx.x % 8 * 8;  // of the first of a thread's pieces; the others lie 32 rows on
-  int64_t const blocks = (w.depth + kFewEdge - 1) / kFewEdge, c0 = blockIdx.x % blocks * kFewEdge, part = blockIdx.x / blocks;
+  int64_t const blocks = (w.depth + kFewEdge - 1) / kFewEdge, c0 = block_number() % blocks * kFewEdge, part = block_number() / blocks;
+  if (part >= w.parts) return;
   int64_t const first = part * w.part, last = first + w.part < w.n ? first + w.part : w.n;
   bool const sum_bias = w.bias_grad && c0 == 0;
 
@@ -777,7 +779,7 @@ struct JoinColumns {
 template <typename T>
 __global__ void __launch_bounds__(kThreads) join_kernel(Join<T> a, int64_t first, Join<T> b, int64_t second, JoinColumns<T> columns)
 {
-  int64_t const block = blockIdx.x;
+  int64_t const block = block_number();
   if (block < first)
     a.run(block);
   else if (block < first + second)
@@ -883,17 +885,17 @@ struct Slopes {
   }
 };
 
-// What the products need, in one launch: `first` workgroups, `second` workgroups, and the slopes'.
+// What the products need, in one launch: `first` workgroups, `second` workgroups, and `third`, the slopes'.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) prepare_kernel(Align<T> a, int64_t first, Align<T> b, int64_t second, Slopes<T> slopes)
+__global__ void __launch_bounds__(kThreads) prepare_kernel(Align<T> a, int64_t first, Align<T> b, int64_t second, Slopes<T> slopes, int64_t third)
 {
   __shared__ float lds[8][kThreads];
-  int64_t const block = blockIdx.x;
+  int64_t const block = block_number();
   if (block < first)
     a.run(block);
   else if (block < first + second)
     b.run(block - first);
-  else
+  else if (block < first + second + third)
     slopes.run(block - first - second, lds);
 }
 
@@ -969,9 +971,10 @@ __global__ void __launch_bounds__(kThreads, 2) product_kernel(Problem<T> problem
   int64_t const m = problem.m, n = problem.n;
   int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id(), wm = wave / 2, wn = wave % 2;
   // workgroups go to the eight XCDs in turn: each takes a run of tiles
-  int32_t const items = gridDim.x, xcd = blockIdx.x % 8, per_xcd = items / 8, more = items % 8;
-  int32_t const item = xcd * per_xcd + (xcd < more ? xcd : more) + blockIdx.x / 8;
-  int32_t const tiles_n = static_cast<int32_t>((n + BN - 1) / BN), tiles = static_cast<int32_t>((m + BM - 1) / BM) * tiles_n, part = item / tiles, tile = item % tiles;
+  int32_t const tiles_n = static_cast<int32_t>((n + BN - 1) / BN), tiles = static_cast<int32_t>((m + BM - 1) / BM) * tiles_n;
+  int32_t const items = tiles * problem.parts, number = static_cast<int32_t>(block_number()), xcd = number % 8, per_xcd = items / 8, more = items % 8;
+  if (number >= items) return;
+  int32_t const item = xcd * per_xcd + (xcd < more ? xcd : more) + number / 8, part = item / tiles, tile = item % tiles;
   int64_t const i0 = static_cast<int64_t>(tile / tiles_n) * BM, j0 = static_cast<int64_t>(tile % tiles_n) * BN;
   int64_t const first = part * problem.part, last = first + problem.part < problem.depth ? first + problem.part : problem.depth;
   Loader32<T, A_NEXT, BM> a;
@@ -1145,7 +1148,7 @@ struct Product {
   float* sums = nullptr;
 
   bool wanted() const { return m > 0 && n > 0; }
-  bool fits() const { return (m + 127) / 128 * ((n + 127) / 128) <= INT32_MAX / 64 && depth <= INT32_MAX - (1 << 20); }
+  bool fits() const { return (m + 127) / 128 * ((n + 63) / 64) <= (1 << 25) && depth <= INT32_MAX - (1 << 20); }
   void make_plan()
   {
     // (what decides follows from sizes alone: rows further apart than they are wide are copied)
@@ -1191,7 +1194,7 @@ struct Product {
   void launch_as(hipStream_t stream) const
   {
     if (plain) {
-      dim3 const grid(static_cast<unsigned>(plan.tiles(m, n) * plan.parts));
+      dim3 const grid = grid_of(plan.tiles(m, n) * plan.parts, kThreads);
       if (plan.tile == Tile::k128)
         hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<T, A_NEXT, B_NEXT, 128>), grid, dim3(kThreads), 0, stream, problem());
       else
@@ -1223,7 +1226,7 @@ void launch_few_rows(Rows<const T> x, Rows<const T> weight, int64_t m, int64_t n
 {
   using std::integral_constant;
   auto const launch = [&](auto rows_of_16, auto waves) {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, decltype(rows_of_16)::value, decltype(waves)::value>), dim3(static_cast<unsigned>((n + 15) / 16)),
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, decltype(rows_of_16)::value, decltype(waves)::value>), grid_of((n + 15) / 16, decltype(waves)::value * kWave),
                        dim3(decltype(waves)::value * kWave), 0, stream, x, weight, m, n, depth, end);
   };
   // enough wavefronts that each has about one round of loads
@@ -1257,10 +1260,10 @@ nvtext_amd_status linear(Rows<const T> x, Rows<const T> weight, int64_t m, int64
   if (p.copy_a) a = p.align(p.a, m, depth, temp.template part<T>(0));
   if (p.copy_b) b = p.align(p.b, n, depth, temp.template part<T>(1));
   int64_t const first = blocks_of(a.rows * ((a.cols + 7) / 8)), second = blocks_of(b.rows * ((b.cols + 7) / 8));
-  if (first + second > 0) hipLaunchKernelGGL(prepare_kernel<T>, dim3(static_cast<unsigned>(first + second)), dim3(kThreads), 0, stream, a, first, b, second, Slopes<T>{});
+  if (first + second > 0) hipLaunchKernelGGL(prepare_kernel<T>, grid_of(first + second, kThreads), dim3(kThreads), 0, stream, a, first, b, second, Slopes<T>{}, 0);
   if (p.plan.parts > 1) p.sums = temp.template part<float>(2);
   p.launch(stream);
-  if (p.sums) hipLaunchKernelGGL(join_kernel<T>, dim3(static_cast<unsigned>(p.join_blocks())), dim3(kThreads), 0, stream, p.join(), p.join_blocks(), Join<T>{}, 0, JoinColumns<T>{});
+  if (p.sums) hipLaunchKernelGGL(join_kernel<T>, grid_of(p.join_blocks(), kThreads), dim3(kThreads), 0, stream, p.join(), p.join_blocks(), Join<T>{}, 0, JoinColumns<T>{});
   return NVTEXT_AMD_SUCCESS;
 }
 
@@ -1303,7 +1306,7 @@ nvtext_amd_status few_rows_backward(FewRowsBackward<T> w, Mr const& mr, hipStrea
   Temp const sums(mr, join ? static_cast<size_t>(parts) * static_cast<size_t>(w.m * w.depth) * sizeof(float) : 0);
   if (!sums.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
   if (join) w.sums = sums.template as<float>();
-  dim3 const grid(static_cast<unsigned>((w.depth + kFewEdge - 1) / kFewEdge * parts));
+  dim3 const grid = grid_of((w.depth + kFewEdge - 1) / kFewEdge * parts, kThreads);
   {
     ProfileScope const scope("linear_few_rows_backward", stream);
     if (w.m <= 16)
@@ -1318,7 +1321,7 @@ nvtext_amd_status few_rows_backward(FewRowsBackward<T> w, Mr const& mr, hipStrea
   if (join) {
     ProfileScope const scope("linear_join_backward", stream);
     Join<T> const j = join_of(w.sums, parts, w.m, w.depth, Epilogue<T>{{nullptr, 0}, {nullptr, 0}, w.x_grad, {nullptr, 0}, NVTEXT_AMD_ACTIVATION_NONE});
-    hipLaunchKernelGGL(join_kernel<T>, dim3(static_cast<unsigned>(j.blocks())), dim3(kThreads), 0, stream, j, j.blocks(), Join<T>{}, 0, JoinColumns<T>{});
+    hipLaunchKernelGGL(join_kernel<T>, grid_of(j.blocks(), kThreads), dim3(kThreads), 0, stream, j, j.blocks(), Join<T>{}, 0, JoinColumns<T>{});
   }
   return NVTEXT_AMD_SUCCESS;
 }
@@ -1364,10 +1367,10 @@ nvtext_amd_status linear_backward(Rows<const T> grad, Rows<const T> x, Rows<cons
   int64_t const third = write_d || bias_grad ? act.workgroups() : 0;
   bool both = false;  // in one launch
   if constexpr (sizeof(T) == 2) both = of_x.wanted() && of_weight.wanted() && !of_x.plain && !of_weight.plain && of_x.plan.tile == Tile::k128 && of_weight.plan.tile == Tile::k128;
-  bool const sums_beside = both && !write_d && first + second == 0;
+  bool const sums_beside = both && !write_d && first + second == 0 && third < (1 << 20);  // (one dimension of the launch)
   if (first + second + third > 0 && !sums_beside) {
     ProfileScope const scope("linear_prepare_backward", stream);
-    hipLaunchKernelGGL(prepare_kernel<T>, dim3(static_cast<unsigned>(first + second + third)), dim3(kThreads), 0, stream, a, first, b, second, act);
+    hipLaunchKernelGGL(prepare_kernel<T>, grid_of(first + second + third, kThreads), dim3(kThreads), 0, stream, a, first, b, second, act, third);
   }
   if (of_x.bytes_sums()) of_x.sums = temp.template part<float>(4);
   if (of_weight.bytes_sums()) of_weight.sums = temp.template part<float>(5);
@@ -1390,7 +1393,7 @@ nvtext_amd_status linear_backward(Rows<const T> grad, Rows<const T> x, Rows<cons
   int64_t const join_x = of_x.join_blocks(), join_weight = of_weight.join_blocks(), join_columns = sums ? (n + kWave - 1) / kWave : 0;
   if (join_x + join_weight + join_columns > 0) {
     ProfileScope const scope("linear_join_backward", stream);
-    hipLaunchKernelGGL(join_kernel<T>, dim3(static_cast<unsigned>(join_x + join_weight + join_columns)), dim3(kThreads), 0, stream, of_x.join(), join_x, of_weight.join(), join_weight,
+    hipLaunchKernelGGL(join_kernel<T>, grid_of(join_x + join_weight + join_columns, kThreads), dim3(kThreads), 0, stream, of_x.join(), join_x, of_weight.join(), join_weight,
                        JoinColumns<T>{act.parts, count, n, bias_grad});
   }
   return NVTEXT_AMD_SUCCESS;

@@ -92,3 +92,74 @@ def test_embedding_of_as_many_tokens_as_a_column_holds():
         if s.stop > inside:
             want[inside - s.start:] = 0
         assert torch.equal(got[s, 0], want)
+
+
+# ------------------------------------------------------------------ launches of 2^32 threads and more
+
+def poison(*bytes_each):
+    """What is allocated next has held NaN: a result that is not written shows."""
+    torch.cuda.empty_cache()
+    held = [torch.full((n // 4,), float("nan"), device="cuda") for n in bytes_each]
+    torch.cuda.synchronize()
+    del held
+
+
+def test_embedding_backward_of_many_places():
+    rows, places, width = 32769, 131072, 1024
+    tokens = nvtext.DeviceListColumn(torch.arange(rows + 1, device="cuda", dtype=torch.int32), torch.zeros(rows, device="cuda", dtype=torch.int32), None, rows, 0,
+                                     np.dtype(np.int32), rows)
+    grad = whole((rows, width), F32, 1)
+    poison(places * width * 4, 3 * width * 4, 16 * places * width * 4 + 2**26)
+    got_tokens, got_places = encoder.embedding_backward(tokens, grad, 3, places)
+    want = grad.double().sum(0).float()
+    assert torch.equal(got_places[0], want) and (got_places[1:] == 0).all()
+    assert torch.equal(got_tokens[0], want) and (got_tokens[1:] == 0).all()
+
+
+def test_linear_of_many_rows_that_are_copied():
+    m, k = 2**31 + 5, 9
+    w, b = whole((1, k), BF16, 1), whole((1,), BF16, 2)
+    x = torch.empty(m, k, device="cuda", dtype=BF16)
+    pieces = [slice(i, min(i + 2**25, m)) for i in range(0, m, 2**25)]
+    for i, s in enumerate(pieces):
+        x[s] = whole((s.stop - s.start, k), BF16, i)
+    poison(m * 2, m * 32)
+    got = encoder.linear(x, w, b)
+    for s in pieces:
+        assert torch.equal(got[s, 0], ((x[s] * w).float().sum(1) + b.float()).to(BF16))
+
+
+def test_linear_of_many_rows():
+    m = 2**31 + 400
+    x = torch.arange(m, device="cuda", dtype=torch.int8).float().view(m, 1)
+    w, b = torch.full((1, 1), 3.0, device="cuda"), torch.ones(1, device="cuda")
+    poison(m * 4)
+    got = encoder.linear(x, w, b)
+    for i in range(0, m, 2**27):
+        assert torch.equal(got[i:i + 2**27], x[i:i + 2**27] * 3 + 1)
+
+
+def test_linear_of_many_outputs():
+    n = 2**28 + 40
+    b = whole((n,), BF16, 1, 9)
+    poison(n * 2)
+    assert torch.equal(encoder.linear(torch.empty(1, 0, device="cuda", dtype=BF16), torch.empty(n, 0, device="cuda", dtype=BF16), b)[0], b)
+
+
+def test_linear_backward_of_a_row_of_many_inputs():
+    k = 2**30 + 200
+    x, w, g = whole((1, k), BF16, 1), whole((1, k), BF16, 2), torch.full((1, 1), 3.0, device="cuda", dtype=BF16)
+    poison(k * 2, k * 2)
+    dx, dw, db = encoder.linear_backward(g, x, w)
+    assert torch.equal(dx, w * 3) and torch.equal(dw, x * 3) and db.item() == 3
+
+
+def test_layer_norm_backward_of_rows_of_many_values():
+    rows, cols = 2, 2**29 + 100
+    s, g, w = whole((rows, cols), BF16, 1), whole((rows, cols), BF16, 2), torch.ones(cols, device="cuda", dtype=BF16)
+    saved = encoder.LayerNormSaved(s, torch.zeros(rows, device="cuda"), torch.ones(rows, device="cuda"))
+    poison(cols * 4, cols * 2, cols * 2, 4 * cols * 4)
+    _, _, dw, db = encoder.layer_norm_backward(g, saved, w)
+    for i in range(0, cols, 2**27):
+        j = slice(i, i + 2**27)
+        assert torch.equal(dw[j], (g[:, j] * s[:, j]).sum(0)) and torch.equal(db[j], g[:, j].sum(0))
