@@ -1123,6 +1123,7 @@ inline Plan plan_product32(int64_t m, int64_t n, int64_t depth, int64_t most)
 // Whether few_rows_kernel takes less time than tiles: microseconds of either, fitted to calls of 1 to 64 rows with 64 to 8192
 // inputs and outputs.  It goes through k in one workgroup for 16 outputs, which takes longer with every 16 rows; tiles may be cut along k and
 // joined, and read the weights as fast as memory gives them.  Rows that tiles cannot read are copied for them, and read at half the rate here.
+// (`aligned`: by their width, not by where they lie: the two add in different orders, and results are to depend on sizes alone.)
 // (16 rows: 1024 to 4096 5.5 us against 9.9, 4096 to 1024 11.5 against 10.5, 8192 to 8192 36 against 29, 2051 to 1003 13.5 against 14.7; 64 rows: 8.6 against 10.6,
 // 21 against 12, 76 against 31, 25 against 16.)
 inline bool few_rows_are_faster(int64_t m, int64_t n, int64_t depth, bool aligned)
@@ -1248,7 +1249,7 @@ template <typename T>
 nvtext_amd_status linear(Rows<const T> x, Rows<const T> weight, int64_t m, int64_t n, int64_t depth, Epilogue<T> const& end, Mr const& mr, hipStream_t stream)
 {
   Product<T> p{{x, true}, {weight, true}, m, n, depth, end};
-  if (few_rows_are_faster(m, n, depth, sizeof(T) == 4 || (p.a.is_aligned(m, depth) && p.b.is_aligned(n, depth)))) {
+  if (few_rows_are_faster(m, n, depth, sizeof(T) == 4 || depth % 8 == 0)) {
     launch_few_rows(x, weight, m, n, depth, end, stream);
     return NVTEXT_AMD_SUCCESS;
   }

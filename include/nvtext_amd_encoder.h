@@ -8,7 +8,8 @@
  * error.  Matrices are views of the caller's memory, the results too (their sizes are known before the call);
  * temporaries come from the nvtext_amd_allocator.  No call waits for the device, and none reads a result of an earlier
  * call but what is passed to it.  A result may not overlap an input, with the exceptions named below.  Sums are held in
- * 32 bits and added in an order that depends on sizes alone, so the same inputs give the same bits.
+ * 32 bits and added in an order that depends on sizes (the embedding's gradients: on the column too) and the device's
+ * number of CUs alone, not on where matrices lie or how far apart their rows are: the same inputs give the same bits.
  */
 #ifndef NVTEXT_AMD_ENCODER_H
 #define NVTEXT_AMD_ENCODER_H

@@ -163,3 +163,36 @@ def test_layer_norm_backward_of_rows_of_many_values():
     for i in range(0, cols, 2**27):
         j = slice(i, i + 2**27)
         assert torch.equal(dw[j], (g[:, j] * s[:, j]).sum(0)) and torch.equal(db[j], g[:, j].sum(0))
+
+
+# ------------------------------------------------------------------ the same values elsewhere
+
+def elsewhere(t):
+    """The same values, one value further on and with one value between the rows."""
+    far = torch.empty(t.shape[0], t.shape[1] + 1, device="cuda", dtype=t.dtype)[:, 1:]
+    return far.copy_(t)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("m,k,n", [(1, 4096, 1024), (16, 4096, 1024), (17, 1024, 4096), (32, 2304, 1024), (48, 1536, 1003), (64, 1024, 512), (64, 2056, 300), (65, 1024, 64), (200, 768, 512),
+                                   (300, 1003, 264)])
+def test_results_do_not_depend_on_where_matrices_lie(m, k, n, dtype):
+    gen = torch.Generator("cuda").manual_seed(m + k)
+    x, w, g = (torch.randn(s, generator=gen, device="cuda").to(dtype) for s in ((m, k), (n, k), (m, n)))
+    b = torch.randn(n, generator=gen, device="cuda").to(dtype)
+    fx, fw, fg = elsewhere(x), elsewhere(w), elsewhere(g)
+    for one, other in zip(encoder.linear(x, w, b, "gelu", g, keep=True), encoder.linear(fx, fw, b, "gelu", fg, keep=True)):
+        assert torch.equal(one, other)
+    for activation in ("none", "silu"):
+        for one, other in zip(encoder.linear_backward(g, x, w, activation, g), encoder.linear_backward(fg, fx, fw, activation, fg)):
+            assert torch.equal(one, other)
+    scale = torch.randn(k, generator=gen, device="cuda").to(dtype)
+    (one, saved), (other, far) = (encoder.layer_norm(a, scale, scale, residual=a, p=0.2, seed=1, keep=True) for a in (x, fx))
+    assert torch.equal(one, other) and all(torch.equal(u, v) for u, v in zip(saved, far))
+    for one, other in zip(*(encoder.layer_norm_backward(a, encoder.LayerNormSaved(s, saved.mean, saved.rstd), scale, 0.2, 1) for a, s in ((x, saved.sum), (fx, elsewhere(saved.sum))))):
+        assert torch.equal(one, other)
+    ids = (torch.arange(m, device="cuda") % 7).int()
+    tokens = nvtext.DeviceListColumn(torch.tensor([0, m // 3, m], device="cuda", dtype=torch.int32), ids, None, 2, 0, np.dtype(np.int32), m)
+    for one, other in zip(encoder.embedding_backward(tokens, x, 9, 5), encoder.embedding_backward(tokens, fx, 9, 5)):
+        assert torch.equal(one, other)
+    assert torch.equal(encoder.embedding(tokens, w[:7], w[:5]), encoder.embedding(tokens, fw[:7], fw[:5])) and torch.equal(encoder.dropout(x, 0.3, 2), encoder.dropout(fx, 0.3, 2))
