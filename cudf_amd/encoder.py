@@ -23,6 +23,11 @@ _INT32 = np.dtype(np.int32)
 _Matrix = _capi.Matrix
 
 
+class UnevenRowsError(ValueError, RuntimeError):
+    """The rows of a tensor of more than two dimensions do not lie at equal distances (a RuntimeError as well, which is what
+    torch's view() raises for them)."""
+
+
 class LayerNormSaved(NamedTuple):
     """What layer_norm keeps for its gradient: what was normalized, and the mean and the reciprocal deviation of each row."""
     sum: torch.Tensor
@@ -50,7 +55,10 @@ def _matrix(t: torch.Tensor, name: str) -> _capi.Matrix:
     elif t.is_contiguous():
         rows, stride = t.numel() // cols if cols else shape[:-1].numel(), cols
     else:
-        u = t.view(-1, cols)  # raises where the rows are not evenly spaced
+        try:
+            u = t.view(-1, cols)
+        except RuntimeError as error:
+            raise UnevenRowsError(f"the rows of {name} must be evenly spaced") from error
         rows, stride = u.shape[0], u.stride(0)
     if rows < 2 and stride < cols:
         stride = cols
