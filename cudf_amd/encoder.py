@@ -2,7 +2,8 @@
 include/nvtext_amd_encoder.h: embedding, dropout, layer norm and linear, each with its gradient.
 
 Tensors are torch's, in HBM, of float32, float16 or bfloat16; the last dimension is contiguous, rows may lie apart.
-Tensors of more than two dimensions are taken as the rows of their last one.  As in cudf_amd.nvtext, torch owns memory and
+Tensors of more than two dimensions are taken as the rows of their last one; what belongs
+to another's rows has its shape, or has them in two dimensions.  As in cudf_amd.nvtext, torch owns memory and
 provides the stream, and every computation happens in libnvtext_amd.so: ValueError for arguments that do not fit.
 """
 from __future__ import annotations
@@ -78,6 +79,15 @@ def _like(t: torch.Tensor) -> torch.Tensor:
 def _vector(t: torch.Tensor, name: str) -> _capi.Matrix:
     if t.dim() != 1:
         raise ValueError(f"{name} must be a vector")
+    return _matrix(t, name)
+
+
+def _like_shape(t: Optional[torch.Tensor], shape, name: str) -> Optional[_capi.Matrix]:
+    """t's rows, which must be those of a tensor of `shape`: given as such or as the rows alone, in at most two dimensions."""
+    if t is None:
+        return None
+    if t.dim() > 2 and len(shape) > 2 and t.shape != shape:
+        raise ValueError(f"{name} must be of shape {tuple(shape)}, or its rows")
     return _matrix(t, name)
 
 
@@ -157,7 +167,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, eps: f
             m_total = _new(total, rows, cols)
         mean, rstd = x.new_empty(x.shape[:-1], dtype=torch.float32), x.new_empty(x.shape[:-1], dtype=torch.float32)
     st = _capi.load().nvtext_amd_layer_norm(
-        m, None if residual is None else _matrix(residual, "residual"), _vector(weight, "weight"), _vector(bias, "bias"), eps, p, seed, offset, _stream_handle(),
+        m, _like_shape(residual, x.shape, "residual"), _vector(weight, "weight"), _vector(bias, "bias"), eps, p, seed, offset, _stream_handle(),
         _new(out, rows, cols), m_total, mean.data_ptr() if keep else None, rstd.data_ptr() if keep else None)
     if st != _capi.SUCCESS:
         _raise(st)
@@ -178,7 +188,7 @@ def layer_norm_backward(grad: torch.Tensor, saved: LayerNormSaved, weight: torch
     residual_grad, weight_grad, bias_grad = _like(grad), _like(weight), _like(weight)
     x_grad = _like(grad) if p != 0 else residual_grad
     st = _capi.load().nvtext_amd_layer_norm_backward(
-        g, _matrix(saved.sum, "sum"), saved.mean.data_ptr(), saved.rstd.data_ptr(), m_weight, None if sum_grad is None else _matrix(sum_grad, "sum_grad"),
+        g, _like_shape(saved.sum, grad.shape, "sum"), saved.mean.data_ptr(), saved.rstd.data_ptr(), m_weight, _like_shape(sum_grad, grad.shape, "sum_grad"),
         p, seed, offset, _stream_handle(), _mr().struct, _new(x_grad, rows, cols) if p != 0 else None, _new(residual_grad, rows, cols),
         _new(weight_grad, 1, m_weight.cols), _new(bias_grad, 1, m_weight.cols))
     if st != _capi.SUCCESS:
@@ -203,7 +213,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     shape = (rows, outputs) if x.dim() == 2 else x.shape[:-1] + (outputs,)
     out = x.new_empty(shape)
     z = torch.empty_like(out) if keep else None
-    st = _capi.load().nvtext_amd_linear(m, w, None if bias is None else _vector(bias, "bias"), act, None if residual is None else _matrix(residual, "residual"),
+    st = _capi.load().nvtext_amd_linear(m, w, None if bias is None else _vector(bias, "bias"), act, _like_shape(residual, shape, "residual"),
                                         _stream_handle(), _mr().struct, _new(out, rows, outputs), _new(z, rows, outputs) if keep else None)
     if st != _capi.SUCCESS:
         _raise(st)
@@ -214,10 +224,11 @@ def linear_backward(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, a
                     preactivation: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(grad of x, grad of weight, grad of bias) of linear(); the residual's gradient is grad itself."""
     act = _activation(activation)
-    g, m, w = _matrix(grad, "grad"), _matrix(x, "x"), _matrix(weight, "weight")
+    m, w = _matrix(x, "x"), _matrix(weight, "weight")
+    g = _like_shape(grad, x.shape[:-1] + (w.rows,), "grad")
     x_grad, weight_grad = _like(x), _like(weight)
     bias_grad = weight.new_empty(w.rows)
-    st = _capi.load().nvtext_amd_linear_backward(g, m, w, act, None if preactivation is None else _matrix(preactivation, "preactivation"), _stream_handle(), _mr().struct,
+    st = _capi.load().nvtext_amd_linear_backward(g, m, w, act, _like_shape(preactivation, grad.shape, "preactivation"), _stream_handle(), _mr().struct,
                                                  _new(x_grad, m.rows, m.cols), _new(weight_grad, w.rows, w.cols), _new(bias_grad, 1, w.rows))
     if st != _capi.SUCCESS:
         _raise(st)
