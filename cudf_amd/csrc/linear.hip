@@ -1209,8 +1209,15 @@ struct Product {
         launch_as<A_NEXT, B_NEXT, 128, 64, 2, 2>(stream);
     }
   }
+  // what the timing record calls it
+  const char* name() const
+  {
+    if (plain) return plan.tile == Tile::k128 ? "linear_product_128" : "linear_product_64";
+    return plan.tile == Tile::k256 ? "linear_tiles_256" : plan.tile == Tile::k128 ? "linear_tiles_128" : "linear_tiles_64";
+  }
   void launch(hipStream_t stream) const
   {
+    ProfileScope const scope(name(), stream);
     if (a.k_next && b.k_next)
       launch_as<true, true>(stream);
     else if (a.k_next)
@@ -1226,6 +1233,7 @@ template <typename T>
 void launch_few_rows(Rows<const T> x, Rows<const T> weight, int64_t m, int64_t n, int64_t depth, Epilogue<T> const& end, hipStream_t stream)
 {
   using std::integral_constant;
+  ProfileScope const scope("linear_few_rows", stream);
   auto const launch = [&](auto rows_of_16, auto waves) {
     hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, decltype(rows_of_16)::value, decltype(waves)::value>), grid_of((n + 15) / 16, decltype(waves)::value * kWave),
                        dim3(decltype(waves)::value * kWave), 0, stream, x, weight, m, n, depth, end);
@@ -1261,10 +1269,16 @@ nvtext_amd_status linear(Rows<const T> x, Rows<const T> weight, int64_t m, int64
   if (p.copy_a) a = p.align(p.a, m, depth, temp.template part<T>(0));
   if (p.copy_b) b = p.align(p.b, n, depth, temp.template part<T>(1));
   int64_t const first = blocks_of(a.rows * ((a.cols + 7) / 8)), second = blocks_of(b.rows * ((b.cols + 7) / 8));
-  if (first + second > 0) hipLaunchKernelGGL(prepare_kernel<T>, grid_of(first + second, kThreads), dim3(kThreads), 0, stream, a, first, b, second, Slopes<T>{}, 0);
+  if (first + second > 0) {
+    ProfileScope const scope("linear_prepare", stream);
+    hipLaunchKernelGGL(prepare_kernel<T>, grid_of(first + second, kThreads), dim3(kThreads), 0, stream, a, first, b, second, Slopes<T>{}, 0);
+  }
   if (p.plan.parts > 1) p.sums = temp.template part<float>(2);
   p.launch(stream);
-  if (p.sums) hipLaunchKernelGGL(join_kernel<T>, grid_of(p.join_blocks(), kThreads), dim3(kThreads), 0, stream, p.join(), p.join_blocks(), Join<T>{}, 0, JoinColumns<T>{});
+  if (p.sums) {
+    ProfileScope const scope("linear_join", stream);
+    hipLaunchKernelGGL(join_kernel<T>, grid_of(p.join_blocks(), kThreads), dim3(kThreads), 0, stream, p.join(), p.join_blocks(), Join<T>{}, 0, JoinColumns<T>{});
+  }
   return NVTEXT_AMD_SUCCESS;
 }
 
@@ -1383,14 +1397,8 @@ nvtext_amd_status linear_backward(Rows<const T> grad, Rows<const T> x, Rows<cons
                          static_cast<int32_t>(from), static_cast<int32_t>(used), static_cast<int32_t>(last), act);
     }
   }
-  if (of_x.wanted() && !both) {
-    ProfileScope const scope("linear_x_backward", stream);
-    of_x.launch(stream);
-  }
-  if (of_weight.wanted() && !both) {
-    ProfileScope const scope("linear_weight_backward", stream);
-    of_weight.launch(stream);
-  }
+  if (of_x.wanted() && !both) of_x.launch(stream);
+  if (of_weight.wanted() && !both) of_weight.launch(stream);
   int64_t const join_x = of_x.join_blocks(), join_weight = of_weight.join_blocks(), join_columns = sums ? (n + kWave - 1) / kWave : 0;
   if (join_x + join_weight + join_columns > 0) {
     ProfileScope const scope("linear_join_backward", stream);
@@ -1437,10 +1445,9 @@ nvtext_amd_status nvtext_amd_linear(const nvtext_amd_matrix* x, const nvtext_amd
   Mr const mr{mr_, stream};
   nvtext_amd_status st = NVTEXT_AMD_SUCCESS;
   with_type(x->type, [&](auto zero) {
-    using T       = decltype(zero);
-    ProfileScope const scope("linear", stream);
-    st = linear<T>(rows_of<const T>(x), rows_of<const T>(weight), m, n, depth, {rows_of<const T>(bias), rows_of<const T>(residual), rows_of<T>(out), rows_of<T>(preactivation), activation},
-                   mr, stream);
+    using T = decltype(zero);
+    st      = linear<T>(rows_of<const T>(x), rows_of<const T>(weight), m, n, depth, {rows_of<const T>(bias), rows_of<const T>(residual), rows_of<T>(out), rows_of<T>(preactivation), activation},
+                        mr, stream);
   });
   if (st != NVTEXT_AMD_SUCCESS) return st;
   NVTEXT_HIP_TRY(hipGetLastError());
