@@ -1238,7 +1238,7 @@ void launch_few_rows(Rows<const T> x, Rows<const T> weight, int64_t m, int64_t n
     hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, decltype(rows_of_16)::value, decltype(waves)::value>), grid_of((n + 15) / 16, decltype(waves)::value * kWave),
                        dim3(decltype(waves)::value * kWave), 0, stream, x, weight, m, n, depth, end);
   };
-  // enough wavefronts that each has about one round of loads
+  // enough wavefronts that each has about one round of loads  (more than 32 rows of 2048 values and more go through tiles)
   auto const by_depth = [&](auto rows_of_16, auto most) {
     if (depth >= 2048)
       launch(rows_of_16, most);
@@ -1250,7 +1250,7 @@ void launch_few_rows(Rows<const T> x, Rows<const T> weight, int64_t m, int64_t n
   else if (m <= 32)
     by_depth(integral_constant<int, 2>{}, integral_constant<int, 8>{});
   else
-    by_depth(integral_constant<int, 4>{}, integral_constant<int, 8>{});
+    launch(integral_constant<int, 4>{}, integral_constant<int, 4>{});
 }
 
 template <typename T>
