@@ -1126,12 +1126,16 @@ inline Plan plan_product32(int64_t m, int64_t n, int64_t depth, int64_t most)
 // (`aligned`: by their width, not by where they lie: the two add in different orders, and results are to depend on sizes alone.)
 // (16 rows: 1024 to 4096 5.5 us against 9.9, 4096 to 1024 11.5 against 10.5, 8192 to 8192 36 against 29, 2051 to 1003 13.5 against 14.7; 64 rows: 8.6 against 10.6,
 // 21 against 12, 76 against 31, 25 against 16.)
+inline double few_rows_time(int64_t m, int64_t n, int64_t depth)
+{
+  double const by_16 = m <= 16 ? 1 : m <= 32 ? 2 : 4;
+  return 3 + 0.95 * (depth / 1024.0) * (1 + by_16) * static_cast<double>((n + 16 * 256 - 1) / (16 * 256));
+}
 inline bool few_rows_are_faster(int64_t m, int64_t n, int64_t depth, bool aligned)
 {
   if (m > 64) return false;
-  double const by_16 = m <= 16 ? 1 : m <= 32 ? 2 : 4, thousands = depth / 1024.0;
-  double const few   = 3 + 0.95 * thousands * (1 + by_16) * static_cast<double>((n + 16 * 256 - 1) / (16 * 256));
-  double const tiles = 2 + std::max(8.5 + 0.7 * thousands, static_cast<double>(n) * depth * 2 / 4.6e6);  // (2: memory for the parts)
+  double const few   = few_rows_time(m, n, depth);
+  double const tiles = 2 + std::max(8.5 + 0.7 * (depth / 1024.0), static_cast<double>(n) * depth * 2 / 4.6e6);  // (2: memory for the parts)
   return aligned ? few < tiles : 1.9 * few < tiles + 5;
 }
 
@@ -1257,12 +1261,16 @@ template <typename T>
 nvtext_amd_status linear(Rows<const T> x, Rows<const T> weight, int64_t m, int64_t n, int64_t depth, Epilogue<T> const& end, Mr const& mr, hipStream_t stream)
 {
   Product<T> p{{x, true}, {weight, true}, m, n, depth, end};
-  if (few_rows_are_faster(m, n, depth, sizeof(T) == 4 || depth % 8 == 0)) {
-    launch_few_rows(x, weight, m, n, depth, end, stream);
-    return NVTEXT_AMD_SUCCESS;
+  bool const few = few_rows_are_faster(m, n, depth, sizeof(T) == 4 || depth % 8 == 0);
+  if (!few) {
+    if (!p.fits()) return fail(NVTEXT_AMD_OVERFLOW, "the product is too large");
+    p.make_plan();
+  } else if (sizeof(T) == 2 && depth % 8 == 0 && 0.9 * few_rows_time(m, n, depth) > 5) {
+    // rows of such a width that lie at odd places (views) are copied, where the copy takes less than reading them at half the rate
+    auto const odd = [](Rows<const T> rows) { return reinterpret_cast<uintptr_t>(rows.data) % 16 != 0 || rows.stride % 8 != 0; };
+    p.copy_a       = odd(x);
+    p.copy_b       = odd(weight);
   }
-  if (!p.fits()) return fail(NVTEXT_AMD_OVERFLOW, "the product is too large");
-  p.make_plan();
   TempParts<3> const temp(mr, {p.bytes_a(), p.bytes_b(), p.bytes_sums()}, p.bytes_a() + p.bytes_b() + p.bytes_sums() > 0);
   if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
   Align<T> a{}, b{};
@@ -1272,6 +1280,10 @@ nvtext_amd_status linear(Rows<const T> x, Rows<const T> weight, int64_t m, int64
   if (first + second > 0) {
     ProfileScope const scope("linear_prepare", stream);
     hipLaunchKernelGGL(prepare_kernel<T>, grid_of(first + second, kThreads), dim3(kThreads), 0, stream, a, first, b, second, Slopes<T>{}, 0);
+  }
+  if (few) {
+    launch_few_rows(p.a.rows, p.b.rows, m, n, depth, end, stream);
+    return NVTEXT_AMD_SUCCESS;
   }
   if (p.plan.parts > 1) p.sums = temp.template part<float>(2);
   p.launch(stream);
