@@ -36,8 +36,9 @@ struct Tokens {
 // on its own, a dozen reads one after the other, took 555 us of what is 294 now), then the rows of the tables are added up, kAtOnce
 // tokens asked for at a time.  VEC = 8 columns a lane; the lanes behind the last column take the last eight once more.  (VEC = 1 for
 // less than eight columns.)  Rows of up to 256 columns lie side by side in a wavefront, LANES lanes each: 1,276,351 tokens of 64
-// columns took 185 us with one.  Bound by memory: 512,011 tokens of 1024 16-bit values move 1.18 GB in 294 us, 4.0 TB/s, where a copy
-// reaches 5; rows of the table that occur again come from the caches, and the results are stored past them (372 us without that).
+// columns took 185 us with one.  Bound by memory: 512,011 tokens of 1024 16-bit values take 294 us and move 1.44 GB, 4.9 TB/s, where a
+// copy reaches 5 (1.18 GB are needed: some rows of the table are read again); the results are stored past the caches, which keep the
+// table (372 us without that).
 // With 8, 32 or 64 tokens a wavefront 308, 308 and 315 us, with 4 at a time 307.
 constexpr int kAtOnce = 8, kMostEach = 16;
 

@@ -96,7 +96,7 @@ struct Epilogue {
         for (int k = 0; k < 8; ++k) bias[k] = 0.f;
     }
   };
-  // PAST: the results are stored past the caches (of a large product: 322 us instead of 344 for 32768 x 1024 x 4096 with two results)
+  // PAST: the results are stored past the caches (of a large product: 342 us instead of 367 for 32768 x 1024 x 4096 with two results)
   template <bool PAST = false>
   __device__ __forceinline__ void finish(float (&z)[8], Columns const& columns, int64_t i, int64_t j, int64_t n) const
   {
@@ -286,7 +286,7 @@ struct Item {
 // A workgroup takes items of BM x BN one after the other.  WAVES_M x WAVES_N wavefronts, each with MI x NI fragments of 16 x 16.
 // The loads are a stream of stages that goes on from an item into the next: the first two stages of an item come while the
 // one before is finished and written, for which the wavefronts have LDS of their own (waiting for them anew at every item
-// cost 30 of 265 us at 32768 x 1024 x 4096).
+// made 32768 x 1024 x 4096 a ninth longer).
 template <typename T, bool A_NEXT, bool B_NEXT, int BM, int BN, int WAVES_M, int WAVES_N>
 struct TileProduct {
   static constexpr int kWaves = WAVES_M * WAVES_N, MI = BM / WAVES_M / 16, NI = BN / WAVES_N / 16;
@@ -530,8 +530,10 @@ __global__ void __launch_bounds__(WAVES * kWave) few_rows_kernel(Rows<const T> x
 // inputs and a part of the outputs, 64 of them at a time: it makes d for them (which every workgroup of the part does anew: it
 // is small), stages it and the 64 x 64 weights in LDS through registers, one stage ahead, and has of both the sums that x's gradient
 // needs, which it keeps, and the weights' gradient, which is complete after one stage.  A wavefront has 16 of the inputs.
-// Rows may lie anyhow.  Bound by launches and, of many weights, by memory: with gelu 7 x 64 x 64 5.9 us (12.6 in three
-// launches with tiles), 34 x 924 x 4928 28 (39).
+// Rows may lie anyhow.  d is rounded to the matrices' type, which is what the matrix instructions take: where there is an activation, the
+// products' gradients are off by two roundings instead of one (0.0023 of a value in bfloat16 instead of 0.0017).  The bias'
+// gradient adds d up before that.  Bound by launches and, of many weights, by memory: with gelu 7 x 64 x 64 4.5 us (11.1 in three
+// launches with tiles), 34 x 924 x 4928 26 (35).
 template <typename T>
 struct FewRowsBackward {
   Rows<const T> grad, z, x, weight;
@@ -696,7 +698,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_backward_kernel(FewRowsB
 // ------------------------------------------------------------------ before and after
 // The parts of a product that was cut along k, eight of them asked for at a time.  Where there are many results a thread has eight of
 // them, else (`spread`) a workgroup has 64 times eight, and each of its wavefronts a run of the parts.  (4 parts of 4096 x 1024
-// 20 us, spread 26; many parts of a small result 55 -> 39 us for the whole of a gradient of 34 x 924 x 4928.)
+// 19 us, spread 26; many parts of a small result 55 -> 39 us for the whole of a gradient of 34 x 924 x 4928.)
 template <typename T>
 struct Join {
   const float* sums;
@@ -810,8 +812,8 @@ struct Align {
   }
 };
 
-// d = grad * activation'(z) where it is wanted (d's rows have a multiple of 8 values, zeros behind the last), and the sums of the
-// columns of it: a workgroup takes up to 512 columns and every count-th run of rows, `lanes` lanes of a wavefront a row (fewer than
+// d = grad * activation'(z) where it is wanted, rounded as in few_rows_backward_kernel (d's rows have a multiple of 8 values, zeros
+// behind the last), and the sums of the columns of it in 32 bits: a workgroup takes up to 512 columns and every count-th run of rows, `lanes` lanes of a wavefront a row (fewer than
 // 64 for narrow rows, which lie side by side then); the sums are added up in order in the end, to the bias' gradient itself if that
 // is all (count = 1).
 template <typename T>
@@ -1064,9 +1066,9 @@ struct Plan {
 
 // The one that takes the least by this measure, in microseconds, fitted to products of 256 x 256 to 4096 x 4096 with 64 to 4096
 // values of k: a launch, then rounds of workgroups, each with so much for a stage of 64 values of k (more where all CUs are busy) and
-// for writing its tile; parts are written and read once more.  (4096 x 4096 x 64: 13.6 us in large tiles, 15.1 in those of 128;
-// x 4096: 111 and 131.  2048 x 2048 x 4096: 80 and 49; 128 x 4096 x 4096: 77 and 43 in one part, 31 and 21 in four.  In tiles of 128
-// and in half ones: 512 x 512 x 512 10.7 and 7.4; 2048 x 1024 x 1024 13.7 and 11.0; 4096 x 1024 x 1024 15.5 and 15.6.)  `halves`:
+// for writing its tile; parts are written and read once more.  (4096 x 4096 x 64: 14.7 us in large tiles, 15.3 in those of 128;
+// x 4096: 108 and 124.  2048 x 2048 x 4096: 80 and 48; 128 x 4096 x 4096: 77 and 44 in one part, 31 and 21 in four.  In tiles of 128
+// and in half ones: 512 x 512 x 512 9.3 and 7.0; 2048 x 1024 x 1024 13.2 and 10.4; 4096 x 1024 x 1024 14.7 and 14.3.)  `halves`:
 // both operands have their k next to each other, which half tiles are made for.  `large`: lines are not too wide for tiles of 256 rows.
 inline Plan plan_product(int64_t m, int64_t n, int64_t depth, bool halves, bool large)
 {
@@ -1124,8 +1126,8 @@ inline Plan plan_product32(int64_t m, int64_t n, int64_t depth, int64_t most)
 // inputs and outputs.  It goes through k in one workgroup for 16 outputs, which takes longer with every 16 rows; tiles may be cut along k and
 // joined, and read the weights as fast as memory gives them.  Rows that tiles cannot read are copied for them, and read at half the rate here.
 // (`aligned`: by their width, not by where they lie: the two add in different orders, and results are to depend on sizes alone.)
-// (16 rows: 1024 to 4096 5.5 us against 9.9, 4096 to 1024 11.5 against 10.5, 8192 to 8192 36 against 29, 2051 to 1003 13.5 against 14.7; 64 rows: 8.6 against 10.6,
-// 21 against 12, 76 against 31, 25 against 16.)
+// (16 rows: 1024 to 4096 4.2 us against 8.7, 4096 to 1024 10.0 against 9.7, 8192 to 8192 34 against 27, 2051 to 1003 12.0 against 13.5; 64 rows: 7.4 against 9.2,
+// 20 against 11, 73 against 29, 24 against 15.)
 inline double few_rows_time(int64_t m, int64_t n, int64_t depth)
 {
   double const by_16 = m <= 16 ? 1 : m <= 32 ? 2 : 4;
@@ -1315,8 +1317,8 @@ inline int64_t few_rows_parts(int64_t m, int64_t n, int64_t depth, bool slopes)
 }
 
 // Whether few_rows_backward_kernel takes less time than tiles.  (d is made once for every 64 inputs, which many weights make dear.  64 rows: 576 x 1064
-// weights with gelu 12.8 us against 33.8, 4096 x 4096 45 against 54, 8192 x 8192 150 against 117; 96 rows: 17.6 against 24.5, 1024 x 1024 18.5 against 19.5,
-// 4096 x 4096 65 against 49.)
+// weights with gelu 11.7 us against 32.5, 4096 x 4096 47 against 52, 8192 x 8192 149 against 111; 96 rows: 15.5 against 22.8, 4096 x 4096 66 against 46, and
+// 1024 x 1024, where the line is drawn, 17.2 against 17.9.)
 inline bool few_rows_backward_is_faster(int64_t m, int64_t n, int64_t depth)
 {
   if (m <= 64) return n * depth <= (int64_t{1} << 31) / m;

@@ -5,6 +5,8 @@ Tensors are torch's, in HBM, of float32, float16 or bfloat16; the last dimension
 Tensors of more than two dimensions are taken as the rows of their last one; what belongs
 to another's rows has its shape, or has them in two dimensions.  As in cudf_amd.nvtext, torch owns memory and
 provides the stream, and every computation happens in libnvtext_amd.so: ValueError for arguments that do not fit.
+Nothing is recorded for torch's autograd: a result does not require a gradient, whatever its arguments do, and the gradients are
+the calls named *_backward.
 """
 from __future__ import annotations
 
@@ -222,7 +224,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 
 def linear_backward(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, activation: str = "none",
                     preactivation: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(grad of x, grad of weight, grad of bias) of linear(); the residual's gradient is grad itself."""
+    """(grad of x, grad of weight, grad of bias) of linear(); the residual's gradient is grad itself.  grad times the activation's
+    slope is rounded to the tensors' type before it is multiplied."""
     act = _activation(activation)
     m, w = _matrix(x, "x"), _matrix(weight, "weight")
     g = _like_shape(grad, x.shape[:-1] + (w.rows,), "grad")

@@ -134,7 +134,8 @@ nvtext_amd_status nvtext_amd_linear(const nvtext_amd_matrix* x,
                                     const nvtext_amd_matrix* preactivation);
 
 /* The gradients of linear (that of the residual is grad itself): with d = grad * activation'(preactivation), rounded to
- * the type of the matrices before it is multiplied,
+ * the type of the matrices before it is multiplied (of 16-bit types and with an activation x_grad and weight_grad are off by two
+ * roundings of that type, then, instead of one),
  *   x_grad = d * weight, weight_grad = d^T * x, bias_grad = the sum over the rows of d (before it is rounded);
  * each NULL where it is not wanted.  preactivation may be NULL for NVTEXT_AMD_ACTIVATION_NONE, where d is grad. */
 nvtext_amd_status nvtext_amd_linear_backward(const nvtext_amd_matrix* grad,
