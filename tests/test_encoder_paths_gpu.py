@@ -147,3 +147,46 @@ def test_layer_norm_of_several_turns(dtype, rows, cols):
 @pytest.mark.parametrize("dtype,rows,cols", TURNS)
 def test_layer_norm_backward_of_several_turns(dtype, rows, cols):
     checks.test_layer_norm_backward(dtype, rows, cols, 0, 0.3, True, True)
+
+
+# ------------------------------------------------------------------ NaN and infinities stay where the formula has them
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("m,k,n", [(5, 72, 40), (64, 100, 301), (120, 72, 104), (300, 75, 260), (513, 72, 104), (1003, 4104, 4090), (4090, 4104, 100)])
+def test_linear_backward_keeps_rows_and_columns_apart(m, k, n, dtype):
+    g, x, w = whole((m, n), dtype, 1), whole((m, k), dtype, 2), whole((n, k), dtype, 3)
+    clean = encoder.linear_backward(g, x, w)
+    bad = g.clone()
+    bad[3], bad[:, n - 1] = float("nan"), float("inf")
+    dx, dw, db = encoder.linear_backward(bad, x, w)
+    assert dx[3].isnan().all() and db[n - 1] == float("inf") and db[:-1].isnan().all()
+    bad = g.clone()
+    bad[m - 2] = float("nan")
+    dx, dw, _ = encoder.linear_backward(bad, x, w)
+    others = torch.arange(m, device="cuda") != m - 2
+    assert torch.equal(dx[others], clean[0][others]) and dx[m - 2].isnan().all() and dw.isnan().all()
+    bad = g.clone()
+    bad[:, n - 1] = float("nan")
+    dx, dw, db = encoder.linear_backward(bad, x, w)
+    assert torch.equal(dw[:-1], clean[1][:-1]) and torch.equal(db[:-1], clean[2][:-1]) and dw[-1].isnan().all() and dx.isnan().all()
+    bad = x.clone()
+    bad[:, k - 1] = float("nan")
+    dx, dw, _ = encoder.linear_backward(g, bad, w)
+    assert torch.equal(dx, clean[0]) and torch.equal(dw[:, :-1], clean[1][:, :-1]) and dw[:, -1].isnan().all()
+    bad = w.clone()
+    bad[:, k - 1] = float("nan")
+    dx, dw, _ = encoder.linear_backward(g, x, bad)
+    assert torch.equal(dw, clean[1]) and torch.equal(dx[:, :-1], clean[0][:, :-1]) and dx[:, -1].isnan().all()
+
+
+def test_embedding_keeps_entries_apart():
+    """NaN in the gradient of a token reaches its entry and its place alone, and none where it belongs to neither."""
+    ids = torch.tensor([0, 1, 2, -1, 1, 7], device="cuda", dtype=torch.int32)
+    column = nvtext.DeviceListColumn(torch.tensor([0, 4, 5], device="cuda", dtype=torch.int32), ids, None, 2, 0, checks.np.dtype(checks.np.int32), 6)
+    g = torch.ones(6, 40, device="cuda")
+    g[2], g[3], g[5] = float("nan"), float("inf"), float("nan")
+    t, p = encoder.embedding_backward(column, g, 8, 2)
+    assert t[2].isnan().all() and t[[0, 1, 3, 4, 5, 6, 7]].sum(1).tolist() == [40, 80, 0, 0, 0, 0, 0] and p.sum(1).tolist() == [80, 40]
+    table = torch.ones(8, 40, device="cuda")
+    table[3:] = float("nan")
+    assert encoder.embedding(column, table).sum(1).tolist() == [40, 40, 40, 0, 40, 0]
