@@ -922,7 +922,7 @@ __global__ void __launch_bounds__(256, 2) gradient_products_kernel(Problem<T> of
 // The same of float, on the matrix cores' products of 16 x 16 x 4, which keep float's precision at a sixteenth of the rate: so slow
 // that plain loads through registers, one stage of 16 values of k ahead, keep up, and rows may lie anyhow.  A stage lies in
 // LDS as [k][row], lines 16 banks apart from each other: the four lines that a fragment is read from take all 64.
-// Bound by the matrix cores: 8192 x 1024 outputs of 4096 values 600 us, 114 TFLOP/s of 157 (a product of plain additions and
+// Bound by the matrix cores: 8192 x 1024 outputs of 4096 values 610 us, 113 TFLOP/s of 157 (a product of plain additions and
 // multiplications in tiles of 64 x 64: 1440).  16-bit types whose lines are too wide for load_to_lds (4 million values and more) are
 // widened on their way and multiplied here: places are counted in 64 bits.
 constexpr int kStage32 = 16;
