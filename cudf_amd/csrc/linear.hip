@@ -923,8 +923,9 @@ __global__ void __launch_bounds__(256, 2) gradient_products_kernel(Problem<T> of
 // that plain loads through registers, one stage of 16 values of k ahead, keep up, and rows may lie anyhow.  A stage lies in
 // LDS as [k][row], lines 16 banks apart from each other: the four lines that a fragment is read from take all 64.
 // Bound by the matrix cores: 8192 x 1024 outputs of 4096 values 610 us, 113 TFLOP/s of 157 (a product of plain additions and
-// multiplications in tiles of 64 x 64: 1440).  16-bit types whose lines are too wide for load_to_lds (4 million values and more) are
-// widened on their way and multiplied here: places are counted in 64 bits.
+// multiplications in tiles of 64 x 64: 1440).  16-bit types whose lines are too wide for load_to_lds (more than 2^23 values next to
+// each other in k, else 2^24) are widened on their way and multiplied here, where places are counted in 64 bits: 128 x 64 outputs of 8388672
+// values 2.0 ms (of 64 values less, in tiles, 6.5).
 constexpr int kStage32 = 16;
 
 template <typename T, bool K_NEXT, int EXT>
