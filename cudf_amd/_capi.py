@@ -43,6 +43,9 @@ EXPORTS = [
     "nvtext_amd_layer_norm_backward",
     "nvtext_amd_linear",
     "nvtext_amd_linear_backward",
+    "nvtext_amd_rotary",
+    "nvtext_amd_attention",
+    "nvtext_amd_attention_backward",
     "nvtext_amd_profile_enable",
     "nvtext_amd_profile_read",
     "nvtext_amd_profile_set_range_tiles",
@@ -132,6 +135,18 @@ class Matrix(C.Structure):
         ("rows", C.c_int64),
         ("cols", C.c_int64),
         ("stride", C.c_int64),
+        ("type", C.c_int32),
+    ]
+
+
+class Heads(C.Structure):
+    _fields_ = [
+        ("data", C.c_void_p),
+        ("tokens", C.c_int64),
+        ("heads", C.c_int64),
+        ("width", C.c_int64),
+        ("stride", C.c_int64),
+        ("head_stride", C.c_int64),
         ("type", C.c_int32),
     ]
 
@@ -259,13 +274,17 @@ def load():
     L.nvtext_amd_list_column_free.argtypes = [C.POINTER(ListColumn), C.c_void_p, C.POINTER(Allocator)]
     column, matrix, mr, ptr = C.POINTER(ListColumn), C.POINTER(Matrix), C.POINTER(Allocator), C.c_void_p
     draws = [C.c_double, C.c_uint64, C.c_uint32, ptr]
+    heads, seen = C.POINTER(Heads), [C.c_int32, ptr, ptr, ptr, C.c_int32, C.c_double]
     for f, args in ((L.nvtext_amd_embedding, [column, matrix, matrix, ptr, matrix]),
                     (L.nvtext_amd_embedding_backward, [column, matrix, ptr, mr, matrix, matrix]),
                     (L.nvtext_amd_dropout, [matrix] + draws + [matrix]),
                     (L.nvtext_amd_layer_norm, [matrix] * 4 + [C.c_double] + draws + [matrix, matrix, ptr, ptr]),
                     (L.nvtext_amd_layer_norm_backward, [matrix, matrix, ptr, ptr, matrix, matrix] + draws + [mr] + [matrix] * 4),
                     (L.nvtext_amd_linear, [matrix] * 3 + [C.c_int32, matrix, ptr, mr, matrix, matrix]),
-                    (L.nvtext_amd_linear_backward, [matrix] * 3 + [C.c_int32, matrix, ptr, mr] + [matrix] * 3)):
+                    (L.nvtext_amd_linear_backward, [matrix] * 3 + [C.c_int32, matrix, ptr, mr] + [matrix] * 3),
+                    (L.nvtext_amd_rotary, [heads, C.c_int32, ptr, ptr, ptr, C.c_int64, C.c_int32, C.c_int32, C.c_double, ptr, heads]),
+                    (L.nvtext_amd_attention, [heads] * 3 + seen + [ptr, mr, heads, ptr]),
+                    (L.nvtext_amd_attention_backward, [heads] * 5 + [ptr] + seen + [ptr, mr] + [heads] * 3)):
         f.restype = C.c_int
         f.argtypes = args
     L.nvtext_amd_profile_enable.restype = None

@@ -1,5 +1,5 @@
 """Operators between the tokenizer's column of ids and a model that learns from it, over the C ABI of
-include/nvtext_amd_encoder.h: embedding, dropout, layer norm and linear, each with its gradient.
+include/nvtext_amd_encoder.h: embedding, dropout, layer norm, linear, rotary positions and attention, each with its gradient.
 
 Tensors are torch's, in HBM, of float32, float16 or bfloat16; the last dimension is contiguous, rows may lie apart.
 Tensors of more than two dimensions are taken as the rows of their last one; what belongs
@@ -11,7 +11,8 @@ the calls named *_backward.
 from __future__ import annotations
 
 import ctypes as C
-from typing import NamedTuple, Optional, Tuple
+import math
+from typing import NamedTuple, Optional, Tuple, Union
 
 import numpy as np
 import torch
@@ -20,6 +21,8 @@ from . import _capi
 from .nvtext import DeviceListColumn, _mr, _raise, _stream_handle
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+ROTARY_LAYOUTS = {"half": 0, "interleaved": 1}
 
 _TYPES = {torch.float32: _capi.TYPE_FLOAT32, torch.float16: _capi.TYPE_FLOAT16, torch.bfloat16: _capi.TYPE_BFLOAT16}
 _INT32 = np.dtype(np.int32)
@@ -36,6 +39,13 @@ class LayerNormSaved(NamedTuple):
     sum: torch.Tensor
     mean: torch.Tensor
     rstd: torch.Tensor
+
+
+class AttentionSaved(NamedTuple):
+    """What attention keeps for its gradient: its result, and of every head of a token the logarithm of what its exponentials
+    add up to, [heads, tokens]."""
+    out: torch.Tensor
+    logsum: torch.Tensor
 
 
 def _matrix(t: torch.Tensor, name: str) -> _capi.Matrix:
@@ -236,3 +246,148 @@ def linear_backward(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, a
     if st != _capi.SUCCESS:
         _raise(st)
     return x_grad, weight_grad, bias_grad
+
+
+Rows = Union[DeviceListColumn, torch.Tensor]
+
+
+def _heads(t: torch.Tensor, name: str) -> _capi.Heads:
+    kind = _TYPES.get(t.dtype)
+    if kind is None:
+        raise ValueError(f"{name} must be float32, float16 or bfloat16")
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be of shape [tokens, heads, width]")
+    _here(t, name)
+    (tokens, heads, width), (stride, head_stride, step) = t.shape, t.stride()
+    if step != 1 and width > 1:
+        raise ValueError(f"{name} must be contiguous in its last dimension")
+    return _capi.Heads(t.data_ptr(), tokens, heads, width, stride, head_stride, kind)
+
+
+def _here(t: torch.Tensor, name: str) -> None:
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be in device memory")
+    # (the calls run on the current device's stream, and take their temporaries there)
+    if t.get_device() != torch._C._cuda_getDevice():
+        raise ValueError(f"{name} must be on the current device")
+
+
+def _int32s(t: Optional[torch.Tensor], count: Optional[int], name: str) -> Optional[int]:
+    """The address of a tensor of `count` int32 values."""
+    if t is None:
+        return None
+    _here(t, name)
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous vector of int32")
+    if count is not None and t.numel() != count:
+        raise ValueError(f"{name} must have {count} values")
+    return t.data_ptr()
+
+
+def _rows(rows: Rows) -> Tuple[int, Optional[int]]:
+    """(how many there are, the address of their offsets)."""
+    if isinstance(rows, DeviceListColumn):
+        if rows.size > 0:
+            _here(rows.offsets, "the column")
+        return rows.size, rows.offsets.data_ptr() if rows.offsets is not None else None
+    address = _int32s(rows, None, "offsets")
+    if rows.numel() == 0:
+        raise ValueError("offsets must have a value more than there are rows")
+    return rows.numel() - 1, address
+
+
+def rotary_frequencies(width: int, base: float = 10000.0, factor: float = 1.0, length: int = 0, slow: float = 1.0, fast: float = 4.0,
+                       device: Union[str, torch.device] = "cuda") -> torch.Tensor:
+    """The frequencies that rotary() takes for `width` values of a head, width / 2 of them, in radians a position: base^(-2 n / width).
+    For contexts `factor` times longer than a model has learned, all of them divided by that; or, where `length` names
+    the positions it has learned, only those that turn up to `slow` times within it, with those that turn `fast` times and
+    more left as they are and those in between passing from one to the other with their turns."""
+    if width < 2 or width % 2:
+        raise ValueError("width must be even, and at least 2")
+    if not (base > 0 and factor > 0 and math.isfinite(base) and math.isfinite(factor)):
+        raise ValueError("base and factor must be positive")
+    if length < 0 or (length and not 0 <= slow < fast):
+        raise ValueError("length must not be negative, and slow less than fast")
+    f = base ** (-np.arange(0, width, 2, dtype=np.float64) / width)
+    share = np.clip((f * length / (2 * math.pi) - slow) / (fast - slow), 0.0, 1.0) if length else 0.0  # of what is left as it is
+    return torch.from_numpy(f * share + f / factor * (1 - share)).to(device)
+
+
+def rotary(x: torch.Tensor, rows: Rows, frequencies: torch.Tensor, starts: Optional[torch.Tensor] = None, layout: str = "half", inverse: bool = False,
+           magnitude: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x, [tokens, heads, width], with the first 2 * len(frequencies) values of every head rotated in pairs by its token's position in its
+    row times the pair's frequency (float64, as rotary_frequencies() gives them), and multiplied by `magnitude`.  The pairs of
+    layout "half" are n and n + len(frequencies), those of "interleaved" 2 n and 2 n + 1.  rows: the tokenizer's column, or int32 offsets;
+    starts: int32, the position of every row's first token (of a text under way).  Query and key heads that lie next to each
+    other take one call.  inverse=True on the gradient of the result gives that of x.  out: where the result goes, x itself
+    if wanted."""
+    code = ROTARY_LAYOUTS.get(layout)
+    if code is None:
+        raise ValueError(f"layout must be one of {', '.join(ROTARY_LAYOUTS)}")
+    m = _heads(x, "x")
+    count, offsets = _rows(rows)
+    _here(frequencies, "frequencies")
+    if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not frequencies.is_contiguous():
+        raise ValueError("frequencies must be a contiguous vector of float64")
+    if out is None:
+        out = _like(x)
+    st = _capi.load().nvtext_amd_rotary(m, count, offsets, _int32s(starts, count, "starts"), frequencies.data_ptr(), frequencies.numel(), code, inverse, magnitude,
+                                        _stream_handle(), _heads(out, "out"))
+    if st != _capi.SUCCESS:
+        _raise(st)
+    return out
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rows: Rows, key_rows: Optional[Rows] = None, key_lengths: Optional[torch.Tensor] = None,
+              causal: bool = False, scale: Optional[float] = None, keep: bool = False):
+    """softmax(scale * q @ k.T) @ v of every row's tokens by themselves, head by head.  q is [tokens, heads, width] with width up to 256, k and v
+    [key tokens, a divisor of heads, width]: as many neighbouring heads of q see one of them.  Any of them may be a part of
+    another tensor (of a projection's result, viewed as heads).  rows: the tokenizer's column, or int32 offsets.
+    Keys and values of other rows than q's (those of texts under way, kept from call to call) have offsets of their own, key_rows, and
+    where these leave room for more, key_lengths, int32.  causal: the last token of a row sees all its keys, each one before it one less.
+    scale: 1 / sqrt(width) if not given.  A token that sees no key has zeros.  keep: returns (out, AttentionSaved) for attention_backward."""
+    m = _heads(q, "q")
+    count, offsets, *keys = _key_rows(rows, key_rows, key_lengths)
+    out = q.new_empty(q.shape)
+    logsum = q.new_empty((m.heads, m.tokens), dtype=torch.float32) if keep else None
+    st = _capi.load().nvtext_amd_attention(m, _heads(k, "k"), _heads(v, "v"), count, offsets, *keys, causal, _scale(scale, m.width), _stream_handle(),
+                                           _mr().struct, _heads(out, "out"), logsum.data_ptr() if keep else None)
+    if st != _capi.SUCCESS:
+        _raise(st)
+    return (out, AttentionSaved(out, logsum)) if keep else out
+
+
+def attention_backward(grad: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, saved: AttentionSaved, rows: Rows, key_rows: Optional[Rows] = None,
+                       key_lengths: Optional[torch.Tensor] = None, causal: bool = False, scale: Optional[float] = None,
+                       out: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(grad of q, grad of k, grad of v) of attention().  The gradient of a key head is the sum over the heads that see it.  out: where they go,
+    views of one projection's gradient for instance."""
+    g, m = _heads(grad, "grad"), _heads(q, "q")
+    count, offsets, *keys = _key_rows(rows, key_rows, key_lengths)
+    _here(saved.logsum, "logsum")
+    if saved.logsum.dtype != torch.float32 or not saved.logsum.is_contiguous() or saved.logsum.shape != (m.heads, m.tokens):
+        raise ValueError("logsum must be a contiguous float32 tensor of shape [heads, tokens]")
+    q_grad, k_grad, v_grad = out if out is not None else (_like(q), _like(k), _like(v))
+    st = _capi.load().nvtext_amd_attention_backward(g, m, _heads(k, "k"), _heads(v, "v"), _heads(saved.out, "out"), saved.logsum.data_ptr(), count, offsets, *keys, causal,
+                                                    _scale(scale, m.width), _stream_handle(), _mr().struct, _heads(q_grad, "the gradient of q"),
+                                                    _heads(k_grad, "the gradient of k"), _heads(v_grad, "the gradient of v"))
+    if st != _capi.SUCCESS:
+        _raise(st)
+    return q_grad, k_grad, v_grad
+
+
+def _scale(scale: Optional[float], width: int) -> float:
+    return scale if scale is not None else max(width, 1) ** -0.5
+
+
+def _key_rows(rows: Rows, key_rows: Optional[Rows], key_lengths: Optional[torch.Tensor]):
+    """(rows, the addresses of their offsets, of their keys' offsets and of their keys' lengths)."""
+    count, offsets = _rows(rows)
+    key_offsets = None
+    if key_rows is not None:
+        key_count, key_offsets = _rows(key_rows)
+        if key_count != count:
+            raise ValueError("there must be as many rows of keys as of tokens")
+    elif key_lengths is not None:
+        raise ValueError("key_lengths need key_rows")
+    return count, offsets, key_offsets, _int32s(key_lengths, count, "key_lengths")

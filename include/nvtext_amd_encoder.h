@@ -1,8 +1,8 @@
 /*
  * nvtext_amd_encoder.h -- C ABI of the operators between wordpiece_tokenize's column of ids and a model that learns
- * from it: embedding of a LIST<INT32> column, dropout, layer norm and the matrix product of a layer (linear), each with
- * its gradient.  The tokens of all rows lie one after the other (packed); every operator but the embedding treats a
- * token by itself.
+ * from it: embedding of a LIST<INT32> column, dropout, layer norm, the matrix product of a layer (linear), rotary positions
+ * and attention, each with its gradient.  The tokens of all rows lie one after the other (packed); every operator but the
+ * embedding, rotary positions and attention treats a token by itself.
  *
  * The conventions are those of nvtext_amd.h: device pointers, the caller's stream, status codes, the text of the last
  * error.  Matrices are views of the caller's memory, the results too (their sizes are known before the call);
@@ -148,6 +148,95 @@ nvtext_amd_status nvtext_amd_linear_backward(const nvtext_amd_matrix* grad,
                                              const nvtext_amd_matrix* x_grad,
                                              const nvtext_amd_matrix* weight_grad,
                                              const nvtext_amd_matrix* bias_grad);
+
+/* The heads of packed tokens: value j of head h of token t lies at data[t * stride + h * head_stride + j], so that those of
+ * queries, keys and values can be parts of the rows of one matrix.  stride and head_stride are in values and not negative;
+ * each is of no meaning where there are fewer than two tokens or heads.  data is aligned to its element type.  Heads of a width that is a multiple of
+ * 8, with both strides multiples of 8 and data at a multiple of 16 bytes, are read fastest (FLOAT32: of 4 each). */
+typedef struct nvtext_amd_heads {
+  void* data; /* device; may be NULL when there are no values */
+  int64_t tokens;
+  int64_t heads;
+  int64_t width;
+  int64_t stride;
+  int64_t head_stride;
+  int32_t type; /* NVTEXT_AMD_TYPE_FLOAT32, _FLOAT16 or _BFLOAT16 */
+} nvtext_amd_heads;
+
+typedef enum nvtext_amd_rotary_layout {
+  NVTEXT_AMD_ROTARY_HALF        = 0, /* pair n of N is values n and n + N of a head */
+  NVTEXT_AMD_ROTARY_INTERLEAVED = 1  /* pair n is values 2 n and 2 n + 1 */
+} nvtext_amd_rotary_layout;
+
+/* Rotary positions: of every head of a token at position t of its row, pair n of the first 2 * pairs values (a, b) becomes
+ *   magnitude * (a cos w - b sin w, a sin w + b cos w),  w = t * frequencies[n], and with `inverse` w = -t * frequencies[n];
+ * the values behind them are copied.  The inverse call with the same magnitude, on the gradient of out, is the backward pass.
+ * Row r's tokens are offsets[r] up to offsets[r + 1] (device, rows + 1 values, ascending); their positions count from
+ * starts[r] on (device, `rows` values; NULL: from 0 on).  A token that belongs to no row is copied.  frequencies: `pairs` values on
+ * the device, radians a position.  Angles are computed in 64 bits and reduced to a part of a turn before they lose any, so positions may be
+ * as far as they come: sine and cosine are off by 2^-22 at most (at position t by t * |frequency| * 2^-52 more); products and sums are
+ * held in 32 bits and rounded once.  out has x's shape and type, and may be x. */
+nvtext_amd_status nvtext_amd_rotary(const nvtext_amd_heads* x,
+                                    int32_t rows,
+                                    const int32_t* offsets,
+                                    const int32_t* starts,
+                                    const double* frequencies,
+                                    int64_t pairs,
+                                    int32_t layout,
+                                    int32_t inverse,
+                                    double magnitude,
+                                    void* stream,
+                                    const nvtext_amd_heads* out);
+
+/* Attention: every head of a token looks at the keys of its row.
+ * Row r has the tokens offsets[r] up to offsets[r + 1] of q, and of k and v those from key_offsets[r] on, key_lengths[r] of
+ * them, or up to key_offsets[r + 1] where key_lengths is NULL (all on the device; offsets ascend, rows + 1 values each; key_offsets
+ * NULL: k and v have q's tokens and offsets).  With key_lengths, keys may lie in places with room for more, which is not read.
+ * Head h of q sees head h / (q's heads / k's heads) of k and v, whose heads are a divisor of q's.  Token i of Q in a row sees key j of K
+ * there, for causal = 0 every one, else j <= i + K - Q: its last token all of them.  Over the keys it sees, with s_j = scale * (q . k_j),
+ *   logsum = log(sum of exp(s_j)),  out = sum of exp(s_j - logsum) * v_j;
+ * a token that sees none, or belongs to no row, has zeros in out and -infinity in logsum.  What a token does not see is without
+ * effect on it, whatever it is, NaN too.
+ * q, k, v and out are of one type and width, of at most 256 values; scale is not negative.  logsum (NULL: not wanted; the gradient needs it)
+ * has a value of FLOAT32 at [h * tokens + t].  Products, exponentials' sums and out are held in 32 bits; of 16-bit types, the exponentials are
+ * rounded to the type before they are multiplied with v (the values that logsum sums are not), as the matrix cores take them. */
+nvtext_amd_status nvtext_amd_attention(const nvtext_amd_heads* q,
+                                       const nvtext_amd_heads* k,
+                                       const nvtext_amd_heads* v,
+                                       int32_t rows,
+                                       const int32_t* offsets,
+                                       const int32_t* key_offsets,
+                                       const int32_t* key_lengths,
+                                       int32_t causal,
+                                       double scale,
+                                       void* stream,
+                                       const nvtext_amd_allocator* mr,
+                                       const nvtext_amd_heads* out,
+                                       float* logsum);
+
+/* The gradients of attention from grad, that of its out, and from its out and logsum, over the same rows.  With p = exp(s - logsum)
+ * and d = p * (grad . v - grad . out), for every token and the keys it sees, each rounded to the type before it is multiplied:
+ *   q_grad = scale * sum over the keys of d * k,
+ *   k_grad = scale * sum over the tokens, and the heads that see one, of d * q,  v_grad = the same sum of p * grad.
+ * All three are wanted, whole: keys that nobody sees, or that belong to no row, have zeros.  They may be parts of one matrix' rows, as q, k and v
+ * may, but overlap no input. */
+nvtext_amd_status nvtext_amd_attention_backward(const nvtext_amd_heads* grad,
+                                                const nvtext_amd_heads* q,
+                                                const nvtext_amd_heads* k,
+                                                const nvtext_amd_heads* v,
+                                                const nvtext_amd_heads* out,
+                                                const float* logsum,
+                                                int32_t rows,
+                                                const int32_t* offsets,
+                                                const int32_t* key_offsets,
+                                                const int32_t* key_lengths,
+                                                int32_t causal,
+                                                double scale,
+                                                void* stream,
+                                                const nvtext_amd_allocator* mr,
+                                                const nvtext_amd_heads* q_grad,
+                                                const nvtext_amd_heads* k_grad,
+                                                const nvtext_amd_heads* v_grad);
 
 #ifdef __cplusplus
 }

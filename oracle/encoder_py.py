@@ -141,3 +141,102 @@ def linear_backward(grad, x, weight, activation="none", z=None):
         d = d * slope(z.astype(np.float64), activation)
     e = np.abs(d)
     return (d @ weight, d.T @ x, d.sum(0)), (e @ np.abs(weight), e.T @ np.abs(x), e.sum(0))
+
+
+def positions(offsets, count, starts=None):
+    """Of every token its position, None for what belongs to no row."""
+    at = [None] * count
+    for r, (first, last) in enumerate(zip(offsets[:-1], offsets[1:])):
+        for t in range(first, last):
+            at[t] = int(t - first) + (int(starts[r]) if starts is not None else 0)
+    return at
+
+
+def rotary(x, offsets, frequencies, starts=None, layout="half", inverse=False, magnitude=1.0):
+    """(out, of every value that was turned the sum of the magnitudes that it was made of, 0 for what is copied)."""
+    x = np.asarray(x, np.float64)
+    out, size, n = x.copy(), np.zeros(x.shape), len(frequencies)
+    a, b = (slice(0, n), slice(n, 2 * n)) if layout == "half" else (slice(0, 2 * n, 2), slice(1, 2 * n, 2))
+    for t, at in enumerate(positions(offsets, len(x), starts)):
+        if at is None:
+            continue
+        angle = np.asarray(at * np.asarray(frequencies, np.longdouble) * (-1 if inverse else 1))
+        c, s = np.cos(angle).astype(np.float64) * magnitude, np.sin(angle).astype(np.float64) * magnitude
+        p, q = x[t][:, a], x[t][:, b]
+        out[t][:, a], out[t][:, b] = p * c - q * s, p * s + q * c
+        size[t][:, a] = size[t][:, b] = (np.abs(p) + np.abs(q)) * abs(magnitude)
+    return out, size
+
+
+def _rows_seen(offsets, key_offsets, key_lengths, causal):
+    """(the tokens, the keys, [tokens, keys] which of them see which) of every row."""
+    for r in range(len(offsets) - 1):
+        t = slice(int(offsets[r]), int(offsets[r + 1]))
+        count = int(key_offsets[r + 1] - key_offsets[r])
+        if key_lengths is not None:
+            count = max(0, min(count, int(key_lengths[r])))
+        u = slice(int(key_offsets[r]), int(key_offsets[r]) + count)
+        i, j = np.arange(t.stop - t.start)[:, None], np.arange(count)[None, :]
+        yield t, u, (j <= i + count - (t.stop - t.start)) if causal else np.ones((len(i), count), bool)
+
+
+def attention(q, k, v, offsets, key_offsets=None, key_lengths=None, causal=False, scale=None, unit=0.0, eps=2.0**-24):
+    """(out, logsum [heads, tokens], what a kernel's out may be off by before it is rounded, the same for logsum).  unit: by how much of itself
+    an exponential may be off that is rounded before it is multiplied.  A score of `width` products held in 32 bits is off by
+    eps a product and addition, in proportion to the magnitudes that it adds up, twice where they are cut off instead of
+    rounded; its difference from the largest score or the logsum by eps of both; the exponential follows."""
+    q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
+    key_offsets = offsets if key_offsets is None else key_offsets
+    scale, each, width = q.shape[2] ** -0.5 if scale is None else scale, q.shape[1] // k.shape[1], q.shape[2]
+    out, off = np.zeros(q.shape), np.zeros(q.shape)
+    logsum, log_off = np.full(q.shape[:2][::-1], -np.inf), np.zeros(q.shape[:2][::-1])
+    for t, u, sees in _rows_seen(offsets, key_offsets, key_lengths, causal):
+        any_seen = sees.any(1)
+        for h in range(q.shape[1]):
+            for i in np.flatnonzero(any_seen):
+                at, keys = t.start + i, np.flatnonzero(sees[i]) + u.start
+                kk, vv = k[keys, h // each], v[keys, h // each]
+                s = scale * (kk @ q[at, h])
+                top = s.max()
+                e = np.exp(s - top)
+                logsum[h, at] = top + np.log(e.sum())
+                p = e / e.sum()
+                out[at, h] = p @ vv
+                score_off = score_error(scale * (np.abs(kk) @ np.abs(q[at, h])), abs(top), width, eps)
+                worst = score_off.max()
+                off[at, h] = (p * (unit + score_off + worst + 2 * (len(keys) + 8) * eps)) @ np.abs(vv)
+                log_off[h, at] = worst + 2 * (len(keys) + 8) * eps
+    return out, logsum, off, log_off
+
+
+def score_error(size, top, width, eps):
+    return eps * (2 * (width + 4) * size + 4 * top + 8)
+
+
+def attention_backward(grad, q, k, v, out, logsum, offsets, key_offsets=None, key_lengths=None, causal=False, scale=None, unit=0.0, eps=2.0**-24):
+    """((gradients of q, k, v), (what a kernel's may be off by before they are rounded)), from out and logsum as they are given."""
+    grad, q, k, v, out, logsum = (np.asarray(x, np.float64) for x in (grad, q, k, v, out, logsum))
+    key_offsets = offsets if key_offsets is None else key_offsets
+    scale, each, width = q.shape[2] ** -0.5 if scale is None else scale, q.shape[1] // k.shape[1], q.shape[2]
+    results, offs = [np.zeros(x.shape) for x in (q, k, v)], [np.zeros(x.shape) for x in (q, k, v)]
+    for t, u, sees in _rows_seen(offsets, key_offsets, key_lengths, causal):
+        if not sees.any():
+            continue
+        for h in range(q.shape[1]):
+            qh, gh, oh, kh, vh = q[t, h], grad[t, h], out[t, h], k[u, h // each], v[u, h // each]
+            log = np.where(sees.any(1), logsum[h, t], 0.0)[:, None]
+            s = scale * (qh @ kh.T)
+            p = np.where(sees, np.exp(np.where(sees, s - log, 0.0)), 0.0)
+            dp, delta = gh @ vh.T, (gh * oh).sum(1)[:, None]
+            ds = p * (dp - delta)
+            e = score_error(scale * (np.abs(qh) @ np.abs(kh).T), np.abs(log), width, eps) + 8 * eps
+            dp_off = 2 * (width + 4) * eps * (np.abs(gh) @ np.abs(vh).T + (np.abs(gh) * np.abs(oh)).sum(1)[:, None])
+            ds_off = 1.1 * (np.abs(ds) * (unit + e) + p * dp_off)
+            longest = 2 * (max(s.shape) * each + 8) * eps
+            results[0][t, h] = scale * (ds @ kh)
+            offs[0][t, h] = scale * ((ds_off + longest * np.abs(ds)) @ np.abs(kh))
+            results[1][u, h // each] += scale * (ds.T @ qh)
+            offs[1][u, h // each] += scale * ((ds_off + longest * np.abs(ds)).T @ np.abs(qh))
+            results[2][u, h // each] += p.T @ gh
+            offs[2][u, h // each] += (1.1 * p * (unit + e + longest)).T @ np.abs(gh)
+    return results, offs
