@@ -1,0 +1,322 @@
+// Shared by attention and its gradient: what the kernels are given, the formulas a row at a time, and tiles of keys in LDS.
+#pragma once
+
+#include "heads.cuh"
+#include "matrix.cuh"
+
+namespace nvtext_amd {
+
+constexpr int kMostWidth  = 256;
+constexpr float kLog2e    = 1.4426950408889634f;
+constexpr float kLn2      = 0.6931471805599453f;
+
+// What the kernels of both directions are given.
+template <typename T>
+struct Problem {
+  Heads<const T> q, k, v;
+  int32_t heads, kv_heads, width;
+  Runs runs, key_runs;
+  const int32_t* key_lengths;
+  bool causal;
+  float scale;
+
+  // The keys of run `i` (a row's), of which there are `length`, from token `first` on.
+  __device__ __forceinline__ void keys_of(int32_t i, int32_t& first, int32_t& length) const
+  {
+    first  = key_runs.begin(i);
+    length = key_runs.begin(i + 1) - first;
+    if (key_lengths) {
+      int32_t const l = key_lengths[i - 1];
+      length          = l < length ? l : length;
+    }
+    length = length > 0 ? length : 0;
+  }
+  __device__ __forceinline__ bool is_row(int32_t i) const { return i > 0 && i <= runs.rows; }
+  // How many keys token `i` of a row of `tokens` sees, of `keys`.
+  __device__ __forceinline__ int32_t seen(int32_t i, int32_t tokens, int32_t keys) const
+  {
+    int64_t const n = causal ? static_cast<int64_t>(i) + 1 + keys - tokens : keys;
+    return static_cast<int32_t>(n < 0 ? 0 : n < keys ? n : keys);
+  }
+};
+
+// ------------------------------------------------------------------ a row at a time
+// The formulas as they stand, a wavefront for a token and a head, 64 keys at a time: a lane for a key in the scores, a lane for a column in the
+// sums.  Nothing that a token does not see is multiplied by anything.
+
+template <typename T>
+__device__ __forceinline__ float dot(const T* a, const T* b, int32_t width)
+{
+  float sum = 0.f;
+  for (int32_t j = 0; j < width; ++j) sum = fmaf(static_cast<float>(a[j]), static_cast<float>(b[j]), sum);
+  return sum;
+}
+
+__device__ __forceinline__ float wave_max(float v)
+{
+#pragma unroll
+  for (int by = 32; by > 0; by /= 2) v = fmaxf(v, __shfl_xor(v, by));
+  return v;
+}
+
+template <typename T>
+struct Forward : Problem<T> {
+  Heads<T> out;
+  float* logsum;
+};
+
+// The run that token t is in.
+__device__ __forceinline__ int32_t run_with(Runs const& runs, int32_t t)
+{
+  int32_t lo = 0, hi = runs.rows + 2;
+  while (hi - lo > 1) {
+    int32_t const mid = lo + (hi - lo) / 2;
+    if (runs.begin(mid) <= t)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+template <typename T>
+__device__ void attend_row(Forward<T> const& f, int32_t t, int32_t h)
+{
+  int const lane    = lane_id();
+  int32_t const run = run_with(f.runs, t);
+  int32_t first = 0, keys = 0, seen = 0;
+  if (f.is_row(run)) {
+    f.keys_of(run, first, keys);
+    seen = f.seen(t - f.runs.begin(run), f.runs.begin(run + 1) - f.runs.begin(run), keys);
+  }
+  int32_t const kh   = h / (f.heads / f.kv_heads);
+  float const scale  = f.scale * kLog2e;
+  const T* const q   = f.q.at(t, h);
+  float top = -INFINITY, sum = 0.f, o[kMostWidth / kWave] = {};
+  for (int32_t base = 0; base < seen; base += kWave) {
+    int32_t const n = seen - base < kWave ? seen - base : kWave;
+    float const s   = lane < n ? dot(q, f.k.at(first + base + lane, kh), f.width) * scale : -INFINITY;
+    float const now = fmaxf(top, wave_max(s));
+    float const p   = lane < n ? __builtin_amdgcn_exp2f(s - now) : 0.f, fade = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - now);
+    sum = sum * fade + wave_sum(p);
+#pragma unroll
+    for (int c = 0; c < kMostWidth / kWave; ++c) o[c] *= fade;
+    for (int32_t j = 0; j < n; ++j) {
+      float const pj = __shfl(p, j);
+#pragma unroll
+      for (int c = 0; c < kMostWidth / kWave; ++c)
+        if (c * kWave + lane < f.width) o[c] = fmaf(pj, static_cast<float>(f.v.at(first + base + j, kh)[c * kWave + lane]), o[c]);
+    }
+    top = now;
+  }
+#pragma unroll
+  for (int c = 0; c < kMostWidth / kWave; ++c)
+    if (c * kWave + lane < f.width) f.out.at(t, h)[c * kWave + lane] = static_cast<T>(seen > 0 ? o[c] / sum : 0.f);
+  if (f.logsum && lane == 0) f.logsum[static_cast<int64_t>(h) * f.runs.tokens + t] = seen > 0 ? (top + __builtin_amdgcn_logf(sum)) * kLn2 : -INFINITY;
+}
+
+template <typename T>
+struct Backward : Problem<T> {
+  Heads<const T> grad, out;
+  const float* logsum;
+  float* deltas;  // [heads, tokens]: grad . out
+  Heads<T> q_grad, k_grad, v_grad;
+};
+
+// The gradient of token t's head h of q, and its delta.
+template <typename T>
+__device__ void query_gradient_row(Backward<T> const& f, int32_t t, int32_t h)
+{
+  int const lane    = lane_id();
+  int32_t const run = run_with(f.runs, t);
+  int32_t first = 0, keys = 0, seen = 0;
+  if (f.is_row(run)) {
+    f.keys_of(run, first, keys);
+    seen = f.seen(t - f.runs.begin(run), f.runs.begin(run + 1) - f.runs.begin(run), keys);
+  }
+  int32_t const kh = h / (f.heads / f.kv_heads);
+  const T *const q = f.q.at(t, h), *const g = f.grad.at(t, h);
+  int64_t const at  = static_cast<int64_t>(h) * f.runs.tokens + t;
+  float const log   = f.logsum[at] * kLog2e, scale = f.scale * kLog2e;
+  float const delta = seen > 0 ? dot(g, f.out.at(t, h), f.width) : 0.f;
+  if (lane == 0) f.deltas[at] = delta;
+  float d[kMostWidth / kWave] = {};
+  for (int32_t base = 0; base < seen; base += kWave) {
+    int32_t const n = seen - base < kWave ? seen - base : kWave;
+    float ds        = 0.f;
+    if (lane < n) {
+      float const p = __builtin_amdgcn_exp2f(dot(q, f.k.at(first + base + lane, kh), f.width) * scale - log);
+      ds            = p * (dot(g, f.v.at(first + base + lane, kh), f.width) - delta) * f.scale;
+    }
+    for (int32_t j = 0; j < n; ++j) {
+      float const dj = __shfl(ds, j);
+#pragma unroll
+      for (int c = 0; c < kMostWidth / kWave; ++c)
+        if (c * kWave + lane < f.width) d[c] = fmaf(dj, static_cast<float>(f.k.at(first + base + j, kh)[c * kWave + lane]), d[c]);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < kMostWidth / kWave; ++c)
+    if (c * kWave + lane < f.width) f.q_grad.at(t, h)[c * kWave + lane] = static_cast<T>(d[c]);
+}
+
+// The gradients of key token t's head kh of k and v.
+template <typename T>
+__device__ void key_gradient_row(Backward<T> const& f, int32_t t, int32_t kh)
+{
+  int const lane    = lane_id();
+  int32_t const run = run_with(f.key_runs, t), each = f.heads / f.kv_heads;
+  float dk[kMostWidth / kWave] = {}, dv[kMostWidth / kWave] = {};
+  int32_t first = 0, keys = 0;
+  if (f.is_row(run)) f.keys_of(run, first, keys);
+  int32_t const j = t - first;
+  if (f.is_row(run) && j < keys) {
+    int32_t const begin = f.runs.begin(run), tokens = f.runs.begin(run + 1) - begin;
+    // token i sees key j from i = j + tokens - keys on
+    int64_t const from = f.causal ? static_cast<int64_t>(j) + tokens - keys : 0;
+    const T *const k = f.k.at(t, kh), *const v = f.v.at(t, kh);
+    float const scale = f.scale * kLog2e;
+    for (int32_t h = kh * each; h < (kh + 1) * each; ++h) {
+      for (int64_t base = from < 0 ? 0 : from; base < tokens; base += kWave) {
+        int32_t const n = static_cast<int32_t>(tokens - base < kWave ? tokens - base : kWave), token = static_cast<int32_t>(begin + base);
+        float p = 0.f, ds = 0.f;
+        if (lane < n) {
+          int64_t const at = static_cast<int64_t>(h) * f.runs.tokens + token + lane;
+          p                = __builtin_amdgcn_exp2f(dot(f.q.at(token + lane, h), k, f.width) * scale - f.logsum[at] * kLog2e);
+          ds               = p * (dot(f.grad.at(token + lane, h), v, f.width) - f.deltas[at]) * f.scale;
+        }
+        for (int32_t i = 0; i < n; ++i) {
+          float const pi = __shfl(p, i), di = __shfl(ds, i);
+#pragma unroll
+          for (int c = 0; c < kMostWidth / kWave; ++c)
+            if (c * kWave + lane < f.width) {
+              dv[c] = fmaf(pi, static_cast<float>(f.grad.at(token + i, h)[c * kWave + lane]), dv[c]);
+              dk[c] = fmaf(di, static_cast<float>(f.q.at(token + i, h)[c * kWave + lane]), dk[c]);
+            }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < kMostWidth / kWave; ++c)
+    if (c * kWave + lane < f.width) {
+      f.k_grad.at(t, kh)[c * kWave + lane] = static_cast<T>(dk[c]);
+      f.v_grad.at(t, kh)[c * kWave + lane] = static_cast<T>(dv[c]);
+    }
+}
+
+// ------------------------------------------------------------------ tiles
+// Products of 32 x 32 on the matrix cores, 16 deep.  A lane has 8 values of a row (or column) of each operand, number l % 32, from 8 * (l / 32) on;
+// of the result column l % 32, and of it rows 8 * (r / 4) + 4 * (l / 32) + r % 4 for r = 0 .. 15.
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ f32x16_t multiply32(Fragment<bf16_t> a, Fragment<bf16_t> b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16_t multiply32(Fragment<half_t> a, Fragment<half_t> b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+constexpr int kTile = 64;  // tokens or keys of a tile in LDS
+
+// A tile of kTile heads of D values (a multiple of 32), as it lies in LDS: 2 * D bytes a head, in units of 32 bytes whose order is turned with the head's
+// number, so that 8 neighbouring heads' units of one number lie in different banks (the reads of rows), and so do two neighbouring units of 4
+// neighbouring heads (the transposing reads).  What turns them depends on where heads begin within the 256 bytes of all banks.
+template <int D>
+struct Tile {
+  static constexpr int kBytes = kTile * D * 2, kPieces = D / 8;  // pieces of 16 bytes of a head
+  __device__ __forceinline__ static constexpr uint32_t turn(uint32_t head)
+  {
+    if constexpr (D % 128 == 0) return (head & 3) << 1 | (head >> 2 & 1);
+    if constexpr (D % 64 == 0) return head & 2 | (head >> 2 & 1);
+    return head >> 2 & 1;
+  }
+};
+
+// What a wavefront of WAVES loads of a tile: straight into LDS, 64 pieces of 16 bytes at a time, zeros for what is not there.
+template <int D, int WAVES>
+struct TileLoader {
+  static constexpr int kAll = kTile * Tile<D>::kPieces / kWave, kLoads = (kAll + WAVES - 1) / WAVES;
+  uint32_t offset[kLoads];
+  uint32_t line, width;  // bytes from a head to the next, of one
+  const char* base;      // of the next tile
+
+  template <typename T>
+  __device__ __forceinline__ void aim(Heads<const T> const& x, int32_t first, int32_t head, int32_t columns, int wave, int lane)
+  {
+    base  = reinterpret_cast<const char*>(x.at(first, head));
+    line  = static_cast<uint32_t>(x.stride * 2);
+    width = static_cast<uint32_t>(columns * 2);
+#pragma unroll
+    for (int p = 0; p < kLoads; ++p) {
+      int const slot = (p * WAVES + wave) * kWave + lane, row = slot / Tile<D>::kPieces, piece = slot % Tile<D>::kPieces;
+      int const from = (static_cast<int>(static_cast<uint32_t>(piece >> 1) ^ Tile<D>::turn(row)) << 1) | (piece & 1);
+      offset[p]      = from * 8 < columns ? row * line + from * 16 : kFar;
+    }
+  }
+  // The next tile, of which `here` heads are there.
+  __device__ __forceinline__ void load(LdsBytes to, int32_t here, int wave)
+  {
+    uint32_t const range = static_cast<uint32_t>(here < kTile ? here - 1 : kTile - 1) * line + width;
+#pragma unroll
+    for (int p = 0; p < kLoads; ++p)
+      if (kAll % WAVES == 0 || p * WAVES + wave < kAll) load_to_lds(base, range, to + (p * WAVES + wave) * 1024, offset[p]);
+    base += static_cast<int64_t>(kTile) * line;
+  }
+};
+
+// Where a lane finds fragments of a tile.
+template <typename T, int D>
+struct TileReader {
+  uint32_t row, column, turn_row, turn_column;
+  __device__ __forceinline__ explicit TileReader(int lane)
+  {
+    int const h = lane / 32, i = lane % 16;
+    row         = (lane % 32) * (2 * D) + h * 16;
+    turn_row    = Tile<D>::turn(lane % 32);
+    int const k = 4 * h + i / 4;
+    column      = k * (2 * D) + i % 4 * 8;
+    turn_column = Tile<D>::turn(k) ^ (lane / 16 & 1);
+  }
+  // 32 heads from 32 * block on, values 16 * step .. 16 * step + 15 of each
+  __device__ __forceinline__ Fragment<T> rows(LdsBytes tile, int block, int step) const
+  {
+    return *reinterpret_cast<__attribute__((address_space(3))) Fragment<T>*>(tile + row + ((step ^ turn_row) * 32) + block * (64 * D));
+  }
+  // transposed: values 32 * block .. 32 * block + 31 of 16 heads from 16 * step on, in the order of heads that a result of 32 x 32 leaves in its registers
+  __device__ __forceinline__ Fragment<T> columns(LdsBytes tile, int block, int step) const
+  {
+    LdsBytes const p   = tile + column + (((2 * block) ^ turn_column) * 32) + step * (32 * D);
+    s16x4_t const low  = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(p));
+    s16x4_t const high = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(p + 16 * D));
+    return __builtin_bit_cast(Fragment<T>, __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+};
+
+// v of the lane of the lower 32 with this one's number among them, and of that of the upper 32
+struct Halves {
+  float low, high;
+};
+__device__ __forceinline__ Halves halves(float v)
+{
+  uint32_t const a = __builtin_bit_cast(uint32_t, v);
+  auto const both  = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  uint32_t const low = both[0], high = both[1];  // (bit_cast of an element of a vector takes the first one, whichever is named)
+  return {__builtin_bit_cast(float, low), __builtin_bit_cast(float, high)};
+}
+
+// Values 8 * step .. 8 * step + 7 of a result's registers, rounded, as an operand.
+template <typename T>
+__device__ __forceinline__ Fragment<T> rounded(f32x16_t const& x, int step)
+{
+  Fragment<T> f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) f[k] = static_cast<T>(x[8 * step + k]);
+  return f;
+}
+
+// 16 bytes of a head's values from j on, zeros behind the last or where it is not `there`; widths and strides are multiples of 8
+template <typename T>
+__device__ __forceinline__ Fragment<T> fragment_of(const T* head, int32_t j, int32_t width, bool there)
+{
+  Fragment<T> f{};
+  if (there && j < width) f = *reinterpret_cast<const Fragment<T>*>(head + j);
+  return f;
+}
+
+}  // namespace nvtext_amd

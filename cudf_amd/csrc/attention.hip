@@ -1,120 +1,12 @@
 // Attention of a row's tokens over its keys, and its gradient.
-#include "heads.cuh"
+#include "attention.cuh"
 
 #include <cmath>
 
 namespace nvtext_amd {
 namespace {
 
-constexpr int kThreads    = 256;
-constexpr int kMostWidth  = 256;
-constexpr float kLog2e    = 1.4426950408889634f;
-constexpr float kLn2      = 0.6931471805599453f;
-
-// What the kernels of both directions are given.
-template <typename T>
-struct Problem {
-  Heads<const T> q, k, v;
-  int32_t heads, kv_heads, width;
-  Runs runs, key_runs;
-  const int32_t* key_lengths;
-  bool causal;
-  float scale;
-
-  // The keys of run `i` (a row's), of which there are `length`, from token `first` on.
-  __device__ __forceinline__ void keys_of(int32_t i, int32_t& first, int32_t& length) const
-  {
-    first  = key_runs.begin(i);
-    length = key_runs.begin(i + 1) - first;
-    if (key_lengths) {
-      int32_t const l = key_lengths[i - 1];
-      length          = l < length ? l : length;
-    }
-    length = length > 0 ? length : 0;
-  }
-  __device__ __forceinline__ bool is_row(int32_t i) const { return i > 0 && i <= runs.rows; }
-  // How many keys token `i` of a row of `tokens` sees, of `keys`.
-  __device__ __forceinline__ int32_t seen(int32_t i, int32_t tokens, int32_t keys) const
-  {
-    int64_t const n = causal ? static_cast<int64_t>(i) + 1 + keys - tokens : keys;
-    return static_cast<int32_t>(n < 0 ? 0 : n < keys ? n : keys);
-  }
-};
-
-// ------------------------------------------------------------------ a row at a time
-// The formulas as they stand, a wavefront for a token and a head, 64 keys at a time: a lane for a key in the scores, a lane for a column in the
-// sums.  Nothing that a token does not see is multiplied by anything.
-
-template <typename T>
-__device__ __forceinline__ float dot(const T* a, const T* b, int32_t width)
-{
-  float sum = 0.f;
-  for (int32_t j = 0; j < width; ++j) sum = fmaf(static_cast<float>(a[j]), static_cast<float>(b[j]), sum);
-  return sum;
-}
-
-__device__ __forceinline__ float wave_max(float v)
-{
-#pragma unroll
-  for (int by = 32; by > 0; by /= 2) v = fmaxf(v, __shfl_xor(v, by));
-  return v;
-}
-
-template <typename T>
-struct Forward : Problem<T> {
-  Heads<T> out;
-  float* logsum;
-};
-
-// The run that token t is in.
-__device__ __forceinline__ int32_t run_with(Runs const& runs, int32_t t)
-{
-  int32_t lo = 0, hi = runs.rows + 2;
-  while (hi - lo > 1) {
-    int32_t const mid = lo + (hi - lo) / 2;
-    if (runs.begin(mid) <= t)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  return lo;
-}
-
-template <typename T>
-__device__ void attend_row(Forward<T> const& f, int32_t t, int32_t h)
-{
-  int const lane    = lane_id();
-  int32_t const run = run_with(f.runs, t);
-  int32_t first = 0, keys = 0, seen = 0;
-  if (f.is_row(run)) {
-    f.keys_of(run, first, keys);
-    seen = f.seen(t - f.runs.begin(run), f.runs.begin(run + 1) - f.runs.begin(run), keys);
-  }
-  int32_t const kh   = h / (f.heads / f.kv_heads);
-  float const scale  = f.scale * kLog2e;
-  const T* const q   = f.q.at(t, h);
-  float top = -INFINITY, sum = 0.f, o[kMostWidth / kWave] = {};
-  for (int32_t base = 0; base < seen; base += kWave) {
-    int32_t const n = seen - base < kWave ? seen - base : kWave;
-    float const s   = lane < n ? dot(q, f.k.at(first + base + lane, kh), f.width) * scale : -INFINITY;
-    float const now = fmaxf(top, wave_max(s));
-    float const p   = lane < n ? __builtin_amdgcn_exp2f(s - now) : 0.f, fade = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - now);
-    sum = sum * fade + wave_sum(p);
-#pragma unroll
-    for (int c = 0; c < kMostWidth / kWave; ++c) o[c] *= fade;
-    for (int32_t j = 0; j < n; ++j) {
-      float const pj = __shfl(p, j);
-#pragma unroll
-      for (int c = 0; c < kMostWidth / kWave; ++c)
-        if (c * kWave + lane < f.width) o[c] = fmaf(pj, static_cast<float>(f.v.at(first + base + j, kh)[c * kWave + lane]), o[c]);
-    }
-    top = now;
-  }
-#pragma unroll
-  for (int c = 0; c < kMostWidth / kWave; ++c)
-    if (c * kWave + lane < f.width) f.out.at(t, h)[c * kWave + lane] = static_cast<T>(seen > 0 ? o[c] / sum : 0.f);
-  if (f.logsum && lane == 0) f.logsum[static_cast<int64_t>(h) * f.runs.tokens + t] = seen > 0 ? (top + __builtin_amdgcn_logf(sum)) * kLn2 : -INFINITY;
-}
+constexpr int kThreads = 256;
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) attend_rows_kernel(Forward<T> f)
@@ -124,94 +16,197 @@ __global__ void __launch_bounds__(kThreads) attend_rows_kernel(Forward<T> f)
   attend_row(f, static_cast<int32_t>(w / f.heads), static_cast<int32_t>(w % f.heads));
 }
 
-template <typename T>
-struct Backward : Problem<T> {
-  Heads<const T> grad, out;
-  const float* logsum;
-  float* deltas;  // [heads, tokens]: grad . out
-  Heads<T> q_grad, k_grad, v_grad;
+// ------------------------------------------------------------------ forward, in tiles
+// The work of a launch: blocks of tokens, of every head.  The heads that share a key head come one after the other on one XCD (workgroups go to
+// the eight XCDs in turn), and so do, where the number of key heads allows, the blocks of a key head: its keys come from that XCD's L2.  The last
+// blocks come first: of a long row they are those with the most keys to see.
+struct Work {
+  int64_t block;
+  int32_t kv_head, head;
 };
-
-// The gradient of token t's head h of q, and its delta.
-template <typename T>
-__device__ void query_gradient_row(Backward<T> const& f, int32_t t, int32_t h)
+constexpr int kXcds = 8;
+inline int64_t work_items(int64_t blocks, int32_t kv_heads, int32_t each) { return (blocks * kv_heads + kXcds - 1) / kXcds * kXcds * each; }
+// false: nothing to do
+__device__ __forceinline__ bool work_of(int64_t item, int64_t blocks, int32_t kv_heads, int32_t each, Work& w)
 {
-  int const lane    = lane_id();
-  int32_t const run = run_with(f.runs, t);
-  int32_t first = 0, keys = 0, seen = 0;
-  if (f.is_row(run)) {
-    f.keys_of(run, first, keys);
-    seen = f.seen(t - f.runs.begin(run), f.runs.begin(run + 1) - f.runs.begin(run), keys);
-  }
-  int32_t const kh = h / (f.heads / f.kv_heads);
-  const T *const q = f.q.at(t, h), *const g = f.grad.at(t, h);
-  int64_t const at  = static_cast<int64_t>(h) * f.runs.tokens + t;
-  float const log   = f.logsum[at] * kLog2e, scale = f.scale * kLog2e;
-  float const delta = seen > 0 ? dot(g, f.out.at(t, h), f.width) : 0.f;
-  if (lane == 0) f.deltas[at] = delta;
-  float d[kMostWidth / kWave] = {};
-  for (int32_t base = 0; base < seen; base += kWave) {
-    int32_t const n = seen - base < kWave ? seen - base : kWave;
-    float ds        = 0.f;
-    if (lane < n) {
-      float const p = __builtin_amdgcn_exp2f(dot(q, f.k.at(first + base + lane, kh), f.width) * scale - log);
-      ds            = p * (dot(g, f.v.at(first + base + lane, kh), f.width) - delta) * f.scale;
-    }
-    for (int32_t j = 0; j < n; ++j) {
-      float const dj = __shfl(ds, j);
-#pragma unroll
-      for (int c = 0; c < kMostWidth / kWave; ++c)
-        if (c * kWave + lane < f.width) d[c] = fmaf(dj, static_cast<float>(f.k.at(first + base + j, kh)[c * kWave + lane]), d[c]);
-    }
-  }
-#pragma unroll
-  for (int c = 0; c < kMostWidth / kWave; ++c)
-    if (c * kWave + lane < f.width) f.q_grad.at(t, h)[c * kWave + lane] = static_cast<T>(d[c]);
+  int64_t const n = item / kXcds, unit = n / each * kXcds + item % kXcds;
+  if (unit >= blocks * kv_heads) return false;
+  w.block   = blocks - 1 - unit / kv_heads;
+  w.kv_head = static_cast<int32_t>(unit % kv_heads);
+  w.head    = w.kv_head * each + static_cast<int32_t>(n % each);
+  return true;
 }
 
-// The gradients of key token t's head kh of k and v.
-template <typename T>
-__device__ void key_gradient_row(Backward<T> const& f, int32_t t, int32_t kh)
+template <int D, int WAVES, int NQ>
+struct ForwardShape {
+  static constexpr int kTokens = 32 * WAVES * NQ, kShift = __builtin_ctz(kTokens), kLds = 4 * Tile<D>::kBytes;
+};
+
+// A workgroup has kTokens tokens of a head, a wavefront 32 * NQ of them, in its registers: q, and the sums of out, transposed.  Keys come through LDS, 64 at a
+// time, the next ones while these are multiplied.  Scores are products with the keys as rows, so a lane has all of a token's scores (with the
+// one 32 further on), and exponentials are in its registers as the second product takes them: no lane needs another's but for the maximum.
+// Sums are kept in proportion to 2^top, where top is a maximum that may be 8 too small: only then are they multiplied anew.
+template <typename T, int D, int WAVES, int NQ>
+__global__ void __launch_bounds__(WAVES * kWave, 2) attend_tiles_kernel(Forward<T> f)
 {
-  int const lane    = lane_id();
-  int32_t const run = run_with(f.key_runs, t), each = f.heads / f.kv_heads;
-  float dk[kMostWidth / kWave] = {}, dv[kMostWidth / kWave] = {};
+  using Shape = ForwardShape<D, WAVES, NQ>;
+  extern __shared__ __align__(16) char lds_[];
+  LdsBytes const lds = (LdsBytes)lds_;
+  constexpr int kSteps = D / 16, kColumns = D / 32;
+  constexpr float kSlack = 8.f;
+  Work w;
+  int32_t const each = f.heads / f.kv_heads;
+  if (!work_of(block_number(), f.runs.template blocks<Shape::kShift>(), f.kv_heads, each, w)) return;
+  int32_t const run   = f.runs.template run_of<Shape::kShift>(w.block);
+  int32_t const begin = uniform(f.runs.begin(run)), tokens = uniform(f.runs.begin(run + 1)) - begin;
+  int64_t const in_run = (w.block - f.runs.template first_block<Shape::kShift>(run)) << Shape::kShift;
+  if (in_run >= tokens) return;
+  int const wave = uniform(threadIdx.x / kWave), lane = lane_id(), column = lane % 32, half = lane / 32;
+  int32_t const block0 = static_cast<int32_t>(in_run), rest = uniform(tokens - block0);  // the first token in the run, tokens from there on
   int32_t first = 0, keys = 0;
   if (f.is_row(run)) f.keys_of(run, first, keys);
-  int32_t const j = t - first;
-  if (f.is_row(run) && j < keys) {
-    int32_t const begin = f.runs.begin(run), tokens = f.runs.begin(run + 1) - begin;
-    // token i sees key j from i = j + tokens - keys on
-    int64_t const from = f.causal ? static_cast<int64_t>(j) + tokens - keys : 0;
-    const T *const k = f.k.at(t, kh), *const v = f.v.at(t, kh);
-    float const scale = f.scale * kLog2e;
-    for (int32_t h = kh * each; h < (kh + 1) * each; ++h) {
-      for (int64_t base = from < 0 ? 0 : from; base < tokens; base += kWave) {
-        int32_t const n = static_cast<int32_t>(tokens - base < kWave ? tokens - base : kWave), token = static_cast<int32_t>(begin + base);
-        float p = 0.f, ds = 0.f;
-        if (lane < n) {
-          int64_t const at = static_cast<int64_t>(h) * f.runs.tokens + token + lane;
-          p                = __builtin_amdgcn_exp2f(dot(f.q.at(token + lane, h), k, f.width) * scale - f.logsum[at] * kLog2e);
-          ds               = p * (dot(f.grad.at(token + lane, h), v, f.width) - f.deltas[at]) * f.scale;
-        }
-        for (int32_t i = 0; i < n; ++i) {
-          float const pi = __shfl(p, i), di = __shfl(ds, i);
+  first = uniform(first);
+  keys  = uniform(keys);
+  // keys that the workgroup's last token sees, and the wavefront's first and last
+  int32_t const wave0 = wave * 32 * NQ, wave1 = wave0 + 32 * NQ < rest ? wave0 + 32 * NQ : rest;
+  int32_t const all  = uniform(f.seen(block0 + (rest < Shape::kTokens ? rest : Shape::kTokens) - 1, tokens, keys));
+  int32_t const least = uniform(wave0 < rest ? f.seen(block0 + wave0, tokens, keys) : 0), most = uniform(wave0 < rest ? f.seen(block0 + wave1 - 1, tokens, keys) : 0);
+
+  Fragment<T> q[NQ][kSteps];
+  int32_t seen[NQ];
 #pragma unroll
-          for (int c = 0; c < kMostWidth / kWave; ++c)
-            if (c * kWave + lane < f.width) {
-              dv[c] = fmaf(pi, static_cast<float>(f.grad.at(token + i, h)[c * kWave + lane]), dv[c]);
-              dk[c] = fmaf(di, static_cast<float>(f.q.at(token + i, h)[c * kWave + lane]), dk[c]);
-            }
-        }
+  for (int n = 0; n < NQ; ++n) {
+    int32_t const i = wave0 + n * 32 + column;
+    seen[n]         = i < rest ? f.seen(block0 + i, tokens, keys) : 0;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) q[n][s] = fragment_of(f.q.at(static_cast<int64_t>(begin) + block0 + (i < rest ? i : 0), w.head), 16 * s + 8 * half, f.width, i < rest);
+  }
+  TileLoader<D, WAVES> load_k, load_v;
+  load_k.aim(f.k, first, w.kv_head, f.width, wave, lane);
+  load_v.aim(f.v, first, w.kv_head, f.width, wave, lane);
+  TileReader<T, D> const read(lane);
+  float const scale = f.scale * kLog2e;
+  f32x16_t o[NQ][kColumns];
+  float top[NQ], sum[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    top[n] = -INFINITY;
+    sum[n] = 0.f;
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) o[n][c] = f32x16_t{};
+  }
+  int32_t const tiles = (all + kTile - 1) / kTile;
+  if (tiles > 0) {
+    load_k.load(lds, keys, wave);
+    load_v.load(lds + Tile<D>::kBytes, keys, wave);
+  }
+  for (int32_t tile = 0; tile < tiles; ++tile) {
+    LdsBytes const k_tile = lds + (tile & 1) * 2 * Tile<D>::kBytes, v_tile = k_tile + Tile<D>::kBytes;
+    stage_barrier<0>();
+    if (tile + 1 < tiles) {
+      LdsBytes const next = lds + (~tile & 1) * 2 * Tile<D>::kBytes;
+      load_k.load(next, keys - (tile + 1) * kTile, wave);
+      load_v.load(next + Tile<D>::kBytes, keys - (tile + 1) * kTile, wave);
+    }
+    int32_t const key0 = tile * kTile;
+    if (key0 >= most) continue;
+    f32x16_t s[NQ][2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) s[n][b] = f32x16_t{};
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step) {
+        Fragment<T> const k = read.rows(k_tile, b, step);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) s[n][b] = multiply32(k, q[n][step], s[n][b]);
       }
     }
-  }
+    if (key0 + kTile > least) {
 #pragma unroll
-  for (int c = 0; c < kMostWidth / kWave; ++c)
-    if (c * kWave + lane < f.width) {
-      f.k_grad.at(t, kh)[c * kWave + lane] = static_cast<T>(dk[c]);
-      f.v_grad.at(t, kh)[c * kWave + lane] = static_cast<T>(dv[c]);
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[n][b][r] = key0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4 < seen[n] ? s[n][b][r] : -INFINITY;
     }
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      float high = s[n][0][0];
+#pragma unroll
+      for (int r = 1; r < 32; ++r) high = fmaxf(high, s[n][r / 16][r % 16]);
+      Halves const both = halves(high);
+      high              = fmaxf(both.low, both.high) * scale;
+      // (a token that sees nothing yet keeps top at -infinity; NaN in a score is found in out at the end)
+      if (__ballot(high > top[n] + kSlack || top[n] == -INFINITY)) {
+        float const now  = fmaxf(top[n], high);
+        float const fade = now == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top[n] - now);
+        top[n]           = now;
+        sum[n] *= fade;
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[n][c][r] *= fade;
+      }
+      float const base = top[n] == -INFINITY ? 0.f : top[n];
+#pragma unroll
+      for (int r = 0; r < 32; ++r) {
+        float const p       = __builtin_amdgcn_exp2f(fmaf(s[n][r / 16][r % 16], scale, -base));
+        s[n][r / 16][r % 16] = p;
+        sum[n] += p;
+      }
+    }
+    Fragment<T> p[NQ][4];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int step = 0; step < 4; ++step) p[n][step] = rounded<T>(s[n][step / 2], step % 2);
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+      for (int step = 0; step < 4; ++step) {
+        Fragment<T> const v = read.columns(v_tile, c, step);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) o[n][c] = multiply32(v, p[n][step], o[n][c]);
+      }
+  }
+  if (wave0 >= rest) return;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    int32_t const i   = wave0 + n * 32 + column;
+    int64_t const t   = static_cast<int64_t>(begin) + block0 + i;
+    Halves const both = halves(sum[n]);
+    float const total = both.low + both.high, part = seen[n] > 0 ? 1.f / total : 0.f;
+    bool finite       = true;
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        o[n][c][r] *= part;
+        finite = finite && fabsf(o[n][c][r]) < INFINITY;
+      }
+    // What is not finite may come from keys that the token does not see, whose exponentials of 0 were multiplied: such tokens are done once more, by themselves.
+    uint64_t odd = __ballot(i < rest && seen[n] > 0 && !finite);
+    odd          = (odd | odd >> 32) & 0xffffffffu;
+    if (i < rest && !(odd >> column & 1)) {
+      T* const out = f.out.at(t, w.head);
+#pragma unroll
+      for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          int32_t const j = 32 * c + 8 * g + 4 * half;
+          typedef T Four __attribute__((ext_vector_type(4)));
+          Four const four = {static_cast<T>(o[n][c][4 * g]), static_cast<T>(o[n][c][4 * g + 1]), static_cast<T>(o[n][c][4 * g + 2]), static_cast<T>(o[n][c][4 * g + 3])};
+          if (j < f.width) *reinterpret_cast<Four*>(out + j) = four;
+        }
+      if (f.logsum && half == 0) f.logsum[static_cast<int64_t>(w.head) * f.runs.tokens + t] = seen[n] > 0 ? (top[n] + __builtin_amdgcn_logf(total)) * kLn2 : -INFINITY;
+    }
+    while (odd) {
+      int const which = __builtin_ctzll(odd);
+      odd &= odd - 1;
+      attend_row(f, static_cast<int32_t>(begin + block0 + wave0 + n * 32 + which), w.head);
+    }
+  }
 }
 
 template <typename T>
@@ -231,9 +226,38 @@ __global__ void __launch_bounds__(kThreads) key_gradient_rows_kernel(Backward<T>
 }
 
 // ------------------------------------------------------------------ launches
+// Whether the tiles' loads can read heads as they lie: pieces of 16 bytes, and lines of a tile within the 31 bits of their offsets.
+template <typename T>
+bool reads_as_it_lies(Heads<const T> const& x, int32_t width)
+{
+  constexpr int kEach = 16 / sizeof(T);
+  return width % kEach == 0 && x.stride % kEach == 0 && x.head_stride % kEach == 0 && reinterpret_cast<uintptr_t>(x.data) % 16 == 0 && x.stride < (int64_t{1} << 23);
+}
+
+template <typename T, int D, int WAVES, int NQ>
+nvtext_amd_status attend_tiles(Forward<T> const& f, hipStream_t stream)
+{
+  using Shape = ForwardShape<D, WAVES, NQ>;
+  ProfileScope const scope("attention_tiles", stream);
+  if constexpr (Shape::kLds > 65536) {
+    NVTEXT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(attend_tiles_kernel<T, D, WAVES, NQ>), hipFuncAttributeMaxDynamicSharedMemorySize, Shape::kLds));
+  }
+  int64_t const items = work_items(f.runs.template blocks<Shape::kShift>(), f.kv_heads, f.heads / f.kv_heads);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_tiles_kernel<T, D, WAVES, NQ>), grid_of(items, WAVES * kWave), dim3(WAVES * kWave), Shape::kLds, stream, f);
+  return NVTEXT_AMD_SUCCESS;
+}
+
 template <typename T>
 nvtext_amd_status attention(Forward<T> const& f, Mr const&, hipStream_t stream)
 {
+  if constexpr (sizeof(T) == 2) {
+    bool const four = f.out.stride % 4 == 0 && f.out.head_stride % 4 == 0 && reinterpret_cast<uintptr_t>(f.out.data) % 8 == 0;  // (as they are written)
+    if (f.width > 0 && four && reads_as_it_lies(f.q, f.width) && reads_as_it_lies(f.k, f.width) && reads_as_it_lies(f.v, f.width)) {
+      if (f.width <= 64) return attend_tiles<T, 64, 4, 1>(f, stream);
+      if (f.width <= 128) return attend_tiles<T, 128, 4, 1>(f, stream);
+      return attend_tiles<T, 256, 4, 1>(f, stream);
+    }
+  }
   ProfileScope const scope("attention_rows", stream);
   hipLaunchKernelGGL(attend_rows_kernel<T>, grid_of((static_cast<int64_t>(f.runs.tokens) * f.heads + 3) / 4, kThreads), dim3(kThreads), 0, stream, f);
   return NVTEXT_AMD_SUCCESS;
