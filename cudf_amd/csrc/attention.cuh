@@ -120,6 +120,7 @@ struct Backward : Problem<T> {
   Heads<const T> grad, out;
   const float* logsum;
   float* deltas;  // [heads, tokens]: grad . out
+  float* logs;    // [heads, tokens]: logsum in powers of 2 (the tiles' own)
   Heads<T> q_grad, k_grad, v_grad;
 };
 
@@ -241,7 +242,7 @@ struct TileLoader {
   {
     base  = reinterpret_cast<const char*>(x.at(first, head));
     line  = static_cast<uint32_t>(x.stride * 2);
-    width = static_cast<uint32_t>(columns * 2);
+    width = static_cast<uint32_t>((columns + 7) / 8 * 16);  // (whole pieces: those of an odd width have been copied, and end in zeros)
 #pragma unroll
     for (int p = 0; p < kLoads; ++p) {
       int const slot = (p * WAVES + wave) * kWave + lane, row = slot / Tile<D>::kPieces, piece = slot % Tile<D>::kPieces;
@@ -317,6 +318,28 @@ __device__ __forceinline__ Fragment<T> fragment_of(const T* head, int32_t j, int
   Fragment<T> f{};
   if (there && j < width) f = *reinterpret_cast<const Fragment<T>*>(head + j);
   return f;
+}
+
+// Writes a lane's column of results, transposed: values of a head, four next to each other (stores of 8 bytes take any
+// address that the type has), and those of a width that is no multiple of four one by one.
+template <typename T, int COLUMNS>
+__device__ __forceinline__ void store_columns(T* head, f32x16_t const (&x)[COLUMNS], int half, int32_t width)
+{
+  typedef T Four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+#pragma unroll
+  for (int c = 0; c < COLUMNS; ++c)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      int32_t const j = 32 * c + 8 * g + 4 * half;
+      Four const four = {static_cast<T>(x[c][4 * g]), static_cast<T>(x[c][4 * g + 1]), static_cast<T>(x[c][4 * g + 2]), static_cast<T>(x[c][4 * g + 3])};
+      if (j + 4 <= width) {
+        *reinterpret_cast<Four*>(head + j) = four;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (j + e < width) head[j + e] = four[e];
+      }
+    }
 }
 
 }  // namespace nvtext_amd

@@ -189,16 +189,7 @@ __global__ void __launch_bounds__(WAVES * kWave, 2) attend_tiles_kernel(Forward<
     uint64_t odd = __ballot(i < rest && seen[n] > 0 && !finite);
     odd          = (odd | odd >> 32) & 0xffffffffu;
     if (i < rest && !(odd >> column & 1)) {
-      T* const out = f.out.at(t, w.head);
-#pragma unroll
-      for (int c = 0; c < kColumns; ++c)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          int32_t const j = 32 * c + 8 * g + 4 * half;
-          typedef T Four __attribute__((ext_vector_type(4)));
-          Four const four = {static_cast<T>(o[n][c][4 * g]), static_cast<T>(o[n][c][4 * g + 1]), static_cast<T>(o[n][c][4 * g + 2]), static_cast<T>(o[n][c][4 * g + 3])};
-          if (j < f.width) *reinterpret_cast<Four*>(out + j) = four;
-        }
+      store_columns<T, kColumns>(f.out.at(t, w.head), o[n], half, f.width);
       if (f.logsum && half == 0) f.logsum[static_cast<int64_t>(w.head) * f.runs.tokens + t] = seen[n] > 0 ? (top[n] + __builtin_amdgcn_logf(total)) * kLn2 : -INFINITY;
     }
     while (odd) {
@@ -225,6 +216,269 @@ __global__ void __launch_bounds__(kThreads) key_gradient_rows_kernel(Backward<T>
   key_gradient_row(f, static_cast<int32_t>(w / f.kv_heads), static_cast<int32_t>(w % f.kv_heads));
 }
 
+// ------------------------------------------------------------------ the gradients, in tiles
+// Two launches, the first for q, the second for k and v: each makes the scores anew and adds up what is its own in registers, in one order at every
+// call.  (One launch for all three would have to add up q's gradient in memory, over all workgroups of keys: in parts of float32 or in any order.)
+template <int D, int WAVES>
+struct GradientShape {
+  static constexpr int kRows = 32 * WAVES, kShift = __builtin_ctz(kRows), kStage = 2 * Tile<D>::kBytes, kLds = 2 * kStage, kWavesASimd = D <= 128 ? 2 : 1;
+  static constexpr int kKeyStage = kStage + 2 * kTile * 4, kKeyLds = 2 * kKeyStage;  // (with logs and deltas)
+};
+
+// The gradient of q: as forward, a lane has a token's scores, and what they are multiplied with comes from LDS, keys as they lie and transposed.
+template <typename T, int D, int WAVES>
+__global__ void __launch_bounds__(WAVES * kWave, (GradientShape<D, WAVES>::kWavesASimd)) query_gradient_tiles_kernel(Backward<T> f)
+{
+  using Shape = GradientShape<D, WAVES>;
+  extern __shared__ __align__(16) char lds_[];
+  LdsBytes const lds = (LdsBytes)lds_;
+  constexpr int kSteps = D / 16, kColumns = D / 32;
+  Work w;
+  int32_t const each = f.heads / f.kv_heads;
+  if (!work_of(block_number(), f.runs.template blocks<Shape::kShift>(), f.kv_heads, each, w)) return;
+  int32_t const run    = f.runs.template run_of<Shape::kShift>(w.block);
+  int32_t const begin  = uniform(f.runs.begin(run)), tokens = uniform(f.runs.begin(run + 1)) - begin;
+  int64_t const in_run = (w.block - f.runs.template first_block<Shape::kShift>(run)) << Shape::kShift;
+  if (in_run >= tokens) return;
+  int const wave = uniform(threadIdx.x / kWave), lane = lane_id(), column = lane % 32, half = lane / 32;
+  int32_t const block0 = static_cast<int32_t>(in_run), rest = uniform(tokens - block0);
+  int32_t first = 0, keys = 0;
+  if (f.is_row(run)) f.keys_of(run, first, keys);
+  first = uniform(first);
+  keys  = uniform(keys);
+  int32_t const wave0 = wave * 32, wave1 = wave0 + 32 < rest ? wave0 + 32 : rest;
+  int32_t const all   = uniform(f.seen(block0 + (rest < Shape::kRows ? rest : Shape::kRows) - 1, tokens, keys));
+  int32_t const least = uniform(wave0 < rest ? f.seen(block0 + wave0, tokens, keys) : 0), most = uniform(wave0 < rest ? f.seen(block0 + wave1 - 1, tokens, keys) : 0);
+  bool const there    = wave0 + column < rest;
+  int64_t const t     = static_cast<int64_t>(begin) + block0 + (there ? wave0 + column : 0), at = static_cast<int64_t>(w.head) * f.runs.tokens + t;
+  int32_t const seen  = there ? f.seen(block0 + wave0 + column, tokens, keys) : 0;
+
+  Fragment<T> q[kSteps], g[kSteps];
+  float delta = 0.f;
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    q[s] = fragment_of(f.q.at(t, w.head), 16 * s + 8 * half, f.width, there);
+    g[s] = fragment_of(f.grad.at(t, w.head), 16 * s + 8 * half, f.width, there);
+    Fragment<T> const out = fragment_of(f.out.at(t, w.head), 16 * s + 8 * half, f.width, there);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) delta = fmaf(static_cast<float>(g[s][k]), static_cast<float>(out[k]), delta);
+  }
+  Halves const both = halves(delta);
+  delta             = seen > 0 ? both.low + both.high : 0.f;
+  float const log   = there ? f.logsum[at] * kLog2e : 0.f;
+  if (there && half == 0) {
+    f.deltas[at] = delta;
+    f.logs[at]   = log;
+  }
+  TileLoader<D, WAVES> load_k, load_v;
+  load_k.aim(f.k, first, w.kv_head, f.width, wave, lane);
+  load_v.aim(f.v, first, w.kv_head, f.width, wave, lane);
+  TileReader<T, D> const read(lane);
+  float const scale = f.scale * kLog2e;
+  f32x16_t d[kColumns];
+#pragma unroll
+  for (int c = 0; c < kColumns; ++c) d[c] = f32x16_t{};
+  int32_t const tiles = (all + kTile - 1) / kTile;
+  if (tiles > 0) {
+    load_k.load(lds, keys, wave);
+    load_v.load(lds + Tile<D>::kBytes, keys, wave);
+  }
+  for (int32_t tile = 0; tile < tiles; ++tile) {
+    LdsBytes const k_tile = lds + (tile & 1) * Shape::kStage, v_tile = k_tile + Tile<D>::kBytes;
+    stage_barrier<0>();
+    if (tile + 1 < tiles) {
+      LdsBytes const next = lds + (~tile & 1) * Shape::kStage;
+      load_k.load(next, keys - (tile + 1) * kTile, wave);
+      load_v.load(next + Tile<D>::kBytes, keys - (tile + 1) * kTile, wave);
+    }
+    int32_t const key0 = tile * kTile;
+    if (key0 >= most) continue;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      f32x16_t s{}, p{};
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step) s = multiply32(read.rows(k_tile, b, step), q[step], s);
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step) p = multiply32(read.rows(v_tile, b, step), g[step], p);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], scale, -log)) * (p[r] - delta);
+      if (key0 + 32 * b + 32 > least) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = key0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4 < seen ? s[r] : 0.f;
+      }
+#pragma unroll
+      for (int step = 0; step < 2; ++step) {
+        Fragment<T> const ds = rounded<T>(s, step);
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c) d[c] = multiply32(read.columns(k_tile, c, 2 * b + step), ds, d[c]);
+      }
+    }
+  }
+  if (wave0 >= rest) return;
+  bool finite = true;
+#pragma unroll
+  for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      d[c][r] *= f.scale;
+      finite = finite && fabsf(d[c][r]) < INFINITY;
+    }
+  // (as forward: a key that is not seen may have been multiplied by 0)
+  uint64_t odd = __ballot(there && seen > 0 && !finite);
+  odd          = (odd | odd >> 32) & 0xffffffffu;
+  if (there && !(odd >> column & 1)) store_columns<T, kColumns>(f.q_grad.at(t, w.head), d, half, f.width);
+  while (odd) {
+    int const which = __builtin_ctzll(odd);
+    odd &= odd - 1;
+    query_gradient_row(f, begin + block0 + wave0 + which, w.head);
+  }
+}
+
+// The gradients of k and v: a wavefront has 32 keys in its registers, a lane a key's scores, and the tokens of all heads that see them come through LDS
+// with their gradients, 64 at a time, with their logs and deltas.
+template <typename T, int D, int WAVES>
+__global__ void __launch_bounds__(WAVES * kWave, (GradientShape<D, WAVES>::kWavesASimd)) key_gradient_tiles_kernel(Backward<T> f)
+{
+  using Shape = GradientShape<D, WAVES>;
+  extern __shared__ __align__(16) char lds_[];
+  LdsBytes const lds = (LdsBytes)lds_;
+  constexpr int kSteps = D / 16, kColumns = D / 32;
+  Work w;
+  if (!work_of(block_number(), f.key_runs.template blocks<Shape::kShift>(), f.kv_heads, 1, w)) return;
+  w.block              = f.key_runs.template blocks<Shape::kShift>() - 1 - w.block;  // (of a long row, the first keys are those that most tokens see)
+  int32_t const run    = f.key_runs.template run_of<Shape::kShift>(w.block), each = f.heads / f.kv_heads;
+  int32_t const first  = uniform(f.key_runs.begin(run)), places = uniform(f.key_runs.begin(run + 1)) - first;
+  int64_t const in_run = (w.block - f.key_runs.template first_block<Shape::kShift>(run)) << Shape::kShift;
+  if (in_run >= places) return;
+  int const wave = uniform(threadIdx.x / kWave), lane = lane_id(), column = lane % 32, half = lane / 32;
+  int32_t const block0 = static_cast<int32_t>(in_run), rest = uniform(places - block0);  // (places: with those behind the row's keys, whose gradients are zeros)
+  int32_t begin = 0, tokens = 0, keys = 0, ignored = 0;
+  if (f.is_row(run)) {
+    f.keys_of(run, ignored, keys);
+    begin  = f.runs.begin(run);
+    tokens = f.runs.begin(run + 1) - begin;
+  }
+  begin  = uniform(begin);
+  tokens = uniform(tokens > 0 ? tokens : 0);
+  keys   = uniform(keys);
+  int32_t const wave0 = wave * 32;
+  bool const there    = wave0 + column < rest;
+  int32_t const key   = block0 + wave0 + column;
+  int64_t const t     = static_cast<int64_t>(first) + (there ? key : block0);
+  // the first token that sees a key, of the row's
+  auto const from_of = [&](int32_t j) {
+    int64_t const i = f.causal ? static_cast<int64_t>(j) + tokens - keys : 0;
+    return static_cast<int32_t>(i < 0 ? 0 : i < tokens ? i : tokens);
+  };
+  int32_t const from = from_of(key), start = uniform(block0 < keys ? from_of(block0) / kTile : 0), tiles = uniform(block0 < keys ? (tokens + kTile - 1) / kTile : 0);
+  int32_t const last_from = uniform(from_of(block0 + wave0 + 31)), first_from = uniform(from_of(block0 + wave0));
+
+  Fragment<T> k[kSteps], v[kSteps];
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    k[s] = fragment_of(f.k.at(t, w.kv_head), 16 * s + 8 * half, f.width, there && key < keys);
+    v[s] = fragment_of(f.v.at(t, w.kv_head), 16 * s + 8 * half, f.width, there && key < keys);
+  }
+  TileReader<T, D> const read(lane);
+  float const scale = f.scale * kLog2e;
+  f32x16_t dk[kColumns], dv[kColumns];
+#pragma unroll
+  for (int c = 0; c < kColumns; ++c) dk[c] = dv[c] = f32x16_t{};
+  // The tiles of one head after another are one stream of loads.
+  int32_t const of_head = tiles - start > 0 ? tiles - start : 0, total = of_head * each;
+  TileLoader<D, WAVES> load_q, load_g;
+  int32_t loaded = 0, next_head = w.kv_head * each;  // the tile of the head that is loaded next
+  auto const load = [&](LdsBytes to) {
+    if (loaded == 0) {
+      load_q.aim(f.q, begin + start * kTile, next_head, f.width, wave, lane);
+      load_g.aim(f.grad, begin + start * kTile, next_head, f.width, wave, lane);
+    }
+    int32_t const token = (start + loaded) * kTile, here = tokens - token;
+    load_q.load(to, here, wave);
+    load_g.load(to + Tile<D>::kBytes, here, wave);
+    int64_t const at = static_cast<int64_t>(next_head) * f.runs.tokens + begin + token;
+    uint32_t const range = static_cast<uint32_t>(here < kTile ? here : kTile) * 4;
+    if (wave == 0) load_words_to_lds(reinterpret_cast<const char*>(f.logs + at), range, to + Shape::kStage, lane * 4);
+    if (wave == WAVES - 1) load_words_to_lds(reinterpret_cast<const char*>(f.deltas + at), range, to + Shape::kStage + kTile * 4, lane * 4);
+    if (++loaded == of_head) {
+      loaded = 0;
+      ++next_head;
+    }
+  };
+  if (total > 0) load(lds);
+  int32_t tile = start - 1;
+  for (int32_t n = 0; n < total; ++n) {
+    LdsBytes const q_tile = lds + (n & 1) * Shape::kKeyStage, g_tile = q_tile + Tile<D>::kBytes, words = q_tile + Shape::kStage + 16 * half;
+    stage_barrier<0>();
+    if (n + 1 < total) load(lds + (~n & 1) * Shape::kKeyStage);
+    if (++tile == tiles) tile = start;
+    int32_t const token0 = tile * kTile;
+    if (token0 + kTile <= first_from) continue;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      f32x16_t s{}, p{};
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step) s = multiply32(read.rows(q_tile, b, step), k[step], s);
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step) p = multiply32(read.rows(g_tile, b, step), v[step], p);
+      int32_t const row0 = token0 + 32 * b;
+      bool const partly  = row0 < last_from || row0 + 32 > tokens;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f32x4_t const log   = *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(words + 128 * b + 32 * i);
+        f32x4_t const delta = *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(words + kTile * 4 + 128 * b + 32 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          int const r = 4 * i + e;
+          s[r]        = __builtin_amdgcn_exp2f(fmaf(s[r], scale, -log[e]));
+          p[r]        = s[r] * (p[r] - delta[e]);
+        }
+      }
+      if (partly) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          int32_t const i = row0 + 8 * (r / 4) + 4 * half + r % 4;
+          bool const sees = i >= from && i < tokens;
+          s[r]            = sees ? s[r] : 0.f;
+          p[r]            = sees ? p[r] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int step = 0; step < 2; ++step) {
+        Fragment<T> const weight = rounded<T>(s, step), ds = rounded<T>(p, step);
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c) dv[c] = multiply32(read.columns(g_tile, c, 2 * b + step), weight, dv[c]);
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c) dk[c] = multiply32(read.columns(q_tile, c, 2 * b + step), ds, dk[c]);
+      }
+    }
+  }
+  if (wave0 >= rest) return;
+  bool finite = true;
+#pragma unroll
+  for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      dk[c][r] *= f.scale;
+      finite = finite && fabsf(dk[c][r]) < INFINITY && fabsf(dv[c][r]) < INFINITY;
+    }
+  uint64_t odd = __ballot(there && key < keys && !finite);
+  odd          = (odd | odd >> 32) & 0xffffffffu;
+  if (there && !(odd >> column & 1)) {
+    if (key >= keys) {
+#pragma unroll
+      for (int c = 0; c < kColumns; ++c) dk[c] = dv[c] = f32x16_t{};
+    }
+    store_columns<T, kColumns>(f.k_grad.at(t, w.kv_head), dk, half, f.width);
+    store_columns<T, kColumns>(f.v_grad.at(t, w.kv_head), dv, half, f.width);
+  }
+  while (odd) {
+    int const which = __builtin_ctzll(odd);
+    odd &= odd - 1;
+    key_gradient_row(f, first + block0 + wave0 + which, w.kv_head);
+  }
+}
+
 // ------------------------------------------------------------------ launches
 // Whether the tiles' loads can read heads as they lie: pieces of 16 bytes, and lines of a tile within the 31 bits of their offsets.
 template <typename T>
@@ -233,6 +487,83 @@ bool reads_as_it_lies(Heads<const T> const& x, int32_t width)
   constexpr int kEach = 16 / sizeof(T);
   return width % kEach == 0 && x.stride % kEach == 0 && x.head_stride % kEach == 0 && reinterpret_cast<uintptr_t>(x.data) % 16 == 0 && x.stride < (int64_t{1} << 23);
 }
+
+// Heads that the tiles cannot read are copied first: head after head, token after token, each filled up with zeros to a multiple of 16 bytes.
+template <typename T>
+struct Copy {
+  static constexpr int kEach = 16 / sizeof(T);
+  Heads<const T> from;
+  T* to;
+  int64_t tokens, pieces;  // of all heads; 0: nothing to copy
+};
+constexpr int kCopies = 5;
+template <typename T>
+struct Copies {
+  Copy<T> copy[kCopies];
+  int32_t width;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) copy_heads_kernel(Copies<T> c)
+{
+  constexpr int kEach   = Copy<T>::kEach;
+  int64_t item          = block_number() * kThreads + threadIdx.x;
+  int32_t const of_head = (c.width + kEach - 1) / kEach;
+#pragma unroll
+  for (int n = 0; n < kCopies; ++n) {
+    Copy<T> const& x = c.copy[n];
+    if (item >= 0 && item < x.pieces) {
+      int64_t const head = item / of_head / x.tokens, t = item / of_head % x.tokens, j = item % of_head * kEach;
+      const T* const from = x.from.at(t, head) + j;
+      typedef T Piece __attribute__((ext_vector_type(kEach)));
+      Piece p{};
+#pragma unroll
+      for (int k = 0; k < kEach; ++k)
+        if (j + k < c.width) p[k] = from[k];
+      *reinterpret_cast<Piece*>(x.to + item * kEach) = p;
+    }
+    item -= x.pieces;
+  }
+}
+
+// Which of up to five heads are copied, what that takes, and the launch that does it.
+template <typename T>
+struct Alignment {
+  Copies<T> copies{};
+  Heads<const T>* heads[kCopies]{};
+  int count{0};
+  explicit Alignment(int32_t width) { copies.width = width; }
+  void add(Heads<const T>& x, int64_t tokens, int64_t of_token)
+  {
+    heads[count]  = &x;
+    Copy<T>& c    = copies.copy[count++];
+    c.from        = x;
+    c.tokens      = tokens;
+    c.pieces      = reads_as_it_lies(x, copies.width) ? 0 : tokens * of_token * ((copies.width + Copy<T>::kEach - 1) / Copy<T>::kEach);
+  }
+  size_t bytes() const
+  {
+    size_t sum = 0;
+    for (auto const& c : copies.copy) sum += static_cast<size_t>(c.pieces) * 16;
+    return sum;
+  }
+  void launch(char* memory, hipStream_t stream)
+  {
+    int64_t all = 0;
+    for (int n = 0; n < count; ++n) {
+      Copy<T>& c = copies.copy[n];
+      if (c.pieces == 0) continue;
+      int64_t const line = (copies.width + Copy<T>::kEach - 1) / Copy<T>::kEach * Copy<T>::kEach;
+      c.to               = reinterpret_cast<T*>(memory);
+      *heads[n]          = {c.to, line, c.tokens * line};
+      memory += c.pieces * 16;
+      all += c.pieces;
+    }
+    if (all == 0) return;
+    ProfileScope const scope("attention_copy", stream);
+    hipLaunchKernelGGL(copy_heads_kernel<T>, grid_of((all + kThreads - 1) / kThreads, kThreads), dim3(kThreads), 0, stream, copies);
+  }
+};
 
 template <typename T, int D, int WAVES, int NQ>
 nvtext_amd_status attend_tiles(Forward<T> const& f, hipStream_t stream)
@@ -248,11 +579,17 @@ nvtext_amd_status attend_tiles(Forward<T> const& f, hipStream_t stream)
 }
 
 template <typename T>
-nvtext_amd_status attention(Forward<T> const& f, Mr const&, hipStream_t stream)
+nvtext_amd_status attention(Forward<T> f, Mr const& mr, hipStream_t stream)
 {
   if constexpr (sizeof(T) == 2) {
-    bool const four = f.out.stride % 4 == 0 && f.out.head_stride % 4 == 0 && reinterpret_cast<uintptr_t>(f.out.data) % 8 == 0;  // (as they are written)
-    if (f.width > 0 && four && reads_as_it_lies(f.q, f.width) && reads_as_it_lies(f.k, f.width) && reads_as_it_lies(f.v, f.width)) {
+    if (f.width > 0) {
+      Alignment<T> align(f.width);
+      align.add(f.q, f.runs.tokens, f.heads);
+      align.add(f.k, f.key_runs.tokens, f.kv_heads);
+      align.add(f.v, f.key_runs.tokens, f.kv_heads);
+      Temp const copies(mr, align.bytes());
+      if (!copies.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
+      align.launch(copies.template as<char>(), stream);
       if (f.width <= 64) return attend_tiles<T, 64, 4, 1>(f, stream);
       if (f.width <= 128) return attend_tiles<T, 128, 4, 1>(f, stream);
       return attend_tiles<T, 256, 4, 1>(f, stream);
@@ -263,12 +600,49 @@ nvtext_amd_status attention(Forward<T> const& f, Mr const&, hipStream_t stream)
   return NVTEXT_AMD_SUCCESS;
 }
 
+template <typename T, int D, int WAVES>
+nvtext_amd_status gradient_tiles(Backward<T> const& f, hipStream_t stream)
+{
+  using Shape = GradientShape<D, WAVES>;
+  if constexpr (Shape::kKeyLds > 65536) {
+    NVTEXT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(query_gradient_tiles_kernel<T, D, WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, Shape::kLds));
+    NVTEXT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(key_gradient_tiles_kernel<T, D, WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, Shape::kKeyLds));
+  }
+  if (f.runs.tokens > 0) {
+    ProfileScope const scope("attention_query_gradient", stream);
+    int64_t const items = work_items(f.runs.template blocks<Shape::kShift>(), f.kv_heads, f.heads / f.kv_heads);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(query_gradient_tiles_kernel<T, D, WAVES>), grid_of(items, WAVES * kWave), dim3(WAVES * kWave), Shape::kLds, stream, f);
+  }
+  if (f.key_runs.tokens > 0) {
+    ProfileScope const scope("attention_key_gradient", stream);
+    int64_t const items = work_items(f.key_runs.template blocks<Shape::kShift>(), f.kv_heads, 1);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(key_gradient_tiles_kernel<T, D, WAVES>), grid_of(items, WAVES * kWave), dim3(WAVES * kWave), Shape::kKeyLds, stream, f);
+  }
+  return NVTEXT_AMD_SUCCESS;
+}
+
 template <typename T>
 nvtext_amd_status attention_backward(Backward<T> f, Mr const& mr, hipStream_t stream)
 {
-  Temp const deltas(mr, static_cast<size_t>(f.heads) * static_cast<size_t>(f.runs.tokens) * sizeof(float));
-  if (!deltas.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
-  f.deltas = deltas.template as<float>();
+  bool const tiles = sizeof(T) == 2 && f.width > 0;
+  Alignment<T> align(f.width);
+  if (tiles) {
+    for (auto* x : {&f.q, &f.grad, &f.out}) align.add(*x, f.runs.tokens, f.heads);
+    for (auto* x : {&f.k, &f.v}) align.add(*x, f.key_runs.tokens, f.kv_heads);
+  }
+  size_t const values = static_cast<size_t>(f.heads) * static_cast<size_t>(f.runs.tokens) * sizeof(float);
+  TempParts<3> const temp(mr, {values, tiles ? values : 0, align.bytes()});
+  if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
+  f.deltas = temp.template part<float>(0);
+  f.logs   = temp.template part<float>(1);
+  align.launch(temp.template part<char>(2), stream);
+  if constexpr (sizeof(T) == 2) {
+    if (tiles) {
+      if (f.width <= 64) return gradient_tiles<T, 64, 4>(f, stream);
+      if (f.width <= 128) return gradient_tiles<T, 128, 4>(f, stream);
+      return gradient_tiles<T, 256, 4>(f, stream);
+    }
+  }
   if (f.runs.tokens > 0) {
     ProfileScope const scope("attention_query_gradient", stream);
     hipLaunchKernelGGL(query_gradient_rows_kernel<T>, grid_of((static_cast<int64_t>(f.runs.tokens) * f.heads + 3) / 4, kThreads), dim3(kThreads), 0, stream, f);

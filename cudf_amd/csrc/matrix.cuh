@@ -32,6 +32,15 @@ __device__ __forceinline__ void load_to_lds(const char* base, uint32_t range, Ld
                : "memory");  // (m0 is set wherever the compiler uses it itself)
 }
 
+// The same with 4 bytes a lane.
+__device__ __forceinline__ void load_words_to_lds(const char* base, uint32_t range, LdsBytes to, uint32_t offset)
+{
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  uint64_t const address = reinterpret_cast<uint64_t>(base);
+  u32x4 const buffer = {static_cast<uint32_t>(address), static_cast<uint32_t>(address >> 32) & 0xffffu, range, 0x00027000u};
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to))), "v"(offset), "s"(buffer) : "memory");
+}
+
 // All wavefronts have come here, their reads of LDS are done, and of the loads of each all but the last N.  (Written out: a fence in
 // front of the barrier would wait for all loads, because they write LDS.)
 template <int N>

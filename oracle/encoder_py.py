@@ -180,9 +180,10 @@ def _rows_seen(offsets, key_offsets, key_lengths, causal):
         yield t, u, (j <= i + count - (t.stop - t.start)) if causal else np.ones((len(i), count), bool)
 
 
-def attention(q, k, v, offsets, key_offsets=None, key_lengths=None, causal=False, scale=None, unit=0.0, eps=2.0**-24):
+def attention(q, k, v, offsets, key_offsets=None, key_lengths=None, causal=False, scale=None, unit=0.0, tiny=0.0, eps=2.0**-24):
     """(out, logsum [heads, tokens], what a kernel's out may be off by before it is rounded, the same for logsum).  unit: by how much of itself
-    an exponential may be off that is rounded before it is multiplied.  A score of `width` products held in 32 bits is off by
+    an exponential may be off that is rounded before it is multiplied, tiny: by how much where it is smaller than its type's normal
+    numbers (next to a sum of at least 1, that of the largest score).  A score of `width` products held in 32 bits is off by
     eps a product and addition, in proportion to the magnitudes that it adds up, twice where they are cut off instead of
     rounded; its difference from the largest score or the logsum by eps of both; the exponential follows."""
     q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
@@ -204,7 +205,7 @@ def attention(q, k, v, offsets, key_offsets=None, key_lengths=None, causal=False
                 out[at, h] = p @ vv
                 score_off = score_error(scale * (np.abs(kk) @ np.abs(q[at, h])), abs(top), width, eps)
                 worst = score_off.max()
-                off[at, h] = (p * (unit + score_off + worst + 2 * (len(keys) + 8) * eps)) @ np.abs(vv)
+                off[at, h] = (p * (unit + score_off + worst + 2 * (len(keys) + 8) * eps) + tiny) @ np.abs(vv)
                 log_off[h, at] = worst + 2 * (len(keys) + 8) * eps
     return out, logsum, off, log_off
 
@@ -213,7 +214,7 @@ def score_error(size, top, width, eps):
     return eps * (2 * (width + 4) * size + 4 * top + 8)
 
 
-def attention_backward(grad, q, k, v, out, logsum, offsets, key_offsets=None, key_lengths=None, causal=False, scale=None, unit=0.0, eps=2.0**-24):
+def attention_backward(grad, q, k, v, out, logsum, offsets, key_offsets=None, key_lengths=None, causal=False, scale=None, unit=0.0, tiny=0.0, eps=2.0**-24):
     """((gradients of q, k, v), (what a kernel's may be off by before they are rounded)), from out and logsum as they are given."""
     grad, q, k, v, out, logsum = (np.asarray(x, np.float64) for x in (grad, q, k, v, out, logsum))
     key_offsets = offsets if key_offsets is None else key_offsets
@@ -231,12 +232,12 @@ def attention_backward(grad, q, k, v, out, logsum, offsets, key_offsets=None, ke
             ds = p * (dp - delta)
             e = score_error(scale * (np.abs(qh) @ np.abs(kh).T), np.abs(log), width, eps) + 8 * eps
             dp_off = 2 * (width + 4) * eps * (np.abs(gh) @ np.abs(vh).T + (np.abs(gh) * np.abs(oh)).sum(1)[:, None])
-            ds_off = 1.1 * (np.abs(ds) * (unit + e) + p * dp_off)
+            ds_off = 1.1 * (np.abs(ds) * (unit + e) + p * dp_off) + np.where(sees, tiny, 0.0)
             longest = 2 * (max(s.shape) * each + 8) * eps
             results[0][t, h] = scale * (ds @ kh)
             offs[0][t, h] = scale * ((ds_off + longest * np.abs(ds)) @ np.abs(kh))
             results[1][u, h // each] += scale * (ds.T @ qh)
             offs[1][u, h // each] += scale * ((ds_off + longest * np.abs(ds)).T @ np.abs(qh))
             results[2][u, h // each] += p.T @ gh
-            offs[2][u, h // each] += (1.1 * p * (unit + e + longest)).T @ np.abs(gh)
+            offs[2][u, h // each] += (1.1 * p * (unit + e + longest) + np.where(sees, tiny, 0.0)).T @ np.abs(gh)
     return results, offs

@@ -14,9 +14,13 @@ pytestmark = pytest.mark.gpu
 
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 UNIT = {F32: 2.0**-24, F16: 2.0**-11, BF16: 2.0**-8}
-ROUNDED = {F32: 0.0, F16: 2.0**-11, BF16: 2.0**-8}  # what is rounded before it is multiplied
 TINY = {F32: 2.0**-149, F16: 2.0**-24, BF16: 2.0**-133}
 TYPES = [F32, F16, BF16]
+
+
+def rounding(dtype):
+    """How far what is rounded before it is multiplied may be off: half a step of its value, or of the smallest one."""
+    return {F32: dict(unit=0.0), F16: dict(unit=2.0**-11, tiny=2.0**-25), BF16: dict(unit=2.0**-8)}[dtype]
 
 
 def near(got, want, off, dtype=None):
@@ -162,7 +166,7 @@ class Made:
         return dict(offsets=self.offsets, key_offsets=self.key_offsets, key_lengths=self.key_lengths)
 
     def check_forward(self, causal, scale=None):
-        want, log, off, log_off = orc.attention(self.q64, self.k64, self.v64, **self.oracle_rows(), causal=causal, scale=scale, unit=ROUNDED[self.dtype])
+        want, log, off, log_off = orc.attention(self.q64, self.k64, self.v64, **self.oracle_rows(), causal=causal, scale=scale, **rounding(self.dtype))
         out, saved = encoder.attention(self.q, self.k, self.v, *self.rows(), causal=causal, scale=scale, keep=True)
         assert saved.out is out
         near(out, want, off)
@@ -174,8 +178,7 @@ class Made:
         want, log, _, _ = orc.attention(self.q64, self.k64, self.v64, **self.oracle_rows(), causal=causal, scale=scale)
         out = torch.from_numpy(want).to(self.dtype).cuda()
         logsum = torch.from_numpy(log).float().cuda()
-        wants, offs = orc.attention_backward(self.g64, self.q64, self.k64, self.v64, out.double().cpu().numpy(), logsum.double().cpu().numpy(), **self.oracle_rows(), causal=causal, scale=scale,
-                                             unit=ROUNDED[self.dtype])
+        wants, offs = orc.attention_backward(self.g64, self.q64, self.k64, self.v64, out.double().cpu().numpy(), logsum.double().cpu().numpy(), **self.oracle_rows(), causal=causal, scale=scale, **rounding(self.dtype))
         saved = encoder.AttentionSaved(out, logsum)
         got = encoder.attention_backward(self.g, self.q, self.k, self.v, saved, *self.rows(), causal=causal, scale=scale)
         for name, x, w, o in zip("qkv", got, wants, offs):
@@ -231,7 +234,7 @@ def test_scores_far_apart():
             q = torch.ones(1, 1, width, dtype=dtype, device="cuda")
             k = torch.from_numpy(np.arange(n)[::order].astype(np.float64)[:, None, None] * np.ones(width)).to(dtype).cuda()
             v, v64 = heads(rng, n, 1, width, dtype)
-            want, log, off, log_off = orc.attention(q.double().cpu().numpy(), k.double().cpu().numpy(), v64, [0, 1], [0, n], unit=ROUNDED[dtype])
+            want, log, off, log_off = orc.attention(q.double().cpu().numpy(), k.double().cpu().numpy(), v64, [0, 1], [0, n], **rounding(dtype))
             out, saved = encoder.attention(q, k, v, ints([0, 1]), ints([0, n]), keep=True)
             near(out, want, off)
             near(saved.logsum, log, log_off)
@@ -243,7 +246,7 @@ def test_what_is_not_seen_has_no_effect(dtype, value):
     """A token's k and v, and what lies in no row, are anything at all: the tokens that do not see them have what they have without."""
     m = Made(([70, 40, 130], None, 4, 2, 64, 0), dtype)
     bad = int(m.offsets[1]) + 21  # a token of the second row
-    want, log, off, log_off = orc.attention(m.q64, m.k64, m.v64, m.offsets, causal=True, unit=ROUNDED[dtype])
+    want, log, off, log_off = orc.attention(m.q64, m.k64, m.v64, m.offsets, causal=True, **rounding(dtype))
     grads = None
     for where in ("k", "v", "both"):
         q, k, v, g = m.q.clone(), m.k.clone(), m.v.clone(), m.g.clone()
@@ -264,7 +267,7 @@ def test_what_is_not_seen_has_no_effect(dtype, value):
         clean = encoder.attention(m.q, m.k, m.v, ints(m.offsets), causal=True, keep=True)[1]
         saved = encoder.AttentionSaved(torch.where(pick[:, None, None], clean.out, out), torch.where(pick[None], clean.logsum, saved.logsum))
         grads = encoder.attention_backward(g, q, k, v, saved, ints(m.offsets), causal=True)
-        wants, offs = orc.attention_backward(m.g64, m.q64, m.k64, m.v64, clean.out.double().cpu().numpy(), clean.logsum.double().cpu().numpy(), m.offsets, causal=True, unit=ROUNDED[dtype])
+        wants, offs = orc.attention_backward(m.g64, m.q64, m.k64, m.v64, clean.out.double().cpu().numpy(), clean.logsum.double().cpu().numpy(), m.offsets, causal=True, **rounding(dtype))
         near(grads[0][pick], wants[0][untouched], offs[0][untouched])
         others = np.ones(len(q), bool)
         others[int(m.offsets[1]):int(m.offsets[2])] = False
@@ -280,7 +283,7 @@ def test_what_is_not_seen_has_no_effect(dtype, value):
     pick = torch.from_numpy(others).cuda()
     near(out[pick], want[others], off[others])
     grads = encoder.attention_backward(g, q, m.k, m.v, saved, ints(m.offsets), causal=True)
-    wants, offs = orc.attention_backward(m.g64, m.q64, m.k64, m.v64, clean.out.double().cpu().numpy(), clean.logsum.double().cpu().numpy(), m.offsets, causal=True, unit=ROUNDED[dtype])
+    wants, offs = orc.attention_backward(m.g64, m.q64, m.k64, m.v64, clean.out.double().cpu().numpy(), clean.logsum.double().cpu().numpy(), m.offsets, causal=True, **rounding(dtype))
     near(grads[0][pick], wants[0][others], offs[0][others])
     behind = np.ones(len(q), bool)
     behind[int(m.offsets[1]):bad + 1] = False
@@ -368,7 +371,7 @@ def test_rows_at_odd_places():
                 y.copy_(x)
                 return y
             q, k, v, g = odd(m.q), odd(m.k), odd(m.v), odd(m.g)
-            want, log, off, log_off = orc.attention(m.q64, m.k64, m.v64, m.offsets, causal=True, unit=ROUNDED[dtype])
+            want, log, off, log_off = orc.attention(m.q64, m.k64, m.v64, m.offsets, causal=True, **rounding(dtype))
             got, kept = encoder.attention(q, k, v, *m.rows(), causal=True, keep=True)
             near(got, want, off)
             near(kept.logsum, log, log_off)
@@ -413,10 +416,10 @@ def test_many_short_rows():
         out, saved = encoder.attention(q, q, q, ints(offsets), keep=True)
         g, g64 = heads(rng, tokens, 2, 16, dtype)
         grads = encoder.attention_backward(g, q, q, q, saved, ints(offsets))
-        want, log, off, log_off = orc.attention(q64, q64, q64, offsets, unit=ROUNDED[dtype])
+        want, log, off, log_off = orc.attention(q64, q64, q64, offsets, **rounding(dtype))
         near(out, want, off)
         near(saved.logsum, log, log_off)
-        wants, offs = orc.attention_backward(g64, q64, q64, q64, out.double().cpu().numpy(), saved.logsum.double().cpu().numpy(), offsets, unit=ROUNDED[dtype])
+        wants, offs = orc.attention_backward(g64, q64, q64, q64, out.double().cpu().numpy(), saved.logsum.double().cpu().numpy(), offsets, **rounding(dtype))
         for x, w, o in zip(grads, wants, offs):
             near(x, w, o)
 
