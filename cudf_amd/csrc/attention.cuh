@@ -161,9 +161,9 @@ __device__ void query_gradient_row(Backward<T> const& f, int32_t t, int32_t h)
     if (c * kWave + lane < f.width) f.q_grad.at(t, h)[c * kWave + lane] = static_cast<T>(d[c]);
 }
 
-// The gradients of key token t's head kh of k and v.
+// The gradients of key token t's head kh of k and v, those that are wanted.
 template <typename T>
-__device__ void key_gradient_row(Backward<T> const& f, int32_t t, int32_t kh)
+__device__ void key_gradient_row(Backward<T> const& f, int32_t t, int32_t kh, bool of_k, bool of_v)
 {
   int const lane    = lane_id();
   int32_t const run = run_with(f.key_runs, t), each = f.heads / f.kv_heads;
@@ -201,8 +201,8 @@ __device__ void key_gradient_row(Backward<T> const& f, int32_t t, int32_t kh)
 #pragma unroll
   for (int c = 0; c < kMostWidth / kWave; ++c)
     if (c * kWave + lane < f.width) {
-      f.k_grad.at(t, kh)[c * kWave + lane] = static_cast<T>(dk[c]);
-      f.v_grad.at(t, kh)[c * kWave + lane] = static_cast<T>(dv[c]);
+      if (of_k) f.k_grad.at(t, kh)[c * kWave + lane] = static_cast<T>(dk[c]);
+      if (of_v) f.v_grad.at(t, kh)[c * kWave + lane] = static_cast<T>(dv[c]);
     }
 }
 
@@ -213,79 +213,107 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 __device__ __forceinline__ f32x16_t multiply32(Fragment<bf16_t> a, Fragment<bf16_t> b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16_t multiply32(Fragment<half_t> a, Fragment<half_t> b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
-constexpr int kTile = 64;  // tokens or keys of a tile in LDS
+// (2 deep, eight times: value k of every lane of a half goes into product k)
+__device__ __forceinline__ f32x16_t multiply32(Fragment<float> a, Fragment<float> b, f32x16_t c)
+{
+#pragma unroll
+  for (int k = 0; k < 8; ++k) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[k], b[k], c, 0, 0, 0);
+  return c;
+}
 
-// A tile of kTile heads of D values (a multiple of 32), as it lies in LDS: 2 * D bytes a head, in units of 32 bytes whose order is turned with the head's
-// number, so that 8 neighbouring heads' units of one number lie in different banks (the reads of rows), and so do two neighbouring units of 4
-// neighbouring heads (the transposing reads).  What turns them depends on where heads begin within the 256 bytes of all banks.
-template <int D>
+// A tile of heads of D values (a multiple of 32) of as many tokens or keys, as it lies in LDS: in units of 32 bytes, whose order is turned with the head's
+// number, so that units of one number of 8 neighbouring heads lie in different banks (the reads of rows), and so does what the reads of columns
+// ask for at once: two neighbouring units of 4 heads, or (32-bit types) 4 units of a head and of the one 4 further on.  What turns them depends on
+// where heads begin within the 256 bytes of all banks.
+template <typename T, int D>
 struct Tile {
-  static constexpr int kBytes = kTile * D * 2, kPieces = D / 8;  // pieces of 16 bytes of a head
+  static constexpr int kHeads = D * sizeof(T) > 512 ? 32 : 64;  // two tiles of each, twice, fill no more than 128 KB
+  static constexpr int kLine = D * sizeof(T), kBytes = kHeads * kLine, kPieces = kLine / 16;  // bytes of a head, of all, pieces of 16 bytes of a head
   __device__ __forceinline__ static constexpr uint32_t turn(uint32_t head)
   {
-    if constexpr (D % 128 == 0) return (head & 3) << 1 | (head >> 2 & 1);
-    if constexpr (D % 64 == 0) return head & 2 | (head >> 2 & 1);
+    if constexpr (kLine % 256 == 0) return sizeof(T) == 2 ? (head & 3) << 1 | (head >> 2 & 1) : head & 7;
+    if constexpr (kLine % 128 == 0) return head & 2 | (head >> 2 & 1);
     return head >> 2 & 1;
   }
 };
 
 // What a wavefront of WAVES loads of a tile: straight into LDS, 64 pieces of 16 bytes at a time, zeros for what is not there.
-template <int D, int WAVES>
+template <typename T, int D, int WAVES>
 struct TileLoader {
-  static constexpr int kAll = kTile * Tile<D>::kPieces / kWave, kLoads = (kAll + WAVES - 1) / WAVES;
+  using Of = Tile<T, D>;
+  static constexpr int kAll = Of::kHeads * Of::kPieces / kWave, kLoads = (kAll + WAVES - 1) / WAVES, kEach = 16 / sizeof(T);
   uint32_t offset[kLoads];
   uint32_t line, width;  // bytes from a head to the next, of one
   const char* base;      // of the next tile
 
-  template <typename T>
   __device__ __forceinline__ void aim(Heads<const T> const& x, int32_t first, int32_t head, int32_t columns, int wave, int lane)
   {
     base  = reinterpret_cast<const char*>(x.at(first, head));
-    line  = static_cast<uint32_t>(x.stride * 2);
-    width = static_cast<uint32_t>((columns + 7) / 8 * 16);  // (whole pieces: those of an odd width have been copied, and end in zeros)
+    line  = static_cast<uint32_t>(x.stride * sizeof(T));
+    width = static_cast<uint32_t>((columns + kEach - 1) / kEach * 16);  // (whole pieces: those of an odd width have been copied, and end in zeros)
 #pragma unroll
     for (int p = 0; p < kLoads; ++p) {
-      int const slot = (p * WAVES + wave) * kWave + lane, row = slot / Tile<D>::kPieces, piece = slot % Tile<D>::kPieces;
-      int const from = (static_cast<int>(static_cast<uint32_t>(piece >> 1) ^ Tile<D>::turn(row)) << 1) | (piece & 1);
-      offset[p]      = from * 8 < columns ? row * line + from * 16 : kFar;
+      int const slot = (p * WAVES + wave) * kWave + lane, row = slot / Of::kPieces, piece = slot % Of::kPieces;
+      int const from = (static_cast<int>(static_cast<uint32_t>(piece >> 1) ^ Of::turn(row)) << 1) | (piece & 1);
+      offset[p]      = from * kEach < columns ? row * line + from * 16 : kFar;
     }
   }
   // The next tile, of which `here` heads are there.
   __device__ __forceinline__ void load(LdsBytes to, int32_t here, int wave)
   {
-    uint32_t const range = static_cast<uint32_t>(here < kTile ? here - 1 : kTile - 1) * line + width;
+    uint32_t const range = static_cast<uint32_t>(here < Of::kHeads ? here - 1 : Of::kHeads - 1) * line + width;
 #pragma unroll
     for (int p = 0; p < kLoads; ++p)
       if (kAll % WAVES == 0 || p * WAVES + wave < kAll) load_to_lds(base, range, to + (p * WAVES + wave) * 1024, offset[p]);
-    base += static_cast<int64_t>(kTile) * line;
+    base += static_cast<int64_t>(Of::kHeads) * line;
   }
 };
 
 // Where a lane finds fragments of a tile.
 template <typename T, int D>
 struct TileReader {
+  static constexpr int kLine = Tile<T, D>::kLine;
   uint32_t row, column, turn_row, turn_column;
   __device__ __forceinline__ explicit TileReader(int lane)
   {
     int const h = lane / 32, i = lane % 16;
-    row         = (lane % 32) * (2 * D) + h * 16;
-    turn_row    = Tile<D>::turn(lane % 32);
-    int const k = 4 * h + i / 4;
-    column      = k * (2 * D) + i % 4 * 8;
-    turn_column = Tile<D>::turn(k) ^ (lane / 16 & 1);
+    row         = (lane % 32) * kLine;
+    turn_row    = Tile<T, D>::turn(lane % 32);
+    if constexpr (sizeof(T) == 2) {
+      row += h * 16;
+      int const k = 4 * h + i / 4;
+      column      = k * kLine + i % 4 * 8;
+      turn_column = Tile<T, D>::turn(k) ^ (lane / 16 & 1);
+    } else {
+      column      = 4 * h * kLine + lane % 8 * 4;
+      turn_column = Tile<T, D>::turn(4 * h) ^ (lane / 8 & 3);
+      turn_row ^= h;
+    }
   }
   // 32 heads from 32 * block on, values 16 * step .. 16 * step + 15 of each
   __device__ __forceinline__ Fragment<T> rows(LdsBytes tile, int block, int step) const
   {
-    return *reinterpret_cast<__attribute__((address_space(3))) Fragment<T>*>(tile + row + ((step ^ turn_row) * 32) + block * (64 * D));
+    constexpr int kUnits = 16 * sizeof(T) / 32;
+    LdsBytes const p     = tile + row + (((step * kUnits) ^ turn_row) * 32) + block * (32 * kLine);
+    return *reinterpret_cast<__attribute__((address_space(3))) Fragment<T>*>(p);
   }
   // transposed: values 32 * block .. 32 * block + 31 of 16 heads from 16 * step on, in the order of heads that a result of 32 x 32 leaves in its registers
   __device__ __forceinline__ Fragment<T> columns(LdsBytes tile, int block, int step) const
   {
-    LdsBytes const p   = tile + column + (((2 * block) ^ turn_column) * 32) + step * (32 * D);
-    s16x4_t const low  = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(p));
-    s16x4_t const high = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(p + 16 * D));
-    return __builtin_bit_cast(Fragment<T>, __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7));
+    if constexpr (sizeof(T) == 2) {
+      LdsBytes const p   = tile + column + (((2 * block) ^ turn_column) * 32) + step * (16 * kLine);
+      s16x4_t const low  = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(p));
+      s16x4_t const high = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(p + 8 * kLine));
+      return __builtin_bit_cast(Fragment<T>, __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      Fragment<T> f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        uint32_t const unit = (4 * block) ^ turn_column ^ Tile<T, D>::turn(k % 4);
+        f[k]                = *reinterpret_cast<__attribute__((address_space(3))) T*>(tile + column + unit * 32 + (16 * step + 8 * (k / 4) + k % 4) * kLine);
+      }
+      return f;
+    }
   }
 };
 
@@ -311,12 +339,19 @@ __device__ __forceinline__ Fragment<T> rounded(f32x16_t const& x, int step)
   return f;
 }
 
-// 16 bytes of a head's values from j on, zeros behind the last or where it is not `there`; widths and strides are multiples of 8
+// Eight of a head's values from j on, zeros behind the last or where it is not `there`; widths and strides are of whole pieces of 16 bytes
 template <typename T>
 __device__ __forceinline__ Fragment<T> fragment_of(const T* head, int32_t j, int32_t width, bool there)
 {
   Fragment<T> f{};
-  if (there && j < width) f = *reinterpret_cast<const Fragment<T>*>(head + j);
+  if constexpr (sizeof(T) == 2) {
+    if (there && j < width) f = *reinterpret_cast<const Fragment<T>*>(head + j);
+  } else {
+    f32x4_t low{}, high{};
+    if (there && j < width) low = *reinterpret_cast<const f32x4_t*>(head + j);
+    if (there && j + 4 < width) high = *reinterpret_cast<const f32x4_t*>(head + j + 4);
+    f = __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
   return f;
 }
 

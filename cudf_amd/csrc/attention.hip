@@ -8,14 +8,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) attend_rows_kernel(Forward<T> f)
-{
-  int64_t const w = block_number() * (kThreads / kWave) + threadIdx.x / kWave;
-  if (w >= static_cast<int64_t>(f.runs.tokens) * f.heads) return;
-  attend_row(f, static_cast<int32_t>(w / f.heads), static_cast<int32_t>(w % f.heads));
-}
-
 // ------------------------------------------------------------------ forward, in tiles
 // The work of a launch: blocks of tokens, of every head.  The heads that share a key head come one after the other on one XCD (workgroups go to
 // the eight XCDs in turn), and so do, where the number of key heads allows, the blocks of a key head: its keys come from that XCD's L2.  The last
@@ -37,9 +29,9 @@ __device__ __forceinline__ bool work_of(int64_t item, int64_t blocks, int32_t kv
   return true;
 }
 
-template <int D, int WAVES, int NQ>
+template <typename T, int D, int WAVES, int NQ>
 struct ForwardShape {
-  static constexpr int kTokens = 32 * WAVES * NQ, kShift = __builtin_ctz(kTokens), kLds = 4 * Tile<D>::kBytes;
+  static constexpr int kTokens = 32 * WAVES * NQ, kShift = __builtin_ctz(kTokens), kTile = Tile<T, D>::kHeads, kLds = 4 * Tile<T, D>::kBytes, kWavesASimd = D * sizeof(T) <= 256 ? 2 : 1;
 };
 
 // A workgroup has kTokens tokens of a head, a wavefront 32 * NQ of them, in its registers: q, and the sums of out, transposed.  Keys come through LDS, 64 at a
@@ -47,12 +39,12 @@ struct ForwardShape {
 // one 32 further on), and exponentials are in its registers as the second product takes them: no lane needs another's but for the maximum.
 // Sums are kept in proportion to 2^top, where top is a maximum that may be 8 too small: only then are they multiplied anew.
 template <typename T, int D, int WAVES, int NQ>
-__global__ void __launch_bounds__(WAVES * kWave, 2) attend_tiles_kernel(Forward<T> f)
+__global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES, NQ>::kWavesASimd)) attend_tiles_kernel(Forward<T> f)
 {
-  using Shape = ForwardShape<D, WAVES, NQ>;
+  using Shape = ForwardShape<T, D, WAVES, NQ>;
   extern __shared__ __align__(16) char lds_[];
   LdsBytes const lds = (LdsBytes)lds_;
-  constexpr int kSteps = D / 16, kColumns = D / 32;
+  constexpr int kSteps = D / 16, kColumns = D / 32, kTile = Shape::kTile, kBlocks = kTile / 32;
   constexpr float kSlack = 8.f;
   Work w;
   int32_t const each = f.heads / f.kv_heads;
@@ -81,7 +73,7 @@ __global__ void __launch_bounds__(WAVES * kWave, 2) attend_tiles_kernel(Forward<
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) q[n][s] = fragment_of(f.q.at(static_cast<int64_t>(begin) + block0 + (i < rest ? i : 0), w.head), 16 * s + 8 * half, f.width, i < rest);
   }
-  TileLoader<D, WAVES> load_k, load_v;
+  TileLoader<T, D, WAVES> load_k, load_v;
   load_k.aim(f.k, first, w.kv_head, f.width, wave, lane);
   load_v.aim(f.v, first, w.kv_head, f.width, wave, lane);
   TileReader<T, D> const read(lane);
@@ -98,21 +90,21 @@ __global__ void __launch_bounds__(WAVES * kWave, 2) attend_tiles_kernel(Forward<
   int32_t const tiles = (all + kTile - 1) / kTile;
   if (tiles > 0) {
     load_k.load(lds, keys, wave);
-    load_v.load(lds + Tile<D>::kBytes, keys, wave);
+    load_v.load(lds + Tile<T, D>::kBytes, keys, wave);
   }
   for (int32_t tile = 0; tile < tiles; ++tile) {
-    LdsBytes const k_tile = lds + (tile & 1) * 2 * Tile<D>::kBytes, v_tile = k_tile + Tile<D>::kBytes;
+    LdsBytes const k_tile = lds + (tile & 1) * 2 * Tile<T, D>::kBytes, v_tile = k_tile + Tile<T, D>::kBytes;
     stage_barrier<0>();
     if (tile + 1 < tiles) {
-      LdsBytes const next = lds + (~tile & 1) * 2 * Tile<D>::kBytes;
+      LdsBytes const next = lds + (~tile & 1) * 2 * Tile<T, D>::kBytes;
       load_k.load(next, keys - (tile + 1) * kTile, wave);
-      load_v.load(next + Tile<D>::kBytes, keys - (tile + 1) * kTile, wave);
+      load_v.load(next + Tile<T, D>::kBytes, keys - (tile + 1) * kTile, wave);
     }
     int32_t const key0 = tile * kTile;
     if (key0 >= most) continue;
-    f32x16_t s[NQ][2];
+    f32x16_t s[NQ][kBlocks];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kBlocks; ++b) {
 #pragma unroll
       for (int n = 0; n < NQ; ++n) s[n][b] = f32x16_t{};
 #pragma unroll
@@ -126,7 +118,7 @@ __global__ void __launch_bounds__(WAVES * kWave, 2) attend_tiles_kernel(Forward<
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[n][b][r] = key0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4 < seen[n] ? s[n][b][r] : -INFINITY;
     }
@@ -134,7 +126,7 @@ __global__ void __launch_bounds__(WAVES * kWave, 2) attend_tiles_kernel(Forward<
     for (int n = 0; n < NQ; ++n) {
       float high = s[n][0][0];
 #pragma unroll
-      for (int r = 1; r < 32; ++r) high = fmaxf(high, s[n][r / 16][r % 16]);
+      for (int r = 1; r < 16 * kBlocks; ++r) high = fmaxf(high, s[n][r / 16][r % 16]);
       Halves const both = halves(high);
       high              = fmaxf(both.low, both.high) * scale;
       // (a token that sees nothing yet keeps top at -infinity; NaN in a score is found in out at the end)
@@ -150,21 +142,21 @@ __global__ void __launch_bounds__(WAVES * kWave, 2) attend_tiles_kernel(Forward<
       }
       float const base = top[n] == -INFINITY ? 0.f : top[n];
 #pragma unroll
-      for (int r = 0; r < 32; ++r) {
+      for (int r = 0; r < 16 * kBlocks; ++r) {
         float const p       = __builtin_amdgcn_exp2f(fmaf(s[n][r / 16][r % 16], scale, -base));
         s[n][r / 16][r % 16] = p;
         sum[n] += p;
       }
     }
-    Fragment<T> p[NQ][4];
+    Fragment<T> p[NQ][2 * kBlocks];
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
-      for (int step = 0; step < 4; ++step) p[n][step] = rounded<T>(s[n][step / 2], step % 2);
+      for (int step = 0; step < 2 * kBlocks; ++step) p[n][step] = rounded<T>(s[n][step / 2], step % 2);
 #pragma unroll
     for (int c = 0; c < kColumns; ++c)
 #pragma unroll
-      for (int step = 0; step < 4; ++step) {
+      for (int step = 0; step < 2 * kBlocks; ++step) {
         Fragment<T> const v = read.columns(v_tile, c, step);
 #pragma unroll
         for (int n = 0; n < NQ; ++n) o[n][c] = multiply32(v, p[n][step], o[n][c]);
@@ -219,20 +211,20 @@ __global__ void __launch_bounds__(kThreads) key_gradient_rows_kernel(Backward<T>
 // ------------------------------------------------------------------ the gradients, in tiles
 // Two launches, the first for q, the second for k and v: each makes the scores anew and adds up what is its own in registers, in one order at every
 // call.  (One launch for all three would have to add up q's gradient in memory, over all workgroups of keys: in parts of float32 or in any order.)
-template <int D, int WAVES>
+template <typename T, int D, int WAVES>
 struct GradientShape {
-  static constexpr int kRows = 32 * WAVES, kShift = __builtin_ctz(kRows), kStage = 2 * Tile<D>::kBytes, kLds = 2 * kStage, kWavesASimd = D <= 128 ? 2 : 1;
-  static constexpr int kKeyStage = kStage + 2 * kTile * 4, kKeyLds = 2 * kKeyStage;  // (with logs and deltas)
+  static constexpr int kRows = 32 * WAVES, kShift = __builtin_ctz(kRows), kTile = Tile<T, D>::kHeads, kStage = 2 * Tile<T, D>::kBytes, kLds = 2 * kStage, kWavesASimd = D * sizeof(T) <= 256 ? 2 : 1;
+  static constexpr int kKeyStage = kStage + 2 * kWave * 4, kKeyLds = 2 * kKeyStage;  // (with logs and deltas)
 };
 
 // The gradient of q: as forward, a lane has a token's scores, and what they are multiplied with comes from LDS, keys as they lie and transposed.
 template <typename T, int D, int WAVES>
-__global__ void __launch_bounds__(WAVES * kWave, (GradientShape<D, WAVES>::kWavesASimd)) query_gradient_tiles_kernel(Backward<T> f)
+__global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kWavesASimd)) query_gradient_tiles_kernel(Backward<T> f)
 {
-  using Shape = GradientShape<D, WAVES>;
+  using Shape = GradientShape<T, D, WAVES>;
   extern __shared__ __align__(16) char lds_[];
   LdsBytes const lds = (LdsBytes)lds_;
-  constexpr int kSteps = D / 16, kColumns = D / 32;
+  constexpr int kSteps = D / 16, kColumns = D / 32, kTile = Shape::kTile, kBlocks = kTile / 32;
   Work w;
   int32_t const each = f.heads / f.kv_heads;
   if (!work_of(block_number(), f.runs.template blocks<Shape::kShift>(), f.kv_heads, each, w)) return;
@@ -270,7 +262,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<D, WAVES>::kWave
     f.deltas[at] = delta;
     f.logs[at]   = log;
   }
-  TileLoader<D, WAVES> load_k, load_v;
+  TileLoader<T, D, WAVES> load_k, load_v;
   load_k.aim(f.k, first, w.kv_head, f.width, wave, lane);
   load_v.aim(f.v, first, w.kv_head, f.width, wave, lane);
   TileReader<T, D> const read(lane);
@@ -281,20 +273,20 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<D, WAVES>::kWave
   int32_t const tiles = (all + kTile - 1) / kTile;
   if (tiles > 0) {
     load_k.load(lds, keys, wave);
-    load_v.load(lds + Tile<D>::kBytes, keys, wave);
+    load_v.load(lds + Tile<T, D>::kBytes, keys, wave);
   }
   for (int32_t tile = 0; tile < tiles; ++tile) {
-    LdsBytes const k_tile = lds + (tile & 1) * Shape::kStage, v_tile = k_tile + Tile<D>::kBytes;
+    LdsBytes const k_tile = lds + (tile & 1) * Shape::kStage, v_tile = k_tile + Tile<T, D>::kBytes;
     stage_barrier<0>();
     if (tile + 1 < tiles) {
       LdsBytes const next = lds + (~tile & 1) * Shape::kStage;
       load_k.load(next, keys - (tile + 1) * kTile, wave);
-      load_v.load(next + Tile<D>::kBytes, keys - (tile + 1) * kTile, wave);
+      load_v.load(next + Tile<T, D>::kBytes, keys - (tile + 1) * kTile, wave);
     }
     int32_t const key0 = tile * kTile;
     if (key0 >= most) continue;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kBlocks; ++b) {
       f32x16_t s{}, p{};
 #pragma unroll
       for (int step = 0; step < kSteps; ++step) s = multiply32(read.rows(k_tile, b, step), q[step], s);
@@ -336,13 +328,16 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<D, WAVES>::kWave
 
 // The gradients of k and v: a wavefront has 32 keys in its registers, a lane a key's scores, and the tokens of all heads that see them come through LDS
 // with their gradients, 64 at a time, with their logs and deltas.
-template <typename T, int D, int WAVES>
-__global__ void __launch_bounds__(WAVES * kWave, (GradientShape<D, WAVES>::kWavesASimd)) key_gradient_tiles_kernel(Backward<T> f)
+// PART: the gradients of both, or of k or v alone (of wide heads there are not the registers for both).
+enum Part { kBoth, kOfK, kOfV };
+template <typename T, int D, int WAVES, Part PART>
+__global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kWavesASimd)) key_gradient_tiles_kernel(Backward<T> f)
 {
-  using Shape = GradientShape<D, WAVES>;
+  using Shape = GradientShape<T, D, WAVES>;
   extern __shared__ __align__(16) char lds_[];
   LdsBytes const lds = (LdsBytes)lds_;
-  constexpr int kSteps = D / 16, kColumns = D / 32;
+  constexpr bool kK = PART != kOfV, kV = PART != kOfK;
+  constexpr int kSteps = D / 16, kColumns = D / 32, kTile = Shape::kTile, kBlocks = kTile / 32;
   Work w;
   if (!work_of(block_number(), f.key_runs.template blocks<Shape::kShift>(), f.kv_heads, 1, w)) return;
   w.block              = f.key_runs.template blocks<Shape::kShift>() - 1 - w.block;  // (of a long row, the first keys are those that most tokens see)
@@ -373,20 +368,23 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<D, WAVES>::kWave
   int32_t const from = from_of(key), start = uniform(block0 < keys ? from_of(block0) / kTile : 0), tiles = uniform(block0 < keys ? (tokens + kTile - 1) / kTile : 0);
   int32_t const last_from = uniform(from_of(block0 + wave0 + 31)), first_from = uniform(from_of(block0 + wave0));
 
-  Fragment<T> k[kSteps], v[kSteps];
+  Fragment<T> k[kSteps], v[kK ? kSteps : 1];
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
     k[s] = fragment_of(f.k.at(t, w.kv_head), 16 * s + 8 * half, f.width, there && key < keys);
-    v[s] = fragment_of(f.v.at(t, w.kv_head), 16 * s + 8 * half, f.width, there && key < keys);
+    if constexpr (kK) v[s] = fragment_of(f.v.at(t, w.kv_head), 16 * s + 8 * half, f.width, there && key < keys);
   }
   TileReader<T, D> const read(lane);
   float const scale = f.scale * kLog2e;
-  f32x16_t dk[kColumns], dv[kColumns];
+  f32x16_t dk[kK ? kColumns : 1], dv[kV ? kColumns : 1];
 #pragma unroll
-  for (int c = 0; c < kColumns; ++c) dk[c] = dv[c] = f32x16_t{};
+  for (int c = 0; c < kColumns; ++c) {
+    if constexpr (kK) dk[c] = f32x16_t{};
+    if constexpr (kV) dv[c] = f32x16_t{};
+  }
   // The tiles of one head after another are one stream of loads.
   int32_t const of_head = tiles - start > 0 ? tiles - start : 0, total = of_head * each;
-  TileLoader<D, WAVES> load_q, load_g;
+  TileLoader<T, D, WAVES> load_q, load_g;
   int32_t loaded = 0, next_head = w.kv_head * each;  // the tile of the head that is loaded next
   auto const load = [&](LdsBytes to) {
     if (loaded == 0) {
@@ -395,11 +393,11 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<D, WAVES>::kWave
     }
     int32_t const token = (start + loaded) * kTile, here = tokens - token;
     load_q.load(to, here, wave);
-    load_g.load(to + Tile<D>::kBytes, here, wave);
+    load_g.load(to + Tile<T, D>::kBytes, here, wave);
     int64_t const at = static_cast<int64_t>(next_head) * f.runs.tokens + begin + token;
     uint32_t const range = static_cast<uint32_t>(here < kTile ? here : kTile) * 4;
     if (wave == 0) load_words_to_lds(reinterpret_cast<const char*>(f.logs + at), range, to + Shape::kStage, lane * 4);
-    if (wave == WAVES - 1) load_words_to_lds(reinterpret_cast<const char*>(f.deltas + at), range, to + Shape::kStage + kTile * 4, lane * 4);
+    if (wave == WAVES - 1) load_words_to_lds(reinterpret_cast<const char*>(f.deltas + at), range, to + Shape::kStage + kWave * 4, lane * 4);
     if (++loaded == of_head) {
       loaded = 0;
       ++next_head;
@@ -408,25 +406,27 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<D, WAVES>::kWave
   if (total > 0) load(lds);
   int32_t tile = start - 1;
   for (int32_t n = 0; n < total; ++n) {
-    LdsBytes const q_tile = lds + (n & 1) * Shape::kKeyStage, g_tile = q_tile + Tile<D>::kBytes, words = q_tile + Shape::kStage + 16 * half;
+    LdsBytes const q_tile = lds + (n & 1) * Shape::kKeyStage, g_tile = q_tile + Tile<T, D>::kBytes, words = q_tile + Shape::kStage + 16 * half;
     stage_barrier<0>();
     if (n + 1 < total) load(lds + (~n & 1) * Shape::kKeyStage);
     if (++tile == tiles) tile = start;
     int32_t const token0 = tile * kTile;
     if (token0 + kTile <= first_from) continue;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kBlocks; ++b) {
       f32x16_t s{}, p{};
 #pragma unroll
       for (int step = 0; step < kSteps; ++step) s = multiply32(read.rows(q_tile, b, step), k[step], s);
+      if constexpr (kK) {
 #pragma unroll
-      for (int step = 0; step < kSteps; ++step) p = multiply32(read.rows(g_tile, b, step), v[step], p);
+        for (int step = 0; step < kSteps; ++step) p = multiply32(read.rows(g_tile, b, step), v[step], p);
+      }
       int32_t const row0 = token0 + 32 * b;
       bool const partly  = row0 < last_from || row0 + 32 > tokens;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         f32x4_t const log   = *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(words + 128 * b + 32 * i);
-        f32x4_t const delta = *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(words + kTile * 4 + 128 * b + 32 * i);
+        f32x4_t const delta = *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(words + kWave * 4 + 128 * b + 32 * i);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           int const r = 4 * i + e;
@@ -446,10 +446,14 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<D, WAVES>::kWave
 #pragma unroll
       for (int step = 0; step < 2; ++step) {
         Fragment<T> const weight = rounded<T>(s, step), ds = rounded<T>(p, step);
+        if constexpr (kV) {
 #pragma unroll
-        for (int c = 0; c < kColumns; ++c) dv[c] = multiply32(read.columns(g_tile, c, 2 * b + step), weight, dv[c]);
+          for (int c = 0; c < kColumns; ++c) dv[c] = multiply32(read.columns(g_tile, c, 2 * b + step), weight, dv[c]);
+        }
+        if constexpr (kK) {
 #pragma unroll
-        for (int c = 0; c < kColumns; ++c) dk[c] = multiply32(read.columns(q_tile, c, 2 * b + step), ds, dk[c]);
+          for (int c = 0; c < kColumns; ++c) dk[c] = multiply32(read.columns(q_tile, c, 2 * b + step), ds, dk[c]);
+        }
       }
     }
   }
@@ -459,23 +463,29 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<D, WAVES>::kWave
   for (int c = 0; c < kColumns; ++c)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      dk[c][r] *= f.scale;
-      finite = finite && fabsf(dk[c][r]) < INFINITY && fabsf(dv[c][r]) < INFINITY;
+      if constexpr (kK) {
+        dk[c][r] *= f.scale;
+        finite = finite && fabsf(dk[c][r]) < INFINITY;
+      }
+      if constexpr (kV) finite = finite && fabsf(dv[c][r]) < INFINITY;
     }
   uint64_t odd = __ballot(there && key < keys && !finite);
   odd          = (odd | odd >> 32) & 0xffffffffu;
   if (there && !(odd >> column & 1)) {
     if (key >= keys) {
 #pragma unroll
-      for (int c = 0; c < kColumns; ++c) dk[c] = dv[c] = f32x16_t{};
+      for (int c = 0; c < kColumns; ++c) {
+        if constexpr (kK) dk[c] = f32x16_t{};
+        if constexpr (kV) dv[c] = f32x16_t{};
+      }
     }
-    store_columns<T, kColumns>(f.k_grad.at(t, w.kv_head), dk, half, f.width);
-    store_columns<T, kColumns>(f.v_grad.at(t, w.kv_head), dv, half, f.width);
+    if constexpr (kK) store_columns<T, kColumns>(f.k_grad.at(t, w.kv_head), dk, half, f.width);
+    if constexpr (kV) store_columns<T, kColumns>(f.v_grad.at(t, w.kv_head), dv, half, f.width);
   }
   while (odd) {
     int const which = __builtin_ctzll(odd);
     odd &= odd - 1;
-    key_gradient_row(f, first + block0 + wave0 + which, w.kv_head);
+    key_gradient_row(f, first + block0 + wave0 + which, w.kv_head, kK, kV);
   }
 }
 
@@ -565,14 +575,19 @@ struct Alignment {
   }
 };
 
+// (where kernels take more than 64 KB of LDS, the runtime wants to be told)
+template <typename Kernel>
+hipError_t allow_lds(Kernel kernel, int bytes)
+{
+  return bytes > 65536 ? hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) : hipSuccess;
+}
+
 template <typename T, int D, int WAVES, int NQ>
 nvtext_amd_status attend_tiles(Forward<T> const& f, hipStream_t stream)
 {
-  using Shape = ForwardShape<D, WAVES, NQ>;
+  using Shape = ForwardShape<T, D, WAVES, NQ>;
   ProfileScope const scope("attention_tiles", stream);
-  if constexpr (Shape::kLds > 65536) {
-    NVTEXT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(attend_tiles_kernel<T, D, WAVES, NQ>), hipFuncAttributeMaxDynamicSharedMemorySize, Shape::kLds));
-  }
+  NVTEXT_HIP_TRY(allow_lds(attend_tiles_kernel<T, D, WAVES, NQ>, Shape::kLds));
   int64_t const items = work_items(f.runs.template blocks<Shape::kShift>(), f.kv_heads, f.heads / f.kv_heads);
   hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_tiles_kernel<T, D, WAVES, NQ>), grid_of(items, WAVES * kWave), dim3(WAVES * kWave), Shape::kLds, stream, f);
   return NVTEXT_AMD_SUCCESS;
@@ -581,77 +596,63 @@ nvtext_amd_status attend_tiles(Forward<T> const& f, hipStream_t stream)
 template <typename T>
 nvtext_amd_status attention(Forward<T> f, Mr const& mr, hipStream_t stream)
 {
-  if constexpr (sizeof(T) == 2) {
-    if (f.width > 0) {
-      Alignment<T> align(f.width);
-      align.add(f.q, f.runs.tokens, f.heads);
-      align.add(f.k, f.key_runs.tokens, f.kv_heads);
-      align.add(f.v, f.key_runs.tokens, f.kv_heads);
-      Temp const copies(mr, align.bytes());
-      if (!copies.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
-      align.launch(copies.template as<char>(), stream);
-      if (f.width <= 64) return attend_tiles<T, 64, 4, 1>(f, stream);
-      if (f.width <= 128) return attend_tiles<T, 128, 4, 1>(f, stream);
-      return attend_tiles<T, 256, 4, 1>(f, stream);
-    }
-  }
-  ProfileScope const scope("attention_rows", stream);
-  hipLaunchKernelGGL(attend_rows_kernel<T>, grid_of((static_cast<int64_t>(f.runs.tokens) * f.heads + 3) / 4, kThreads), dim3(kThreads), 0, stream, f);
+  Alignment<T> align(f.width);
+  align.add(f.q, f.runs.tokens, f.heads);
+  align.add(f.k, f.key_runs.tokens, f.kv_heads);
+  align.add(f.v, f.key_runs.tokens, f.kv_heads);
+  Temp const copies(mr, align.bytes());
+  if (!copies.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
+  align.launch(copies.template as<char>(), stream);
+  if (f.width <= 64) return attend_tiles<T, 64, 4, 1>(f, stream);
+  if (f.width <= 128) return attend_tiles<T, 128, 4, 1>(f, stream);
+  return attend_tiles<T, 256, 4, 1>(f, stream);
+}
+
+template <typename T, int D, int WAVES, Part PART>
+nvtext_amd_status key_gradient_tiles(Backward<T> const& f, hipStream_t stream)
+{
+  using Shape = GradientShape<T, D, WAVES>;
+  ProfileScope const scope("attention_key_gradient", stream);
+  NVTEXT_HIP_TRY(allow_lds(key_gradient_tiles_kernel<T, D, WAVES, PART>, Shape::kKeyLds));
+  int64_t const items = work_items(f.key_runs.template blocks<Shape::kShift>(), f.kv_heads, 1);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(key_gradient_tiles_kernel<T, D, WAVES, PART>), grid_of(items, WAVES * kWave), dim3(WAVES * kWave), Shape::kKeyLds, stream, f);
   return NVTEXT_AMD_SUCCESS;
 }
 
 template <typename T, int D, int WAVES>
 nvtext_amd_status gradient_tiles(Backward<T> const& f, hipStream_t stream)
 {
-  using Shape = GradientShape<D, WAVES>;
-  if constexpr (Shape::kKeyLds > 65536) {
-    NVTEXT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(query_gradient_tiles_kernel<T, D, WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, Shape::kLds));
-    NVTEXT_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(key_gradient_tiles_kernel<T, D, WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, Shape::kKeyLds));
-  }
+  using Shape = GradientShape<T, D, WAVES>;
   if (f.runs.tokens > 0) {
     ProfileScope const scope("attention_query_gradient", stream);
+    NVTEXT_HIP_TRY(allow_lds(query_gradient_tiles_kernel<T, D, WAVES>, Shape::kLds));
     int64_t const items = work_items(f.runs.template blocks<Shape::kShift>(), f.kv_heads, f.heads / f.kv_heads);
     hipLaunchKernelGGL(HIP_KERNEL_NAME(query_gradient_tiles_kernel<T, D, WAVES>), grid_of(items, WAVES * kWave), dim3(WAVES * kWave), Shape::kLds, stream, f);
   }
-  if (f.key_runs.tokens > 0) {
-    ProfileScope const scope("attention_key_gradient", stream);
-    int64_t const items = work_items(f.key_runs.template blocks<Shape::kShift>(), f.kv_heads, 1);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(key_gradient_tiles_kernel<T, D, WAVES>), grid_of(items, WAVES * kWave), dim3(WAVES * kWave), Shape::kKeyLds, stream, f);
+  if (f.key_runs.tokens == 0) return NVTEXT_AMD_SUCCESS;
+  if constexpr (D > 128) {
+    nvtext_amd_status const st = key_gradient_tiles<T, D, WAVES, kOfK>(f, stream);
+    return st != NVTEXT_AMD_SUCCESS ? st : key_gradient_tiles<T, D, WAVES, kOfV>(f, stream);
+  } else {
+    return key_gradient_tiles<T, D, WAVES, kBoth>(f, stream);
   }
-  return NVTEXT_AMD_SUCCESS;
 }
 
 template <typename T>
 nvtext_amd_status attention_backward(Backward<T> f, Mr const& mr, hipStream_t stream)
 {
-  bool const tiles = sizeof(T) == 2 && f.width > 0;
   Alignment<T> align(f.width);
-  if (tiles) {
-    for (auto* x : {&f.q, &f.grad, &f.out}) align.add(*x, f.runs.tokens, f.heads);
-    for (auto* x : {&f.k, &f.v}) align.add(*x, f.key_runs.tokens, f.kv_heads);
-  }
+  for (auto* x : {&f.q, &f.grad, &f.out}) align.add(*x, f.runs.tokens, f.heads);
+  for (auto* x : {&f.k, &f.v}) align.add(*x, f.key_runs.tokens, f.kv_heads);
   size_t const values = static_cast<size_t>(f.heads) * static_cast<size_t>(f.runs.tokens) * sizeof(float);
-  TempParts<3> const temp(mr, {values, tiles ? values : 0, align.bytes()});
+  TempParts<3> const temp(mr, {values, values, align.bytes()});
   if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
   f.deltas = temp.template part<float>(0);
   f.logs   = temp.template part<float>(1);
   align.launch(temp.template part<char>(2), stream);
-  if constexpr (sizeof(T) == 2) {
-    if (tiles) {
-      if (f.width <= 64) return gradient_tiles<T, 64, 4>(f, stream);
-      if (f.width <= 128) return gradient_tiles<T, 128, 4>(f, stream);
-      return gradient_tiles<T, 256, 4>(f, stream);
-    }
-  }
-  if (f.runs.tokens > 0) {
-    ProfileScope const scope("attention_query_gradient", stream);
-    hipLaunchKernelGGL(query_gradient_rows_kernel<T>, grid_of((static_cast<int64_t>(f.runs.tokens) * f.heads + 3) / 4, kThreads), dim3(kThreads), 0, stream, f);
-  }
-  if (f.key_runs.tokens > 0) {
-    ProfileScope const scope("attention_key_gradient", stream);
-    hipLaunchKernelGGL(key_gradient_rows_kernel<T>, grid_of((static_cast<int64_t>(f.key_runs.tokens) * f.kv_heads + 3) / 4, kThreads), dim3(kThreads), 0, stream, f);
-  }
-  return NVTEXT_AMD_SUCCESS;
+  if (f.width <= 64) return gradient_tiles<T, 64, 4>(f, stream);
+  if (f.width <= 128) return gradient_tiles<T, 128, 4>(f, stream);
+  return gradient_tiles<T, 256, 4>(f, stream);
 }
 
 // What both directions ask of their arguments; nullptr if it holds.
