@@ -2,6 +2,7 @@
 #include "attention.cuh"
 
 #include <cmath>
+#include <type_traits>
 
 namespace nvtext_amd {
 namespace {
@@ -34,74 +35,32 @@ struct ForwardShape {
   static constexpr int kTokens = 32 * WAVES * NQ, kShift = __builtin_ctz(kTokens), kTile = Tile<T, D>::kHeads, kLds = 4 * Tile<T, D>::kBytes, kWavesASimd = D * sizeof(T) <= 256 ? 2 : 1;
 };
 
-// A workgroup has kTokens tokens of a head, a wavefront 32 * NQ of them, in its registers: q, and the sums of out, transposed.  Keys come through LDS, 64 at a
-// time, the next ones while these are multiplied.  Scores are products with the keys as rows, so a lane has all of a token's scores (with the
-// one 32 further on), and exponentials are in its registers as the second product takes them: no lane needs another's but for the maximum.
-// Sums are kept in proportion to 2^top, where top is a maximum that may be 8 too small: only then are they multiplied anew.
-template <typename T, int D, int WAVES, int NQ>
-__global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES, NQ>::kWavesASimd)) attend_tiles_kernel(Forward<T> f)
-{
-  using Shape = ForwardShape<T, D, WAVES, NQ>;
-  extern __shared__ __align__(16) char lds_[];
-  LdsBytes const lds = (LdsBytes)lds_;
-  constexpr int kSteps = D / 16, kColumns = D / 32, kTile = Shape::kTile, kBlocks = kTile / 32;
-  constexpr float kSlack = 8.f;
-  Work w;
-  int32_t const each = f.heads / f.kv_heads;
-  if (!work_of(block_number(), f.runs.template blocks<Shape::kShift>(), f.kv_heads, each, w)) return;
-  int32_t const run   = f.runs.template run_of<Shape::kShift>(w.block);
-  int32_t const begin = uniform(f.runs.begin(run)), tokens = uniform(f.runs.begin(run + 1)) - begin;
-  int64_t const in_run = (w.block - f.runs.template first_block<Shape::kShift>(run)) << Shape::kShift;
-  if (in_run >= tokens) return;
-  int const wave = uniform(threadIdx.x / kWave), lane = lane_id(), column = lane % 32, half = lane / 32;
-  int32_t const block0 = static_cast<int32_t>(in_run), rest = uniform(tokens - block0);  // the first token in the run, tokens from there on
-  int32_t first = 0, keys = 0;
-  if (f.is_row(run)) f.keys_of(run, first, keys);
-  first = uniform(first);
-  keys  = uniform(keys);
-  // keys that the workgroup's last token sees, and the wavefront's first and last
-  int32_t const wave0 = wave * 32 * NQ, wave1 = wave0 + 32 * NQ < rest ? wave0 + 32 * NQ : rest;
-  int32_t const all  = uniform(f.seen(block0 + (rest < Shape::kTokens ? rest : Shape::kTokens) - 1, tokens, keys));
-  int32_t const least = uniform(wave0 < rest ? f.seen(block0 + wave0, tokens, keys) : 0), most = uniform(wave0 < rest ? f.seen(block0 + wave1 - 1, tokens, keys) : 0);
-
+// What a wavefront holds of 32 * NQ heads of tokens, columns of the products, while keys pass: q, and the sums of out, transposed.  Scores are products with the
+// keys as rows, so a lane has all of a column's scores (with the one 32 further on), and exponentials are in its registers as the second product
+// takes them: no lane needs another's but for the maximum.  Sums are kept in proportion to 2^top, where top is a maximum that may be 8 too small:
+// only then are they multiplied anew.
+template <typename T, int D, int NQ>
+struct Attending {
+  static constexpr int kSteps = D / 16, kColumns = D / 32, kTile = Tile<T, D>::kHeads, kBlocks = kTile / 32;
+  static constexpr float kSlack = 8.f;
   Fragment<T> q[NQ][kSteps];
-  int32_t seen[NQ];
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    int32_t const i = wave0 + n * 32 + column;
-    seen[n]         = i < rest ? f.seen(block0 + i, tokens, keys) : 0;
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) q[n][s] = fragment_of(f.q.at(static_cast<int64_t>(begin) + block0 + (i < rest ? i : 0), w.head), 16 * s + 8 * half, f.width, i < rest);
-  }
-  TileLoader<T, D, WAVES> load_k, load_v;
-  load_k.aim(f.k, first, w.kv_head, f.width, wave, lane);
-  load_v.aim(f.v, first, w.kv_head, f.width, wave, lane);
-  TileReader<T, D> const read(lane);
-  float const scale = f.scale * kLog2e;
   f32x16_t o[NQ][kColumns];
   float top[NQ], sum[NQ];
+  int32_t seen[NQ];  // keys that the column sees
+
+  __device__ __forceinline__ void begin(int n, const T* head, int32_t width, bool there, int half)
+  {
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
+    for (int s = 0; s < kSteps; ++s) q[n][s] = fragment_of(head, 16 * s + 8 * half, width, there);
     top[n] = -INFINITY;
     sum[n] = 0.f;
 #pragma unroll
     for (int c = 0; c < kColumns; ++c) o[n][c] = f32x16_t{};
   }
-  int32_t const tiles = (all + kTile - 1) / kTile;
-  if (tiles > 0) {
-    load_k.load(lds, keys, wave);
-    load_v.load(lds + Tile<T, D>::kBytes, keys, wave);
-  }
-  for (int32_t tile = 0; tile < tiles; ++tile) {
-    LdsBytes const k_tile = lds + (tile & 1) * 2 * Tile<T, D>::kBytes, v_tile = k_tile + Tile<T, D>::kBytes;
-    stage_barrier<0>();
-    if (tile + 1 < tiles) {
-      LdsBytes const next = lds + (~tile & 1) * 2 * Tile<T, D>::kBytes;
-      load_k.load(next, keys - (tile + 1) * kTile, wave);
-      load_v.load(next + Tile<T, D>::kBytes, keys - (tile + 1) * kTile, wave);
-    }
-    int32_t const key0 = tile * kTile;
-    if (key0 >= most) continue;
+
+  // A tile of keys from key0 on; partly: not all columns see all of it.
+  __device__ __forceinline__ void pass(LdsBytes k_tile, LdsBytes v_tile, TileReader<T, D> const& read, int32_t key0, bool partly, float scale, int half)
+  {
     f32x16_t s[NQ][kBlocks];
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
@@ -114,7 +73,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES, NQ>:
         for (int n = 0; n < NQ; ++n) s[n][b] = multiply32(k, q[n][step], s[n][b]);
       }
     }
-    if (key0 + kTile > least) {
+    if (partly) {
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -129,7 +88,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES, NQ>:
       for (int r = 1; r < 16 * kBlocks; ++r) high = fmaxf(high, s[n][r / 16][r % 16]);
       Halves const both = halves(high);
       high              = fmaxf(both.low, both.high) * scale;
-      // (a token that sees nothing yet keeps top at -infinity; NaN in a score is found in out at the end)
+      // (a column that sees nothing yet keeps top at -infinity; NaN in a score is found in out at the end)
       if (__ballot(high > top[n] + kSlack || top[n] == -INFINITY)) {
         float const now  = fmaxf(top[n], high);
         float const fade = now == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top[n] - now);
@@ -143,7 +102,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES, NQ>:
       float const base = top[n] == -INFINITY ? 0.f : top[n];
 #pragma unroll
       for (int r = 0; r < 16 * kBlocks; ++r) {
-        float const p       = __builtin_amdgcn_exp2f(fmaf(s[n][r / 16][r % 16], scale, -base));
+        float const p        = __builtin_amdgcn_exp2f(fmaf(s[n][r / 16][r % 16], scale, -base));
         s[n][r / 16][r % 16] = p;
         sum[n] += p;
       }
@@ -162,11 +121,11 @@ __global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES, NQ>:
         for (int n = 0; n < NQ; ++n) o[n][c] = multiply32(v, p[n][step], o[n][c]);
       }
   }
-  if (wave0 >= rest) return;
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    int32_t const i   = wave0 + n * 32 + column;
-    int64_t const t   = static_cast<int64_t>(begin) + block0 + i;
+
+  // Writes out and logsum of a column, head h of token t, where it is `there`; of those whose result is not finite, the lanes' numbers.  That may come from keys that the
+  // token does not see, whose exponentials of 0 were multiplied: such columns are done once more, by themselves.
+  __device__ __forceinline__ uint32_t finish(int n, Forward<T> const& f, int64_t t, int32_t h, bool there, int half, int column)
+  {
     Halves const both = halves(sum[n]);
     float const total = both.low + both.high, part = seen[n] > 0 ? 1.f / total : 0.f;
     bool finite       = true;
@@ -177,35 +136,233 @@ __global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES, NQ>:
         o[n][c][r] *= part;
         finite = finite && fabsf(o[n][c][r]) < INFINITY;
       }
-    // What is not finite may come from keys that the token does not see, whose exponentials of 0 were multiplied: such tokens are done once more, by themselves.
-    uint64_t odd = __ballot(i < rest && seen[n] > 0 && !finite);
+    uint64_t odd = __ballot(there && seen[n] > 0 && !finite);
     odd          = (odd | odd >> 32) & 0xffffffffu;
-    if (i < rest && !(odd >> column & 1)) {
-      store_columns<T, kColumns>(f.out.at(t, w.head), o[n], half, f.width);
-      if (f.logsum && half == 0) f.logsum[static_cast<int64_t>(w.head) * f.runs.tokens + t] = seen[n] > 0 ? (top[n] + __builtin_amdgcn_logf(total)) * kLn2 : -INFINITY;
+    if (there && !(odd >> column & 1)) {
+      store_columns<T, kColumns>(f.out.at(t, h), o[n], half, f.width);
+      if (f.logsum && half == 0) f.logsum[static_cast<int64_t>(h) * f.runs.tokens + t] = seen[n] > 0 ? (top[n] + __builtin_amdgcn_logf(total)) * kLn2 : -INFINITY;
     }
-    while (odd) {
-      int const which = __builtin_ctzll(odd);
-      odd &= odd - 1;
-      attend_row(f, static_cast<int32_t>(begin + block0 + wave0 + n * 32 + which), w.head);
+    return static_cast<uint32_t>(odd);
+  }
+};
+
+// A workgroup has kTokens tokens of a head, a wavefront 32 * NQ of them.  Keys come through LDS, 64 at a time, the next ones while these are multiplied.
+template <typename T, int D, int WAVES, int NQ>
+__global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES, NQ>::kWavesASimd)) attend_tiles_kernel(Forward<T> f)
+{
+  using Shape = ForwardShape<T, D, WAVES, NQ>;
+  extern __shared__ __align__(16) char lds_[];
+  LdsBytes const lds = (LdsBytes)lds_;
+  constexpr int kTile = Shape::kTile;
+  Work w;
+  int32_t const each = f.heads / f.kv_heads;
+  if (!work_of(block_number(), f.runs.blocks(Shape::kShift), f.kv_heads, each, w)) return;
+  int32_t const run   = f.runs.run_of(w.block, Shape::kShift);
+  int32_t const begin = uniform(f.runs.begin(run)), tokens = uniform(f.runs.begin(run + 1)) - begin;
+  int64_t const in_run = (w.block - f.runs.first_block(run, Shape::kShift)) << Shape::kShift;
+  if (in_run >= tokens) return;
+  int const wave = uniform(threadIdx.x / kWave), lane = lane_id(), column = lane % 32, half = lane / 32;
+  int32_t const block0 = static_cast<int32_t>(in_run), rest = uniform(tokens - block0);  // the first token in the run, tokens from there on
+  int32_t first = 0, keys = 0;
+  if (f.is_row(run)) f.keys_of(run, first, keys);
+  first = uniform(first);
+  keys  = uniform(keys);
+  // keys that the workgroup's last token sees, and the wavefront's first and last
+  int32_t const wave0 = wave * 32 * NQ, wave1 = wave0 + 32 * NQ < rest ? wave0 + 32 * NQ : rest;
+  int32_t const all   = uniform(f.seen(block0 + (rest < Shape::kTokens ? rest : Shape::kTokens) - 1, tokens, keys));
+  int32_t const least = uniform(wave0 < rest ? f.seen(block0 + wave0, tokens, keys) : 0), most = uniform(wave0 < rest ? f.seen(block0 + wave1 - 1, tokens, keys) : 0);
+  int64_t const t0    = static_cast<int64_t>(begin) + block0 + wave0;
+
+  Attending<T, D, NQ> a;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    int32_t const i  = n * 32 + column;
+    bool const there = wave0 + i < rest;
+    a.seen[n]        = there ? f.seen(block0 + wave0 + i, tokens, keys) : 0;
+    a.begin(n, f.q.at(there ? t0 + i : begin, w.head), f.width, there, half);
+  }
+  TileLoader<T, D, WAVES> load_k, load_v;
+  load_k.aim(f.k, first, w.kv_head, f.width, wave, lane);
+  load_v.aim(f.v, first, w.kv_head, f.width, wave, lane);
+  TileReader<T, D> const read(lane);
+  float const scale   = f.scale * kLog2e;
+  int32_t const tiles = (all + kTile - 1) / kTile;
+  if (tiles > 0) {
+    load_k.load(lds, keys, wave);
+    load_v.load(lds + Tile<T, D>::kBytes, keys, wave);
+  }
+  for (int32_t tile = 0; tile < tiles; ++tile) {
+    LdsBytes const k_tile = lds + (tile & 1) * 2 * Tile<T, D>::kBytes;
+    stage_barrier<0>();
+    if (tile + 1 < tiles) {
+      LdsBytes const next = lds + (~tile & 1) * 2 * Tile<T, D>::kBytes;
+      load_k.load(next, keys - (tile + 1) * kTile, wave);
+      load_v.load(next + Tile<T, D>::kBytes, keys - (tile + 1) * kTile, wave);
+    }
+    int32_t const key0 = tile * kTile;
+    if (key0 < most) a.pass(k_tile, k_tile + Tile<T, D>::kBytes, read, key0, key0 + kTile > least, scale, half);
+  }
+  if (wave0 >= rest) return;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    uint32_t odd = a.finish(n, f, t0 + n * 32 + column, w.head, wave0 + n * 32 + column < rest, half, column);
+    for (; odd; odd &= odd - 1) attend_row(f, static_cast<int32_t>(t0) + n * 32 + __builtin_ctz(odd), w.head);
+  }
+}
+
+// ------------------------------------------------------------------ forward, in chunks of keys
+// Few tokens a row, as where texts go on token by token: one wavefront has all of a row's tokens and of all heads that share a key head, up to 32 together,
+// as the columns of its products, and a chunk of 2^shift of the row's keys; what it adds up is joined with that of the row's other chunks by another
+// launch.  Bound by memory: the keys are read once.  The chunks of key tokens are numbered as the blocks of tokens are elsewhere, so they are
+// alike in size however long the rows are.  A row of a single chunk is finished at once; so is one of more columns, by the workgroup of its first chunk
+// alone, 32 columns after the other.
+// Parts of a row of several chunks lie from number 2 * first / 2^shift on: it has at least half as many numbers up to the next row's as it has chunks.
+constexpr int kPartColumns = 32;
+
+template <typename T>
+struct ForwardChunks : Forward<T> {
+  int shift;
+  float* sums;    // [part][key head][column][D]
+  float2* tops;   // [part][key head][column]: top, and the sum of the exponentials
+  __device__ __forceinline__ int64_t part(int32_t first, int32_t chunk, int32_t kv_head) const
+  {
+    return ((static_cast<int64_t>(first) * 2 >> shift) + chunk) * this->kv_heads + kv_head;
+  }
+  __device__ __forceinline__ int32_t chunks_of(int32_t keys) const { return keys > 0 ? ((keys - 1) >> shift) + 1 : 1; }
+  __device__ __forceinline__ bool is_split(int32_t tokens, int32_t chunks) const { return chunks > 1 && static_cast<int64_t>(tokens) * (this->heads / this->kv_heads) <= kPartColumns; }
+};
+inline int64_t most_parts(int64_t key_tokens, int shift) { return (key_tokens * 2 >> shift) + 2; }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kWave, 1) attend_chunks_kernel(ForwardChunks<T> f)
+{
+  extern __shared__ __align__(16) char lds_[];
+  LdsBytes const lds  = (LdsBytes)lds_;
+  constexpr int kTile = Tile<T, D>::kHeads;
+  Work w;
+  if (!work_of(block_number(), f.key_runs.blocks(f.shift), f.kv_heads, 1, w)) return;
+  int32_t const run = f.key_runs.run_of(w.block, f.shift), each = f.heads / f.kv_heads;
+  int32_t first = 0, keys = 0;
+  if (f.is_row(run)) f.keys_of(run, first, keys);
+  first = uniform(first);
+  keys  = uniform(keys);
+  int32_t const begin = uniform(f.runs.begin(run)), tokens = uniform(f.runs.begin(run + 1)) - begin, chunks = f.chunks_of(keys);
+  int64_t const chunk = w.block - f.key_runs.first_block(run, f.shift);
+  bool const split    = f.is_split(tokens, chunks);
+  if (chunk >= (split ? chunks : 1)) return;
+  int const lane = lane_id(), column = lane % 32, half = lane / 32;
+  int32_t const key_first = split ? static_cast<int32_t>(chunk << f.shift) : 0, key_last = split && keys - key_first > 1 << f.shift ? key_first + (1 << f.shift) : keys;
+  int64_t const columns   = static_cast<int64_t>(tokens > 0 ? tokens : 0) * each;
+  TileReader<T, D> const read(lane);
+  float const scale = f.scale * kLog2e;
+  for (int64_t column0 = 0; column0 < columns; column0 += kPartColumns) {
+    int64_t const mine = column0 + column;
+    bool const there   = mine < columns;
+    int32_t const i    = there ? static_cast<int32_t>(mine / each) : 0, head = w.kv_head * each + (there ? static_cast<int32_t>(mine - static_cast<int64_t>(i) * each) : 0);
+    int64_t const t    = static_cast<int64_t>(begin) + i;
+    int32_t const last = static_cast<int32_t>(((column0 + kPartColumns < columns ? column0 + kPartColumns : columns) - 1) / each);  // the last column's token
+    Attending<T, D, 1> a;
+    a.seen[0] = there ? f.seen(i, tokens, keys) : 0;
+    a.begin(0, f.q.at(t, head), f.width, there, half);
+    int32_t const least = uniform(f.seen(static_cast<int32_t>(column0 / each), tokens, keys)), all = uniform(f.seen(last, tokens, keys)), end = all < key_last ? all : key_last;
+    int32_t const tiles = end > key_first ? (end - key_first + kTile - 1) / kTile : 0;
+    TileLoader<T, D, 1> load_k, load_v;
+    load_k.aim(f.k, first + key_first, w.kv_head, f.width, 0, lane);
+    load_v.aim(f.v, first + key_first, w.kv_head, f.width, 0, lane);
+    if (tiles > 0) {
+      load_k.load(lds, key_last - key_first, 0);
+      load_v.load(lds + Tile<T, D>::kBytes, key_last - key_first, 0);
+    }
+    for (int32_t tile = 0; tile < tiles; ++tile) {
+      LdsBytes const k_tile = lds + (tile & 1) * 2 * Tile<T, D>::kBytes;
+      int32_t const key0    = key_first + tile * kTile;
+      stage_barrier<0>();
+      if (tile + 1 < tiles) {
+        LdsBytes const next = lds + (~tile & 1) * 2 * Tile<T, D>::kBytes;
+        load_k.load(next, key_last - key0 - kTile, 0);
+        load_v.load(next + Tile<T, D>::kBytes, key_last - key0 - kTile, 0);
+      }
+      a.pass(k_tile, k_tile + Tile<T, D>::kBytes, read, key0, key0 + kTile > least || key0 + kTile > key_last, scale, half);
+    }
+    stage_barrier<0>();  // (the next columns' loads come into the same places)
+    if (split) {
+      int64_t const part = f.part(first, static_cast<int32_t>(chunk), w.kv_head) * kPartColumns + column;
+      Halves const both  = halves(a.sum[0]);
+      if (there) {
+        store_columns<float, D / 32>(f.sums + part * D, a.o[0], half, D);
+        if (half == 0) f.tops[part] = make_float2(a.top[0], both.low + both.high);
+      }
+      continue;
+    }
+    for (uint32_t odd = a.finish(0, f, t, head, there, half, column); odd; odd &= odd - 1) {
+      int const which = __builtin_ctz(odd);
+      attend_row(f, __builtin_amdgcn_readlane(static_cast<int32_t>(t), which), __builtin_amdgcn_readlane(head, which));
     }
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) query_gradient_rows_kernel(Backward<T> f)
+// Joins the parts of a head of a token, a workgroup for each: its wavefronts take every fourth part.
+constexpr int kJoinWaves = 4;
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinWaves * kWave) attend_join_kernel(ForwardChunks<T> f)
 {
-  int64_t const w = block_number() * (kThreads / kWave) + threadIdx.x / kWave;
-  if (w >= static_cast<int64_t>(f.runs.tokens) * f.heads) return;
-  query_gradient_row(f, static_cast<int32_t>(w / f.heads), static_cast<int32_t>(w % f.heads));
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) key_gradient_rows_kernel(Backward<T> f)
-{
-  int64_t const w = block_number() * (kThreads / kWave) + threadIdx.x / kWave;
-  if (w >= static_cast<int64_t>(f.key_runs.tokens) * f.kv_heads) return;
-  key_gradient_row(f, static_cast<int32_t>(w / f.kv_heads), static_cast<int32_t>(w % f.kv_heads));
+  constexpr int kEach = D / kWave;
+  typedef float Some __attribute__((ext_vector_type(kEach)));
+  __shared__ float tops[kJoinWaves], totals[kJoinWaves];
+  __shared__ Some sums[kJoinWaves][kWave];
+  int64_t const item = block_number();
+  if (item >= static_cast<int64_t>(f.runs.tokens) * f.heads) return;
+  int32_t const t = static_cast<int32_t>(item / f.heads), head = static_cast<int32_t>(item % f.heads), run = run_with(f.runs, t);
+  if (!f.is_row(run)) return;
+  int32_t first, keys;
+  f.keys_of(run, first, keys);
+  int32_t const begin = f.runs.begin(run), tokens = f.runs.begin(run + 1) - begin, chunks = f.chunks_of(keys), each = f.heads / f.kv_heads;
+  if (!f.is_split(tokens, chunks)) return;
+  int const wave = threadIdx.x / kWave, lane = lane_id();
+  int32_t const column = (t - begin) * each + head % each;
+  int64_t const at = f.part(first, 0, head / each) * kPartColumns + column, step = static_cast<int64_t>(f.kv_heads) * kPartColumns;
+  float top = -INFINITY;
+  for (int32_t c = threadIdx.x; c < chunks; c += kJoinWaves * kWave) top = fmaxf(top, f.tops[at + c * step].x);
+  top = wave_max(top);
+  if (lane == 0) tops[wave] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinWaves; ++w) top = fmaxf(top, tops[w]);
+  float total = 0.f;
+  Some sum{};
+#pragma unroll 8
+  for (int32_t c = wave; c < chunks; c += kJoinWaves) {
+    float2 const of     = f.tops[at + c * step];
+    float const weight  = of.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(of.x - top);
+    Some const part     = *reinterpret_cast<const Some*>(f.sums + (at + c * step) * D + lane * kEach);
+    total += of.y * weight;
+    sum += part * weight;
+  }
+  sums[wave][lane] = sum;
+  if (lane == 0) totals[wave] = total;
+  __syncthreads();
+  if (wave != 0) return;
+#pragma unroll
+  for (int w = 1; w < kJoinWaves; ++w) {
+    total += totals[w];
+    sum += sums[w][lane];
+  }
+  int32_t const seen = f.seen(t - begin, tokens, keys);
+  bool finite        = true;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    sum[k] = seen > 0 ? sum[k] / total : 0.f;
+    finite = finite && fabsf(sum[k]) < INFINITY;
+  }
+  if (seen > 0 && __ballot(!finite)) {  // (as in finish)
+    attend_row(f, t, head);
+    return;
+  }
+  T* const out = f.out.at(t, head);
+#pragma unroll
+  for (int k = 0; k < kEach; ++k)
+    if (lane * kEach + k < f.width) out[lane * kEach + k] = static_cast<T>(sum[k]);
+  if (f.logsum && lane == 0) f.logsum[static_cast<int64_t>(head) * f.runs.tokens + t] = seen > 0 ? (top + __builtin_amdgcn_logf(total)) * kLn2 : -INFINITY;
 }
 
 // ------------------------------------------------------------------ the gradients, in tiles
@@ -227,10 +384,10 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
   constexpr int kSteps = D / 16, kColumns = D / 32, kTile = Shape::kTile, kBlocks = kTile / 32;
   Work w;
   int32_t const each = f.heads / f.kv_heads;
-  if (!work_of(block_number(), f.runs.template blocks<Shape::kShift>(), f.kv_heads, each, w)) return;
-  int32_t const run    = f.runs.template run_of<Shape::kShift>(w.block);
+  if (!work_of(block_number(), f.runs.blocks(Shape::kShift), f.kv_heads, each, w)) return;
+  int32_t const run    = f.runs.run_of(w.block, Shape::kShift);
   int32_t const begin  = uniform(f.runs.begin(run)), tokens = uniform(f.runs.begin(run + 1)) - begin;
-  int64_t const in_run = (w.block - f.runs.template first_block<Shape::kShift>(run)) << Shape::kShift;
+  int64_t const in_run = (w.block - f.runs.first_block(run, Shape::kShift)) << Shape::kShift;
   if (in_run >= tokens) return;
   int const wave = uniform(threadIdx.x / kWave), lane = lane_id(), column = lane % 32, half = lane / 32;
   int32_t const block0 = static_cast<int32_t>(in_run), rest = uniform(tokens - block0);
@@ -339,11 +496,11 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
   constexpr bool kK = PART != kOfV, kV = PART != kOfK;
   constexpr int kSteps = D / 16, kColumns = D / 32, kTile = Shape::kTile, kBlocks = kTile / 32;
   Work w;
-  if (!work_of(block_number(), f.key_runs.template blocks<Shape::kShift>(), f.kv_heads, 1, w)) return;
-  w.block              = f.key_runs.template blocks<Shape::kShift>() - 1 - w.block;  // (of a long row, the first keys are those that most tokens see)
-  int32_t const run    = f.key_runs.template run_of<Shape::kShift>(w.block), each = f.heads / f.kv_heads;
+  if (!work_of(block_number(), f.key_runs.blocks(Shape::kShift), f.kv_heads, 1, w)) return;
+  w.block              = f.key_runs.blocks(Shape::kShift) - 1 - w.block;  // (of a long row, the first keys are those that most tokens see)
+  int32_t const run    = f.key_runs.run_of(w.block, Shape::kShift), each = f.heads / f.kv_heads;
   int32_t const first  = uniform(f.key_runs.begin(run)), places = uniform(f.key_runs.begin(run + 1)) - first;
-  int64_t const in_run = (w.block - f.key_runs.template first_block<Shape::kShift>(run)) << Shape::kShift;
+  int64_t const in_run = (w.block - f.key_runs.first_block(run, Shape::kShift)) << Shape::kShift;
   if (in_run >= places) return;
   int const wave = uniform(threadIdx.x / kWave), lane = lane_id(), column = lane % 32, half = lane / 32;
   int32_t const block0 = static_cast<int32_t>(in_run), rest = uniform(places - block0);  // (places: with those behind the row's keys, whose gradients are zeros)
@@ -588,9 +745,32 @@ nvtext_amd_status attend_tiles(Forward<T> const& f, hipStream_t stream)
   using Shape = ForwardShape<T, D, WAVES, NQ>;
   ProfileScope const scope("attention_tiles", stream);
   NVTEXT_HIP_TRY(allow_lds(attend_tiles_kernel<T, D, WAVES, NQ>, Shape::kLds));
-  int64_t const items = work_items(f.runs.template blocks<Shape::kShift>(), f.kv_heads, f.heads / f.kv_heads);
+  int64_t const items = work_items(f.runs.blocks(Shape::kShift), f.kv_heads, f.heads / f.kv_heads);
   hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_tiles_kernel<T, D, WAVES, NQ>), grid_of(items, WAVES * kWave), dim3(WAVES * kWave), Shape::kLds, stream, f);
   return NVTEXT_AMD_SUCCESS;
+}
+
+template <typename T, int D>
+nvtext_amd_status attend_chunks(ForwardChunks<T> const& f, hipStream_t stream)
+{
+  constexpr int kLds = 4 * Tile<T, D>::kBytes;
+  NVTEXT_HIP_TRY(allow_lds(attend_chunks_kernel<T, D>, kLds));
+  {
+    ProfileScope const scope("attention_chunks", stream);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_chunks_kernel<T, D>), grid_of(work_items(f.key_runs.blocks(f.shift), f.kv_heads, 1), kWave), dim3(kWave), kLds, stream, f);
+  }
+  ProfileScope const scope("attention_join", stream);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_join_kernel<T, D>), grid_of(static_cast<int64_t>(f.runs.tokens) * f.heads, kJoinWaves * kWave), dim3(kJoinWaves * kWave), 0, stream, f);
+  return NVTEXT_AMD_SUCCESS;
+}
+
+// calls f with the width of the tiles that heads of `width` values go through
+template <typename F>
+nvtext_amd_status with_tiles(int32_t width, F&& f)
+{
+  if (width <= 64) return f(std::integral_constant<int, 64>{});
+  if (width <= 128) return f(std::integral_constant<int, 128>{});
+  return f(std::integral_constant<int, 256>{});
 }
 
 template <typename T>
@@ -600,12 +780,18 @@ nvtext_amd_status attention(Forward<T> f, Mr const& mr, hipStream_t stream)
   align.add(f.q, f.runs.tokens, f.heads);
   align.add(f.k, f.key_runs.tokens, f.kv_heads);
   align.add(f.v, f.key_runs.tokens, f.kv_heads);
-  Temp const copies(mr, align.bytes());
-  if (!copies.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
-  align.launch(copies.template as<char>(), stream);
-  if (f.width <= 64) return attend_tiles<T, 64, 4, 1>(f, stream);
-  if (f.width <= 128) return attend_tiles<T, 128, 4, 1>(f, stream);
-  return attend_tiles<T, 256, 4, 1>(f, stream);
+  bool const chunks = f.runs.rows > 0 && static_cast<int64_t>(f.runs.tokens) * (f.heads / f.kv_heads) <= static_cast<int64_t>(f.runs.rows) * kPartColumns;
+  int shift = 7;
+  while (shift < 30 && (static_cast<int64_t>(f.key_runs.tokens) * f.kv_heads >> shift) > 2048) ++shift;
+  return with_tiles(f.width, [&](auto d) {
+    constexpr int kD        = decltype(d)::value;
+    size_t const parts      = chunks ? static_cast<size_t>(most_parts(f.key_runs.tokens, shift)) * static_cast<size_t>(f.kv_heads) * kPartColumns : 0;
+    TempParts<3> const temp(mr, {align.bytes(), parts * kD * sizeof(float), parts * sizeof(float2)});
+    if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
+    align.launch(temp.template part<char>(0), stream);
+    if (chunks) return attend_chunks<T, kD>({f, shift, temp.template part<float>(1), temp.template part<float2>(2)}, stream);
+    return attend_tiles<T, kD, 4, 1>(f, stream);
+  });
 }
 
 template <typename T, int D, int WAVES, Part PART>
@@ -614,7 +800,7 @@ nvtext_amd_status key_gradient_tiles(Backward<T> const& f, hipStream_t stream)
   using Shape = GradientShape<T, D, WAVES>;
   ProfileScope const scope("attention_key_gradient", stream);
   NVTEXT_HIP_TRY(allow_lds(key_gradient_tiles_kernel<T, D, WAVES, PART>, Shape::kKeyLds));
-  int64_t const items = work_items(f.key_runs.template blocks<Shape::kShift>(), f.kv_heads, 1);
+  int64_t const items = work_items(f.key_runs.blocks(Shape::kShift), f.kv_heads, 1);
   hipLaunchKernelGGL(HIP_KERNEL_NAME(key_gradient_tiles_kernel<T, D, WAVES, PART>), grid_of(items, WAVES * kWave), dim3(WAVES * kWave), Shape::kKeyLds, stream, f);
   return NVTEXT_AMD_SUCCESS;
 }
@@ -626,7 +812,7 @@ nvtext_amd_status gradient_tiles(Backward<T> const& f, hipStream_t stream)
   if (f.runs.tokens > 0) {
     ProfileScope const scope("attention_query_gradient", stream);
     NVTEXT_HIP_TRY(allow_lds(query_gradient_tiles_kernel<T, D, WAVES>, Shape::kLds));
-    int64_t const items = work_items(f.runs.template blocks<Shape::kShift>(), f.kv_heads, f.heads / f.kv_heads);
+    int64_t const items = work_items(f.runs.blocks(Shape::kShift), f.kv_heads, f.heads / f.kv_heads);
     hipLaunchKernelGGL(HIP_KERNEL_NAME(query_gradient_tiles_kernel<T, D, WAVES>), grid_of(items, WAVES * kWave), dim3(WAVES * kWave), Shape::kLds, stream, f);
   }
   if (f.key_runs.tokens == 0) return NVTEXT_AMD_SUCCESS;
@@ -650,9 +836,7 @@ nvtext_amd_status attention_backward(Backward<T> f, Mr const& mr, hipStream_t st
   f.deltas = temp.template part<float>(0);
   f.logs   = temp.template part<float>(1);
   align.launch(temp.template part<char>(2), stream);
-  if (f.width <= 64) return gradient_tiles<T, 64, 4>(f, stream);
-  if (f.width <= 128) return gradient_tiles<T, 128, 4>(f, stream);
-  return gradient_tiles<T, 256, 4>(f, stream);
+  return with_tiles(f.width, [&](auto d) { return gradient_tiles<T, decltype(d)::value, 4>(f, stream); });
 }
 
 // What both directions ask of their arguments; nullptr if it holds.

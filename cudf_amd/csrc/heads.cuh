@@ -66,29 +66,20 @@ struct Runs {
   // where run i begins, i up to rows + 2
   __device__ __forceinline__ int32_t begin(int32_t i) const { return i <= 0 || rows == 0 ? (i <= 1 ? 0 : tokens) : i >= rows + 2 ? tokens : clamped(offsets[i - 1]); }
 
-  // Runs are cut into blocks of 2^SHIFT tokens, each run from its own begin.  A run's blocks have numbers from
-  // begin / 2^SHIFT + its own number on: as many as it needs or one more, so no block is two runs' and nobody has to count
+  // Runs are cut into blocks of 2^shift tokens, each run from its own begin.  A run's blocks have numbers from
+  // begin / 2^shift + its own number on: as many as it needs or one more, so no block is two runs' and nobody has to count
   // blocks before the kernel.  Block numbers are below blocks().
-  template <int SHIFT>
-  __host__ __device__ __forceinline__ int64_t blocks() const
-  {
-    return (static_cast<int64_t>(tokens) >> SHIFT) + rows + 2;
-  }
-  template <int SHIFT>
-  __device__ __forceinline__ int64_t first_block(int32_t i) const
-  {
-    return (static_cast<int64_t>(begin(i)) >> SHIFT) + i;
-  }
+  __host__ __device__ __forceinline__ int64_t blocks(int shift) const { return (static_cast<int64_t>(tokens) >> shift) + rows + 2; }
+  __device__ __forceinline__ int64_t first_block(int32_t i, int shift) const { return (static_cast<int64_t>(begin(i)) >> shift) + i; }
   // The run that block `b` is one of, the same in all lanes of the (whole) wavefront: the last whose first block is not behind b.
   // The lanes look at 64 runs at once: two rounds of reads for 4,000 rows, where halving takes twelve, one after the other.
-  template <int SHIFT>
-  __device__ __forceinline__ int32_t run_of(int64_t b) const
+  __device__ __forceinline__ int32_t run_of(int64_t b, int shift) const
   {
     int32_t lo = 0, count = rows + 2;  // the run is one of lo .. lo + count - 1, and lo's first block is not behind b
     while (count > 1) {
       int32_t const each = (count + kWave - 1) / kWave;
       int32_t const i    = lane_id() * each;
-      bool const reached = i < count && first_block<SHIFT>(lo + i) <= b;
+      bool const reached = i < count && first_block(lo + i, shift) <= b;
       uint64_t const all = __ballot(reached) | 1;
       int32_t const last = 63 - __clzll(static_cast<long long>(all));
       lo += last * each;
