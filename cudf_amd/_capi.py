@@ -283,8 +283,8 @@ def load():
                     (L.nvtext_amd_linear, [matrix] * 3 + [C.c_int32, matrix, ptr, mr, matrix, matrix]),
                     (L.nvtext_amd_linear_backward, [matrix] * 3 + [C.c_int32, matrix, ptr, mr] + [matrix] * 3),
                     (L.nvtext_amd_rotary, [heads, C.c_int32, ptr, ptr, ptr, C.c_int64, C.c_int32, C.c_int32, C.c_double, ptr, heads]),
-                    (L.nvtext_amd_attention, [heads] * 3 + seen + [ptr, mr, heads, ptr]),
-                    (L.nvtext_amd_attention_backward, [heads] * 5 + [ptr] + seen + [ptr, mr] + [heads] * 3)):
+                    (L.nvtext_amd_attention, [heads] * 3 + seen + [ptr, mr, heads, ptr, ptr]),
+                    (L.nvtext_amd_attention_backward, [heads] * 5 + [ptr, ptr] + seen + [ptr, mr] + [heads] * 3)):
         f.restype = C.c_int
         f.argtypes = args
     L.nvtext_amd_profile_enable.restype = None

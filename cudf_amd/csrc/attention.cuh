@@ -4,6 +4,8 @@
 #include "heads.cuh"
 #include "matrix.cuh"
 
+#include <type_traits>
+
 namespace nvtext_amd {
 
 constexpr int kMostWidth  = 256;
@@ -59,10 +61,30 @@ __device__ __forceinline__ float wave_max(float v)
   return v;
 }
 
+// What rounding to a 16-bit type leaves off, in 8 bits more: the difference of the two values' bits as float32, in 2^-8 of a step of the type.  (Signs
+// are alike, so bits differ as values do; zeros and the smallest numbers, whose steps are others, get what 8 bits hold of it.)  With them a sum of products
+// with out is as good as one with out in float32 for what is rounded to 16 bits afterwards.
+template <typename T>
+__device__ __forceinline__ int8_t rest_of(float x, T rounded)
+{
+  constexpr int kShift = sizeof(T) == 4 ? 0 : std::is_same_v<T, half_t> ? 5 : 8;
+  float const y        = static_cast<float>(rounded);
+  if (!(fabsf(y) < INFINITY)) return 0;
+  int32_t const off = (__builtin_bit_cast(int32_t, x) - __builtin_bit_cast(int32_t, y) + (1 << kShift >> 1)) >> kShift;
+  return static_cast<int8_t>(off < -127 ? -127 : off > 127 ? 127 : off);
+}
+template <typename T>
+__device__ __forceinline__ float with_rest(T rounded, int32_t rest)
+{
+  constexpr int kShift = std::is_same_v<T, half_t> ? 5 : 8;
+  return __builtin_bit_cast(float, __builtin_bit_cast(int32_t, static_cast<float>(rounded)) + rest * (1 << kShift));
+}
+
 template <typename T>
 struct Forward : Problem<T> {
   Heads<T> out;
   float* logsum;
+  int8_t* rest;  // [tokens, heads, width], of 16-bit types; or nullptr
 };
 
 // The run that token t is in.
@@ -111,7 +133,11 @@ __device__ void attend_row(Forward<T> const& f, int32_t t, int32_t h)
   }
 #pragma unroll
   for (int c = 0; c < kMostWidth / kWave; ++c)
-    if (c * kWave + lane < f.width) f.out.at(t, h)[c * kWave + lane] = static_cast<T>(seen > 0 ? o[c] / sum : 0.f);
+    if (c * kWave + lane < f.width) {
+      float const x                      = seen > 0 ? o[c] / sum : 0.f;
+      f.out.at(t, h)[c * kWave + lane] = static_cast<T>(x);
+      if (f.rest) f.rest[(static_cast<int64_t>(t) * f.heads + h) * f.width + c * kWave + lane] = rest_of(x, static_cast<T>(x));
+    }
   if (f.logsum && lane == 0) f.logsum[static_cast<int64_t>(h) * f.runs.tokens + t] = seen > 0 ? (top + __builtin_amdgcn_logf(sum)) * kLn2 : -INFINITY;
 }
 
@@ -119,6 +145,7 @@ template <typename T>
 struct Backward : Problem<T> {
   Heads<const T> grad, out;
   const float* logsum;
+  const int8_t* rest;  // out's, or nullptr
   float* deltas;  // [heads, tokens]: grad . out
   float* logs;    // [heads, tokens]: logsum in powers of 2 (the tiles' own)
   Heads<T> q_grad, k_grad, v_grad;
@@ -139,7 +166,13 @@ __device__ void query_gradient_row(Backward<T> const& f, int32_t t, int32_t h)
   const T *const q = f.q.at(t, h), *const g = f.grad.at(t, h);
   int64_t const at  = static_cast<int64_t>(h) * f.runs.tokens + t;
   float const log   = f.logsum[at] * kLog2e, scale = f.scale * kLog2e;
-  float const delta = seen > 0 ? dot(g, f.out.at(t, h), f.width) : 0.f;
+  float delta       = 0.f;
+  if (seen > 0 && f.rest) {
+    for (int32_t j = 0; j < f.width; ++j)
+      delta = fmaf(static_cast<float>(g[j]), with_rest(f.out.at(t, h)[j], f.rest[(static_cast<int64_t>(t) * f.heads + h) * f.width + j]), delta);
+  } else if (seen > 0) {
+    delta = dot(g, f.out.at(t, h), f.width);
+  }
   if (lane == 0) f.deltas[at] = delta;
   float d[kMostWidth / kWave] = {};
   for (int32_t base = 0; base < seen; base += kWave) {
@@ -261,10 +294,11 @@ struct TileLoader {
   // The next tile, of which `here` heads are there.
   __device__ __forceinline__ void load(LdsBytes to, int32_t here, int wave)
   {
-    uint32_t const range = static_cast<uint32_t>(here < Of::kHeads ? here - 1 : Of::kHeads - 1) * line + width;
+    uint32_t const range = uniform(static_cast<uint32_t>(here < Of::kHeads ? here - 1 : Of::kHeads - 1) * line + width);
+    const char* const at = uniform(base);
 #pragma unroll
     for (int p = 0; p < kLoads; ++p)
-      if (kAll % WAVES == 0 || p * WAVES + wave < kAll) load_to_lds(base, range, to + (p * WAVES + wave) * 1024, offset[p]);
+      if (kAll % WAVES == 0 || p * WAVES + wave < kAll) load_to_lds(at, range, to + (p * WAVES + wave) * 1024, offset[p]);
     base += static_cast<int64_t>(Of::kHeads) * line;
   }
 };
@@ -367,6 +401,29 @@ __device__ __forceinline__ void store_columns(T* head, f32x16_t const (&x)[COLUM
     for (int g = 0; g < 4; ++g) {
       int32_t const j = 32 * c + 8 * g + 4 * half;
       Four const four = {static_cast<T>(x[c][4 * g]), static_cast<T>(x[c][4 * g + 1]), static_cast<T>(x[c][4 * g + 2]), static_cast<T>(x[c][4 * g + 3])};
+      if (j + 4 <= width) {
+        *reinterpret_cast<Four*>(head + j) = four;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (j + e < width) head[j + e] = four[e];
+      }
+    }
+}
+
+// Writes what rounding left off a lane's column of results, in the same places of a head's.
+template <typename T, int COLUMNS>
+__device__ __forceinline__ void store_rests(int8_t* head, f32x16_t const (&x)[COLUMNS], int half, int32_t width)
+{
+  typedef int8_t Four __attribute__((ext_vector_type(4), aligned(1)));
+#pragma unroll
+  for (int c = 0; c < COLUMNS; ++c)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      int32_t const j = 32 * c + 8 * g + 4 * half;
+      Four four;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) four[e] = rest_of(x[c][4 * g + e], static_cast<T>(x[c][4 * g + e]));
       if (j + 4 <= width) {
         *reinterpret_cast<Four*>(head + j) = four;
       } else {

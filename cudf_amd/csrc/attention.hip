@@ -140,6 +140,8 @@ struct Attending {
     odd          = (odd | odd >> 32) & 0xffffffffu;
     if (there && !(odd >> column & 1)) {
       store_columns<T, kColumns>(f.out.at(t, h), o[n], half, f.width);
+      if constexpr (sizeof(T) == 2)
+        if (f.rest) store_rests<T, kColumns>(f.rest + (t * f.heads + h) * f.width, o[n], half, f.width);
       if (f.logsum && half == 0) f.logsum[static_cast<int64_t>(h) * f.runs.tokens + t] = seen[n] > 0 ? (top[n] + __builtin_amdgcn_logf(total)) * kLn2 : -INFINITY;
     }
     return static_cast<uint32_t>(odd);
@@ -361,7 +363,10 @@ __global__ void __launch_bounds__(kJoinWaves * kWave) attend_join_kernel(Forward
   T* const out = f.out.at(t, head);
 #pragma unroll
   for (int k = 0; k < kEach; ++k)
-    if (lane * kEach + k < f.width) out[lane * kEach + k] = static_cast<T>(sum[k]);
+    if (lane * kEach + k < f.width) {
+      out[lane * kEach + k] = static_cast<T>(sum[k]);
+      if (f.rest) f.rest[item * f.width + lane * kEach + k] = rest_of(sum[k], static_cast<T>(sum[k]));
+    }
   if (f.logsum && lane == 0) f.logsum[static_cast<int64_t>(head) * f.runs.tokens + t] = seen > 0 ? (top + __builtin_amdgcn_logf(total)) * kLn2 : -INFINITY;
 }
 
@@ -409,8 +414,16 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
     q[s] = fragment_of(f.q.at(t, w.head), 16 * s + 8 * half, f.width, there);
     g[s] = fragment_of(f.grad.at(t, w.head), 16 * s + 8 * half, f.width, there);
     Fragment<T> const out = fragment_of(f.out.at(t, w.head), 16 * s + 8 * half, f.width, there);
+    bool rests = false;
+    if constexpr (sizeof(T) == 2) rests = f.rest != nullptr;
+    if (rests) {
+      auto const rest = load_raw8(f.rest + (t * f.heads + w.head) * f.width + 16 * s + 8 * half, there ? f.width - 16 * s - 8 * half : 0);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) delta = fmaf(static_cast<float>(g[s][k]), static_cast<float>(out[k]), delta);
+      for (int k = 0; k < 8; ++k) delta = fmaf(static_cast<float>(g[s][k]), with_rest(out[k], rest[k]), delta);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) delta = fmaf(static_cast<float>(g[s][k]), static_cast<float>(out[k]), delta);
+    }
   }
   Halves const both = halves(delta);
   delta             = seen > 0 ? both.low + both.high : 0.f;
@@ -872,7 +885,8 @@ Problem<T> problem_of(const nvtext_amd_heads* q, const nvtext_amd_heads* k, cons
 extern "C" {
 
 nvtext_amd_status nvtext_amd_attention(const nvtext_amd_heads* q, const nvtext_amd_heads* k, const nvtext_amd_heads* v, int32_t rows, const int32_t* offsets, const int32_t* key_offsets,
-                                       const int32_t* key_lengths, int32_t causal, double scale, void* stream_, const nvtext_amd_allocator* mr_, const nvtext_amd_heads* out, float* logsum)
+                                       const int32_t* key_lengths, int32_t causal, double scale, void* stream_, const nvtext_amd_allocator* mr_, const nvtext_amd_heads* out, float* logsum,
+                                       int8_t* rest)
 {
   using namespace nvtext_amd;
   EntryScope const entry("nvtext_amd_attention");
@@ -886,7 +900,7 @@ nvtext_amd_status nvtext_amd_attention(const nvtext_amd_heads* q, const nvtext_a
   nvtext_amd_status st = NVTEXT_AMD_SUCCESS;
   with_type(q->type, [&](auto zero) {
     using T = decltype(zero);
-    st      = attention<T>({problem_of<T>(q, k, v, rows, offsets, key_offsets, key_lengths, causal, scale), heads_of<T>(out), logsum}, mr, stream);
+    st      = attention<T>({problem_of<T>(q, k, v, rows, offsets, key_offsets, key_lengths, causal, scale), heads_of<T>(out), logsum, q->type == NVTEXT_AMD_TYPE_FLOAT32 ? nullptr : rest}, mr, stream);
   });
   if (st != NVTEXT_AMD_SUCCESS) return st;
   NVTEXT_HIP_TRY(hipGetLastError());
@@ -894,7 +908,7 @@ nvtext_amd_status nvtext_amd_attention(const nvtext_amd_heads* q, const nvtext_a
 }
 
 nvtext_amd_status nvtext_amd_attention_backward(const nvtext_amd_heads* grad, const nvtext_amd_heads* q, const nvtext_amd_heads* k, const nvtext_amd_heads* v, const nvtext_amd_heads* out,
-                                                const float* logsum, int32_t rows, const int32_t* offsets, const int32_t* key_offsets, const int32_t* key_lengths, int32_t causal,
+                                                const float* logsum, const int8_t* rest, int32_t rows, const int32_t* offsets, const int32_t* key_offsets, const int32_t* key_lengths, int32_t causal,
                                                 double scale, void* stream_, const nvtext_amd_allocator* mr_, const nvtext_amd_heads* q_grad, const nvtext_amd_heads* k_grad,
                                                 const nvtext_amd_heads* v_grad)
 {
@@ -921,6 +935,7 @@ nvtext_amd_status nvtext_amd_attention_backward(const nvtext_amd_heads* grad, co
     b.grad   = heads_of<const T>(grad);
     b.out    = heads_of<const T>(out);
     b.logsum = logsum;
+    b.rest   = q->type == NVTEXT_AMD_TYPE_FLOAT32 ? nullptr : rest;
     b.q_grad = heads_of<T>(q_grad);
     b.k_grad = heads_of<T>(k_grad);
     b.v_grad = heads_of<T>(v_grad);

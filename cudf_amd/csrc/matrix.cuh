@@ -19,6 +19,13 @@ using LdsBytes = __attribute__((address_space(3))) char*;
 // The same in every lane, and known to be.
 __device__ __forceinline__ int32_t uniform(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 
+__device__ __forceinline__ const char* uniform(const char* p)
+{
+  uint64_t const v    = reinterpret_cast<uint64_t>(p);
+  uint32_t const low  = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v)), high = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+  return reinterpret_cast<const char*>(static_cast<uint64_t>(high) << 32 | low);
+}
+
 // 16 bytes a lane from base + offset to 16 bytes a lane from `to` on; zeros where the offset is not less than `range`.  Written out: the
 // compiler would wait for loads that it knows to write LDS before every transposing read of LDS (a product of which one operand
 // is read that way took 153 us instead of 118).  It has no register as a result, so it is waited for by stage_barrier alone.

@@ -198,7 +198,8 @@ nvtext_amd_status nvtext_amd_rotary(const nvtext_amd_heads* x,
  * a token that sees none, or belongs to no row, has zeros in out and -infinity in logsum.  What a token does not see is without
  * effect on it, whatever it is, NaN too.
  * q, k, v and out are of one type and width, of at most 256 values; scale is not negative.  logsum (NULL: not wanted; the gradient needs it)
- * has a value of FLOAT32 at [h * tokens + t].  Products, exponentials' sums and out are held in 32 bits; of 16-bit types, the exponentials are
+ * has a value of FLOAT32 at [h * tokens + t].  rest (NULL: not wanted; FLOAT32 has none), of a value for each of out's, [tokens, heads, width]
+ * one after the other: what rounding left off it, in 8 bits, for the gradient.  Products, exponentials' sums and out are held in 32 bits; of 16-bit types, the exponentials are
  * rounded to the type before they are multiplied with v (the values that logsum sums are not), as the matrix cores take them. */
 nvtext_amd_status nvtext_amd_attention(const nvtext_amd_heads* q,
                                        const nvtext_amd_heads* k,
@@ -212,9 +213,11 @@ nvtext_amd_status nvtext_amd_attention(const nvtext_amd_heads* q,
                                        void* stream,
                                        const nvtext_amd_allocator* mr,
                                        const nvtext_amd_heads* out,
-                                       float* logsum);
+                                       float* logsum,
+                                       int8_t* rest);
 
-/* The gradients of attention from grad, that of its out, and from its out and logsum, over the same rows.  With p = exp(s - logsum)
+/* The gradients of attention from grad, that of its out, and from its out, logsum and rest, over the same rows.  (rest may be NULL: the
+ * gradients of q and k are off by a rounding of out more, then.)  With p = exp(s - logsum)
  * and d = p * (grad . v - grad . out), for every token and the keys it sees, each rounded to the type before it is multiplied:
  *   q_grad = scale * sum over the keys of d * k,
  *   k_grad = scale * sum over the tokens, and the heads that see one, of d * q,  v_grad = the same sum of p * grad.
@@ -226,6 +229,7 @@ nvtext_amd_status nvtext_amd_attention_backward(const nvtext_amd_heads* grad,
                                                 const nvtext_amd_heads* v,
                                                 const nvtext_amd_heads* out,
                                                 const float* logsum,
+                                                const int8_t* rest,
                                                 int32_t rows,
                                                 const int32_t* offsets,
                                                 const int32_t* key_offsets,

@@ -46,6 +46,14 @@ def ints(values):
     return torch.tensor(values, dtype=torch.int32, device="cuda")
 
 
+def unrounded(saved):
+    """out's values with what rounding left off them: its bits as float32 with the rest's behind them."""
+    if saved.rest is None:
+        return saved.out.double().cpu().numpy()
+    shift = {F16: 5, BF16: 8}[saved.out.dtype]
+    return (saved.out.float().view(torch.int32) + saved.rest.int() * 2**shift).view(torch.float32).double().cpu().numpy()
+
+
 def offsets_of(lengths, first=0):
     return np.concatenate([[first], first + np.cumsum(lengths)]).astype(np.int32)
 
@@ -204,6 +212,23 @@ def test_attention_backward(case, causal, dtype):
     Made(case, dtype).check_backward(causal)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("case", [CASES[2], CASES[5], CASES[12], CASES[15], CASES[17], CASES[21], CASES[25]], ids=str)
+def test_what_rounding_leaves_off(case, dtype):
+    """Both directions together: the gradients from the out that was rounded and its rest are those from out as it is, up to a 2^-8 of a step
+    of it, and what the forward pass may be off by."""
+    m = Made(case, dtype, seed=3)
+    want, log, off, log_off = orc.attention(m.q64, m.k64, m.v64, **m.oracle_rows(), causal=True, **rounding(dtype))
+    out, saved = encoder.attention(m.q, m.k, m.v, *m.rows(), causal=True, keep=True)
+    assert saved.rest.dtype == torch.int8 and saved.rest.shape == out.shape
+    more = unrounded(saved)
+    assert (np.abs(more - want) <= off * 1.01 + UNIT[dtype] * 2.0**-7 * np.abs(want) + 2 * TINY[dtype]).all()
+    wants, offs = orc.attention_backward(m.g64, m.q64, m.k64, m.v64, more, saved.logsum.double().cpu().numpy(), **m.oracle_rows(), causal=True, **rounding(dtype))
+    got = encoder.attention_backward(m.g, m.q, m.k, m.v, saved, *m.rows(), causal=True)
+    for x, w, o in zip(got, wants, offs):
+        near(x, w, o)
+
+
 @pytest.mark.parametrize("case", [CASES[1], CASES[5], CASES[11], CASES[17], CASES[20], CASES[22], CASES[25]], ids=str)
 def test_keys_in_places_with_room(case):
     """What lies behind a row's keys is not read: NaN there."""
@@ -265,9 +290,10 @@ def test_what_is_not_seen_has_no_effect(dtype, value):
             assert not torch.isfinite(out[bad]).any()
         # and the way back: of q, what does not see it; of k and v, what only tokens see that do not (none in its row behind it)
         clean = encoder.attention(m.q, m.k, m.v, ints(m.offsets), causal=True, keep=True)[1]
-        saved = encoder.AttentionSaved(torch.where(pick[:, None, None], clean.out, out), torch.where(pick[None], clean.logsum, saved.logsum))
+        saved = encoder.AttentionSaved(torch.where(pick[:, None, None], clean.out, out), torch.where(pick[None], clean.logsum, saved.logsum),
+                                       None if saved.rest is None else torch.where(pick[:, None, None], clean.rest, saved.rest))
         grads = encoder.attention_backward(g, q, k, v, saved, ints(m.offsets), causal=True)
-        wants, offs = orc.attention_backward(m.g64, m.q64, m.k64, m.v64, clean.out.double().cpu().numpy(), clean.logsum.double().cpu().numpy(), m.offsets, causal=True, **rounding(dtype))
+        wants, offs = orc.attention_backward(m.g64, m.q64, m.k64, m.v64, unrounded(clean), clean.logsum.double().cpu().numpy(), m.offsets, causal=True, **rounding(dtype))
         near(grads[0][pick], wants[0][untouched], offs[0][untouched])
         others = np.ones(len(q), bool)
         others[int(m.offsets[1]):int(m.offsets[2])] = False
@@ -283,7 +309,7 @@ def test_what_is_not_seen_has_no_effect(dtype, value):
     pick = torch.from_numpy(others).cuda()
     near(out[pick], want[others], off[others])
     grads = encoder.attention_backward(g, q, m.k, m.v, saved, ints(m.offsets), causal=True)
-    wants, offs = orc.attention_backward(m.g64, m.q64, m.k64, m.v64, clean.out.double().cpu().numpy(), clean.logsum.double().cpu().numpy(), m.offsets, causal=True, **rounding(dtype))
+    wants, offs = orc.attention_backward(m.g64, m.q64, m.k64, m.v64, unrounded(clean), clean.logsum.double().cpu().numpy(), m.offsets, causal=True, **rounding(dtype))
     near(grads[0][pick], wants[0][others], offs[0][others])
     behind = np.ones(len(q), bool)
     behind[int(m.offsets[1]):bad + 1] = False
@@ -376,7 +402,7 @@ def test_rows_at_odd_places():
             near(got, want, off)
             near(kept.logsum, log, log_off)
             into = tuple(odd(torch.zeros_like(x)) for x in (q, k, v))
-            for a, b in zip(encoder.attention_backward(g, q, k, v, encoder.AttentionSaved(odd(out), saved.logsum), *m.rows(), causal=True, out=into), grads):
+            for a, b in zip(encoder.attention_backward(g, q, k, v, saved._replace(out=odd(out)), *m.rows(), causal=True, out=into), grads):
                 assert torch.equal(a, b)
 
 
@@ -419,7 +445,7 @@ def test_many_short_rows():
         want, log, off, log_off = orc.attention(q64, q64, q64, offsets, **rounding(dtype))
         near(out, want, off)
         near(saved.logsum, log, log_off)
-        wants, offs = orc.attention_backward(g64, q64, q64, q64, out.double().cpu().numpy(), saved.logsum.double().cpu().numpy(), offsets, **rounding(dtype))
+        wants, offs = orc.attention_backward(g64, q64, q64, q64, unrounded(saved), saved.logsum.double().cpu().numpy(), offsets, **rounding(dtype))
         for x, w, o in zip(grads, wants, offs):
             near(x, w, o)
 
@@ -488,6 +514,7 @@ def test_refusals():
         ("scale", lambda: encoder.attention(x, x, x, rows, scale=-0.5)),
         ("256", lambda: encoder.attention(*[torch.zeros(6, 1, 257, device="cuda")] * 3, rows)),
         ("logsum", lambda: encoder.attention_backward(x, x, x, x, encoder.AttentionSaved(x, torch.zeros(6, 4, device="cuda")), rows)),
+        ("rest", lambda: encoder.attention_backward(x, x, x, x, encoder.AttentionSaved(x, torch.zeros(4, 6, device="cuda"), x.to(torch.int8)[:5]), rows)),
         ("grad and out", lambda: encoder.attention_backward(x[:5], x, x, x, encoder.AttentionSaved(x, torch.zeros(4, 6, device="cuda")), rows)),
         ("those of", lambda: encoder.attention_backward(x, x, x, x, encoder.AttentionSaved(x, torch.zeros(4, 6, device="cuda")), rows, out=(x, x, x[:, :2]))),
     ]:

@@ -110,7 +110,7 @@ SHARED = [
 def test_attention_refusals(change, text):
     a = dict(q=h(), k=h(heads=2), v=h(heads=2), rows=2, offsets=AT, key_offsets=None, key_lengths=None, causal=0, scale=1.0, out=h(), logsum=None)
     a.update(change)
-    refused(_capi.load().nvtext_amd_attention(a["q"], a["k"], a["v"], a["rows"], a["offsets"], a["key_offsets"], a["key_lengths"], a["causal"], a["scale"], None, None, a["out"], a["logsum"]), text)
+    refused(_capi.load().nvtext_amd_attention(a["q"], a["k"], a["v"], a["rows"], a["offsets"], a["key_offsets"], a["key_lengths"], a["causal"], a["scale"], None, None, a["out"], a["logsum"], None), text)
 
 
 @pytest.mark.parametrize("change,text", SHARED + [
@@ -121,7 +121,7 @@ def test_attention_refusals(change, text):
 def test_attention_backward_refusals(change, text):
     a = dict(grad=h(), q=h(), k=h(heads=2), v=h(heads=2), out=h(), logsum=AT, rows=2, offsets=AT, key_offsets=None, key_lengths=None, causal=0, scale=1.0, dq=h(), dk=h(heads=2), dv=h(heads=2))
     a.update(change)
-    refused(_capi.load().nvtext_amd_attention_backward(a["grad"], a["q"], a["k"], a["v"], a["out"], a["logsum"], a["rows"], a["offsets"], a["key_offsets"], a["key_lengths"], a["causal"], a["scale"],
+    refused(_capi.load().nvtext_amd_attention_backward(a["grad"], a["q"], a["k"], a["v"], a["out"], a["logsum"], None, a["rows"], a["offsets"], a["key_offsets"], a["key_lengths"], a["causal"], a["scale"],
                                                        None, None, a["dq"], a["dk"], a["dv"]), text)
 
 
@@ -130,9 +130,9 @@ def test_calls_without_values_need_no_gpu():
     none = h(0, data=None)
     assert L.nvtext_amd_rotary(none, 0, None, None, AT, 4, 0, 0, 1.0, None, none) == _capi.SUCCESS
     assert L.nvtext_amd_rotary(h(heads=0), 2, AT, None, AT, 4, 0, 0, 1.0, None, h(heads=0)) == _capi.SUCCESS
-    assert L.nvtext_amd_attention(none, none, none, 0, None, None, None, 0, 1.0, None, None, none, None) == _capi.SUCCESS
-    assert L.nvtext_amd_attention(none, h(), h(), 2, AT, AT, None, 0, 1.0, None, None, none, None) == _capi.SUCCESS
-    assert L.nvtext_amd_attention_backward(none, none, none, none, none, None, 0, None, None, None, 0, 1.0, None, None, none, none, none) == _capi.SUCCESS
+    assert L.nvtext_amd_attention(none, none, none, 0, None, None, None, 0, 1.0, None, None, none, None, None) == _capi.SUCCESS
+    assert L.nvtext_amd_attention(none, h(), h(), 2, AT, AT, None, 0, 1.0, None, None, none, None, None) == _capi.SUCCESS
+    assert L.nvtext_amd_attention_backward(none, none, none, none, none, None, None, 0, None, None, None, 0, 1.0, None, None, none, none, none) == _capi.SUCCESS
 
 
 def test_rotary_frequencies():
