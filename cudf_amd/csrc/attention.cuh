@@ -84,7 +84,7 @@ template <typename T>
 struct Forward : Problem<T> {
   Heads<T> out;
   float* logsum;
-  int8_t* rest;  // [tokens, heads, width], of 16-bit types; or nullptr
+  int8_t* rest;  // [heads, tokens, width], of 16-bit types; or nullptr
 };
 
 // The run that token t is in.
@@ -136,7 +136,7 @@ __device__ void attend_row(Forward<T> const& f, int32_t t, int32_t h)
     if (c * kWave + lane < f.width) {
       float const x                      = seen > 0 ? o[c] / sum : 0.f;
       f.out.at(t, h)[c * kWave + lane] = static_cast<T>(x);
-      if (f.rest) f.rest[(static_cast<int64_t>(t) * f.heads + h) * f.width + c * kWave + lane] = rest_of(x, static_cast<T>(x));
+      if (f.rest) f.rest[(static_cast<int64_t>(h) * f.runs.tokens + t) * f.width + c * kWave + lane] = rest_of(x, static_cast<T>(x));
     }
   if (f.logsum && lane == 0) f.logsum[static_cast<int64_t>(h) * f.runs.tokens + t] = seen > 0 ? (top + __builtin_amdgcn_logf(sum)) * kLn2 : -INFINITY;
 }
@@ -169,7 +169,7 @@ __device__ void query_gradient_row(Backward<T> const& f, int32_t t, int32_t h)
   float delta       = 0.f;
   if (seen > 0 && f.rest) {
     for (int32_t j = 0; j < f.width; ++j)
-      delta = fmaf(static_cast<float>(g[j]), with_rest(f.out.at(t, h)[j], f.rest[(static_cast<int64_t>(t) * f.heads + h) * f.width + j]), delta);
+      delta = fmaf(static_cast<float>(g[j]), with_rest(f.out.at(t, h)[j], f.rest[at * f.width + j]), delta);
   } else if (seen > 0) {
     delta = dot(g, f.out.at(t, h), f.width);
   }
@@ -254,19 +254,21 @@ __device__ __forceinline__ f32x16_t multiply32(Fragment<float> a, Fragment<float
   return c;
 }
 
-// A tile of heads of D values (a multiple of 32) of as many tokens or keys, as it lies in LDS: in units of 32 bytes, whose order is turned with the head's
-// number, so that units of one number of 8 neighbouring heads lie in different banks (the reads of rows), and so does what the reads of columns
-// ask for at once: two neighbouring units of 4 heads, or (32-bit types) 4 units of a head and of the one 4 further on.  What turns them depends on
-// where heads begin within the 256 bytes of all banks.
+// A tile of heads of D values (a multiple of 32) of as many tokens or keys, as it lies in LDS: in pieces of 16 bytes, whose order is turned with the head's
+// number so that what is read at once lies in all of the 256 bytes of LDS's banks: pieces of one number of 16 neighbouring heads (the reads of rows), units
+// of two pieces of 4 neighbouring heads and the units beside them (the transposing reads of columns), 8 pieces of a head and of the one 4 further
+// on (columns of 32-bit types).
 template <typename T, int D>
 struct Tile {
   static constexpr int kHeads = D * sizeof(T) > 512 ? 32 : 64;  // two tiles of each, twice, fill no more than 128 KB
   static constexpr int kLine = D * sizeof(T), kBytes = kHeads * kLine, kPieces = kLine / 16;  // bytes of a head, of all, pieces of 16 bytes of a head
   __device__ __forceinline__ static constexpr uint32_t turn(uint32_t head)
   {
-    if constexpr (kLine % 256 == 0) return sizeof(T) == 2 ? (head & 3) << 1 | (head >> 2 & 1) : head & 7;
-    if constexpr (kLine % 128 == 0) return head & 2 | (head >> 2 & 1);
-    return head >> 2 & 1;
+    uint32_t const last = head >> 3 & 1, third = head >> 2 & 1;
+    if constexpr (sizeof(T) == 4) return third << 3 | (head & 3) << 1 | last;
+    if constexpr (kLine % 256 == 0) return (head & 3) << 2 | third << 1 | last;
+    if constexpr (kLine % 128 == 0) return (head & 2) << 1 | third << 1 | last;  // (neighbouring heads begin 128 bytes apart)
+    return third << 1 | last;                                                   // (they begin 64 bytes apart, in some order)
   }
 };
 
@@ -287,7 +289,7 @@ struct TileLoader {
 #pragma unroll
     for (int p = 0; p < kLoads; ++p) {
       int const slot = (p * WAVES + wave) * kWave + lane, row = slot / Of::kPieces, piece = slot % Of::kPieces;
-      int const from = (static_cast<int>(static_cast<uint32_t>(piece >> 1) ^ Of::turn(row)) << 1) | (piece & 1);
+      int const from = static_cast<int>(static_cast<uint32_t>(piece) ^ Of::turn(row));
       offset[p]      = from * kEach < columns ? row * line + from * 16 : kFar;
     }
   }
@@ -314,37 +316,42 @@ struct TileReader {
     row         = (lane % 32) * kLine;
     turn_row    = Tile<T, D>::turn(lane % 32);
     if constexpr (sizeof(T) == 2) {
-      row += h * 16;
-      int const k = 4 * h + i / 4;
-      column      = k * kLine + i % 4 * 8;
-      turn_column = Tile<T, D>::turn(k) ^ (lane / 16 & 1);
-    } else {
-      column      = 4 * h * kLine + lane % 8 * 4;
-      turn_column = Tile<T, D>::turn(4 * h) ^ (lane / 8 & 3);
       turn_row ^= h;
+      int const k = 4 * h + i / 4;
+      column      = k * kLine + i % 2 * 8;
+      turn_column = Tile<T, D>::turn(k) ^ (lane / 16 % 2 * 2 + i / 2 % 2);
+    } else {
+      turn_row ^= 2 * h;
+      column      = 4 * h * kLine + lane % 4 * 4;
+      turn_column = Tile<T, D>::turn(4 * h) ^ (lane % 32 / 4);
     }
   }
   // 32 heads from 32 * block on, values 16 * step .. 16 * step + 15 of each
   __device__ __forceinline__ Fragment<T> rows(LdsBytes tile, int block, int step) const
   {
-    constexpr int kUnits = 16 * sizeof(T) / 32;
-    LdsBytes const p     = tile + row + (((step * kUnits) ^ turn_row) * 32) + block * (32 * kLine);
-    return *reinterpret_cast<__attribute__((address_space(3))) Fragment<T>*>(p);
+    LdsBytes const p = tile + row + block * (32 * kLine);
+    if constexpr (sizeof(T) == 2) {
+      return *reinterpret_cast<__attribute__((address_space(3))) Fragment<T>*>(p + ((2 * step) ^ turn_row) * 16);
+    } else {
+      f32x4_t const low  = *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(p + ((4 * step) ^ turn_row) * 16);
+      f32x4_t const high = *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(p + ((4 * step + 1) ^ turn_row) * 16);
+      return __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
   }
   // transposed: values 32 * block .. 32 * block + 31 of 16 heads from 16 * step on, in the order of heads that a result of 32 x 32 leaves in its registers
   __device__ __forceinline__ Fragment<T> columns(LdsBytes tile, int block, int step) const
   {
     if constexpr (sizeof(T) == 2) {
-      LdsBytes const p   = tile + column + (((2 * block) ^ turn_column) * 32) + step * (16 * kLine);
-      s16x4_t const low  = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(p));
-      s16x4_t const high = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(p + 8 * kLine));
+      LdsBytes const p   = tile + column + step * (16 * kLine);
+      s16x4_t const low  = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(p + ((4 * block) ^ turn_column) * 16));
+      s16x4_t const high = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(p + ((4 * block + 1) ^ turn_column) * 16 + 8 * kLine));
       return __builtin_bit_cast(Fragment<T>, __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
       Fragment<T> f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        uint32_t const unit = (4 * block) ^ turn_column ^ Tile<T, D>::turn(k % 4);
-        f[k]                = *reinterpret_cast<__attribute__((address_space(3))) T*>(tile + column + unit * 32 + (16 * step + 8 * (k / 4) + k % 4) * kLine);
+        uint32_t const piece = (8 * block) ^ turn_column ^ Tile<T, D>::turn(8 * (k / 4) + k % 4);
+        f[k]                 = *reinterpret_cast<__attribute__((address_space(3))) T*>(tile + column + piece * 16 + (16 * step + 8 * (k / 4) + k % 4) * kLine);
       }
       return f;
     }

@@ -10,25 +10,47 @@ namespace {
 constexpr int kThreads = 256;
 
 // ------------------------------------------------------------------ forward, in tiles
-// The work of a launch: blocks of tokens, of every head.  The heads that share a key head come one after the other on one XCD (workgroups go to
-// the eight XCDs in turn), and so do, where the number of key heads allows, the blocks of a key head: its keys come from that XCD's L2.  The last
+// The work of a launch: blocks of tokens, of every head, in `splits` shares.  The heads that share a key head come one after the other on one XCD (workgroups go
+// to the eight XCDs in turn), and so do, where the number of key heads allows, the blocks of a key head: its keys come from that XCD's L2.  The last
 // blocks come first: of a long row they are those with the most keys to see.
 struct Work {
   int64_t block;
-  int32_t kv_head, head;
+  int32_t kv_head, head, share;
 };
 constexpr int kXcds = 8;
-inline int64_t work_items(int64_t blocks, int32_t kv_heads, int32_t each) { return (blocks * kv_heads + kXcds - 1) / kXcds * kXcds * each; }
+inline int64_t work_items(int64_t blocks, int32_t kv_heads, int32_t each, int32_t splits) { return (blocks * kv_heads + kXcds - 1) / kXcds * kXcds * each * splits; }
 // false: nothing to do
-__device__ __forceinline__ bool work_of(int64_t item, int64_t blocks, int32_t kv_heads, int32_t each, Work& w)
+template <typename Int>
+__device__ __forceinline__ bool work_in(Int item, Int blocks, int32_t kv_heads, int32_t each, int32_t splits, Work& w)
 {
-  int64_t const n = item / kXcds, unit = n / each * kXcds + item % kXcds;
-  if (unit >= blocks * kv_heads) return false;
-  w.block   = blocks - 1 - unit / kv_heads;
-  w.kv_head = static_cast<int32_t>(unit % kv_heads);
-  w.head    = w.kv_head * each + static_cast<int32_t>(n % each);
+  Int const n = item / kXcds / static_cast<Int>(splits), units = n / static_cast<Int>(each), unit = units * kXcds + item % kXcds;
+  if (unit >= blocks * static_cast<Int>(kv_heads)) return false;
+  Int const behind = unit / static_cast<Int>(kv_heads);
+  w.block          = static_cast<int64_t>(blocks - 1 - behind);
+  w.kv_head        = static_cast<int32_t>(unit - behind * static_cast<Int>(kv_heads));
+  w.head           = w.kv_head * each + static_cast<int32_t>(n - units * static_cast<Int>(each));
+  w.share          = static_cast<int32_t>(item / kXcds - n * static_cast<Int>(splits));
   return true;
 }
+__device__ __forceinline__ bool work_of(int64_t item, int64_t blocks, int32_t kv_heads, int32_t each, int32_t splits, Work& w)
+{
+  // (divisions of 64 bits take a hundred instructions each)
+  if (blocks * kv_heads < (int64_t{1} << 32) - kXcds && item < int64_t{1} << 32) return work_in<uint32_t>(item, blocks, kv_heads, each, splits, w);
+  return work_in<uint64_t>(item, blocks, kv_heads, each, splits, w);
+}
+
+// Where there are few workgroups, each one's tiles are shared by up to `splits`, which leave what they add up in memory, [block][head][share][row][D] in
+// float32, for another launch to join.  A share has at least kLeastTiles: in how many shares `tiles` go, and what one of them has.
+constexpr int kLeastTiles = 2;
+__device__ __forceinline__ int32_t shares_of(int32_t tiles, int32_t splits) { return splits == 1 || tiles < 2 * kLeastTiles ? 1 : min(splits, tiles / kLeastTiles); }
+__device__ __forceinline__ int32_t share_begin(int32_t tiles, int32_t share, int32_t shares) { return static_cast<int32_t>(static_cast<int64_t>(tiles) * share / shares); }
+
+struct Split {
+  int32_t splits;
+  float* sums;
+  float2* tops;  // (forward) [block][head][share][row]: top, and the sum of the exponentials
+  __device__ __forceinline__ int64_t slot(int64_t block, int32_t head, int32_t heads, int32_t share) const { return (block * heads + head) * splits + share; }
+};
 
 template <typename T, int D, int WAVES, int NQ>
 struct ForwardShape {
@@ -141,7 +163,7 @@ struct Attending {
     if (there && !(odd >> column & 1)) {
       store_columns<T, kColumns>(f.out.at(t, h), o[n], half, f.width);
       if constexpr (sizeof(T) == 2)
-        if (f.rest) store_rests<T, kColumns>(f.rest + (t * f.heads + h) * f.width, o[n], half, f.width);
+        if (f.rest) store_rests<T, kColumns>(f.rest + (static_cast<int64_t>(h) * f.runs.tokens + t) * f.width, o[n], half, f.width);
       if (f.logsum && half == 0) f.logsum[static_cast<int64_t>(h) * f.runs.tokens + t] = seen[n] > 0 ? (top[n] + __builtin_amdgcn_logf(total)) * kLn2 : -INFINITY;
     }
     return static_cast<uint32_t>(odd);
@@ -150,7 +172,7 @@ struct Attending {
 
 // A workgroup has kTokens tokens of a head, a wavefront 32 * NQ of them.  Keys come through LDS, 64 at a time, the next ones while these are multiplied.
 template <typename T, int D, int WAVES, int NQ>
-__global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES, NQ>::kWavesASimd)) attend_tiles_kernel(Forward<T> f)
+__global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES, NQ>::kWavesASimd)) attend_tiles_kernel(Forward<T> f, Split split)
 {
   using Shape = ForwardShape<T, D, WAVES, NQ>;
   extern __shared__ __align__(16) char lds_[];
@@ -158,7 +180,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES, NQ>:
   constexpr int kTile = Shape::kTile;
   Work w;
   int32_t const each = f.heads / f.kv_heads;
-  if (!work_of(block_number(), f.runs.blocks(Shape::kShift), f.kv_heads, each, w)) return;
+  if (!work_of(block_number(), f.runs.blocks(Shape::kShift), f.kv_heads, each, split.splits, w)) return;
   int32_t const run   = f.runs.run_of(w.block, Shape::kShift);
   int32_t const begin = uniform(f.runs.begin(run)), tokens = uniform(f.runs.begin(run + 1)) - begin;
   int64_t const in_run = (w.block - f.runs.first_block(run, Shape::kShift)) << Shape::kShift;
@@ -175,6 +197,10 @@ __global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES, NQ>:
   int32_t const least = uniform(wave0 < rest ? f.seen(block0 + wave0, tokens, keys) : 0), most = uniform(wave0 < rest ? f.seen(block0 + wave1 - 1, tokens, keys) : 0);
   int64_t const t0    = static_cast<int64_t>(begin) + block0 + wave0;
 
+  int32_t const all_tiles = (all + kTile - 1) / kTile, shares = shares_of(all_tiles, split.splits);
+  if (w.share >= shares) return;
+  int32_t const from = uniform(share_begin(all_tiles, w.share, shares)), tiles = uniform(share_begin(all_tiles, w.share + 1, shares));
+
   Attending<T, D, NQ> a;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
@@ -184,16 +210,15 @@ __global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES, NQ>:
     a.begin(n, f.q.at(there ? t0 + i : begin, w.head), f.width, there, half);
   }
   TileLoader<T, D, WAVES> load_k, load_v;
-  load_k.aim(f.k, first, w.kv_head, f.width, wave, lane);
-  load_v.aim(f.v, first, w.kv_head, f.width, wave, lane);
+  load_k.aim(f.k, first + from * kTile, w.kv_head, f.width, wave, lane);
+  load_v.aim(f.v, first + from * kTile, w.kv_head, f.width, wave, lane);
   TileReader<T, D> const read(lane);
-  float const scale   = f.scale * kLog2e;
-  int32_t const tiles = (all + kTile - 1) / kTile;
-  if (tiles > 0) {
-    load_k.load(lds, keys, wave);
-    load_v.load(lds + Tile<T, D>::kBytes, keys, wave);
+  float const scale = f.scale * kLog2e;
+  if (tiles > from) {
+    load_k.load(lds + (from & 1) * 2 * Tile<T, D>::kBytes, keys - from * kTile, wave);
+    load_v.load(lds + (from & 1) * 2 * Tile<T, D>::kBytes + Tile<T, D>::kBytes, keys - from * kTile, wave);
   }
-  for (int32_t tile = 0; tile < tiles; ++tile) {
+  for (int32_t tile = from; tile < tiles; ++tile) {
     LdsBytes const k_tile = lds + (tile & 1) * 2 * Tile<T, D>::kBytes;
     stage_barrier<0>();
     if (tile + 1 < tiles) {
@@ -205,6 +230,18 @@ __global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES, NQ>:
     if (key0 < most) a.pass(k_tile, k_tile + Tile<T, D>::kBytes, read, key0, key0 + kTile > least, scale, half);
   }
   if (wave0 >= rest) return;
+  if (shares > 1) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      int64_t const part = split.slot(w.block, w.head, f.heads, w.share) * Shape::kTokens + wave0 + n * 32 + column;
+      Halves const both  = halves(a.sum[n]);
+      if (wave0 + n * 32 + column < rest) {
+        store_columns<float, D / 32>(split.sums + part * D, a.o[n], half, D);
+        if (half == 0) split.tops[part] = make_float2(a.top[n], both.low + both.high);
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     uint32_t odd = a.finish(n, f, t0 + n * 32 + column, w.head, wave0 + n * 32 + column < rest, half, column);
@@ -242,7 +279,7 @@ __global__ void __launch_bounds__(kWave, 1) attend_chunks_kernel(ForwardChunks<T
   LdsBytes const lds  = (LdsBytes)lds_;
   constexpr int kTile = Tile<T, D>::kHeads;
   Work w;
-  if (!work_of(block_number(), f.key_runs.blocks(f.shift), f.kv_heads, 1, w)) return;
+  if (!work_of(block_number(), f.key_runs.blocks(f.shift), f.kv_heads, 1, 1, w)) return;
   int32_t const run = f.key_runs.run_of(w.block, f.shift), each = f.heads / f.kv_heads;
   int32_t first = 0, keys = 0;
   if (f.is_row(run)) f.keys_of(run, first, keys);
@@ -303,15 +340,51 @@ __global__ void __launch_bounds__(kWave, 1) attend_chunks_kernel(ForwardChunks<T
   }
 }
 
+// A wavefront's share of a row of D values.
+template <int D>
+using Some = float __attribute__((ext_vector_type(D / kWave)));
+
+template <int D>
+__device__ __forceinline__ void add_part(Some<D>& sum, float& total, float top, float2 of, const float* part)
+{
+  float const weight = of.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(of.x - top);
+  total += of.y * weight;
+  sum += *reinterpret_cast<const Some<D>*>(part + lane_id() * (D / kWave)) * weight;
+}
+
+// What Attending::finish does, for sums that a wavefront holds side by side.
+template <typename T, int D>
+__device__ __forceinline__ void finish_row(Forward<T> const& f, int32_t t, int32_t head, int32_t seen, Some<D> sum, float total, float top)
+{
+  constexpr int kEach = D / kWave;
+  int const lane      = lane_id();
+  bool finite         = true;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    sum[k] = seen > 0 ? sum[k] / total : 0.f;
+    finite = finite && (lane * kEach + k >= f.width || fabsf(sum[k]) < INFINITY);
+  }
+  if (seen > 0 && __ballot(!finite)) {
+    attend_row(f, t, head);
+    return;
+  }
+  T* const out = f.out.at(t, head);
+#pragma unroll
+  for (int k = 0; k < kEach; ++k)
+    if (lane * kEach + k < f.width) {
+      out[lane * kEach + k] = static_cast<T>(sum[k]);
+      if (f.rest) f.rest[(static_cast<int64_t>(head) * f.runs.tokens + t) * f.width + lane * kEach + k] = rest_of(sum[k], static_cast<T>(sum[k]));
+    }
+  if (f.logsum && lane == 0) f.logsum[static_cast<int64_t>(head) * f.runs.tokens + t] = seen > 0 ? (top + __builtin_amdgcn_logf(total)) * kLn2 : -INFINITY;
+}
+
 // Joins the parts of a head of a token, a workgroup for each: its wavefronts take every fourth part.
 constexpr int kJoinWaves = 4;
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinWaves * kWave) attend_join_kernel(ForwardChunks<T> f)
 {
-  constexpr int kEach = D / kWave;
-  typedef float Some __attribute__((ext_vector_type(kEach)));
   __shared__ float tops[kJoinWaves], totals[kJoinWaves];
-  __shared__ Some sums[kJoinWaves][kWave];
+  __shared__ Some<D> sums[kJoinWaves][kWave];
   int64_t const item = block_number();
   if (item >= static_cast<int64_t>(f.runs.tokens) * f.heads) return;
   int32_t const t = static_cast<int32_t>(item / f.heads), head = static_cast<int32_t>(item % f.heads), run = run_with(f.runs, t);
@@ -331,15 +404,9 @@ __global__ void __launch_bounds__(kJoinWaves * kWave) attend_join_kernel(Forward
 #pragma unroll
   for (int w = 0; w < kJoinWaves; ++w) top = fmaxf(top, tops[w]);
   float total = 0.f;
-  Some sum{};
+  Some<D> sum{};
 #pragma unroll 8
-  for (int32_t c = wave; c < chunks; c += kJoinWaves) {
-    float2 const of     = f.tops[at + c * step];
-    float const weight  = of.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(of.x - top);
-    Some const part     = *reinterpret_cast<const Some*>(f.sums + (at + c * step) * D + lane * kEach);
-    total += of.y * weight;
-    sum += part * weight;
-  }
+  for (int32_t c = wave; c < chunks; c += kJoinWaves) add_part<D>(sum, total, top, f.tops[at + c * step], f.sums + (at + c * step) * D);
   sums[wave][lane] = sum;
   if (lane == 0) totals[wave] = total;
   __syncthreads();
@@ -349,25 +416,31 @@ __global__ void __launch_bounds__(kJoinWaves * kWave) attend_join_kernel(Forward
     total += totals[w];
     sum += sums[w][lane];
   }
-  int32_t const seen = f.seen(t - begin, tokens, keys);
-  bool finite        = true;
-#pragma unroll
-  for (int k = 0; k < kEach; ++k) {
-    sum[k] = seen > 0 ? sum[k] / total : 0.f;
-    finite = finite && fabsf(sum[k]) < INFINITY;
-  }
-  if (seen > 0 && __ballot(!finite)) {  // (as in finish)
-    attend_row(f, t, head);
-    return;
-  }
-  T* const out = f.out.at(t, head);
-#pragma unroll
-  for (int k = 0; k < kEach; ++k)
-    if (lane * kEach + k < f.width) {
-      out[lane * kEach + k] = static_cast<T>(sum[k]);
-      if (f.rest) f.rest[item * f.width + lane * kEach + k] = rest_of(sum[k], static_cast<T>(sum[k]));
-    }
-  if (f.logsum && lane == 0) f.logsum[static_cast<int64_t>(head) * f.runs.tokens + t] = seen > 0 ? (top + __builtin_amdgcn_logf(total)) * kLn2 : -INFINITY;
+  finish_row<T, D>(f, t, head, f.seen(t - begin, tokens, keys), sum, total, top);
+}
+
+// The same for the shares of a block of 2^shift tokens, a wavefront for each head of a token.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) attend_join_shares_kernel(Forward<T> f, Split split, int shift)
+{
+  constexpr int kTile = Tile<T, D>::kHeads;
+  int64_t const item = block_number() * (kThreads / kWave) + threadIdx.x / kWave;
+  if (item >= static_cast<int64_t>(f.runs.tokens) * f.heads) return;
+  int32_t const t = static_cast<int32_t>(item / f.heads), head = static_cast<int32_t>(item % f.heads), run = run_with(f.runs, t);
+  if (!f.is_row(run)) return;
+  int32_t first, keys;
+  f.keys_of(run, first, keys);
+  int32_t const begin = f.runs.begin(run), tokens = f.runs.begin(run + 1) - begin, i = t - begin, last = i | ((1 << shift) - 1);
+  int32_t const all = f.seen(last < tokens ? last : tokens - 1, tokens, keys), shares = shares_of((all + kTile - 1) / kTile, split.splits);
+  if (shares < 2) return;
+  int64_t const at = (split.slot(f.runs.first_block(run, shift) + (i >> shift), head, f.heads, 0) << shift) + (i & ((1 << shift) - 1));
+  float top = -INFINITY;
+  for (int32_t c = 0; c < shares; ++c) top = fmaxf(top, split.tops[at + (static_cast<int64_t>(c) << shift)].x);
+  Some<D> sum{};
+  float total = 0.f;
+#pragma unroll 4
+  for (int32_t c = 0; c < shares; ++c) add_part<D>(sum, total, top, split.tops[at + (static_cast<int64_t>(c) << shift)], split.sums + (at + (static_cast<int64_t>(c) << shift)) * D);
+  finish_row<T, D>(f, t, head, f.seen(i, tokens, keys), sum, total, top);
 }
 
 // ------------------------------------------------------------------ the gradients, in tiles
@@ -376,12 +449,11 @@ __global__ void __launch_bounds__(kJoinWaves * kWave) attend_join_kernel(Forward
 template <typename T, int D, int WAVES>
 struct GradientShape {
   static constexpr int kRows = 32 * WAVES, kShift = __builtin_ctz(kRows), kTile = Tile<T, D>::kHeads, kStage = 2 * Tile<T, D>::kBytes, kLds = 2 * kStage, kWavesASimd = D * sizeof(T) <= 256 ? 2 : 1;
-  static constexpr int kKeyStage = kStage + 2 * kWave * 4, kKeyLds = 2 * kKeyStage;  // (with logs and deltas)
 };
 
 // The gradient of q: as forward, a lane has a token's scores, and what they are multiplied with comes from LDS, keys as they lie and transposed.
 template <typename T, int D, int WAVES>
-__global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kWavesASimd)) query_gradient_tiles_kernel(Backward<T> f)
+__global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kWavesASimd)) query_gradient_tiles_kernel(Backward<T> f, Split split)
 {
   using Shape = GradientShape<T, D, WAVES>;
   extern __shared__ __align__(16) char lds_[];
@@ -389,7 +461,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
   constexpr int kSteps = D / 16, kColumns = D / 32, kTile = Shape::kTile, kBlocks = kTile / 32;
   Work w;
   int32_t const each = f.heads / f.kv_heads;
-  if (!work_of(block_number(), f.runs.blocks(Shape::kShift), f.kv_heads, each, w)) return;
+  if (!work_of(block_number(), f.runs.blocks(Shape::kShift), f.kv_heads, each, split.splits, w)) return;
   int32_t const run    = f.runs.run_of(w.block, Shape::kShift);
   int32_t const begin  = uniform(f.runs.begin(run)), tokens = uniform(f.runs.begin(run + 1)) - begin;
   int64_t const in_run = (w.block - f.runs.first_block(run, Shape::kShift)) << Shape::kShift;
@@ -403,6 +475,9 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
   int32_t const wave0 = wave * 32, wave1 = wave0 + 32 < rest ? wave0 + 32 : rest;
   int32_t const all   = uniform(f.seen(block0 + (rest < Shape::kRows ? rest : Shape::kRows) - 1, tokens, keys));
   int32_t const least = uniform(wave0 < rest ? f.seen(block0 + wave0, tokens, keys) : 0), most = uniform(wave0 < rest ? f.seen(block0 + wave1 - 1, tokens, keys) : 0);
+  int32_t const all_tiles = (all + kTile - 1) / kTile, shares = shares_of(all_tiles, split.splits);
+  if (w.share >= shares) return;
+  int32_t const first_tile = uniform(share_begin(all_tiles, w.share, shares)), tiles = uniform(share_begin(all_tiles, w.share + 1, shares));
   bool const there    = wave0 + column < rest;
   int64_t const t     = static_cast<int64_t>(begin) + block0 + (there ? wave0 + column : 0), at = static_cast<int64_t>(w.head) * f.runs.tokens + t;
   int32_t const seen  = there ? f.seen(block0 + wave0 + column, tokens, keys) : 0;
@@ -417,7 +492,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
     bool rests = false;
     if constexpr (sizeof(T) == 2) rests = f.rest != nullptr;
     if (rests) {
-      auto const rest = load_raw8(f.rest + (t * f.heads + w.head) * f.width + 16 * s + 8 * half, there ? f.width - 16 * s - 8 * half : 0);
+      auto const rest = load_raw8(f.rest + at * f.width + 16 * s + 8 * half, there ? f.width - 16 * s - 8 * half : 0);
 #pragma unroll
       for (int k = 0; k < 8; ++k) delta = fmaf(static_cast<float>(g[s][k]), with_rest(out[k], rest[k]), delta);
     } else {
@@ -428,24 +503,23 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
   Halves const both = halves(delta);
   delta             = seen > 0 ? both.low + both.high : 0.f;
   float const log   = there ? f.logsum[at] * kLog2e : 0.f;
-  if (there && half == 0) {
+  if (there && half == 0 && w.share == 0) {
     f.deltas[at] = delta;
     f.logs[at]   = log;
   }
   TileLoader<T, D, WAVES> load_k, load_v;
-  load_k.aim(f.k, first, w.kv_head, f.width, wave, lane);
-  load_v.aim(f.v, first, w.kv_head, f.width, wave, lane);
+  load_k.aim(f.k, first + first_tile * kTile, w.kv_head, f.width, wave, lane);
+  load_v.aim(f.v, first + first_tile * kTile, w.kv_head, f.width, wave, lane);
   TileReader<T, D> const read(lane);
   float const scale = f.scale * kLog2e;
   f32x16_t d[kColumns];
 #pragma unroll
   for (int c = 0; c < kColumns; ++c) d[c] = f32x16_t{};
-  int32_t const tiles = (all + kTile - 1) / kTile;
-  if (tiles > 0) {
-    load_k.load(lds, keys, wave);
-    load_v.load(lds + Tile<T, D>::kBytes, keys, wave);
+  if (tiles > first_tile) {
+    load_k.load(lds + (first_tile & 1) * Shape::kStage, keys - first_tile * kTile, wave);
+    load_v.load(lds + (first_tile & 1) * Shape::kStage + Tile<T, D>::kBytes, keys - first_tile * kTile, wave);
   }
-  for (int32_t tile = 0; tile < tiles; ++tile) {
+  for (int32_t tile = first_tile; tile < tiles; ++tile) {
     LdsBytes const k_tile = lds + (tile & 1) * Shape::kStage, v_tile = k_tile + Tile<T, D>::kBytes;
     stage_barrier<0>();
     if (tile + 1 < tiles) {
@@ -477,6 +551,10 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
     }
   }
   if (wave0 >= rest) return;
+  if (shares > 1) {
+    if (there) store_columns<float, kColumns>(split.sums + (split.slot(w.block, w.head, f.heads, w.share) * Shape::kRows + wave0 + column) * D, d, half, D);
+    return;
+  }
   bool finite = true;
 #pragma unroll
   for (int c = 0; c < kColumns; ++c)
@@ -496,20 +574,26 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
   }
 }
 
-// The gradients of k and v: a wavefront has 32 keys in its registers, a lane a key's scores, and the tokens of all heads that see them come through LDS
+// The gradients of k and v: a wavefront has 32 * NK keys in its registers, a lane a key's scores, and the tokens of all heads that see them come through LDS
 // with their gradients, 64 at a time, with their logs and deltas.
+template <typename T, int D, int WAVES, int NK>
+struct KeyShape {
+  static constexpr int kRows = 32 * WAVES * NK, kShift = __builtin_ctz(kRows), kTile = Tile<T, D>::kHeads, kTiles = 2 * Tile<T, D>::kBytes;
+  static constexpr int kStage = kTiles + 2 * kWave * 4, kLds = 2 * kStage;  // (with logs and deltas)
+  static constexpr int kWavesASimd = D * sizeof(T) * NK <= 256 ? 2 : 1;
+};
 // PART: the gradients of both, or of k or v alone (of wide heads there are not the registers for both).
 enum Part { kBoth, kOfK, kOfV };
-template <typename T, int D, int WAVES, Part PART>
-__global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kWavesASimd)) key_gradient_tiles_kernel(Backward<T> f)
+template <typename T, int D, int WAVES, int NK, Part PART>
+__global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES, NK>::kWavesASimd)) key_gradient_tiles_kernel(Backward<T> f, Split split)
 {
-  using Shape = GradientShape<T, D, WAVES>;
+  using Shape = KeyShape<T, D, WAVES, NK>;
   extern __shared__ __align__(16) char lds_[];
   LdsBytes const lds = (LdsBytes)lds_;
   constexpr bool kK = PART != kOfV, kV = PART != kOfK;
   constexpr int kSteps = D / 16, kColumns = D / 32, kTile = Shape::kTile, kBlocks = kTile / 32;
   Work w;
-  if (!work_of(block_number(), f.key_runs.blocks(Shape::kShift), f.kv_heads, 1, w)) return;
+  if (!work_of(block_number(), f.key_runs.blocks(Shape::kShift), f.kv_heads, 1, split.splits, w)) return;
   w.block              = f.key_runs.blocks(Shape::kShift) - 1 - w.block;  // (of a long row, the first keys are those that most tokens see)
   int32_t const run    = f.key_runs.run_of(w.block, Shape::kShift), each = f.heads / f.kv_heads;
   int32_t const first  = uniform(f.key_runs.begin(run)), places = uniform(f.key_runs.begin(run + 1)) - first;
@@ -526,71 +610,93 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
   begin  = uniform(begin);
   tokens = uniform(tokens > 0 ? tokens : 0);
   keys   = uniform(keys);
-  int32_t const wave0 = wave * 32;
-  bool const there    = wave0 + column < rest;
-  int32_t const key   = block0 + wave0 + column;
-  int64_t const t     = static_cast<int64_t>(first) + (there ? key : block0);
+  int32_t const wave0 = wave * 32 * NK;
   // the first token that sees a key, of the row's
   auto const from_of = [&](int32_t j) {
     int64_t const i = f.causal ? static_cast<int64_t>(j) + tokens - keys : 0;
     return static_cast<int32_t>(i < 0 ? 0 : i < tokens ? i : tokens);
   };
-  int32_t const from = from_of(key), start = uniform(block0 < keys ? from_of(block0) / kTile : 0), tiles = uniform(block0 < keys ? (tokens + kTile - 1) / kTile : 0);
-  int32_t const last_from = uniform(from_of(block0 + wave0 + 31)), first_from = uniform(from_of(block0 + wave0));
+  int32_t const start = uniform(block0 < keys ? from_of(block0) / kTile : 0), tiles = uniform(block0 < keys ? (tokens + kTile - 1) / kTile : 0);
+  // The tiles of one head after another are one stream of loads, of which this is a share.
+  int32_t const of_head = tiles - start > 0 ? tiles - start : 0, total = of_head * each, shares = shares_of(total, split.splits);
+  if (w.share >= shares) return;
+  int32_t const begin_tile = uniform(share_begin(total, w.share, shares)), end_tile = uniform(share_begin(total, w.share + 1, shares));
+  int32_t const last_from = uniform(from_of(block0 + wave0 + 32 * NK - 1)), first_from = uniform(from_of(block0 + wave0));
 
-  Fragment<T> k[kSteps], v[kK ? kSteps : 1];
+  Fragment<T> k[NK][kSteps], v[NK][kK ? kSteps : 1];
+  int32_t from[NK];
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    k[s] = fragment_of(f.k.at(t, w.kv_head), 16 * s + 8 * half, f.width, there && key < keys);
-    if constexpr (kK) v[s] = fragment_of(f.v.at(t, w.kv_head), 16 * s + 8 * half, f.width, there && key < keys);
+  for (int n = 0; n < NK; ++n) {
+    int32_t const i  = wave0 + 32 * n + column, key = block0 + i;
+    bool const there = i < rest && key < keys;
+    int64_t const t  = static_cast<int64_t>(first) + (there ? key : block0);
+    from[n]          = from_of(key);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      k[n][s] = fragment_of(f.k.at(t, w.kv_head), 16 * s + 8 * half, f.width, there);
+      if constexpr (kK) v[n][s] = fragment_of(f.v.at(t, w.kv_head), 16 * s + 8 * half, f.width, there);
+    }
   }
   TileReader<T, D> const read(lane);
   float const scale = f.scale * kLog2e;
-  f32x16_t dk[kK ? kColumns : 1], dv[kV ? kColumns : 1];
+  f32x16_t dk[NK][kK ? kColumns : 1], dv[NK][kV ? kColumns : 1];
 #pragma unroll
-  for (int c = 0; c < kColumns; ++c) {
-    if constexpr (kK) dk[c] = f32x16_t{};
-    if constexpr (kV) dv[c] = f32x16_t{};
-  }
-  // The tiles of one head after another are one stream of loads.
-  int32_t const of_head = tiles - start > 0 ? tiles - start : 0, total = of_head * each;
+  for (int n = 0; n < NK; ++n)
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) {
+      if constexpr (kK) dk[n][c] = f32x16_t{};
+      if constexpr (kV) dv[n][c] = f32x16_t{};
+    }
   TileLoader<T, D, WAVES> load_q, load_g;
-  int32_t loaded = 0, next_head = w.kv_head * each;  // the tile of the head that is loaded next
+  int32_t loaded = uniform(of_head > 0 ? begin_tile % of_head : 0), next_head = uniform(w.kv_head * each + (of_head > 0 ? begin_tile / of_head : 0));  // the tile of the head that is loaded next
+  bool aimed = false;
   auto const load = [&](LdsBytes to) {
-    if (loaded == 0) {
-      load_q.aim(f.q, begin + start * kTile, next_head, f.width, wave, lane);
-      load_g.aim(f.grad, begin + start * kTile, next_head, f.width, wave, lane);
+    if (loaded == 0 || !aimed) {
+      load_q.aim(f.q, begin + (start + loaded) * kTile, next_head, f.width, wave, lane);
+      load_g.aim(f.grad, begin + (start + loaded) * kTile, next_head, f.width, wave, lane);
+      aimed = true;
     }
     int32_t const token = (start + loaded) * kTile, here = tokens - token;
     load_q.load(to, here, wave);
     load_g.load(to + Tile<T, D>::kBytes, here, wave);
     int64_t const at = static_cast<int64_t>(next_head) * f.runs.tokens + begin + token;
     uint32_t const range = static_cast<uint32_t>(here < kTile ? here : kTile) * 4;
-    if (wave == 0) load_words_to_lds(reinterpret_cast<const char*>(f.logs + at), range, to + Shape::kStage, lane * 4);
-    if (wave == WAVES - 1) load_words_to_lds(reinterpret_cast<const char*>(f.deltas + at), range, to + Shape::kStage + kWave * 4, lane * 4);
+    if (wave == 0) load_words_to_lds(reinterpret_cast<const char*>(f.logs + at), range, to + Shape::kTiles, lane * 4);
+    if (wave == WAVES - 1) load_words_to_lds(reinterpret_cast<const char*>(f.deltas + at), range, to + Shape::kTiles + kWave * 4, lane * 4);
     if (++loaded == of_head) {
       loaded = 0;
       ++next_head;
     }
   };
-  if (total > 0) load(lds);
-  int32_t tile = start - 1;
-  for (int32_t n = 0; n < total; ++n) {
-    LdsBytes const q_tile = lds + (n & 1) * Shape::kKeyStage, g_tile = q_tile + Tile<T, D>::kBytes, words = q_tile + Shape::kStage + 16 * half;
+  int32_t tile = start + loaded - 1;
+  if (end_tile > begin_tile) load(lds + (begin_tile & 1) * Shape::kStage);
+  for (int32_t n = begin_tile; n < end_tile; ++n) {
+    LdsBytes const q_tile = lds + (n & 1) * Shape::kStage, g_tile = q_tile + Tile<T, D>::kBytes, words = q_tile + Shape::kTiles + 16 * half;
     stage_barrier<0>();
-    if (n + 1 < total) load(lds + (~n & 1) * Shape::kKeyStage);
+    if (n + 1 < end_tile) load(lds + (~n & 1) * Shape::kStage);
     if (++tile == tiles) tile = start;
     int32_t const token0 = tile * kTile;
     if (token0 + kTile <= first_from) continue;
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
-      f32x16_t s{}, p{};
+      f32x16_t s[NK], p[NK];
 #pragma unroll
-      for (int step = 0; step < kSteps; ++step) s = multiply32(read.rows(q_tile, b, step), k[step], s);
+      for (int n = 0; n < NK; ++n) s[n] = p[n] = f32x16_t{};
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step) {
+        Fragment<T> const q = read.rows(q_tile, b, step);
+#pragma unroll
+        for (int n = 0; n < NK; ++n) s[n] = multiply32(q, k[n][step], s[n]);
+      }
       if constexpr (kK) {
 #pragma unroll
-        for (int step = 0; step < kSteps; ++step) p = multiply32(read.rows(g_tile, b, step), v[step], p);
+        for (int step = 0; step < kSteps; ++step) {
+          Fragment<T> const g = read.rows(g_tile, b, step);
+#pragma unroll
+          for (int n = 0; n < NK; ++n) p[n] = multiply32(g, v[n][step], p[n]);
+        }
       }
+      __builtin_amdgcn_sched_barrier(0);
       int32_t const row0 = token0 + 32 * b;
       bool const partly  = row0 < last_from || row0 + 32 > tokens;
 #pragma unroll
@@ -598,65 +704,159 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
         f32x4_t const log   = *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(words + 128 * b + 32 * i);
         f32x4_t const delta = *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(words + kWave * 4 + 128 * b + 32 * i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          int const r = 4 * i + e;
-          s[r]        = __builtin_amdgcn_exp2f(fmaf(s[r], scale, -log[e]));
-          p[r]        = s[r] * (p[r] - delta[e]);
-        }
+        for (int n = 0; n < NK; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            int const r = 4 * i + e;
+            s[n][r]     = __builtin_amdgcn_exp2f(fmaf(s[n][r], scale, -log[e]));
+            p[n][r]     = s[n][r] * (p[n][r] - delta[e]);
+          }
       }
       if (partly) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          int32_t const i = row0 + 8 * (r / 4) + 4 * half + r % 4;
-          bool const sees = i >= from && i < tokens;
-          s[r]            = sees ? s[r] : 0.f;
-          p[r]            = sees ? p[r] : 0.f;
-        }
+        for (int n = 0; n < NK; ++n)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            int32_t const i = row0 + 8 * (r / 4) + 4 * half + r % 4;
+            bool const sees = i >= from[n] && i < tokens;
+            s[n][r]         = sees ? s[n][r] : 0.f;
+            p[n][r]         = sees ? p[n][r] : 0.f;
+          }
       }
 #pragma unroll
       for (int step = 0; step < 2; ++step) {
-        Fragment<T> const weight = rounded<T>(s, step), ds = rounded<T>(p, step);
-        if constexpr (kV) {
+        Fragment<T> weight[NK], ds[NK];
 #pragma unroll
-          for (int c = 0; c < kColumns; ++c) dv[c] = multiply32(read.columns(g_tile, c, 2 * b + step), weight, dv[c]);
+        for (int n = 0; n < NK; ++n) {
+          weight[n] = rounded<T>(s[n], step);
+          ds[n]     = rounded<T>(p[n], step);
         }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c) {
+          if constexpr (kV) {
+            Fragment<T> const g = read.columns(g_tile, c, 2 * b + step);
+#pragma unroll
+            for (int n = 0; n < NK; ++n) dv[n][c] = multiply32(g, weight[n], dv[n][c]);
+          }
+          if constexpr (kK) {
+            Fragment<T> const q = read.columns(q_tile, c, 2 * b + step);
+#pragma unroll
+            for (int n = 0; n < NK; ++n) dk[n][c] = multiply32(q, ds[n], dk[n][c]);
+          }
+        }
+      }
+    }
+  }
+  if (shares > 1) {
+#pragma unroll
+    for (int n = 0; n < NK; ++n) {
+      int32_t const i = wave0 + 32 * n + column;
+      float* const part = split.sums + (split.slot(w.block, w.kv_head, f.kv_heads, w.share) * Shape::kRows + i) * (2 * D);
+      if (i >= rest) continue;
+      if constexpr (kK) store_columns<float, kColumns>(part, dk[n], half, D);
+      if constexpr (kV) store_columns<float, kColumns>(part + D, dv[n], half, D);
+      if (block0 + i >= keys && w.share == 0) {  // (which is no key: nothing is joined for it)
+        f32x16_t const zeros[kColumns] = {};
+        int64_t const t                = static_cast<int64_t>(first) + block0 + i;
+        if constexpr (kK) store_columns<T, kColumns>(f.k_grad.at(t, w.kv_head), zeros, half, f.width);
+        if constexpr (kV) store_columns<T, kColumns>(f.v_grad.at(t, w.kv_head), zeros, half, f.width);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int n = 0; n < NK; ++n) {
+    int32_t const i  = wave0 + 32 * n + column, key = block0 + i;
+    bool const there = i < rest;
+    int64_t const t  = static_cast<int64_t>(first) + (there ? key : block0);
+    bool finite      = true;
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
         if constexpr (kK) {
-#pragma unroll
-          for (int c = 0; c < kColumns; ++c) dk[c] = multiply32(read.columns(q_tile, c, 2 * b + step), ds, dk[c]);
+          dk[n][c][r] = key < keys ? dk[n][c][r] * f.scale : 0.f;
+          finite      = finite && fabsf(dk[n][c][r]) < INFINITY;
+        }
+        if constexpr (kV) {
+          dv[n][c][r] = key < keys ? dv[n][c][r] : 0.f;
+          finite      = finite && fabsf(dv[n][c][r]) < INFINITY;
         }
       }
+    uint64_t odd = __ballot(there && !finite);
+    odd          = (odd | odd >> 32) & 0xffffffffu;
+    if (there && !(odd >> column & 1)) {
+      if constexpr (kK) store_columns<T, kColumns>(f.k_grad.at(t, w.kv_head), dk[n], half, f.width);
+      if constexpr (kV) store_columns<T, kColumns>(f.v_grad.at(t, w.kv_head), dv[n], half, f.width);
     }
+    for (; odd; odd &= odd - 1) key_gradient_row(f, first + block0 + wave0 + 32 * n + __builtin_ctzll(odd), w.kv_head, kK, kV);
   }
-  if (wave0 >= rest) return;
-  bool finite = true;
+}
+
+// Adds up the shares of a head of a token (of q) or a key, a wavefront for each; the numbers of shares are those that the kernels before found.
+template <int D>
+__device__ __forceinline__ Some<D> add_shares(const float* at, int64_t step, int32_t shares)
+{
+  Some<D> sum{};
+#pragma unroll 4
+  for (int32_t c = 0; c < shares; ++c) sum += *reinterpret_cast<const Some<D>*>(at + c * step + lane_id() * (D / kWave));
+  return sum;
+}
+
+// Writes a row of a gradient; false: not, what it holds is not finite.
+template <typename T, int D>
+__device__ __forceinline__ bool write_row(T* head, Some<D> sum, int32_t width)
+{
+  constexpr int kEach = D / kWave;
+  bool finite         = true;
 #pragma unroll
-  for (int c = 0; c < kColumns; ++c)
+  for (int k = 0; k < kEach; ++k) finite = finite && (lane_id() * kEach + k >= width || fabsf(sum[k]) < INFINITY);
+  if (__ballot(!finite)) return false;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      if constexpr (kK) {
-        dk[c][r] *= f.scale;
-        finite = finite && fabsf(dk[c][r]) < INFINITY;
-      }
-      if constexpr (kV) finite = finite && fabsf(dv[c][r]) < INFINITY;
-    }
-  uint64_t odd = __ballot(there && key < keys && !finite);
-  odd          = (odd | odd >> 32) & 0xffffffffu;
-  if (there && !(odd >> column & 1)) {
-    if (key >= keys) {
-#pragma unroll
-      for (int c = 0; c < kColumns; ++c) {
-        if constexpr (kK) dk[c] = f32x16_t{};
-        if constexpr (kV) dv[c] = f32x16_t{};
-      }
-    }
-    if constexpr (kK) store_columns<T, kColumns>(f.k_grad.at(t, w.kv_head), dk, half, f.width);
-    if constexpr (kV) store_columns<T, kColumns>(f.v_grad.at(t, w.kv_head), dv, half, f.width);
-  }
-  while (odd) {
-    int const which = __builtin_ctzll(odd);
-    odd &= odd - 1;
-    key_gradient_row(f, first + block0 + wave0 + which, w.kv_head, kK, kV);
-  }
+  for (int k = 0; k < kEach; ++k)
+    if (lane_id() * kEach + k < width) head[lane_id() * kEach + k] = static_cast<T>(sum[k]);
+  return true;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) query_gradient_join_kernel(Backward<T> f, Split split, int shift)
+{
+  constexpr int kTile = Tile<T, D>::kHeads;
+  int64_t const item  = block_number() * (kThreads / kWave) + threadIdx.x / kWave;
+  if (item >= static_cast<int64_t>(f.runs.tokens) * f.heads) return;
+  int32_t const t = static_cast<int32_t>(item / f.heads), head = static_cast<int32_t>(item % f.heads), run = run_with(f.runs, t);
+  if (!f.is_row(run)) return;
+  int32_t first, keys;
+  f.keys_of(run, first, keys);
+  int32_t const begin = f.runs.begin(run), tokens = f.runs.begin(run + 1) - begin, i = t - begin, last = i | ((1 << shift) - 1);
+  int32_t const all = f.seen(last < tokens ? last : tokens - 1, tokens, keys), shares = shares_of((all + kTile - 1) / kTile, split.splits);
+  if (shares < 2) return;
+  int64_t const at = (split.slot(f.runs.first_block(run, shift) + (i >> shift), head, f.heads, 0) << shift) + (i & ((1 << shift) - 1));
+  if (!write_row<T, D>(f.q_grad.at(t, head), add_shares<D>(split.sums + at * D, static_cast<int64_t>(D) << shift, shares) * f.scale, f.width)) query_gradient_row(f, t, head);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) key_gradient_join_kernel(Backward<T> f, Split split, int shift)
+{
+  constexpr int kTile = Tile<T, D>::kHeads;
+  int64_t const item  = block_number() * (kThreads / kWave) + threadIdx.x / kWave;
+  if (item >= static_cast<int64_t>(f.key_runs.tokens) * f.kv_heads) return;
+  int32_t const t = static_cast<int32_t>(item / f.kv_heads), head = static_cast<int32_t>(item % f.kv_heads), run = run_with(f.key_runs, t);
+  if (!f.is_row(run)) return;
+  int32_t first, keys;
+  f.keys_of(run, first, keys);
+  int32_t const tokens = f.runs.begin(run + 1) - f.runs.begin(run), i = t - first, block0 = i >> shift << shift;
+  if (i >= keys || tokens <= 0) return;
+  int64_t const from = f.causal ? static_cast<int64_t>(block0) + tokens - keys : 0;
+  int32_t const start = static_cast<int32_t>(from < 0 ? 0 : from < tokens ? from : tokens) / kTile, tiles = (tokens + kTile - 1) / kTile;
+  int32_t const shares = shares_of((tiles - start) * (f.heads / f.kv_heads), split.splits);
+  if (shares < 2) return;
+  int64_t const at   = (split.slot(f.key_runs.first_block(run, shift) + (i >> shift), head, f.kv_heads, 0) << shift) + (i & ((1 << shift) - 1));
+  int64_t const step = static_cast<int64_t>(2 * D) << shift;
+  bool const of_k    = write_row<T, D>(f.k_grad.at(t, head), add_shares<D>(split.sums + at * (2 * D), step, shares) * f.scale, f.width);
+  bool const of_v    = write_row<T, D>(f.v_grad.at(t, head), add_shares<D>(split.sums + at * (2 * D) + D, step, shares), f.width);
+  if (!of_k || !of_v) key_gradient_row(f, t, head, !of_k, !of_v);
 }
 
 // ------------------------------------------------------------------ launches
@@ -752,14 +952,50 @@ hipError_t allow_lds(Kernel kernel, int bytes)
   return bytes > 65536 ? hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) : hipSuccess;
 }
 
-template <typename T, int D, int WAVES, int NQ>
-nvtext_amd_status attend_tiles(Forward<T> const& f, hipStream_t stream)
+// In how many shares the tiles of a workgroup go: so many that there are twice as many workgroups as run at once, two a CU, if that many have kLeastTiles
+// tiles on average; and none where there are that many workgroups, or tiles take no longer than another launch.
+inline int32_t splits_of(int64_t workgroups, int64_t tiles)
 {
-  using Shape = ForwardShape<T, D, WAVES, NQ>;
-  ProfileScope const scope("attention_tiles", stream);
+  int64_t const at_once = 2 * device_cus();
+  if (workgroups >= at_once || workgroups <= 0 || tiles < 3 * kLeastTiles) return 1;
+  return static_cast<int32_t>(std::min<int64_t>({(2 * at_once + workgroups - 1) / workgroups, tiles / kLeastTiles, 16}));
+}
+
+// Workgroups with something to do, and what they have, as far as the host knows: rows are taken to be alike.
+struct Estimate {
+  int64_t workgroups, tiles;
+};
+template <typename T>
+Estimate estimate(Problem<T> const& p, Runs const& blocks, int32_t heads, int shift, Runs const& other, int tile, int64_t times)
+{
+  int64_t const rows = std::max(1, blocks.rows), length = (blocks.tokens + rows - 1) / rows;
+  int64_t const seen = (other.tokens + rows - 1) / rows, tiles = (seen + tile - 1) / tile;
+  // (causal, with as many tokens as keys: half of them on average)
+  return {rows * ((length + (1 << shift) - 1) >> shift) * heads, (p.causal && other.tokens <= blocks.tokens ? (tiles + 1) / 2 : tiles) * times};
+}
+
+template <typename T, int D, int WAVES, int NQ>
+nvtext_amd_status attend_tiles(Forward<T> const& f, Mr const& mr, hipStream_t stream)
+{
+  using Shape      = ForwardShape<T, D, WAVES, NQ>;
+  Estimate const e = estimate(f, f.runs, f.heads, Shape::kShift, f.key_runs, Shape::kTile, 1);
+  Split split{splits_of(e.workgroups, e.tiles), nullptr, nullptr};
+  size_t const rows = split.splits > 1 ? static_cast<size_t>(f.runs.blocks(Shape::kShift) * f.heads * split.splits) << Shape::kShift : 0;
+  TempParts<2> const temp(mr, {rows * D * sizeof(float), rows * sizeof(float2)});
+  if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
+  split.sums = temp.template part<float>(0);
+  split.tops = temp.template part<float2>(1);
   NVTEXT_HIP_TRY(allow_lds(attend_tiles_kernel<T, D, WAVES, NQ>, Shape::kLds));
-  int64_t const items = work_items(f.runs.blocks(Shape::kShift), f.kv_heads, f.heads / f.kv_heads);
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_tiles_kernel<T, D, WAVES, NQ>), grid_of(items, WAVES * kWave), dim3(WAVES * kWave), Shape::kLds, stream, f);
+  {
+    ProfileScope const scope("attention_tiles", stream);
+    int64_t const items = work_items(f.runs.blocks(Shape::kShift), f.kv_heads, f.heads / f.kv_heads, split.splits);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_tiles_kernel<T, D, WAVES, NQ>), grid_of(items, WAVES * kWave), dim3(WAVES * kWave), Shape::kLds, stream, f, split);
+  }
+  if (split.splits > 1) {
+    ProfileScope const scope("attention_join", stream);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_join_shares_kernel<T, D>), grid_of((static_cast<int64_t>(f.runs.tokens) * f.heads + 3) / 4, kThreads), dim3(kThreads), 0, stream, f, split,
+                       int{Shape::kShift});
+  }
   return NVTEXT_AMD_SUCCESS;
 }
 
@@ -770,7 +1006,7 @@ nvtext_amd_status attend_chunks(ForwardChunks<T> const& f, hipStream_t stream)
   NVTEXT_HIP_TRY(allow_lds(attend_chunks_kernel<T, D>, kLds));
   {
     ProfileScope const scope("attention_chunks", stream);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_chunks_kernel<T, D>), grid_of(work_items(f.key_runs.blocks(f.shift), f.kv_heads, 1), kWave), dim3(kWave), kLds, stream, f);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_chunks_kernel<T, D>), grid_of(work_items(f.key_runs.blocks(f.shift), f.kv_heads, 1, 1), kWave), dim3(kWave), kLds, stream, f);
   }
   ProfileScope const scope("attention_join", stream);
   hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_join_kernel<T, D>), grid_of(static_cast<int64_t>(f.runs.tokens) * f.heads, kJoinWaves * kWave), dim3(kJoinWaves * kWave), 0, stream, f);
@@ -803,38 +1039,58 @@ nvtext_amd_status attention(Forward<T> f, Mr const& mr, hipStream_t stream)
     if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
     align.launch(temp.template part<char>(0), stream);
     if (chunks) return attend_chunks<T, kD>({f, shift, temp.template part<float>(1), temp.template part<float2>(2)}, stream);
-    return attend_tiles<T, kD, 4, 1>(f, stream);
+    return attend_tiles<T, kD, 4, 1>(f, mr, stream);
   });
 }
 
-template <typename T, int D, int WAVES, Part PART>
-nvtext_amd_status key_gradient_tiles(Backward<T> const& f, hipStream_t stream)
+template <typename T, int D, int WAVES, int NK, Part PART>
+nvtext_amd_status key_gradient_tiles(Backward<T> const& f, Split const& split, hipStream_t stream)
 {
-  using Shape = GradientShape<T, D, WAVES>;
+  using Shape = KeyShape<T, D, WAVES, NK>;
   ProfileScope const scope("attention_key_gradient", stream);
-  NVTEXT_HIP_TRY(allow_lds(key_gradient_tiles_kernel<T, D, WAVES, PART>, Shape::kKeyLds));
-  int64_t const items = work_items(f.key_runs.blocks(Shape::kShift), f.kv_heads, 1);
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(key_gradient_tiles_kernel<T, D, WAVES, PART>), grid_of(items, WAVES * kWave), dim3(WAVES * kWave), Shape::kKeyLds, stream, f);
+  NVTEXT_HIP_TRY(allow_lds(key_gradient_tiles_kernel<T, D, WAVES, NK, PART>, Shape::kLds));
+  int64_t const items = work_items(f.key_runs.blocks(Shape::kShift), f.kv_heads, 1, split.splits);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(key_gradient_tiles_kernel<T, D, WAVES, NK, PART>), grid_of(items, WAVES * kWave), dim3(WAVES * kWave), Shape::kLds, stream, f, split);
   return NVTEXT_AMD_SUCCESS;
 }
 
-template <typename T, int D, int WAVES>
-nvtext_amd_status gradient_tiles(Backward<T> const& f, hipStream_t stream)
+template <typename T, int D>
+nvtext_amd_status gradient_tiles(Backward<T> const& f, Mr const& mr, hipStream_t stream)
 {
-  using Shape = GradientShape<T, D, WAVES>;
+  constexpr int kWaves = 4;
+  using OfQ            = GradientShape<T, D, kWaves>;
+  using OfK            = KeyShape<T, D, kWaves, 1>;
+  Estimate const q = estimate(f, f.runs, f.heads, OfQ::kShift, f.key_runs, OfQ::kTile, 1), k = estimate(f, f.key_runs, f.kv_heads, OfK::kShift, f.runs, OfK::kTile, f.heads / f.kv_heads);
+  Split of_q{f.runs.tokens > 0 ? splits_of(q.workgroups, q.tiles) : 1, nullptr, nullptr}, of_k{f.key_runs.tokens > 0 ? splits_of(k.workgroups, k.tiles) : 1, nullptr, nullptr};
+  TempParts<2> const temp(mr, {of_q.splits > 1 ? static_cast<size_t>(f.runs.blocks(OfQ::kShift) * f.heads * of_q.splits * OfQ::kRows * D) * sizeof(float) : 0,
+                               of_k.splits > 1 ? static_cast<size_t>(f.key_runs.blocks(OfK::kShift) * f.kv_heads * of_k.splits * OfK::kRows * D) * 2 * sizeof(float) : 0});
+  if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
+  of_q.sums = temp.template part<float>(0);
+  of_k.sums = temp.template part<float>(1);
   if (f.runs.tokens > 0) {
     ProfileScope const scope("attention_query_gradient", stream);
-    NVTEXT_HIP_TRY(allow_lds(query_gradient_tiles_kernel<T, D, WAVES>, Shape::kLds));
-    int64_t const items = work_items(f.runs.blocks(Shape::kShift), f.kv_heads, f.heads / f.kv_heads);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(query_gradient_tiles_kernel<T, D, WAVES>), grid_of(items, WAVES * kWave), dim3(WAVES * kWave), Shape::kLds, stream, f);
+    NVTEXT_HIP_TRY(allow_lds(query_gradient_tiles_kernel<T, D, kWaves>, OfQ::kLds));
+    int64_t const items = work_items(f.runs.blocks(OfQ::kShift), f.kv_heads, f.heads / f.kv_heads, of_q.splits);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(query_gradient_tiles_kernel<T, D, kWaves>), grid_of(items, kWaves * kWave), dim3(kWaves * kWave), OfQ::kLds, stream, f, of_q);
+  }
+  if (of_q.splits > 1) {
+    ProfileScope const scope("attention_query_gradient_join", stream);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(query_gradient_join_kernel<T, D>), grid_of((static_cast<int64_t>(f.runs.tokens) * f.heads + 3) / 4, kThreads), dim3(kThreads), 0, stream, f, of_q,
+                       int{OfQ::kShift});
   }
   if (f.key_runs.tokens == 0) return NVTEXT_AMD_SUCCESS;
-  if constexpr (D > 128) {
-    nvtext_amd_status const st = key_gradient_tiles<T, D, WAVES, kOfK>(f, stream);
-    return st != NVTEXT_AMD_SUCCESS ? st : key_gradient_tiles<T, D, WAVES, kOfV>(f, stream);
+  nvtext_amd_status st;
+  if constexpr (D * sizeof(T) > 128 && (sizeof(T) == 2 || D > 128)) {
+    st = key_gradient_tiles<T, D, kWaves, 1, kOfK>(f, of_k, stream);
+    if (st == NVTEXT_AMD_SUCCESS) st = key_gradient_tiles<T, D, kWaves, 1, kOfV>(f, of_k, stream);
   } else {
-    return key_gradient_tiles<T, D, WAVES, kBoth>(f, stream);
+    st = key_gradient_tiles<T, D, kWaves, 1, kBoth>(f, of_k, stream);
   }
+  if (st != NVTEXT_AMD_SUCCESS || of_k.splits == 1) return st;
+  ProfileScope const scope("attention_key_gradient_join", stream);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(key_gradient_join_kernel<T, D>), grid_of((static_cast<int64_t>(f.key_runs.tokens) * f.kv_heads + 3) / 4, kThreads), dim3(kThreads), 0, stream, f, of_k,
+                     int{OfK::kShift});
+  return NVTEXT_AMD_SUCCESS;
 }
 
 template <typename T>
@@ -849,7 +1105,7 @@ nvtext_amd_status attention_backward(Backward<T> f, Mr const& mr, hipStream_t st
   f.deltas = temp.template part<float>(0);
   f.logs   = temp.template part<float>(1);
   align.launch(temp.template part<char>(2), stream);
-  return with_tiles(f.width, [&](auto d) { return gradient_tiles<T, decltype(d)::value, 4>(f, stream); });
+  return with_tiles(f.width, [&](auto d) { return gradient_tiles<T, decltype(d)::value>(f, mr, stream); });
 }
 
 // What both directions ask of their arguments; nullptr if it holds.

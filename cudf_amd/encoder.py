@@ -43,7 +43,8 @@ class LayerNormSaved(NamedTuple):
 
 class AttentionSaved(NamedTuple):
     """What attention keeps for its gradient: its result, of every head of a token the logarithm of what its exponentials
-    add up to, [heads, tokens], and, of 16-bit types, what rounding left off the result, an int8 for each of its values.
+    add up to, [heads, tokens], and, of 16-bit types, what rounding left off the result, an int8 for each of its values,
+    [heads, tokens, width].
     (Without that, the gradients of q and k are off by a rounding more.)"""
     out: torch.Tensor
     logsum: torch.Tensor
@@ -352,7 +353,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rows: Rows, key
     count, offsets, *keys = _key_rows(rows, key_rows, key_lengths)
     out = q.new_empty(q.shape)
     logsum = q.new_empty((m.heads, m.tokens), dtype=torch.float32) if keep else None
-    rest = q.new_empty(q.shape, dtype=torch.int8) if keep and q.dtype != torch.float32 else None
+    rest = q.new_empty((m.heads, m.tokens, m.width), dtype=torch.int8) if keep and q.dtype != torch.float32 else None
     st = _capi.load().nvtext_amd_attention(m, _heads(k, "k"), _heads(v, "v"), count, offsets, *keys, causal, _scale(scale, m.width), _stream_handle(),
                                            _mr().struct, _heads(out, "out"), logsum.data_ptr() if keep else None,
                                            None if rest is None else rest.data_ptr())
@@ -373,8 +374,8 @@ def attention_backward(grad: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
         raise ValueError("logsum must be a contiguous float32 tensor of shape [heads, tokens]")
     if saved.rest is not None:
         _here(saved.rest, "rest")
-        if saved.rest.dtype != torch.int8 or not saved.rest.is_contiguous() or saved.rest.shape != q.shape:
-            raise ValueError("rest must be a contiguous int8 tensor of q's shape")
+        if saved.rest.dtype != torch.int8 or not saved.rest.is_contiguous() or saved.rest.shape != (m.heads, m.tokens, m.width):
+            raise ValueError("rest must be a contiguous int8 tensor of shape [heads, tokens, width]")
     q_grad, k_grad, v_grad = out if out is not None else (_like(q), _like(k), _like(v))
     st = _capi.load().nvtext_amd_attention_backward(g, m, _heads(k, "k"), _heads(v, "v"), _heads(saved.out, "out"), saved.logsum.data_ptr(),
                                                     None if saved.rest is None else saved.rest.data_ptr(), count, offsets, *keys, causal, _scale(scale, m.width),

@@ -51,7 +51,7 @@ def unrounded(saved):
     if saved.rest is None:
         return saved.out.double().cpu().numpy()
     shift = {F16: 5, BF16: 8}[saved.out.dtype]
-    return (saved.out.float().view(torch.int32) + saved.rest.int() * 2**shift).view(torch.float32).double().cpu().numpy()
+    return (saved.out.float().view(torch.int32) + saved.rest.transpose(0, 1).int() * 2**shift).view(torch.float32).double().cpu().numpy()
 
 
 def offsets_of(lengths, first=0):
@@ -146,6 +146,14 @@ CASES = [
 ]
 
 
+# what one or another way through the kernels needs: rows of many columns among rows of few, chunks and shares of many tiles, and of causal ones that end
+# before others
+CASES += [
+    ([40, 1, 1, 1, 0, 2], [900, 300, 129, 128, 700, 127], 2, 2, 64, 0), ([1, 9], [2000, 1500], 4, 1, 128, 0), ([200], [1500], 2, 1, 64, 0), ([150, 3], [900, 1200], 2, 2, 128, 0),
+    ([1300], None, 2, 1, 64, 0), ([900, 40], None, 1, 1, 128, 0), ([700, 1], None, 2, 2, 256, 0), ([260], [1000], 8, 1, 40, 0), ([800], [200], 2, 1, 64, 0),
+]
+
+
 class Made:
     """A case's tensors, with tokens in front of the first row and behind the last, and keys in places with room."""
 
@@ -220,7 +228,7 @@ def test_what_rounding_leaves_off(case, dtype):
     m = Made(case, dtype, seed=3)
     want, log, off, log_off = orc.attention(m.q64, m.k64, m.v64, **m.oracle_rows(), causal=True, **rounding(dtype))
     out, saved = encoder.attention(m.q, m.k, m.v, *m.rows(), causal=True, keep=True)
-    assert saved.rest.dtype == torch.int8 and saved.rest.shape == out.shape
+    assert saved.rest.dtype == torch.int8 and saved.rest.shape == out.transpose(0, 1).shape
     more = unrounded(saved)
     assert (np.abs(more - want) <= off * 1.01 + UNIT[dtype] * 2.0**-7 * np.abs(want) + 2 * TINY[dtype]).all()
     wants, offs = orc.attention_backward(m.g64, m.q64, m.k64, m.v64, more, saved.logsum.double().cpu().numpy(), **m.oracle_rows(), causal=True, **rounding(dtype))
@@ -291,7 +299,7 @@ def test_what_is_not_seen_has_no_effect(dtype, value):
         # and the way back: of q, what does not see it; of k and v, what only tokens see that do not (none in its row behind it)
         clean = encoder.attention(m.q, m.k, m.v, ints(m.offsets), causal=True, keep=True)[1]
         saved = encoder.AttentionSaved(torch.where(pick[:, None, None], clean.out, out), torch.where(pick[None], clean.logsum, saved.logsum),
-                                       None if saved.rest is None else torch.where(pick[:, None, None], clean.rest, saved.rest))
+                                       None if saved.rest is None else torch.where(pick[None, :, None], clean.rest, saved.rest))
         grads = encoder.attention_backward(g, q, k, v, saved, ints(m.offsets), causal=True)
         wants, offs = orc.attention_backward(m.g64, m.q64, m.k64, m.v64, unrounded(clean), clean.logsum.double().cpu().numpy(), m.offsets, causal=True, **rounding(dtype))
         near(grads[0][pick], wants[0][untouched], offs[0][untouched])
