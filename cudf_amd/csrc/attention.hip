@@ -80,39 +80,51 @@ struct Attending {
     for (int c = 0; c < kColumns; ++c) o[n][c] = f32x16_t{};
   }
 
-  // A tile of keys from key0 on; partly: not all columns see all of it.
+  // A tile of keys from key0 on; partly: not all columns see all of it.  Fragments are read kAhead products before they are multiplied, and what vector instructions
+  // have to do is spread between the products: the maximum of a block of 32 keys while the next one's scores are made, exponentials of 16 keys while those
+  // before are multiplied with v.  (Left to itself, the compiler reads a fragment, waits for it and multiplies.)
   __device__ __forceinline__ void pass(LdsBytes k_tile, LdsBytes v_tile, TileReader<T, D> const& read, int32_t key0, bool partly, float scale, int half)
   {
     f32x16_t s[NQ][kBlocks];
+    float high[NQ];
+    {
+      constexpr int kSlots = kBlocks * kSteps, kAhead = sizeof(T) == 2 ? 4 : 1;
+      Fragment<T> k[kAhead + 1];
+      for_each<kAhead>([&](auto i) { k[i] = read.rows(k_tile, i / kSteps, i % kSteps); });
+      __builtin_amdgcn_sched_barrier(0);
+      for_each<kSlots>([&](auto slot) {
+        constexpr int i = decltype(slot)::value, b = i / kSteps, step = i % kSteps;
+        if constexpr (i + kAhead < kSlots) k[(i + kAhead) % (kAhead + 1)] = read.rows(k_tile, (i + kAhead) / kSteps, (i + kAhead) % kSteps);
 #pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
+        for (int n = 0; n < NQ; ++n) {
+          if constexpr (step == 0) s[n][b] = f32x16_t{};
+          s[n][b] = multiply32(k[i % (kAhead + 1)], q[n][step], s[n][b]);
+          if constexpr (b > 0) {
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) s[n][b] = f32x16_t{};
-#pragma unroll
-      for (int step = 0; step < kSteps; ++step) {
-        Fragment<T> const k = read.rows(k_tile, b, step);
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) s[n][b] = multiply32(k, q[n][step], s[n][b]);
-      }
-    }
-    if (partly) {
-#pragma unroll
-      for (int n = 0; n < NQ; ++n)
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[n][b][r] = key0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4 < seen[n] ? s[n][b][r] : -INFINITY;
+            for (int r = step * 16 / kSteps; r < (step + 1) * 16 / kSteps; ++r) high[n] = b == 1 && r == 0 ? s[n][0][0] : fmaxf(high[n], s[n][b - 1][r]);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
     }
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      float high = s[n][0][0];
 #pragma unroll
-      for (int r = 1; r < 16 * kBlocks; ++r) high = fmaxf(high, s[n][r / 16][r % 16]);
-      Halves const both = halves(high);
-      high              = fmaxf(both.low, both.high) * scale;
+      for (int r = 0; r < 16; ++r) high[n] = kBlocks == 1 && r == 0 ? s[n][0][0] : fmaxf(high[n], s[n][kBlocks - 1][r]);
+      if (partly) {
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            s[n][b][r] = key0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4 < seen[n] ? s[n][b][r] : -INFINITY;
+            high[n]    = b == 0 && r == 0 ? s[n][0][0] : fmaxf(high[n], s[n][b][r]);
+          }
+      }
+      Halves const both = halves(high[n]);
+      high[n]           = fmaxf(both.low, both.high) * scale;
       // (a column that sees nothing yet keeps top at -infinity; NaN in a score is found in out at the end)
-      if (__ballot(high > top[n] + kSlack || top[n] == -INFINITY)) {
-        float const now  = fmaxf(top[n], high);
+      if (__ballot(high[n] > top[n] + kSlack || top[n] == -INFINITY)) {
+        float const now  = fmaxf(top[n], high[n]);
         float const fade = now == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top[n] - now);
         top[n]           = now;
         sum[n] *= fade;
@@ -121,27 +133,43 @@ struct Attending {
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[n][c][r] *= fade;
       }
-      float const base = top[n] == -INFINITY ? 0.f : top[n];
-#pragma unroll
-      for (int r = 0; r < 16 * kBlocks; ++r) {
-        float const p        = __builtin_amdgcn_exp2f(fmaf(s[n][r / 16][r % 16], scale, -base));
-        s[n][r / 16][r % 16] = p;
-        sum[n] += p;
-      }
     }
-    Fragment<T> p[NQ][2 * kBlocks];
+    {
+      constexpr int kRounds = 2 * kBlocks, kSlots = kRounds * kColumns, kAhead = sizeof(T) == 2 ? 3 : 1;
+      Fragment<T> v[kAhead + 1], p[NQ];
+      float base[NQ];
 #pragma unroll
-    for (int n = 0; n < NQ; ++n)
+      for (int n = 0; n < NQ; ++n) base[n] = top[n] == -INFINITY ? 0.f : top[n];
+      auto const exponential = [&](int n, int step, int e) {
+        int const r       = 8 * (step % 2) + e;
+        float const x     = __builtin_amdgcn_exp2f(fmaf(s[n][step / 2][r], scale, -base[n]));
+        s[n][step / 2][r] = x;
+        sum[n] += x;
+      };
+      for_each<kAhead>([&](auto i) { v[i] = read.columns(v_tile, i % kColumns, i / kColumns); });
 #pragma unroll
-      for (int step = 0; step < 2 * kBlocks; ++step) p[n][step] = rounded<T>(s[n][step / 2], step % 2);
+      for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-    for (int c = 0; c < kColumns; ++c)
-#pragma unroll
-      for (int step = 0; step < 2 * kBlocks; ++step) {
-        Fragment<T> const v = read.columns(v_tile, c, step);
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) o[n][c] = multiply32(v, p[n][step], o[n][c]);
+        for (int e = 0; e < 8; ++e) exponential(n, 0, e);
+        p[n] = rounded<T>(s[n][0], 0);
       }
+      __builtin_amdgcn_sched_barrier(0);
+      for_each<kSlots>([&](auto slot) {
+        constexpr int i = decltype(slot)::value, step = i / kColumns, c = i % kColumns;
+        if constexpr (i + kAhead < kSlots) v[(i + kAhead) % (kAhead + 1)] = read.columns(v_tile, (i + kAhead) % kColumns, (i + kAhead) / kColumns);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) o[n][c] = multiply32(v[i % (kAhead + 1)], p[n], o[n][c]);
+        if constexpr (step + 1 < kRounds) {
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+            for (int e = c * 8 / kColumns; e < (c + 1) * 8 / kColumns; ++e) exponential(n, step + 1, e);
+            if constexpr (c == kColumns - 1) p[n] = rounded<T>(s[n][(step + 1) / 2], (step + 1) % 2);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    }
   }
 
   // Writes out and logsum of a column, head h of token t, where it is `there`; of those whose result is not finite, the lanes' numbers.  That may come from keys that the
