@@ -358,6 +358,23 @@ struct TileReader {
   }
 };
 
+// use(0, read(0)), ... use(SLOTS - 1, read(SLOTS - 1)), with each fragment read some uses before its own: a read of LDS takes as long as a few products, and
+// the compiler, left to itself, reads a fragment, waits for it and multiplies.
+template <typename T, int SLOTS, typename Read, typename Use>
+__device__ __forceinline__ void stream(Read&& read, Use&& use)
+{
+  constexpr int kAhead = sizeof(T) == 2 ? 3 : 1;
+  Fragment<T> x[kAhead + 1];
+  for_each<kAhead>([&](auto i) { x[i] = read(i); });
+  __builtin_amdgcn_sched_barrier(0);
+  for_each<SLOTS>([&](auto slot) {
+    constexpr int i = decltype(slot)::value;
+    if constexpr (i + kAhead < SLOTS) x[(i + kAhead) % (kAhead + 1)] = read(std::integral_constant<int, i + kAhead>{});
+    use(slot, x[i % (kAhead + 1)]);
+    __builtin_amdgcn_sched_barrier(0);
+  });
+}
+
 // v of the lane of the lower 32 with this one's number among them, and of that of the upper 32
 struct Halves {
   float low, high;

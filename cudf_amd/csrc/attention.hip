@@ -557,26 +557,40 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
     }
     int32_t const key0 = tile * kTile;
     if (key0 >= most) continue;
+    // Of each block of 32 keys, scores and products of g and v, then what they come to, multiplied with the keys: a stream of fragments, read kAhead before
+    // they are multiplied.
+    constexpr int kFirst = 2 * kSteps, kOfBlock = kFirst + 2 * kColumns;
+    f32x16_t s, p;
+    Fragment<T> ds[2];
+    stream<T, kBlocks * kOfBlock>(
+      [&](auto slot) {
+        constexpr int b = slot / kOfBlock, i = slot % kOfBlock;
+        if constexpr (i < kSteps) return read.rows(k_tile, b, i);
+        else if constexpr (i < kFirst) return read.rows(v_tile, b, i - kSteps);
+        else return read.columns(k_tile, (i - kFirst) % kColumns, 2 * b + (i - kFirst) / kColumns);
+      },
+      [&](auto slot, Fragment<T> const& x) {
+        constexpr int b = slot / kOfBlock, i = slot % kOfBlock;
+        if constexpr (i < kSteps) {
+          if constexpr (i == 0) s = f32x16_t{};
+          s = multiply32(x, q[i], s);
+        } else if constexpr (i < kFirst) {
+          if constexpr (i == kSteps) p = f32x16_t{};
+          p = multiply32(x, g[i - kSteps], p);
+        } else {
+          if constexpr (i == kFirst) {
 #pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
-      f32x16_t s{}, p{};
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], scale, -log)) * (p[r] - delta);
+            if (key0 + 32 * b + 32 > least) {
 #pragma unroll
-      for (int step = 0; step < kSteps; ++step) s = multiply32(read.rows(k_tile, b, step), q[step], s);
-#pragma unroll
-      for (int step = 0; step < kSteps; ++step) p = multiply32(read.rows(v_tile, b, step), g[step], p);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], scale, -log)) * (p[r] - delta);
-      if (key0 + 32 * b + 32 > least) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = key0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4 < seen ? s[r] : 0.f;
-      }
-#pragma unroll
-      for (int step = 0; step < 2; ++step) {
-        Fragment<T> const ds = rounded<T>(s, step);
-#pragma unroll
-        for (int c = 0; c < kColumns; ++c) d[c] = multiply32(read.columns(k_tile, c, 2 * b + step), ds, d[c]);
-      }
-    }
+              for (int r = 0; r < 16; ++r) s[r] = key0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4 < seen ? s[r] : 0.f;
+            }
+            ds[0] = rounded<T>(s, 0);
+            ds[1] = rounded<T>(s, 1);
+          }
+          d[(i - kFirst) % kColumns] = multiply32(x, ds[(i - kFirst) / kColumns], d[(i - kFirst) % kColumns]);
+        }
+      });
   }
   if (wave0 >= rest) return;
   if (shares > 1) {
@@ -608,7 +622,7 @@ template <typename T, int D, int WAVES, int NK>
 struct KeyShape {
   static constexpr int kRows = 32 * WAVES * NK, kShift = __builtin_ctz(kRows), kTile = Tile<T, D>::kHeads, kTiles = 2 * Tile<T, D>::kBytes;
   static constexpr int kStage = kTiles + 2 * kWave * 4, kLds = 2 * kStage;  // (with logs and deltas)
-  static constexpr int kWavesASimd = D * sizeof(T) * NK <= 256 ? 2 : 1;
+  static constexpr int kWavesASimd = sizeof(T) == 2 && D * NK <= 128 ? 2 : 1;
 };
 // PART: the gradients of both, or of k or v alone (of wide heads there are not the registers for both).
 enum Part { kBoth, kOfK, kOfV };
@@ -688,9 +702,9 @@ __global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES, NK>::kWa
     load_q.load(to, here, wave);
     load_g.load(to + Tile<T, D>::kBytes, here, wave);
     int64_t const at = static_cast<int64_t>(next_head) * f.runs.tokens + begin + token;
-    uint32_t const range = static_cast<uint32_t>(here < kTile ? here : kTile) * 4;
-    if (wave == 0) load_words_to_lds(reinterpret_cast<const char*>(f.logs + at), range, to + Shape::kTiles, lane * 4);
-    if (wave == WAVES - 1) load_words_to_lds(reinterpret_cast<const char*>(f.deltas + at), range, to + Shape::kTiles + kWave * 4, lane * 4);
+    uint32_t const range = uniform(static_cast<uint32_t>(here < kTile ? here : kTile) * 4);
+    if (wave == 0) load_words_to_lds(uniform(reinterpret_cast<const char*>(f.logs + at)), range, to + Shape::kTiles, lane * 4);
+    if (wave == WAVES - 1) load_words_to_lds(uniform(reinterpret_cast<const char*>(f.deltas + at)), range, to + Shape::kTiles + kWave * 4, lane * 4);
     if (++loaded == of_head) {
       loaded = 0;
       ++next_head;
@@ -705,76 +719,80 @@ __global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES, NK>::kWa
     if (++tile == tiles) tile = start;
     int32_t const token0 = tile * kTile;
     if (token0 + kTile <= first_from) continue;
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
-      f32x16_t s[NK], p[NK];
-#pragma unroll
-      for (int n = 0; n < NK; ++n) s[n] = p[n] = f32x16_t{};
-#pragma unroll
-      for (int step = 0; step < kSteps; ++step) {
-        Fragment<T> const q = read.rows(q_tile, b, step);
-#pragma unroll
-        for (int n = 0; n < NK; ++n) s[n] = multiply32(q, k[n][step], s[n]);
-      }
-      if constexpr (kK) {
-#pragma unroll
-        for (int step = 0; step < kSteps; ++step) {
-          Fragment<T> const g = read.rows(g_tile, b, step);
-#pragma unroll
-          for (int n = 0; n < NK; ++n) p[n] = multiply32(g, v[n][step], p[n]);
+    // (as in the gradient of q: a stream of fragments)
+    constexpr int kFirst = (kK ? 2 : 1) * kSteps, kOfBlock = kFirst + 2 * (kK && kV ? 2 : 1) * kColumns;
+    f32x16_t s[NK], p[NK];
+    Fragment<T> weight[NK][2], ds[NK][2];
+    stream<T, kBlocks * kOfBlock>(
+      [&](auto slot) {
+        constexpr int b = slot / kOfBlock, i = slot % kOfBlock;
+        if constexpr (i < kSteps) return read.rows(q_tile, b, i);
+        else if constexpr (i < kFirst) return read.rows(g_tile, b, i - kSteps);
+        else {
+          constexpr int j = i - kFirst, step = j / ((kK && kV ? 2 : 1) * kColumns), c = j % ((kK && kV ? 2 : 1) * kColumns);
+          if constexpr (kV && c < kColumns) return read.columns(g_tile, c, 2 * b + step);
+          else return read.columns(q_tile, c % kColumns, 2 * b + step);
         }
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      int32_t const row0 = token0 + 32 * b;
-      bool const partly  = row0 < last_from || row0 + 32 > tokens;
+      },
+      [&](auto slot, Fragment<T> const& x) {
+        constexpr int b = slot / kOfBlock, i = slot % kOfBlock;
+        if constexpr (i < kSteps) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f32x4_t const log   = *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(words + 128 * b + 32 * i);
-        f32x4_t const delta = *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(words + kWave * 4 + 128 * b + 32 * i);
-#pragma unroll
-        for (int n = 0; n < NK; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            int const r = 4 * i + e;
-            s[n][r]     = __builtin_amdgcn_exp2f(fmaf(s[n][r], scale, -log[e]));
-            p[n][r]     = s[n][r] * (p[n][r] - delta[e]);
+          for (int n = 0; n < NK; ++n) {
+            if constexpr (i == 0) s[n] = f32x16_t{};
+            s[n] = multiply32(x, k[n][i], s[n]);
           }
-      }
-      if (partly) {
+        } else if constexpr (i < kFirst) {
 #pragma unroll
-        for (int n = 0; n < NK; ++n)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            int32_t const i = row0 + 8 * (r / 4) + 4 * half + r % 4;
-            bool const sees = i >= from[n] && i < tokens;
-            s[n][r]         = sees ? s[n][r] : 0.f;
-            p[n][r]         = sees ? p[n][r] : 0.f;
+          for (int n = 0; n < NK; ++n) {
+            if constexpr (i == kSteps) p[n] = f32x16_t{};
+            p[n] = multiply32(x, v[n][i - kSteps], p[n]);
           }
-      }
+        } else {
+          if constexpr (i == kFirst) {
+            int32_t const row0 = token0 + 32 * b;
+            bool const partly  = row0 < last_from || row0 + 32 > tokens;
 #pragma unroll
-      for (int step = 0; step < 2; ++step) {
-        Fragment<T> weight[NK], ds[NK];
+            for (int j = 0; j < 4; ++j) {
+              f32x4_t const log = *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(words + 128 * b + 32 * j);
+              f32x4_t delta{};
+              if constexpr (kK) delta = *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(words + kWave * 4 + 128 * b + 32 * j);
 #pragma unroll
-        for (int n = 0; n < NK; ++n) {
-          weight[n] = rounded<T>(s[n], step);
-          ds[n]     = rounded<T>(p[n], step);
+              for (int n = 0; n < NK; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  int const r = 4 * j + e;
+                  s[n][r]     = __builtin_amdgcn_exp2f(fmaf(s[n][r], scale, -log[e]));
+                  if constexpr (kK) p[n][r] = s[n][r] * (p[n][r] - delta[e]);
+                }
+            }
+            if (partly) {
+#pragma unroll
+              for (int n = 0; n < NK; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                  int32_t const t = row0 + 8 * (r / 4) + 4 * half + r % 4;
+                  bool const sees = t >= from[n] && t < tokens;
+                  if constexpr (kV) s[n][r] = sees ? s[n][r] : 0.f;
+                  if constexpr (kK) p[n][r] = sees ? p[n][r] : 0.f;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NK; ++n)
+#pragma unroll
+              for (int step = 0; step < 2; ++step) {
+                if constexpr (kV) weight[n][step] = rounded<T>(s[n], step);
+                if constexpr (kK) ds[n][step] = rounded<T>(p[n], step);
+              }
+          }
+          constexpr int j = i - kFirst, step = j / ((kK && kV ? 2 : 1) * kColumns), c = j % ((kK && kV ? 2 : 1) * kColumns);
+#pragma unroll
+          for (int n = 0; n < NK; ++n) {
+            if constexpr (kV && c < kColumns) dv[n][c] = multiply32(x, weight[n][step], dv[n][c]);
+            else dk[n][c % kColumns] = multiply32(x, ds[n][step], dk[n][c % kColumns]);
+          }
         }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int c = 0; c < kColumns; ++c) {
-          if constexpr (kV) {
-            Fragment<T> const g = read.columns(g_tile, c, 2 * b + step);
-#pragma unroll
-            for (int n = 0; n < NK; ++n) dv[n][c] = multiply32(g, weight[n], dv[n][c]);
-          }
-          if constexpr (kK) {
-            Fragment<T> const q = read.columns(q_tile, c, 2 * b + step);
-#pragma unroll
-            for (int n = 0; n < NK; ++n) dk[n][c] = multiply32(q, ds[n], dk[n][c]);
-          }
-        }
-      }
-    }
+      });
   }
   if (shares > 1) {
 #pragma unroll
