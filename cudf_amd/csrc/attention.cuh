@@ -62,15 +62,14 @@ __device__ __forceinline__ float wave_max(float v)
 }
 
 // What rounding to a 16-bit type leaves off, in 8 bits more: the difference of the two values' bits as float32, in 2^-8 of a step of the type.  (Signs
-// are alike, so bits differ as values do; zeros and the smallest numbers, whose steps are others, get what 8 bits hold of it.)  With them a sum of products
+// are alike, so bits differ as values do; zeros and the smallest numbers, whose steps are others, get what 8 bits hold of it, and
+// beside an infinity they are of no meaning.)  With them a sum of products
 // with out is as good as one with out in float32 for what is rounded to 16 bits afterwards.
 template <typename T>
 __device__ __forceinline__ int8_t rest_of(float x, T rounded)
 {
   constexpr int kShift = sizeof(T) == 4 ? 0 : std::is_same_v<T, half_t> ? 5 : 8;
-  float const y        = static_cast<float>(rounded);
-  if (!(fabsf(y) < INFINITY)) return 0;
-  int32_t const off = (__builtin_bit_cast(int32_t, x) - __builtin_bit_cast(int32_t, y) + (1 << kShift >> 1)) >> kShift;
+  int32_t const off    = (__builtin_bit_cast(int32_t, x) - __builtin_bit_cast(int32_t, static_cast<float>(rounded)) + (1 << kShift >> 1)) >> kShift;
   return static_cast<int8_t>(off < -127 ? -127 : off > 127 ? 127 : off);
 }
 template <typename T>
@@ -413,49 +412,66 @@ __device__ __forceinline__ Fragment<T> fragment_of(const T* head, int32_t j, int
   return f;
 }
 
-// Writes a lane's column of results, transposed: values of a head, four next to each other (stores of 8 bytes take any
-// address that the type has), and those of a width that is no multiple of four one by one.
-template <typename T, int COLUMNS>
-__device__ __forceinline__ void store_columns(T* head, f32x16_t const (&x)[COLUMNS], int half, int32_t width)
+// Writes a lane's column of results, transposed: with what its neighbour of the other half has, eight values of a head next to each other (stores of 16 bytes take
+// any address that the type has).  Those of a width that is no multiple of eight end one by one.
+template <typename U, int COLUMNS, typename Make>
+__device__ __forceinline__ void store_eights(U* head, int half, int32_t width, Make&& make)
 {
-  typedef T Four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  typedef U Eight_t __attribute__((ext_vector_type(8), aligned(sizeof(U))));
+  typedef uint32_t Words __attribute__((ext_vector_type(sizeof(U))));  // four values
 #pragma unroll
   for (int c = 0; c < COLUMNS; ++c)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      int32_t const j = 32 * c + 8 * g + 4 * half;
-      Four const four = {static_cast<T>(x[c][4 * g]), static_cast<T>(x[c][4 * g + 1]), static_cast<T>(x[c][4 * g + 2]), static_cast<T>(x[c][4 * g + 3])};
-      if (j + 4 <= width) {
-        *reinterpret_cast<Four*>(head + j) = four;
-      } else {
+    for (int g = 0; g < 4; g += 2) {
+      // (this lane has values 4 * half .. 4 * half + 3 of the eight from 32 c + 8 g on, and of the next eight; each half gives one of them away)
+      Words a = make(c, g), b = make(c, g + 1);
 #pragma unroll
-        for (int e = 0; e < 3; ++e)
-          if (j + e < width) head[j + e] = four[e];
+      for (int w = 0; w < static_cast<int>(sizeof(U)); ++w) {
+        uint32_t const x = a[w], y = b[w];
+        auto const both  = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+        a[w]             = both[0];
+        b[w]             = both[1];
+      }
+      typedef uint32_t Both __attribute__((ext_vector_type(2 * sizeof(U))));
+      Both words;
+#pragma unroll
+      for (int w = 0; w < static_cast<int>(sizeof(U)); ++w) {
+        words[w]             = a[w];
+        words[w + sizeof(U)] = b[w];
+      }
+      Eight_t const eight = __builtin_bit_cast(Eight_t, words);
+      int32_t const j     = 32 * c + 8 * g + 8 * half;
+      if (width == 32 * COLUMNS || j + 8 <= width) {
+        *reinterpret_cast<Eight_t*>(head + j) = eight;
+      } else {
+        for (int e = 0; e < 7; ++e)
+          if (j + e < width) head[j + e] = eight[e];
       }
     }
 }
 
-// Writes what rounding left off a lane's column of results, in the same places of a head's.
+template <typename T, int COLUMNS>
+__device__ __forceinline__ void store_columns(T* head, f32x16_t const (&x)[COLUMNS], int half, int32_t width)
+{
+  store_eights<T, COLUMNS>(head, half, width, [&](int c, int g) {
+    typedef T Four __attribute__((ext_vector_type(4)));
+    Four const four = {static_cast<T>(x[c][4 * g]), static_cast<T>(x[c][4 * g + 1]), static_cast<T>(x[c][4 * g + 2]), static_cast<T>(x[c][4 * g + 3])};
+    typedef uint32_t Words __attribute__((ext_vector_type(sizeof(T))));
+    return __builtin_bit_cast(Words, four);
+  });
+}
+
+// The same for what rounding left off.
 template <typename T, int COLUMNS>
 __device__ __forceinline__ void store_rests(int8_t* head, f32x16_t const (&x)[COLUMNS], int half, int32_t width)
 {
-  typedef int8_t Four __attribute__((ext_vector_type(4), aligned(1)));
+  store_eights<int8_t, COLUMNS>(head, half, width, [&](int c, int g) {
+    uint32_t four = 0;
 #pragma unroll
-  for (int c = 0; c < COLUMNS; ++c)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      int32_t const j = 32 * c + 8 * g + 4 * half;
-      Four four;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) four[e] = rest_of(x[c][4 * g + e], static_cast<T>(x[c][4 * g + e]));
-      if (j + 4 <= width) {
-        *reinterpret_cast<Four*>(head + j) = four;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 3; ++e)
-          if (j + e < width) head[j + e] = four[e];
-      }
-    }
+    for (int e = 0; e < 4; ++e) four |= static_cast<uint32_t>(static_cast<uint8_t>(rest_of(x[c][4 * g + e], static_cast<T>(x[c][4 * g + e])))) << 8 * e;
+    typedef uint32_t Words __attribute__((ext_vector_type(1)));
+    return Words{four};
+  });
 }
 
 }  // namespace nvtext_amd

@@ -8,6 +8,7 @@ namespace nvtext_amd {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kTileWaves = 4;  // wavefronts that share the tiles in LDS
 
 // ------------------------------------------------------------------ forward, in tiles
 // The work of a launch: blocks of tokens, of every head, in `splits` shares.  The heads that share a key head come one after the other on one XCD (workgroups go
@@ -52,32 +53,32 @@ struct Split {
   __device__ __forceinline__ int64_t slot(int64_t block, int32_t head, int32_t heads, int32_t share) const { return (block * heads + head) * splits + share; }
 };
 
-template <typename T, int D, int WAVES, int NQ>
+template <typename T, int D, int WAVES>
 struct ForwardShape {
-  static constexpr int kTokens = 32 * WAVES * NQ, kShift = __builtin_ctz(kTokens), kTile = Tile<T, D>::kHeads, kLds = 4 * Tile<T, D>::kBytes, kWavesASimd = D * sizeof(T) <= 256 ? 2 : 1;
+  static constexpr int kTokens = 32 * WAVES, kShift = __builtin_ctz(kTokens), kTile = Tile<T, D>::kHeads, kLds = 4 * Tile<T, D>::kBytes, kWavesASimd = D * sizeof(T) <= 128 ? 4 : D * sizeof(T) <= 256 ? 2 : 1;
 };
 
-// What a wavefront holds of 32 * NQ heads of tokens, columns of the products, while keys pass: q, and the sums of out, transposed.  Scores are products with the
+// What a wavefront holds of 32 heads of tokens, columns of the products, while keys pass: q, and the sums of out, transposed.  Scores are products with the
 // keys as rows, so a lane has all of a column's scores (with the one 32 further on), and exponentials are in its registers as the second product
 // takes them: no lane needs another's but for the maximum.  Sums are kept in proportion to 2^top, where top is a maximum that may be 8 too small:
 // only then are they multiplied anew.
-template <typename T, int D, int NQ>
+template <typename T, int D>
 struct Attending {
   static constexpr int kSteps = D / 16, kColumns = D / 32, kTile = Tile<T, D>::kHeads, kBlocks = kTile / 32;
   static constexpr float kSlack = 8.f;
-  Fragment<T> q[NQ][kSteps];
-  f32x16_t o[NQ][kColumns];
-  float top[NQ], sum[NQ];
-  int32_t seen[NQ];  // keys that the column sees
+  Fragment<T> q[kSteps];
+  f32x16_t o[kColumns];
+  float top, sum;
+  int32_t seen;  // keys that the column sees
 
-  __device__ __forceinline__ void begin(int n, const T* head, int32_t width, bool there, int half)
+  __device__ __forceinline__ void begin(const T* head, int32_t width, bool there, int half)
   {
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) q[n][s] = fragment_of(head, 16 * s + 8 * half, width, there);
-    top[n] = -INFINITY;
-    sum[n] = 0.f;
+    for (int s = 0; s < kSteps; ++s) q[s] = fragment_of(head, 16 * s + 8 * half, width, there);
+    top = -INFINITY;
+    sum = 0.f;
 #pragma unroll
-    for (int c = 0; c < kColumns; ++c) o[n][c] = f32x16_t{};
+    for (int c = 0; c < kColumns; ++c) o[c] = f32x16_t{};
   }
 
   // A tile of keys from key0 on; partly: not all columns see all of it.  Fragments are read kAhead products before they are multiplied, and what vector instructions
@@ -85,127 +86,100 @@ struct Attending {
   // before are multiplied with v.  (Left to itself, the compiler reads a fragment, waits for it and multiplies.)
   __device__ __forceinline__ void pass(LdsBytes k_tile, LdsBytes v_tile, TileReader<T, D> const& read, int32_t key0, bool partly, float scale, int half)
   {
-    f32x16_t s[NQ][kBlocks];
-    float high[NQ];
+    f32x16_t s[kBlocks];
     {
-      constexpr int kSlots = kBlocks * kSteps, kAhead = sizeof(T) == 2 ? 4 : 1;
-      Fragment<T> k[kAhead + 1];
-      for_each<kAhead>([&](auto i) { k[i] = read.rows(k_tile, i / kSteps, i % kSteps); });
-      __builtin_amdgcn_sched_barrier(0);
-      for_each<kSlots>([&](auto slot) {
-        constexpr int i = decltype(slot)::value, b = i / kSteps, step = i % kSteps;
-        if constexpr (i + kAhead < kSlots) k[(i + kAhead) % (kAhead + 1)] = read.rows(k_tile, (i + kAhead) / kSteps, (i + kAhead) % kSteps);
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-          if constexpr (step == 0) s[n][b] = f32x16_t{};
-          s[n][b] = multiply32(k[i % (kAhead + 1)], q[n][step], s[n][b]);
-          if constexpr (b > 0) {
-#pragma unroll
-            for (int r = step * 16 / kSteps; r < (step + 1) * 16 / kSteps; ++r) high[n] = b == 1 && r == 0 ? s[n][0][0] : fmaxf(high[n], s[n][b - 1][r]);
-          }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      });
+      constexpr int kSlots = kBlocks * kSteps;
+      stream<T, kSlots>([&](auto i) { return read.rows(k_tile, i / kSteps, i % kSteps); },
+                        [&](auto i, Fragment<T> const& k) {
+                          constexpr int b = i / kSteps, step = i % kSteps;
+                          if constexpr (step == 0) s[b] = f32x16_t{};
+                          s[b] = multiply32(k, q[step], s[b]);
+                        });
     }
+    if (partly) {
+      int32_t const left = seen - key0 - 4 * half;
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
+      for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) high[n] = kBlocks == 1 && r == 0 ? s[n][0][0] : fmaxf(high[n], s[n][kBlocks - 1][r]);
-      if (partly) {
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            s[n][b][r] = key0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4 < seen[n] ? s[n][b][r] : -INFINITY;
-            high[n]    = b == 0 && r == 0 ? s[n][0][0] : fmaxf(high[n], s[n][b][r]);
-          }
-      }
-      Halves const both = halves(high[n]);
-      high[n]           = fmaxf(both.low, both.high) * scale;
-      // (a column that sees nothing yet keeps top at -infinity; NaN in a score is found in out at the end)
-      if (__ballot(high[n] > top[n] + kSlack || top[n] == -INFINITY)) {
-        float const now  = fmaxf(top[n], high[n]);
-        float const fade = now == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top[n] - now);
-        top[n]           = now;
-        sum[n] *= fade;
-#pragma unroll
-        for (int c = 0; c < kColumns; ++c)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[n][c][r] *= fade;
-      }
+        for (int r = 0; r < 16; ++r) s[b][r] = 32 * b + 8 * (r / 4) + r % 4 < left ? s[b][r] : -INFINITY;
     }
-    {
-      constexpr int kRounds = 2 * kBlocks, kSlots = kRounds * kColumns, kAhead = sizeof(T) == 2 ? 3 : 1;
-      Fragment<T> v[kAhead + 1], p[NQ];
-      float base[NQ];
+    float high = s[0][0];
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) base[n] = top[n] == -INFINITY ? 0.f : top[n];
-      auto const exponential = [&](int n, int step, int e) {
-        int const r       = 8 * (step % 2) + e;
-        float const x     = __builtin_amdgcn_exp2f(fmaf(s[n][step / 2][r], scale, -base[n]));
-        s[n][step / 2][r] = x;
-        sum[n] += x;
-      };
-      for_each<kAhead>([&](auto i) { v[i] = read.columns(v_tile, i % kColumns, i / kColumns); });
+    for (int r = 1; r < 16 * kBlocks; ++r) high = fmaxf(high, s[r / 16][r % 16]);
+    Halves const both = halves(high);
+    high              = fmaxf(both.low, both.high) * scale;
+    // (a column that sees nothing yet keeps top at -infinity; NaN in a score is found in out at the end)
+    if (__ballot(high > top + kSlack || top == -INFINITY)) {
+      float const now  = fmaxf(top, high);
+      float const fade = now == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - now);
+      top              = now;
+      sum *= fade;
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) {
+      for (int c = 0; c < kColumns; ++c)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) exponential(n, 0, e);
-        p[n] = rounded<T>(s[n][0], 0);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      for_each<kSlots>([&](auto slot) {
-        constexpr int i = decltype(slot)::value, step = i / kColumns, c = i % kColumns;
-        if constexpr (i + kAhead < kSlots) v[(i + kAhead) % (kAhead + 1)] = read.columns(v_tile, (i + kAhead) % kColumns, (i + kAhead) / kColumns);
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) o[n][c] = multiply32(v[i % (kAhead + 1)], p[n], o[n][c]);
-        if constexpr (step + 1 < kRounds) {
-#pragma unroll
-          for (int n = 0; n < NQ; ++n) {
-#pragma unroll
-            for (int e = c * 8 / kColumns; e < (c + 1) * 8 / kColumns; ++e) exponential(n, step + 1, e);
-            if constexpr (c == kColumns - 1) p[n] = rounded<T>(s[n][(step + 1) / 2], (step + 1) % 2);
-          }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      });
+        for (int r = 0; r < 16; ++r) o[c][r] *= fade;
     }
+    constexpr int kRounds = 2 * kBlocks;
+    float const base = top == -INFINITY ? 0.f : top;
+    auto const exponential = [&](int step, int e) {
+      int const r    = 8 * (step % 2) + e;
+      float const x  = __builtin_amdgcn_exp2f(fmaf(s[step / 2][r], scale, -base));
+      s[step / 2][r] = x;
+      sum += x;
+    };
+    Fragment<T> p;
+    stream<T, kRounds * kColumns>([&](auto i) { return read.columns(v_tile, i % kColumns, i / kColumns); },
+                                  [&](auto i, Fragment<T> const& v) {
+                                    constexpr int step = i / kColumns, c = i % kColumns;
+                                    if constexpr (i == 0) {
+#pragma unroll
+                                      for (int e = 0; e < 8; ++e) exponential(0, e);
+                                      p = rounded<T>(s[0], 0);
+                                    }
+                                    o[c] = multiply32(v, p, o[c]);
+                                    if constexpr (step + 1 < kRounds) {
+#pragma unroll
+                                      for (int e = c * 8 / kColumns; e < (c + 1) * 8 / kColumns; ++e) exponential(step + 1, e);
+                                      if constexpr (c == kColumns - 1) p = rounded<T>(s[(step + 1) / 2], (step + 1) % 2);
+                                    }
+                                  });
   }
 
   // Writes out and logsum of a column, head h of token t, where it is `there`; of those whose result is not finite, the lanes' numbers.  That may come from keys that the
   // token does not see, whose exponentials of 0 were multiplied: such columns are done once more, by themselves.
-  __device__ __forceinline__ uint32_t finish(int n, Forward<T> const& f, int64_t t, int32_t h, bool there, int half, int column)
+  __device__ __forceinline__ uint32_t finish(Forward<T> const& f, int64_t t, int32_t h, bool there, int half, int column)
   {
-    Halves const both = halves(sum[n]);
-    float const total = both.low + both.high, part = seen[n] > 0 ? 1.f / total : 0.f;
-    bool finite       = true;
+    Halves const both = halves(sum);
+    float const total = both.low + both.high, part = seen > 0 ? 1.f / total : 0.f;
+    float check       = 0.f;  // (NaN if any is infinite or NaN)
 #pragma unroll
     for (int c = 0; c < kColumns; ++c)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        o[n][c][r] *= part;
-        finite = finite && fabsf(o[n][c][r]) < INFINITY;
+        o[c][r] *= part;
+        check = fmaf(o[c][r], 0.f, check);
       }
-    uint64_t odd = __ballot(there && seen[n] > 0 && !finite);
+    uint64_t odd = __ballot(there && seen > 0 && check != 0.f);
     odd          = (odd | odd >> 32) & 0xffffffffu;
     if (there && !(odd >> column & 1)) {
-      store_columns<T, kColumns>(f.out.at(t, h), o[n], half, f.width);
+      store_columns<T, kColumns>(f.out.at(t, h), o, half, f.width);
+      int64_t const at = static_cast<int64_t>(h) * f.runs.tokens + t;
       if constexpr (sizeof(T) == 2)
-        if (f.rest) store_rests<T, kColumns>(f.rest + (static_cast<int64_t>(h) * f.runs.tokens + t) * f.width, o[n], half, f.width);
-      if (f.logsum && half == 0) f.logsum[static_cast<int64_t>(h) * f.runs.tokens + t] = seen[n] > 0 ? (top[n] + __builtin_amdgcn_logf(total)) * kLn2 : -INFINITY;
+        if (f.rest) store_rests<T, kColumns>(f.rest + at * f.width, o, half, f.width);
+      if (f.logsum && half == 0) f.logsum[at] = seen > 0 ? (top + __builtin_amdgcn_logf(total)) * kLn2 : -INFINITY;
     }
     return static_cast<uint32_t>(odd);
   }
 };
 
-// A workgroup has kTokens tokens of a head, a wavefront 32 * NQ of them.  Keys come through LDS, 64 at a time, the next ones while these are multiplied.
-template <typename T, int D, int WAVES, int NQ>
-__global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES, NQ>::kWavesASimd)) attend_tiles_kernel(Forward<T> f, Split split)
+// A workgroup has kTokens tokens of a head, a wavefront 32 of them.  Keys come through LDS, 64 at a time, the next ones while these are multiplied.
+template <typename T, int D, int WAVES>
+__global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES>::kWavesASimd)) attend_tiles_kernel(Forward<T> f, Split split)
 {
-  using Shape = ForwardShape<T, D, WAVES, NQ>;
+  using Shape = ForwardShape<T, D, WAVES>;
   extern __shared__ __align__(16) char lds_[];
-  LdsBytes const lds = (LdsBytes)lds_;
-  constexpr int kTile = Shape::kTile;
+  LdsBytes const lds  = (LdsBytes)lds_;
+  constexpr int kTile = Shape::kTile, kStage = 2 * Tile<T, D>::kBytes;
   Work w;
   int32_t const each = f.heads / f.kv_heads;
   if (!work_of(block_number(), f.runs.blocks(Shape::kShift), f.kv_heads, each, split.splits, w)) return;
@@ -220,61 +194,49 @@ __global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES, NQ>:
   first = uniform(first);
   keys  = uniform(keys);
   // keys that the workgroup's last token sees, and the wavefront's first and last
-  int32_t const wave0 = wave * 32 * NQ, wave1 = wave0 + 32 * NQ < rest ? wave0 + 32 * NQ : rest;
+  int32_t const wave0 = wave * 32, wave1 = wave0 + 32 < rest ? wave0 + 32 : rest;
   int32_t const all   = uniform(f.seen(block0 + (rest < Shape::kTokens ? rest : Shape::kTokens) - 1, tokens, keys));
   int32_t const least = uniform(wave0 < rest ? f.seen(block0 + wave0, tokens, keys) : 0), most = uniform(wave0 < rest ? f.seen(block0 + wave1 - 1, tokens, keys) : 0);
-  int64_t const t0    = static_cast<int64_t>(begin) + block0 + wave0;
+  bool const there    = wave0 + column < rest;
+  int64_t const t     = static_cast<int64_t>(begin) + block0 + (there ? wave0 + column : 0);
 
   int32_t const all_tiles = (all + kTile - 1) / kTile, shares = shares_of(all_tiles, split.splits);
   if (w.share >= shares) return;
   int32_t const from = uniform(share_begin(all_tiles, w.share, shares)), tiles = uniform(share_begin(all_tiles, w.share + 1, shares));
 
-  Attending<T, D, NQ> a;
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    int32_t const i  = n * 32 + column;
-    bool const there = wave0 + i < rest;
-    a.seen[n]        = there ? f.seen(block0 + wave0 + i, tokens, keys) : 0;
-    a.begin(n, f.q.at(there ? t0 + i : begin, w.head), f.width, there, half);
-  }
+  Attending<T, D> a;
+  a.seen = there ? f.seen(block0 + wave0 + column, tokens, keys) : 0;
+  a.begin(f.q.at(t, w.head), f.width, there, half);
   TileLoader<T, D, WAVES> load_k, load_v;
   load_k.aim(f.k, first + from * kTile, w.kv_head, f.width, wave, lane);
   load_v.aim(f.v, first + from * kTile, w.kv_head, f.width, wave, lane);
+  auto const load = [&](int32_t tile) {
+    LdsBytes const to = lds + (tile & 1) * kStage;
+    load_k.load(to, keys - tile * kTile, wave);
+    load_v.load(to + Tile<T, D>::kBytes, keys - tile * kTile, wave);
+  };
   TileReader<T, D> const read(lane);
   float const scale = f.scale * kLog2e;
-  if (tiles > from) {
-    load_k.load(lds + (from & 1) * 2 * Tile<T, D>::kBytes, keys - from * kTile, wave);
-    load_v.load(lds + (from & 1) * 2 * Tile<T, D>::kBytes + Tile<T, D>::kBytes, keys - from * kTile, wave);
-  }
+  if (tiles > from) load(from);
   for (int32_t tile = from; tile < tiles; ++tile) {
-    LdsBytes const k_tile = lds + (tile & 1) * 2 * Tile<T, D>::kBytes;
+    LdsBytes const k_tile = lds + (tile & 1) * kStage;
     stage_barrier<0>();
-    if (tile + 1 < tiles) {
-      LdsBytes const next = lds + (~tile & 1) * 2 * Tile<T, D>::kBytes;
-      load_k.load(next, keys - (tile + 1) * kTile, wave);
-      load_v.load(next + Tile<T, D>::kBytes, keys - (tile + 1) * kTile, wave);
-    }
+    if (tile + 1 < tiles) load(tile + 1);
     int32_t const key0 = tile * kTile;
     if (key0 < most) a.pass(k_tile, k_tile + Tile<T, D>::kBytes, read, key0, key0 + kTile > least, scale, half);
   }
   if (wave0 >= rest) return;
   if (shares > 1) {
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      int64_t const part = split.slot(w.block, w.head, f.heads, w.share) * Shape::kTokens + wave0 + n * 32 + column;
-      Halves const both  = halves(a.sum[n]);
-      if (wave0 + n * 32 + column < rest) {
-        store_columns<float, D / 32>(split.sums + part * D, a.o[n], half, D);
-        if (half == 0) split.tops[part] = make_float2(a.top[n], both.low + both.high);
-      }
+    int64_t const part = split.slot(w.block, w.head, f.heads, w.share) * Shape::kTokens + wave0 + column;
+    Halves const both  = halves(a.sum);
+    if (there) {
+      store_columns<float, D / 32>(split.sums + part * D, a.o, half, D);
+      if (half == 0) split.tops[part] = make_float2(a.top, both.low + both.high);
     }
     return;
   }
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    uint32_t odd = a.finish(n, f, t0 + n * 32 + column, w.head, wave0 + n * 32 + column < rest, half, column);
-    for (; odd; odd &= odd - 1) attend_row(f, static_cast<int32_t>(t0) + n * 32 + __builtin_ctz(odd), w.head);
-  }
+  uint32_t odd = a.finish(f, t, w.head, there, half, column);
+  for (; odd; odd &= odd - 1) attend_row(f, begin + block0 + wave0 + __builtin_ctz(odd), w.head);
 }
 
 // ------------------------------------------------------------------ forward, in chunks of keys
@@ -328,9 +290,9 @@ __global__ void __launch_bounds__(kWave, 1) attend_chunks_kernel(ForwardChunks<T
     int32_t const i    = there ? static_cast<int32_t>(mine / each) : 0, head = w.kv_head * each + (there ? static_cast<int32_t>(mine - static_cast<int64_t>(i) * each) : 0);
     int64_t const t    = static_cast<int64_t>(begin) + i;
     int32_t const last = static_cast<int32_t>(((column0 + kPartColumns < columns ? column0 + kPartColumns : columns) - 1) / each);  // the last column's token
-    Attending<T, D, 1> a;
-    a.seen[0] = there ? f.seen(i, tokens, keys) : 0;
-    a.begin(0, f.q.at(t, head), f.width, there, half);
+    Attending<T, D> a;
+    a.seen = there ? f.seen(i, tokens, keys) : 0;
+    a.begin(f.q.at(t, head), f.width, there, half);
     int32_t const least = uniform(f.seen(static_cast<int32_t>(column0 / each), tokens, keys)), all = uniform(f.seen(last, tokens, keys)), end = all < key_last ? all : key_last;
     int32_t const tiles = end > key_first ? (end - key_first + kTile - 1) / kTile : 0;
     TileLoader<T, D, 1> load_k, load_v;
@@ -354,14 +316,14 @@ __global__ void __launch_bounds__(kWave, 1) attend_chunks_kernel(ForwardChunks<T
     stage_barrier<0>();  // (the next columns' loads come into the same places)
     if (split) {
       int64_t const part = f.part(first, static_cast<int32_t>(chunk), w.kv_head) * kPartColumns + column;
-      Halves const both  = halves(a.sum[0]);
+      Halves const both  = halves(a.sum);
       if (there) {
-        store_columns<float, D / 32>(f.sums + part * D, a.o[0], half, D);
-        if (half == 0) f.tops[part] = make_float2(a.top[0], both.low + both.high);
+        store_columns<float, D / 32>(f.sums + part * D, a.o, half, D);
+        if (half == 0) f.tops[part] = make_float2(a.top, both.low + both.high);
       }
       continue;
     }
-    for (uint32_t odd = a.finish(0, f, t, head, there, half, column); odd; odd &= odd - 1) {
+    for (uint32_t odd = a.finish(f, t, head, there, half, column); odd; odd &= odd - 1) {
       int const which = __builtin_ctz(odd);
       attend_row(f, __builtin_amdgcn_readlane(static_cast<int32_t>(t), which), __builtin_amdgcn_readlane(head, which));
     }
@@ -507,9 +469,19 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
   if (w.share >= shares) return;
   int32_t const first_tile = uniform(share_begin(all_tiles, w.share, shares)), tiles = uniform(share_begin(all_tiles, w.share + 1, shares));
   bool const there    = wave0 + column < rest;
-  int64_t const t     = static_cast<int64_t>(begin) + block0 + (there ? wave0 + column : 0), at = static_cast<int64_t>(w.head) * f.runs.tokens + t;
+  int64_t const t     = static_cast<int64_t>(begin) + block0 + (there ? wave0 + column : 0);
   int32_t const seen  = there ? f.seen(block0 + wave0 + column, tokens, keys) : 0;
 
+  TileLoader<T, D, WAVES> load_k, load_v;
+  load_k.aim(f.k, first + first_tile * kTile, w.kv_head, f.width, wave, lane);
+  load_v.aim(f.v, first + first_tile * kTile, w.kv_head, f.width, wave, lane);
+  auto const load = [&](int32_t tile) {
+    LdsBytes const to = lds + (tile & 1) * Shape::kStage;
+    load_k.load(to, keys - tile * kTile, wave);
+    load_v.load(to + Tile<T, D>::kBytes, keys - tile * kTile, wave);
+  };
+  if (tiles > first_tile) load(first_tile);
+  int64_t const at = static_cast<int64_t>(w.head) * f.runs.tokens + t;
   Fragment<T> q[kSteps], g[kSteps];
   float delta = 0.f;
 #pragma unroll
@@ -535,26 +507,15 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
     f.deltas[at] = delta;
     f.logs[at]   = log;
   }
-  TileLoader<T, D, WAVES> load_k, load_v;
-  load_k.aim(f.k, first + first_tile * kTile, w.kv_head, f.width, wave, lane);
-  load_v.aim(f.v, first + first_tile * kTile, w.kv_head, f.width, wave, lane);
-  TileReader<T, D> const read(lane);
-  float const scale = f.scale * kLog2e;
   f32x16_t d[kColumns];
 #pragma unroll
   for (int c = 0; c < kColumns; ++c) d[c] = f32x16_t{};
-  if (tiles > first_tile) {
-    load_k.load(lds + (first_tile & 1) * Shape::kStage, keys - first_tile * kTile, wave);
-    load_v.load(lds + (first_tile & 1) * Shape::kStage + Tile<T, D>::kBytes, keys - first_tile * kTile, wave);
-  }
+  TileReader<T, D> const read(lane);
+  float const scale = f.scale * kLog2e;
   for (int32_t tile = first_tile; tile < tiles; ++tile) {
     LdsBytes const k_tile = lds + (tile & 1) * Shape::kStage, v_tile = k_tile + Tile<T, D>::kBytes;
     stage_barrier<0>();
-    if (tile + 1 < tiles) {
-      LdsBytes const next = lds + (~tile & 1) * Shape::kStage;
-      load_k.load(next, keys - (tile + 1) * kTile, wave);
-      load_v.load(next + Tile<T, D>::kBytes, keys - (tile + 1) * kTile, wave);
-    }
+    if (tile + 1 < tiles) load(tile + 1);
     int32_t const key0 = tile * kTile;
     if (key0 >= most) continue;
     // Of each block of 32 keys, scores and products of g and v, then what they come to, multiplied with the keys: a stream of fragments, read kAhead before
@@ -582,8 +543,9 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], scale, -log)) * (p[r] - delta);
             if (key0 + 32 * b + 32 > least) {
+              int32_t const left = seen - key0 - 32 * b - 4 * half;
 #pragma unroll
-              for (int r = 0; r < 16; ++r) s[r] = key0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4 < seen ? s[r] : 0.f;
+              for (int r = 0; r < 16; ++r) s[r] = 8 * (r / 4) + r % 4 < left ? s[r] : 0.f;
             }
             ds[0] = rounded<T>(s, 0);
             ds[1] = rounded<T>(s, 1);
@@ -597,39 +559,35 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
     if (there) store_columns<float, kColumns>(split.sums + (split.slot(w.block, w.head, f.heads, w.share) * Shape::kRows + wave0 + column) * D, d, half, D);
     return;
   }
-  bool finite = true;
+  float check = 0.f;
 #pragma unroll
   for (int c = 0; c < kColumns; ++c)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       d[c][r] *= f.scale;
-      finite = finite && fabsf(d[c][r]) < INFINITY;
+      check = fmaf(d[c][r], 0.f, check);
     }
   // (as forward: a key that is not seen may have been multiplied by 0)
-  uint64_t odd = __ballot(there && seen > 0 && !finite);
+  uint64_t odd = __ballot(there && seen > 0 && check != 0.f);
   odd          = (odd | odd >> 32) & 0xffffffffu;
   if (there && !(odd >> column & 1)) store_columns<T, kColumns>(f.q_grad.at(t, w.head), d, half, f.width);
-  while (odd) {
-    int const which = __builtin_ctzll(odd);
-    odd &= odd - 1;
-    query_gradient_row(f, begin + block0 + wave0 + which, w.head);
-  }
+  for (; odd; odd &= odd - 1) query_gradient_row(f, begin + block0 + wave0 + __builtin_ctzll(odd), w.head);
 }
 
-// The gradients of k and v: a wavefront has 32 * NK keys in its registers, a lane a key's scores, and the tokens of all heads that see them come through LDS
+// The gradients of k and v: a wavefront has 32 keys in its registers, a lane a key's scores, and the tokens of all heads that see them come through LDS
 // with their gradients, 64 at a time, with their logs and deltas.
-template <typename T, int D, int WAVES, int NK>
+template <typename T, int D, int WAVES>
 struct KeyShape {
-  static constexpr int kRows = 32 * WAVES * NK, kShift = __builtin_ctz(kRows), kTile = Tile<T, D>::kHeads, kTiles = 2 * Tile<T, D>::kBytes;
+  static constexpr int kRows = 32 * WAVES, kShift = __builtin_ctz(kRows), kTile = Tile<T, D>::kHeads, kTiles = 2 * Tile<T, D>::kBytes;
   static constexpr int kStage = kTiles + 2 * kWave * 4, kLds = 2 * kStage;  // (with logs and deltas)
-  static constexpr int kWavesASimd = sizeof(T) == 2 && D * NK <= 128 ? 2 : 1;
+  static constexpr int kWavesASimd = sizeof(T) == 2 && D <= 128 ? 2 : 1;
 };
 // PART: the gradients of both, or of k or v alone (of wide heads there are not the registers for both).
 enum Part { kBoth, kOfK, kOfV };
-template <typename T, int D, int WAVES, int NK, Part PART>
-__global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES, NK>::kWavesASimd)) key_gradient_tiles_kernel(Backward<T> f, Split split)
+template <typename T, int D, int WAVES, Part PART>
+__global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES>::kWavesASimd)) key_gradient_tiles_kernel(Backward<T> f, Split split)
 {
-  using Shape = KeyShape<T, D, WAVES, NK>;
+  using Shape = KeyShape<T, D, WAVES>;
   extern __shared__ __align__(16) char lds_[];
   LdsBytes const lds = (LdsBytes)lds_;
   constexpr bool kK = PART != kOfV, kV = PART != kOfK;
@@ -652,7 +610,9 @@ __global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES, NK>::kWa
   begin  = uniform(begin);
   tokens = uniform(tokens > 0 ? tokens : 0);
   keys   = uniform(keys);
-  int32_t const wave0 = wave * 32 * NK;
+  int32_t const wave0 = wave * 32, key = block0 + wave0 + column;
+  bool const there    = wave0 + column < rest;
+  int64_t const t     = static_cast<int64_t>(first) + (there ? key : block0);
   // the first token that sees a key, of the row's
   auto const from_of = [&](int32_t j) {
     int64_t const i = f.causal ? static_cast<int64_t>(j) + tokens - keys : 0;
@@ -663,32 +623,23 @@ __global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES, NK>::kWa
   int32_t const of_head = tiles - start > 0 ? tiles - start : 0, total = of_head * each, shares = shares_of(total, split.splits);
   if (w.share >= shares) return;
   int32_t const begin_tile = uniform(share_begin(total, w.share, shares)), end_tile = uniform(share_begin(total, w.share + 1, shares));
-  int32_t const last_from = uniform(from_of(block0 + wave0 + 32 * NK - 1)), first_from = uniform(from_of(block0 + wave0));
+  int32_t const last_from = uniform(from_of(block0 + wave0 + 31)), first_from = uniform(from_of(block0 + wave0));
 
-  Fragment<T> k[NK][kSteps], v[NK][kK ? kSteps : 1];
-  int32_t from[NK];
+  Fragment<T> k[kSteps], v[kK ? kSteps : 1];
+  int32_t const from = from_of(key);
 #pragma unroll
-  for (int n = 0; n < NK; ++n) {
-    int32_t const i  = wave0 + 32 * n + column, key = block0 + i;
-    bool const there = i < rest && key < keys;
-    int64_t const t  = static_cast<int64_t>(first) + (there ? key : block0);
-    from[n]          = from_of(key);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      k[n][s] = fragment_of(f.k.at(t, w.kv_head), 16 * s + 8 * half, f.width, there);
-      if constexpr (kK) v[n][s] = fragment_of(f.v.at(t, w.kv_head), 16 * s + 8 * half, f.width, there);
-    }
+  for (int s = 0; s < kSteps; ++s) {
+    k[s] = fragment_of(f.k.at(t, w.kv_head), 16 * s + 8 * half, f.width, there && key < keys);
+    if constexpr (kK) v[s] = fragment_of(f.v.at(t, w.kv_head), 16 * s + 8 * half, f.width, there && key < keys);
   }
   TileReader<T, D> const read(lane);
   float const scale = f.scale * kLog2e;
-  f32x16_t dk[NK][kK ? kColumns : 1], dv[NK][kV ? kColumns : 1];
+  f32x16_t dk[kK ? kColumns : 1], dv[kV ? kColumns : 1];
 #pragma unroll
-  for (int n = 0; n < NK; ++n)
-#pragma unroll
-    for (int c = 0; c < kColumns; ++c) {
-      if constexpr (kK) dk[n][c] = f32x16_t{};
-      if constexpr (kV) dv[n][c] = f32x16_t{};
-    }
+  for (int c = 0; c < kColumns; ++c) {
+    if constexpr (kK) dk[c] = f32x16_t{};
+    if constexpr (kV) dv[c] = f32x16_t{};
+  }
   TileLoader<T, D, WAVES> load_q, load_g;
   int32_t loaded = uniform(of_head > 0 ? begin_tile % of_head : 0), next_head = uniform(w.kv_head * each + (of_head > 0 ? begin_tile / of_head : 0));  // the tile of the head that is loaded next
   bool aimed = false;
@@ -721,8 +672,8 @@ __global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES, NK>::kWa
     if (token0 + kTile <= first_from) continue;
     // (as in the gradient of q: a stream of fragments)
     constexpr int kFirst = (kK ? 2 : 1) * kSteps, kOfBlock = kFirst + 2 * (kK && kV ? 2 : 1) * kColumns;
-    f32x16_t s[NK], p[NK];
-    Fragment<T> weight[NK][2], ds[NK][2];
+    f32x16_t s, p;
+    Fragment<T> weight[2], ds[2];
     stream<T, kBlocks * kOfBlock>(
       [&](auto slot) {
         constexpr int b = slot / kOfBlock, i = slot % kOfBlock;
@@ -737,17 +688,11 @@ __global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES, NK>::kWa
       [&](auto slot, Fragment<T> const& x) {
         constexpr int b = slot / kOfBlock, i = slot % kOfBlock;
         if constexpr (i < kSteps) {
-#pragma unroll
-          for (int n = 0; n < NK; ++n) {
-            if constexpr (i == 0) s[n] = f32x16_t{};
-            s[n] = multiply32(x, k[n][i], s[n]);
-          }
+          if constexpr (i == 0) s = f32x16_t{};
+          s = multiply32(x, k[i], s);
         } else if constexpr (i < kFirst) {
-#pragma unroll
-          for (int n = 0; n < NK; ++n) {
-            if constexpr (i == kSteps) p[n] = f32x16_t{};
-            p[n] = multiply32(x, v[n][i - kSteps], p[n]);
-          }
+          if constexpr (i == kSteps) p = f32x16_t{};
+          p = multiply32(x, v[i - kSteps], p);
         } else {
           if constexpr (i == kFirst) {
             int32_t const row0 = token0 + 32 * b;
@@ -758,86 +703,66 @@ __global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES, NK>::kWa
               f32x4_t delta{};
               if constexpr (kK) delta = *reinterpret_cast<__attribute__((address_space(3))) f32x4_t*>(words + kWave * 4 + 128 * b + 32 * j);
 #pragma unroll
-              for (int n = 0; n < NK; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  int const r = 4 * j + e;
-                  s[n][r]     = __builtin_amdgcn_exp2f(fmaf(s[n][r], scale, -log[e]));
-                  if constexpr (kK) p[n][r] = s[n][r] * (p[n][r] - delta[e]);
-                }
+              for (int e = 0; e < 4; ++e) {
+                int const r = 4 * j + e;
+                s[r]        = __builtin_amdgcn_exp2f(fmaf(s[r], scale, -log[e]));
+                if constexpr (kK) p[r] = s[r] * (p[r] - delta[e]);
+              }
             }
             if (partly) {
 #pragma unroll
-              for (int n = 0; n < NK; ++n)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                  int32_t const t = row0 + 8 * (r / 4) + 4 * half + r % 4;
-                  bool const sees = t >= from[n] && t < tokens;
-                  if constexpr (kV) s[n][r] = sees ? s[n][r] : 0.f;
-                  if constexpr (kK) p[n][r] = sees ? p[n][r] : 0.f;
-                }
+              for (int r = 0; r < 16; ++r) {
+                int32_t const token = row0 + 8 * (r / 4) + 4 * half + r % 4;
+                bool const sees     = token >= from && token < tokens;
+                if constexpr (kV) s[r] = sees ? s[r] : 0.f;
+                if constexpr (kK) p[r] = sees ? p[r] : 0.f;
+              }
             }
 #pragma unroll
-            for (int n = 0; n < NK; ++n)
-#pragma unroll
-              for (int step = 0; step < 2; ++step) {
-                if constexpr (kV) weight[n][step] = rounded<T>(s[n], step);
-                if constexpr (kK) ds[n][step] = rounded<T>(p[n], step);
-              }
+            for (int step = 0; step < 2; ++step) {
+              if constexpr (kV) weight[step] = rounded<T>(s, step);
+              if constexpr (kK) ds[step] = rounded<T>(p, step);
+            }
           }
           constexpr int j = i - kFirst, step = j / ((kK && kV ? 2 : 1) * kColumns), c = j % ((kK && kV ? 2 : 1) * kColumns);
-#pragma unroll
-          for (int n = 0; n < NK; ++n) {
-            if constexpr (kV && c < kColumns) dv[n][c] = multiply32(x, weight[n][step], dv[n][c]);
-            else dk[n][c % kColumns] = multiply32(x, ds[n][step], dk[n][c % kColumns]);
-          }
+          if constexpr (kV && c < kColumns) dv[c] = multiply32(x, weight[step], dv[c]);
+          else dk[c % kColumns] = multiply32(x, ds[step], dk[c % kColumns]);
         }
       });
   }
   if (shares > 1) {
-#pragma unroll
-    for (int n = 0; n < NK; ++n) {
-      int32_t const i = wave0 + 32 * n + column;
-      float* const part = split.sums + (split.slot(w.block, w.kv_head, f.kv_heads, w.share) * Shape::kRows + i) * (2 * D);
-      if (i >= rest) continue;
-      if constexpr (kK) store_columns<float, kColumns>(part, dk[n], half, D);
-      if constexpr (kV) store_columns<float, kColumns>(part + D, dv[n], half, D);
-      if (block0 + i >= keys && w.share == 0) {  // (which is no key: nothing is joined for it)
-        f32x16_t const zeros[kColumns] = {};
-        int64_t const t                = static_cast<int64_t>(first) + block0 + i;
-        if constexpr (kK) store_columns<T, kColumns>(f.k_grad.at(t, w.kv_head), zeros, half, f.width);
-        if constexpr (kV) store_columns<T, kColumns>(f.v_grad.at(t, w.kv_head), zeros, half, f.width);
-      }
+    if (!there) return;
+    float* const part = split.sums + (split.slot(w.block, w.kv_head, f.kv_heads, w.share) * Shape::kRows + wave0 + column) * (2 * D);
+    if constexpr (kK) store_columns<float, kColumns>(part, dk, half, D);
+    if constexpr (kV) store_columns<float, kColumns>(part + D, dv, half, D);
+    if (key >= keys && w.share == 0) {  // (which is no key: nothing is joined for it)
+      f32x16_t const zeros[kColumns] = {};
+      if constexpr (kK) store_columns<T, kColumns>(f.k_grad.at(t, w.kv_head), zeros, half, f.width);
+      if constexpr (kV) store_columns<T, kColumns>(f.v_grad.at(t, w.kv_head), zeros, half, f.width);
     }
     return;
   }
+  float check = 0.f;
 #pragma unroll
-  for (int n = 0; n < NK; ++n) {
-    int32_t const i  = wave0 + 32 * n + column, key = block0 + i;
-    bool const there = i < rest;
-    int64_t const t  = static_cast<int64_t>(first) + (there ? key : block0);
-    bool finite      = true;
+  for (int c = 0; c < kColumns; ++c)
 #pragma unroll
-    for (int c = 0; c < kColumns; ++c)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        if constexpr (kK) {
-          dk[n][c][r] = key < keys ? dk[n][c][r] * f.scale : 0.f;
-          finite      = finite && fabsf(dk[n][c][r]) < INFINITY;
-        }
-        if constexpr (kV) {
-          dv[n][c][r] = key < keys ? dv[n][c][r] : 0.f;
-          finite      = finite && fabsf(dv[n][c][r]) < INFINITY;
-        }
+    for (int r = 0; r < 16; ++r) {
+      if constexpr (kK) {
+        dk[c][r] = key < keys ? dk[c][r] * f.scale : 0.f;
+        check    = fmaf(dk[c][r], 0.f, check);
       }
-    uint64_t odd = __ballot(there && !finite);
-    odd          = (odd | odd >> 32) & 0xffffffffu;
-    if (there && !(odd >> column & 1)) {
-      if constexpr (kK) store_columns<T, kColumns>(f.k_grad.at(t, w.kv_head), dk[n], half, f.width);
-      if constexpr (kV) store_columns<T, kColumns>(f.v_grad.at(t, w.kv_head), dv[n], half, f.width);
+      if constexpr (kV) {
+        dv[c][r] = key < keys ? dv[c][r] : 0.f;
+        check    = fmaf(dv[c][r], 0.f, check);
+      }
     }
-    for (; odd; odd &= odd - 1) key_gradient_row(f, first + block0 + wave0 + 32 * n + __builtin_ctzll(odd), w.kv_head, kK, kV);
+  uint64_t odd = __ballot(there && check != 0.f);
+  odd          = (odd | odd >> 32) & 0xffffffffu;
+  if (there && !(odd >> column & 1)) {
+    if constexpr (kK) store_columns<T, kColumns>(f.k_grad.at(t, w.kv_head), dk, half, f.width);
+    if constexpr (kV) store_columns<T, kColumns>(f.v_grad.at(t, w.kv_head), dv, half, f.width);
   }
+  for (; odd; odd &= odd - 1) key_gradient_row(f, first + block0 + wave0 + __builtin_ctzll(odd), w.kv_head, kK, kV);
 }
 
 // Adds up the shares of a head of a token (of q) or a key, a wavefront for each; the numbers of shares are those that the kernels before found.
@@ -1020,10 +945,10 @@ Estimate estimate(Problem<T> const& p, Runs const& blocks, int32_t heads, int sh
   return {rows * ((length + (1 << shift) - 1) >> shift) * heads, (p.causal && other.tokens <= blocks.tokens ? (tiles + 1) / 2 : tiles) * times};
 }
 
-template <typename T, int D, int WAVES, int NQ>
+template <typename T, int D>
 nvtext_amd_status attend_tiles(Forward<T> const& f, Mr const& mr, hipStream_t stream)
 {
-  using Shape      = ForwardShape<T, D, WAVES, NQ>;
+  using Shape      = ForwardShape<T, D, kTileWaves>;
   Estimate const e = estimate(f, f.runs, f.heads, Shape::kShift, f.key_runs, Shape::kTile, 1);
   Split split{splits_of(e.workgroups, e.tiles), nullptr, nullptr};
   size_t const rows = split.splits > 1 ? static_cast<size_t>(f.runs.blocks(Shape::kShift) * f.heads * split.splits) << Shape::kShift : 0;
@@ -1031,17 +956,16 @@ nvtext_amd_status attend_tiles(Forward<T> const& f, Mr const& mr, hipStream_t st
   if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
   split.sums = temp.template part<float>(0);
   split.tops = temp.template part<float2>(1);
-  NVTEXT_HIP_TRY(allow_lds(attend_tiles_kernel<T, D, WAVES, NQ>, Shape::kLds));
+  NVTEXT_HIP_TRY(allow_lds(attend_tiles_kernel<T, D, kTileWaves>, Shape::kLds));
   {
     ProfileScope const scope("attention_tiles", stream);
     int64_t const items = work_items(f.runs.blocks(Shape::kShift), f.kv_heads, f.heads / f.kv_heads, split.splits);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_tiles_kernel<T, D, WAVES, NQ>), grid_of(items, WAVES * kWave), dim3(WAVES * kWave), Shape::kLds, stream, f, split);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_tiles_kernel<T, D, kTileWaves>), grid_of(items, kTileWaves * kWave), dim3(kTileWaves * kWave), Shape::kLds, stream, f, split);
   }
-  if (split.splits > 1) {
-    ProfileScope const scope("attention_join", stream);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_join_shares_kernel<T, D>), grid_of((static_cast<int64_t>(f.runs.tokens) * f.heads + 3) / 4, kThreads), dim3(kThreads), 0, stream, f, split,
-                       int{Shape::kShift});
-  }
+  if (split.splits == 1) return NVTEXT_AMD_SUCCESS;
+  ProfileScope const scope("attention_join", stream);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_join_shares_kernel<T, D>), grid_of((static_cast<int64_t>(f.runs.tokens) * f.heads + 3) / 4, kThreads), dim3(kThreads), 0, stream, f, split,
+                     int{Shape::kShift});
   return NVTEXT_AMD_SUCCESS;
 }
 
@@ -1085,27 +1009,26 @@ nvtext_amd_status attention(Forward<T> f, Mr const& mr, hipStream_t stream)
     if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
     align.launch(temp.template part<char>(0), stream);
     if (chunks) return attend_chunks<T, kD>({f, shift, temp.template part<float>(1), temp.template part<float2>(2)}, stream);
-    return attend_tiles<T, kD, 4, 1>(f, mr, stream);
+    return attend_tiles<T, kD>(f, mr, stream);
   });
 }
 
-template <typename T, int D, int WAVES, int NK, Part PART>
+template <typename T, int D, Part PART>
 nvtext_amd_status key_gradient_tiles(Backward<T> const& f, Split const& split, hipStream_t stream)
 {
-  using Shape = KeyShape<T, D, WAVES, NK>;
+  using Shape = KeyShape<T, D, kTileWaves>;
   ProfileScope const scope("attention_key_gradient", stream);
-  NVTEXT_HIP_TRY(allow_lds(key_gradient_tiles_kernel<T, D, WAVES, NK, PART>, Shape::kLds));
+  NVTEXT_HIP_TRY(allow_lds(key_gradient_tiles_kernel<T, D, kTileWaves, PART>, Shape::kLds));
   int64_t const items = work_items(f.key_runs.blocks(Shape::kShift), f.kv_heads, 1, split.splits);
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(key_gradient_tiles_kernel<T, D, WAVES, NK, PART>), grid_of(items, WAVES * kWave), dim3(WAVES * kWave), Shape::kLds, stream, f, split);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(key_gradient_tiles_kernel<T, D, kTileWaves, PART>), grid_of(items, kTileWaves * kWave), dim3(kTileWaves * kWave), Shape::kLds, stream, f, split);
   return NVTEXT_AMD_SUCCESS;
 }
 
 template <typename T, int D>
 nvtext_amd_status gradient_tiles(Backward<T> const& f, Mr const& mr, hipStream_t stream)
 {
-  constexpr int kWaves = 4;
-  using OfQ            = GradientShape<T, D, kWaves>;
-  using OfK            = KeyShape<T, D, kWaves, 1>;
+  using OfQ        = GradientShape<T, D, kTileWaves>;
+  using OfK        = KeyShape<T, D, kTileWaves>;
   Estimate const q = estimate(f, f.runs, f.heads, OfQ::kShift, f.key_runs, OfQ::kTile, 1), k = estimate(f, f.key_runs, f.kv_heads, OfK::kShift, f.runs, OfK::kTile, f.heads / f.kv_heads);
   Split of_q{f.runs.tokens > 0 ? splits_of(q.workgroups, q.tiles) : 1, nullptr, nullptr}, of_k{f.key_runs.tokens > 0 ? splits_of(k.workgroups, k.tiles) : 1, nullptr, nullptr};
   TempParts<2> const temp(mr, {of_q.splits > 1 ? static_cast<size_t>(f.runs.blocks(OfQ::kShift) * f.heads * of_q.splits * OfQ::kRows * D) * sizeof(float) : 0,
@@ -1115,9 +1038,9 @@ nvtext_amd_status gradient_tiles(Backward<T> const& f, Mr const& mr, hipStream_t
   of_k.sums = temp.template part<float>(1);
   if (f.runs.tokens > 0) {
     ProfileScope const scope("attention_query_gradient", stream);
-    NVTEXT_HIP_TRY(allow_lds(query_gradient_tiles_kernel<T, D, kWaves>, OfQ::kLds));
+    NVTEXT_HIP_TRY(allow_lds(query_gradient_tiles_kernel<T, D, kTileWaves>, OfQ::kLds));
     int64_t const items = work_items(f.runs.blocks(OfQ::kShift), f.kv_heads, f.heads / f.kv_heads, of_q.splits);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(query_gradient_tiles_kernel<T, D, kWaves>), grid_of(items, kWaves * kWave), dim3(kWaves * kWave), OfQ::kLds, stream, f, of_q);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(query_gradient_tiles_kernel<T, D, kTileWaves>), grid_of(items, kTileWaves * kWave), dim3(kTileWaves * kWave), OfQ::kLds, stream, f, of_q);
   }
   if (of_q.splits > 1) {
     ProfileScope const scope("attention_query_gradient_join", stream);
@@ -1126,11 +1049,11 @@ nvtext_amd_status gradient_tiles(Backward<T> const& f, Mr const& mr, hipStream_t
   }
   if (f.key_runs.tokens == 0) return NVTEXT_AMD_SUCCESS;
   nvtext_amd_status st;
-  if constexpr (D * sizeof(T) > 128 && (sizeof(T) == 2 || D > 128)) {
-    st = key_gradient_tiles<T, D, kWaves, 1, kOfK>(f, of_k, stream);
-    if (st == NVTEXT_AMD_SUCCESS) st = key_gradient_tiles<T, D, kWaves, 1, kOfV>(f, of_k, stream);
+  if constexpr (D > 64) {
+    st = key_gradient_tiles<T, D, kOfK>(f, of_k, stream);
+    if (st == NVTEXT_AMD_SUCCESS) st = key_gradient_tiles<T, D, kOfV>(f, of_k, stream);
   } else {
-    st = key_gradient_tiles<T, D, kWaves, 1, kBoth>(f, of_k, stream);
+    st = key_gradient_tiles<T, D, kBoth>(f, of_k, stream);
   }
   if (st != NVTEXT_AMD_SUCCESS || of_k.splits == 1) return st;
   ProfileScope const scope("attention_key_gradient_join", stream);
