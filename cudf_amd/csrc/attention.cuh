@@ -4,6 +4,8 @@
 #include "heads.cuh"
 #include "matrix.cuh"
 
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace nvtext_amd {
@@ -259,12 +261,13 @@ __device__ __forceinline__ f32x16_t multiply32(Fragment<float> a, Fragment<float
 // on (columns of 32-bit types).
 template <typename T, int D>
 struct Tile {
+  static_assert(D % 32 == 0 && D <= kMostWidth);
   static constexpr int kHeads = D * sizeof(T) > 512 ? 32 : 64;  // two tiles of each, twice, fill no more than 128 KB
   static constexpr int kLine = D * sizeof(T), kBytes = kHeads * kLine, kPieces = kLine / 16;  // bytes of a head, of all, pieces of 16 bytes of a head
   __device__ __forceinline__ static constexpr uint32_t turn(uint32_t head)
   {
     uint32_t const last = head >> 3 & 1, third = head >> 2 & 1;
-    if constexpr (sizeof(T) == 4) return third << 3 | (head & 3) << 1 | last;
+    if constexpr (sizeof(T) == 4) return (kPieces % 16 == 0 ? third << 3 : 0) | (head & 3) << 1 | last;  // (no piece leaves its head)
     if constexpr (kLine % 256 == 0) return (head & 3) << 2 | third << 1 | last;
     if constexpr (kLine % 128 == 0) return (head & 2) << 1 | third << 1 | last;  // (neighbouring heads begin 128 bytes apart)
     return third << 1 | last;                                                   // (they begin 64 bytes apart, in some order)
@@ -472,6 +475,228 @@ __device__ __forceinline__ void store_rests(int8_t* head, f32x16_t const (&x)[CO
     typedef uint32_t Words __attribute__((ext_vector_type(1)));
     return Words{four};
   });
+}
+
+// ------------------------------------------------------------------ work
+constexpr int kThreads = 256;
+constexpr int kTileWaves = 4;  // wavefronts that share the tiles in LDS
+
+// The work of a launch: blocks of tokens, of every head, in `splits` shares.  The heads that share a key head come one after the other on one XCD (workgroups go
+// to the eight XCDs in turn), and so do, where the number of key heads allows, the blocks of a key head: its keys come from that XCD's L2.  The last
+// blocks come first: of a long row they are those with the most keys to see.
+struct Work {
+  int64_t block;
+  int32_t kv_head, head, share;
+};
+constexpr int kXcds = 8;
+inline int64_t work_items(int64_t blocks, int32_t kv_heads, int32_t each, int32_t splits) { return (blocks * kv_heads + kXcds - 1) / kXcds * kXcds * each * splits; }
+// false: nothing to do
+template <typename Int>
+__device__ __forceinline__ bool work_in(Int item, Int blocks, int32_t kv_heads, int32_t each, int32_t splits, Work& w)
+{
+  Int const n = item / kXcds / static_cast<Int>(splits), units = n / static_cast<Int>(each), unit = units * kXcds + item % kXcds;
+  if (unit >= blocks * static_cast<Int>(kv_heads)) return false;
+  Int const behind = unit / static_cast<Int>(kv_heads);
+  w.block          = static_cast<int64_t>(blocks - 1 - behind);
+  w.kv_head        = static_cast<int32_t>(unit - behind * static_cast<Int>(kv_heads));
+  w.head           = w.kv_head * each + static_cast<int32_t>(n - units * static_cast<Int>(each));
+  w.share          = static_cast<int32_t>(item / kXcds - n * static_cast<Int>(splits));
+  return true;
+}
+__device__ __forceinline__ bool work_of(int64_t item, int64_t blocks, int32_t kv_heads, int32_t each, int32_t splits, Work& w)
+{
+  // (divisions of 64 bits take a hundred instructions each)
+  if (blocks * kv_heads < (int64_t{1} << 32) - kXcds && item < int64_t{1} << 32) return work_in<uint32_t>(item, blocks, kv_heads, each, splits, w);
+  return work_in<uint64_t>(item, blocks, kv_heads, each, splits, w);
+}
+
+// Where there are few workgroups, each one's tiles are shared by up to `splits`, which leave what they add up in memory, [block][head][share][row][D] in
+// float32, for another launch to join.  A share has at least kLeastTiles: in how many shares `tiles` go, and what one of them has.
+constexpr int kLeastTiles = 2;
+__device__ __forceinline__ int32_t shares_of(int32_t tiles, int32_t splits) { return splits == 1 || tiles < 2 * kLeastTiles ? 1 : min(splits, tiles / kLeastTiles); }
+__device__ __forceinline__ int32_t share_begin(int32_t tiles, int32_t share, int32_t shares) { return static_cast<int32_t>(static_cast<int64_t>(tiles) * share / shares); }
+
+struct Split {
+  int32_t splits;
+  float* sums;
+  float2* tops;  // (forward) [block][head][share][row]: top, and the sum of the exponentials
+  __device__ __forceinline__ int64_t slot(int64_t block, int32_t head, int32_t heads, int32_t share) const { return (block * heads + head) * splits + share; }
+};
+
+// A lane's part of a row of D values that a wavefront holds side by side: values first() .. first() + kEach - 1, of the lanes that have any.
+template <int D>
+struct Some {
+  static constexpr int kEach = (D + kWave - 1) / kWave;
+  float v[kEach] = {};
+  __device__ __forceinline__ static int first() { return lane_id() * kEach; }
+  __device__ __forceinline__ void add(const float* row, float weight)
+  {
+    if (first() < D) {
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) v[k] = fmaf(row[first() + k], weight, v[k]);
+    }
+  }
+  // whether the first `width` values of the row are all finite
+  __device__ __forceinline__ bool finite(int32_t width) const
+  {
+    float check = 0.f;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) check = first() + k < width ? fmaf(v[k], 0.f, check) : check;
+    return __ballot(check != 0.f) == 0;
+  }
+};
+
+// ------------------------------------------------------------------ launches
+// Whether the tiles' loads can read heads as they lie: pieces of 16 bytes, and lines of a tile within the 31 bits of their offsets.
+template <typename T>
+bool reads_as_it_lies(Heads<const T> const& x, int32_t width)
+{
+  constexpr int kEach = 16 / sizeof(T);
+  return width % kEach == 0 && x.stride % kEach == 0 && x.head_stride % kEach == 0 && reinterpret_cast<uintptr_t>(x.data) % 16 == 0 && x.stride < (int64_t{1} << 23);
+}
+
+// Heads that the tiles cannot read are copied first: head after head, token after token, each filled up with zeros to a multiple of 16 bytes.
+template <typename T>
+struct Copy {
+  static constexpr int kEach = 16 / sizeof(T);
+  Heads<const T> from;
+  T* to;
+  int64_t tokens, pieces;  // of all heads; 0: nothing to copy
+};
+constexpr int kCopies = 5;
+template <typename T>
+struct Copies {
+  Copy<T> copy[kCopies];
+  int32_t width;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) copy_heads_kernel(Copies<T> c)
+{
+  constexpr int kEach   = Copy<T>::kEach;
+  int64_t item          = block_number() * kThreads + threadIdx.x;
+  int32_t const of_head = (c.width + kEach - 1) / kEach;
+#pragma unroll
+  for (int n = 0; n < kCopies; ++n) {
+    Copy<T> const& x = c.copy[n];
+    if (item >= 0 && item < x.pieces) {
+      int64_t const head = item / of_head / x.tokens, t = item / of_head % x.tokens, j = item % of_head * kEach;
+      const T* const from = x.from.at(t, head) + j;
+      typedef T Piece __attribute__((ext_vector_type(kEach)));
+      Piece p{};
+#pragma unroll
+      for (int k = 0; k < kEach; ++k)
+        if (j + k < c.width) p[k] = from[k];
+      *reinterpret_cast<Piece*>(x.to + item * kEach) = p;
+    }
+    item -= x.pieces;
+  }
+}
+
+// Which of up to five heads are copied, what that takes, and the launch that does it.
+template <typename T>
+struct Alignment {
+  Copies<T> copies{};
+  Heads<const T>* heads[kCopies]{};
+  int count{0};
+  explicit Alignment(int32_t width) { copies.width = width; }
+  void add(Heads<const T>& x, int64_t tokens, int64_t of_token)
+  {
+    heads[count]  = &x;
+    Copy<T>& c    = copies.copy[count++];
+    c.from        = x;
+    c.tokens      = tokens;
+    c.pieces      = reads_as_it_lies(x, copies.width) ? 0 : tokens * of_token * ((copies.width + Copy<T>::kEach - 1) / Copy<T>::kEach);
+  }
+  size_t bytes() const
+  {
+    size_t sum = 0;
+    for (auto const& c : copies.copy) sum += static_cast<size_t>(c.pieces) * 16;
+    return sum;
+  }
+  void launch(char* memory, hipStream_t stream)
+  {
+    int64_t all = 0;
+    for (int n = 0; n < count; ++n) {
+      Copy<T>& c = copies.copy[n];
+      if (c.pieces == 0) continue;
+      int64_t const line = (copies.width + Copy<T>::kEach - 1) / Copy<T>::kEach * Copy<T>::kEach;
+      c.to               = reinterpret_cast<T*>(memory);
+      *heads[n]          = {c.to, line, c.tokens * line};
+      memory += c.pieces * 16;
+      all += c.pieces;
+    }
+    if (all == 0) return;
+    ProfileScope const scope("attention_copy", stream);
+    hipLaunchKernelGGL(copy_heads_kernel<T>, grid_of((all + kThreads - 1) / kThreads, kThreads), dim3(kThreads), 0, stream, copies);
+  }
+};
+
+// (where kernels take more than 64 KB of LDS, the runtime wants to be told)
+template <typename Kernel>
+hipError_t allow_lds(Kernel kernel, int bytes)
+{
+  return bytes > 65536 ? hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) : hipSuccess;
+}
+
+// In how many shares the tiles of a workgroup go: so many that there are twice as many workgroups as run at once, two a CU, if that many have kLeastTiles
+// tiles on average; and none where there are that many workgroups, or tiles take no longer than another launch.
+inline int32_t splits_of(int64_t workgroups, int64_t tiles)
+{
+  int64_t const at_once = 2 * device_cus();
+  if (workgroups >= at_once || workgroups <= 0 || tiles < 3 * kLeastTiles) return 1;
+  return static_cast<int32_t>(std::min<int64_t>({(2 * at_once + workgroups - 1) / workgroups, tiles / kLeastTiles, 16}));
+}
+
+// Workgroups with something to do, and what they have, as far as the host knows: rows are taken to be alike.
+struct Estimate {
+  int64_t workgroups, tiles;
+};
+template <typename T>
+Estimate estimate(Problem<T> const& p, Runs const& blocks, int32_t heads, int shift, Runs const& other, int tile, int64_t times)
+{
+  int64_t const rows = std::max(1, blocks.rows), length = (blocks.tokens + rows - 1) / rows;
+  int64_t const seen = (other.tokens + rows - 1) / rows, tiles = (seen + tile - 1) / tile;
+  // (causal, with as many tokens as keys: half of them on average)
+  return {rows * ((length + (1 << shift) - 1) >> shift) * heads, (p.causal && other.tokens <= blocks.tokens ? (tiles + 1) / 2 : tiles) * times};
+}
+
+// calls f with the width of the tiles that heads of `width` values go through
+template <typename F>
+nvtext_amd_status with_tiles(int32_t width, F&& f)
+{
+  if (width <= 64) return f(std::integral_constant<int, 64>{});
+  if (width <= 96) return f(std::integral_constant<int, 96>{});
+  if (width <= 128) return f(std::integral_constant<int, 128>{});
+  if (width <= 192) return f(std::integral_constant<int, 192>{});
+  return f(std::integral_constant<int, 256>{});
+}
+
+// What both directions ask of their arguments; nullptr if it holds.
+inline const char* bad_attention(const nvtext_amd_heads* q, const nvtext_amd_heads* k, const nvtext_amd_heads* v, int32_t rows, const int32_t* offsets, const int32_t* key_offsets,
+                          const int32_t* key_lengths, double scale)
+{
+  for (auto* x : {q, k, v})
+    if (const char* bad = bad_heads(x)) return bad;
+  if (k->type != q->type || v->type != q->type) return "q, k and v must be of one type";
+  if (!is_like(v, k)) return "v must be of k's size";
+  if (k->width != q->width) return "k and v must be of q's width";
+  if (q->width > kMostWidth) return "heads may have 256 values at most";
+  if (q->heads > 0 ? k->heads == 0 || q->heads % k->heads != 0 : k->heads != 0) return "the heads of k and v must be a divisor of q's";
+  if (const char* bad = bad_rows(rows, offsets)) return bad;
+  if (key_lengths && !key_offsets) return "key_lengths need key_offsets";
+  if (!key_offsets && k->tokens != q->tokens) return "without offsets of their own, k and v must have q's tokens";
+  if (!(scale >= 0) || !std::isfinite(static_cast<float>(scale))) return "scale must be finite and not negative";
+  return nullptr;
+}
+
+template <typename T>
+Problem<T> problem_of(const nvtext_amd_heads* q, const nvtext_amd_heads* k, const nvtext_amd_heads* v, int32_t rows, const int32_t* offsets, const int32_t* key_offsets,
+                      const int32_t* key_lengths, int32_t causal, double scale)
+{
+  return {heads_of<const T>(q), heads_of<const T>(k), heads_of<const T>(v), static_cast<int32_t>(q->heads), static_cast<int32_t>(k->heads), static_cast<int32_t>(q->width),
+          Runs{offsets, rows, static_cast<int32_t>(q->tokens)}, Runs{key_offsets ? key_offsets : offsets, rows, static_cast<int32_t>(k->tokens)}, key_lengths, causal != 0,
+          static_cast<float>(scale)};
 }
 
 }  // namespace nvtext_amd
