@@ -1,13 +1,14 @@
 """A text encoder, from strings to a training step, on one GPU:
 
     normalize_characters -> wordpiece_tokenize -> embedding -> layer_norm
-        -> per layer: linear with gelu -> linear -> layer_norm of residual + dropout
+        -> per layer: with heads, linear -> rotary positions of queries and keys -> attention -> linear -> layer_norm of residual + dropout;
+                      linear with gelu -> linear -> layer_norm of residual + dropout
         -> linear
 
 and the way back through the gradients of each.  The task is a small one that needs no labels: of every token, what stands next
 to it in its text, as a row of a fixed random table of codes; the loss is the mean square of the differences.
 
-    python -m cudf_amd.examples.text_encoder [--steps 100] [--rows 2000] [--width 256] [--layers 2] [--dtype bfloat16]
+    python -m cudf_amd.examples.text_encoder [--steps 100] [--rows 2000] [--width 256] [--layers 2] [--heads 0] [--dtype bfloat16]
 """
 from __future__ import annotations
 
@@ -24,10 +25,15 @@ from cudf_amd.arrow_host import HostStringsColumn
 
 class TextEncoder:
     """The parameters by name, and the two directions through the layers.  Matrices are of `dtype`, what the layer norms scale
-    by is float32."""
+    by is float32.  With `heads`, which divide the width, every token sees those in front of it in its text; without, itself alone.
+    `key_heads` of them, a divisor (as many as heads if not given), have keys and values."""
 
-    def __init__(self, vocabulary_size: int, positions: int, width: int, layers: int, outputs: int, dtype: torch.dtype = torch.bfloat16, seed: int = 0):
+    def __init__(self, vocabulary_size: int, positions: int, width: int, layers: int, outputs: int, dtype: torch.dtype = torch.bfloat16, seed: int = 0, heads: int = 0,
+                 key_heads: int = 0):
         self.layers, self.vocabulary_size, self.positions = layers, vocabulary_size, positions
+        self.heads, self.key_heads = heads, key_heads or heads
+        if heads and (width % heads or width // heads % 2 or heads % self.key_heads):
+            raise ValueError("heads must divide the width into an even number of values each, and key_heads divide heads")
         gen = torch.Generator().manual_seed(seed)
 
         def random(*shape, scale):
@@ -50,16 +56,61 @@ class TextEncoder:
                 f"{i}.norm.weight": torch.ones(width, device="cuda"),
                 f"{i}.norm.bias": torch.zeros(width, device="cuda"),
             })
+        if heads:
+            of_head = width // heads
+            self.frequencies = encoder.rotary_frequencies(of_head)
+            for i in range(layers):
+                self.parameters.update({
+                    f"{i}.heads.weight": random((heads + 2 * self.key_heads) * of_head, width, scale=width**-0.5),
+                    f"{i}.heads.bias": torch.zeros((heads + 2 * self.key_heads) * of_head, device="cuda", dtype=dtype),
+                    f"{i}.mix.weight": random(width, width, scale=0.5 * width**-0.5),
+                    f"{i}.mix.bias": torch.zeros(width, device="cuda", dtype=dtype),
+                    f"{i}.mix_norm.weight": torch.ones(width, device="cuda"),
+                    f"{i}.mix_norm.bias": torch.zeros(width, device="cuda"),
+                })
+
+    def _parts(self, x: torch.Tensor) -> Tuple[torch.Tensor, ...]:
+        """(queries and keys, which are rotated; queries; keys; values) of a tensor of all heads side by side."""
+        n, m = self.heads, self.key_heads
+        x = x.unflatten(1, (n + 2 * m, -1))
+        return x[:, : n + m], x[:, :n], x[:, n : n + m], x[:, n + m :]
+
+    def _attend(self, i: int, h: torch.Tensor, tokens: nvtext.DeviceListColumn):
+        """What every token takes from those up to it in its text, and what the way back needs."""
+        q = self.parameters
+        x = encoder.linear(h, q[f"{i}.heads.weight"], q[f"{i}.heads.bias"])
+        turned, queries, keys, values = self._parts(x)
+        encoder.rotary(turned, tokens, self.frequencies, out=turned)
+        out, saved = encoder.attention(queries, keys, values, tokens, causal=True, keep=True)
+        out = out.flatten(1)
+        return encoder.linear(out, q[f"{i}.mix.weight"], q[f"{i}.mix.bias"]), (h, x, out, saved)
+
+    def _attend_backward(self, i: int, g: torch.Tensor, kept: Tuple, tokens: nvtext.DeviceListColumn, grads: Dict[str, torch.Tensor]) -> torch.Tensor:
+        q, (h, x, out, saved) = self.parameters, kept
+        g, grads[f"{i}.mix.weight"], grads[f"{i}.mix.bias"] = encoder.linear_backward(g, out, q[f"{i}.mix.weight"])
+        _, queries, keys, values = self._parts(x)
+        x_grad = torch.empty_like(x)
+        turned, *parts = self._parts(x_grad)
+        encoder.attention_backward(g.view(queries.shape), queries, keys, values, saved, tokens, causal=True, out=tuple(parts))
+        encoder.rotary(turned, tokens, self.frequencies, inverse=True, out=turned)
+        g, grads[f"{i}.heads.weight"], grads[f"{i}.heads.bias"] = encoder.linear_backward(x_grad, h, q[f"{i}.heads.weight"])
+        return g
 
     def forward(self, tokens: nvtext.DeviceListColumn, p: float = 0.0, seed: int = 0) -> Tuple[torch.Tensor, List]:
-        """The outputs, a row a token, and what backward() needs.  Dropout call i draws under the number i of the seed."""
+        """The outputs, a row a token, and what backward() needs.  Dropout call i draws under the number i of the seed, that behind
+        the attention of layer i under the number of layers more."""
         q = self.parameters
         h, saved = encoder.layer_norm(encoder.embedding(tokens, q["tokens"], q["positions"]), q["norm.weight"], q["norm.bias"], keep=True)
         kept = [saved]
         for i in range(self.layers):
+            mixed = None
+            if self.heads:
+                v, attended = self._attend(i, h, tokens)
+                h, saved = encoder.layer_norm(v, q[f"{i}.mix_norm.weight"], q[f"{i}.mix_norm.bias"], residual=saved.sum, p=p, seed=seed, offset=self.layers + i, keep=True)
+                mixed = (attended, saved)
             u, z = encoder.linear(h, q[f"{i}.up.weight"], q[f"{i}.up.bias"], "gelu", keep=True)
             v = encoder.linear(u, q[f"{i}.down.weight"], q[f"{i}.down.bias"])
-            kept.append((h, z, u))
+            kept.append((h, z, u, mixed))
             h, saved = encoder.layer_norm(v, q[f"{i}.norm.weight"], q[f"{i}.norm.bias"], residual=saved.sum, p=p, seed=seed, offset=i, keep=True)
             kept.append(saved)
         kept.append(h)
@@ -71,11 +122,16 @@ class TextEncoder:
         g, grads["out.weight"], grads["out.bias"] = encoder.linear_backward(grad, kept[-1], q["out.weight"])
         stream = None  # the gradient that comes back along the residual stream
         for i in reversed(range(self.layers)):
-            h, z, u = kept[1 + 2 * i]
+            h, z, u, mixed = kept[1 + 2 * i]
             g, stream, grads[f"{i}.norm.weight"], grads[f"{i}.norm.bias"] = encoder.layer_norm_backward(
                 g, kept[2 + 2 * i], q[f"{i}.norm.weight"], p=p, seed=seed, offset=i, sum_grad=stream)
             g, grads[f"{i}.down.weight"], grads[f"{i}.down.bias"] = encoder.linear_backward(g, u, q[f"{i}.down.weight"])
             g, grads[f"{i}.up.weight"], grads[f"{i}.up.bias"] = encoder.linear_backward(g, h, q[f"{i}.up.weight"], "gelu", z)
+            if mixed is not None:
+                attended, saved = mixed
+                g, stream, grads[f"{i}.mix_norm.weight"], grads[f"{i}.mix_norm.bias"] = encoder.layer_norm_backward(
+                    g, saved, q[f"{i}.mix_norm.weight"], p=p, seed=seed, offset=self.layers + i, sum_grad=stream)
+                g = self._attend_backward(i, g, attended, tokens, grads)
         g, _, grads["norm.weight"], grads["norm.bias"] = encoder.layer_norm_backward(g, kept[0], q["norm.weight"], sum_grad=stream)
         grads["tokens"], grads["positions"] = encoder.embedding_backward(tokens, g, self.vocabulary_size, self.positions)
         return grads
@@ -135,13 +191,14 @@ def main(argv=None) -> None:
     parser.add_argument("--rows", type=int, default=2000)
     parser.add_argument("--width", type=int, default=256)
     parser.add_argument("--layers", type=int, default=2)
+    parser.add_argument("--heads", type=int, default=0, help="of attention; 0: every token by itself")
     parser.add_argument("--dtype", choices=["float32", "float16", "bfloat16"], default="bfloat16")
     parser.add_argument("--rate", type=float, default=4.0)
     args = parser.parse_args(argv)
     dtype = getattr(torch, args.dtype)
     texts, vocabulary = synthetic_text(args.rows)
     tokens = tokenize(texts, vocabulary)
-    model = TextEncoder(vocabulary.size, positions=64, width=args.width, layers=args.layers, outputs=32, dtype=dtype)
+    model = TextEncoder(vocabulary.size, positions=64, width=args.width, layers=args.layers, outputs=32, dtype=dtype, heads=args.heads)
     codes = torch.randn(vocabulary.size, 32, generator=torch.Generator().manual_seed(1)).to("cuda", dtype)
     target = encoder.embedding(next_tokens(tokens), codes)
     for step in range(args.steps):

@@ -126,4 +126,81 @@ inline void linear_backward(matrix const& grad, matrix const& x, matrix const& w
                                                             mr.c_allocator(storage), x_grad.c_view(), weight_grad.c_view(), bias_grad.c_view()));
 }
 
+enum class rotary_layout : int32_t { HALF = NVTEXT_AMD_ROTARY_HALF, INTERLEAVED = NVTEXT_AMD_ROTARY_INTERLEAVED };
+
+// The heads of `tokens` tokens, `count` of `width` values each, one token every `stride` values (0: every count * width) and one head every
+// `head_stride` (0: every width).
+class heads {
+ public:
+  heads() = default;
+  heads(void* data, element type, int64_t tokens, int64_t count, int64_t width, int64_t stride = 0, int64_t head_stride = 0)
+    : _there{true}, _h{data, tokens, count, width, stride == 0 ? count * width : stride, head_stride == 0 ? width : head_stride, static_cast<int32_t>(type)}
+  {
+  }
+  [[nodiscard]] nvtext_amd_heads const* c_view() const { return _there ? &_h : nullptr; }
+
+ private:
+  bool _there{false};
+  nvtext_amd_heads _h{};
+};
+
+// Which tokens make up a row: offsets, one more than there are rows; of keys with room behind a row's, how many there are, too.
+struct rows {
+  cudf::device_span<int32_t const> offsets{};
+  cudf::device_span<int32_t const> lengths{};
+  [[nodiscard]] int32_t size() const
+  {
+    if (offsets.size() == 0) throw std::invalid_argument("offsets must have a value more than there are rows");
+    return static_cast<int32_t>(offsets.size() - 1);
+  }
+};
+
+namespace detail {
+// (offsets and lengths of the keys; neither where they are those of the tokens)
+inline rows keys_of(rows const& tokens, rows const& keys)
+{
+  if (tokens.lengths.data()) throw std::invalid_argument("only keys have lengths");
+  if (keys.offsets.size() != 0 && keys.size() != tokens.size()) throw std::invalid_argument("there must be as many rows of keys as of tokens");
+  if (keys.lengths.data() && static_cast<int64_t>(keys.lengths.size()) != tokens.size()) throw std::invalid_argument("there must be a length for every row");
+  return keys;
+}
+}  // namespace detail
+
+inline void rotary(heads const& x, rows const& tokens, cudf::device_span<double const> frequencies, rotary_layout layout, heads const& out,
+                   cudf::device_span<int32_t const> starts = {}, bool inverse = false, double magnitude = 1.0, cuda::stream_ref stream = cudf::get_default_stream())
+{
+  if (starts.data() && static_cast<int64_t>(starts.size()) != tokens.size()) throw std::invalid_argument("there must be a start for every row");
+  nvtext::detail::throw_on_error(nvtext_amd_rotary(x.c_view(), tokens.size(), tokens.offsets.data(), starts.data(), frequencies.data(), static_cast<int64_t>(frequencies.size()),
+                                                   static_cast<int32_t>(layout), inverse, magnitude, stream.get(), out.c_view()));
+}
+
+// keys: left out where they are the tokens' own
+inline void attention(heads const& q, heads const& k, heads const& v, rows const& tokens, rows const& keys, bool causal, double scale, heads const& out,
+                      cudf::device_span<float> logsum = {}, cudf::device_span<int8_t> rest = {}, cuda::stream_ref stream = cudf::get_default_stream(),
+                      rmm::device_async_resource_ref mr = cudf::get_current_device_resource_ref())
+{
+  auto const* c = q.c_view();
+  if (c && logsum.data() && static_cast<int64_t>(logsum.size()) != c->heads * c->tokens) throw std::invalid_argument("logsum holds a value a head of a token");
+  if (c && rest.data() && static_cast<int64_t>(rest.size()) != c->heads * c->tokens * c->width) throw std::invalid_argument("rest holds a value for each of q's");
+  rows const of_keys = detail::keys_of(tokens, keys);
+  nvtext_amd_allocator storage{};
+  nvtext::detail::throw_on_error(nvtext_amd_attention(q.c_view(), k.c_view(), v.c_view(), tokens.size(), tokens.offsets.data(), of_keys.offsets.data(), of_keys.lengths.data(), causal,
+                                                      scale, stream.get(), mr.c_allocator(storage), out.c_view(), logsum.data(), rest.data()));
+}
+
+inline void attention_backward(heads const& grad, heads const& q, heads const& k, heads const& v, heads const& out, cudf::device_span<float const> logsum,
+                               cudf::device_span<int8_t const> rest, rows const& tokens, rows const& keys, bool causal, double scale, heads const& q_grad, heads const& k_grad,
+                               heads const& v_grad, cuda::stream_ref stream = cudf::get_default_stream(),
+                               rmm::device_async_resource_ref mr = cudf::get_current_device_resource_ref())
+{
+  auto const* c = q.c_view();
+  if (c && static_cast<int64_t>(logsum.size()) != c->heads * c->tokens) throw std::invalid_argument("logsum holds a value a head of a token");
+  if (c && rest.data() && static_cast<int64_t>(rest.size()) != c->heads * c->tokens * c->width) throw std::invalid_argument("rest holds a value for each of q's");
+  rows const of_keys = detail::keys_of(tokens, keys);
+  nvtext_amd_allocator storage{};
+  nvtext::detail::throw_on_error(nvtext_amd_attention_backward(grad.c_view(), q.c_view(), k.c_view(), v.c_view(), out.c_view(), logsum.data(), rest.data(), tokens.size(),
+                                                               tokens.offsets.data(), of_keys.offsets.data(), of_keys.lengths.data(), causal, scale, stream.get(),
+                                                               mr.c_allocator(storage), q_grad.c_view(), k_grad.c_view(), v_grad.c_view()));
+}
+
 }  // namespace nvtext::encoder
