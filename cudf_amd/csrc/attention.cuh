@@ -399,6 +399,22 @@ __device__ __forceinline__ Fragment<T> rounded(f32x16_t const& x, int step)
   return f;
 }
 
+// sum and eight values, as they are after rounding
+__device__ __forceinline__ float plus(float sum, Fragment<bf16_t> const& x)
+{
+  typedef bf16_t Two __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int k = 0; k < 8; k += 2) sum = __builtin_amdgcn_fdot2_f32_bf16(Two{x[k], x[k + 1]}, Two{bf16_t(1.f), bf16_t(1.f)}, sum, false);
+  return sum;
+}
+__device__ __forceinline__ float plus(float sum, Fragment<half_t> const& x)
+{
+  typedef half_t Two __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int k = 0; k < 8; k += 2) sum = __builtin_amdgcn_fdot2(Two{x[k], x[k + 1]}, Two{half_t(1.f), half_t(1.f)}, sum, false);
+  return sum;
+}
+
 // Eight of a head's values from j on, zeros behind the last or where it is not `there`; widths and strides are of whole pieces of 16 bytes
 template <typename T>
 __device__ __forceinline__ Fragment<T> fragment_of(const T* head, int32_t j, int32_t width, bool there)
@@ -519,7 +535,7 @@ __device__ __forceinline__ int32_t share_begin(int32_t tiles, int32_t share, int
 struct Split {
   int32_t splits;
   float* sums;
-  float2* tops;  // (forward) [block][head][share][row]: top, and the sum of the exponentials
+  float4* tops;  // (forward) [block][head][share][row]: top, the sum of the exponentials, and what out is divided by
   __device__ __forceinline__ int64_t slot(int64_t block, int32_t head, int32_t heads, int32_t share) const { return (block * heads + head) * splits + share; }
 };
 

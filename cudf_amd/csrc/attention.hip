@@ -21,6 +21,7 @@ struct Attending {
   Fragment<T> q[kSteps];
   f32x16_t o[kColumns];
   float top, sum;
+  float weight;  // (16-bit types) the sum of the exponentials as they are multiplied with v, rounded: what out is divided by, so that weights add up to 1
   int32_t seen;  // keys that the column sees
 
   __device__ __forceinline__ void begin(const T* head, int32_t width, bool there, int half)
@@ -28,7 +29,7 @@ struct Attending {
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) q[s] = fragment_of(head, 16 * s + 8 * half, width, there);
     top = -INFINITY;
-    sum = 0.f;
+    sum = weight = 0.f;
 #pragma unroll
     for (int c = 0; c < kColumns; ++c) o[c] = f32x16_t{};
   }
@@ -66,6 +67,7 @@ struct Attending {
       float const fade = now == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - now);
       top              = now;
       sum *= fade;
+      weight *= fade;
 #pragma unroll
       for (int c = 0; c < kColumns; ++c)
 #pragma unroll
@@ -80,29 +82,40 @@ struct Attending {
       sum += x;
     };
     Fragment<T> p;
+    auto const round = [&](int step) {
+      p = rounded<T>(s[step / 2], step % 2);
+      if constexpr (sizeof(T) == 2) weight = plus(weight, p);
+    };
     stream<T, kRounds * kColumns>([&](auto i) { return read.columns(v_tile, i % kColumns, i / kColumns); },
                                   [&](auto i, Fragment<T> const& v) {
                                     constexpr int step = i / kColumns, c = i % kColumns;
                                     if constexpr (i == 0) {
 #pragma unroll
                                       for (int e = 0; e < 8; ++e) exponential(0, e);
-                                      p = rounded<T>(s[0], 0);
+                                      round(0);
                                     }
                                     o[c] = multiply32(v, p, o[c]);
                                     if constexpr (step + 1 < kRounds) {
 #pragma unroll
                                       for (int e = c * 8 / kColumns; e < (c + 1) * 8 / kColumns; ++e) exponential(step + 1, e);
-                                      if constexpr (c == kColumns - 1) p = rounded<T>(s[(step + 1) / 2], (step + 1) % 2);
+                                      if constexpr (c == kColumns - 1) round(step + 1);
                                     }
                                   });
   }
+
+  // what both lanes of a column have of a sum; what its o is divided by
+  __device__ __forceinline__ static float whole(float part)
+  {
+    Halves const both = halves(part);
+    return both.low + both.high;
+  }
+  __device__ __forceinline__ float divisor() const { return whole(sizeof(T) == 2 ? weight : sum); }
 
   // Writes out and logsum of a column, head h of token t, where it is `there`; of those whose result is not finite, the lanes' numbers.  That may come from keys that the
   // token does not see, whose exponentials of 0 were multiplied: such columns are done once more, by themselves.
   __device__ __forceinline__ uint32_t finish(Forward<T> const& f, int64_t t, int32_t h, bool there, int half, int column)
   {
-    Halves const both = halves(sum);
-    float const total = both.low + both.high, part = seen > 0 ? 1.f / total : 0.f;
+    float const total = whole(sum), part = seen > 0 ? 1.f / divisor() : 0.f;
     float check       = 0.f;  // (NaN if any is infinite or NaN)
 #pragma unroll
     for (int c = 0; c < kColumns; ++c)
@@ -180,10 +193,10 @@ __global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES>::kWa
   if (wave0 >= rest) return;
   if (shares > 1) {
     int64_t const part = split.slot(w.block, w.head, f.heads, w.share) * Shape::kTokens + wave0 + column;
-    Halves const both  = halves(a.sum);
+    float const total = a.whole(a.sum), divisor = a.divisor();
     if (there) {
       store_columns<float, D / 32>(split.sums + part * D, a.o, half, D);
-      if (half == 0) split.tops[part] = make_float2(a.top, both.low + both.high);
+      if (half == 0) split.tops[part] = make_float4(a.top, total, divisor, 0.f);
     }
     return;
   }
@@ -204,7 +217,7 @@ template <typename T>
 struct ForwardChunks : Forward<T> {
   int shift;
   float* sums;    // [part][key head][column][D]
-  float2* tops;   // [part][key head][column]: top, and the sum of the exponentials
+  float4* tops;   // [part][key head][column]: top, the sum of the exponentials, and what out is divided by
   __device__ __forceinline__ int64_t part(int32_t first, int32_t chunk, int32_t kv_head) const
   {
     return ((static_cast<int64_t>(first) * 2 >> shift) + chunk) * this->kv_heads + kv_head;
@@ -268,10 +281,10 @@ __global__ void __launch_bounds__(kWave, 1) attend_chunks_kernel(ForwardChunks<T
     stage_barrier<0>();  // (the next columns' loads come into the same places)
     if (split) {
       int64_t const part = f.part(first, static_cast<int32_t>(chunk), w.kv_head) * kPartColumns + column;
-      Halves const both  = halves(a.sum);
+      float const total = a.whole(a.sum), divisor = a.divisor();
       if (there) {
         store_columns<float, D / 32>(f.sums + part * D, a.o, half, D);
-        if (half == 0) f.tops[part] = make_float2(a.top, both.low + both.high);
+        if (half == 0) f.tops[part] = make_float4(a.top, total, divisor, 0.f);
       }
       continue;
     }
@@ -283,19 +296,20 @@ __global__ void __launch_bounds__(kWave, 1) attend_chunks_kernel(ForwardChunks<T
 }
 
 template <int D>
-__device__ __forceinline__ void add_part(Some<D>& sum, float& total, float top, float2 of, const float* part)
+__device__ __forceinline__ void add_part(Some<D>& sum, float2& total, float top, float4 of, const float* part)
 {
   float const weight = of.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(of.x - top);
-  total += of.y * weight;
+  total.x += of.y * weight;
+  total.y += of.z * weight;
   sum.add(part, weight);
 }
 
 // What Attending::finish does, for sums that a wavefront holds side by side.
 template <typename T, int D>
-__device__ __forceinline__ void finish_row(Forward<T> const& f, int32_t t, int32_t head, int32_t seen, Some<D> sum, float total, float top)
+__device__ __forceinline__ void finish_row(Forward<T> const& f, int32_t t, int32_t head, int32_t seen, Some<D> sum, float2 total, float top)
 {
 #pragma unroll
-  for (int k = 0; k < Some<D>::kEach; ++k) sum.v[k] = seen > 0 ? sum.v[k] / total : 0.f;
+  for (int k = 0; k < Some<D>::kEach; ++k) sum.v[k] = seen > 0 ? sum.v[k] / total.y : 0.f;
   if (!sum.finite(f.width)) {
     attend_row(f, t, head);
     return;
@@ -310,7 +324,7 @@ __device__ __forceinline__ void finish_row(Forward<T> const& f, int32_t t, int32
       if (f.rest) f.rest[at * f.width + j] = rest_of(sum.v[k], static_cast<T>(sum.v[k]));
     }
   }
-  if (f.logsum && lane_id() == 0) f.logsum[at] = seen > 0 ? (top + __builtin_amdgcn_logf(total)) * kLn2 : -INFINITY;
+  if (f.logsum && lane_id() == 0) f.logsum[at] = seen > 0 ? (top + __builtin_amdgcn_logf(total.x)) * kLn2 : -INFINITY;
 }
 
 // Joins the parts of a head of a token, a workgroup for each: its wavefronts take every fourth part.
@@ -318,7 +332,8 @@ constexpr int kJoinWaves = 4;
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinWaves * kWave) attend_join_kernel(ForwardChunks<T> f)
 {
-  __shared__ float tops[kJoinWaves], totals[kJoinWaves];
+  __shared__ float tops[kJoinWaves];
+  __shared__ float2 totals[kJoinWaves];
   __shared__ float sums_[kJoinWaves * kWave * Some<D>::kEach];
   auto const sums = reinterpret_cast<Some<D>(*)[kWave]>(sums_);
   int64_t const item = block_number();
@@ -339,7 +354,7 @@ __global__ void __launch_bounds__(kJoinWaves * kWave) attend_join_kernel(Forward
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kJoinWaves; ++w) top = fmaxf(top, tops[w]);
-  float total = 0.f;
+  float2 total{};
   Some<D> sum{};
 #pragma unroll 8
   for (int32_t c = wave; c < chunks; c += kJoinWaves) add_part<D>(sum, total, top, f.tops[at + c * step], f.sums + (at + c * step) * D);
@@ -349,7 +364,8 @@ __global__ void __launch_bounds__(kJoinWaves * kWave) attend_join_kernel(Forward
   if (wave != 0) return;
 #pragma unroll
   for (int w = 1; w < kJoinWaves; ++w) {
-    total += totals[w];
+    total.x += totals[w].x;
+    total.y += totals[w].y;
 #pragma unroll
     for (int k = 0; k < Some<D>::kEach; ++k) sum.v[k] += sums[w][lane].v[k];
   }
@@ -374,7 +390,7 @@ __global__ void __launch_bounds__(kThreads) attend_join_shares_kernel(Forward<T>
   float top = -INFINITY;
   for (int32_t c = 0; c < shares; ++c) top = fmaxf(top, split.tops[at + (static_cast<int64_t>(c) << shift)].x);
   Some<D> sum{};
-  float total = 0.f;
+  float2 total{};
 #pragma unroll 4
   for (int32_t c = 0; c < shares; ++c) add_part<D>(sum, total, top, split.tops[at + (static_cast<int64_t>(c) << shift)], split.sums + (at + (static_cast<int64_t>(c) << shift)) * D);
   finish_row<T, D>(f, t, head, f.seen(i, tokens, keys), sum, total, top);
@@ -388,10 +404,10 @@ nvtext_amd_status attend_tiles(Forward<T> const& f, Mr const& mr, hipStream_t st
   Estimate const e = estimate(f, f.runs, f.heads, Shape::kShift, f.key_runs, Shape::kTile, 1);
   Split split{splits_of(e.workgroups, e.tiles), nullptr, nullptr};
   size_t const rows = split.splits > 1 ? static_cast<size_t>(f.runs.blocks(Shape::kShift) * f.heads * split.splits) << Shape::kShift : 0;
-  TempParts<2> const temp(mr, {rows * D * sizeof(float), rows * sizeof(float2)});
+  TempParts<2> const temp(mr, {rows * D * sizeof(float), rows * sizeof(float4)});
   if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
   split.sums = temp.template part<float>(0);
-  split.tops = temp.template part<float2>(1);
+  split.tops = temp.template part<float4>(1);
   NVTEXT_HIP_TRY(allow_lds(attend_tiles_kernel<T, D, kTileWaves>, Shape::kLds));
   {
     ProfileScope const scope("attention_tiles", stream);
@@ -432,10 +448,10 @@ nvtext_amd_status attention(Forward<T> f, Mr const& mr, hipStream_t stream)
   return with_tiles(f.width, [&](auto d) {
     constexpr int kD        = decltype(d)::value;
     size_t const parts      = chunks ? static_cast<size_t>(most_parts(f.key_runs.tokens, shift)) * static_cast<size_t>(f.kv_heads) * kPartColumns : 0;
-    TempParts<3> const temp(mr, {align.bytes(), parts * kD * sizeof(float), parts * sizeof(float2)});
+    TempParts<3> const temp(mr, {align.bytes(), parts * kD * sizeof(float), parts * sizeof(float4)});
     if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
     align.launch(temp.template part<char>(0), stream);
-    if (chunks) return attend_chunks<T, kD>({f, shift, temp.template part<float>(1), temp.template part<float2>(2)}, stream);
+    if (chunks) return attend_chunks<T, kD>({f, shift, temp.template part<float>(1), temp.template part<float4>(2)}, stream);
     return attend_tiles<T, kD>(f, mr, stream);
   });
 }

@@ -162,9 +162,9 @@ void launch(Rotary<T> r, bool half, hipStream_t stream)
   r.each             = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>({most, 8, r.runs.tokens / (4 * device_cus())})));
   ProfileScope const scope("rotary", stream);
   dim3 const grid = grid_of((static_cast<int64_t>(r.runs.tokens) + r.each - 1) / r.each, kThreads);
-  constexpr int kVec = 16 / sizeof(T) / 2;  // an interleaved load has 16 bytes, one of a half 8
+  constexpr int kVec = 16 / sizeof(T);  // (pairs of a thread at a time: two loads of 16 bytes)
   if (half)
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(rotary_kernel<T, 2 * kVec, true>), grid, dim3(kThreads), 0, stream, r);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(rotary_kernel<T, kVec, true>), grid, dim3(kThreads), 0, stream, r);
   else
     hipLaunchKernelGGL(HIP_KERNEL_NAME(rotary_kernel<T, kVec, false>), grid, dim3(kThreads), 0, stream, r);
 }

@@ -200,7 +200,8 @@ nvtext_amd_status nvtext_amd_rotary(const nvtext_amd_heads* x,
  * q, k, v and out are of one type and width, of at most 256 values; scale is not negative.  logsum (NULL: not wanted; the gradient needs it)
  * has a value of FLOAT32 at [h * tokens + t].  rest (NULL: not wanted; FLOAT32 has none), of a value for each of out's, [heads, tokens, width]
  * one after the other: what rounding left off it, in 8 bits, for the gradient.  Products, exponentials' sums and out are held in 32 bits; of 16-bit types, the exponentials are
- * rounded to the type before they are multiplied with v (the values that logsum sums are not), as the matrix cores take them. */
+ * rounded to the type before they are multiplied with v, as the matrix cores take them, and out is divided by their sum as they are then
+ * (logsum is that of the values before). */
 nvtext_amd_status nvtext_amd_attention(const nvtext_amd_heads* q,
                                        const nvtext_amd_heads* k,
                                        const nvtext_amd_heads* v,

@@ -183,7 +183,7 @@ def _rows_seen(offsets, key_offsets, key_lengths, causal):
 def attention(q, k, v, offsets, key_offsets=None, key_lengths=None, causal=False, scale=None, unit=0.0, tiny=0.0, eps=2.0**-24):
     """(out, logsum [heads, tokens], what a kernel's out may be off by before it is rounded, the same for logsum).  unit: by how much of itself
     an exponential may be off that is rounded before it is multiplied, tiny: by how much where it is smaller than its type's normal
-    numbers (next to a sum of at least 1, that of the largest score).  A score of `width` products held in 32 bits is off by
+    numbers (next to a sum of at least 1, that of the largest score); out is divided by the sum of what was rounded, which is off by as much of itself.  A score of `width` products held in 32 bits is off by
     eps a product and addition, in proportion to the magnitudes that it adds up, twice where they are cut off instead of
     rounded; its difference from the largest score or the logsum by eps of both; the exponential follows."""
     q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
@@ -205,7 +205,7 @@ def attention(q, k, v, offsets, key_offsets=None, key_lengths=None, causal=False
                 out[at, h] = p @ vv
                 score_off = score_error(scale * (np.abs(kk) @ np.abs(q[at, h])), abs(top), width, eps)
                 worst = score_off.max()
-                off[at, h] = (p * (unit + score_off + worst + 2 * (len(keys) + 8) * eps) + tiny) @ np.abs(vv)
+                off[at, h] = (p * (unit + score_off + worst + 2 * (len(keys) + 8) * eps) + tiny) @ np.abs(vv) + (unit + tiny * len(keys)) * np.abs(out[at, h])
                 log_off[h, at] = worst + 2 * (len(keys) + 8) * eps
     return out, logsum, off, log_off
 
