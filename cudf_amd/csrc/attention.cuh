@@ -88,18 +88,19 @@ struct Forward : Problem<T> {
   int8_t* rest;  // [heads, tokens, width], of 16-bit types; or nullptr
 };
 
-// The run that token t is in.
+// The run that token t is in, the same in all lanes of the (whole) wavefront, which look at 64 runs at once as in Runs::run_of().
 __device__ __forceinline__ int32_t run_with(Runs const& runs, int32_t t)
 {
-  int32_t lo = 0, hi = runs.rows + 2;
-  while (hi - lo > 1) {
-    int32_t const mid = lo + (hi - lo) / 2;
-    if (runs.begin(mid) <= t)
-      lo = mid;
-    else
-      hi = mid;
+  int32_t lo = 0, count = runs.rows + 2;
+  while (count > 1) {
+    int32_t const each = (count + kWave - 1) / kWave;
+    int32_t const i    = lane_id() * each;
+    uint64_t const all = __ballot(i < count && runs.begin(lo + i) <= t) | 1;
+    int32_t const last = 63 - __clzll(static_cast<long long>(all));
+    lo += last * each;
+    count = count - last * each < each ? count - last * each : each;
   }
-  return lo;
+  return __builtin_amdgcn_readfirstlane(lo);
 }
 
 template <typename T>
@@ -362,10 +363,11 @@ struct TileReader {
 
 // use(0, read(0)), ... use(SLOTS - 1, read(SLOTS - 1)), with each fragment read some uses before its own: a read of LDS takes as long as a few products, and
 // the compiler, left to itself, reads a fragment, waits for it and multiplies.
-template <typename T, int SLOTS, typename Read, typename Use>
+template <typename T, int D, int SLOTS, typename Read, typename Use>
 __device__ __forceinline__ void stream(Read&& read, Use&& use)
 {
-  constexpr int kAhead = sizeof(T) == 2 ? 3 : 1;
+  // (a fragment of 32-bit values is eight products: there is less to wait for, and of wide heads no register for it)
+  constexpr int kAhead = sizeof(T) == 2 ? 3 : D < 192 ? 1 : 0;
   Fragment<T> x[kAhead + 1];
   for_each<kAhead>([&](auto i) { x[i] = read(i); });
   __builtin_amdgcn_sched_barrier(0);
@@ -657,11 +659,12 @@ hipError_t allow_lds(Kernel kernel, int bytes)
 
 // In how many shares the tiles of a workgroup go: so many that there are twice as many workgroups as run at once, two a CU, if that many have kLeastTiles
 // tiles on average; and none where there are that many workgroups, or tiles take no longer than another launch.
+constexpr int64_t kMostShares = 16;
 inline int32_t splits_of(int64_t workgroups, int64_t tiles)
 {
   int64_t const at_once = 2 * device_cus();
   if (workgroups >= at_once || workgroups <= 0 || tiles < 3 * kLeastTiles) return 1;
-  return static_cast<int32_t>(std::min<int64_t>({(2 * at_once + workgroups - 1) / workgroups, tiles / kLeastTiles, 16}));
+  return static_cast<int32_t>(std::min<int64_t>({(2 * at_once + workgroups - 1) / workgroups, tiles / kLeastTiles, kMostShares}));
 }
 
 // Workgroups with something to do, and what they have, as far as the host knows: rows are taken to be alike.

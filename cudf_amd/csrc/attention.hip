@@ -42,7 +42,7 @@ struct Attending {
     f32x16_t s[kBlocks];
     {
       constexpr int kSlots = kBlocks * kSteps;
-      stream<T, kSlots>([&](auto i) { return read.rows(k_tile, i / kSteps, i % kSteps); },
+      stream<T, D, kSlots>([&](auto i) { return read.rows(k_tile, i / kSteps, i % kSteps); },
                         [&](auto i, Fragment<T> const& k) {
                           constexpr int b = i / kSteps, step = i % kSteps;
                           if constexpr (step == 0) s[b] = f32x16_t{};
@@ -86,7 +86,7 @@ struct Attending {
       p = rounded<T>(s[step / 2], step % 2);
       if constexpr (sizeof(T) == 2) weight = plus(weight, p);
     };
-    stream<T, kRounds * kColumns>([&](auto i) { return read.columns(v_tile, i % kColumns, i / kColumns); },
+    stream<T, D, kRounds * kColumns>([&](auto i) { return read.columns(v_tile, i % kColumns, i / kColumns); },
                                   [&](auto i, Fragment<T> const& v) {
                                     constexpr int step = i / kColumns, c = i % kColumns;
                                     if constexpr (i == 0) {
@@ -387,12 +387,13 @@ __global__ void __launch_bounds__(kThreads) attend_join_shares_kernel(Forward<T>
   int32_t const all = f.seen(last < tokens ? last : tokens - 1, tokens, keys), shares = shares_of((all + kTile - 1) / kTile, split.splits);
   if (shares < 2) return;
   int64_t const at = (split.slot(f.runs.first_block(run, shift) + (i >> shift), head, f.heads, 0) << shift) + (i & ((1 << shift) - 1));
-  float top = -INFINITY;
-  for (int32_t c = 0; c < shares; ++c) top = fmaxf(top, split.tops[at + (static_cast<int64_t>(c) << shift)].x);
+  // (at most kMostShares shares: a lane has the sums of one)
+  float4 const mine  = lane_id() < shares ? split.tops[at + (static_cast<int64_t>(lane_id()) << shift)] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+  float const top    = wave_max(mine.x), weight = mine.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mine.x - top);
+  float2 const total = make_float2(wave_sum(mine.y * weight), wave_sum(mine.z * weight));
   Some<D> sum{};
-  float2 total{};
-#pragma unroll 4
-  for (int32_t c = 0; c < shares; ++c) add_part<D>(sum, total, top, split.tops[at + (static_cast<int64_t>(c) << shift)], split.sums + (at + (static_cast<int64_t>(c) << shift)) * D);
+#pragma unroll 8
+  for (int32_t c = 0; c < shares; ++c) sum.add(split.sums + (at + (static_cast<int64_t>(c) << shift)) * D, __shfl(weight, c));
   finish_row<T, D>(f, t, head, f.seen(i, tokens, keys), sum, total, top);
 }
 

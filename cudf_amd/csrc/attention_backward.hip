@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
 #pragma unroll 1
     for (int32_t from = key0; from < key0 + kTile && from < most; from += 32 * kAtOnce) {
       LdsBytes const k_block = k_tile + (from - key0) * Tile<T, D>::kLine, v_block = k_block + Tile<T, D>::kBytes;
-      stream<T, kAtOnce * kOfBlock>(
+      stream<T, D, kAtOnce * kOfBlock>(
         [&](auto slot) {
           constexpr int b = slot / kOfBlock, i = slot % kOfBlock;
           if constexpr (i < kSteps) return read.rows(k_block, b, i);
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES>::kWavesA
     for (int32_t block = token0; block < token0 + kTile && block < tokens; block += 32 * kAtOnce) {
       if (block + 32 * kAtOnce <= first_from) continue;
       LdsBytes const q_block = q_tile + (block - token0) * Tile<T, D>::kLine, g_block = q_block + Tile<T, D>::kBytes, words = q_tile + Shape::kTiles + 16 * half + (block - token0) * 4;
-      stream<T, kAtOnce * kOfBlock>(
+      stream<T, D, kAtOnce * kOfBlock>(
         [&](auto slot) {
           constexpr int b = slot / kOfBlock, i = slot % kOfBlock;
           if constexpr (i < kSteps) return read.rows(q_block, b, i);
@@ -351,7 +351,7 @@ template <int D>
 __device__ __forceinline__ Some<D> add_shares(const float* at, int64_t step, int32_t shares, float scale)
 {
   Some<D> sum;
-#pragma unroll 4
+#pragma unroll 8
   for (int32_t c = 0; c < shares; ++c) sum.add(at + c * step, scale);
   return sum;
 }
