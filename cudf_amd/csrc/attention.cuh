@@ -24,6 +24,8 @@ struct Problem {
   bool causal;
   float scale;
 
+  // whether keys are those of the tokens themselves, all of them
+  bool own_keys() const { return key_runs.offsets == runs.offsets && key_runs.tokens == runs.tokens && !key_lengths; }
   // The keys of run `i` (a row's), of which there are `length`, from token `first` on.
   __device__ __forceinline__ void keys_of(int32_t i, int32_t& first, int32_t& length) const
   {
@@ -86,6 +88,9 @@ struct Forward : Problem<T> {
   Heads<T> out;
   float* logsum;
   int8_t* rest;  // [heads, tokens, width], of 16-bit types; or nullptr
+  // Which launches there are; and of the one in chunks, that a chunk has 2^shift keys.
+  bool in_tiles, in_chunks;
+  int32_t shift;
 };
 
 // The run that token t is in, the same in all lanes of the (whole) wavefront, which look at 64 runs at once as in Runs::run_of().
@@ -260,10 +265,12 @@ __device__ __forceinline__ f32x16_t multiply32(Fragment<float> a, Fragment<float
 // number so that what is read at once lies in all of the 256 bytes of LDS's banks: pieces of one number of 16 neighbouring heads (the reads of rows), units
 // of two pieces of 4 neighbouring heads and the units beside them (the transposing reads of columns), 8 pieces of a head and of the one 4 further
 // on (columns of 32-bit types).
-template <typename T, int D>
+// There are 64 heads in a tile, of 1024 bytes 32: two tiles, twice, fill no more than 128 KB.
+constexpr int heads_of_tile(int bytes) { return bytes > 512 ? 32 : 64; }
+template <typename T, int D, int HEADS = heads_of_tile(D * sizeof(T))>
 struct Tile {
   static_assert(D % 32 == 0 && D <= kMostWidth);
-  static constexpr int kHeads = D * sizeof(T) > 512 ? 32 : 64;  // two tiles of each, twice, fill no more than 128 KB
+  static constexpr int kHeads = HEADS;
   static constexpr int kLine = D * sizeof(T), kBytes = kHeads * kLine, kPieces = kLine / 16;  // bytes of a head, of all, pieces of 16 bytes of a head
   __device__ __forceinline__ static constexpr uint32_t turn(uint32_t head)
   {
@@ -276,9 +283,9 @@ struct Tile {
 };
 
 // What a wavefront of WAVES loads of a tile: straight into LDS, 64 pieces of 16 bytes at a time, zeros for what is not there.
-template <typename T, int D, int WAVES>
+template <typename T, int D, int WAVES, int HEADS = Tile<T, D>::kHeads>
 struct TileLoader {
-  using Of = Tile<T, D>;
+  using Of = Tile<T, D, HEADS>;
   static constexpr int kAll = Of::kHeads * Of::kPieces / kWave, kLoads = (kAll + WAVES - 1) / WAVES, kEach = 16 / sizeof(T);
   uint32_t offset[kLoads];
   uint32_t line, width;  // bytes from a head to the next, of one
@@ -657,12 +664,12 @@ hipError_t allow_lds(Kernel kernel, int bytes)
   return bytes > 65536 ? hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) : hipSuccess;
 }
 
-// In how many shares the tiles of a workgroup go: so many that there are twice as many workgroups as run at once, two a CU, if that many have kLeastTiles
-// tiles on average; and none where there are that many workgroups, or tiles take no longer than another launch.
+// In how many shares the tiles of a workgroup go: so many that there are twice as many workgroups as run at once, two a CU (one, if two have no room in its
+// LDS), if that many have kLeastTiles tiles on average; and none where there are that many workgroups, or tiles take no longer than another launch.
 constexpr int64_t kMostShares = 16;
-inline int32_t splits_of(int64_t workgroups, int64_t tiles)
+inline int32_t splits_of(int64_t workgroups, int64_t tiles, int lds)
 {
-  int64_t const at_once = 2 * device_cus();
+  int64_t const at_once = (2 * lds > 160 * 1024 ? 1 : 2) * device_cus();
   if (workgroups >= at_once || workgroups <= 0 || tiles < 3 * kLeastTiles) return 1;
   return static_cast<int32_t>(std::min<int64_t>({(2 * at_once + workgroups - 1) / workgroups, tiles / kLeastTiles, kMostShares}));
 }

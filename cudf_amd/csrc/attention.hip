@@ -4,6 +4,17 @@
 namespace nvtext_amd {
 namespace {
 
+// Rows of few tokens go in chunks of keys, where all tokens and heads that share a key head are columns of one wavefront's products, the others in tiles:
+// rows of at most kPartColumns columns, and, if they have a tile's keys or fewer, of kFewColumns.
+constexpr int kPartColumns = 32, kFewColumns = 64, kFewKeys = 128;
+template <typename T>
+__device__ __forceinline__ bool goes_in_chunks(Forward<T> const& f, int32_t tokens, int32_t keys)
+{
+  if (!f.in_tiles || !f.in_chunks) return f.in_chunks;
+  int64_t const columns = static_cast<int64_t>(tokens) * (f.heads / f.kv_heads);
+  return columns <= kPartColumns || (columns <= kFewColumns && keys <= kFewKeys);
+}
+
 // ------------------------------------------------------------------ forward, in tiles
 template <typename T, int D, int WAVES>
 struct ForwardShape {
@@ -14,9 +25,9 @@ struct ForwardShape {
 // keys as rows, so a lane has all of a column's scores (with the one 32 further on), and exponentials are in its registers as the second product
 // takes them: no lane needs another's but for the maximum.  Sums are kept in proportion to 2^top, where top is a maximum that may be 8 too small:
 // only then are they multiplied anew.
-template <typename T, int D>
+template <typename T, int D, int TILE = Tile<T, D>::kHeads>
 struct Attending {
-  static constexpr int kSteps = D / 16, kColumns = D / 32, kTile = Tile<T, D>::kHeads, kBlocks = kTile / 32;
+  static constexpr int kSteps = D / 16, kColumns = D / 32, kTile = TILE, kBlocks = kTile / 32;
   static constexpr float kSlack = 8.f;
   Fragment<T> q[kSteps];
   f32x16_t o[kColumns];
@@ -158,6 +169,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES>::kWa
   if (f.is_row(run)) f.keys_of(run, first, keys);
   first = uniform(first);
   keys  = uniform(keys);
+  if (goes_in_chunks(f, tokens, keys)) return;
   // keys that the workgroup's last token sees, and the wavefront's first and last
   int32_t const wave0 = wave * 32, wave1 = wave0 + 32 < rest ? wave0 + 32 : rest;
   int32_t const all   = uniform(f.seen(block0 + (rest < Shape::kTokens ? rest : Shape::kTokens) - 1, tokens, keys));
@@ -208,21 +220,19 @@ __global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES>::kWa
 // Few tokens a row, as where texts go on token by token: one wavefront has all of a row's tokens and of all heads that share a key head, up to 32 together,
 // as the columns of its products, and a chunk of 2^shift of the row's keys; what it adds up is joined with that of the row's other chunks by another
 // launch.  Bound by memory: the keys are read once.  The chunks of key tokens are numbered as the blocks of tokens are elsewhere, so they are
-// alike in size however long the rows are.  A row of a single chunk is finished at once; so is one of more columns, by the workgroup of its first chunk
-// alone, 32 columns after the other.
+// alike in size however long the rows are.  A row of a single chunk is finished at once; so is one of more columns, 32 of them after the other by each of
+// the workgroups that its chunks have.
 // Parts of a row of several chunks lie from number 2 * first / 2^shift on: it has at least half as many numbers up to the next row's as it has chunks.
-constexpr int kPartColumns = 32;
-
+constexpr int kChunkTile = 32;
 template <typename T>
 struct ForwardChunks : Forward<T> {
-  int shift;
   float* sums;    // [part][key head][column][D]
   float4* tops;   // [part][key head][column]: top, the sum of the exponentials, and what out is divided by
   __device__ __forceinline__ int64_t part(int32_t first, int32_t chunk, int32_t kv_head) const
   {
-    return ((static_cast<int64_t>(first) * 2 >> shift) + chunk) * this->kv_heads + kv_head;
+    return ((static_cast<int64_t>(first) * 2 >> this->shift) + chunk) * this->kv_heads + kv_head;
   }
-  __device__ __forceinline__ int32_t chunks_of(int32_t keys) const { return keys > 0 ? ((keys - 1) >> shift) + 1 : 1; }
+  __device__ __forceinline__ int32_t chunks_of(int32_t keys) const { return keys > 0 ? ((keys - 1) >> this->shift) + 1 : 1; }
   __device__ __forceinline__ bool is_split(int32_t tokens, int32_t chunks) const { return chunks > 1 && static_cast<int64_t>(tokens) * (this->heads / this->kv_heads) <= kPartColumns; }
 };
 inline int64_t most_parts(int64_t key_tokens, int shift) { return (key_tokens * 2 >> shift) + 2; }
@@ -232,7 +242,7 @@ __global__ void __launch_bounds__(kWave, 1) attend_chunks_kernel(ForwardChunks<T
 {
   extern __shared__ __align__(16) char lds_[];
   LdsBytes const lds  = (LdsBytes)lds_;
-  constexpr int kTile = Tile<T, D>::kHeads;
+  constexpr int kTile = kChunkTile, kBytes = Tile<T, D, kTile>::kBytes;
   Work w;
   if (!work_of(block_number(), f.key_runs.blocks(f.shift), f.kv_heads, 1, 1, w)) return;
   int32_t const run = f.key_runs.run_of(w.block, f.shift), each = f.heads / f.kv_heads;
@@ -243,40 +253,40 @@ __global__ void __launch_bounds__(kWave, 1) attend_chunks_kernel(ForwardChunks<T
   int32_t const begin = uniform(f.runs.begin(run)), tokens = uniform(f.runs.begin(run + 1)) - begin, chunks = f.chunks_of(keys);
   int64_t const chunk = w.block - f.key_runs.first_block(run, f.shift);
   bool const split    = f.is_split(tokens, chunks);
-  if (chunk >= (split ? chunks : 1)) return;
+  if (chunk >= chunks || !goes_in_chunks<T>(f, tokens, keys)) return;
   int const lane = lane_id(), column = lane % 32, half = lane / 32;
   int32_t const key_first = split ? static_cast<int32_t>(chunk << f.shift) : 0, key_last = split && keys - key_first > 1 << f.shift ? key_first + (1 << f.shift) : keys;
   int64_t const columns   = static_cast<int64_t>(tokens > 0 ? tokens : 0) * each;
   TileReader<T, D> const read(lane);
   float const scale = f.scale * kLog2e;
-  for (int64_t column0 = 0; column0 < columns; column0 += kPartColumns) {
+  for (int64_t column0 = split ? 0 : chunk * kPartColumns; column0 < columns; column0 += split ? columns : static_cast<int64_t>(chunks) * kPartColumns) {
     int64_t const mine = column0 + column;
     bool const there   = mine < columns;
     int32_t const i    = there ? static_cast<int32_t>(mine / each) : 0, head = w.kv_head * each + (there ? static_cast<int32_t>(mine - static_cast<int64_t>(i) * each) : 0);
     int64_t const t    = static_cast<int64_t>(begin) + i;
     int32_t const last = static_cast<int32_t>(((column0 + kPartColumns < columns ? column0 + kPartColumns : columns) - 1) / each);  // the last column's token
-    Attending<T, D> a;
+    Attending<T, D, kTile> a;
     a.seen = there ? f.seen(i, tokens, keys) : 0;
     a.begin(f.q.at(t, head), f.width, there, half);
     int32_t const least = uniform(f.seen(static_cast<int32_t>(column0 / each), tokens, keys)), all = uniform(f.seen(last, tokens, keys)), end = all < key_last ? all : key_last;
     int32_t const tiles = end > key_first ? (end - key_first + kTile - 1) / kTile : 0;
-    TileLoader<T, D, 1> load_k, load_v;
+    TileLoader<T, D, 1, kTile> load_k, load_v;
     load_k.aim(f.k, first + key_first, w.kv_head, f.width, 0, lane);
     load_v.aim(f.v, first + key_first, w.kv_head, f.width, 0, lane);
     if (tiles > 0) {
       load_k.load(lds, key_last - key_first, 0);
-      load_v.load(lds + Tile<T, D>::kBytes, key_last - key_first, 0);
+      load_v.load(lds + kBytes, key_last - key_first, 0);
     }
     for (int32_t tile = 0; tile < tiles; ++tile) {
-      LdsBytes const k_tile = lds + (tile & 1) * 2 * Tile<T, D>::kBytes;
+      LdsBytes const k_tile = lds + (tile & 1) * 2 * kBytes;
       int32_t const key0    = key_first + tile * kTile;
       stage_barrier<0>();
       if (tile + 1 < tiles) {
-        LdsBytes const next = lds + (~tile & 1) * 2 * Tile<T, D>::kBytes;
+        LdsBytes const next = lds + (~tile & 1) * 2 * kBytes;
         load_k.load(next, key_last - key0 - kTile, 0);
-        load_v.load(next + Tile<T, D>::kBytes, key_last - key0 - kTile, 0);
+        load_v.load(next + kBytes, key_last - key0 - kTile, 0);
       }
-      a.pass(k_tile, k_tile + Tile<T, D>::kBytes, read, key0, key0 + kTile > least || key0 + kTile > key_last, scale, half);
+      a.pass(k_tile, k_tile + kBytes, read, key0, key0 + kTile > least || key0 + kTile > key_last, scale, half);
     }
     stage_barrier<0>();  // (the next columns' loads come into the same places)
     if (split) {
@@ -327,49 +337,49 @@ __device__ __forceinline__ void finish_row(Forward<T> const& f, int32_t t, int32
   if (f.logsum && lane_id() == 0) f.logsum[at] = seen > 0 ? (top + __builtin_amdgcn_logf(total.x)) * kLn2 : -INFINITY;
 }
 
-// Joins the parts of a head of a token, a workgroup for each: its wavefronts take every fourth part.
-constexpr int kJoinWaves = 4;
-template <typename T, int D>
-__global__ void __launch_bounds__(kJoinWaves * kWave) attend_join_kernel(ForwardChunks<T> f)
+// Joins the parts of a head of a row's tokens, a workgroup for every `apart`th token, whose wavefronts take the parts in turn.
+template <typename T, int D, int WAVES>
+__global__ void __launch_bounds__(WAVES * kWave) attend_join_kernel(ForwardChunks<T> f, int32_t apart)
 {
-  __shared__ float tops[kJoinWaves];
-  __shared__ float2 totals[kJoinWaves];
-  __shared__ float sums_[kJoinWaves * kWave * Some<D>::kEach];
-  auto const sums = reinterpret_cast<Some<D>(*)[kWave]>(sums_);
-  int64_t const item = block_number();
-  if (item >= static_cast<int64_t>(f.runs.tokens) * f.heads) return;
-  int32_t const t = static_cast<int32_t>(item / f.heads), head = static_cast<int32_t>(item % f.heads), run = run_with(f.runs, t);
-  if (!f.is_row(run)) return;
+  __shared__ float tops[WAVES];
+  __shared__ float2 totals[WAVES];
+  __shared__ float sums_[WAVES * kWave * Some<D>::kEach];
+  auto const sums    = reinterpret_cast<Some<D>(*)[kWave]>(sums_);
+  int64_t const item = block_number(), of_row = static_cast<int64_t>(f.heads) * apart;
+  if (item >= f.runs.rows * of_row) return;
+  int32_t const row = static_cast<int32_t>(item / of_row), head = static_cast<int32_t>(item - row * of_row) / apart, run = row + 1;
   int32_t first, keys;
   f.keys_of(run, first, keys);
   int32_t const begin = f.runs.begin(run), tokens = f.runs.begin(run + 1) - begin, chunks = f.chunks_of(keys), each = f.heads / f.kv_heads;
-  if (!f.is_split(tokens, chunks)) return;
-  int const wave = threadIdx.x / kWave, lane = lane_id();
-  int32_t const column = (t - begin) * each + head % each;
-  int64_t const at = f.part(first, 0, head / each) * kPartColumns + column, step = static_cast<int64_t>(f.kv_heads) * kPartColumns;
-  float top = -INFINITY;
-  for (int32_t c = threadIdx.x; c < chunks; c += kJoinWaves * kWave) top = fmaxf(top, f.tops[at + c * step].x);
-  top = wave_max(top);
-  if (lane == 0) tops[wave] = top;
-  __syncthreads();
+  if (!f.is_split(tokens, chunks)) return;  // (what is split goes in chunks)
+  int const wave     = threadIdx.x / kWave, lane = lane_id();
+  int64_t const step = static_cast<int64_t>(f.kv_heads) * kPartColumns;
+  for (int32_t i = static_cast<int32_t>(item % apart); i < tokens; i += apart) {
+    int64_t const at = f.part(first, 0, head / each) * kPartColumns + i * each + head % each;
+    float top        = -INFINITY;
+    for (int32_t c = threadIdx.x; c < chunks; c += WAVES * kWave) top = fmaxf(top, f.tops[at + c * step].x);
+    top = wave_max(top);
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kJoinWaves; ++w) top = fmaxf(top, tops[w]);
-  float2 total{};
-  Some<D> sum{};
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, tops[w]);
+    float2 total{};
+    Some<D> sum{};
 #pragma unroll 8
-  for (int32_t c = wave; c < chunks; c += kJoinWaves) add_part<D>(sum, total, top, f.tops[at + c * step], f.sums + (at + c * step) * D);
-  sums[wave][lane] = sum;
-  if (lane == 0) totals[wave] = total;
-  __syncthreads();
-  if (wave != 0) return;
+    for (int32_t c = wave; c < chunks; c += WAVES) add_part<D>(sum, total, top, f.tops[at + c * step], f.sums + (at + c * step) * D);
+    sums[wave][lane] = sum;
+    if (lane == 0) totals[wave] = total;
+    __syncthreads();
+    if (wave != 0) continue;  // (they write totals and sums again behind the next token's first barrier)
 #pragma unroll
-  for (int w = 1; w < kJoinWaves; ++w) {
-    total.x += totals[w].x;
-    total.y += totals[w].y;
+    for (int w = 1; w < WAVES; ++w) {
+      total.x += totals[w].x;
+      total.y += totals[w].y;
 #pragma unroll
-    for (int k = 0; k < Some<D>::kEach; ++k) sum.v[k] += sums[w][lane].v[k];
+      for (int k = 0; k < Some<D>::kEach; ++k) sum.v[k] += sums[w][lane].v[k];
+    }
+    finish_row<T, D>(f, begin + i, head, f.seen(i, tokens, keys), sum, total, top);
   }
-  finish_row<T, D>(f, t, head, f.seen(t - begin, tokens, keys), sum, total, top);
 }
 
 // The same for the shares of a block of 2^shift tokens, a wavefront for each head of a token.
@@ -384,6 +394,7 @@ __global__ void __launch_bounds__(kThreads) attend_join_shares_kernel(Forward<T>
   int32_t first, keys;
   f.keys_of(run, first, keys);
   int32_t const begin = f.runs.begin(run), tokens = f.runs.begin(run + 1) - begin, i = t - begin, last = i | ((1 << shift) - 1);
+  if (goes_in_chunks(f, tokens, keys)) return;
   int32_t const all = f.seen(last < tokens ? last : tokens - 1, tokens, keys), shares = shares_of((all + kTile - 1) / kTile, split.splits);
   if (shares < 2) return;
   int64_t const at = (split.slot(f.runs.first_block(run, shift) + (i >> shift), head, f.heads, 0) << shift) + (i & ((1 << shift) - 1));
@@ -403,7 +414,7 @@ nvtext_amd_status attend_tiles(Forward<T> const& f, Mr const& mr, hipStream_t st
 {
   using Shape      = ForwardShape<T, D, kTileWaves>;
   Estimate const e = estimate(f, f.runs, f.heads, Shape::kShift, f.key_runs, Shape::kTile, 1);
-  Split split{splits_of(e.workgroups, e.tiles), nullptr, nullptr};
+  Split split{splits_of(e.workgroups, e.tiles, Shape::kLds), nullptr, nullptr};
   size_t const rows = split.splits > 1 ? static_cast<size_t>(f.runs.blocks(Shape::kShift) * f.heads * split.splits) << Shape::kShift : 0;
   TempParts<2> const temp(mr, {rows * D * sizeof(float), rows * sizeof(float4)});
   if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
@@ -425,14 +436,28 @@ nvtext_amd_status attend_tiles(Forward<T> const& f, Mr const& mr, hipStream_t st
 template <typename T, int D>
 nvtext_amd_status attend_chunks(ForwardChunks<T> const& f, hipStream_t stream)
 {
-  constexpr int kLds = 4 * Tile<T, D>::kBytes;
+  constexpr int kLds = 4 * Tile<T, D, kChunkTile>::kBytes;
   NVTEXT_HIP_TRY(allow_lds(attend_chunks_kernel<T, D>, kLds));
   {
     ProfileScope const scope("attention_chunks", stream);
     hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_chunks_kernel<T, D>), grid_of(work_items(f.key_runs.blocks(f.shift), f.kv_heads, 1, 1), kWave), dim3(kWave), kLds, stream, f);
   }
+  // A row that sees its own tokens has a single chunk.
+  if (f.own_keys()) return NVTEXT_AMD_SUCCESS;
+  // As many workgroups a head of a row as it has tokens on average, and no more than one that is split can have, nor than one where rows have a chunk on average.
+  int64_t const rows = f.runs.rows, tokens = (f.runs.tokens + rows - 1) / rows, most = rows << f.shift < f.key_runs.tokens ? std::max(1, kPartColumns / (f.heads / f.kv_heads)) : 1;
+  int32_t const apart = static_cast<int32_t>(std::clamp<int64_t>(tokens, 1, most));
+  int64_t const items = rows * f.heads * apart;
   ProfileScope const scope("attention_join", stream);
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_join_kernel<T, D>), grid_of(static_cast<int64_t>(f.runs.tokens) * f.heads, kJoinWaves * kWave), dim3(kJoinWaves * kWave), 0, stream, f);
+  auto const join = [&](auto waves) {
+    constexpr int kWaves = decltype(waves)::value;
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_join_kernel<T, D, kWaves>), grid_of(items, kWaves * kWave), dim3(kWaves * kWave), 0, stream, f, apart);
+  };
+  // (where there are fewer than CUs, a row's parts are many: 1 row of 131,071 keys, 32 heads 18.8 us with 4 wavefronts)
+  if (items < device_cus())
+    join(std::integral_constant<int, 16>{});
+  else
+    join(std::integral_constant<int, 4>{});
   return NVTEXT_AMD_SUCCESS;
 }
 
@@ -443,17 +468,22 @@ nvtext_amd_status attention(Forward<T> f, Mr const& mr, hipStream_t stream)
   align.add(f.q, f.runs.tokens, f.heads);
   align.add(f.k, f.key_runs.tokens, f.kv_heads);
   align.add(f.v, f.key_runs.tokens, f.kv_heads);
-  bool const chunks = f.runs.rows > 0 && static_cast<int64_t>(f.runs.tokens) * (f.heads / f.kv_heads) <= static_cast<int64_t>(f.runs.rows) * kPartColumns;
-  int shift = 7;
-  while (shift < 30 && (static_cast<int64_t>(f.key_runs.tokens) * f.kv_heads >> shift) > 2048) ++shift;
+  // By what rows have on average; where there are more tokens than rows, some may have many all the same.  Rows that see their own tokens go in chunks
+  // where heads share keys: 1000 rows of 12 tokens, 16 heads over 4 of keys, 184 us in tiles, 130 in both; but 16, 28 and 48 tokens, 16 heads over 16, are
+  // 98, 108 and 148 us in tiles, 100, 114 and 166 in both.
+  int64_t const columns = static_cast<int64_t>(f.runs.tokens) * (f.heads / f.kv_heads), rows = f.runs.rows;
+  f.in_chunks           = rows > 0 && (f.own_keys() ? f.heads > f.kv_heads && columns <= rows * kFewColumns : columns <= rows * kPartColumns);
+  f.in_tiles            = !f.in_chunks || f.runs.tokens > rows;
+  f.shift               = 7;
+  while (f.shift < 30 && (static_cast<int64_t>(f.key_runs.tokens) * f.kv_heads >> f.shift) > 2048) ++f.shift;
   return with_tiles(f.width, [&](auto d) {
     constexpr int kD        = decltype(d)::value;
-    size_t const parts      = chunks ? static_cast<size_t>(most_parts(f.key_runs.tokens, shift)) * static_cast<size_t>(f.kv_heads) * kPartColumns : 0;
+    size_t const parts      = f.in_chunks ? static_cast<size_t>(most_parts(f.key_runs.tokens, f.shift)) * static_cast<size_t>(f.kv_heads) * kPartColumns : 0;
     TempParts<3> const temp(mr, {align.bytes(), parts * kD * sizeof(float), parts * sizeof(float4)});
     if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
     align.launch(temp.template part<char>(0), stream);
-    if (chunks) return attend_chunks<T, kD>({f, shift, temp.template part<float>(1), temp.template part<float4>(2)}, stream);
-    return attend_tiles<T, kD>(f, mr, stream);
+    nvtext_amd_status const st = f.in_chunks ? attend_chunks<T, kD>({f, temp.template part<float>(1), temp.template part<float4>(2)}, stream) : NVTEXT_AMD_SUCCESS;
+    return st == NVTEXT_AMD_SUCCESS && f.in_tiles ? attend_tiles<T, kD>(f, mr, stream) : st;
   });
 }
 
@@ -478,7 +508,7 @@ nvtext_amd_status nvtext_amd_attention(const nvtext_amd_heads* q, const nvtext_a
   nvtext_amd_status st = NVTEXT_AMD_SUCCESS;
   with_type(q->type, [&](auto zero) {
     using T = decltype(zero);
-    st      = attention<T>({problem_of<T>(q, k, v, rows, offsets, key_offsets, key_lengths, causal, scale), heads_of<T>(out), logsum, q->type == NVTEXT_AMD_TYPE_FLOAT32 ? nullptr : rest}, mr, stream);
+    st      = attention<T>({problem_of<T>(q, k, v, rows, offsets, key_offsets, key_lengths, causal, scale), heads_of<T>(out), logsum, q->type == NVTEXT_AMD_TYPE_FLOAT32 ? nullptr : rest, true, false, 0}, mr, stream);
   });
   if (st != NVTEXT_AMD_SUCCESS) return st;
   NVTEXT_HIP_TRY(hipGetLastError());

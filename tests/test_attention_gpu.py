@@ -542,3 +542,142 @@ def test_no_memory_for_temporaries():
     finally:
         mr.fail_after = None
     assert len(mr.live) == live
+
+
+# rows of few tokens among rows of many: some go in chunks of their keys and some in tiles, or a row of many columns through the chunks that it has
+MIXED = [
+    ([1] * 40 + [60], [3 * i for i in range(40)] + [300], 8, 2, 64, 0),
+    ([0] * 30 + [20, 1, 1, 1], [5] * 30 + [700, 200, 0, 129], 8, 2, 64, 0),
+    ([1, 2, 5, 9, 17, 40, 0, 3] * 4, None, 8, 2, 72, 0),
+    ([1, 1, 30], [900, 129, 1100], 2, 1, 128, 0),
+    ([2] * 9 + [33, 16, 17], [128, 127, 129, 1, 0, 2, 256, 257, 700, 128, 128, 129], 4, 2, 40, 8),
+    ([1] * 300, [1 + i % 140 for i in range(300)], 40, 8, 32, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("roomy", [False, True])
+@pytest.mark.parametrize("case", MIXED, ids=lambda c: f"{len(c[0])}x{sum(c[0])}")
+def test_rows_of_few_tokens_among_others(case, roomy, causal, dtype):
+    m = Made(case, dtype, roomy)
+    if roomy:
+        for first, last, n in zip(m.key_offsets[:-1], m.key_offsets[1:], m.key_lengths):
+            m.k[first + n:last] = m.v[first + n:last] = float("nan")
+    m.check_forward(causal)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_the_same_offsets_over_more_keys_than_tokens(dtype):
+    """One array of offsets for both, that ends behind the tokens: they are its first ones, and the keys are all there."""
+    rng = np.random.default_rng(16)
+    q, q64 = heads(rng, 12, 4, 64, dtype)
+    k, k64 = heads(rng, 1200, 2, 64, dtype)
+    rows = ints([0, 10, 1200])
+    for causal in (False, True):
+        want, log, off, log_off = orc.attention(q64, k64, k64, [0, 10, 12], [0, 10, 1200], causal=causal, **rounding(dtype))
+        out, saved = encoder.attention(q, k, k, rows, rows, causal=causal, keep=True)
+        near(out, want, off)
+        near(saved.logsum, log, log_off)
+
+
+@pytest.mark.parametrize("lengths,keys", [([4, 3, 1], [300, 200, 500]), ([150, 60], [1500, 100])])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_a_key_that_only_the_last_tokens_see(lengths, keys, value):
+    """In chunks and in shares of tiles: the tokens in front of it have what they have without."""
+    for dtype in TYPES:
+        m = Made((lengths, keys, 4, 2, 64, 0), dtype)
+        want, log, off, log_off = orc.attention(m.q64, m.k64, m.v64, **m.oracle_rows(), causal=True, **rounding(dtype))
+        last = [int(m.key_offsets[1]) - 1, int(m.key_offsets[2]) - 1]
+        m.k[last[0]] = value
+        m.v[last] = value
+        out, saved = encoder.attention(m.q, m.k, m.v, *m.rows(), causal=True, keep=True)
+        seen = [int(m.offsets[1]) - 1, int(m.offsets[2]) - 1]
+        pick = np.ones(len(m.q), bool)
+        pick[seen] = False
+        where = torch.from_numpy(pick).cuda()
+        near(out[where], want[pick], off[pick])
+        near(saved.logsum[:, where], log[:, pick], log_off[:, pick])
+        assert not torch.isfinite(out[seen[1]]).any()
+
+
+def test_two_streams_at_once():
+    rng = np.random.default_rng(17)
+    made = [Made((lengths, keys, 8, 2, 64, 0), BF16, seed=i) for i, (lengths, keys) in enumerate([([1] * 20, [400] * 20), ([500, 20], None), ([3000], None), ([1, 50], [900, 2000])])]
+    calls = [lambda m=m: encoder.attention(m.q, m.k, m.v, *m.rows(), causal=True) for m in made]
+    calls += [lambda m=m: encoder.attention_backward(m.g, m.q, m.k, m.v, m.saved, *m.rows(), causal=True) for m in made]
+    for m in made:
+        m.saved = encoder.attention(m.q, m.k, m.v, *m.rows(), causal=True, keep=True)[1]
+    wants = [c() for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for order in range(len(calls)):
+        for s, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[s].append(calls[order if s == 0 else len(calls) - 1 - order]())
+    torch.cuda.synchronize()
+    got[1].reverse()
+    for results in got:
+        for a, b in zip(results, wants):
+            assert all(torch.equal(x, y) for x, y in zip(a, b)) if isinstance(b, tuple) else torch.equal(a, b)
+
+
+@pytest.mark.parametrize("single", [True, False])
+def test_a_cache_of_more_than_2_to_31_values(single):
+    """Rows at its begin, across the value that no 32 bits count, and at its end, against the same rows in caches of their own."""
+    torch.manual_seed(18)
+    tokens, lengths = 17 * 2**20 + 5, [700, 600, 900]
+    cache = torch.empty(tokens, 1, 128, dtype=BF16, device="cuda")
+    starts = [3, 2**24 - 300, tokens - 900]
+    assert starts[1] * 128 < 2**31 < (starts[1] + 600) * 128
+    key_offsets = ints([starts[0], starts[1], starts[2], tokens])
+    for first, n in zip(starts, lengths):
+        cache[first:first + n] = torch.randn(n, 1, 128, device="cuda")
+    count = 1 if single else 140
+    offsets = ints([0, count, 2 * count, 3 * count])
+    q = torch.randn(3 * count, 4, 128, device="cuda").to(BF16)
+    out, saved = encoder.attention(q, cache, cache, offsets, key_offsets, ints(lengths), causal=True, keep=True)
+    small = torch.cat([cache[first:first + n] for first, n in zip(starts, lengths)])
+    want, want_saved = encoder.attention(q, small, small, offsets, ints(offsets_of(lengths)), causal=True, keep=True)
+    # (other numbers of chunks and shares: sums in another order, of exponentials that another maximum rounds)
+    assert ((out.float() - want.float()).abs() <= 2 * 2.0**-8 * (want.float().abs() + small.float().abs().max())).all()
+    assert ((saved.logsum - want_saved.logsum).abs() <= 1e-5 * (1 + want_saved.logsum.abs())).all()
+    del out
+    grads = encoder.attention_backward(q, q, cache, cache, saved, offsets, key_offsets, ints(lengths), causal=True)
+    wants = encoder.attention_backward(q, q, small, small, saved, offsets, ints(offsets_of(lengths)), causal=True)
+    bounds = [2.0**-7 * (w.float().abs() + w.float().abs().max()) for w in wants]
+    assert ((grads[0].float() - wants[0].float()).abs() <= bounds[0]).all()
+    for g, w, b in zip(grads[1:], wants[1:], bounds[1:]):
+        got = torch.cat([g[first:first + n] for first, n in zip(starts, lengths)])
+        assert ((got.float() - w.float()).abs() <= b).all()
+        assert not g[starts[0] + 700:starts[0] + 5000].any() and not g[starts[1] + 600:starts[1] + 5000].any()
+
+
+def test_tokens_far_apart():
+    """Tokens 2^23 values and more from one to the next."""
+    rng = np.random.default_rng(19)
+    for dtype in (F32, BF16):
+        m = Made(([3, 17], None, 2, 1, 64, 0), dtype)
+        far = torch.zeros(len(m.k), 2**23 + 8, dtype=dtype, device="cuda")
+        for i, x in enumerate((m.k, m.v)):
+            far[:, 64 * i:64 * i + 64] = x[:, 0]
+        m.k, m.v = far[:, None, :64], far[:, None, 64:128]
+        m.check_forward(True)
+        m.check_backward(True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_broadcast_inputs(dtype):
+    """One head's, or one token's, values in place of all: the gradients are those of every one of them."""
+    m = Made(([30, 45, 1], None, 4, 4, 64, 0), dtype)
+    for name in ("k", "v", "g"):
+        x = getattr(m, name)[:, :1].expand(-1, 4, -1)
+        setattr(m, name, x)
+        setattr(m, name + "64", x.double().cpu().numpy())
+    m.check_forward(True)
+    m.check_backward(True)
+    x = m.k[:1, :1].expand(len(m.q), 4, -1)
+    m.k, m.k64 = x, x.double().cpu().numpy()
+    m.check_forward(False)
+    m.check_backward(False)
