@@ -4,13 +4,18 @@
 namespace nvtext_amd {
 namespace {
 
-// Two launches, the first for q, the second for k and v: each makes the scores anew and adds up what is its own in registers, in one order at every
+// Two launches, the first for q, the second (of wide heads, a second and a third) for k and v: each makes the scores anew and adds up what is its own in registers, in one order at every
 // call.  (One launch for all three would have to add up q's gradient in memory, over all workgroups of keys: in parts of float32 or in any order.)
+//
 // Blocks of 32 rows of a tile that go through one stream of fragments.  Of narrow heads, whose rows are often short, one, so that none is gone through that has no row; of
 // wider ones two, which spares the wait for the first fragments of the second (16384 tokens in four rows, heads of 128: 3.56 -> 3.12 ms with the forward
 // pass; 131071 in 1024, heads of 64: 1.12 either way).
 template <typename T, int D>
 constexpr int kBlocksAtOnce = sizeof(T) == 2 && D == 128 ? 2 : 1;
+// Two rows' values and a sum of 1024 bytes are more than a lane's registers hold with the rest: one of the rows is read again, two products ahead, for every block
+// of 32, whose 384 products take longer than that (1135 tokens, 12 heads of 216 values in float32: that of q 307 -> 288 us, of k 253 -> 213).
+template <typename T, int D>
+constexpr bool kReadAgain = D * sizeof(T) > 768;
 
 template <typename T, int D, int WAVES>
 struct GradientShape {
@@ -58,22 +63,25 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
   };
   if (tiles > first_tile) load(first_tile);
   int64_t const at = static_cast<int64_t>(w.head) * f.runs.tokens + t;
-  Fragment<T> q[kSteps], g[kSteps];
-  float delta = 0.f;
+  constexpr bool kAgain = kReadAgain<T, D>;
+  Fragment<T> q[kSteps], g[kAgain ? 3 : kSteps];
+  const T* const grad = f.grad.at(t, w.head);
+  float delta         = 0.f;
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
-    q[s] = fragment_of(f.q.at(t, w.head), 16 * s + 8 * half, f.width, there);
-    g[s] = fragment_of(f.grad.at(t, w.head), 16 * s + 8 * half, f.width, there);
+    q[s]                  = fragment_of(f.q.at(t, w.head), 16 * s + 8 * half, f.width, there);
+    Fragment<T> const of  = fragment_of(grad, 16 * s + 8 * half, f.width, there);
+    if constexpr (!kAgain) g[s] = of;
     Fragment<T> const out = fragment_of(f.out.at(t, w.head), 16 * s + 8 * half, f.width, there);
     bool rests = false;
     if constexpr (sizeof(T) == 2) rests = f.rest != nullptr;
     if (rests) {
       auto const rest = load_raw8(f.rest + at * f.width + 16 * s + 8 * half, there ? f.width - 16 * s - 8 * half : 0);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) delta = fmaf(static_cast<float>(g[s][k]), with_rest(out[k], rest[k]), delta);
+      for (int k = 0; k < 8; ++k) delta = fmaf(static_cast<float>(of[k]), with_rest(out[k], rest[k]), delta);
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) delta = fmaf(static_cast<float>(g[s][k]), static_cast<float>(out[k]), delta);
+      for (int k = 0; k < 8; ++k) delta = fmaf(static_cast<float>(of[k]), static_cast<float>(out[k]), delta);
     }
   }
   Halves const both = halves(delta);
@@ -108,14 +116,15 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
           else return read.columns(k_block, (i - kFirst) % kColumns, 2 * b + (i - kFirst) / kColumns);
         },
         [&](auto slot, Fragment<T> const& x) {
-          constexpr int b = slot / kOfBlock, i = slot % kOfBlock;
+          constexpr int b = slot / kOfBlock, i = slot % kOfBlock, ahead = i + 2 - kSteps;
           int32_t const key = from + 32 * b;
+          if constexpr (kAgain && ahead >= 0 && ahead < kSteps) g[ahead % 3] = fragment_of(grad, 16 * ahead + 8 * half, f.width, there);
           if constexpr (i < kSteps) {
             if constexpr (i == 0) s = f32x16_t{};
             s = multiply32(x, q[i], s);
           } else if constexpr (i < kFirst) {
             if constexpr (i == kSteps) p = f32x16_t{};
-            p = multiply32(x, g[i - kSteps], p);
+            p = multiply32(x, g[kAgain ? (i - kSteps) % 3 : i - kSteps], p);
           } else {
             if constexpr (i == kFirst) {
 #pragma unroll
@@ -204,12 +213,14 @@ __global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES>::kWavesA
   int32_t const begin_tile = uniform(share_begin(total, w.share, shares)), end_tile = uniform(share_begin(total, w.share + 1, shares));
   int32_t const last_from = uniform(from_of(block0 + wave0 + 31)), first_from = uniform(from_of(block0 + wave0));
 
-  Fragment<T> k[kSteps], v[kK ? kSteps : 1];
+  constexpr bool kAgain = kReadAgain<T, D>;
+  Fragment<T> k[kSteps], v[kAgain ? 3 : kK ? kSteps : 1];
+  const T* const values = f.v.at(t, w.kv_head);
   int32_t const from = from_of(key);
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
     k[s] = fragment_of(f.k.at(t, w.kv_head), 16 * s + 8 * half, f.width, there && key < keys);
-    if constexpr (kK) v[s] = fragment_of(f.v.at(t, w.kv_head), 16 * s + 8 * half, f.width, there && key < keys);
+    if constexpr (kK && !kAgain) v[s] = fragment_of(values, 16 * s + 8 * half, f.width, there && key < keys);
   }
   TileReader<T, D> const read(lane);
   float const scale = f.scale * kLog2e;
@@ -267,14 +278,15 @@ __global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES>::kWavesA
           }
         },
         [&](auto slot, Fragment<T> const& x) {
-          constexpr int b = slot / kOfBlock, i = slot % kOfBlock;
+          constexpr int b = slot / kOfBlock, i = slot % kOfBlock, ahead = i + 2 - kSteps;
           int32_t const row0 = block + 32 * b;
+          if constexpr (kK && kAgain && ahead >= 0 && ahead < kSteps) v[ahead % 3] = fragment_of(values, 16 * ahead + 8 * half, f.width, there && key < keys);
           if constexpr (i < kSteps) {
             if constexpr (i == 0) s = f32x16_t{};
             s = multiply32(x, k[i], s);
           } else if constexpr (i < kFirst) {
             if constexpr (i == kSteps) p = f32x16_t{};
-            p = multiply32(x, v[i - kSteps], p);
+            p = multiply32(x, v[kAgain ? (i - kSteps) % 3 : i - kSteps], p);
           } else {
             if constexpr (i == kFirst) {
 #pragma unroll
