@@ -664,27 +664,30 @@ hipError_t allow_lds(Kernel kernel, int bytes)
   return bytes > 65536 ? hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) : hipSuccess;
 }
 
-// In how many shares the tiles of a workgroup go: so many that there are twice as many workgroups as run at once, two a CU (one, if two have no room in its
-// LDS), if that many have kLeastTiles tiles on average; and none where there are that many workgroups, or tiles take no longer than another launch.
-constexpr int64_t kMostShares = 16;
-inline int32_t splits_of(int64_t workgroups, int64_t tiles, int lds)
+// In how many shares a launch's tiles go: the number for which this time is least.  A tile takes PRODUCTS matrix products of 32 x 32 heads a wavefront, of 16-bit
+// types 0.33 + 0.0031 D us each for 64 keys while a CU has one workgroup (of two, each takes 3/2 of that, as far as LDS has room for two), of float32, whose products are
+// all that counts, 0.045 D.  Shares of a tile's rows are written and read again, at 2.5 TB/s, by another launch, 6 us.  Rows are taken to be alike, which is all the
+// host knows; of causal ones the last blocks have twice as many tiles as the average.  (bfloat16, us without and with: two rows of 1536 tokens, 8 heads of
+// 64 28 and 43, in 3 shares; one row of 8000, one head of 128 139 and 66, in 8; a step over one row of 2000, 12 heads of 64 117, 115 in 3, 144 in 6.)
+constexpr int kMostShares = 16;
+template <typename T, int D, int PRODUCTS>
+int32_t splits_of(Problem<T> const& p, Runs const& blocks, int32_t heads, int shift, Runs const& other, int64_t times, int lds)
 {
-  int64_t const at_once = (2 * lds > 160 * 1024 ? 1 : 2) * device_cus();
-  if (workgroups >= at_once || workgroups <= 0 || tiles < 3 * kLeastTiles) return 1;
-  return static_cast<int32_t>(std::min<int64_t>({(2 * at_once + workgroups - 1) / workgroups, tiles / kLeastTiles, kMostShares}));
-}
-
-// Workgroups with something to do, and what they have, as far as the host knows: rows are taken to be alike.
-struct Estimate {
-  int64_t workgroups, tiles;
-};
-template <typename T>
-Estimate estimate(Problem<T> const& p, Runs const& blocks, int32_t heads, int shift, Runs const& other, int tile, int64_t times)
-{
-  int64_t const rows = std::max(1, blocks.rows), length = (blocks.tokens + rows - 1) / rows;
-  int64_t const seen = (other.tokens + rows - 1) / rows, tiles = (seen + tile - 1) / tile;
-  // (causal, with as many tokens as keys: half of them on average)
-  return {rows * ((length + (1 << shift) - 1) >> shift) * heads, (p.causal && other.tokens <= blocks.tokens ? (tiles + 1) / 2 : tiles) * times};
+  constexpr int kTile  = Tile<T, D>::kHeads;
+  int64_t const rows   = std::max(1, blocks.rows), length = (blocks.tokens + rows - 1) / rows, seen = (other.tokens + rows - 1) / rows;
+  bool const half      = p.causal && other.tokens <= blocks.tokens;
+  double const most    = static_cast<double>((seen + kTile - 1) / kTile * times), tiles = half ? (most + times) / 2 : most;
+  double const tile    = PRODUCTS * (sizeof(T) == 2 ? 0.33 + 0.0031 * D : 0.045 * D) * kTile / 64;
+  double const per_cu  = static_cast<double>(rows * ((length + (1 << shift) - 1) >> shift) * heads) / device_cus();
+  double const bytes   = static_cast<double>(rows * length) * heads * D * sizeof(float) * (PRODUCTS > 3 ? 2 : 1);
+  auto const at_once   = [&](double n) { return n <= 1 ? n : 2 * lds > 160 * 1024 ? 1. : std::min(1 + (n - 1) / 2, 1.5); };
+  int32_t best         = 1;
+  double least         = INFINITY;
+  for (int32_t n = 1; n == 1 || (n <= kMostShares && n * kLeastTiles <= tiles); ++n) {
+    double const time = tile * std::max(tiles * per_cu / at_once(per_cu * n), most / n) + (n > 1 ? 6 + 2 * n * bytes / 2.5e6 : 0);
+    if (time < least) least = time, best = n;
+  }
+  return best;
 }
 
 // calls f with the width of the tiles that heads of `width` values go through

@@ -412,9 +412,8 @@ __global__ void __launch_bounds__(kThreads) attend_join_shares_kernel(Forward<T>
 template <typename T, int D>
 nvtext_amd_status attend_tiles(Forward<T> const& f, Mr const& mr, hipStream_t stream)
 {
-  using Shape      = ForwardShape<T, D, kTileWaves>;
-  Estimate const e = estimate(f, f.runs, f.heads, Shape::kShift, f.key_runs, Shape::kTile, 1);
-  Split split{splits_of(e.workgroups, e.tiles, Shape::kLds), nullptr, nullptr};
+  using Shape = ForwardShape<T, D, kTileWaves>;
+  Split split{splits_of<T, D, 2>(f, f.runs, f.heads, Shape::kShift, f.key_runs, 1, Shape::kLds), nullptr, nullptr};
   size_t const rows = split.splits > 1 ? static_cast<size_t>(f.runs.blocks(Shape::kShift) * f.heads * split.splits) << Shape::kShift : 0;
   TempParts<2> const temp(mr, {rows * D * sizeof(float), rows * sizeof(float4)});
   if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");

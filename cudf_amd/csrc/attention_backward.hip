@@ -434,10 +434,10 @@ nvtext_amd_status key_gradient_tiles(Backward<T> const& f, Split const& split, h
 template <typename T, int D>
 nvtext_amd_status gradient_tiles(Backward<T> const& f, Mr const& mr, hipStream_t stream)
 {
-  using OfQ        = GradientShape<T, D, kTileWaves>;
-  using OfK        = KeyShape<T, D, kTileWaves>;
-  Estimate const q = estimate(f, f.runs, f.heads, OfQ::kShift, f.key_runs, OfQ::kTile, 1), k = estimate(f, f.key_runs, f.kv_heads, OfK::kShift, f.runs, OfK::kTile, f.heads / f.kv_heads);
-  Split of_q{f.runs.tokens > 0 ? splits_of(q.workgroups, q.tiles, OfQ::kLds) : 1, nullptr, nullptr}, of_k{f.key_runs.tokens > 0 ? splits_of(k.workgroups, k.tiles, OfK::kLds) : 1, nullptr, nullptr};
+  using OfQ = GradientShape<T, D, kTileWaves>;
+  using OfK = KeyShape<T, D, kTileWaves>;
+  Split of_q{splits_of<T, D, 3>(f, f.runs, f.heads, OfQ::kShift, f.key_runs, 1, OfQ::kLds), nullptr, nullptr};
+  Split of_k{splits_of<T, D, (D > 96 ? 5 : 4)>(f, f.key_runs, f.kv_heads, OfK::kShift, f.runs, f.heads / f.kv_heads, OfK::kLds), nullptr, nullptr};
   TempParts<2> const temp(mr, {of_q.splits > 1 ? static_cast<size_t>(f.runs.blocks(OfQ::kShift) * f.heads * of_q.splits * OfQ::kRows * D) * sizeof(float) : 0,
                                of_k.splits > 1 ? static_cast<size_t>(f.key_runs.blocks(OfK::kShift) * f.kv_heads * of_k.splits * OfK::kRows * D) * 2 * sizeof(float) : 0});
   if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
