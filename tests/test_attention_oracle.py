@@ -148,3 +148,13 @@ def test_rotary_frequencies():
     for bad in (dict(width=7), dict(width=0), dict(width=8, base=0.0), dict(width=8, factor=-1.0), dict(width=8, factor=float("nan")), dict(width=8, length=-1), dict(width=8, length=5, slow=2.0, fast=2.0)):
         with pytest.raises(ValueError):
             encoder.rotary_frequencies(device="cpu", **bad)
+
+
+@pytest.mark.parametrize("tokens,count,kv,text", [(2**31 - 1, 1, 1, "at most"), (1, 65537, 1, "at most"), (1, 65537, 65537, "at most"), (2**31 - 2000, 65536, 1, "too many tokens")])
+def test_sizes_that_are_not_counted(tokens, count, kv, text):
+    """More tokens than 32 bits count to a tile's end, and heads without end."""
+    q, k = (_capi.Heads(4096, tokens, n, 8, 0, 0, _capi.TYPE_FLOAT32) for n in (count, kv))
+    out, more = (_capi.Heads(4096, tokens, n, 8, n * 8, 8, _capi.TYPE_FLOAT32) for n in (count, kv))
+    lib = _capi.load()
+    refused(lib.nvtext_amd_attention(q, k, k, 1, 4096, None, None, 0, 1.0, None, None, out, None, None), text)
+    refused(lib.nvtext_amd_attention_backward(q, q, k, k, q, 4096, None, 1, 4096, None, None, 0, 1.0, None, None, out, more, more), text)
