@@ -505,6 +505,13 @@ __device__ __forceinline__ void store_rests(int8_t* head, f32x16_t const (&x)[CO
 // ------------------------------------------------------------------ work
 constexpr int kThreads = 256;
 constexpr int kTileWaves = 4;  // wavefronts that share the tiles in LDS
+// Of rows that have at most kShortRow tokens on average, a wavefront alone: blocks of 32 tokens and tiles of 32 keys, so that nothing waits for what is not there.
+// (60,000 tokens, 8 heads, a step in bfloat16, us with four wavefronts and with one: rows of 12 tokens, heads of 64 1127 and 478, of 128 2547 and 1445; of 48 tokens
+// 435 and 330, 945 and 841; of 100 367 and 352, 784 and 882.  Where tiles go in shares, keys are many, and four go on sharing them.)
+constexpr int kShortRow = 64;
+inline bool is_short(Runs const& runs) { return runs.rows > 0 && runs.tokens <= static_cast<int64_t>(runs.rows) * kShortRow; }
+template <typename T, int D, int WAVES>
+constexpr int kTileOf = WAVES == 1 ? 32 : Tile<T, D>::kHeads;
 
 // The work of a launch: blocks of tokens, of every head, in `splits` shares.  The heads that share a key head come one after the other on one XCD (workgroups go
 // to the eight XCDs in turn), and so do, where the number of key heads allows, the blocks of a key head: its keys come from that XCD's L2.  The last

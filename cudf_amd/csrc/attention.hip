@@ -18,7 +18,8 @@ __device__ __forceinline__ bool goes_in_chunks(Forward<T> const& f, int32_t toke
 // ------------------------------------------------------------------ forward, in tiles
 template <typename T, int D, int WAVES>
 struct ForwardShape {
-  static constexpr int kTokens = 32 * WAVES, kShift = __builtin_ctz(kTokens), kTile = Tile<T, D>::kHeads, kLds = 4 * Tile<T, D>::kBytes, kWavesASimd = D * sizeof(T) <= 128 ? 4 : D * sizeof(T) <= 256 ? 2 : 1;
+  static constexpr int kTokens = 32 * WAVES, kShift = __builtin_ctz(kTokens), kTile = kTileOf<T, D, WAVES>, kBytes = Tile<T, D, kTile>::kBytes, kLds = 4 * kBytes;
+  static constexpr int kWavesASimd = D * sizeof(T) <= 128 ? 4 : D * sizeof(T) <= 256 ? 2 : 1;
 };
 
 // What a wavefront holds of 32 heads of tokens, columns of the products, while keys pass: q, and the sums of out, transposed.  Scores are products with the
@@ -160,7 +161,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES>::kWa
   using Shape = ForwardShape<T, D, WAVES>;
   extern __shared__ __align__(16) char lds_[];
   LdsBytes const lds  = (LdsBytes)lds_;
-  constexpr int kTile = Shape::kTile, kStage = 2 * Tile<T, D>::kBytes;
+  constexpr int kTile = Shape::kTile, kStage = 2 * Shape::kBytes;
   Work w;
   int32_t const each = f.heads / f.kv_heads;
   if (!work_of(block_number(), f.runs.blocks(Shape::kShift), f.kv_heads, each, split.splits, w)) return;
@@ -186,16 +187,16 @@ __global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES>::kWa
   if (w.share >= shares) return;
   int32_t const from = uniform(share_begin(all_tiles, w.share, shares)), tiles = uniform(share_begin(all_tiles, w.share + 1, shares));
 
-  Attending<T, D> a;
+  Attending<T, D, kTile> a;
   a.seen = there ? f.seen(block0 + wave0 + column, tokens, keys) : 0;
   a.begin(f.q.at(t, w.head), f.width, there, half);
-  TileLoader<T, D, WAVES> load_k, load_v;
+  TileLoader<T, D, WAVES, kTile> load_k, load_v;
   load_k.aim(f.k, first + from * kTile, w.kv_head, f.width, wave, lane);
   load_v.aim(f.v, first + from * kTile, w.kv_head, f.width, wave, lane);
   auto const load = [&](int32_t tile) {
     LdsBytes const to = lds + (tile & 1) * kStage;
     load_k.load(to, keys - tile * kTile, wave);
-    load_v.load(to + Tile<T, D>::kBytes, keys - tile * kTile, wave);
+    load_v.load(to + Shape::kBytes, keys - tile * kTile, wave);
   };
   TileReader<T, D> const read(lane);
   float const scale = f.scale * kLog2e;
@@ -205,7 +206,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES>::kWa
     stage_barrier<0>();
     if (tile + 1 < tiles) load(tile + 1);
     int32_t const key0 = tile * kTile;
-    if (key0 < most) a.pass(k_tile, k_tile + Tile<T, D>::kBytes, read, key0, key0 + kTile > least, scale, half);
+    if (key0 < most) a.pass(k_tile, k_tile + Shape::kBytes, read, key0, key0 + kTile > least, scale, half);
   }
   if (wave0 >= rest) return;
   if (shares > 1) {
@@ -415,6 +416,17 @@ __global__ void __launch_bounds__(kThreads) attend_join_shares_kernel(Forward<T>
 }
 
 // ------------------------------------------------------------------ launches
+template <typename T, int D, int WAVES>
+nvtext_amd_status launch_tiles(Forward<T> const& f, Split const& split, hipStream_t stream)
+{
+  using Shape = ForwardShape<T, D, WAVES>;
+  ProfileScope const scope("attention_tiles", stream);
+  NVTEXT_HIP_TRY(allow_lds(attend_tiles_kernel<T, D, WAVES>, Shape::kLds));
+  int64_t const items = work_items(f.runs.blocks(Shape::kShift), f.kv_heads, f.heads / f.kv_heads, split.splits);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_tiles_kernel<T, D, WAVES>), grid_of(items, WAVES * kWave), dim3(WAVES * kWave), Shape::kLds, stream, f, split);
+  return NVTEXT_AMD_SUCCESS;
+}
+
 template <typename T, int D>
 nvtext_amd_status attend_tiles(Forward<T> const& f, Mr const& mr, hipStream_t stream)
 {
@@ -425,13 +437,9 @@ nvtext_amd_status attend_tiles(Forward<T> const& f, Mr const& mr, hipStream_t st
   if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
   split.sums = temp.template part<float>(0);
   split.tops = temp.template part<float4>(1);
-  NVTEXT_HIP_TRY(allow_lds(attend_tiles_kernel<T, D, kTileWaves>, Shape::kLds));
-  {
-    ProfileScope const scope("attention_tiles", stream);
-    int64_t const items = work_items(f.runs.blocks(Shape::kShift), f.kv_heads, f.heads / f.kv_heads, split.splits);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_tiles_kernel<T, D, kTileWaves>), grid_of(items, kTileWaves * kWave), dim3(kTileWaves * kWave), Shape::kLds, stream, f, split);
-  }
-  if (split.splits == 1) return NVTEXT_AMD_SUCCESS;
+  if (split.splits == 1) return is_short(f.runs) ? launch_tiles<T, D, 1>(f, split, stream) : launch_tiles<T, D, kTileWaves>(f, split, stream);
+  nvtext_amd_status const st = launch_tiles<T, D, kTileWaves>(f, split, stream);
+  if (st != NVTEXT_AMD_SUCCESS) return st;
   ProfileScope const scope("attention_join", stream);
   hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_join_shares_kernel<T, D>), grid_of((static_cast<int64_t>(f.runs.tokens) * f.heads + 3) / 4, kThreads), dim3(kThreads), 0, stream, f, split,
                      int{Shape::kShift});
@@ -474,10 +482,10 @@ nvtext_amd_status attention(Forward<T> f, Mr const& mr, hipStream_t stream)
   align.add(f.k, f.key_runs.tokens, f.kv_heads);
   align.add(f.v, f.key_runs.tokens, f.kv_heads);
   // By what rows have on average; where there are more tokens than rows, some may have many all the same.  Rows that see their own tokens go in chunks
-  // where heads share keys: 1000 rows of 12 tokens, 16 heads over 4 of keys, 184 us in tiles, 130 in both; but 16, 28 and 48 tokens, 16 heads over 16, are
-  // 98, 108 and 148 us in tiles, 100, 114 and 166 in both.
+  // where four heads or more share keys: 1000 rows of 12 tokens, 16 heads of 128 over 4 of keys, 100 us in tiles, 92 in both; of 20 tokens, 16 heads of 64 over 8, 54
+  // and 71.
   int64_t const columns = static_cast<int64_t>(f.runs.tokens) * (f.heads / f.kv_heads), rows = f.runs.rows;
-  f.in_chunks           = rows > 0 && (f.own_keys() ? f.heads > f.kv_heads && columns <= rows * kFewColumns : columns <= rows * kPartColumns);
+  f.in_chunks           = rows > 0 && (f.own_keys() ? f.heads >= 4 * static_cast<int64_t>(f.kv_heads) && columns <= rows * kFewColumns : columns <= rows * kPartColumns);
   f.in_tiles            = !f.in_chunks || f.runs.tokens > rows;
   f.shift               = 7;
   while (f.shift < 30 && (static_cast<int64_t>(f.key_runs.tokens) * f.kv_heads >> f.shift) > 2048) ++f.shift;

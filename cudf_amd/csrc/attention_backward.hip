@@ -19,7 +19,8 @@ constexpr bool kReadAgain = D * sizeof(T) > 768;
 
 template <typename T, int D, int WAVES>
 struct GradientShape {
-  static constexpr int kRows = 32 * WAVES, kShift = __builtin_ctz(kRows), kTile = Tile<T, D>::kHeads, kStage = 2 * Tile<T, D>::kBytes, kLds = 2 * kStage, kWavesASimd = D * sizeof(T) <= 256 ? 2 : 1;
+  static constexpr int kRows = 32 * WAVES, kShift = __builtin_ctz(kRows), kTile = kTileOf<T, D, WAVES>, kBytes = Tile<T, D, kTile>::kBytes, kStage = 2 * kBytes, kLds = 2 * kStage;
+  static constexpr int kWavesASimd = D * sizeof(T) <= 256 ? 2 : 1;
 };
 
 // The gradient of q: as forward, a lane has a token's scores, and what they are multiplied with comes from LDS, keys as they lie and transposed.
@@ -31,7 +32,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
   using Shape = GradientShape<T, D, WAVES>;
   extern __shared__ __align__(16) char lds_[];
   LdsBytes const lds = (LdsBytes)lds_;
-  constexpr int kSteps = D / 16, kColumns = D / 32, kTile = Shape::kTile, kAtOnce = kBlocksAtOnce<T, D>;
+  constexpr int kSteps = D / 16, kColumns = D / 32, kTile = Shape::kTile, kAtOnce = kTile == 32 ? 1 : kBlocksAtOnce<T, D>;
   Work w;
   int32_t const each = f.heads / f.kv_heads;
   if (!work_of(block_number(), f.runs.blocks(Shape::kShift), f.kv_heads, each, split.splits, w)) return;
@@ -55,13 +56,13 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
   int64_t const t     = static_cast<int64_t>(begin) + block0 + (there ? wave0 + column : 0);
   int32_t const seen  = there ? f.seen(block0 + wave0 + column, tokens, keys) : 0;
 
-  TileLoader<T, D, WAVES> load_k, load_v;
+  TileLoader<T, D, WAVES, kTile> load_k, load_v;
   load_k.aim(f.k, first + first_tile * kTile, w.kv_head, f.width, wave, lane);
   load_v.aim(f.v, first + first_tile * kTile, w.kv_head, f.width, wave, lane);
   auto const load = [&](int32_t tile) {
     LdsBytes const to = lds + (tile & 1) * Shape::kStage;
     load_k.load(to, keys - tile * kTile, wave);
-    load_v.load(to + Tile<T, D>::kBytes, keys - tile * kTile, wave);
+    load_v.load(to + Shape::kBytes, keys - tile * kTile, wave);
   };
   if (tiles > first_tile) load(first_tile);
   int64_t const at = static_cast<int64_t>(w.head) * f.runs.tokens + t;
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
     Fragment<T> ds[2];
 #pragma unroll 1
     for (int32_t from = key0; from < key0 + kTile && from < most; from += 32 * kAtOnce) {
-      LdsBytes const k_block = k_tile + (from - key0) * Tile<T, D>::kLine, v_block = k_block + Tile<T, D>::kBytes;
+      LdsBytes const k_block = k_tile + (from - key0) * Tile<T, D>::kLine, v_block = k_block + Shape::kBytes;
       stream<T, D, kAtOnce * kOfBlock>(
         [&](auto slot) {
           constexpr int b = slot / kOfBlock, i = slot % kOfBlock;
@@ -169,7 +170,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
 // heads that share keys go through one wavefront: each key's gradient is added up in one place.)
 template <typename T, int D, int WAVES>
 struct KeyShape {
-  static constexpr int kRows = 32 * WAVES, kShift = __builtin_ctz(kRows), kTile = Tile<T, D>::kHeads, kTiles = 2 * Tile<T, D>::kBytes;
+  static constexpr int kRows = 32 * WAVES, kShift = __builtin_ctz(kRows), kTile = kTileOf<T, D, WAVES>, kBytes = Tile<T, D, kTile>::kBytes, kTiles = 2 * kBytes;
   static constexpr int kStage = kTiles + 2 * kWave * 4, kLds = 2 * kStage;  // (with logs and deltas)
   static constexpr int kWavesASimd = sizeof(T) == 2 && D <= 128 ? 2 : 1;
 };
@@ -183,7 +184,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES>::kWavesA
   extern __shared__ __align__(16) char lds_[];
   LdsBytes const lds = (LdsBytes)lds_;
   constexpr bool kK = PART != kOfV, kV = PART != kOfK;
-  constexpr int kSteps = D / 16, kColumns = D / 32, kTile = Shape::kTile, kAtOnce = kBlocksAtOnce<T, D>;
+  constexpr int kSteps = D / 16, kColumns = D / 32, kTile = Shape::kTile, kAtOnce = kTile == 32 ? 1 : kBlocksAtOnce<T, D>;
   Work w;
   if (!work_of(block_number(), f.key_runs.blocks(Shape::kShift), f.kv_heads, 1, split.splits, w)) return;
   w.block              = f.key_runs.blocks(Shape::kShift) - 1 - w.block;  // (of a long row, the first keys are those that most tokens see)
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES>::kWavesA
     if constexpr (kK) dk[c] = f32x16_t{};
     if constexpr (kV) dv[c] = f32x16_t{};
   }
-  TileLoader<T, D, WAVES> load_q, load_g;
+  TileLoader<T, D, WAVES, kTile> load_q, load_g;
   int32_t loaded = uniform(of_head > 0 ? begin_tile % of_head : 0), next_head = uniform(w.kv_head * each + (of_head > 0 ? begin_tile / of_head : 0));  // the tile of the head that is loaded next
   bool aimed = false;
   auto const load = [&](LdsBytes to) {
@@ -245,7 +246,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES>::kWavesA
     }
     int32_t const token = (start + loaded) * kTile, here = tokens - token;
     load_q.load(to, here, wave);
-    load_g.load(to + Tile<T, D>::kBytes, here, wave);
+    load_g.load(to + Shape::kBytes, here, wave);
     int64_t const at = static_cast<int64_t>(next_head) * f.runs.tokens + begin + token;
     uint32_t const range = uniform(static_cast<uint32_t>(here < kTile ? here : kTile) * 4);
     if (wave == 0) load_words_to_lds(uniform(reinterpret_cast<const char*>(f.logs + at)), range, to + Shape::kTiles, lane * 4);
@@ -269,7 +270,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES>::kWavesA
 #pragma unroll 1
     for (int32_t block = token0; block < token0 + kTile && block < tokens; block += 32 * kAtOnce) {
       if (block + 32 * kAtOnce <= first_from) continue;
-      LdsBytes const q_block = q_tile + (block - token0) * Tile<T, D>::kLine, g_block = q_block + Tile<T, D>::kBytes, words = q_tile + Shape::kTiles + 16 * half + (block - token0) * 4;
+      LdsBytes const q_block = q_tile + (block - token0) * Tile<T, D>::kLine, g_block = q_block + Shape::kBytes, words = q_tile + Shape::kTiles + 16 * half + (block - token0) * 4;
       stream<T, D, kAtOnce * kOfBlock>(
         [&](auto slot) {
           constexpr int b = slot / kOfBlock, i = slot % kOfBlock;
@@ -424,14 +425,36 @@ __global__ void __launch_bounds__(kThreads) key_gradient_join_kernel(Backward<T>
 }
 
 // ------------------------------------------------------------------ launches
-template <typename T, int D, Part PART>
+template <typename T, int D, int WAVES, Part PART>
 nvtext_amd_status key_gradient_tiles(Backward<T> const& f, Split const& split, hipStream_t stream)
 {
-  using Shape = KeyShape<T, D, kTileWaves>;
+  using Shape = KeyShape<T, D, WAVES>;
   ProfileScope const scope("attention_key_gradient", stream);
-  NVTEXT_HIP_TRY(allow_lds(key_gradient_tiles_kernel<T, D, kTileWaves, PART>, Shape::kLds));
+  NVTEXT_HIP_TRY(allow_lds(key_gradient_tiles_kernel<T, D, WAVES, PART>, Shape::kLds));
   int64_t const items = work_items(f.key_runs.blocks(Shape::kShift), f.kv_heads, 1, split.splits);
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(key_gradient_tiles_kernel<T, D, kTileWaves, PART>), grid_of(items, kTileWaves * kWave), dim3(kTileWaves * kWave), Shape::kLds, stream, f, split);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(key_gradient_tiles_kernel<T, D, WAVES, PART>), grid_of(items, WAVES * kWave), dim3(WAVES * kWave), Shape::kLds, stream, f, split);
+  return NVTEXT_AMD_SUCCESS;
+}
+
+template <typename T, int D, int WAVES>
+nvtext_amd_status key_gradient_parts(Backward<T> const& f, Split const& split, hipStream_t stream)
+{
+  if constexpr (D > 96) {
+    nvtext_amd_status const st = key_gradient_tiles<T, D, WAVES, kOfK>(f, split, stream);
+    return st == NVTEXT_AMD_SUCCESS ? key_gradient_tiles<T, D, WAVES, kOfV>(f, split, stream) : st;
+  } else {
+    return key_gradient_tiles<T, D, WAVES, kBoth>(f, split, stream);
+  }
+}
+
+template <typename T, int D, int WAVES>
+nvtext_amd_status query_gradient_tiles(Backward<T> const& f, Split const& split, hipStream_t stream)
+{
+  using Shape = GradientShape<T, D, WAVES>;
+  ProfileScope const scope("attention_query_gradient", stream);
+  NVTEXT_HIP_TRY(allow_lds(query_gradient_tiles_kernel<T, D, WAVES>, Shape::kLds));
+  int64_t const items = work_items(f.runs.blocks(Shape::kShift), f.kv_heads, f.heads / f.kv_heads, split.splits);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(query_gradient_tiles_kernel<T, D, WAVES>), grid_of(items, WAVES * kWave), dim3(WAVES * kWave), Shape::kLds, stream, f, split);
   return NVTEXT_AMD_SUCCESS;
 }
 
@@ -447,25 +470,16 @@ nvtext_amd_status gradient_tiles(Backward<T> const& f, Mr const& mr, hipStream_t
   if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
   of_q.sums = temp.template part<float>(0);
   of_k.sums = temp.template part<float>(1);
-  if (f.runs.tokens > 0) {
-    ProfileScope const scope("attention_query_gradient", stream);
-    NVTEXT_HIP_TRY(allow_lds(query_gradient_tiles_kernel<T, D, kTileWaves>, OfQ::kLds));
-    int64_t const items = work_items(f.runs.blocks(OfQ::kShift), f.kv_heads, f.heads / f.kv_heads, of_q.splits);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(query_gradient_tiles_kernel<T, D, kTileWaves>), grid_of(items, kTileWaves * kWave), dim3(kTileWaves * kWave), OfQ::kLds, stream, f, of_q);
-  }
+  nvtext_amd_status st = NVTEXT_AMD_SUCCESS;
+  if (f.runs.tokens > 0) st = of_q.splits == 1 && is_short(f.runs) ? query_gradient_tiles<T, D, 1>(f, of_q, stream) : query_gradient_tiles<T, D, kTileWaves>(f, of_q, stream);
+  if (st != NVTEXT_AMD_SUCCESS) return st;
   if (of_q.splits > 1) {
     ProfileScope const scope("attention_query_gradient_join", stream);
     hipLaunchKernelGGL(HIP_KERNEL_NAME(query_gradient_join_kernel<T, D>), grid_of((static_cast<int64_t>(f.runs.tokens) * f.heads + 3) / 4, kThreads), dim3(kThreads), 0, stream, f, of_q,
                        int{OfQ::kShift});
   }
   if (f.key_runs.tokens == 0) return NVTEXT_AMD_SUCCESS;
-  nvtext_amd_status st;
-  if constexpr (D > 96) {
-    st = key_gradient_tiles<T, D, kOfK>(f, of_k, stream);
-    if (st == NVTEXT_AMD_SUCCESS) st = key_gradient_tiles<T, D, kOfV>(f, of_k, stream);
-  } else {
-    st = key_gradient_tiles<T, D, kBoth>(f, of_k, stream);
-  }
+  st = of_k.splits == 1 && is_short(f.key_runs) ? key_gradient_parts<T, D, 1>(f, of_k, stream) : key_gradient_parts<T, D, kTileWaves>(f, of_k, stream);
   if (st != NVTEXT_AMD_SUCCESS || of_k.splits == 1) return st;
   ProfileScope const scope("attention_key_gradient_join", stream);
   hipLaunchKernelGGL(HIP_KERNEL_NAME(key_gradient_join_kernel<T, D>), grid_of((static_cast<int64_t>(f.key_runs.tokens) * f.kv_heads + 3) / 4, kThreads), dim3(kThreads), 0, stream, f, of_k,

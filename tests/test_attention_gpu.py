@@ -694,3 +694,14 @@ def test_heads_without_values():
         near(saved.logsum[:, :8], np.broadcast_to(np.log(counts), (4, 8)), np.full((4, 8), 2.0**-20))
         assert encoder.attention(q, k, k, rows, keys).shape == q.shape
         assert [g.shape for g in encoder.attention_backward(q, q, k, k, saved, rows, keys, causal=True)] == [q.shape, k.shape, k.shape]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [64, 72, 128, 160, 256])
+@pytest.mark.parametrize("count,kv", [(3, 3), (4, 2), (4, 1)])
+def test_short_rows_among_longer_ones(count, kv, width, dtype):
+    """Rows that a wavefront has alone, of no token up to several of its blocks."""
+    m = Made(([3, 32, 0, 33, 1, 64, 20, 150, 2, 31] * 3, None, count, kv, width, 0), dtype)
+    for causal in (False, True):
+        m.check_forward(causal)
+        m.check_backward(causal)
