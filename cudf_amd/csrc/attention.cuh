@@ -509,7 +509,7 @@ constexpr int kTileWaves = 4;  // wavefronts that share the tiles in LDS
 // (60,000 tokens, 8 heads, a step in bfloat16, us with four wavefronts and with one: rows of 12 tokens, heads of 64 1127 and 478, of 128 2547 and 1445; of 48 tokens
 // 435 and 330, 945 and 841; of 100 367 and 352, 784 and 882.  Where tiles go in shares, keys are many, and four go on sharing them.)
 constexpr int kShortRow = 64;
-inline bool is_short(Runs const& runs) { return runs.rows > 0 && runs.tokens <= static_cast<int64_t>(runs.rows) * kShortRow; }
+inline bool is_short(Runs const& runs, int32_t most = kShortRow) { return runs.rows > 0 && runs.tokens <= static_cast<int64_t>(runs.rows) * most; }
 template <typename T, int D, int WAVES>
 constexpr int kTileOf = WAVES == 1 ? 32 : Tile<T, D>::kHeads;
 

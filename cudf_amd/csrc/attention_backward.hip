@@ -17,6 +17,10 @@ constexpr int kBlocksAtOnce = sizeof(T) == 2 && D == 128 ? 2 : 1;
 template <typename T, int D>
 constexpr bool kReadAgain = D * sizeof(T) > 768;
 
+// Which rows a wavefront has alone (in float32, where the products take longest, rows of 128 tokens, 8 heads of 64: 1350 us with four wavefronts, 1150 with one).
+template <typename T>
+constexpr int32_t kShort = sizeof(T) == 4 ? 2 * kShortRow : kShortRow;
+
 template <typename T, int D, int WAVES>
 struct GradientShape {
   static constexpr int kRows = 32 * WAVES, kShift = __builtin_ctz(kRows), kTile = kTileOf<T, D, WAVES>, kBytes = Tile<T, D, kTile>::kBytes, kStage = 2 * kBytes, kLds = 2 * kStage;
@@ -471,7 +475,7 @@ nvtext_amd_status gradient_tiles(Backward<T> const& f, Mr const& mr, hipStream_t
   of_q.sums = temp.template part<float>(0);
   of_k.sums = temp.template part<float>(1);
   nvtext_amd_status st = NVTEXT_AMD_SUCCESS;
-  if (f.runs.tokens > 0) st = of_q.splits == 1 && is_short(f.runs) ? query_gradient_tiles<T, D, 1>(f, of_q, stream) : query_gradient_tiles<T, D, kTileWaves>(f, of_q, stream);
+  if (f.runs.tokens > 0) st = of_q.splits == 1 && is_short(f.runs, kShort<T>) ? query_gradient_tiles<T, D, 1>(f, of_q, stream) : query_gradient_tiles<T, D, kTileWaves>(f, of_q, stream);
   if (st != NVTEXT_AMD_SUCCESS) return st;
   if (of_q.splits > 1) {
     ProfileScope const scope("attention_query_gradient_join", stream);
@@ -479,7 +483,7 @@ nvtext_amd_status gradient_tiles(Backward<T> const& f, Mr const& mr, hipStream_t
                        int{OfQ::kShift});
   }
   if (f.key_runs.tokens == 0) return NVTEXT_AMD_SUCCESS;
-  st = of_k.splits == 1 && is_short(f.key_runs) ? key_gradient_parts<T, D, 1>(f, of_k, stream) : key_gradient_parts<T, D, kTileWaves>(f, of_k, stream);
+  st = of_k.splits == 1 && is_short(f.key_runs, kShort<T>) ? key_gradient_parts<T, D, 1>(f, of_k, stream) : key_gradient_parts<T, D, kTileWaves>(f, of_k, stream);
   if (st != NVTEXT_AMD_SUCCESS || of_k.splits == 1) return st;
   ProfileScope const scope("attention_key_gradient_join", stream);
   hipLaunchKernelGGL(HIP_KERNEL_NAME(key_gradient_join_kernel<T, D>), grid_of((static_cast<int64_t>(f.key_runs.tokens) * f.kv_heads + 3) / 4, kThreads), dim3(kThreads), 0, stream, f, of_k,
