@@ -24,6 +24,9 @@ struct Problem {
   bool causal;
   float scale;
 
+  // What the tiles multiply a score with for an exponent of 2: at least the smallest number there is, which changes no exponent by more than 2^-21 and leaves the -infinity of a masked
+  // one what it is; a scale of 0 would make it NaN.
+  __device__ __forceinline__ float exponent_scale() const { return fmaxf(scale * kLog2e, 0x1p-149f); }
   // whether keys are those of the tokens themselves, all of them
   bool own_keys() const { return key_runs.offsets == runs.offsets && key_runs.tokens == runs.tokens && !key_lengths; }
   // The keys of run `i` (a row's), of which there are `length`, from token `first` on.

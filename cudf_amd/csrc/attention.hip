@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES>::kWa
     load_v.load(to + Shape::kBytes, keys - tile * kTile, wave);
   };
   TileReader<T, D> const read(lane);
-  float const scale = f.scale * kLog2e;
+  float const scale = f.exponent_scale();
   if (tiles > from) load(from);
   for (int32_t tile = from; tile < tiles; ++tile) {
     LdsBytes const k_tile = lds + (tile & 1) * kStage;
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kWave, 1) attend_chunks_kernel(ForwardChunks<T
   int32_t const key_first = split ? static_cast<int32_t>(chunk << f.shift) : 0, key_last = split && keys - key_first > 1 << f.shift ? key_first + (1 << f.shift) : keys;
   int64_t const columns   = static_cast<int64_t>(tokens > 0 ? tokens : 0) * each;
   TileReader<T, D> const read(lane);
-  float const scale = f.scale * kLog2e;
+  float const scale = f.exponent_scale();
   for (int64_t column0 = split ? 0 : chunk * kPartColumns; column0 < columns; column0 += split ? columns : static_cast<int64_t>(chunks) * kPartColumns) {
     int64_t const mine = column0 + column;
     bool const there   = mine < columns;
