@@ -124,19 +124,19 @@ struct Attending {
   __device__ __forceinline__ float divisor() const { return whole(sizeof(T) == 2 ? weight : sum); }
 
   // Writes out and logsum of a column, head h of token t, where it is `there`; of those whose result is not finite, the lanes' numbers.  That may come from keys that the
-  // token does not see, whose exponentials of 0 were multiplied: such columns are done once more, by themselves.
+  // token does not see, whose exponentials of 0 were multiplied: such columns are done once more, by themselves.  One that sees nothing has zeros, whatever was added up.
   __device__ __forceinline__ uint32_t finish(Forward<T> const& f, int64_t t, int32_t h, bool there, int half, int column)
   {
-    float const total = whole(sum), part = seen > 0 ? 1.f / divisor() : 0.f;
+    float const total = whole(sum), part = 1.f / divisor();
     float check       = 0.f;  // (NaN if any is infinite or NaN)
 #pragma unroll
     for (int c = 0; c < kColumns; ++c)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        o[c][r] *= part;
-        check = fmaf(o[c][r], 0.f, check);
+        o[c][r] = seen > 0 ? o[c][r] * part : 0.f;
+        check   = fmaf(o[c][r], 0.f, check);
       }
-    uint64_t odd = __ballot(there && seen > 0 && check != 0.f);
+    uint64_t odd = __ballot(there && check != 0.f);
     odd          = (odd | odd >> 32) & 0xffffffffu;
     if (there && !(odd >> column & 1)) {
       store_columns<T, kColumns>(f.out.at(t, h), o, half, f.width);

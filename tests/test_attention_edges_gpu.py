@@ -4,7 +4,8 @@ import pytest
 import torch
 
 from cudf_amd import encoder
-from tests.test_attention_gpu import TYPES, Made
+from oracle import encoder_py as orc
+from tests.test_attention_gpu import TYPES, Made, near, rounding
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +34,23 @@ def test_a_scale_of_zero_and_tokens_that_see_nothing(case, dtype):
     out, saved = encoder.attention(m.q, m.k, m.v, *m.rows(), causal=True, scale=0.0, keep=True)
     assert not out[none].any() and (saved.logsum[:, none] == float("-inf")).all() and not (saved.rest is not None and saved.rest[:, none].any())
     m.check_backward(True, 0.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("case", UNSEEING, ids=str)
+def test_tokens_that_see_nothing(case, value, dtype):
+    """The last key of every row, which its last token alone sees, holds anything: those that see nothing have zeros, the others what they have without."""
+    m = Made(case, dtype)
+    want, log, off, log_off = orc.attention(m.q64, m.k64, m.v64, **m.oracle_rows(), causal=True, **rounding(dtype))
+    last = [int(b) - 1 for a, b in zip(m.key_offsets[:-1], m.key_offsets[1:]) if b > a]
+    m.v[last] = value
+    if value != value:
+        m.k[last] = value
+    out, saved = encoder.attention(m.q, m.k, m.v, *m.rows(), causal=True, keep=True)
+    pick = np.ones(len(m.q), bool)
+    pick[[int(b) - 1 for a, b in zip(m.offsets[:-1], m.offsets[1:]) if b > a]] = False
+    where, none = torch.from_numpy(pick).cuda(), torch.from_numpy(unseeing(m)).cuda()
+    near(out[where], want[pick], off[pick])
+    near(saved.logsum[:, where], log[:, pick], log_off[:, pick])
+    assert not out[none].any() and (saved.logsum[:, none] == float("-inf")).all() and not (saved.rest is not None and saved.rest[:, none].any())
