@@ -159,11 +159,11 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
   for (int c = 0; c < kColumns; ++c)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      d[c][r] *= f.scale;
-      check = fmaf(d[c][r], 0.f, check);
+      d[c][r] = seen > 0 ? d[c][r] * f.scale : 0.f;
+      check   = fmaf(d[c][r], 0.f, check);
     }
   // (as forward: a key that is not seen may have been multiplied by 0)
-  uint64_t odd = __ballot(there && seen > 0 && check != 0.f);
+  uint64_t odd = __ballot(there && check != 0.f);
   odd          = (odd | odd >> 32) & 0xffffffffu;
   if (there && !(odd >> column & 1)) store_columns<T, kColumns>(f.q_grad.at(t, w.head), d, half, f.width);
   for (; odd; odd &= odd - 1) query_gradient_row(f, begin + block0 + wave0 + __builtin_ctzll(odd), w.head);

@@ -54,3 +54,21 @@ def test_tokens_that_see_nothing(case, value, dtype):
     near(out[where], want[pick], off[pick])
     near(saved.logsum[:, where], log[:, pick], log_off[:, pick])
     assert not out[none].any() and (saved.logsum[:, none] == float("-inf")).all() and not (saved.rest is not None and saved.rest[:, none].any())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("case", UNSEEING, ids=str)
+def test_gradients_of_tokens_that_see_nothing(case, value, dtype):
+    """The same on the way back, with infinities in keys too."""
+    m = Made(case, dtype)
+    want, log, _, _ = orc.attention(m.q64, m.k64, m.v64, **m.oracle_rows(), causal=True)
+    out, logsum = torch.from_numpy(want).to(dtype).cuda(), torch.from_numpy(log).float().cuda()
+    wants, offs = orc.attention_backward(m.g64, m.q64, m.k64, m.v64, out.double().cpu().numpy(), logsum.double().cpu().numpy(), **m.oracle_rows(), causal=True, **rounding(dtype))
+    last = [int(b) - 1 for a, b in zip(m.key_offsets[:-1], m.key_offsets[1:]) if b > a]
+    m.k[last] = m.v[last] = value
+    q_grad, _, _ = encoder.attention_backward(m.g, m.q, m.k, m.v, encoder.AttentionSaved(out, logsum), *m.rows(), causal=True)
+    pick = np.ones(len(m.q), bool)
+    pick[[int(b) - 1 for a, b in zip(m.offsets[:-1], m.offsets[1:]) if b > a]] = False
+    near(q_grad[torch.from_numpy(pick).cuda()], wants[0][pick], offs[0][pick])
+    assert not q_grad[torch.from_numpy(unseeing(m)).cuda()].any()
