@@ -128,8 +128,8 @@ __device__ void attend_row(Forward<T> const& f, int32_t t, int32_t h)
   for (int32_t base = 0; base < seen; base += kWave) {
     int32_t const n = seen - base < kWave ? seen - base : kWave;
     float const s   = lane < n ? dot(q, f.k.at(first + base + lane, kh), f.width) * scale : -INFINITY;
-    float const now = fmaxf(top, wave_max(s));
-    float const p   = lane < n ? __builtin_amdgcn_exp2f(s - now) : 0.f, fade = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - now);
+    float const now = fmaxf(top, wave_max(s)), level = now == -INFINITY ? 0.f : now;  // (keys of no weight in front of others are no reason for NaN)
+    float const p   = lane < n ? __builtin_amdgcn_exp2f(s - level) : 0.f, fade = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - now);
     sum = sum * fade + wave_sum(p);
 #pragma unroll
     for (int c = 0; c < kMostWidth / kWave; ++c) o[c] *= fade;

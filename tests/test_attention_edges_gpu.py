@@ -1,4 +1,4 @@
-"""Attention where its kernels could go wrong unnoticed: tokens that see nothing next to tokens that do."""
+"""Attention where its kernels could go wrong unnoticed: tokens that see nothing next to tokens that do, keys of no weight in front of others."""
 import numpy as np
 import pytest
 import torch
@@ -72,3 +72,21 @@ def test_gradients_of_tokens_that_see_nothing(case, value, dtype):
     pick[[int(b) - 1 for a, b in zip(m.offsets[:-1], m.offsets[1:]) if b > a]] = False
     near(q_grad[torch.from_numpy(pick).cuda()], wants[0][pick], offs[0][pick])
     assert not q_grad[torch.from_numpy(unseeing(m)).cuda()].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("count,kv", [(2, 2), (4, 1)])
+def test_keys_of_no_weight_in_front_of_others(count, kv, dtype):
+    """The first 64 keys have scores of -infinity, so the first 64 tokens have no result, and a key that the last token alone sees holds NaN: the tokens
+    between have what the keys from 64 on come to."""
+    m = Made(([150], None, count, kv, 64, 0), dtype)
+    first, last = int(m.offsets[0]), int(m.offsets[1])
+    m.q[:, :, 0] = 1.0
+    m.k[first:first + 64, :, 0] = float("-inf")
+    q64, k64 = m.q.double().cpu().numpy(), m.k.double().cpu().numpy()
+    want, log, off, log_off = orc.attention(q64[first + 64:last], k64[first + 64:last], m.v64[first + 64:last], [0, 86], causal=True, **rounding(dtype))
+    m.v[last - 1] = float("nan")
+    out, saved = encoder.attention(m.q, m.k, m.v, *m.rows(), causal=True, keep=True)
+    near(out[first + 64:last - 1], want[:-1], off[:-1])
+    near(saved.logsum[:, first + 64:last - 1], log[:, :-1], log_off[:, :-1])
+    assert torch.isnan(out[first:first + 64]).all() and torch.isnan(out[last - 1]).all()
