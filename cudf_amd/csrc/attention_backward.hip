@@ -21,9 +21,47 @@ constexpr bool kReadAgain = D * sizeof(T) > 768;
 template <typename T>
 constexpr int32_t kShort = sizeof(T) == 4 ? 2 * kShortRow : kShortRow;
 
+// What is rounded to float16 before it is multiplied is brought into its range first.  d = p (grad . v - grad . out) lies anywhere: with gradients of 1e-3, a row of 4096 tokens
+// has d of 1e-6, where float16 has steps of 6e-8 (q's gradient was off by 0.25 %, of 1e-4 over 8192 tokens by 6 %; that of float16's own rounding is 0.04 and 0.9 %), and of a
+// loss that has been scaled up it may pass 65504.  So a column multiplies its d by a power of 2 of its own and its sums by the reciprocal at the end.  Its largest d so far lies between
+// 2^8 and 2^15 (or below, while the power is the first one), and only a larger one changes the power, and with it what has been added up: what is 2^-22 of
+// it and more keeps all its bits, and the rest is off by 2^-33 of it.  bfloat16 has the exponents of float32.  (Steps take 3 to 4 % longer for it: 131071 tokens in 1024 rows, 12 heads
+// of 64, 1121 -> 1159 us; 8192 in eight rows, 16 heads of 192, 720 -> 795, of 256 917 -> 1043.)
+template <typename T>
+constexpr bool kLifted = std::is_same_v<T, half_t>;
+struct Lift {
+  static constexpr float kMost = 0x1p15f;
+  float up = 0x1p60f;  // (d of inputs in float16 is below 2^41)
+  // d of 32 rows, of which this lane has 16, times the power; where that changes, what has been added up as well
+  template <int COLUMNS>
+  __device__ __forceinline__ void apply(f32x16_t& d, f32x16_t (&sums)[COLUMNS])
+  {
+    float high = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      d[r] *= up;
+      high = fmaxf(high, fabsf(d[r]));
+    }
+    Halves const both = halves(high);
+    high              = fmaxf(both.low, both.high);
+    if (__ballot(high > kMost)) {
+      float const by = high > kMost ? __builtin_amdgcn_ldexpf(1.f, 9 - __builtin_amdgcn_frexp_expf(high)) : 1.f;
+      up *= by;
+      d *= by;
+#pragma unroll
+      for (int c = 0; c < COLUMNS; ++c) sums[c] *= by;
+    }
+  }
+};
+
+// Wide heads in float16 go through tiles of one block of 32 rows: with a second loop, over a tile's blocks, around the place where the sums may change their power, the compiler keeps
+// 61 to 111 registers of them in memory.
+template <typename T, int D, int WAVES>
+constexpr int kTileOfGradient = kLifted<T> && D > 192 ? 32 : kTileOf<T, D, WAVES>;
+
 template <typename T, int D, int WAVES>
 struct GradientShape {
-  static constexpr int kRows = 32 * WAVES, kShift = __builtin_ctz(kRows), kTile = kTileOf<T, D, WAVES>, kBytes = Tile<T, D, kTile>::kBytes, kStage = 2 * kBytes, kLds = 2 * kStage;
+  static constexpr int kRows = 32 * WAVES, kShift = __builtin_ctz(kRows), kTile = kTileOfGradient<T, D, WAVES>, kBytes = Tile<T, D, kTile>::kBytes, kStage = 2 * kBytes, kLds = 2 * kStage;
   static constexpr int kWavesASimd = D * sizeof(T) <= 256 ? 2 : 1;
 };
 
@@ -98,6 +136,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
     f.deltas[at] = delta;
     f.logs[at]   = log;
   }
+  Lift lift;
   f32x16_t d[kColumns];
 #pragma unroll
   for (int c = 0; c < kColumns; ++c) d[c] = f32x16_t{};
@@ -141,6 +180,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = 8 * (r / 4) + r % 4 < left ? s[r] : 0.f;
               }
+              if constexpr (kLifted<T>) lift.apply(s, d);
               ds[0] = rounded<T>(s, 0);
               ds[1] = rounded<T>(s, 1);
             }
@@ -150,6 +190,11 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
     }
   }
   if (wave0 >= rest) return;
+  if constexpr (kLifted<T>) {
+    float const down = 1.f / lift.up;
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) d[c] *= down;
+  }
   if (shares > 1) {
     if (there) store_columns<float, kColumns>(split.sums + (split.slot(w.block, w.head, f.heads, w.share) * Shape::kRows + wave0 + column) * D, d, half, D);
     return;
@@ -174,7 +219,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
 // heads that share keys go through one wavefront: each key's gradient is added up in one place.)
 template <typename T, int D, int WAVES>
 struct KeyShape {
-  static constexpr int kRows = 32 * WAVES, kShift = __builtin_ctz(kRows), kTile = kTileOf<T, D, WAVES>, kBytes = Tile<T, D, kTile>::kBytes, kTiles = 2 * kBytes;
+  static constexpr int kRows = 32 * WAVES, kShift = __builtin_ctz(kRows), kTile = kTileOfGradient<T, D, WAVES>, kBytes = Tile<T, D, kTile>::kBytes, kTiles = 2 * kBytes;
   static constexpr int kStage = kTiles + 2 * kWave * 4, kLds = 2 * kStage;  // (with logs and deltas)
   static constexpr int kWavesASimd = sizeof(T) == 2 && D <= 128 ? 2 : 1;
 };
@@ -239,6 +284,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES>::kWavesA
     if constexpr (kK) dk[c] = f32x16_t{};
     if constexpr (kV) dv[c] = f32x16_t{};
   }
+  Lift lift;
   TileLoader<T, D, WAVES, kTile> load_q, load_g;
   int32_t loaded = uniform(of_head > 0 ? begin_tile % of_head : 0), next_head = uniform(w.kv_head * each + (of_head > 0 ? begin_tile / of_head : 0));  // the tile of the head that is loaded next
   bool aimed = false;
@@ -319,6 +365,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES>::kWavesA
                   if constexpr (kK) p[r] = sees ? p[r] : 0.f;
                 }
               }
+              if constexpr (kK && kLifted<T>) lift.apply(p, dk);
 #pragma unroll
               for (int step = 0; step < 2; ++step) {
                 if constexpr (kV) weight[step] = rounded<T>(s, step);
@@ -331,6 +378,11 @@ __global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES>::kWavesA
           }
         });
     }
+  }
+  if constexpr (kK && kLifted<T>) {
+    float const down = 1.f / lift.up;
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) dk[c] *= down;
   }
   if (shares > 1) {
     if (!there) return;
@@ -391,7 +443,7 @@ __device__ __forceinline__ bool write_row(T* head, Some<D> const& sum, int32_t w
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) query_gradient_join_kernel(Backward<T> f, Split split, int shift)
 {
-  constexpr int kTile = Tile<T, D>::kHeads;
+  constexpr int kTile = kTileOfGradient<T, D, kTileWaves>;
   int64_t const item  = block_number() * (kThreads / kWave) + threadIdx.x / kWave;
   if (item >= static_cast<int64_t>(f.runs.tokens) * f.heads) return;
   int32_t const t = static_cast<int32_t>(item / f.heads), head = static_cast<int32_t>(item % f.heads), run = run_with(f.runs, t);
@@ -408,7 +460,7 @@ __global__ void __launch_bounds__(kThreads) query_gradient_join_kernel(Backward<
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) key_gradient_join_kernel(Backward<T> f, Split split, int shift)
 {
-  constexpr int kTile = Tile<T, D>::kHeads;
+  constexpr int kTile = kTileOfGradient<T, D, kTileWaves>;
   int64_t const item  = block_number() * (kThreads / kWave) + threadIdx.x / kWave;
   if (item >= static_cast<int64_t>(f.key_runs.tokens) * f.kv_heads) return;
   int32_t const t = static_cast<int32_t>(item / f.kv_heads), head = static_cast<int32_t>(item % f.kv_heads), run = run_with(f.key_runs, t);

@@ -1,11 +1,12 @@
-"""Attention where its kernels could go wrong unnoticed: tokens that see nothing next to tokens that do, keys of no weight in front of others."""
+"""Attention where its kernels could go wrong unnoticed: tokens that see nothing next to tokens that do, keys of no weight in front of others, and
+float16 where what is multiplied is far below 1."""
 import numpy as np
 import pytest
 import torch
 
 from cudf_amd import encoder
 from oracle import encoder_py as orc
-from tests.test_attention_gpu import TYPES, Made, near, rounding
+from tests.test_attention_gpu import F16, TYPES, Made, ints, near, offsets_of, rounding
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +91,75 @@ def test_keys_of_no_weight_in_front_of_others(count, kv, dtype):
     near(out[first + 64:last - 1], want[:-1], off[:-1])
     near(saved.logsum[:, first + 64:last - 1], log[:, :-1], log_off[:, :-1])
     assert torch.isnan(out[first:first + 64]).all() and torch.isnan(out[last - 1]).all()
+
+
+class Long:
+    """Rows of many tokens in float16, and the gradients in 64 bits from out and logsum as they are given, with how far off a kernel's are to be expected: next to the rounding
+    of a result, of each product that is added up half a step of the value (`unit`) that is rounded before it is multiplied, wherever that value lies, and what 32 bits leave of it.
+    Roundings are independent of one another, so it is their squares that add up."""
+
+    def __init__(self, lengths, count, kv, width, causal, grad, raise_first=0.0, q_scale=1.0):
+        torch.manual_seed(len(lengths) + width)
+        self.lengths, self.causal, self.each, tokens = lengths, causal, count // kv, sum(lengths)
+        self.q, self.k, self.v, self.g = (torch.randn(tokens, n, width, device="cuda") * s for n, s in ((count, q_scale), (kv, 1.0), (kv, 1.0), (count, grad)))
+        self.offsets = offsets_of(lengths)
+        if raise_first:  # the first key of every row is what all its tokens look at
+            self.q[:, :, 0] = raise_first**0.5 * width**0.25
+            self.k[:, :, 0] = 0.0
+            self.k[self.offsets[:-1].tolist(), :, 0] = raise_first**0.5 * width**0.25
+        self.q, self.k, self.v, self.g = (x.to(F16) for x in (self.q, self.k, self.v, self.g))
+        self.scale = width**-0.5
+
+    def check(self):
+        unit, eps, width = 2.0**-11, 2.0**-24, self.q.shape[2]
+        out, logsum = torch.zeros_like(self.q), torch.full((self.q.shape[1], len(self.q)), float("-inf"), device="cuda")
+        wants = [torch.zeros(x.shape, dtype=torch.float64, device="cuda") for x in (self.q, self.k, self.v)]
+        squares = [torch.zeros_like(w) for w in wants]
+        for first, last in zip(self.offsets[:-1], self.offsets[1:]):
+            for h in range(self.q.shape[1]):
+                t, u = slice(first, last), h // self.each
+                q, k, v, g = self.q[t, h].double(), self.k[t, u].double(), self.v[t, u].double(), self.g[t, h].double()
+                s = q @ k.T.contiguous() * self.scale
+                if self.causal:
+                    s = s.masked_fill(torch.ones_like(s, dtype=torch.bool).triu(1), float("-inf"))
+                log = torch.logsumexp(s, 1)
+                out[t, h], logsum[h, t] = (torch.exp(s - log[:, None]) @ v).to(F16), log.float()
+                o, log = out[t, h].double(), logsum[h, t].double()
+                p = torch.exp(s - log[:, None])
+                product = g @ v.T.contiguous()
+                ds = p * (product - (g * o).sum(1)[:, None])
+                size = self.scale * (q.abs() @ k.abs().T.contiguous())
+                e = unit + orc.score_error(size, log.abs()[:, None], width, eps) + 8 * eps
+                more = 2 * (width + 4) * eps * (g.abs() @ v.abs().T.contiguous() + (g * o).abs().sum(1)[:, None])
+                ds_off, p_off = (e * ds.abs() + p * more) ** 2, (e * p) ** 2
+                wants[0][t, h] = self.scale * (ds @ k)
+                squares[0][t, h] = self.scale**2 * (ds_off @ k**2)
+                wants[1][t, u] += self.scale * (ds.T.contiguous() @ q)
+                squares[1][t, u] += self.scale**2 * (ds_off.T.contiguous() @ q**2)
+                wants[2][t, u] += p.T.contiguous() @ g
+                squares[2][t, u] += p_off.T.contiguous() @ g**2
+        self.wants, self.squares = wants, squares
+        got = encoder.attention_backward(self.g, self.q, self.k, self.v, encoder.AttentionSaved(out, logsum), ints(self.offsets), causal=self.causal)
+        return [self.error(x, w, s) for x, w, s in zip(got, wants, squares)]
+
+    def error(self, got, want, square, pick=slice(None)):
+        """(how far off, how far to be expected): (of a result, half a step, which is 2^-25 where it is smallest).  A result of more than float16 holds,
+        65520 and more as it is rounded, is an infinity; those that are off by less from that than by 2^-8 may be either."""
+        got, want, square = got[pick].double(), want[pick], square[pick]
+        beyond, below = want.abs() >= 65520 * (1 + 2.0**-8), want.abs() <= 65520 * (1 - 2.0**-8)
+        assert torch.equal(got[beyond], torch.copysign(torch.full_like(want[beyond], float("inf")), want[beyond]))
+        got, want, square = got[below], want[below], square[below]
+        half = torch.maximum(2.0**-11 * want.abs(), torch.full_like(want, 2.0**-25))
+        return (got - want).norm().item(), (square + half**2).sum().sqrt().item()
+
+
+@pytest.mark.parametrize("lengths,count,kv,width,causal,grad", [
+    ([4096], 2, 2, 64, False, 1e-3), ([2000], 4, 1, 64, True, 1e-3), ([2000], 4, 1, 128, True, 1e-4), ([8192], 1, 1, 64, False, 1e-4), ([1500, 700], 2, 1, 72, True, 1e-3),
+    ([300] * 12, 12, 6, 64, True, 1e-3), ([300] * 12, 12, 6, 128, False, 1e-3), ([40] * 50, 4, 2, 64, True, 1e-4), ([40] * 50, 4, 2, 256, False, 1e-4), ([1000], 2, 2, 256, True, 1e-3),
+    ([500], 2, 2, 64, False, 8e3), ([40] * 50, 4, 2, 128, True, 8e3),
+])
+def test_float16_gradients_keep_their_bits(lengths, count, kv, width, causal, grad):
+    """Probabilities of some thousandths and gradients of a loss that is a mean, or that has been scaled up: what is rounded before it is multiplied lies below float16's normal
+    numbers, or beyond its largest, but its sums do not."""
+    for name, (error, expected) in zip("qkv", Long(lengths, count, kv, width, causal, grad).check()):
+        assert error <= expected, (name, error, expected)
