@@ -157,7 +157,7 @@ struct Backward : Problem<T> {
   const float* logsum;
   const int8_t* rest;  // out's, or nullptr
   float* deltas;  // [heads, tokens]: grad . out
-  float* logs;    // [heads, tokens]: logsum in powers of 2 (the tiles' own)
+  float* logs;    // [heads, tokens]: logsum in powers of 2, as the tiles of k's and v's gradients take it
   Heads<T> q_grad, k_grad, v_grad;
 };
 

@@ -26,12 +26,16 @@ constexpr int32_t kShort = sizeof(T) == 4 ? 2 * kShortRow : kShortRow;
 // loss that has been scaled up it may pass 65504.  So a column multiplies its d by a power of 2 of its own and its sums by the reciprocal at the end.  Its largest d so far lies between
 // 2^8 and 2^15 (or below, while the power is the first one), and only a larger one changes the power, and with it what has been added up: what is 2^-22 of
 // it and more keeps all its bits, and the rest is off by 2^-33 of it.  bfloat16 has the exponents of float32.  (Steps take 3 to 4 % longer for it: 131071 tokens in 1024 rows, 12 heads
-// of 64, 1121 -> 1159 us; 8192 in eight rows, 16 heads of 192, 720 -> 795, of 256 917 -> 1043.)
+// of 64, 1121 -> 1165 us; 8192 in eight rows, 16 heads of 192, 720 -> 795, of 256 920 -> 968.)
 template <typename T>
 constexpr bool kLifted = std::is_same_v<T, half_t>;
+// And so are the probabilities that the gradient of v adds up, in which a key of little weight has 2^-20 (where one of 2000 keys has nearly all, the others' gradients were off by 2.5 %): they
+// are 1 at most, and go through the products 2^15 times as large.
+template <typename T>
+constexpr float kWeightLift = kLifted<T> ? 15.f : 0.f;
 struct Lift {
   static constexpr float kMost = 0x1p15f;
-  float up = 0x1p60f;  // (d of inputs in float16 is below 2^41)
+  float up = 0x1p60f;  // (d of inputs in float16 is below 2^41, of such probabilities 2^56)
   // d of 32 rows, of which this lane has 16, times the power; where that changes, what has been added up as well
   template <int COLUMNS>
   __device__ __forceinline__ void apply(f32x16_t& d, f32x16_t (&sums)[COLUMNS])
@@ -134,7 +138,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
   float const log   = there ? f.logsum[at] * kLog2e : 0.f;
   if (there && half == 0 && w.share == 0) {
     f.deltas[at] = delta;
-    f.logs[at]   = log;
+    f.logs[at]   = log - kWeightLift<T>;
   }
   Lift lift;
   f32x16_t d[kColumns];
@@ -379,10 +383,14 @@ __global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES>::kWavesA
         });
     }
   }
-  if constexpr (kK && kLifted<T>) {
-    float const down = 1.f / lift.up;
+  if constexpr (kLifted<T>) {
+    constexpr float kDown = 1.f / (1 << static_cast<int>(kWeightLift<T>));
+    float const down      = kDown / lift.up;
 #pragma unroll
-    for (int c = 0; c < kColumns; ++c) dk[c] *= down;
+    for (int c = 0; c < kColumns; ++c) {
+      if constexpr (kK) dk[c] *= down;  // (whose d are made of the same probabilities)
+      if constexpr (kV) dv[c] *= kDown;
+    }
   }
   if (shares > 1) {
     if (!there) return;

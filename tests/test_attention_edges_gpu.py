@@ -163,3 +163,24 @@ def test_float16_gradients_keep_their_bits(lengths, count, kv, width, causal, gr
     numbers, or beyond its largest, but its sums do not."""
     for name, (error, expected) in zip("qkv", Long(lengths, count, kv, width, causal, grad).check()):
         assert error <= expected, (name, error, expected)
+
+
+def self_log(m, first, last, h):
+    s = m.q[first:last, h].double() @ m.k[first:last, h // m.each].double().T.contiguous() * m.scale
+    if m.causal:
+        s = s.masked_fill(torch.ones_like(s, dtype=torch.bool).triu(1), float("-inf"))
+    return torch.logsumexp(s, 1).float()
+
+
+@pytest.mark.parametrize("lengths,count,kv,width,causal", [([2000], 2, 1, 64, True), ([900] * 3, 4, 4, 128, False), ([60] * 40, 4, 2, 64, True), ([500] * 4, 4, 4, 256, False)])
+def test_float16_probabilities_keep_their_bits(lengths, count, kv, width, causal):
+    """One key has nearly all the weight of all tokens: the gradients of the others' values are sums of probabilities of 2^-20."""
+    m = Long(lengths, count, kv, width, causal, 50.0, raise_first=14.0, q_scale=0.3)
+    m.check()
+    out = torch.zeros_like(m.q)
+    others = torch.ones(len(m.q), dtype=torch.bool, device="cuda")
+    others[m.offsets[:-1].tolist()] = False
+    logsum = torch.stack([torch.cat([self_log(m, a, b, h) for a, b in zip(m.offsets[:-1], m.offsets[1:])]) for h in range(count)])
+    v_grad = encoder.attention_backward(m.g, m.q, m.k, m.v, encoder.AttentionSaved(out, logsum), ints(m.offsets), causal=causal)[2]
+    error, expected = m.error(v_grad, m.wants[2], m.squares[2], others)
+    assert error <= expected, (error, expected)
