@@ -25,11 +25,12 @@ struct ForwardShape {
 // What a wavefront holds of 32 heads of tokens, columns of the products, while keys pass: q, and the sums of out, transposed.  Scores are products with the
 // keys as rows, so a lane has all of a column's scores (with the one 32 further on), and exponentials are in its registers as the second product
 // takes them: no lane needs another's but for the maximum.  Sums are kept in proportion to 2^top, where top is a maximum that may be 8 too small:
-// only then are they multiplied anew.
+// only then are they multiplied anew.  In float16 top is 7 less, so that exponentials go up to 2^15 of the 65504 that it holds: its normal numbers end at 2^-14, and a weight is off by 2^-32 of
+// the largest at most, where without these 7 a long row's many weights of less than 2^-25 were lost (131071 of 2^-24.4: 0.6 % of the sum, a third of it off).
 template <typename T, int D, int TILE = Tile<T, D>::kHeads>
 struct Attending {
   static constexpr int kSteps = D / 16, kColumns = D / 32, kTile = TILE, kBlocks = kTile / 32;
-  static constexpr float kSlack = 8.f;
+  static constexpr float kSlack = 8.f, kRoom = std::is_same_v<T, half_t> ? 7.f : 0.f;
   Fragment<T> q[kSteps];
   f32x16_t o[kColumns];
   float top, sum;
@@ -72,7 +73,7 @@ struct Attending {
 #pragma unroll
     for (int r = 1; r < 16 * kBlocks; ++r) high = fmaxf(high, s[r / 16][r % 16]);
     Halves const both = halves(high);
-    high              = fmaxf(both.low, both.high) * scale;
+    high              = fmaf(fmaxf(both.low, both.high), scale, -kRoom);
     // (a column that sees nothing yet keeps top at -infinity; NaN in a score is found in out at the end)
     if (__ballot(high > top + kSlack || top == -INFINITY)) {
       float const now  = fmaxf(top, high);

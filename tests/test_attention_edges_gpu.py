@@ -184,3 +184,19 @@ def test_float16_probabilities_keep_their_bits(lengths, count, kv, width, causal
     v_grad = encoder.attention_backward(m.g, m.q, m.k, m.v, encoder.AttentionSaved(out, logsum), ints(m.offsets), causal=causal)[2]
     error, expected = m.error(v_grad, m.wants[2], m.squares[2], others)
     assert error <= expected, (error, expected)
+
+
+@pytest.mark.parametrize("gap", [16.0, 22.0, 22.59375, 24.40625])
+@pytest.mark.parametrize("tokens,count", [(128, 1024), (33, 512)])
+def test_float16_weights_far_below_the_largest(gap, tokens, count):
+    """One key's weight is 2^gap times that of each of 131071 others, which have values of 1 where it has 0: a weight is off by half a step of it (unit) or by 2^-32, half of
+    float16's smallest number next to a largest weight of 2^7 and more; of their two sums, the scores and the exponentials 32 bits are left, n additions of 2^-24."""
+    n, unit = 131072, 2.0**-11
+    q, k, v = (torch.zeros(t, c, 64, dtype=F16, device="cuda") for t, c in ((tokens, count), (n, 1), (n, 1)))
+    q[:, :, 0], k[0, :, 0], v[1:] = 1.0, gap, 1.0
+    out, saved = encoder.attention(q, k, v, ints([0, tokens]), ints([0, n]), scale=float(np.log(2.0)), keep=True)
+    mass = (n - 1) * 2.0**-gap
+    want = mass / (1 + mass)
+    most = want * (3 * unit + 2 * n * 2.0**-24 + 2.0**-18) + n * 2.0**-32
+    assert (out.double() - want).abs().max().item() <= most
+    assert (saved.logsum.double() - (gap * np.log(2.0) + np.log1p(mass))).abs().max().item() <= 2.0**-18 * gap + n * 2.0**-24
