@@ -5,7 +5,7 @@ namespace nvtext_amd {
 namespace {
 
 // Rows of few tokens go in chunks of keys, where all tokens and heads that share a key head are columns of one wavefront's products, the others in tiles:
-// rows of at most kPartColumns columns, and, if they have a tile's keys or fewer, of kFewColumns.
+// rows of at most kPartColumns columns, and, if they have the smallest chunk's keys or fewer, of kFewColumns.
 constexpr int kPartColumns = 32, kFewColumns = 64, kFewKeys = 128;
 template <typename T>
 __device__ __forceinline__ bool goes_in_chunks(Forward<T> const& f, int32_t tokens, int32_t keys)
@@ -492,7 +492,8 @@ nvtext_amd_status attention(Forward<T> f, Mr const& mr, hipStream_t stream)
   while (f.shift < 30 && (static_cast<int64_t>(f.key_runs.tokens) * f.kv_heads >> f.shift) > 2048) ++f.shift;
   return with_tiles(f.width, [&](auto d) {
     constexpr int kD        = decltype(d)::value;
-    size_t const parts      = f.in_chunks ? static_cast<size_t>(most_parts(f.key_runs.tokens, f.shift)) * static_cast<size_t>(f.kv_heads) * kPartColumns : 0;
+    // (rows over their own keys have one chunk each, or are not split)
+    size_t const parts      = f.in_chunks && !f.own_keys() ? static_cast<size_t>(most_parts(f.key_runs.tokens, f.shift)) * static_cast<size_t>(f.kv_heads) * kPartColumns : 0;
     TempParts<3> const temp(mr, {align.bytes(), parts * kD * sizeof(float), parts * sizeof(float4)});
     if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
     align.launch(temp.template part<char>(0), stream);

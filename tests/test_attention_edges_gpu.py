@@ -200,3 +200,16 @@ def test_float16_weights_far_below_the_largest(gap, tokens, count):
     most = want * (3 * unit + 2 * n * 2.0**-24 + 2.0**-18) + n * 2.0**-32
     assert (out.double() - want).abs().max().item() <= most
     assert (saved.logsum.double() - (gap * np.log(2.0) + np.log1p(mass))).abs().max().item() <= 2.0**-18 * gap + n * 2.0**-24
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_over_their_own_keys_take_no_memory_for_parts(dtype):
+    """No row of few tokens over its own keys is in several chunks: the call needs no memory but its result."""
+    q, k = torch.randn(8192, 8, 128, device="cuda").to(dtype), torch.randn(8192, 1, 128, device="cuda").to(dtype)
+    rows = torch.arange(0, 8193, 4, dtype=torch.int32, device="cuda")
+    encoder.attention(q, k, k, rows)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = encoder.attention(q, k, k, rows)
+    assert torch.cuda.max_memory_allocated() - before <= out.numel() * out.element_size() + 4096
