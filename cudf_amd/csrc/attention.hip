@@ -124,9 +124,11 @@ struct Attending {
   }
   __device__ __forceinline__ float divisor() const { return whole(sizeof(T) == 2 ? weight : sum); }
 
-  // Writes out and logsum of a column, head h of token t, where it is `there`; of those whose result is not finite, the lanes' numbers.  That may come from keys that the
-  // token does not see, whose exponentials of 0 were multiplied: such columns are done once more, by themselves.  One that sees nothing has zeros, whatever was added up.
-  __device__ __forceinline__ uint32_t finish(Forward<T> const& f, int64_t t, int32_t h, bool there, int half, int column)
+  // Writes out and logsum of a column, head h of token t, where it is `there`.  Returns the lanes' numbers of those whose result is not finite for keys that
+  // they do not see, of which `border` says whether one is not finite: they are made once more, by themselves.  (NaN in a score makes NaN of the sum, and of all.)  A column that sees
+  // nothing has zeros, whatever was added up.
+  template <typename Border>
+  __device__ __forceinline__ uint32_t finish(Forward<T> const& f, int64_t t, int32_t h, bool there, int half, int column, Border&& border)
   {
     float const total = whole(sum), part = 1.f / divisor();
     float check       = 0.f;  // (NaN if any is infinite or NaN)
@@ -137,8 +139,9 @@ struct Attending {
         o[c][r] = seen > 0 ? o[c][r] * part : 0.f;
         check   = fmaf(o[c][r], 0.f, check);
       }
-    uint64_t odd = __ballot(there && check != 0.f);
-    odd          = (odd | odd >> 32) & 0xffffffffu;
+    uint64_t odd = f.causal ? __ballot(there && check != 0.f && total == total) : 0;
+    if (odd != 0 && !border()) odd = 0;
+    odd = (odd | odd >> 32) & 0xffffffffu;
     if (there && !(odd >> column & 1)) {
       store_columns<T, kColumns>(f.out.at(t, h), o, half, f.width);
       int64_t const at = static_cast<int64_t>(h) * f.runs.tokens + t;
@@ -219,7 +222,10 @@ __global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES>::kWa
     }
     return;
   }
-  uint32_t odd = a.finish(f, t, w.head, there, half, column);
+  uint32_t odd = a.finish(f, t, w.head, there, half, column, [&] {
+    int32_t const loaded = (most + kTile - 1) / kTile * kTile;
+    return holds_odd(f.v, static_cast<int64_t>(first) + least, (loaded < keys ? loaded : keys) - least, w.kv_head, f.width);
+  });
   for (; odd; odd &= odd - 1) attend_row(f, begin + block0 + wave0 + __builtin_ctz(odd), w.head);
 }
 
@@ -306,7 +312,11 @@ __global__ void __launch_bounds__(kWave, 1) attend_chunks_kernel(ForwardChunks<T
       }
       continue;
     }
-    for (uint32_t odd = a.finish(f, t, head, there, half, column); odd; odd &= odd - 1) {
+    auto const border = [&] {
+      int32_t const loaded = tiles * kTile;  // (from the first key on: what is not split is a whole row)
+      return holds_odd(f.v, static_cast<int64_t>(first) + least, (loaded < keys ? loaded : keys) - least, w.kv_head, f.width);
+    };
+    for (uint32_t odd = a.finish(f, t, head, there, half, column, border); odd; odd &= odd - 1) {
       int const which = __builtin_ctz(odd);
       attend_row(f, __builtin_amdgcn_readlane(static_cast<int32_t>(t), which), __builtin_amdgcn_readlane(head, which));
     }
@@ -322,13 +332,13 @@ __device__ __forceinline__ void add_part(Some<D>& sum, float2& total, float top,
   sum.add(part, weight);
 }
 
-// What Attending::finish does, for sums that a wavefront holds side by side.
+// What Attending::finish does, for sums that a wavefront holds side by side; `border`: keys behind those that the token sees, which lie from `first` on, that have been multiplied as well.
 template <typename T, int D>
-__device__ __forceinline__ void finish_row(Forward<T> const& f, int32_t t, int32_t head, int32_t seen, Some<D> sum, float2 total, float top)
+__device__ __forceinline__ void finish_row(Forward<T> const& f, int32_t t, int32_t head, int32_t first, int32_t seen, int32_t border, Some<D> sum, float2 total, float top)
 {
 #pragma unroll
   for (int k = 0; k < Some<D>::kEach; ++k) sum.v[k] = seen > 0 ? sum.v[k] / total.y : 0.f;
-  if (!sum.finite(f.width)) {
+  if (f.causal && total.x == total.x && !sum.finite(f.width) && holds_odd(f.v, static_cast<int64_t>(first) + seen, border, head / (f.heads / f.kv_heads), f.width)) {
     attend_row(f, t, head);
     return;
   }
@@ -386,7 +396,8 @@ __global__ void __launch_bounds__(WAVES * kWave) attend_join_kernel(ForwardChunk
 #pragma unroll
       for (int k = 0; k < Some<D>::kEach; ++k) sum.v[k] += sums[w][lane].v[k];
     }
-    finish_row<T, D>(f, begin + i, head, f.seen(i, tokens, keys), sum, total, top);
+    int32_t const seen = f.seen(i, tokens, keys);
+    finish_row<T, D>(f, begin + i, head, first, seen, keys - seen, sum, total, top);
   }
 }
 
@@ -413,7 +424,8 @@ __global__ void __launch_bounds__(kThreads) attend_join_shares_kernel(Forward<T>
   Some<D> sum{};
 #pragma unroll 8
   for (int32_t c = 0; c < shares; ++c) sum.add(split.sums + (at + (static_cast<int64_t>(c) << shift)) * D, __shfl(weight, c));
-  finish_row<T, D>(f, t, head, f.seen(i, tokens, keys), sum, total, top);
+  int32_t const seen = f.seen(i, tokens, keys), loaded = (all + kTile - 1) / kTile * kTile;
+  finish_row<T, D>(f, t, head, first, seen, (loaded < keys ? loaded : keys) - seen, sum, total, top);
 }
 
 // ------------------------------------------------------------------ launches

@@ -211,9 +211,13 @@ __global__ void __launch_bounds__(WAVES * kWave, (GradientShape<T, D, WAVES>::kW
       d[c][r] = seen > 0 ? d[c][r] * f.scale : 0.f;
       check   = fmaf(d[c][r], 0.f, check);
     }
-  // (as forward: a key that is not seen may have been multiplied by 0)
-  uint64_t odd = __ballot(there && check != 0.f);
-  odd          = (odd | odd >> 32) & 0xffffffffu;
+  // (as forward: a key that is not seen may have been multiplied by 0; NaN in the log or in delta makes NaN of all)
+  uint64_t odd = f.causal ? __ballot(there && check != 0.f && log == log && delta == delta) : 0;
+  if (odd != 0) {
+    int32_t const loaded = (most + kTile - 1) / kTile * kTile;
+    if (!holds_odd(f.k, static_cast<int64_t>(first) + least, (loaded < keys ? loaded : keys) - least, w.kv_head, f.width)) odd = 0;
+  }
+  odd = (odd | odd >> 32) & 0xffffffffu;
   if (there && !(odd >> column & 1)) store_columns<T, kColumns>(f.q_grad.at(t, w.head), d, half, f.width);
   for (; odd; odd &= odd - 1) query_gradient_row(f, begin + block0 + wave0 + __builtin_ctzll(odd), w.head);
 }
@@ -227,6 +231,16 @@ struct KeyShape {
   static constexpr int kStage = kTiles + 2 * kWave * 4, kLds = 2 * kStage;  // (with logs and deltas)
   static constexpr int kWavesASimd = sizeof(T) == 2 && D <= 128 ? 2 : 1;
 };
+// Whether one of `count` tokens from `first` on holds an infinity or NaN in what the gradients of k and v, those that are wanted, add up.
+template <typename T>
+__device__ __forceinline__ bool tokens_hold_odd(Backward<T> const& f, int32_t first, int32_t count, int32_t kv_head, bool of_k, bool of_v)
+{
+  int32_t const each = f.heads / f.kv_heads;
+#pragma unroll 1
+  for (int32_t h = kv_head * each; h < (kv_head + 1) * each; ++h)
+    if ((of_k && holds_odd(f.q, first, count, h, f.width)) || (of_v && holds_odd(f.grad, first, count, h, f.width))) return true;
+  return false;
+}
 // PART: the gradients of both, or of k or v alone: of heads of more than 96 values there are not the registers for both, and what the compiler keeps in memory instead
 // waits for the loads of the next tile at every use.
 enum Part { kBoth, kOfK, kOfV };
@@ -418,8 +432,13 @@ __global__ void __launch_bounds__(WAVES * kWave, (KeyShape<T, D, WAVES>::kWavesA
         check    = fmaf(dv[c][r], 0.f, check);
       }
     }
-  uint64_t odd = __ballot(there && check != 0.f);
-  odd          = (odd | odd >> 32) & 0xffffffffu;
+  uint64_t odd = f.causal ? __ballot(there && check != 0.f) : 0;
+  if (odd != 0) {
+    // (tokens that went through the products, up to the first that sees all of the keys)
+    int32_t const border = first_from / (32 * kAtOnce) * (32 * kAtOnce), count = (last_from < tokens ? last_from : tokens) - border;
+    if (!tokens_hold_odd(f, begin + border, count, w.kv_head, kK, kV) || is_odd_anyway(f, begin, last_from, tokens, w.kv_head, kK, kV)) odd = 0;
+  }
+  odd = (odd | odd >> 32) & 0xffffffffu;
   if (there && !(odd >> column & 1)) {
     if constexpr (kK) store_columns<T, kColumns>(f.k_grad.at(t, w.kv_head), dk, half, f.width);
     if constexpr (kV) store_columns<T, kColumns>(f.v_grad.at(t, w.kv_head), dv, half, f.width);
@@ -437,15 +456,13 @@ __device__ __forceinline__ Some<D> add_shares(const float* at, int64_t step, int
   return sum;
 }
 
-// Writes a row of a gradient; false: not, what it holds is not finite.
+// Writes a row of a gradient.
 template <typename T, int D>
-__device__ __forceinline__ bool write_row(T* head, Some<D> const& sum, int32_t width)
+__device__ __forceinline__ void write_row(T* head, Some<D> const& sum, int32_t width)
 {
-  if (!sum.finite(width)) return false;
 #pragma unroll
   for (int k = 0; k < Some<D>::kEach; ++k)
     if (sum.first() + k < width) head[sum.first() + k] = static_cast<T>(sum.v[k]);
-  return true;
 }
 
 template <typename T, int D>
@@ -462,7 +479,16 @@ __global__ void __launch_bounds__(kThreads) query_gradient_join_kernel(Backward<
   int32_t const all = f.seen(last < tokens ? last : tokens - 1, tokens, keys), shares = shares_of((all + kTile - 1) / kTile, split.splits);
   if (shares < 2) return;
   int64_t const at = (split.slot(f.runs.first_block(run, shift) + (i >> shift), head, f.heads, 0) << shift) + (i & ((1 << shift) - 1));
-  if (!write_row<T, D>(f.q_grad.at(t, head), add_shares<D>(split.sums + at * D, static_cast<int64_t>(D) << shift, shares, f.scale), f.width)) query_gradient_row(f, t, head);
+  int32_t const seen = f.seen(i, tokens, keys), loaded = (all + kTile - 1) / kTile * kTile;
+  // (a token that sees nothing may have 0 times what others see among its sums)
+  Some<D> sum{};
+  if (seen > 0) sum = add_shares<D>(split.sums + at * D, static_cast<int64_t>(D) << shift, shares, f.scale);
+  int64_t const row = static_cast<int64_t>(head) * f.runs.tokens + t;
+  if (f.causal && !sum.finite(f.width) && f.logs[row] == f.logs[row] && f.deltas[row] == f.deltas[row] &&
+      holds_odd(f.k, static_cast<int64_t>(first) + seen, (loaded < keys ? loaded : keys) - seen, head / (f.heads / f.kv_heads), f.width))
+    query_gradient_row(f, t, head);
+  else
+    write_row<T, D>(f.q_grad.at(t, head), sum, f.width);
 }
 
 template <typename T, int D>
@@ -483,9 +509,19 @@ __global__ void __launch_bounds__(kThreads) key_gradient_join_kernel(Backward<T>
   if (shares < 2) return;
   int64_t const at   = (split.slot(f.key_runs.first_block(run, shift) + (i >> shift), head, f.kv_heads, 0) << shift) + (i & ((1 << shift) - 1));
   int64_t const step = static_cast<int64_t>(2 * D) << shift;
-  bool const of_k    = write_row<T, D>(f.k_grad.at(t, head), add_shares<D>(split.sums + at * (2 * D), step, shares, f.scale), f.width);
-  bool const of_v    = write_row<T, D>(f.v_grad.at(t, head), add_shares<D>(split.sums + at * (2 * D) + D, step, shares, 1.f), f.width);
-  if (!of_k || !of_v) key_gradient_row(f, t, head, !of_k, !of_v);
+  Some<D> const sum_k = add_shares<D>(split.sums + at * (2 * D), step, shares, f.scale), sum_v = add_shares<D>(split.sums + at * (2 * D) + D, step, shares, 1.f);
+  bool of_k = false, of_v = false;  // (what is made once more)
+  if (f.causal) {
+    int32_t const begin = f.runs.begin(run), own = static_cast<int32_t>(std::min<int64_t>(std::max<int64_t>(static_cast<int64_t>(i) + tokens - keys, 0), tokens));
+    auto const again    = [&](Some<D> const& sum, bool k) {
+      return !sum.finite(f.width) && tokens_hold_odd(f, begin + start * kTile, own - start * kTile, head, k, !k) && !is_odd_anyway(f, begin, own, tokens, head, k, !k);
+    };
+    of_k = again(sum_k, true);
+    of_v = again(sum_v, false);
+    if (of_k || of_v) key_gradient_row(f, t, head, of_k, of_v);
+  }
+  if (!of_k) write_row<T, D>(f.k_grad.at(t, head), sum_k, f.width);
+  if (!of_v) write_row<T, D>(f.v_grad.at(t, head), sum_v, f.width);
 }
 
 // ------------------------------------------------------------------ launches

@@ -196,7 +196,8 @@ nvtext_amd_status nvtext_amd_rotary(const nvtext_amd_heads* x,
  * there, for causal = 0 every one, else j <= i + K - Q: its last token all of them.  Over the keys it sees, with s_j = scale * (q . k_j),
  *   logsum = log(sum of exp(s_j)),  out = sum of exp(s_j - logsum) * v_j;
  * a token that sees none, or belongs to no row, has zeros in out and -infinity in logsum.  What a token does not see is without
- * effect on it, whatever it is, NaN too.
+ * effect on it, whatever it is, NaN too.  (Of a result that cannot be finite for what its token sees, it is not laid down whether it is an infinity or NaN.  Of
+ * causal rows, infinities or NaN that all over the values or the gradient lie among what is finite cost a lot of time.)
  * q, k, v and out are of one type and width, of at most 256 values, in at most 65536 heads of 2^31 - 1025 tokens; scale is not negative.  logsum (NULL: not wanted; the gradient needs it)
  * has a value of FLOAT32 at [h * tokens + t].  rest (NULL: not wanted; FLOAT32 has none), of a value for each of out's, [heads, tokens, width]
  * one after the other: what rounding left off it, in 8 bits, for the gradient.  Products, exponentials' sums and out are held in 32 bits; of 16-bit types, the exponentials are

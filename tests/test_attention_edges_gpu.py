@@ -6,7 +6,7 @@ import torch
 
 from cudf_amd import encoder
 from oracle import encoder_py as orc
-from tests.test_attention_gpu import F16, TYPES, Made, ints, near, offsets_of, rounding
+from tests.test_attention_gpu import BF16, F16, F32, TYPES, UNIT, Made, ints, near, offsets_of, rounding
 
 pytestmark = pytest.mark.gpu
 
@@ -213,3 +213,117 @@ def test_rows_over_their_own_keys_take_no_memory_for_parts(dtype):
     before = torch.cuda.memory_allocated()
     out = encoder.attention(q, k, k, rows)
     assert torch.cuda.max_memory_allocated() - before <= out.numel() * out.element_size() + 4096
+
+
+def by_what_is_seen(m):
+    """Forward results and gradients in 64 bits where inputs are infinite or NaN: each token's sums over what it sees alone, with 0 times such a value NaN; out and logsum
+    of the forward pass go on as they are."""
+    q, k, v, g = (x.double().cpu().numpy() for x in (m.q, m.k, m.v, m.g))
+    scale, each = q.shape[2] ** -0.5, q.shape[1] // k.shape[1]
+    out, log = np.zeros(q.shape), np.full(q.shape[:2][::-1], -np.inf)
+    grads = [np.zeros(x.shape) for x in (q, k, v)]
+    with np.errstate(all="ignore"):
+        for first, last in zip(m.offsets[:-1], m.offsets[1:]):
+            for h in range(q.shape[1]):
+                for t in range(first, last):
+                    keys = slice(first, t + 1)
+                    kk, vv = k[keys, h // each], v[keys, h // each]
+                    s = scale * (kk * q[t, h]).sum(1)
+                    top = s.max()
+                    e = np.exp(s - (0.0 if top == -np.inf else top))
+                    log[h, t] = top + np.log(e.sum())
+                    p = e / e.sum()
+                    out[t, h] = (p[:, None] * vv).sum(0)
+                    ds = p * ((vv * g[t, h]).sum(1) - (g[t, h] * out[t, h]).sum())
+                    grads[0][t, h] = scale * (ds[:, None] * kk).sum(0)
+                    grads[1][keys, h // each] += scale * ds[:, None] * q[t, h]
+                    grads[2][keys, h // each] += p[:, None] * g[t, h]
+    return out, log, grads
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths,count,kv,width", [([150, 40, 3], 2, 1, 64), ([33] * 6, 4, 2, 72), ([700], 2, 2, 64), ([140, 20], 2, 1, 256)])
+@pytest.mark.parametrize("where", ["v", "g", "k", "tokens", "all of g"])
+def test_what_is_not_finite_stays_with_those_that_see_it(where, lengths, count, kv, width, dtype):
+    """Infinities and NaN here and there in values or gradients, in keys, of whole tokens, and everywhere: results are finite where they are for what is seen, and as they are without the
+    others (to twice what a kernel's may be off by: 16-bit types and sums of 700 in 32 bits, of magnitudes of about 1)."""
+    m = Made((lengths, None, count, kv, width, 0), dtype, seed=5)
+    odd = torch.tensor([float("inf"), float("-inf"), float("nan")], device="cuda").to(dtype)
+    pick = lambda shape, n: tuple(torch.from_numpy(m.rng.integers(0, s, n)).cuda() for s in shape)
+    tokens = sum(lengths)
+    if where in ("v", "g", "k"):
+        x = getattr(m, where)
+        at = pick(x.shape, tokens // 8)
+        x[at] = odd[torch.from_numpy(m.rng.integers(0, 3, tokens // 8)).cuda()] if where != "k" else float("nan")
+    elif where == "tokens":
+        for t in m.rng.integers(m.offsets[0], m.offsets[-1], 3):
+            m.q[t] = m.k[t] = m.v[t] = m.g[t] = float("nan")
+    else:
+        m.g[:] = float("inf")
+    want, log, wants = by_what_is_seen(m)
+    out, saved = encoder.attention(m.q, m.k, m.v, *m.rows(), causal=True, keep=True)
+    grads = encoder.attention_backward(m.g, m.q, m.k, m.v, saved, *m.rows(), causal=True)
+    near_where_finite(out, want, dtype, 1.0)
+    near_where_finite(saved.logsum, log, F32, 16.0)
+    for x, w in zip(grads, wants):
+        near_where_finite(x, w, dtype, 32.0)
+
+
+def near_where_finite(got, want, dtype, size):
+    got = got.double().cpu().numpy()
+    finite = np.isfinite(want) | (want == -np.inf if got.ndim == 2 else False)
+    assert np.array_equal(np.isfinite(got) | (got == -np.inf if got.ndim == 2 else False), finite)
+    inside = np.isfinite(want)
+    assert (np.abs(got[inside] - want[inside]) <= 4 * (UNIT[dtype] + 2.0**-13) * (np.abs(want[inside]) + size)).all()
+
+
+@pytest.mark.parametrize("back", [3, 11])
+def test_tokens_that_overlap(back):
+    """Keys and values that lie a few values apart, each within the last: NaN behind the last one's 64 values (which end 8 in front of the memory's end) is nobody's, and among them it
+    is that key's, and nobody else's."""
+    for dtype in TYPES:
+        memory = torch.randn(33 * 8 + 64, device="cuda").to(dtype)
+        x = memory.as_strided((33, 1, 64), (8, 64, 1))
+        q = torch.randn(33, 2, 64, device="cuda").to(dtype)
+        memory[-back] = float("nan")
+        apart = x.contiguous()
+        assert torch.isnan(apart).sum() == (1 if back > 8 else 0)
+        out, want = encoder.attention(q, x, x, ints([0, 33])), encoder.attention(q, apart, apart, ints([0, 33]))
+        assert torch.equal(torch.isnan(out), torch.isnan(want))
+        k = torch.randn(33, 1, 64, device="cuda").to(dtype)
+        out, want = encoder.attention(q, k, x, ints([0, 33])), encoder.attention(q, k, apart, ints([0, 33]))
+        odd = torch.isnan(apart).any(0)[0]
+        assert torch.equal(torch.isnan(out), odd.expand(33, 2, 64)) and torch.equal(out[:, :, ~odd], want[:, :, ~odd])
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("which", ["token", "tokens", "gradient", "gradients"])
+def test_what_is_not_finite_does_not_take_long(which, causal):
+    """NaN in one token or in all, or a gradient that has overflowed: a step over 4096 tokens takes less than 30 times as long as one without (it took 300 to 1000 times as long
+    where every row that is not finite was made once more)."""
+    torch.manual_seed(3)
+    n = 4096
+    q, k, v, g = (torch.randn(n, h, 64, device="cuda").to(BF16) for h in (8, 4, 4, 8))
+
+    def step(q, k, v, g):
+        out, saved = encoder.attention(q, k, v, ints([0, n]), causal=causal, keep=True)
+        return encoder.attention_backward(g, q, k, v, saved, ints([0, n]), causal=causal)
+
+    def time(*args):
+        step(*args)
+        torch.cuda.synchronize()
+        begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        begin.record()
+        for _ in range(3):
+            step(*args)
+        end.record()
+        torch.cuda.synchronize()
+        return begin.elapsed_time(end)
+
+    clean = time(q, k, v, g)
+    if which in ("token", "tokens"):
+        for x in (q, k, v, g):
+            x[7 if which == "token" else slice(None)] = float("nan")
+    else:
+        g[n - 7 if which == "gradient" else slice(None)] = float("inf")
+    assert time(q, k, v, g) < 30 * clean
