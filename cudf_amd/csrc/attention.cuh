@@ -549,11 +549,16 @@ __device__ __forceinline__ void store_rests(int8_t* head, f32x16_t const (&x)[CO
 // ------------------------------------------------------------------ work
 constexpr int kThreads = 256;
 constexpr int kTileWaves = 4;  // wavefronts that share the tiles in LDS
-// Of rows that have at most kShortRow tokens on average, a wavefront alone: blocks of 32 tokens and tiles of 32 keys, so that nothing waits for what is not there.
-// (60,000 tokens, 8 heads, a step in bfloat16, us with four wavefronts and with one: rows of 12 tokens, heads of 64 1127 and 478, of 128 2547 and 1445; of 48 tokens
-// 435 and 330, 945 and 841; of 100 367 and 352, 784 and 882.  Where tiles go in shares, keys are many, and four go on sharing them.)
+// Of rows that have at most kShortRow tokens and keys on average, a wavefront alone: blocks of 32 tokens and tiles of 32 keys, so that nothing waits for what is not there.
+// (60,000 tokens over their own keys, 8 heads, a step in bfloat16, us with four wavefronts and with one: rows of 12 tokens, heads of 64 1127 and 478, of 128 2547 and 1445; of 48 tokens
+// 435 and 330, 945 and 841; of 100 367 and 352, 784 and 882.  Over more keys than that, four share them, forward: 16 rows of 48 tokens, 64 heads of 128 over 8, 2000 keys a row
+// 142 and 162, 40000 keys 2440 and 2900; 1000 rows of 50 tokens, 8 heads of 64, 250 keys 153 and 173, 850 keys 437 and 540; of 20 tokens, 420 keys 294 and 291.)
 constexpr int kShortRow = 64;
-inline bool is_short(Runs const& runs, int32_t most = kShortRow) { return runs.rows > 0 && runs.tokens <= static_cast<int64_t>(runs.rows) * most; }
+template <typename T>
+bool is_short(Problem<T> const& p, int32_t most = kShortRow)
+{
+  return p.runs.rows > 0 && std::max(p.runs.tokens, p.key_runs.tokens) <= static_cast<int64_t>(p.runs.rows) * most;
+}
 template <typename T, int D, int WAVES>
 constexpr int kTileOf = WAVES == 1 ? 32 : Tile<T, D>::kHeads;
 

@@ -450,7 +450,7 @@ nvtext_amd_status attend_tiles(Forward<T> const& f, Mr const& mr, hipStream_t st
   if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");
   split.sums = temp.template part<float>(0);
   split.tops = temp.template part<float4>(1);
-  if (split.splits == 1) return is_short(f.runs) ? launch_tiles<T, D, 1>(f, split, stream) : launch_tiles<T, D, kTileWaves>(f, split, stream);
+  if (split.splits == 1) return is_short(f) ? launch_tiles<T, D, 1>(f, split, stream) : launch_tiles<T, D, kTileWaves>(f, split, stream);
   nvtext_amd_status const st = launch_tiles<T, D, kTileWaves>(f, split, stream);
   if (st != NVTEXT_AMD_SUCCESS) return st;
   ProfileScope const scope("attention_join", stream);

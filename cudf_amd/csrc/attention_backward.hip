@@ -571,7 +571,7 @@ nvtext_amd_status gradient_tiles(Backward<T> const& f, Mr const& mr, hipStream_t
   of_q.sums = temp.template part<float>(0);
   of_k.sums = temp.template part<float>(1);
   nvtext_amd_status st = NVTEXT_AMD_SUCCESS;
-  if (f.runs.tokens > 0) st = of_q.splits == 1 && is_short(f.runs, kShort<T>) ? query_gradient_tiles<T, D, 1>(f, of_q, stream) : query_gradient_tiles<T, D, kTileWaves>(f, of_q, stream);
+  if (f.runs.tokens > 0) st = of_q.splits == 1 && is_short(f, kShort<T>) ? query_gradient_tiles<T, D, 1>(f, of_q, stream) : query_gradient_tiles<T, D, kTileWaves>(f, of_q, stream);
   if (st != NVTEXT_AMD_SUCCESS) return st;
   if (of_q.splits > 1) {
     ProfileScope const scope("attention_query_gradient_join", stream);
@@ -579,7 +579,7 @@ nvtext_amd_status gradient_tiles(Backward<T> const& f, Mr const& mr, hipStream_t
                        int{OfQ::kShift});
   }
   if (f.key_runs.tokens == 0) return NVTEXT_AMD_SUCCESS;
-  st = of_k.splits == 1 && is_short(f.key_runs, kShort<T>) ? key_gradient_parts<T, D, 1>(f, of_k, stream) : key_gradient_parts<T, D, kTileWaves>(f, of_k, stream);
+  st = of_k.splits == 1 && is_short(f, kShort<T>) ? key_gradient_parts<T, D, 1>(f, of_k, stream) : key_gradient_parts<T, D, kTileWaves>(f, of_k, stream);
   if (st != NVTEXT_AMD_SUCCESS || of_k.splits == 1) return st;
   ProfileScope const scope("attention_key_gradient_join", stream);
   hipLaunchKernelGGL(HIP_KERNEL_NAME(key_gradient_join_kernel<T, D>), grid_of((static_cast<int64_t>(f.key_runs.tokens) * f.kv_heads + 3) / 4, kThreads), dim3(kThreads), 0, stream, f, of_k,

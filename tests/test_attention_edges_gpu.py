@@ -327,3 +327,12 @@ def test_what_is_not_finite_does_not_take_long(which, causal):
     else:
         g[n - 7 if which == "gradient" else slice(None)] = float("inf")
     assert time(q, k, v, g) < 30 * clean
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths,keys", [([40, 33, 0, 50] * 8, [150, 90, 3, 260] * 8), ([20, 90] * 12, [30, 95] * 12), ([60] * 20, [61] * 20)])
+def test_short_rows_over_more_keys_than_tokens(lengths, keys, dtype):
+    """Short rows of tokens over caches of more keys, which four wavefronts share, and over few, which one has alone."""
+    m = Made((lengths, keys, 8, 8, 64, 0), dtype, roomy=True)
+    m.check_forward(True)
+    m.check_backward(True)
