@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(WAVES * kWave, (ForwardShape<T, D, WAVES>::kWa
 // ------------------------------------------------------------------ forward, in chunks of keys
 // Few tokens a row, as where texts go on token by token: one wavefront has all of a row's tokens and of all heads that share a key head, up to 32 together,
 // as the columns of its products, and a chunk of 2^shift of the row's keys; what it adds up is joined with that of the row's other chunks by another
-// launch.  Bound by memory: the keys are read once (256 rows of one token over 2064 keys on average, 32 heads of 128 over 8: 35 us, 4.2 TB/s, and 6 for the join; one token over
+// launch.  Bound by memory: the keys are read once (24 rows of one token over 1501 keys on average, 32 heads of 128 over 8: 35 us, 4.2 TB/s, and 6 for the join; one token over
 // 131071: 100 us, 5.4 TB/s, and 11).  Tiles of 32 keys, so that a CU has room for five workgroups of heads of 128: 35 and 100 us where 64 take 40 and 102.  The chunks of key tokens are numbered as the blocks of tokens are elsewhere, so they are
 // alike in size however long the rows are.  A row of a single chunk is finished at once; so is one of more columns, 32 of them after the other by each of
 // the workgroups that its chunks have.

@@ -7,13 +7,14 @@ namespace {
 // Two launches, the first for q, the second (of wide heads, a second and a third) for k and v: each makes the scores anew and adds up what is its own in registers, in one order at every
 // call.  (One launch for all three would have to add up q's gradient in memory, over all workgroups of keys: in parts of float32 or in any order.)
 //
-// Blocks of 32 rows of a tile that go through one stream of fragments.  Of narrow heads, whose rows are often short, one, so that none is gone through that has no row; of
-// wider ones two, which spares the wait for the first fragments of the second (16384 tokens in four rows, heads of 128: 3.56 -> 3.12 ms with the forward
-// pass; 131071 in 1024, heads of 64: 1.12 either way).
+// Blocks of 32 rows of a tile that go through one stream of fragments.  Of heads of 128, two, which spares the wait for the first fragments of the second (16384 tokens in four rows: 3.56 -> 3.12 ms
+// with the forward pass).  Of narrower ones, whose rows are often short, one, so that none is gone through that has no row (131071 in 1024, heads of 64: 1.12 ms either way; 32768 in 64, of 96:
+// 660 us, with two 650); of wider ones one, whose registers are few as it is (8192 in eight rows, 16 heads of 192 in bfloat16 720 us, with two 748, in float16 794 and 766, of 256 907 and 940).
 template <typename T, int D>
 constexpr int kBlocksAtOnce = sizeof(T) == 2 && D == 128 ? 2 : 1;
 // Two rows' values and a sum of 1024 bytes are more than a lane's registers hold with the rest: one of the rows is read again, two products ahead, for every block
-// of 32, whose 384 products take longer than that (1135 tokens, 12 heads of 216 values in float32: that of q 307 -> 288 us, of k 253 -> 213).
+// of 32, whose 384 products take longer than that (1135 tokens, 12 heads of 216 values in float32: that of q 307 -> 288 us, of k 253 -> 213).  Some stay in memory all the same: 39 registers
+// of q's with four wavefronts, 87 with one; with one, of k's about as many.
 template <typename T, int D>
 constexpr bool kReadAgain = D * sizeof(T) > 768;
 

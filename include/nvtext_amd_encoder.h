@@ -174,7 +174,7 @@ typedef enum nvtext_amd_rotary_layout {
  * Row r's tokens are offsets[r] up to offsets[r + 1] (device, rows + 1 values, ascending); their positions count from
  * starts[r] on (device, `rows` values; NULL: from 0 on).  A token that belongs to no row is copied.  frequencies: `pairs` values on
  * the device, radians a position.  Angles are computed in 64 bits and reduced to a part of a turn before they lose any, so positions may be
- * as far as they come: sine and cosine are off by 2^-22 at most (at position t by t * |frequency| * 2^-52 more); products and sums are
+ * as far as they come: sine and cosine are off by 2^-22 at most (at position t by t * |frequency| * 2^-51 more); products and sums are
  * held in 32 bits and rounded once.  out has x's shape and type, and may be x. */
 nvtext_amd_status nvtext_amd_rotary(const nvtext_amd_heads* x,
                                     int32_t rows,
