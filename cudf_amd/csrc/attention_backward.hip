@@ -23,7 +23,7 @@ template <typename T>
 constexpr int32_t kShort = sizeof(T) == 4 ? 2 * kShortRow : kShortRow;
 
 // What is rounded to float16 before it is multiplied is brought into its range first.  d = p (grad . v - grad . out) lies anywhere: with gradients of 1e-3, a row of 4096 tokens
-// has d of 1e-6, where float16 has steps of 6e-8 (q's gradient was off by 0.25 %, of 1e-4 over 8192 tokens by 6 %; that of float16's own rounding is 0.04 and 0.9 %), and of a
+// has d of 1e-6, where float16 has steps of 6e-8 (q's gradient was off by 0.53 %, of 1e-4 over 8192 tokens by 10 %; with its bits it is by 0.07 and 0.93, its own rounding), and of a
 // loss that has been scaled up it may pass 65504.  So a column multiplies its d by a power of 2 of its own and its sums by the reciprocal at the end.  Its largest d so far lies between
 // 2^8 and 2^15 (or below, while the power is the first one), and only a larger one changes the power, and with it what has been added up: what is 2^-22 of
 // it and more keeps all its bits, and the rest is off by 2^-33 of it.  bfloat16 has the exponents of float32.  (Steps take 3 to 4 % longer for it: 131071 tokens in 1024 rows, 12 heads
