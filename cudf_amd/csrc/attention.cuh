@@ -55,7 +55,8 @@ struct Problem {
 // so one is only made again where its sums are not finite and need not be so for what it sees, and where something that it does not see, at the border between what the block's
 // tokens see and what they do not, is not finite.  (Without `causal` there is no such border.)  A step over 8192 tokens, 32 heads of 128 over 8, causal, bfloat16, takes 2.7 ms, and 4.7 to 6.9 with
 // NaN in one token's k or v, in a late token's gradient, or everywhere, where it took 1.5 to 2.8 s with all rows made again; with NaN in an early q, whose block's
-// other 31 keys are made again over all tokens, 32.  Values or gradients that are not finite here and there in nearly every block of tokens still take as long as rows do.
+// other 31 keys are made again over all tokens, 32.  Values or gradients that are not finite here and there in nearly every block of tokens still take as long as rows do: 0.4 s forward
+// and 1.4 s back, one in 1000 infinite.
 
 template <typename T>
 __device__ __forceinline__ float dot(const T* a, const T* b, int32_t width)

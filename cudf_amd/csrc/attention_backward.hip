@@ -30,7 +30,7 @@ constexpr int32_t kShort = sizeof(T) == 4 ? 2 * kShortRow : kShortRow;
 // of 64, 1121 -> 1165 us; 8192 in eight rows, 16 heads of 192, 720 -> 795, of 256 920 -> 968.)
 template <typename T>
 constexpr bool kLifted = std::is_same_v<T, half_t>;
-// And so are the probabilities that the gradient of v adds up, in which a key of little weight has 2^-20 (where one of 2000 keys has nearly all, the others' gradients were off by 2.5 %): they
+// And so are the probabilities that the gradient of v adds up, in which a key of little weight has 2^-20 (where one of 2000 keys has nearly all, the others' gradients were off by 1.9 %, and are by 0.03): they
 // are 1 at most, and go through the products 2^15 times as large.
 template <typename T>
 constexpr float kWeightLift = kLifted<T> ? 15.f : 0.f;
@@ -564,8 +564,9 @@ nvtext_amd_status gradient_tiles(Backward<T> const& f, Mr const& mr, hipStream_t
 {
   using OfQ = GradientShape<T, D, kTileWaves>;
   using OfK = KeyShape<T, D, kTileWaves>;
-  Split of_q{splits_of<T, D, 3>(f, f.runs, f.heads, OfQ::kShift, f.key_runs, 1, OfQ::kLds), nullptr, nullptr};
-  Split of_k{splits_of<T, D, (D > 96 ? 5 : 4)>(f, f.key_runs, f.kv_heads, OfK::kShift, f.runs, f.heads / f.kv_heads, OfK::kLds), nullptr, nullptr};
+  constexpr int kLds = 4 * Tile<T, D>::kBytes;  // (where tiles are smaller, a CU has one workgroup for the registers that it takes)
+  Split of_q{splits_of<T, D, 3>(f, f.runs, f.heads, OfQ::kShift, f.key_runs, 1, kLds), nullptr, nullptr};
+  Split of_k{splits_of<T, D, (D > 96 ? 5 : 4)>(f, f.key_runs, f.kv_heads, OfK::kShift, f.runs, f.heads / f.kv_heads, kLds), nullptr, nullptr};
   TempParts<2> const temp(mr, {of_q.splits > 1 ? static_cast<size_t>(f.runs.blocks(OfQ::kShift) * f.heads * of_q.splits * OfQ::kRows * D) * sizeof(float) : 0,
                                of_k.splits > 1 ? static_cast<size_t>(f.key_runs.blocks(OfK::kShift) * f.kv_heads * of_k.splits * OfK::kRows * D) * 2 * sizeof(float) : 0});
   if (!temp.ok()) return fail(NVTEXT_AMD_ALLOC_FAILED, "temporary allocation failed");

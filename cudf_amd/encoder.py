@@ -323,7 +323,7 @@ def rotary(x: torch.Tensor, rows: Rows, frequencies: torch.Tensor, starts: Optio
     layout "half" are n and n + len(frequencies), those of "interleaved" 2 n and 2 n + 1.  rows: the tokenizer's column, or int32 offsets;
     starts: int32, the position of every row's first token (of a text under way).  Query and key heads that lie next to each
     other take one call.  inverse=True on the gradient of the result gives that of x.  out: where the result goes, x itself
-    if wanted."""
+    if wanted, but nothing that holds values of x in other places."""
     code = ROTARY_LAYOUTS.get(layout)
     if code is None:
         raise ValueError(f"layout must be one of {', '.join(ROTARY_LAYOUTS)}")
@@ -366,7 +366,7 @@ def attention_backward(grad: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
                        key_lengths: Optional[torch.Tensor] = None, causal: bool = False, scale: Optional[float] = None,
                        out: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(grad of q, grad of k, grad of v) of attention().  The gradient of a key head is the sum over the heads that see it.  out: where they go,
-    views of one projection's gradient for instance."""
+    views of one projection's gradient for instance, which hold no value of the other arguments."""
     g, m = _heads(grad, "grad"), _heads(q, "q")
     count, offsets, *keys = _key_rows(rows, key_rows, key_lengths)
     _here(saved.logsum, "logsum")

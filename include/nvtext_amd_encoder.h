@@ -175,7 +175,7 @@ typedef enum nvtext_amd_rotary_layout {
  * starts[r] on (device, `rows` values; NULL: from 0 on).  A token that belongs to no row is copied.  frequencies: `pairs` values on
  * the device, radians a position.  Angles are computed in 64 bits and reduced to a part of a turn before they lose any, so positions may be
  * as far as they come: sine and cosine are off by 2^-22 at most (at position t by t * |frequency| * 2^-51 more); products and sums are
- * held in 32 bits and rounded once.  out has x's shape and type, and may be x. */
+ * held in 32 bits and rounded once.  out has x's shape and type, and may be x, but not hold values of it in other places. */
 nvtext_amd_status nvtext_amd_rotary(const nvtext_amd_heads* x,
                                     int32_t rows,
                                     const int32_t* offsets,
